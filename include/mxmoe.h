@@ -333,6 +333,49 @@ int mx_acc_add_rows(mx_ctx* ctx, float* sum, const uint16_t* rows_bf16, const in
 int mx_acc_add(mx_ctx* ctx, float* sum, const uint16_t* values_bf16, int64_t count, void* stream); /* moe_add_shared */
 int mx_acc_finish(mx_ctx* ctx, const float* sum, uint16_t* out_bf16, int64_t count, void* stream); /* moe_finish     */
 
+/* ---- tokens sorted by expert and back, for experts of any format (the batched, device-side form of participation
+ *      and MoEAccumulator, src/vesper/moe.py:18-148), and the gradients of both ----
+ *
+ * A token t names top_k groups (experts) by ids[t][j]; pair p = t * top_k + j. Ids outside [0, groups) are experts of
+ * other devices (or none): their pairs get no row. The other pairs' rows are ordered by group, then by pair, so a
+ * group's rows are in ascending token order; a token may name one group twice (two rows). All arrays are contiguous
+ * device memory; tokens in [0, 2^18], top_k in [1, 32], groups in [1, 1024], width in [1, 2^24] values per row. Row
+ * buffers hold tokens * top_k rows; the rows from first[groups] on are neither read nor written. */
+typedef struct mx_row_plan {
+  int32_t* first;     /* [groups + 1] first row of each group; first[groups] = the rows in use           */
+  int32_t* pair_row;  /* [T][top_k] row of each pair, -1 without one                                     */
+  int32_t* row_pair;  /* [T top_k] pair of each row; the pairs without a row last, in ascending order     */
+} mx_row_plan;
+
+#define MX_ROWS_BF16 0
+#define MX_ROWS_F32 1
+#define MX_ROWS_U8 2    /* mx_dispatch only: width bytes a row (E4M3 codes, E8M0 scales) */
+
+/* ids [T][top_k] -> plan, and rows[pair_row[p]] = x[t] for every pair with a row, with row_weights[pair_row[p]] =
+ * weights[p] (both or neither; the route_w that the expert calls take). x = rows = NULL: the plan alone. ids = NULL:
+ * rows by the plan of an earlier call with the same tokens, top_k and groups (a second tensor of the same tokens).
+ * The outputs overlap no input. */
+int mx_dispatch(mx_ctx* ctx, const int32_t* ids, int32_t tokens, int32_t top_k, int32_t groups, const mx_row_plan* plan,
+                const void* x, int32_t dtype, int64_t width, const float* weights, void* rows, float* row_weights,
+                void* stream);
+/* y[t] = sum over the token's rows r, in ascending row (so ascending expert) order, of weights[p] * rows[r], plus
+ * shared[t] last: in FP32, rounded once. weights NULL = unweighted (the route weights acted before the experts' last
+ * product), shared NULL = none; a token without rows gets zero (plus shared). Without weights the sums are
+ * MoEAccumulator's, bit for bit. y may be shared. */
+int mx_combine(mx_ctx* ctx, const void* rows, int32_t dtype, const int32_t* pair_row, const float* weights,
+               const void* shared, int32_t tokens, int32_t top_k, int64_t width, void* y, void* stream);
+/* Gradients of mx_combine for dy [T][width]: drows[r] = weights[p] * dy[t] (rounded once; weights NULL = 1) and
+ * dweights[p] = <rows[r], dy[t]> in FP32, 0 for a pair without a row. Either may be NULL; rows may be NULL without
+ * dweights. (The gradient of shared is dy.) drows may be rows. */
+int mx_combine_backward(mx_ctx* ctx, const void* dy, const void* rows, int32_t dtype, const int32_t* pair_row,
+                        const float* weights, int32_t tokens, int32_t top_k, int64_t width, void* drows,
+                        float* dweights, void* stream);
+/* Gradients of mx_dispatch: dx[t] = the sum of the token's drows in ascending row order, in FP32, rounded once, and
+ * dweights[p] = drow_weights[pair_row[p]], 0 for a pair without a row (both or neither of these two). */
+int mx_dispatch_backward(mx_ctx* ctx, const void* drows, int32_t dtype, const int32_t* pair_row,
+                         const float* drow_weights, int32_t tokens, int32_t top_k, int64_t width, void* dx,
+                         float* dweights, void* stream);
+
 /* ---- routed MoE layer (replaces ConnectedMoE.forward, src/vesper/connected.py:125-186) ---- */
 
 typedef struct mx_moe_config {

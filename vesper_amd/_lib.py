@@ -19,6 +19,7 @@ LIB_PATH = PKG / "libmxmoe.so"
 
 MX_OK, MX_ERR_INVALID, MX_ERR_MEMORY, MX_ERR_STATE, MX_ERR_HIP = 0, -1, -2, -3, -4
 MX_FMT_MXFP4, MX_FMT_FP8_BLOCK32 = 0, 1
+MX_ROWS = {"bf16": 0, "f32": 1, "u8": 2}
 MX_SCORE = {"sigmoid": 0, "sqrtsoftplus": 1}
 BUFFERS = {"logits": 0, "scores": 1, "selection": 2, "indices": 3, "weights": 4, "xq": 5, "xs": 6, "plan": 7,
            "w1": 8, "w3": 9, "down_input": 10, "down_q": 11, "down_s": 12, "expert_out": 13, "trace": 14,
@@ -51,6 +52,10 @@ class MxMoeConfig(C.Structure):
     _fields_ = [("hidden", C.c_int32), ("intermediate", C.c_int32), ("experts", C.c_int32),
                 ("top_k", C.c_int32), ("score_func", C.c_int32), ("route_scale", C.c_float),
                 ("swiglu_limit", C.c_float), ("shared_format", C.c_int32), ("max_tokens", C.c_int32)]
+
+
+class MxRowPlan(C.Structure):
+    _fields_ = [(name, C.c_void_p) for name in ("first", "pair_row", "row_pair")]
 
 
 _P, _I32, _I64, _U64, _F = C.c_void_p, C.c_int32, C.c_int64, C.c_uint64, C.c_float
@@ -95,6 +100,10 @@ SIGNATURES = {
     "mx_acc_add_rows": ([_P, _P, _P, _P, _I32, _I32, _P], C.c_int),
     "mx_acc_add": ([_P, _P, _P, _I64, _P], C.c_int),
     "mx_acc_finish": ([_P, _P, _P, _I64, _P], C.c_int),
+    "mx_dispatch": ([_P, _P, _I32, _I32, _I32, C.POINTER(MxRowPlan), _P, _I32, _I64, _P, _P, _P, _P], C.c_int),
+    "mx_combine": ([_P, _P, _I32, _P, _P, _P, _I32, _I32, _I64, _P, _P], C.c_int),
+    "mx_combine_backward": ([_P, _P, _P, _I32, _P, _P, _I32, _I32, _I64, _P, _P, _P], C.c_int),
+    "mx_dispatch_backward": ([_P, _P, _I32, _P, _P, _I32, _I32, _I64, _P, _P, _P], C.c_int),
     "mx_tiled_expert_bytes": ([_I32, _I32], _U64),
     "mx_tile_expert": ([_P, C.POINTER(MxExpertPtrs), _I32, _I32, _P, _P], C.c_int),
     "mx_untile_expert": ([_P, _P, _I32, _I32, C.POINTER(MxExpertPtrs), _P], C.c_int),

@@ -1,0 +1,467 @@
+// Tokens sorted by expert and back: the plan, the rows in expert order, the weighted sum per token, and the gradients
+// of both, for experts of any format (the fused MXFP4 layer, mx_moe_prefill, keeps a plan and rows of its own).
+//
+// P = T k pairs p = t k + j; key(p) = ids[p] where that is in [0, G), else G. The plan is the stable order by key:
+//   row(p) = #{q: key(q) < key(p)} + #{q < p: key(q) = key(p)},   first[g] = #{q: key(q) < g}
+// so a group's rows are in ascending token order, as the reference's participation orders them
+// (src/vesper/moe.py:18-30), and pairs without a group come last. Everything is counted with ballots over the ids: no
+// atomics, the same plan on every run.
+//
+// combine adds a token's rows in ascending row (so ascending expert) order in FP32 from zero, the shared row last, and
+// rounds once: without weights the sums of MoEAccumulator (src/vesper/moe.py:42-148), bit for bit.
+#include "mx_device.h"
+#include "mx_internal.h"
+#include "mx_numerics.h"
+
+namespace {
+
+constexpr int kMaxTokens = 1 << 18;   // keeps every grid below 2^32 threads
+constexpr int kMaxTopK = 32, kMaxGroups = 1024;
+constexpr int64_t kMaxWidth = 1 << 24;
+
+// ---- plan ----
+
+constexpr int kPlanThreads = 1024, kPlanWaves = kPlanThreads / 64;
+
+struct PlanArgs {
+  const int32_t* ids;
+  int32_t pairs, groups;
+  int32_t* first;
+  int32_t* pair_row;
+  int32_t* row_pair;
+};
+
+__device__ __forceinline__ int pair_key(const PlanArgs& a, int p) {
+  const int id = a.ids[p];
+  return id >= 0 && id < a.groups ? id : a.groups;
+}
+
+// Workgroup g places the pairs of key g (g = G: the pairs without a group). Each wave takes a contiguous section of the
+// pairs, 64 at a time: the pairs of smaller keys and of its own are counted with ballots, and the second walk places
+// its own in order.
+__global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanArgs a) {
+  __shared__ int less[kPlanWaves], same[kPlanWaves];
+  const int g = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int section = (a.pairs + kPlanThreads - 1) / kPlanThreads * 64;
+  const int p0 = min(wave * section, a.pairs), p1 = min(p0 + section, a.pairs);
+  int n_less = 0, n_same = 0;
+  for (int p = p0; p < p1; p += 64) {
+    const bool in = p + lane < p1;
+    const int key = in ? pair_key(a, p + lane) : kMaxGroups + 1;
+    n_less += __popcll(__ballot(key < g));
+    n_same += __popcll(__ballot(key == g));
+  }
+  if (lane == 0) {
+    less[wave] = n_less;
+    same[wave] = n_same;
+  }
+  __syncthreads();
+  int base = 0, row = 0;
+  for (int w = 0; w < kPlanWaves; ++w) {
+    base += less[w];
+    if (w < wave) row += same[w];
+  }
+  if (tid == 0) a.first[g] = base;
+  row += base;
+  for (int p = p0; p < p1; p += 64) {
+    const bool mine = p + lane < p1 && pair_key(a, p + lane) == g;
+    const uint64_t mask = __ballot(mine);
+    if (mine) {
+      const int r = row + __popcll(mask & ((1ull << lane) - 1));
+      a.row_pair[r] = p + lane;
+      a.pair_row[p + lane] = g < a.groups ? r : -1;
+    }
+    row += __popcll(mask);
+  }
+}
+
+// ---- dispatch ----
+
+struct DispatchArgs {
+  const int32_t* pair_row;
+  int32_t tokens, k;
+  const uint8_t* x;
+  uint8_t* rows;
+  int64_t units;          // units of the copy per row
+  const float* weights;
+  float* row_weights;
+};
+
+// grid (T, chunks): the token's row is read once and written to each of its rows. U is the widest unit that the row's
+// bytes and the pointers allow.
+template <typename U>
+__global__ __launch_bounds__(256) void dispatch_kernel(DispatchArgs a) {
+  __shared__ int dst[kMaxTopK];
+  const int t = blockIdx.x, tid = threadIdx.x, k = a.k, pairs = a.tokens * k;
+  if (tid < k) {
+    const int r = a.pair_row[t * k + tid];
+    const bool ok = r >= 0 && r < pairs;
+    dst[tid] = ok ? r : -1;
+    if (ok && a.row_weights && blockIdx.y == 0) a.row_weights[r] = a.weights[t * k + tid];
+  }
+  __syncthreads();
+  const U* x = (const U*)a.x + (int64_t)t * a.units;
+  for (int64_t c = (int64_t)blockIdx.y * 256 + tid; c < a.units; c += (int64_t)gridDim.y * 256) {
+    const U v = x[c];
+    for (int j = 0; j < k; ++j) {
+      const int r = __builtin_amdgcn_readfirstlane(dst[j]);
+      if (r >= 0) ((U*)a.rows)[(int64_t)r * a.units + c] = v;
+    }
+  }
+}
+
+// ---- units of a row as FP32 values ----
+
+template <int kType, int V>
+struct Unit;
+
+template <>
+struct Unit<MX_ROWS_BF16, 8> {
+  typedef uint4 Raw;
+  static __device__ __forceinline__ void values(const Raw& r, float* v) {
+    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[2 * i] = mx::u2f(w[i] << 16);
+      v[2 * i + 1] = mx::u2f(w[i] & 0xFFFF0000u);
+    }
+  }
+  static __device__ __forceinline__ Raw round(const float* v) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = mx::bf16_bits(v[2 * i]) | (mx::bf16_bits(v[2 * i + 1]) << 16);
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+};
+
+template <>
+struct Unit<MX_ROWS_BF16, 1> {
+  typedef uint16_t Raw;
+  static __device__ __forceinline__ void values(const Raw& r, float* v) { v[0] = mx::bf16_value(r); }
+  static __device__ __forceinline__ Raw round(const float* v) { return (uint16_t)mx::bf16_bits(v[0]); }
+};
+
+template <>
+struct Unit<MX_ROWS_F32, 4> {
+  typedef uint4 Raw;
+  static __device__ __forceinline__ void values(const Raw& r, float* v) {
+    v[0] = mx::u2f(r.x), v[1] = mx::u2f(r.y), v[2] = mx::u2f(r.z), v[3] = mx::u2f(r.w);
+  }
+  static __device__ __forceinline__ Raw round(const float* v) {
+    return make_uint4(mx::f2u(v[0]), mx::f2u(v[1]), mx::f2u(v[2]), mx::f2u(v[3]));
+  }
+};
+
+template <>
+struct Unit<MX_ROWS_F32, 1> {
+  typedef float Raw;
+  static __device__ __forceinline__ void values(const Raw& r, float* v) { v[0] = r; }
+  static __device__ __forceinline__ Raw round(const float* v) { return v[0]; }
+};
+
+// ---- combine, and the backward pass of dispatch ----
+
+struct CombineArgs {
+  const void* rows;
+  const int32_t* pair_row;
+  const float* weights;        // [T][k] or null
+  const void* shared;          // [T][width] or null
+  void* y;
+  int32_t tokens, k;
+  int64_t units;               // units per row
+  const float* row_weights;    // dispatch_backward: the gradient of each row's weight, and
+  float* dweights;             // where it goes
+};
+
+// grid (T, chunks), a unit of 16 bytes (or one value) a thread. The wave that finds the order counts, for each of the
+// token's rows, the rows before it.
+template <int kType, int V>
+__global__ __launch_bounds__(128) void combine_kernel(CombineArgs a) {
+  using X = Unit<kType, V>;
+  using Raw = typename X::Raw;
+  __shared__ int row[kMaxTopK];
+  __shared__ float weight[kMaxTopK];
+  __shared__ int count;
+  const int t = blockIdx.x, tid = threadIdx.x, k = a.k, pairs = a.tokens * k;
+  if (tid < 64) {
+    int r = -1;
+    if (tid < k) {
+      r = a.pair_row[t * k + tid];
+      r = r >= 0 && r < pairs ? r : -1;
+    }
+    int before = 0;
+    for (int j = 0; j < k; ++j) {
+      const int o = __shfl(r, j, 64);
+      before += o >= 0 && (o < r || (o == r && j < tid));
+    }
+    if (r >= 0) {
+      row[before] = r;
+      weight[before] = a.weights ? a.weights[t * k + tid] : 1.f;
+    }
+    const uint64_t live = __ballot(r >= 0);
+    if (tid == 0) count = __popcll(live);
+    if (a.dweights && blockIdx.y == 0 && tid < k) a.dweights[t * k + tid] = r >= 0 ? a.row_weights[r] : 0.f;
+  }
+  __syncthreads();
+  const int n = __builtin_amdgcn_readfirstlane(count);
+  const bool weighted = a.weights != nullptr;
+  for (int64_t c = (int64_t)blockIdx.y * 128 + tid; c < a.units; c += (int64_t)gridDim.y * 128) {
+    float acc[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) acc[i] = 0.f;
+    for (int j0 = 0; j0 < n; j0 += 8) {
+      Raw raw[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (j0 + j < n)
+          raw[j] = ((const Raw*)a.rows)[(int64_t)__builtin_amdgcn_readfirstlane(row[j0 + j]) * a.units + c];
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (j0 + j < n) {
+          float v[V];
+          X::values(raw[j], v);
+          const float w = weight[j0 + j];
+#pragma unroll
+          for (int i = 0; i < V; ++i) acc[i] = acc[i] + (weighted ? w * v[i] : v[i]);
+        }
+    }
+    if (a.shared) {
+      float v[V];
+      X::values(((const Raw*)a.shared)[(int64_t)t * a.units + c], v);
+#pragma unroll
+      for (int i = 0; i < V; ++i) acc[i] = acc[i] + v[i];
+    }
+    ((Raw*)a.y)[(int64_t)t * a.units + c] = X::round(acc);
+  }
+}
+
+// ---- the backward pass of combine ----
+
+struct CombineBwdArgs {
+  const void* dy;
+  const void* rows;            // null: no gradient of the weights
+  const int32_t* pair_row;
+  const float* weights;
+  void* drows;                 // null: no gradient of the rows
+  float* dweights;
+  int32_t tokens, k;
+  int64_t units;
+};
+
+// One workgroup a pair: drows[row] = w dy[t] and dw = <rows[row], dy[t]>, both from one read of dy and of the row. Each
+// thread adds its products in order, the lanes are added as a tree and the waves in order. A token's pairs run on one
+// XCD (workgroups go round the eight of them), so its dy comes from HBM once and from that L2 after.
+template <int kType, int V>
+__global__ __launch_bounds__(256) void combine_backward_kernel(CombineBwdArgs a) {
+  using X = Unit<kType, V>;
+  using Raw = typename X::Raw;
+  __shared__ float part[4];
+  const int tid = threadIdx.x, k = a.k, pairs = a.tokens * k;
+  const int i = blockIdx.x >> 3;
+  const int t = i / k * 8 + (blockIdx.x & 7), j = i % k;
+  if (t >= a.tokens) return;
+  const int r = a.pair_row[t * k + j];
+  if (r < 0 || r >= pairs) {
+    if (a.dweights && tid == 0) a.dweights[t * k + j] = 0.f;
+    return;
+  }
+  const float w = a.weights ? a.weights[t * k + j] : 1.f;
+  const Raw* dy = (const Raw*)a.dy + (int64_t)t * a.units;
+  const Raw* row = (const Raw*)a.rows + (int64_t)r * a.units;
+  Raw* out = (Raw*)a.drows + (int64_t)r * a.units;
+  float dot = 0.f;
+  for (int64_t c = tid; c < a.units; c += 256) {
+    float g[V], v[V];
+    X::values(dy[c], g);
+    if (a.dweights) {
+      X::values(row[c], v);
+#pragma unroll
+      for (int e = 0; e < V; ++e) dot = dot + g[e] * v[e];
+    }
+    if (a.drows) {
+#pragma unroll
+      for (int e = 0; e < V; ++e) g[e] = a.weights ? w * g[e] : g[e];
+      out[c] = X::round(g);
+    }
+  }
+  if (!a.dweights) return;
+#pragma unroll
+  for (int m = 32; m >= 1; m >>= 1) dot = dot + __shfl_xor(dot, m, 64);
+  if ((tid & 63) == 0) part[tid >> 6] = dot;
+  __syncthreads();
+  if (tid == 0) a.dweights[t * k + j] = ((part[0] + part[1]) + part[2]) + part[3];
+}
+
+bool is_aligned(const void* p, uintptr_t a) { return ((uintptr_t)p & (a - 1)) == 0; }
+
+int check_routing(const char* who, int32_t tokens, int32_t top_k) {
+  MX_REQUIRE(tokens >= 0 && tokens <= kMaxTokens, "%s: token count %d outside [0, %d]", who, tokens, kMaxTokens);
+  MX_REQUIRE(top_k >= 1 && top_k <= kMaxTopK, "%s: %d groups per token outside [1, %d]", who, top_k, kMaxTopK);
+  return MX_OK;
+}
+
+int check_plan(const char* who, const mx_row_plan* plan) {
+  MX_REQUIRE(plan && plan->first && plan->pair_row && plan->row_pair, "%s: plan pointer is null", who);
+  MX_REQUIRE(is_aligned(plan->first, 4) && is_aligned(plan->pair_row, 4) && is_aligned(plan->row_pair, 4),
+             "%s: plan arrays must be 4-byte aligned", who);
+  return MX_OK;
+}
+
+int check_rows(const char* who, int32_t dtype, int64_t width, bool bytes_too) {
+  MX_REQUIRE(dtype == MX_ROWS_BF16 || dtype == MX_ROWS_F32 || (bytes_too && dtype == MX_ROWS_U8), "%s: row type %d",
+             who, dtype);
+  MX_REQUIRE(width >= 1 && width <= kMaxWidth, "%s: row width %lld outside [1, %lld]", who, (long long)width,
+             (long long)kMaxWidth);
+  return MX_OK;
+}
+
+int64_t element_bytes(int32_t dtype) { return dtype == MX_ROWS_F32 ? 4 : dtype == MX_ROWS_BF16 ? 2 : 1; }
+
+// workgroups along a row of `units`, `per` of them a workgroup
+unsigned chunks_of(int64_t units, int per) {
+  const int64_t n = (units + per - 1) / per;
+  return (unsigned)(n < 64 ? n : 64);
+}
+
+template <typename U>
+int launch_dispatch(DispatchArgs a, int64_t row_bytes, hipStream_t st) {
+  a.units = row_bytes / (int64_t)sizeof(U);
+  hipLaunchKernelGGL((dispatch_kernel<U>), dim3(a.tokens, chunks_of(a.units, 256)), dim3(256), 0, st, a);
+  MX_LAUNCH_CHECK("dispatch_kernel");
+  return MX_OK;
+}
+
+template <int kType, int V>
+int launch_combine(CombineArgs a, int64_t width, hipStream_t st) {
+  a.units = width / V;
+  hipLaunchKernelGGL((combine_kernel<kType, V>), dim3(a.tokens, chunks_of(a.units, 128)), dim3(128), 0, st, a);
+  MX_LAUNCH_CHECK("combine_kernel");
+  return MX_OK;
+}
+
+int combine_any(const CombineArgs& a, int32_t dtype, int64_t width, hipStream_t st) {
+  const bool wide = (width * element_bytes(dtype)) % 16 == 0 && is_aligned(a.rows, 16) && is_aligned(a.y, 16) &&
+                    (!a.shared || is_aligned(a.shared, 16));
+  if (dtype == MX_ROWS_BF16)
+    return wide ? launch_combine<MX_ROWS_BF16, 8>(a, width, st) : launch_combine<MX_ROWS_BF16, 1>(a, width, st);
+  return wide ? launch_combine<MX_ROWS_F32, 4>(a, width, st) : launch_combine<MX_ROWS_F32, 1>(a, width, st);
+}
+
+template <int kType, int V>
+int launch_combine_backward(CombineBwdArgs a, int64_t width, hipStream_t st) {
+  a.units = width / V;
+  const unsigned grid = (unsigned)((a.tokens + 7) / 8 * 8 * a.k);
+  hipLaunchKernelGGL((combine_backward_kernel<kType, V>), dim3(grid), dim3(256), 0, st, a);
+  MX_LAUNCH_CHECK("combine_backward_kernel");
+  return MX_OK;
+}
+
+}  // namespace
+
+using mxi::as_stream;
+using mxi::use;
+
+int mxi::row_plan(const int32_t* ids, int32_t pairs, int32_t groups, const mx_row_plan& plan, hipStream_t st) {
+  const PlanArgs a{ids, pairs, groups, plan.first, plan.pair_row, plan.row_pair};
+  hipLaunchKernelGGL(plan_kernel, dim3(groups + 1), dim3(kPlanThreads), 0, st, a);
+  MX_LAUNCH_CHECK("plan_kernel");
+  return MX_OK;
+}
+
+extern "C" {
+
+int mx_dispatch(mx_ctx* ctx, const int32_t* ids, int32_t tokens, int32_t top_k, int32_t groups, const mx_row_plan* plan,
+                const void* x, int32_t dtype, int64_t width, const float* weights, void* rows, float* row_weights,
+                void* stream) {
+  const char* who = "mx_dispatch";
+  if (int s = check_routing(who, tokens, top_k)) return s;
+  MX_REQUIRE(groups >= 1 && groups <= kMaxGroups, "%s: %d groups outside [1, %d]", who, groups, kMaxGroups);
+  if (int s = check_plan(who, plan)) return s;
+  MX_REQUIRE((x == nullptr) == (rows == nullptr), "%s: x and rows are given together or not at all", who);
+  MX_REQUIRE((weights == nullptr) == (row_weights == nullptr), "%s: weights and row_weights are given together", who);
+  MX_REQUIRE(ids || x, "%s: neither ids for a plan nor rows to move", who);
+  MX_REQUIRE(x || !weights, "%s: weights move with rows", who);
+  MX_REQUIRE(is_aligned(ids, 4) && is_aligned(weights, 4) && is_aligned(row_weights, 4),
+             "%s: ids and weights must be 4-byte aligned", who);
+  if (x) {
+    if (int s = check_rows(who, dtype, width, true)) return s;
+    MX_REQUIRE(is_aligned(x, element_bytes(dtype)) && is_aligned(rows, element_bytes(dtype)),
+               "%s: x and rows must be aligned to their elements", who);
+  }
+  if (int s = use(ctx)) return s;
+  hipStream_t st = as_stream(stream);
+  if (ids)
+    if (int s = mxi::row_plan(ids, tokens * top_k, groups, *plan, st)) return s;
+  if (!x || !tokens) return MX_OK;
+  DispatchArgs a{plan->pair_row, tokens, top_k, (const uint8_t*)x, (uint8_t*)rows, 0, weights, row_weights};
+  const int64_t bytes = width * element_bytes(dtype);
+  const uint64_t low = (uint64_t)(uintptr_t)x | (uint64_t)(uintptr_t)rows | (uint64_t)bytes;
+  if (low % 16 == 0) return launch_dispatch<uint4>(a, bytes, st);
+  if (low % 4 == 0) return launch_dispatch<uint32_t>(a, bytes, st);
+  if (low % 2 == 0) return launch_dispatch<uint16_t>(a, bytes, st);
+  return launch_dispatch<uint8_t>(a, bytes, st);
+}
+
+int mx_combine(mx_ctx* ctx, const void* rows, int32_t dtype, const int32_t* pair_row, const float* weights,
+               const void* shared, int32_t tokens, int32_t top_k, int64_t width, void* y, void* stream) {
+  const char* who = "mx_combine";
+  if (int s = check_routing(who, tokens, top_k)) return s;
+  if (int s = check_rows(who, dtype, width, false)) return s;
+  MX_REQUIRE(rows && pair_row && y, "%s: null pointer", who);
+  const int64_t size = element_bytes(dtype);
+  MX_REQUIRE(is_aligned(rows, size) && is_aligned(y, size) && is_aligned(shared, size) && is_aligned(pair_row, 4) &&
+                 is_aligned(weights, 4),
+             "%s: pointers must be aligned to their elements", who);
+  if (int s = use(ctx)) return s;
+  if (!tokens) return MX_OK;
+  const CombineArgs a{rows, pair_row, weights, shared, y, tokens, top_k, 0, nullptr, nullptr};
+  return combine_any(a, dtype, width, as_stream(stream));
+}
+
+int mx_combine_backward(mx_ctx* ctx, const void* dy, const void* rows, int32_t dtype, const int32_t* pair_row,
+                        const float* weights, int32_t tokens, int32_t top_k, int64_t width, void* drows,
+                        float* dweights, void* stream) {
+  const char* who = "mx_combine_backward";
+  if (int s = check_routing(who, tokens, top_k)) return s;
+  if (int s = check_rows(who, dtype, width, false)) return s;
+  MX_REQUIRE(dy && pair_row, "%s: null pointer", who);
+  MX_REQUIRE(drows || dweights, "%s: no gradient asked for", who);
+  MX_REQUIRE(!dweights || rows, "%s: the gradient of the weights needs the rows", who);
+  const int64_t size = element_bytes(dtype);
+  MX_REQUIRE(is_aligned(dy, size) && is_aligned(rows, size) && is_aligned(drows, size) && is_aligned(pair_row, 4) &&
+                 is_aligned(weights, 4) && is_aligned(dweights, 4),
+             "%s: pointers must be aligned to their elements", who);
+  if (int s = use(ctx)) return s;
+  if (!tokens) return MX_OK;
+  const CombineBwdArgs a{dy, rows, pair_row, weights, drows, dweights, tokens, top_k, 0};
+  const bool wide = (width * size) % 16 == 0 && is_aligned(dy, 16) && (!dweights || is_aligned(rows, 16)) &&
+                    is_aligned(drows, 16);
+  hipStream_t st = as_stream(stream);
+  if (dtype == MX_ROWS_BF16)
+    return wide ? launch_combine_backward<MX_ROWS_BF16, 8>(a, width, st)
+                : launch_combine_backward<MX_ROWS_BF16, 1>(a, width, st);
+  return wide ? launch_combine_backward<MX_ROWS_F32, 4>(a, width, st)
+              : launch_combine_backward<MX_ROWS_F32, 1>(a, width, st);
+}
+
+int mx_dispatch_backward(mx_ctx* ctx, const void* drows, int32_t dtype, const int32_t* pair_row,
+                         const float* drow_weights, int32_t tokens, int32_t top_k, int64_t width, void* dx,
+                         float* dweights, void* stream) {
+  const char* who = "mx_dispatch_backward";
+  if (int s = check_routing(who, tokens, top_k)) return s;
+  if (int s = check_rows(who, dtype, width, false)) return s;
+  MX_REQUIRE(drows && pair_row && dx, "%s: null pointer", who);
+  MX_REQUIRE((drow_weights == nullptr) == (dweights == nullptr), "%s: drow_weights and dweights are given together",
+             who);
+  const int64_t size = element_bytes(dtype);
+  MX_REQUIRE(is_aligned(drows, size) && is_aligned(dx, size) && is_aligned(pair_row, 4) &&
+                 is_aligned(drow_weights, 4) && is_aligned(dweights, 4),
+             "%s: pointers must be aligned to their elements", who);
+  if (int s = use(ctx)) return s;
+  if (!tokens) return MX_OK;
+  const CombineArgs a{drows, pair_row, nullptr, nullptr, dx, tokens, top_k, 0, drow_weights, dweights};
+  return combine_any(a, dtype, width, as_stream(stream));
+}
+
+}  // extern "C"
