@@ -376,6 +376,32 @@ int mx_dispatch_backward(mx_ctx* ctx, const void* drows, int32_t dtype, const in
                          const float* drow_weights, int32_t tokens, int32_t top_k, int64_t width, void* dx,
                          float* dweights, void* stream);
 
+/* ---- low-rank adapters of many requests beside a projection (no counterpart in the reference) ----
+ *
+ * A bank holds `slots` adapters of one projection of n rows by k columns: down [rank][k] and up [n][rank], BF16, rank
+ * up to max_rank, and an FP32 scale each. n and k are multiples of 8 in [8, 2^20], slots in [1, 1024], max_rank in
+ * [1, 256]. Slots start empty. The bank's device memory counts towards the context's cap and goes back with
+ * mx_adapters_destroy, before the context's end. */
+typedef struct mx_adapters mx_adapters;
+int mx_adapters_create(mx_ctx* ctx, int32_t n, int32_t k, int32_t slots, int32_t max_rank, mx_adapters** out);
+int mx_adapters_destroy(mx_adapters* a);
+/* Fill `slot` from device memory, ordered on `stream` (rank 0, with NULL weights: empty it). Calls of
+ * mx_adapters_apply ordered after it see the new adapter. */
+int mx_adapters_load(mx_adapters* a, int32_t slot, const uint16_t* down, const uint16_t* up, int32_t rank, float scale,
+                     void* stream);
+/* Bytes of workspace (256-byte aligned device memory) for calls of up to `tokens` tokens. */
+uint64_t mx_adapters_workspace_bytes(const mx_adapters* a, int32_t tokens);
+/* y[t] = BF16(base[t] + scale up (down x[t])) with the adapter of slot ids[t] (device int32), in FP32 and rounded once
+ * (down x is taken into the second product as two BF16 terms, about 16 significant bits); BF16(base[t]) where ids[t] is
+ * outside [0, slots) or its slot empty. x BF16 [T][k], base [T][n] BF16 or FP32 (base_type MX_ROWS_BF16 / _F32: a
+ * projection's output, or its trace), y BF16 [T][n]; rows `stride` values apart (a multiple of 8; 4 for an FP32 base),
+ * all 16-byte aligned. y may be base (BF16, one stride); other overlaps are not supported. tokens in [0, 2^18].
+ * plan NULL, or mx_dispatch's plan of ids with top_k 1 and groups = slots (made once for all projections of a step);
+ * calls of few tokens do not use it. Calls that share a workspace must not overlap. */
+int mx_adapters_apply(mx_adapters* a, const uint16_t* x, int64_t x_stride, const int32_t* ids, const mx_row_plan* plan,
+                      int32_t tokens, const void* base, int32_t base_type, int64_t base_stride, uint16_t* y,
+                      int64_t y_stride, void* workspace, uint64_t workspace_bytes, void* stream);
+
 /* ---- routed MoE layer (replaces ConnectedMoE.forward, src/vesper/connected.py:125-186) ---- */
 
 typedef struct mx_moe_config {

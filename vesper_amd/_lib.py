@@ -104,6 +104,12 @@ SIGNATURES = {
     "mx_combine": ([_P, _P, _I32, _P, _P, _P, _I32, _I32, _I64, _P, _P], C.c_int),
     "mx_combine_backward": ([_P, _P, _P, _I32, _P, _P, _I32, _I32, _I64, _P, _P, _P], C.c_int),
     "mx_dispatch_backward": ([_P, _P, _I32, _P, _P, _I32, _I32, _I64, _P, _P, _P], C.c_int),
+    "mx_adapters_create": ([_P, _I32, _I32, _I32, _I32, C.POINTER(_P)], C.c_int),
+    "mx_adapters_destroy": ([_P], C.c_int),
+    "mx_adapters_load": ([_P, _I32, _P, _P, _I32, _F, _P], C.c_int),
+    "mx_adapters_workspace_bytes": ([_P, _I32], _U64),
+    "mx_adapters_apply": ([_P, _P, _I64, _P, C.POINTER(MxRowPlan), _I32, _P, _I32, _I64, _P, _I64, _P, _U64, _P],
+                          C.c_int),
     "mx_tiled_expert_bytes": ([_I32, _I32], _U64),
     "mx_tile_expert": ([_P, C.POINTER(MxExpertPtrs), _I32, _I32, _P, _P], C.c_int),
     "mx_untile_expert": ([_P, _P, _I32, _I32, C.POINTER(MxExpertPtrs), _P], C.c_int),

@@ -10,6 +10,10 @@ block 128 is BASELINE configuration 3 (FP32 scales per 128 x 128 block, per-toke
 activation scales, CONFIG3_LAYOUT shapes). Inputs are validated before any device work. The
 reference bounds a call to 8 rows; here any number of rows runs in one launch (16 tokens per MFMA
 column group), and `project_device` is the pointer-level fast path.
+
+`open_adapters(name, ...)` opens a bank of low-rank adapters beside a projection; `fp8(name, values, adapters=ids)` and
+`project_device(..., adapters_ptr=...)` then add each row's adapter to the projection's FP32 sums before the one rounding
+of the output.
 """
 
 from __future__ import annotations
@@ -21,6 +25,7 @@ import threading
 import numpy as np
 
 from . import _lib
+from .adapters import AdapterBank
 from .resources import MiB, MemoryBudget
 
 FP8_LAYOUT = {"wq_a": (1280, 5120), "wq_b": (32768, 1280), "wkv": (512, 5120), "wo_b": (5120, 8192)}
@@ -77,6 +82,7 @@ class NativeProjections:
         self.arrays, self.ordinal, self.layer, self.block = arrays, ordinal, layer, block
         self.lock, self.opened, self.ctx = threading.Lock(), False, None
         self.tiled = {}
+        self.banks = {}          # projection name -> its AdapterBank
         self.budget = MemoryBudget(cap=HOST_ALLOWANCE, owner="projections")
         self._device_peak = 0   # the context's peak owned bytes, kept past close for stats()
 
@@ -112,6 +118,8 @@ class NativeProjections:
                 raise
 
     def _close_context(self):
+        while self.banks:
+            self.banks.popitem()[1].close()
         self._device_peak = max(self._device_peak, self.ctx.owned_bytes()[1])
         self.ctx.close()
         self.ctx = None
@@ -133,15 +141,47 @@ class NativeProjections:
                 "owned_context_active": self.ctx is not None, "reservation_is_RSS_limit": False,
                 "driver_module_memory_excluded": True}
 
-    def project_device(self, name, x_ptr, tokens, y_ptr, stream=None, trace_ptr=None, q_ptr=None, s_ptr=None):
-        """y[T][rows] BF16 = projection of device BF16 x[T][width]; no host synchronisation."""
+    def open_adapters(self, name, slots, max_rank, max_tokens=4096) -> AdapterBank:
+        """The bank of `slots` low-rank adapters beside projection `name`, for calls of up to max_tokens rows; it
+        closes with the runtime (or earlier, by its close())."""
+        with self.lock:
+            self._ready()
+            if name not in self.layout:
+                raise ValueError("Unknown FP8 Attention projection")
+            if name in self.banks and self.banks[name].handle:
+                raise RuntimeError("Adapters of this projection are already open")
+            rows, width = self.layout[name]
+            self.banks[name] = AdapterBank(self.ctx, rows, width, slots, max_rank, min(max_tokens, MAX_ROWS))
+            return self.banks[name]
+
+    def _bank(self, name, tokens):
+        bank = self.banks.get(name)
+        if bank is None or not bank.handle:
+            raise ValueError("No adapters are open beside this projection")
+        if tokens > bank.max_tokens:
+            raise ValueError(f"the adapters of {name} were opened for {bank.max_tokens} rows a call")
+        return bank
+
+    def project_device(self, name, x_ptr, tokens, y_ptr, stream=None, trace_ptr=None, q_ptr=None, s_ptr=None,
+                       adapters_ptr=None, plan=None):
+        """y[T][rows] BF16 = projection of device BF16 x[T][width]; no host synchronisation.
+
+        adapters_ptr (device int32 [T], the slots of open_adapters, -1 for none) adds each row's adapter: to the FP32
+        sums where trace_ptr keeps them, else to y. x must then outlive the projection (y and trace apart from x);
+        plan as in AdapterBank.apply_device."""
         self._ready()
         rows, width = self.layout[name]
+        bank = None if adapters_ptr is None else self._bank(name, int(tokens))
         self.ctx.lib.fp8_projection(self.ctx._h(), C.c_void_p(self.tiled[name]), rows, width, self.block,
                                     C.c_void_p(int(x_ptr)), int(tokens), C.c_void_p(int(y_ptr)),
                                     _lib.vp(trace_ptr), _lib.vp(q_ptr), _lib.vp(s_ptr), _lib._stream(stream))
+        if bank is not None:
+            base, dtype = (y_ptr, "bf16") if trace_ptr is None else (trace_ptr, "f32")
+            bank.apply_device(x_ptr, adapters_ptr, tokens, base, y_ptr, dtype, plan=plan, stream=stream)
 
-    def fp8(self, name, values):
+    def fp8(self, name, values, adapters=None):
+        """The stage dict of one projection. adapters (int32 of values' leading shape, -1 for none): the slots whose
+        low-rank pairs are added to output_fp32 (which stays the projection's own) in output_bf16."""
         with self.lock:
             self._ready()
             if name not in self.layout:
@@ -149,21 +189,28 @@ class NativeProjections:
             rows, width = self.layout[name]
             tokens = validate_values(values, width)
             lead = values.shape[:-1]
+            ids = None
+            if adapters is not None:
+                ids = np.asarray(adapters)
+                if ids.shape != lead:
+                    raise ValueError("adapters must name one slot per row of values")
+                ids = self._bank(name, tokens).check_ids(ids.reshape(tokens), tokens)
             sdt, sw = (np.uint8, width // 32) if self.block == 32 else (np.float32, width // 128)
             x = self.ctx.upload(np.ascontiguousarray(values).reshape(tokens, width))
             q = self.ctx.empty((tokens, width), np.uint8)
             s = self.ctx.empty((tokens, sw), sdt)
             trace = self.ctx.empty((tokens, rows), np.float32)
             out = self.ctx.empty((tokens, rows), np.uint16)
+            slots = None if ids is None else self.ctx.upload(ids)
             try:
-                self.project_device(name, x.ptr, tokens, out.ptr, trace_ptr=trace, q_ptr=q, s_ptr=s)
+                self.project_device(name, x.ptr, tokens, out.ptr, trace_ptr=trace, q_ptr=q, s_ptr=s, adapters_ptr=slots)
                 scale_key = "scale_e8m0" if self.block == 32 else "scale_f32"
                 return {"input_fp8": q.download().reshape(*lead, width),
                         scale_key: s.download().reshape(*lead, sw),
                         "output_fp32": trace.download().reshape(*lead, rows),
                         "output_bf16": out.download().reshape(*lead, rows)}
             finally:
-                for d in (x, q, s, trace, out):
+                for d in (x, q, s, trace, out) + (() if slots is None else (slots,)):
                     d.free()
 
     def grouped(self, values):
