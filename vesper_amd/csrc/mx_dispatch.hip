@@ -9,6 +9,8 @@
 //
 // combine adds a token's rows in ascending row (so ascending expert) order in FP32 from zero, the shared row last, and
 // rounds once: without weights the sums of MoEAccumulator (src/vesper/moe.py:42-148), bit for bit.
+#include <algorithm>
+
 #include "mx_device.h"
 #include "mx_internal.h"
 #include "mx_numerics.h"
@@ -18,6 +20,8 @@ namespace {
 constexpr int kMaxTokens = 1 << 18;   // keeps every grid below 2^32 threads
 constexpr int kMaxTopK = 32, kMaxGroups = 1024;
 constexpr int64_t kMaxWidth = 1 << 24;
+constexpr int kFusedPairs = 2048;   // up to this many pairs the plan is made within the dispatch launch
+constexpr int kFewTokens = 512;     // below, a token's row is cut over several workgroups
 
 // ---- plan ----
 
@@ -36,50 +40,109 @@ __device__ __forceinline__ int pair_key(const PlanArgs& a, int p) {
   return id >= 0 && id < a.groups ? id : a.groups;
 }
 
-// Workgroup g places the pairs of key g (g = G: the pairs without a group). Each wave takes a contiguous section of the
-// pairs, 64 at a time: the pairs of smaller keys and of its own are counted with ballots, and the second walk places
-// its own in order.
-__global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanArgs a) {
-  __shared__ int less[kPlanWaves], same[kPlanWaves];
-  const int g = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
+// Workgroup g places the pairs of key g (kAbsent: g = G, the pairs without a group). Each wave takes a contiguous section
+// of the pairs, 64 at a time: every lane counts the smaller keys and its own key among its pairs (as unsigned numbers,
+// ids below zero are no smaller key; pairs past the section count as ids past the last), and the second walk places the
+// key's pairs in order. kBatch loads are in flight together, and a section of one batch stays in registers for the
+// second walk. Every workgroup reads all the ids, from the L2s: what counts is the instructions per 64 of them.
+template <bool kAbsent, int kBatch>
+__device__ __forceinline__ void place_key(const PlanArgs& a, int g, int (*sums)[2]) {
+  const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int section = (a.pairs + kPlanThreads - 1) / kPlanThreads * 64;
   const int p0 = min(wave * section, a.pairs), p1 = min(p0 + section, a.pairs);
-  int n_less = 0, n_same = 0;
-  for (int p = p0; p < p1; p += 64) {
-    const bool in = p + lane < p1;
-    const int key = in ? pair_key(a, p + lane) : kMaxGroups + 1;
-    n_less += __popcll(__ballot(key < g));
-    n_same += __popcll(__ballot(key == g));
+  uint32_t id[kBatch];
+  auto load = [&](int at) {
+    if (at + 64 * kBatch <= p1) {
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) id[i] = (uint32_t)a.ids[at + 64 * i + lane];
+    } else {
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) id[i] = (uint32_t)a.ids[min(at + 64 * i + lane, a.pairs - 1)];
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) id[i] = at + 64 * i + lane < p1 ? id[i] : ~0u;
+    }
+  };
+  auto own = [&](int at, int i) {
+    if constexpr (kAbsent) return id[i] >= (uint32_t)g && at + 64 * i + lane < p1;
+    return id[i] == (uint32_t)g;
+  };
+  int less = 0, same = 0;
+  for (int at = p0; at < p1; at += 64 * kBatch) {
+    load(at);
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      less += id[i] < (uint32_t)g;
+      same += own(at, i);
+    }
+  }
+#pragma unroll
+  for (int m = 32; m >= 1; m >>= 1) {
+    less += __shfl_xor(less, m, 64);
+    same += __shfl_xor(same, m, 64);
   }
   if (lane == 0) {
-    less[wave] = n_less;
-    same[wave] = n_same;
+    sums[wave][0] = less;
+    sums[wave][1] = same;
   }
   __syncthreads();
   int base = 0, row = 0;
+#pragma unroll
   for (int w = 0; w < kPlanWaves; ++w) {
-    base += less[w];
-    if (w < wave) row += same[w];
+    base += sums[w][0];
+    row += w < wave ? sums[w][1] : 0;
   }
   if (tid == 0) a.first[g] = base;
+  if (__builtin_amdgcn_readfirstlane(same) == 0) return;
   row += base;
-  for (int p = p0; p < p1; p += 64) {
-    const bool mine = p + lane < p1 && pair_key(a, p + lane) == g;
-    const uint64_t mask = __ballot(mine);
-    if (mine) {
-      const int r = row + __popcll(mask & ((1ull << lane) - 1));
-      a.row_pair[r] = p + lane;
-      a.pair_row[p + lane] = g < a.groups ? r : -1;
+  const bool reload = section > 64 * kBatch;
+  for (int at = p0; at < p1; at += 64 * kBatch) {
+    if (reload) load(at);
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      const bool mine = own(at, i);
+      const uint64_t mask = __ballot(mine);
+      if (mask == 0) continue;
+      if (mine) {
+        const int r = row + __popcll(mask & ((1ull << lane) - 1)), p = at + 64 * i + lane;
+        a.row_pair[r] = p;
+        a.pair_row[p] = kAbsent ? -1 : r;
+      }
+      row += __popcll(mask);
     }
-    row += __popcll(mask);
+  }
+}
+
+template <int kBatch>
+__global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanArgs a) {
+  __shared__ int sums[kPlanWaves][2];
+  const int g = blockIdx.x;
+  if (g == a.groups) place_key<true, kBatch>(a, g, sums);
+  else place_key<false, kBatch>(a, g, sums);
+}
+
+// Streaming access to rows that a call touches once.
+template <typename R>
+__device__ __forceinline__ R load_once(const R* p) {
+  if constexpr (sizeof(R) == 16) {
+    return __builtin_bit_cast(R, __builtin_nontemporal_load((const mxd::u32x4_t*)p));
+  } else {
+    return __builtin_nontemporal_load(p);
+  }
+}
+template <typename R>
+__device__ __forceinline__ void store_once(R* p, const R& v) {
+  if constexpr (sizeof(R) == 16) {
+    __builtin_nontemporal_store(__builtin_bit_cast(mxd::u32x4_t, v), (mxd::u32x4_t*)p);
+  } else {
+    __builtin_nontemporal_store(v, p);
   }
 }
 
 // ---- dispatch ----
 
 struct DispatchArgs {
-  const int32_t* pair_row;
+  PlanArgs plan;
   int32_t tokens, k;
   const uint8_t* x;
   uint8_t* rows;
@@ -88,17 +151,103 @@ struct DispatchArgs {
   float* row_weights;
 };
 
-// grid (T, chunks): the token's row is read once and written to each of its rows. U is the widest unit that the row's
-// bytes and the pointers allow.
+// The rows of the plan for one token by counting, for each of its pairs, the pairs before it: wave w counts over a
+// quarter of the ids, which it holds in registers. dst[j] is the row (past first[G] for a pair without a group).
+__device__ __forceinline__ void count_rows(const DispatchArgs& a, int t, int* dst, int (*part)[kMaxTopK]) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int quarter = (a.plan.pairs + 255) / 256 * 64, p0 = wave * quarter, p1 = min(p0 + quarter, a.plan.pairs);
+  int key[kFusedPairs / 256];
+#pragma unroll
+  for (int i = 0; i < kFusedPairs / 256; ++i)
+    if (p0 + 64 * i < p1) key[i] = p0 + 64 * i + lane < p1 ? pair_key(a.plan, p0 + 64 * i + lane) : kMaxGroups + 1;
+  for (int j = 0; j < a.k; ++j) {
+    const int p = t * a.k + j, own = pair_key(a.plan, p);
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < kFusedPairs / 256; ++i)
+      if (p0 + 64 * i < p1) n += __popcll(__ballot(key[i] < own || (key[i] == own && p0 + 64 * i + lane < p)));
+    if (lane == 0) part[wave][j] = n;
+  }
+  __syncthreads();
+  if (tid < a.k) dst[tid] = part[0][tid] + part[1][tid] + part[2][tid] + part[3][tid];
+}
+
+// first[0..G] by one workgroup: the keys counted in LDS (integer additions: any order gives the same counts), then
+// summed.
+__device__ __forceinline__ void count_groups(const PlanArgs& a, int* count) {
+  __shared__ int wave_sum[4];
+  const int tid = threadIdx.x, lane = tid & 63;
+  for (int g = tid; g < kMaxGroups; g += 256) count[g] = 0;
+  __syncthreads();
+  for (int p = tid; p < a.pairs; p += 256) {
+    const int key = pair_key(a, p);
+    if (key < a.groups) atomicAdd(&count[key], 1);
+  }
+  __syncthreads();
+  int own = 0;
+#pragma unroll
+  for (int i = 0; i < kMaxGroups / 256; ++i) own += count[tid * (kMaxGroups / 256) + i];
+  int upto = own;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int o = __shfl_up(upto, d, 64);
+    if (lane >= d) upto += o;
+  }
+  if (lane == 63) wave_sum[tid >> 6] = upto;
+  __syncthreads();
+  int base = upto - own;
+  for (int w = 0; w < (tid >> 6); ++w) base += wave_sum[w];
+  for (int i = 0; i < kMaxGroups / 256; ++i) {
+    const int g = tid * (kMaxGroups / 256) + i;
+    if (g <= a.groups) a.first[g] = base;
+    base += count[g];
+  }
+  if (tid == 255 && a.groups == kMaxGroups) a.first[kMaxGroups] = base;
+}
+
+// The token's row is read once and written to each of its rows. U is the widest unit that the row's bytes and the
+// pointers allow.
+//
+// By a plan: one wave per token and piece of 64 units (chunks pieces a row; more units, more rounds).
+template <typename U>
+__global__ __launch_bounds__(64) void move_rows_kernel(DispatchArgs a, int chunks) {
+  const int t = blockIdx.x / chunks, chunk = blockIdx.x % chunks, lane = threadIdx.x, k = a.k, pairs = a.tokens * k;
+  if (a.row_weights && chunk == 0 && lane < k) {
+    const int r = a.plan.pair_row[t * k + lane];
+    if (r >= 0 && r < pairs) a.row_weights[r] = a.weights[t * k + lane];
+  }
+  const U* x = (const U*)a.x + (int64_t)t * a.units;
+  for (int64_t c = 64 * chunk + lane; c < a.units; c += 64 * chunks) {
+    const U v = x[c];
+    for (int j = 0; j < k; ++j) {
+      const int r = a.plan.pair_row[t * k + j];
+      if (r >= 0 && r < pairs) store_once((U*)a.rows + (int64_t)r * a.units + c, v);
+    }
+  }
+}
+
+// With the plan, in one launch for few pairs: grid (T + 1, chunks); every workgroup finds its own token's rows, the
+// first chunk's writes them, and the last column the groups' first rows.
 template <typename U>
 __global__ __launch_bounds__(256) void dispatch_kernel(DispatchArgs a) {
   __shared__ int dst[kMaxTopK];
-  const int t = blockIdx.x, tid = threadIdx.x, k = a.k, pairs = a.tokens * k;
+  __shared__ int part[4][kMaxTopK];
+  __shared__ int count[kMaxGroups];
+  const int t = blockIdx.x, tid = threadIdx.x, k = a.k;
+  if (t == a.tokens) {
+    if (blockIdx.y == 0) count_groups(a.plan, count);
+    return;
+  }
+  count_rows(a, t, dst, part);
   if (tid < k) {
-    const int r = a.pair_row[t * k + tid];
-    const bool ok = r >= 0 && r < pairs;
-    dst[tid] = ok ? r : -1;
-    if (ok && a.row_weights && blockIdx.y == 0) a.row_weights[r] = a.weights[t * k + tid];
+    const int p = t * k + tid, r = dst[tid];
+    const bool absent = pair_key(a.plan, p) == a.plan.groups;
+    if (blockIdx.y == 0) {
+      a.plan.row_pair[r] = p;
+      a.plan.pair_row[p] = absent ? -1 : r;
+      if (!absent && a.row_weights) a.row_weights[r] = a.weights[p];
+    }
+    dst[tid] = absent ? -1 : r;
   }
   __syncthreads();
   const U* x = (const U*)a.x + (int64_t)t * a.units;
@@ -106,7 +255,7 @@ __global__ __launch_bounds__(256) void dispatch_kernel(DispatchArgs a) {
     const U v = x[c];
     for (int j = 0; j < k; ++j) {
       const int r = __builtin_amdgcn_readfirstlane(dst[j]);
-      if (r >= 0) ((U*)a.rows)[(int64_t)r * a.units + c] = v;
+      if (r >= 0) store_once((U*)a.rows + (int64_t)r * a.units + c, v);
     }
   }
 }
@@ -177,7 +326,7 @@ struct CombineArgs {
 // grid (T, chunks), a unit of 16 bytes (or one value) a thread. The wave that finds the order counts, for each of the
 // token's rows, the rows before it.
 template <int kType, int V>
-__global__ __launch_bounds__(128) void combine_kernel(CombineArgs a) {
+__global__ __launch_bounds__(512) void combine_kernel(CombineArgs a) {
   using X = Unit<kType, V>;
   using Raw = typename X::Raw;
   __shared__ int row[kMaxTopK];
@@ -206,7 +355,7 @@ __global__ __launch_bounds__(128) void combine_kernel(CombineArgs a) {
   __syncthreads();
   const int n = __builtin_amdgcn_readfirstlane(count);
   const bool weighted = a.weights != nullptr;
-  for (int64_t c = (int64_t)blockIdx.y * 128 + tid; c < a.units; c += (int64_t)gridDim.y * 128) {
+  for (int64_t c = (int64_t)blockIdx.y * blockDim.x + tid; c < a.units; c += (int64_t)gridDim.y * blockDim.x) {
     float acc[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) acc[i] = 0.f;
@@ -215,7 +364,7 @@ __global__ __launch_bounds__(128) void combine_kernel(CombineArgs a) {
 #pragma unroll
       for (int j = 0; j < 8; ++j)
         if (j0 + j < n)
-          raw[j] = ((const Raw*)a.rows)[(int64_t)__builtin_amdgcn_readfirstlane(row[j0 + j]) * a.units + c];
+          raw[j] = load_once((const Raw*)a.rows + (int64_t)__builtin_amdgcn_readfirstlane(row[j0 + j]) * a.units + c);
 #pragma unroll
       for (int j = 0; j < 8; ++j)
         if (j0 + j < n) {
@@ -228,7 +377,7 @@ __global__ __launch_bounds__(128) void combine_kernel(CombineArgs a) {
     }
     if (a.shared) {
       float v[V];
-      X::values(((const Raw*)a.shared)[(int64_t)t * a.units + c], v);
+      X::values(load_once((const Raw*)a.shared + (int64_t)t * a.units + c), v);
 #pragma unroll
       for (int i = 0; i < V; ++i) acc[i] = acc[i] + v[i];
     }
@@ -275,14 +424,14 @@ __global__ __launch_bounds__(256) void combine_backward_kernel(CombineBwdArgs a)
     float g[V], v[V];
     X::values(dy[c], g);
     if (a.dweights) {
-      X::values(row[c], v);
+      X::values(load_once(row + c), v);
 #pragma unroll
       for (int e = 0; e < V; ++e) dot = dot + g[e] * v[e];
     }
     if (a.drows) {
 #pragma unroll
       for (int e = 0; e < V; ++e) g[e] = a.weights ? w * g[e] : g[e];
-      out[c] = X::round(g);
+      store_once(out + c, X::round(g));
     }
   }
   if (!a.dweights) return;
@@ -318,16 +467,27 @@ int check_rows(const char* who, int32_t dtype, int64_t width, bool bytes_too) {
 
 int64_t element_bytes(int32_t dtype) { return dtype == MX_ROWS_F32 ? 4 : dtype == MX_ROWS_BF16 ? 2 : 1; }
 
-// workgroups along a row of `units`, `per` of them a workgroup
-unsigned chunks_of(int64_t units, int per) {
-  const int64_t n = (units + per - 1) / per;
-  return (unsigned)(n < 64 ? n : 64);
+// Threads and workgroups for rows of `units`: a workgroup takes whole rows in as few equal steps of up to 512 threads
+// as it can; where the tokens alone would leave the chip idle, the row is cut into pieces of 128 units.
+struct Shape {
+  unsigned threads, chunks;
+};
+Shape shape_of(int tokens, int64_t units) {
+  if (tokens < kFewTokens) return Shape{128, (unsigned)std::min<int64_t>((units + 127) / 128, 256)};
+  const int64_t steps = (units + 511) / 512;
+  return Shape{(unsigned)(((units + steps - 1) / steps + 63) / 64 * 64), 1};
 }
 
 template <typename U>
-int launch_dispatch(DispatchArgs a, int64_t row_bytes, hipStream_t st) {
+int launch_dispatch(DispatchArgs a, int64_t row_bytes, bool fused, hipStream_t st) {
   a.units = row_bytes / (int64_t)sizeof(U);
-  hipLaunchKernelGGL((dispatch_kernel<U>), dim3(a.tokens, chunks_of(a.units, 256)), dim3(256), 0, st, a);
+  if (fused) {
+    const unsigned chunks = (unsigned)std::min<int64_t>((a.units + 255) / 256, 64);
+    hipLaunchKernelGGL((dispatch_kernel<U>), dim3(a.tokens + 1, chunks), dim3(256), 0, st, a);
+  } else {
+    const int chunks = (int)std::min<int64_t>((a.units + 63) / 64, (1 << 25) / a.tokens);
+    hipLaunchKernelGGL((move_rows_kernel<U>), dim3(a.tokens * chunks), dim3(64), 0, st, a, chunks);
+  }
   MX_LAUNCH_CHECK("dispatch_kernel");
   return MX_OK;
 }
@@ -335,7 +495,8 @@ int launch_dispatch(DispatchArgs a, int64_t row_bytes, hipStream_t st) {
 template <int kType, int V>
 int launch_combine(CombineArgs a, int64_t width, hipStream_t st) {
   a.units = width / V;
-  hipLaunchKernelGGL((combine_kernel<kType, V>), dim3(a.tokens, chunks_of(a.units, 128)), dim3(128), 0, st, a);
+  const Shape s = shape_of(a.tokens, a.units);
+  hipLaunchKernelGGL((combine_kernel<kType, V>), dim3(a.tokens, s.chunks), dim3(s.threads), 0, st, a);
   MX_LAUNCH_CHECK("combine_kernel");
   return MX_OK;
 }
@@ -364,7 +525,8 @@ using mxi::use;
 
 int mxi::row_plan(const int32_t* ids, int32_t pairs, int32_t groups, const mx_row_plan& plan, hipStream_t st) {
   const PlanArgs a{ids, pairs, groups, plan.first, plan.pair_row, plan.row_pair};
-  hipLaunchKernelGGL(plan_kernel, dim3(groups + 1), dim3(kPlanThreads), 0, st, a);
+  if (pairs <= 8 * kPlanThreads) hipLaunchKernelGGL(plan_kernel<8>, dim3(groups + 1), dim3(kPlanThreads), 0, st, a);
+  else hipLaunchKernelGGL(plan_kernel<32>, dim3(groups + 1), dim3(kPlanThreads), 0, st, a);
   MX_LAUNCH_CHECK("plan_kernel");
   return MX_OK;
 }
@@ -391,16 +553,19 @@ int mx_dispatch(mx_ctx* ctx, const int32_t* ids, int32_t tokens, int32_t top_k, 
   }
   if (int s = use(ctx)) return s;
   hipStream_t st = as_stream(stream);
-  if (ids)
-    if (int s = mxi::row_plan(ids, tokens * top_k, groups, *plan, st)) return s;
-  if (!x || !tokens) return MX_OK;
-  DispatchArgs a{plan->pair_row, tokens, top_k, (const uint8_t*)x, (uint8_t*)rows, 0, weights, row_weights};
+  const int32_t pairs = tokens * top_k;
+  const bool fused = ids && x && pairs <= kFusedPairs;
+  if (ids && !fused)
+    if (int s = mxi::row_plan(ids, pairs, groups, *plan, st)) return s;
+  if (!x || (!tokens && !fused)) return MX_OK;
+  DispatchArgs a{{ids, pairs, groups, plan->first, plan->pair_row, plan->row_pair}, tokens, top_k, (const uint8_t*)x,
+                 (uint8_t*)rows, 0, weights, row_weights};
   const int64_t bytes = width * element_bytes(dtype);
   const uint64_t low = (uint64_t)(uintptr_t)x | (uint64_t)(uintptr_t)rows | (uint64_t)bytes;
-  if (low % 16 == 0) return launch_dispatch<uint4>(a, bytes, st);
-  if (low % 4 == 0) return launch_dispatch<uint32_t>(a, bytes, st);
-  if (low % 2 == 0) return launch_dispatch<uint16_t>(a, bytes, st);
-  return launch_dispatch<uint8_t>(a, bytes, st);
+  if (low % 16 == 0) return launch_dispatch<uint4>(a, bytes, fused, st);
+  if (low % 4 == 0) return launch_dispatch<uint32_t>(a, bytes, fused, st);
+  if (low % 2 == 0) return launch_dispatch<uint16_t>(a, bytes, fused, st);
+  return launch_dispatch<uint8_t>(a, bytes, fused, st);
 }
 
 int mx_combine(mx_ctx* ctx, const void* rows, int32_t dtype, const int32_t* pair_row, const float* weights,
