@@ -3,8 +3,9 @@
 The plan and the moved rows are exact. A sum of n terms in FP32 is within n 2^-24 of the sum of the terms' magnitudes
 (one rounding per addition, each at most half a step of a partial sum that the magnitudes bound; one more for a weighted
 term's product); a BF16 result adds half a BF16 step, 2^-8 of its value. A weight's gradient is a dot product over the
-row: a thread adds at most width / 256 + 8 products in order, six lane steps and three waves follow, and each product
-was rounded once.
+row: in n = ceil(units / 1024) rounds of four units of up to eight values, a thread adds at most 32 n <= width / 256 + 32
+products in order (units of one value: 4 n), six lane steps and up to three more waves follow, and each product was
+rounded once.
 """
 
 import ctypes as C
@@ -112,7 +113,7 @@ def test_combine_backward(gpu_ctx, tokens, k, experts, width, dtype, weighted):
     drows, dweights, size = oracle.combine_backward(values(dy), values(rows), pair_row, weights)
     check(got["drows"], drows, np.abs(drows), 1, dtype)
     assert not got["drows"][first[-1]:].any()
-    depth = -(-width // 256) + 8 + 6 + 3
+    depth = -(-width // 256) + 32 + 6 + 3
     check(got["dweights"], dweights, size, depth + 1, "f32")
 
 

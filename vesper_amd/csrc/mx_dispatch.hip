@@ -20,8 +20,10 @@ namespace {
 constexpr int kMaxTokens = 1 << 18;   // keeps every grid below 2^32 threads
 constexpr int kMaxTopK = 32, kMaxGroups = 1024;
 constexpr int64_t kMaxWidth = 1 << 24;
-constexpr int kFusedPairs = 2048;   // up to this many pairs the plan is made within the dispatch launch
-constexpr int kFewTokens = 512;     // below, a token's row is cut over several workgroups
+constexpr int kFusedPairs = 1024;   // up to this many pairs the plan is made within the dispatch launch
+// Calls that move more than this go past the caches with what they touch once. The sum of a token counts only with all
+// its pairs here: an expert-parallel rank moves a fraction of what the host can tell.
+constexpr int64_t kStreamBytes = 96 << 20;
 
 // ---- plan ----
 
@@ -121,25 +123,27 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanArgs a) {
   else place_key<false, kBatch>(a, g, sums);
 }
 
-// Streaming access to rows that a call touches once.
-template <typename R>
+// Access to rows that the call touches once: past the caches where the call moves more than they hold (kStream).
+template <bool kStream, typename R>
 __device__ __forceinline__ R load_once(const R* p) {
-  if constexpr (sizeof(R) == 16) {
+  if constexpr (!kStream) {
+    return *p;
+  } else if constexpr (sizeof(R) == 16) {
     return __builtin_bit_cast(R, __builtin_nontemporal_load((const mxd::u32x4_t*)p));
   } else {
     return __builtin_nontemporal_load(p);
   }
 }
-template <typename R>
+template <bool kStream, typename R>
 __device__ __forceinline__ void store_once(R* p, const R& v) {
-  if constexpr (sizeof(R) == 16) {
+  if constexpr (!kStream) {
+    *p = v;
+  } else if constexpr (sizeof(R) == 16) {
     __builtin_nontemporal_store(__builtin_bit_cast(mxd::u32x4_t, v), (mxd::u32x4_t*)p);
   } else {
     __builtin_nontemporal_store(v, p);
   }
 }
-
-// ---- dispatch ----
 
 struct DispatchArgs {
   PlanArgs plan;
@@ -209,7 +213,7 @@ __device__ __forceinline__ void count_groups(const PlanArgs& a, int* count) {
 // pointers allow.
 //
 // By a plan: one wave per token and piece of 64 units (chunks pieces a row; more units, more rounds).
-template <typename U>
+template <typename U, bool kStream>
 __global__ __launch_bounds__(64) void move_rows_kernel(DispatchArgs a, int chunks) {
   const int t = blockIdx.x / chunks, chunk = blockIdx.x % chunks, lane = threadIdx.x, k = a.k, pairs = a.tokens * k;
   if (a.row_weights && chunk == 0 && lane < k) {
@@ -221,7 +225,7 @@ __global__ __launch_bounds__(64) void move_rows_kernel(DispatchArgs a, int chunk
     const U v = x[c];
     for (int j = 0; j < k; ++j) {
       const int r = a.plan.pair_row[t * k + j];
-      if (r >= 0 && r < pairs) store_once((U*)a.rows + (int64_t)r * a.units + c, v);
+      if (r >= 0 && r < pairs) store_once<kStream>((U*)a.rows + (int64_t)r * a.units + c, v);
     }
   }
 }
@@ -255,7 +259,7 @@ __global__ __launch_bounds__(256) void dispatch_kernel(DispatchArgs a) {
     const U v = x[c];
     for (int j = 0; j < k; ++j) {
       const int r = __builtin_amdgcn_readfirstlane(dst[j]);
-      if (r >= 0) store_once((U*)a.rows + (int64_t)r * a.units + c, v);
+      if (r >= 0) ((U*)a.rows)[(int64_t)r * a.units + c] = v;
     }
   }
 }
@@ -321,63 +325,48 @@ struct CombineArgs {
   int64_t units;               // units per row
   const float* row_weights;    // dispatch_backward: the gradient of each row's weight, and
   float* dweights;             // where it goes
+  bool stream;
 };
 
-// grid (T, chunks), a unit of 16 bytes (or one value) a thread. The wave that finds the order counts, for each of the
-// token's rows, the rows before it.
-template <int kType, int V>
-__global__ __launch_bounds__(512) void combine_kernel(CombineArgs a) {
+// acc += (w *) rows, N of them in flight together; row and weight j are those of lane j0 + j.
+template <int N, bool kStream, typename X, int V>
+__device__ __forceinline__ void add_rows(const typename X::Raw* rows, int64_t units, int64_t c, int row, float weight,
+                                         int j0, bool weighted, float* acc) {
+  typename X::Raw raw[N];
+#pragma unroll
+  for (int j = 0; j < N; ++j)
+    raw[j] = load_once<kStream>(rows + (int64_t)__builtin_amdgcn_readlane(row, j0 + j) * units + c);
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    float v[V];
+    X::values(raw[j], v);
+    const float w = mx::u2f(__builtin_amdgcn_readlane(mx::f2u(weight), j0 + j));
+#pragma unroll
+    for (int i = 0; i < V; ++i) acc[i] = acc[i] + (weighted ? w * v[i] : v[i]);
+  }
+}
+
+template <int kType, int V, bool kStream>
+__device__ __forceinline__ void combine_units(const CombineArgs& a, int t, int64_t c0, int64_t step, int row,
+                                              float weight, int n) {
   using X = Unit<kType, V>;
   using Raw = typename X::Raw;
-  __shared__ int row[kMaxTopK];
-  __shared__ float weight[kMaxTopK];
-  __shared__ int count;
-  const int t = blockIdx.x, tid = threadIdx.x, k = a.k, pairs = a.tokens * k;
-  if (tid < 64) {
-    int r = -1;
-    if (tid < k) {
-      r = a.pair_row[t * k + tid];
-      r = r >= 0 && r < pairs ? r : -1;
-    }
-    int before = 0;
-    for (int j = 0; j < k; ++j) {
-      const int o = __shfl(r, j, 64);
-      before += o >= 0 && (o < r || (o == r && j < tid));
-    }
-    if (r >= 0) {
-      row[before] = r;
-      weight[before] = a.weights ? a.weights[t * k + tid] : 1.f;
-    }
-    const uint64_t live = __ballot(r >= 0);
-    if (tid == 0) count = __popcll(live);
-    if (a.dweights && blockIdx.y == 0 && tid < k) a.dweights[t * k + tid] = r >= 0 ? a.row_weights[r] : 0.f;
-  }
-  __syncthreads();
-  const int n = __builtin_amdgcn_readfirstlane(count);
+  const Raw* rows = (const Raw*)a.rows;
   const bool weighted = a.weights != nullptr;
-  for (int64_t c = (int64_t)blockIdx.y * blockDim.x + tid; c < a.units; c += (int64_t)gridDim.y * blockDim.x) {
+  for (int64_t c = c0; c < a.units; c += step) {
     float acc[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) acc[i] = 0.f;
-    for (int j0 = 0; j0 < n; j0 += 8) {
-      Raw raw[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (j0 + j < n)
-          raw[j] = load_once((const Raw*)a.rows + (int64_t)__builtin_amdgcn_readfirstlane(row[j0 + j]) * a.units + c);
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (j0 + j < n) {
-          float v[V];
-          X::values(raw[j], v);
-          const float w = weight[j0 + j];
-#pragma unroll
-          for (int i = 0; i < V; ++i) acc[i] = acc[i] + (weighted ? w * v[i] : v[i]);
-        }
-    }
+    Raw shared{};
+    if (a.shared) shared = load_once<kStream>((const Raw*)a.shared + (int64_t)t * a.units + c);
+    int j = 0;
+    for (; j + 8 <= n; j += 8) add_rows<8, kStream, X, V>(rows, a.units, c, row, weight, j, weighted, acc);
+    if (n & 4) add_rows<4, kStream, X, V>(rows, a.units, c, row, weight, j, weighted, acc), j += 4;
+    if (n & 2) add_rows<2, kStream, X, V>(rows, a.units, c, row, weight, j, weighted, acc), j += 2;
+    if (n & 1) add_rows<1, kStream, X, V>(rows, a.units, c, row, weight, j, weighted, acc);
     if (a.shared) {
       float v[V];
-      X::values(load_once((const Raw*)a.shared + (int64_t)t * a.units + c), v);
+      X::values(shared, v);
 #pragma unroll
       for (int i = 0; i < V; ++i) acc[i] = acc[i] + v[i];
     }
@@ -385,7 +374,37 @@ __global__ __launch_bounds__(512) void combine_kernel(CombineArgs a) {
   }
 }
 
+// One wave per token and piece of 64 units (chunks pieces a row; more units, more rounds), a unit of 16 bytes (or one
+// value) a lane, up to eight rows in flight. Lane j holds the token's pair j; each counts the rows before its own and
+// sends it to the lane of that number.
+template <int kType, int V>
+__global__ __launch_bounds__(64) void combine_kernel(CombineArgs a, int chunks) {
+  const int t = blockIdx.x / chunks, chunk = blockIdx.x % chunks, lane = threadIdx.x, k = a.k, pairs = a.tokens * k;
+  int r = -1;
+  float w = 1.f;
+  if (lane < k) {
+    r = a.pair_row[t * k + lane];
+    r = r >= 0 && r < pairs ? r : -1;
+    if (a.weights) w = a.weights[t * k + lane];
+  }
+  if (a.dweights && chunk == 0 && lane < k) a.dweights[t * k + lane] = r >= 0 ? a.row_weights[r] : 0.f;
+  int before = 0;
+  for (int j = 0; j < k; ++j) {
+    const int o = __builtin_amdgcn_readlane(r, j);
+    before += o >= 0 && (o < r || (o == r && j < lane));
+  }
+  const int n = __popcll(__ballot(r >= 0));
+  const int to = 4 * (r >= 0 ? before : 63);   // lane 63 is no one's: k <= 32
+  const int row = __builtin_amdgcn_ds_permute(to, r);
+  const float weight = mx::u2f(__builtin_amdgcn_ds_permute(to, (int)mx::f2u(w)));
+  const int64_t c0 = 64 * (int64_t)chunk + lane, step = 64 * (int64_t)chunks;
+  if (a.stream && n == k) combine_units<kType, V, true>(a, t, c0, step, row, weight, n);
+  else combine_units<kType, V, false>(a, t, c0, step, row, weight, n);
+}
+
 // ---- the backward pass of combine ----
+
+constexpr int kInFlight = 4;   // units of a row, and of dy, that a thread has in flight
 
 struct CombineBwdArgs {
   const void* dy;
@@ -396,50 +415,80 @@ struct CombineBwdArgs {
   float* dweights;
   int32_t tokens, k;
   int64_t units;
+  bool stream;
 };
 
-// One workgroup a pair: drows[row] = w dy[t] and dw = <rows[row], dy[t]>, both from one read of dy and of the row. Each
-// thread adds its products in order, the lanes are added as a tree and the waves in order. A token's pairs run on one
-// XCD (workgroups go round the eight of them), so its dy comes from HBM once and from that L2 after.
-template <int kType, int V>
-__global__ __launch_bounds__(256) void combine_backward_kernel(CombineBwdArgs a) {
+template <int kType, int V, bool kStream>
+__device__ __forceinline__ float backward_units(const CombineBwdArgs& a, int t, int r, float w) {
   using X = Unit<kType, V>;
   using Raw = typename X::Raw;
+  const Raw* dy = (const Raw*)a.dy + (int64_t)t * a.units;
+  const Raw* row = (const Raw*)a.rows + (int64_t)r * a.units;
+  Raw* out = (Raw*)a.drows + (int64_t)r * a.units;
+  const int threads = blockDim.x;
+  float dot = 0.f;
+  for (int64_t c0 = threadIdx.x; c0 < a.units; c0 += kInFlight * threads) {
+    Raw dy_raw[kInFlight], row_raw[kInFlight];
+#pragma unroll
+    for (int s = 0; s < kInFlight; ++s) {
+      const int64_t c = c0 + s * threads;
+      if (c < a.units) {
+        if (a.dweights) row_raw[s] = load_once<kStream>(row + c);
+        dy_raw[s] = dy[c];
+      }
+    }
+#pragma unroll
+    for (int s = 0; s < kInFlight; ++s) {
+      const int64_t c = c0 + s * threads;
+      if (c >= a.units) continue;
+      float g[V], v[V];
+      X::values(dy_raw[s], g);
+      if (a.dweights) {
+        X::values(row_raw[s], v);
+#pragma unroll
+        for (int e = 0; e < V; ++e) dot = dot + g[e] * v[e];
+      }
+      if (a.drows) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) g[e] = a.weights ? w * g[e] : g[e];
+        store_once<kStream>(out + c, X::round(g));
+      }
+    }
+  }
+  return dot;
+}
+
+// One workgroup a pair: drows[row] = w dy[t] and dw = <rows[row], dy[t]>, both from one read of dy and of the row.
+// Each thread adds its products in order, the lanes are added as a tree and the waves in order.
+// A token's pairs run on one XCD (workgroups go round the eight of them), so its dy comes from HBM once and from that L2
+// after.
+template <int kType, int V>
+__global__ __launch_bounds__(256) void combine_backward_kernel(CombineBwdArgs a) {
   __shared__ float part[4];
-  const int tid = threadIdx.x, k = a.k, pairs = a.tokens * k;
+  const int tid = threadIdx.x, lane = tid & 63, k = a.k, pairs = a.tokens * k;
   const int i = blockIdx.x >> 3;
   const int t = i / k * 8 + (blockIdx.x & 7), j = i % k;
   if (t >= a.tokens) return;
-  const int r = a.pair_row[t * k + j];
+  int own = -1;
+  if (lane < k) own = a.pair_row[t * k + lane];
+  const int n = __popcll(__ballot(own >= 0));
+  const int r = __builtin_amdgcn_readlane(own, j);
   if (r < 0 || r >= pairs) {
     if (a.dweights && tid == 0) a.dweights[t * k + j] = 0.f;
     return;
   }
   const float w = a.weights ? a.weights[t * k + j] : 1.f;
-  const Raw* dy = (const Raw*)a.dy + (int64_t)t * a.units;
-  const Raw* row = (const Raw*)a.rows + (int64_t)r * a.units;
-  Raw* out = (Raw*)a.drows + (int64_t)r * a.units;
-  float dot = 0.f;
-  for (int64_t c = tid; c < a.units; c += 256) {
-    float g[V], v[V];
-    X::values(dy[c], g);
-    if (a.dweights) {
-      X::values(load_once(row + c), v);
-#pragma unroll
-      for (int e = 0; e < V; ++e) dot = dot + g[e] * v[e];
-    }
-    if (a.drows) {
-#pragma unroll
-      for (int e = 0; e < V; ++e) g[e] = a.weights ? w * g[e] : g[e];
-      store_once(out + c, X::round(g));
-    }
-  }
+  float dot = a.stream && n == k ? backward_units<kType, V, true>(a, t, r, w) : backward_units<kType, V, false>(a, t, r, w);
   if (!a.dweights) return;
 #pragma unroll
   for (int m = 32; m >= 1; m >>= 1) dot = dot + __shfl_xor(dot, m, 64);
-  if ((tid & 63) == 0) part[tid >> 6] = dot;
+  if (lane == 0) part[tid >> 6] = dot;
   __syncthreads();
-  if (tid == 0) a.dweights[t * k + j] = ((part[0] + part[1]) + part[2]) + part[3];
+  if (tid == 0) {
+    float sum = part[0];
+    for (int v = 1; v < (int)blockDim.x / 64; ++v) sum = sum + part[v];
+    a.dweights[t * k + j] = sum;
+  }
 }
 
 bool is_aligned(const void* p, uintptr_t a) { return ((uintptr_t)p & (a - 1)) == 0; }
@@ -467,15 +516,12 @@ int check_rows(const char* who, int32_t dtype, int64_t width, bool bytes_too) {
 
 int64_t element_bytes(int32_t dtype) { return dtype == MX_ROWS_F32 ? 4 : dtype == MX_ROWS_BF16 ? 2 : 1; }
 
-// Threads and workgroups for rows of `units`: a workgroup takes whole rows in as few equal steps of up to 512 threads
-// as it can; where the tokens alone would leave the chip idle, the row is cut into pieces of 128 units.
-struct Shape {
-  unsigned threads, chunks;
-};
-Shape shape_of(int tokens, int64_t units) {
-  if (tokens < kFewTokens) return Shape{128, (unsigned)std::min<int64_t>((units + 127) / 128, 256)};
-  const int64_t steps = (units + 511) / 512;
-  return Shape{(unsigned)(((units + steps - 1) / steps + 63) / 64 * 64), 1};
+// Pieces of 64 units of a row, as many as keep the grid below 2^25 waves.
+int chunks_of(int tokens, int64_t units) { return (int)std::min<int64_t>((units + 63) / 64, (1 << 25) / tokens); }
+
+// Whether a call of `row_bytes` rows, `moves` of them a pair and one a token, goes past the caches.
+bool streams(int tokens, int k, int64_t row_bytes, int moves) {
+  return (int64_t)tokens * (moves * k + 1) * row_bytes > kStreamBytes;
 }
 
 template <typename U>
@@ -485,8 +531,10 @@ int launch_dispatch(DispatchArgs a, int64_t row_bytes, bool fused, hipStream_t s
     const unsigned chunks = (unsigned)std::min<int64_t>((a.units + 255) / 256, 64);
     hipLaunchKernelGGL((dispatch_kernel<U>), dim3(a.tokens + 1, chunks), dim3(256), 0, st, a);
   } else {
-    const int chunks = (int)std::min<int64_t>((a.units + 63) / 64, (1 << 25) / a.tokens);
-    hipLaunchKernelGGL((move_rows_kernel<U>), dim3(a.tokens * chunks), dim3(64), 0, st, a, chunks);
+    const int chunks = chunks_of(a.tokens, a.units);
+    const bool stream = streams(a.tokens, a.k, row_bytes, 1);
+    hipLaunchKernelGGL((stream ? move_rows_kernel<U, true> : move_rows_kernel<U, false>), dim3(a.tokens * chunks),
+                       dim3(64), 0, st, a, chunks);
   }
   MX_LAUNCH_CHECK("dispatch_kernel");
   return MX_OK;
@@ -495,8 +543,9 @@ int launch_dispatch(DispatchArgs a, int64_t row_bytes, bool fused, hipStream_t s
 template <int kType, int V>
 int launch_combine(CombineArgs a, int64_t width, hipStream_t st) {
   a.units = width / V;
-  const Shape s = shape_of(a.tokens, a.units);
-  hipLaunchKernelGGL((combine_kernel<kType, V>), dim3(a.tokens, s.chunks), dim3(s.threads), 0, st, a);
+  const int chunks = chunks_of(a.tokens, a.units);
+  a.stream = streams(a.tokens, a.k, a.units * (int64_t)sizeof(typename Unit<kType, V>::Raw), 1);
+  hipLaunchKernelGGL((combine_kernel<kType, V>), dim3(a.tokens * chunks), dim3(64), 0, st, a, chunks);
   MX_LAUNCH_CHECK("combine_kernel");
   return MX_OK;
 }
@@ -513,7 +562,11 @@ template <int kType, int V>
 int launch_combine_backward(CombineBwdArgs a, int64_t width, hipStream_t st) {
   a.units = width / V;
   const unsigned grid = (unsigned)((a.tokens + 7) / 8 * 8 * a.k);
-  hipLaunchKernelGGL((combine_backward_kernel<kType, V>), dim3(grid), dim3(256), 0, st, a);
+  // as few equal rounds as kInFlight units a thread of 256 allow
+  const int64_t rounds = (a.units + 256 * kInFlight - 1) / (256 * kInFlight), per = rounds * kInFlight;
+  const unsigned threads = (unsigned)(((a.units + per - 1) / per + 63) / 64 * 64);
+  a.stream = streams(a.tokens, a.k, a.units * (int64_t)sizeof(typename Unit<kType, V>::Raw), 2);
+  hipLaunchKernelGGL((combine_backward_kernel<kType, V>), dim3(grid), dim3(threads), 0, st, a);
   MX_LAUNCH_CHECK("combine_backward_kernel");
   return MX_OK;
 }
@@ -580,7 +633,7 @@ int mx_combine(mx_ctx* ctx, const void* rows, int32_t dtype, const int32_t* pair
              "%s: pointers must be aligned to their elements", who);
   if (int s = use(ctx)) return s;
   if (!tokens) return MX_OK;
-  const CombineArgs a{rows, pair_row, weights, shared, y, tokens, top_k, 0, nullptr, nullptr};
+  const CombineArgs a{rows, pair_row, weights, shared, y, tokens, top_k, 0, nullptr, nullptr, false};
   return combine_any(a, dtype, width, as_stream(stream));
 }
 
@@ -599,7 +652,7 @@ int mx_combine_backward(mx_ctx* ctx, const void* dy, const void* rows, int32_t d
              "%s: pointers must be aligned to their elements", who);
   if (int s = use(ctx)) return s;
   if (!tokens) return MX_OK;
-  const CombineBwdArgs a{dy, rows, pair_row, weights, drows, dweights, tokens, top_k, 0};
+  const CombineBwdArgs a{dy, rows, pair_row, weights, drows, dweights, tokens, top_k, 0, false};
   const bool wide = (width * size) % 16 == 0 && is_aligned(dy, 16) && (!dweights || is_aligned(rows, 16)) &&
                     is_aligned(drows, 16);
   hipStream_t st = as_stream(stream);
@@ -625,7 +678,7 @@ int mx_dispatch_backward(mx_ctx* ctx, const void* drows, int32_t dtype, const in
              "%s: pointers must be aligned to their elements", who);
   if (int s = use(ctx)) return s;
   if (!tokens) return MX_OK;
-  const CombineArgs a{drows, pair_row, nullptr, nullptr, dx, tokens, top_k, 0, drow_weights, dweights};
+  const CombineArgs a{drows, pair_row, nullptr, nullptr, dx, tokens, top_k, 0, drow_weights, dweights, false};
   return combine_any(a, dtype, width, as_stream(stream));
 }
 
