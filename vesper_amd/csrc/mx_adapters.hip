@@ -12,9 +12,9 @@
 //
 // The bank stores each slot in operand order, padded with zeros to whole tiles:
 //   down: [rank tile][K chunk of 32][lane] 16 bytes: rank 16 rt + l % 16, K 32 c + 8 (l / 16) + 0..7
-//   up: [block of 64 outputs][rank tile][half][lane] 16 bytes: two tiles j = 2 half, 2 half + 1 of four ranks each;
-//   row m of tile j is output 64 b + 16 (m / 4) + 4 j + m % 4, so a lane's D registers of the four tiles are 16
-//   consecutive outputs of its token.
+//   up: [block of 64 outputs][rank tile][half][lane] 16 bytes: two tiles j = 0, 1 of four ranks each; row m of tile j of
+//   a half is output 64 b + 32 half + 8 (m / 4) + 4 j + m % 4, so a lane's D registers of a half's two tiles are 8
+//   consecutive outputs of its token and the four lanes of a token 32 (64 bytes of y).
 #include <algorithm>
 #include <new>
 
@@ -32,11 +32,11 @@ typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 constexpr int kMaxTokens = 1 << 18, kMaxSlots = 1024, kMaxRank = 256;
 constexpr int kMaxWidth = 1 << 20;
 constexpr int kTokenForm = 32;     // calls of up to this many tokens run a token at a time
-constexpr int kColumns = 2;        // 16-token column tiles of a workgroup in the grouped form
-constexpr int kTileTokens = 16 * kColumns;
+constexpr int kTileTokens = 64;    // tokens of a workgroup in the grouped form
+constexpr int kColumns = kTileTokens / 16;
 constexpr int kMaxParts = 32;      // parts of K
+constexpr int64_t kStreamBytes = 96 << 20;   // an x of more than this is read past the caches
 constexpr int kWantGroups = 512;   // workgroups that the split of K aims at
-constexpr int kRankGroup = 4;      // rank tiles in registers at once
 
 struct AdapterSlot {
   int32_t rank;   // 0: empty
@@ -48,7 +48,7 @@ struct Bank {
   const uint8_t* up;
   const AdapterSlot* table;
   int32_t n, k, slots;
-  int32_t rank_tiles, chunks, blocks;   // of the largest rank; K chunks of 32; blocks of 64 outputs
+  int32_t rank_tiles, chunks, blocks;   // of the largest rank; K chunks of 32 (an even count); blocks of 64 outputs
   __host__ __device__ int64_t down_bytes() const { return (int64_t)rank_tiles * chunks * 1024; }
   __host__ __device__ int64_t up_bytes() const { return (int64_t)blocks * rank_tiles * 2048; }
 };
@@ -57,7 +57,7 @@ __device__ __forceinline__ v8bf as_bf(uint4 v) { return __builtin_bit_cast(v8bf,
 
 // ---- loading a slot ----
 
-__global__ __launch_bounds__(64) void adapter_down_kernel(Bank b, uint8_t* bank, int slot, const uint16_t* src, int rank) {
+__global__ __launch_bounds__(64) void adapter_store_down_kernel(Bank b, uint8_t* bank, int slot, const uint16_t* src, int rank) {
   const int lane = threadIdx.x, c = blockIdx.x, rt = blockIdx.y;
   const int r = 16 * rt + (lane & 15), k0 = 32 * c + 8 * (lane >> 4);
   uint32_t w[4] = {0, 0, 0, 0};
@@ -69,7 +69,7 @@ __global__ __launch_bounds__(64) void adapter_down_kernel(Bank b, uint8_t* bank,
   *(uint4*)dst = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-__global__ __launch_bounds__(128) void adapter_up_kernel(Bank b, uint8_t* bank, AdapterSlot* table, int slot,
+__global__ __launch_bounds__(128) void adapter_store_up_kernel(Bank b, uint8_t* bank, AdapterSlot* table, int slot,
                                                          const uint16_t* src, int rank, float scale) {
   const int lane = threadIdx.x & 63, half = threadIdx.x >> 6, block = blockIdx.x, rt = blockIdx.y;
   if (block == 0 && rt == 0 && threadIdx.x == 0) table[slot] = AdapterSlot{rank, scale};
@@ -77,7 +77,7 @@ __global__ __launch_bounds__(128) void adapter_up_kernel(Bank b, uint8_t* bank, 
   const int m = lane & 15, r0 = 16 * rt + 4 * (lane >> 4);
   uint32_t w[4] = {0, 0, 0, 0};
   for (int i = 0; i < 8; ++i) {
-    const int n = 64 * block + 16 * (m >> 2) + 4 * (2 * half + (i >> 2)) + (m & 3), r = r0 + (i & 3);
+    const int n = 64 * block + 32 * half + 8 * (m >> 2) + 4 * (i >> 2) + (m & 3), r = r0 + (i & 3);
     const uint32_t v = n < b.n && r < rank ? src[(int64_t)n * rank + r] : 0;
     w[i >> 1] |= v << (16 * (i & 1));
   }
@@ -100,7 +100,7 @@ struct Call {
   int64_t base_stride;
   uint16_t* y;
   int64_t y_stride;
-  int32_t blocks_per_group;  // output blocks of a workgroup
+  int32_t tiles;             // grouped form: the most tiles that there can be
 };
 
 struct Tile {
@@ -113,11 +113,12 @@ struct Tile {
 __device__ __forceinline__ Tile find_tile(const Call& c, int index) {
   const int lane = threadIdx.x & 63, slots = c.bank.slots;
   int before = 0;
+  Tile t{-1, 0, 0};
   for (int g0 = 0; g0 <= slots; g0 += 64) {
     const int g = g0 + lane;
-    int lo = g <= slots ? c.first[g] : c.tokens, hi = g < slots ? c.first[g + 1] : c.tokens;
-    lo = min(max(lo, 0), c.tokens);
-    hi = min(max(hi, lo), c.tokens);
+    int lo = c.first[min(g, slots)], hi = c.first[min(g + 1, slots)];
+    lo = g <= slots ? min(max(lo, 0), c.tokens) : c.tokens;
+    hi = g < slots ? min(max(hi, lo), c.tokens) : c.tokens;
     const int count = (hi - lo + kTileTokens - 1) / kTileTokens;
     int upto = count;
 #pragma unroll
@@ -130,222 +131,449 @@ __device__ __forceinline__ Tile find_tile(const Call& c, int index) {
       const int at = __ffsll((unsigned long long)__ballot(upto > index - before)) - 1;
       const int skip = index - before - (__shfl(upto, at, 64) - __shfl(count, at, 64));
       const int l = __shfl(lo, at, 64) + skip * kTileTokens, h = __shfl(hi, at, 64);
-      return Tile{g0 + at < slots ? g0 + at : -1, l, min(kTileTokens, h - l)};
+      t = Tile{g0 + at < slots ? g0 + at : -1, l, min(kTileTokens, h - l)};
+      break;
     }
     before += total;
-  }
-  return Tile{-1, 0, 0};
-}
-
-template <bool kGrouped>
-__device__ __forceinline__ Tile tile_of(const Call& c) {
-  Tile t;
-  if constexpr (kGrouped) {
-    t = find_tile(c, blockIdx.x);
-  } else {
-    const int id = c.ids[blockIdx.x];
-    t = Tile{id >= 0 && id < c.bank.slots ? id : -1, (int)blockIdx.x, 1};
   }
   return Tile{__builtin_amdgcn_readfirstlane(t.slot), __builtin_amdgcn_readfirstlane(t.row),
               __builtin_amdgcn_readfirstlane(t.rows)};
 }
 
-// The token of column `col` of the tile; columns past the last repeat it.
-template <bool kGrouped>
-__device__ __forceinline__ int token_of(const Call& c, const Tile& t, int col) {
-  if constexpr (!kGrouped) return t.row;
-  const int p = c.row_pair[t.row + min(col, t.rows - 1)];
+__device__ __forceinline__ Tile one_token(const Call& c, int token) {
+  const int id = __builtin_amdgcn_readfirstlane(c.ids[token]);
+  return Tile{id >= 0 && id < c.bank.slots ? id : -1, token, 1};
+}
+
+// The tokens of the tile's 64 columns, one a lane; columns past the last repeat it.
+__device__ __forceinline__ int tile_tokens(const Call& c, const Tile& t) {
+  const int p = c.row_pair[t.row + min((int)(threadIdx.x & 63), t.rows - 1)];
   return p >= 0 && p < c.tokens ? p : 0;
+}
+
+// Workgroups go round the eight XCDs; this numbers them so that each XCD takes a contiguous range of `count`.
+__device__ __forceinline__ int on_xcd(int id, int count) { return (id & 7) * ((count + 7) >> 3) + (id >> 3); }
+
+// Four ranks of h, from r0 on, as operand B's K slots: bf16(scale s), then bf16 of what that leaves.
+__device__ __forceinline__ uint4 h_operand(const AdapterSlot& slot, int r0, v4f s) {
+  uint32_t hi[2], lo[2];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    float h[2], rest[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) h[i] = r0 + 2 * k + i < slot.rank ? slot.scale * s[2 * k + i] : 0.f;
+    hi[k] = mxd::bf16_pair(h[0], h[1]);
+    rest[0] = h[0] - mx::u2f(hi[k] << 16);
+    rest[1] = h[1] - mx::u2f(hi[k] & 0xFFFF0000u);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)   // an infinite term has no second one
+      if ((hi[k] >> (16 * i) & 0x7F80u) == 0x7F80u) rest[i] = 0.f;
+    lo[k] = mxd::bf16_pair(rest[0], rest[1]);
+  }
+  return make_uint4(hi[0], hi[1], lo[0], lo[1]);
 }
 
 // ---- down: partial sums of h ----
 
-// grid (tiles, parts), 4 waves: a part of the K chunks for the tile's tokens and all ranks, the waves taking the chunks
-// in turn and added in wave order.
-template <bool kGrouped>
-__global__ __launch_bounds__(256) void adapter_down_gemm_kernel(Call c) {
-  constexpr int CT = kGrouped ? kColumns : 1;
-  __shared__ v4f red[4][CT][kRankGroup][64];
-  const Tile t = tile_of<kGrouped>(c);
-  if (t.rows == 0 || t.slot < 0) return;
+// Token form, grid (T, parts), 4 waves: a part of K for one token, given to every column, and RT rank tiles at a time
+// (those past the last repeat it). The waves take the K units (of 64: two chunks) in turn, the next one's loads in
+// flight while one is multiplied, and their sums are added in wave order.
+template <int RT>
+__device__ __forceinline__ void token_down(const Call& c, int token, int slot, int r0, int tiles, int first_tiles,
+                                           v4f (*red)[RT][64]) {
   const Bank& b = c.bank;
-  const int rank = b.table[t.slot].rank, tiles = (rank + 15) >> 4;
   const int tid = threadIdx.x, lane = tid & 63, q = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int c0 = (int)((int64_t)b.chunks * blockIdx.y / c.parts), c1 = (int)((int64_t)b.chunks * (blockIdx.y + 1) / c.parts);
-  int token[CT];
-  const uint8_t* x[CT];
+  const int units = b.chunks / 2, whole = b.k / 64;
+  const int u1 = (int)((int64_t)units * (blockIdx.y + 1) / c.parts);
+  int u = (int)((int64_t)units * blockIdx.y / c.parts) + wave;
+  const uint8_t* x = (const uint8_t*)(c.x + token * c.x_stride) + 16 * q;
+  const int64_t tile_bytes = (int64_t)b.chunks * 1024;
+  const uint8_t* w = b.down + slot * b.down_bytes() + r0 * tile_bytes + 16 * lane;
+  struct Unit {
+    uint4 x[2], w[2][RT];
+  } unit[2];
+  v4f acc[RT];
 #pragma unroll
-  for (int i = 0; i < CT; ++i) {
-    token[i] = token_of<kGrouped>(c, t, 16 * i + (lane & 15));
-    x[i] = (const uint8_t*)(c.x + token[i] * c.x_stride) + 16 * q;
-  }
-  const uint8_t* w = b.down + t.slot * b.down_bytes() + 16 * lane;
-  for (int r0 = 0; r0 < tiles; r0 += kRankGroup) {
-    v4f acc[CT][kRankGroup];
+  for (int r = 0; r < RT; ++r) acc[r] = v4f{0.f, 0.f, 0.f, 0.f};
+  auto load_w = [&](Unit& n, int at, int last) {
 #pragma unroll
-    for (int i = 0; i < CT; ++i)
+    for (int s = 0; s < 2; ++s)
 #pragma unroll
-      for (int r = 0; r < kRankGroup; ++r) acc[i][r] = v4f{0.f, 0.f, 0.f, 0.f};
-    for (int ch = c0 + wave; ch < c1; ch += 4) {
-      uint4 xv[CT], wv[kRankGroup];
+      for (int r = 0; r < RT; ++r) n.w[s][r] = ldg128(w + min(r, last) * tile_bytes + 2048 * (int64_t)at + 1024 * s);
+  };
+  auto load = [&](Unit& n, int at, int last) {
+    load_w(n, at, last);
 #pragma unroll
-      for (int i = 0; i < CT; ++i)
-        xv[i] = 32 * ch + 8 * q < b.k ? ldg128(x[i] + 64 * ch) : make_uint4(0, 0, 0, 0);
+    for (int s = 0; s < 2; ++s) n.x[s] = ldg128(x + 128 * at + 64 * s);
+  };
+  auto multiply = [&](const Unit& n) {
 #pragma unroll
-      for (int r = 0; r < kRankGroup; ++r)
-        if (r0 + r < tiles) wv[r] = ldg128(w + ((int64_t)(r0 + r) * b.chunks + ch) * 1024);
+    for (int s = 0; s < 2; ++s)
 #pragma unroll
-      for (int r = 0; r < kRankGroup; ++r)
-        if (r0 + r < tiles)
-#pragma unroll
-          for (int i = 0; i < CT; ++i)
-            acc[i][r] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf(wv[r]), as_bf(xv[i]), acc[i][r], 0, 0, 0);
+      for (int r = 0; r < RT; ++r)
+        acc[r] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf(n.w[s][r]), as_bf(n.x[s]), acc[r], 0, 0, 0);
+  };
+  const int end = min(u1, whole);
+  if (u < end) {
+    load(unit[0], u, first_tiles - 1);
+    const int last = max(tiles - r0 - 1, 0);
+    while (true) {
+      load(unit[1], min(u + 4, end - 1), last);
+      multiply(unit[0]);
+      u += 4;
+      if (u >= end) break;
+      load(unit[0], min(u + 4, end - 1), last);
+      multiply(unit[1]);
+      u += 4;
+      if (u >= end) break;
     }
+  }
+  if (tiles <= r0) return;
+  if (u < u1) {   // the last unit of a K that is no multiple of 64: zeros past the end of x
+    load_w(unit[0], u, tiles - r0 - 1);
 #pragma unroll
-    for (int i = 0; i < CT; ++i)
+    for (int s = 0; s < 2; ++s)
+      unit[0].x[s] = 64 * u + 32 * s + 8 * q < b.k ? ldg128(x + 128 * u + 64 * s) : make_uint4(0, 0, 0, 0);
+    multiply(unit[0]);
+  }
 #pragma unroll
-      for (int r = 0; r < kRankGroup; ++r) red[wave][i][r][lane] = acc[i][r];
-    __syncthreads();
-    for (int e = wave; e < CT * kRankGroup; e += 4) {
-      const int i = e / kRankGroup, r = e % kRankGroup, col = 16 * i + (lane & 15);
-      if (r0 + r < tiles && col < t.rows) {
-        const v4f s = ((red[0][i][r][lane] + red[1][i][r][lane]) + red[2][i][r][lane]) + red[3][i][r][lane];
-        const int tok = token_of<kGrouped>(c, t, col);
-        *(v4f*)(c.low + ((int64_t)blockIdx.y * c.tokens + tok) * (16 * b.rank_tiles) + 16 * (r0 + r) + 4 * q) = s;
+  for (int r = 0; r < RT; ++r) red[wave][r][lane] = acc[r];
+  __syncthreads();
+  for (int r = wave; r < RT; r += 4)
+    if (r0 + r < tiles && (lane & 15) == 0) {
+      const v4f s = ((red[0][r][lane] + red[1][r][lane]) + red[2][r][lane]) + red[3][r][lane];
+      *(v4f*)(c.low + ((int64_t)blockIdx.y * c.tokens + token) * (16 * b.rank_tiles) + 16 * (r0 + r) + 4 * q) = s;
+    }
+  __syncthreads();
+}
+
+// The first unit's weights are asked for by the bank's largest rank, before the slot's own has arrived.
+template <int RT>
+__global__ __launch_bounds__(256) void adapter_token_down_kernel(Call c) {
+  __shared__ v4f red[4][RT][64];
+  const Tile t = one_token(c, blockIdx.x);
+  if (t.slot < 0) return;
+  const int tiles = (c.bank.table[t.slot].rank + 15) >> 4;
+  token_down<RT>(c, t.row, t.slot, 0, tiles, min(RT, c.bank.rank_tiles), red);
+  for (int r0 = RT; r0 < tiles; r0 += RT) token_down<RT>(c, t.row, t.slot, r0, tiles, min(RT, tiles - r0), red);
+}
+
+// Grouped form: a part of K for a tile of 64 tokens and RT rank tiles, 4 waves. x comes through LDS in stages of 256 K,
+// so that rows are read 512 bytes at a time (in operand order a load takes 64 bytes of each of 16 rows: with rows a
+// power of two apart those meet in the same memory channels); each wave multiplies its K unit of 64 of every stage,
+// its weights straight from the L2 of its XCD, which holds one part's. Two stages: one in flight while one is
+// multiplied. The rows of a pair lie 512 bytes apart and the pairs 1040, and a second row's 16-byte pieces are swapped
+// in halves of 128 bytes, so that the 16 rows of an operand read lie in different banks.
+constexpr int kStageK = 256, kPairBytes = 1040, kStageBytes = kTileTokens / 2 * kPairBytes;
+
+template <int RT, bool kStream>
+__global__ __launch_bounds__(256, 2) void adapter_down_kernel(Call c, int rank_groups) {
+  extern __shared__ uint4 stage_lds[];   // two stages; then the waves' sums [4][kColumns][RT][64]
+  const Bank& b = c.bank;
+  const int work = on_xcd(blockIdx.x, c.parts * c.tiles * rank_groups);
+  const int part = work / (c.tiles * rank_groups), r0 = RT * (work % rank_groups);
+  if (part >= c.parts) return;
+  const Tile t = find_tile(c, work / rank_groups % c.tiles);
+  if (t.rows == 0 || t.slot < 0) return;
+  const AdapterSlot slot = b.table[t.slot];
+  const int tiles = (slot.rank + 15) >> 4;
+  if (r0 >= tiles) return;
+  const int tid = threadIdx.x, lane = tid & 63, q = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int stages = (b.k + kStageK - 1) / kStageK, units = b.chunks / 2;
+  const int s0 = (int)((int64_t)stages * part / c.parts), s1 = (int)((int64_t)stages * (part + 1) / c.parts);
+  const uint32_t lds = mxd::lds_addr(stage_lds);
+  const int piece = (lane & 31) ^ (lane >> 5 << 3);   // of its row that this lane copies
+  const int tokens = tile_tokens(c, t);
+  const uint8_t* src[kColumns * 2];
+#pragma unroll
+  for (int j = 0; j < kColumns * 2; ++j)
+    src[j] = (const uint8_t*)(c.x + __shfl(tokens, 2 * (wave + 4 * j) + (lane >> 5), 64) * c.x_stride);
+  auto copy = [&](int stage, int buffer) {
+    const bool in = kStageK * stage + 8 * piece < b.k;
+    const int64_t at = in ? (int64_t)(2 * kStageK) * stage + 16 * piece : 0;
+#pragma unroll
+    for (int j = 0; j < kColumns * 2; ++j)
+      if (2 * (wave + 4 * j) < t.rows) {
+        const uint32_t to = __builtin_amdgcn_readfirstlane(lds + buffer * kStageBytes + (wave + 4 * j) * kPairBytes);
+        if constexpr (kStream) mxd::global_to_lds16_nt(src[j] + at, to);
+        else mxd::global_to_lds16(src[j] + at, to);
       }
+  };
+  const int64_t tile_bytes = (int64_t)b.chunks * 1024;
+  const uint8_t* w = b.down + t.slot * b.down_bytes() + r0 * tile_bytes + 16 * lane;
+  const int last = tiles - r0 - 1;
+  auto load_w = [&](uint4 (*n)[RT], int stage) {
+    const int u = min(4 * stage + wave, units - 1);
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int r = 0; r < RT; ++r) n[s][r] = ldg128(w + min(r, last) * tile_bytes + 2048 * (int64_t)u + 1024 * s);
+  };
+  v4f acc[kColumns][RT];
+#pragma unroll
+  for (int i = 0; i < kColumns; ++i)
+#pragma unroll
+    for (int r = 0; r < RT; ++r) acc[i][r] = v4f{0.f, 0.f, 0.f, 0.f};
+  // this lane's row of column tile 0: pair (l % 16) / 2, half l % 2
+  const uint8_t* rows = (const uint8_t*)stage_lds + ((lane & 15) >> 1) * kPairBytes + (lane & 1) * 512;
+  auto multiply = [&](const uint4 (*n)[RT], int stage, int buffer) {
+    const int u = 4 * stage + wave;
+    if (64 * u >= b.k) return;
+    const bool ragged = 64 * u + 64 > b.k;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const int at = 16 * ((8 * wave + 4 * s + q) ^ ((lane & 1) << 3));
+      uint4 x[kColumns];
+#pragma unroll
+      for (int i = 0; i < kColumns; ++i) x[i] = *(const uint4*)(rows + buffer * kStageBytes + i * 8 * kPairBytes + at);
+      if (ragged && 64 * u + 32 * s + 8 * q >= b.k) {
+#pragma unroll
+        for (int i = 0; i < kColumns; ++i) x[i] = make_uint4(0, 0, 0, 0);
+      }
+#pragma unroll
+      for (int r = 0; r < RT; ++r)
+#pragma unroll
+        for (int i = 0; i < kColumns; ++i)
+          acc[i][r] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf(n[s][r]), as_bf(x[i]), acc[i][r], 0, 0, 0);
     }
-    __syncthreads();
+  };
+  uint4 wv[2][2][RT];
+  // the weights before the copies: the wait for the weights then leaves the copies behind them in flight
+  load_w(wv[0], s0);
+  copy(s0, 0);
+  for (int stage = s0; stage < s1; stage += 2) {
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+      if (stage + n >= s1) break;
+      __builtin_amdgcn_s_waitcnt(mxd::vm_wait_imm(0));
+      mxd::copy_barrier();
+      if (stage + n + 1 < s1) {
+        load_w(wv[n ^ 1], stage + n + 1);
+        copy(stage + n + 1, n ^ 1);
+      }
+      multiply(wv[n], stage + n, n);
+    }
   }
+  mxd::copy_barrier();
+  v4f* red = (v4f*)stage_lds;
+#pragma unroll
+  for (int i = 0; i < kColumns; ++i)
+#pragma unroll
+    for (int r = 0; r < RT; ++r) red[((wave * kColumns + i) * RT + r) * 64 + lane] = acc[i][r];
+  __syncthreads();
+  const int col = 16 * wave + (lane & 15), token = __shfl(tokens, col, 64);   // wave i finishes column tile i
+  if (col >= t.rows) return;
+  float* low = c.low + ((int64_t)part * c.tokens + token) * (16 * b.rank_tiles) + 16 * r0 + 4 * q;
+#pragma unroll
+  for (int r = 0; r < RT; ++r) {
+    if (r0 + r >= tiles) break;
+    v4f s = red[(wave * RT + r) * 64 + lane];
+#pragma unroll
+    for (int v = 1; v < 4; ++v) s = s + red[((v * kColumns + wave) * RT + r) * 64 + lane];
+    if (c.parts == 1) *(uint4*)(low + 16 * r) = h_operand(slot, 16 * (r0 + r) + 4 * q, s);
+    else *(v4f*)(low + 16 * r) = s;
+  }
+}
+
+// Grouped form: the parts of four ranks of a token added in order, as operand B in the first part's place.
+__global__ __launch_bounds__(256) void adapter_sum_kernel(Call c) {
+  const Bank& b = c.bank;
+  const int per = 4 * b.rank_tiles;   // entries of a token
+  const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (e >= (int64_t)c.tokens * per) return;
+  v4f* p = (v4f*)c.low + e;
+  const int64_t stride = (int64_t)c.tokens * per;
+  v4f s = p[0];
+#pragma unroll 8
+  for (int n = 1; n < c.parts; ++n) s = s + p[n * stride];
+  const int id = c.ids[e / per], r0 = 4 * (int)(e % per);
+  if (id < 0 || id >= b.slots) return;   // the sums of a token without an adapter, or past a slot's rank, are no one's
+  *(uint4*)p = h_operand(b.table[id], r0, s);
 }
 
 // ---- up: y = base + up h ----
 
 template <bool kF32>
-struct BaseValues;   // 16 consecutive values of base, the second eight where they exist
+struct Eight;   // 8 consecutive values of base
 
 template <>
-struct BaseValues<true> {
-  float4 v[4];
-  __device__ __forceinline__ void load(const void* p, bool second) {
-    const float4* s = (const float4*)p;
+struct Eight<true> {
+  float4 v[2];
+  __device__ __forceinline__ void load(const Call& c, int64_t at) {
+    const float4* s = (const float4*)((const float*)c.base + at);
     v[0] = s[0], v[1] = s[1];
-    if (second) v[2] = s[2], v[3] = s[3];
   }
   __device__ __forceinline__ v4f four(int j) const { return v4f{v[j].x, v[j].y, v[j].z, v[j].w}; }
 };
 
 template <>
-struct BaseValues<false> {
-  uint4 v[2];
-  __device__ __forceinline__ void load(const void* p, bool second) {
-    const uint4* s = (const uint4*)p;
-    v[0] = s[0];
-    if (second) v[1] = s[1];
-  }
+struct Eight<false> {
+  uint4 v;
+  __device__ __forceinline__ void load(const Call& c, int64_t at) { v = *(const uint4*)((const uint16_t*)c.base + at); }
   __device__ __forceinline__ v4f four(int j) const {
-    const uint4 u = v[j >> 1];
-    const uint32_t a = j & 1 ? u.z : u.x, b = j & 1 ? u.w : u.y;
+    const uint32_t a = j ? v.z : v.x, b = j ? v.w : v.y;
     return v4f{mx::u2f(a << 16), mx::u2f(a & 0xFFFF0000u), mx::u2f(b << 16), mx::u2f(b & 0xFFFF0000u)};
   }
 };
 
-// grid (tiles, groups of output blocks), 4 waves. The tile's h (the parts' sums, in order, times the slot's scale) goes
-// to LDS as operand B; then each wave takes output blocks of 64 in turn.
-template <bool kGrouped, bool kF32>
-__global__ __launch_bounds__(256) void adapter_up_gemm_kernel(Call c) {
-  constexpr int CT = kGrouped ? kColumns : 1;
-  extern __shared__ uint4 h_lds[];   // [CT][rank tiles][64]
-  const Tile t = tile_of<kGrouped>(c);
-  if (t.rows == 0) return;
+__device__ __forceinline__ uint4 eight_bf16(v4f a, v4f b) {
+  return make_uint4(mxd::bf16_pair(a[0], a[1]), mxd::bf16_pair(a[2], a[3]), mxd::bf16_pair(b[0], b[1]),
+                    mxd::bf16_pair(b[2], b[3]));
+}
+
+// 16 rows (of two tiles of a half each) against the 16 ranks of `h`: acc[0..3] are the tiles of the block.
+__device__ __forceinline__ void up_tile(const uint4 (&w)[2], uint4 h, v4f (&acc)[4]) {
+  const uint4 a[4] = {make_uint4(w[0].x, w[0].y, w[0].x, w[0].y), make_uint4(w[0].z, w[0].w, w[0].z, w[0].w),
+                      make_uint4(w[1].x, w[1].y, w[1].x, w[1].y), make_uint4(w[1].z, w[1].w, w[1].z, w[1].w)};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf(a[j]), as_bf(h), acc[j], 0, 0, 0);
+}
+
+// Token form, grid (T, output blocks / 4), 4 waves, a block of 64 outputs each. What does not depend
+// on h is asked for before h is put together: thread (entry e, share s) adds the parts s, s + shares, ... of four ranks,
+// and the shares are added in order.
+template <bool kF32>
+__global__ __launch_bounds__(256) void adapter_token_up_kernel(Call c) {
+  constexpr int RT = 4;   // rank tiles in registers at once
+  __shared__ v4f sums[256];
+  __shared__ uint4 h_lds[kMaxRank / 4];
+  const Tile t = one_token(c, blockIdx.x);
   const Bank& b = c.bank;
+  const int tid = threadIdx.x, lane = tid & 63, q = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  // all 16 columns are the token: column 0 finishes the block's first half, column 1 the second
+  const int half = lane & 1;
+  const bool live = (lane & 15) < 2;
+  const int64_t at_base = t.row * c.base_stride, at_y = t.row * c.y_stride;
+  const uint8_t* up = b.up + (t.slot >= 0 ? t.slot : 0) * b.up_bytes() + 16 * lane;
+  const int block = 4 * blockIdx.y + wave, n = 64 * block + 32 * half + 8 * q;   // past the last block: no one's
+  uint4 w[RT][2];
+  Eight<kF32> base = {};
+  auto load_up = [&](int r0, int count) {
+    const uint8_t* p = up + ((int64_t)min(block, b.blocks - 1) * b.rank_tiles + r0) * 2048;
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+      const int at = min(r, count - 1);
+      w[r][0] = ldg128(p + 2048 * at), w[r][1] = ldg128(p + 2048 * at + 1024);
+    }
+  };
+  if (live && n < b.n) base.load(c, at_base + n);
+  load_up(0, min(RT, b.rank_tiles));   // of the largest rank: the slot's own is still on its way
+  const AdapterSlot slot = t.slot >= 0 ? b.table[t.slot] : AdapterSlot{0, 0.f};
+  const int tiles = (slot.rank + 15) >> 4;
+  const int entries = 4 * tiles, shares = entries ? 256 / entries : 0;
+  const int64_t part_stride = (int64_t)c.tokens * 16 * b.rank_tiles;
+  if (tid < entries * shares) {
+    const float* p = c.low + (int64_t)t.row * 16 * b.rank_tiles + 4 * (tid % entries);
+    v4f sum = v4f{0.f, 0.f, 0.f, 0.f};
+    for (int n = tid / entries; n < c.parts; n += shares) sum = sum + *(const v4f*)(p + n * part_stride);
+    sums[tid] = sum;
+  }
+  __syncthreads();
+  if (tid < entries) {
+    v4f sum = sums[tid];
+    for (int s = 1; s < min(shares, c.parts); ++s) sum = sum + sums[s * entries + tid];
+    h_lds[tid] = h_operand(slot, 4 * tid, sum);
+  }
+  __syncthreads();
+  // the sums start from base, in the half of the block that the lane finishes
+  const v4f zero = v4f{0.f, 0.f, 0.f, 0.f}, v0 = base.four(0), v1 = base.four(1);
+  v4f acc[4] = {half ? zero : v0, half ? zero : v1, half ? v0 : zero, half ? v1 : zero};
+  for (int r0 = 0; r0 < tiles; r0 += RT) {
+    if (r0) load_up(r0, min(RT, tiles - r0));
+#pragma unroll
+    for (int r = 0; r < RT; ++r)
+      if (r0 + r < tiles) up_tile(w[r], h_lds[4 * (r0 + r) + q], acc);
+  }
+  if (live && n < b.n) *(uint4*)(c.y + at_y + n) = eight_bf16(half ? acc[2] : acc[0], half ? acc[3] : acc[1]);
+}
+
+// Grouped form: a tile of 64 tokens and four blocks of 64 outputs, one a wave, its weights of all ranks in registers for
+// the tile's columns, 16 tokens at a time. What does not depend on h is asked for before h goes to LDS.
+template <int RT, bool kF32>
+__global__ __launch_bounds__(256) void adapter_up_kernel(Call c) {
+  __shared__ uint4 h_lds[kColumns * RT * 64];
+  const Bank& b = c.bank;
+  const int groups = (b.blocks + 3) / 4;
+  const int work = on_xcd(blockIdx.x, groups * c.tiles), group = work / c.tiles;
+  if (group >= groups) return;
+  const Tile t = find_tile(c, work % c.tiles);
+  if (t.rows == 0) return;
   const AdapterSlot slot = t.slot >= 0 ? b.table[t.slot] : AdapterSlot{0, 0.f};
   const int tiles = (slot.rank + 15) >> 4;
   const int tid = threadIdx.x, lane = tid & 63, q = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int block = 4 * group + wave, n = 64 * block + 8 * q;   // past the last block: no output is a lane's
+  // every load below goes out before the first of them is waited for; lanes without an output repeat another's address
+  const int tokens = tile_tokens(c, t);
   const int64_t rank_stride = 16 * b.rank_tiles;
-  for (int e = tid; e < CT * tiles * 64; e += 256) {
-    const int l = e & 63, r = (e >> 6) % tiles, i = (e >> 6) / tiles;
-    const int tok = token_of<kGrouped>(c, t, 16 * i + (l & 15)), r0 = 16 * r + 4 * (l >> 4);
-    const float* p = c.low + tok * rank_stride + r0;
-    v4f s = *(const v4f*)p;
-    for (int n = 1; n < c.parts; ++n) s = s + *(const v4f*)(p + n * c.tokens * rank_stride);
-    uint32_t hi[4], lo[4];
+  uint4 h[RT];   // of the wave's column tile
+  {
+    const float* p = c.low + __shfl(tokens, 16 * wave + (lane & 15), 64) * rank_stride + 4 * q;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const float h = r0 + k < slot.rank ? slot.scale * s[k] : 0.f;
-      hi[k] = mx::bf16_bits(h);
-      const bool finite = (hi[k] & 0x7F80u) != 0x7F80u;   // an infinite h has no second term
-      lo[k] = finite ? mx::bf16_bits(h - mx::bf16_value(hi[k])) : 0u;
-    }
-    h_lds[e] = make_uint4(hi[0] | hi[1] << 16, hi[2] | hi[3] << 16, lo[0] | lo[1] << 16, lo[2] | lo[3] << 16);
+    for (int r = 0; r < RT; ++r) h[r] = ldg128((const uint8_t*)(p + 16 * max(min(r, tiles - 1), 0)));
   }
-  __syncthreads();
-  int64_t at_base[CT], at_y[CT];
-  bool live[CT];
+  uint4 w[RT][2];
+  {
+    const uint8_t* p = b.up + max(t.slot, 0) * b.up_bytes() + (int64_t)min(block, b.blocks - 1) * b.rank_tiles * 2048 + 16 * lane;
 #pragma unroll
-  for (int i = 0; i < CT; ++i) {
-    const int col = 16 * i + (lane & 15);
-    const int64_t tok = token_of<kGrouped>(c, t, col);
-    live[i] = col < t.rows;
-    at_base[i] = tok * c.base_stride;
-    at_y[i] = tok * c.y_stride;
+    for (int r = 0; r < RT; ++r) {
+      const int at = max(min(r, tiles - 1), 0);
+      w[r][0] = ldg128(p + 2048 * at), w[r][1] = ldg128(p + 2048 * at + 1024);
+    }
   }
-  const uint8_t* up = b.up + (t.slot >= 0 ? t.slot : 0) * b.up_bytes() + 16 * lane;
-  const int b0 = blockIdx.y * c.blocks_per_group, b1 = min(b0 + c.blocks_per_group, b.blocks);
-  for (int block = b0 + wave; block < b1; block += 4) {
-    const int n = 64 * block + 16 * q;
-    const bool any = n < b.n, second = n + 8 < b.n;
-    BaseValues<kF32> base[CT];
+  Eight<kF32> base[kColumns][2];
+  uint16_t* y[kColumns];
 #pragma unroll
-    for (int i = 0; i < CT; ++i)
-      if (live[i] && any)
-        base[i].load(kF32 ? (const void*)((const float*)c.base + at_base[i] + n)
-                          : (const void*)((const uint16_t*)c.base + at_base[i] + n), second);
-    v4f acc[CT][4];
+  for (int i = 0; i < kColumns; ++i) {
+    const int64_t token = __shfl(tokens, 16 * i + (lane & 15), 64);
+    y[i] = c.y + token * c.y_stride + n;
 #pragma unroll
-    for (int i = 0; i < CT; ++i)
+    for (int k = 0; k < 2; ++k) base[i][k].load(c, token * c.base_stride + (n + 32 * k < b.n ? n + 32 * k : 0));
+  }
 #pragma unroll
-      for (int j = 0; j < 4; ++j) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
-    const uint8_t* w = up + (int64_t)block * b.rank_tiles * 2048;
-    for (int r = 0; r < tiles; ++r) {
-      const uint4 w01 = ldg128(w + 2048 * r), w23 = ldg128(w + 2048 * r + 1024);
-      const uint4 a[4] = {make_uint4(w01.x, w01.y, w01.x, w01.y), make_uint4(w01.z, w01.w, w01.z, w01.w),
-                          make_uint4(w23.x, w23.y, w23.x, w23.y), make_uint4(w23.z, w23.w, w23.z, w23.w)};
+  for (int r = 0; r < RT; ++r) {
+    const int ranks = slot.rank - 16 * r - 4 * q;   // the sums past the slot's rank are not its own
+    if (ranks <= 0) h[r] = make_uint4(0, 0, 0, 0);
+    h_lds[(wave * RT + r) * 64 + lane] = h[r];
+  }
+  mxd::lds_barrier();
 #pragma unroll
-      for (int i = 0; i < CT; ++i) {
-        const v8bf h = as_bf(h_lds[(i * tiles + r) * 64 + lane]);
+  for (int i = 0; i < kColumns; ++i) {
+    if (16 * i >= t.rows) break;
+    v4f acc[4] = {base[i][0].four(0), base[i][0].four(1), base[i][1].four(0), base[i][1].four(1)};
+    if (tiles == RT) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf(a[j]), h, acc[i][j], 0, 0, 0);
-      }
+      for (int r = 0; r < RT; ++r) up_tile(w[r], h_lds[(i * RT + r) * 64 + lane], acc);
+    } else {
+#pragma unroll
+      for (int r = 0; r < RT; ++r)
+        if (r < tiles) up_tile(w[r], h_lds[(i * RT + r) * 64 + lane], acc);
     }
 #pragma unroll
-    for (int i = 0; i < CT; ++i) {
-      if (!live[i] || !any || (!kGrouped && (lane & 15))) continue;
-      uint32_t out[8];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        v4f v = base[i].four(j);
-        if (tiles) v = v + acc[i][j];
-        out[2 * j] = mx::bf16_bits(v[0]) | mx::bf16_bits(v[1]) << 16;
-        out[2 * j + 1] = mx::bf16_bits(v[2]) | mx::bf16_bits(v[3]) << 16;
-      }
-      uint4* y = (uint4*)(c.y + at_y[i] + n);
-      y[0] = make_uint4(out[0], out[1], out[2], out[3]);
-      if (second) y[1] = make_uint4(out[4], out[5], out[6], out[7]);
-    }
+    for (int k = 0; k < 2; ++k)
+      if (16 * i + (lane & 15) < t.rows && n + 32 * k < b.n) *(uint4*)(y[i] + 32 * k) = eight_bf16(acc[2 * k], acc[2 * k + 1]);
   }
 }
 
 bool is_aligned(const void* p, uintptr_t a) { return ((uintptr_t)p & (a - 1)) == 0; }
 uint64_t round256(uint64_t n) { return (n + 255) & ~(uint64_t)255; }
 
-// Parts of K for T tokens: enough workgroups for the chip, at least 8 chunks a part. parts T <= 16 kWantGroups kColumns + T.
-int parts_of(int chunks, int tokens) {
-  const int tiles = tokens <= kTokenForm ? tokens : (tokens + kTileTokens - 1) / kTileTokens;
-  const int most = std::min(kMaxParts, std::max(1, chunks / 8));
-  return std::max(1, std::min(most, (kWantGroups + tiles - 1) / tiles));
+// Tiles that T tokens in `slots` groups and the one without can make at most.
+int tiles_of(const Bank& b, int tokens) {
+  const int groups = std::min(b.slots + 1, tokens);
+  return (int)(((int64_t)tokens + (int64_t)groups * (kTileTokens - 1)) / kTileTokens);
+}
+
+// Parts of K. Token form: enough workgroups for the chip, at least one unit of 64 a wave. Grouped form: as many as are
+// resident together (two a CU) and no more, since a few beyond would run alone after the rest; at least two stages each.
+// In both, parts T is at most kWantGroups kTileTokens + T.
+int parts_of(const Bank& b, int tokens) {
+  if (tokens <= kTokenForm)
+    return std::max(1, std::min({kMaxParts, b.chunks / 8, (kWantGroups + tokens - 1) / tokens}));
+  return std::max(1, std::min({kMaxParts, b.k / (2 * kStageK), kWantGroups / tiles_of(b, tokens)}));
 }
 
 }  // namespace
@@ -378,17 +606,55 @@ Workspace workspace_of(const Bank& b, int32_t tokens) {
   return w;
 }
 
-template <bool kGrouped>
-int launch(const Call& c, int tiles, bool f32, hipStream_t st) {
-  const Bank& b = c.bank;
-  hipLaunchKernelGGL((adapter_down_gemm_kernel<kGrouped>), dim3(tiles, c.parts), dim3(256), 0, st, c);
-  MX_LAUNCH_CHECK("adapter_down_gemm_kernel");
-  const size_t lds = (size_t)(kGrouped ? kColumns : 1) * b.rank_tiles * 1024;
-  const dim3 grid(tiles, (b.blocks + c.blocks_per_group - 1) / c.blocks_per_group);
-  if (f32) hipLaunchKernelGGL((adapter_up_gemm_kernel<kGrouped, true>), grid, dim3(256), lds, st, c);
-  else hipLaunchKernelGGL((adapter_up_gemm_kernel<kGrouped, false>), grid, dim3(256), lds, st, c);
-  MX_LAUNCH_CHECK("adapter_up_gemm_kernel");
+int launch_tokens(const Call& c, bool f32, hipStream_t st) {
+  const int rt = c.bank.rank_tiles;
+  hipLaunchKernelGGL((rt == 1 ? adapter_token_down_kernel<1> : rt == 2 ? adapter_token_down_kernel<2>
+                                                                       : adapter_token_down_kernel<4>),
+                     dim3(c.tokens, c.parts), dim3(256), 0, st, c);
+  MX_LAUNCH_CHECK("adapter_token_down_kernel");
+  const dim3 grid(c.tokens, (c.bank.blocks + 3) / 4);
+  hipLaunchKernelGGL((f32 ? adapter_token_up_kernel<true> : adapter_token_up_kernel<false>), grid, dim3(256), 0, st, c);
+  MX_LAUNCH_CHECK("adapter_token_up_kernel");
   return MX_OK;
+}
+
+unsigned round8(int64_t n) { return (unsigned)((n + 7) / 8 * 8); }
+
+template <int RT, bool kStream>
+int launch_down(const Call& c, hipStream_t st) {
+  const int rank_groups = (c.bank.rank_tiles + RT - 1) / RT;
+  constexpr size_t lds = std::max(2 * kStageBytes, 4 * kColumns * RT * 1024);
+  hipLaunchKernelGGL((adapter_down_kernel<RT, kStream>), dim3(round8((int64_t)c.parts * c.tiles * rank_groups)), dim3(256), lds,
+                     st, c, rank_groups);
+  MX_LAUNCH_CHECK("adapter_down_kernel");
+  return MX_OK;
+}
+
+template <int RT>
+int launch_up(const Call& c, bool f32, hipStream_t st) {
+  const int groups = (c.bank.blocks + 3) / 4;
+  hipLaunchKernelGGL((f32 ? adapter_up_kernel<RT, true> : adapter_up_kernel<RT, false>),
+                     dim3(round8((int64_t)groups * c.tiles)), dim3(256), 0, st, c);
+  MX_LAUNCH_CHECK("adapter_up_kernel");
+  return MX_OK;
+}
+
+int launch_groups(const Call& c, bool f32, hipStream_t st) {
+  const int rt = c.bank.rank_tiles;
+  const bool stream = rt <= 4 && 2 * (int64_t)c.tokens * c.bank.k > kStreamBytes;   // more rank tiles read x again
+  if (int s = rt == 1   ? (stream ? launch_down<1, true>(c, st) : launch_down<1, false>(c, st))
+              : rt == 2 ? (stream ? launch_down<2, true>(c, st) : launch_down<2, false>(c, st))
+                        : (stream ? launch_down<4, true>(c, st) : launch_down<4, false>(c, st)))
+    return s;
+  if (c.parts > 1) {
+    const int64_t entries = (int64_t)c.tokens * 4 * rt;
+    hipLaunchKernelGGL(adapter_sum_kernel, dim3((unsigned)((entries + 255) / 256)), dim3(256), 0, st, c);
+    MX_LAUNCH_CHECK("adapter_sum_kernel");
+  }
+  if (rt == 1) return launch_up<1>(c, f32, st);
+  if (rt == 2) return launch_up<2>(c, f32, st);
+  if (rt <= 4) return launch_up<4>(c, f32, st);
+  return rt <= 8 ? launch_up<8>(c, f32, st) : launch_up<16>(c, f32, st);
 }
 
 }  // namespace
@@ -405,7 +671,7 @@ int mx_adapters_create(mx_ctx* ctx, int32_t n, int32_t k, int32_t slots, int32_t
   if (int s = use(ctx)) return s;
   Bank b{};
   b.n = n, b.k = k, b.slots = slots;
-  b.rank_tiles = (max_rank + 15) / 16, b.chunks = (k + 31) / 32, b.blocks = (n + 63) / 64;
+  b.rank_tiles = (max_rank + 15) / 16, b.chunks = (k + 63) / 64 * 2, b.blocks = (n + 63) / 64;
   const uint64_t down = (uint64_t)slots * b.down_bytes(), up = (uint64_t)slots * b.up_bytes();
   void* base = nullptr;
   if (int s = mx_malloc(ctx, down + up + round256(slots * sizeof(AdapterSlot)), &base)) return s;
@@ -443,12 +709,12 @@ int mx_adapters_load(mx_adapters* a, int32_t slot, const uint16_t* down, const u
   hipStream_t st = as_stream(stream);
   const int tiles = (rank + 15) / 16;
   if (rank) {
-    hipLaunchKernelGGL(adapter_down_kernel, dim3(b.chunks, tiles), dim3(64), 0, st, b, a->down, slot, down, rank);
-    MX_LAUNCH_CHECK("adapter_down_kernel");
+    hipLaunchKernelGGL(adapter_store_down_kernel, dim3(b.chunks, tiles), dim3(64), 0, st, b, a->down, slot, down, rank);
+    MX_LAUNCH_CHECK("adapter_store_down_kernel");
   }
-  hipLaunchKernelGGL(adapter_up_kernel, dim3(rank ? b.blocks : 1, rank ? tiles : 1), dim3(128), 0, st, b, a->up,
+  hipLaunchKernelGGL(adapter_store_up_kernel, dim3(rank ? b.blocks : 1, rank ? tiles : 1), dim3(128), 0, st, b, a->up,
                      a->table, slot, up, rank, scale);
-  MX_LAUNCH_CHECK("adapter_up_kernel");
+  MX_LAUNCH_CHECK("adapter_store_up_kernel");
   return MX_OK;
 }
 
@@ -486,9 +752,9 @@ int mx_adapters_apply(mx_adapters* a, const uint16_t* x, int64_t x_stride, const
   if (int s = use(a->ctx)) return s;
   hipStream_t st = as_stream(stream);
   uint8_t* ws = (uint8_t*)workspace;
-  Call c{b, x, x_stride, ids, nullptr, nullptr, tokens, parts_of(b.chunks, tokens), (float*)(ws + w.low),
-         base, base_stride, y, y_stride, 4};
-  if (tokens <= kTokenForm) return launch<false>(c, tokens, f32, st);
+  Call c{b, x, x_stride, ids, nullptr, nullptr, tokens, parts_of(b, tokens), (float*)(ws + w.low),
+         base, base_stride, y, y_stride, 0};
+  if (tokens <= kTokenForm) return launch_tokens(c, f32, st);
   mx_row_plan own{(int32_t*)ws, (int32_t*)(ws + w.pair_row), (int32_t*)(ws + w.row_pair)};
   if (!plan) {
     if (int s = mxi::row_plan(ids, tokens, b.slots, own, st)) return s;
@@ -496,10 +762,8 @@ int mx_adapters_apply(mx_adapters* a, const uint16_t* x, int64_t x_stride, const
   }
   c.first = plan->first;
   c.row_pair = plan->row_pair;
-  c.blocks_per_group = 16;
-  const int groups = std::min(b.slots + 1, tokens);
-  const int tiles = (int)(((int64_t)tokens + (int64_t)groups * (kTileTokens - 1)) / kTileTokens);
-  return launch<true>(c, tiles, f32, st);
+  c.tiles = tiles_of(b, tokens);
+  return launch_groups(c, f32, st);
 }
 
 }  // extern "C"

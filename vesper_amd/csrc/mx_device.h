@@ -147,6 +147,14 @@ __device__ __forceinline__ float bf16_round_sel(float f) {
   return mx::u2f((b & 0x7FFFFFFFu) > 0x7F800000u ? qnan : rne);
 }
 
+// mx::bf16_bits of two values, the first in the low half: one V_CVT_PK_BF16_F32, equal to the software rounding on
+// every FP32 bit pattern (NaN included; checked on gfx950 over all 2^32).
+__device__ __forceinline__ uint32_t bf16_pair(float lo, float hi) {
+  typedef float f2 __attribute__((ext_vector_type(2)));
+  typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2{lo, hi}), b2));
+}
+
 __device__ __forceinline__ v4f mfma_fp8_fp8(uint4 a0, uint4 a1, uint4 b0, uint4 b1, v4f c, int sa, int sb) {
   const v8i av = {(int)a0.x, (int)a0.y, (int)a0.z, (int)a0.w, (int)a1.x, (int)a1.y, (int)a1.z, (int)a1.w};
   const v8i bv = {(int)b0.x, (int)b0.y, (int)b0.z, (int)b0.w, (int)b1.x, (int)b1.y, (int)b1.z, (int)b1.w};

@@ -283,7 +283,7 @@ struct Unit<MX_ROWS_BF16, 8> {
   static __device__ __forceinline__ Raw round(const float* v) {
     uint32_t w[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = mx::bf16_bits(v[2 * i]) | (mx::bf16_bits(v[2 * i + 1]) << 16);
+    for (int i = 0; i < 4; ++i) w[i] = mxd::bf16_pair(v[2 * i], v[2 * i + 1]);
     return make_uint4(w[0], w[1], w[2], w[3]);
   }
 };
