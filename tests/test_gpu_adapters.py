@@ -68,7 +68,7 @@ def check(got, x, ids, base, adapters, exact):
 
 # (tokens, rows, width, slots, max_rank): either form and its border, ragged tiles, one value more than a chunk or block
 SHAPES = [(1, 8, 8, 1, 1), (1, 64, 32, 1, 16), (1, 2112, 1536, 3, 64), (2, 72, 40, 2, 7), (5, 24, 520, 8, 256),
-          (31, 576, 128, 5, 17), (32, 136, 1600, 4, 33), (33, 64, 72, 3, 16), (47, 200, 264, 8, 256),
+          (31, 576, 128, 5, 17), (32, 136, 1600, 4, 33), (33, 64, 72, 3, 16), (40, 1032, 2048, 2, 32), (47, 200, 264, 8, 256), (60, 24, 104, 1, 128),
           (64, 1024, 96, 70, 64), (65, 8, 1536, 1, 100), (100, 320, 8, 90, 8), (257, 88, 160, 6, 64),
           (1000, 264, 520, 8, 128)]
 
@@ -90,7 +90,7 @@ def test_apply(gpu_ctx, tokens, rows, width, slots, max_rank, dtype, exact):
         check(bank.apply(x, ids, base), x, ids, base, adapters, exact)
 
 
-@pytest.mark.parametrize("tokens", [4, 90])
+@pytest.mark.parametrize("tokens", [4, 17, 64, 90])
 def test_all_or_no_tokens_of_one_adapter(gpu_ctx, tokens):
     rng = np.random.default_rng(tokens)
     rows, width = 72, 136

@@ -193,12 +193,14 @@ class Library:
 
     def __getattr__(self, name):
         fn = getattr(self.cdll, "mx_" + name)
+        checked = fn.restype is C.c_int and name not in ("device_count",)
 
         def call(*args):
             status = fn(*args)
-            if fn.restype is C.c_int and name not in ("device_count",):
+            if checked and status != MX_OK:
                 self.check(status, "mx_" + name)
             return status
+        self.__dict__[name] = call   # found directly from the next call on
         return call
 
 

@@ -109,15 +109,15 @@ class AdapterBank:
         values (None: contiguous). plan: the MxRowPlan of ids (ExpertDispatch(ctx, slots, 1, tokens).plan after
         plan_device), made once for all projections of a step; None makes it within the call. No synchronisation."""
         self._open()
-        if not 0 <= int(tokens) <= self.max_tokens:
+        if not 0 <= tokens <= self.max_tokens:
             raise ValueError(f"token count outside [0, {self.max_tokens}]")
         if base_dtype not in ("bf16", "f32"):
             raise ValueError("base type must be bf16 or f32")
-        self.ctx.lib.adapters_apply(self.handle, _lib.vp(x_ptr), x_stride or self.width, _lib.vp(ids_ptr),
-                                    None if plan is None else C.byref(plan), int(tokens), _lib.vp(base_ptr),
-                                    _lib.MX_ROWS[base_dtype], base_stride or self.rows, _lib.vp(y_ptr),
-                                    y_stride or self.rows, C.c_void_p(self.workspace), self.workspace_bytes,
-                                    _lib._stream(stream))
+        ptr = _lib.ptr
+        self.ctx.lib.adapters_apply(self.handle, ptr(x_ptr), x_stride or self.width, ptr(ids_ptr),
+                                    None if plan is None else C.byref(plan), tokens, ptr(base_ptr),
+                                    _lib.MX_ROWS[base_dtype], base_stride or self.rows, ptr(y_ptr),
+                                    y_stride or self.rows, self.workspace, self.workspace_bytes, stream)
 
     def check_ids(self, ids, tokens: int) -> np.ndarray:
         """Host slot ids [tokens] as int32: each a slot of the bank, or -1 for none."""

@@ -31,10 +31,11 @@ typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 
 constexpr int kMaxTokens = 1 << 18, kMaxSlots = 1024, kMaxRank = 256;
 constexpr int kMaxWidth = 1 << 20;
-constexpr int kTokenForm = 32;     // calls of up to this many tokens run a token at a time
+constexpr int kFewTokens = 64;     // calls of up to this many tokens need no plan: a wave holds their ids
 constexpr int kTileTokens = 64;    // tokens of a workgroup in the grouped form
 constexpr int kColumns = kTileTokens / 16;
 constexpr int kMaxParts = 32;      // parts of K
+constexpr int kFusedChunks = 256;  // KB of down up to which a call of few tokens is one launch
 constexpr int64_t kStreamBytes = 96 << 20;   // an x of more than this is read past the caches
 constexpr int kWantGroups = 512;   // workgroups that the split of K aims at
 
@@ -105,7 +106,7 @@ struct Call {
 
 struct Tile {
   int slot;        // -1: tokens without an adapter
-  int row, rows;   // grouped: sorted rows; token form: the token, 1
+  int row, rows;   // sorted rows
 };
 
 // Tile `index` of the plan's groups, kTileTokens sorted rows each (a group's last one short), the tokens without an
@@ -140,9 +141,24 @@ __device__ __forceinline__ Tile find_tile(const Call& c, int index) {
               __builtin_amdgcn_readfirstlane(t.rows)};
 }
 
-__device__ __forceinline__ Tile one_token(const Call& c, int token) {
-  const int id = __builtin_amdgcn_readfirstlane(c.ids[token]);
-  return Tile{id >= 0 && id < c.bank.slots ? id : -1, token, 1};
+// Few tokens: the workgroups of token t take the tokens of t's adapter, up to 16 a workgroup. The first of each 16 does
+// it; rows = 0 for the others.
+struct Few {
+  int slot, rows;
+  int token;   // of this lane's column, lane % 16; columns past the last repeat it
+};
+
+__device__ __forceinline__ Few few_tokens(const Call& c, int t) {
+  const int lane = threadIdx.x & 63;
+  int id = c.ids[min(lane, c.tokens - 1)];
+  id = lane >= c.tokens ? -2 : id >= 0 && id < c.bank.slots ? id : -1;
+  const int slot = __builtin_amdgcn_readlane(id, t);
+  const uint64_t mask = __ballot(id == slot);
+  const int before = __popcll(mask & ((1ull << t) - 1)), rows = before & 15 ? 0 : min(16, (int)__popcll(mask) - before);
+  const int place = __popcll(mask & ((1ull << lane) - 1)) - before;
+  const bool mine = id == slot && place >= 0 && place < 16;
+  const int tokens = __builtin_amdgcn_ds_permute(4 * (mine ? place : 63), lane);   // lane 63 is no column's
+  return Few{slot, rows, __shfl(tokens, min(lane & 15, max(rows, 1) - 1), 64)};
 }
 
 // The tokens of the tile's 64 columns, one a lane; columns past the last repeat it.
@@ -175,21 +191,21 @@ __device__ __forceinline__ uint4 h_operand(const AdapterSlot& slot, int r0, v4f 
 
 // ---- down: partial sums of h ----
 
-// Token form, grid (T, parts), 4 waves: a part of K for one token, given to every column, and RT rank tiles at a time
-// (those past the last repeat it). The waves take the K units (of 64: two chunks) in turn, the next one's loads in
+// Few tokens, grid (T, parts), 4 waves: a part of K for up to 16 tokens of an adapter, RT rank tiles at a time (those past
+// the last repeat it). The waves take the K units (of 64: two chunks) in turn, the next one's loads in
 // flight while one is multiplied, and their sums are added in wave order.
 template <int RT>
-__device__ __forceinline__ void token_down(const Call& c, int token, int slot, int r0, int tiles, int first_tiles,
-                                           v4f (*red)[RT][64]) {
+__device__ __forceinline__ void few_down(const Call& c, const Few& f, int r0, int tiles, int first_tiles,
+                                         v4f (*red)[RT][64]) {
   const Bank& b = c.bank;
   const int tid = threadIdx.x, lane = tid & 63, q = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int units = b.chunks / 2, whole = b.k / 64;
   const int u1 = (int)((int64_t)units * (blockIdx.y + 1) / c.parts);
   int u = (int)((int64_t)units * blockIdx.y / c.parts) + wave;
-  const uint8_t* x = (const uint8_t*)(c.x + token * c.x_stride) + 16 * q;
+  const uint8_t* x = (const uint8_t*)(c.x + f.token * c.x_stride) + 16 * q;
   const int64_t tile_bytes = (int64_t)b.chunks * 1024;
-  const uint8_t* w = b.down + slot * b.down_bytes() + r0 * tile_bytes + 16 * lane;
+  const uint8_t* w = b.down + f.slot * b.down_bytes() + r0 * tile_bytes + 16 * lane;
   struct Unit {
     uint4 x[2], w[2][RT];
   } unit[2];
@@ -241,22 +257,22 @@ __device__ __forceinline__ void token_down(const Call& c, int token, int slot, i
   for (int r = 0; r < RT; ++r) red[wave][r][lane] = acc[r];
   __syncthreads();
   for (int r = wave; r < RT; r += 4)
-    if (r0 + r < tiles && (lane & 15) == 0) {
+    if (r0 + r < tiles && (lane & 15) < f.rows) {
       const v4f s = ((red[0][r][lane] + red[1][r][lane]) + red[2][r][lane]) + red[3][r][lane];
-      *(v4f*)(c.low + ((int64_t)blockIdx.y * c.tokens + token) * (16 * b.rank_tiles) + 16 * (r0 + r) + 4 * q) = s;
+      *(v4f*)(c.low + ((int64_t)blockIdx.y * c.tokens + f.token) * (16 * b.rank_tiles) + 16 * (r0 + r) + 4 * q) = s;
     }
   __syncthreads();
 }
 
 // The first unit's weights are asked for by the bank's largest rank, before the slot's own has arrived.
 template <int RT>
-__global__ __launch_bounds__(256) void adapter_token_down_kernel(Call c) {
+__global__ __launch_bounds__(256) void adapter_few_down_kernel(Call c) {
   __shared__ v4f red[4][RT][64];
-  const Tile t = one_token(c, blockIdx.x);
-  if (t.slot < 0) return;
-  const int tiles = (c.bank.table[t.slot].rank + 15) >> 4;
-  token_down<RT>(c, t.row, t.slot, 0, tiles, min(RT, c.bank.rank_tiles), red);
-  for (int r0 = RT; r0 < tiles; r0 += RT) token_down<RT>(c, t.row, t.slot, r0, tiles, min(RT, tiles - r0), red);
+  const Few f = few_tokens(c, blockIdx.x);
+  if (f.rows == 0 || f.slot < 0) return;
+  const int tiles = (c.bank.table[f.slot].rank + 15) >> 4;
+  few_down<RT>(c, f, 0, tiles, min(RT, c.bank.rank_tiles), red);
+  for (int r0 = RT; r0 < tiles; r0 += RT) few_down<RT>(c, f, r0, tiles, min(RT, tiles - r0), red);
 }
 
 // Grouped form: a part of K for a tile of 64 tokens and RT rank tiles, 4 waves. x comes through LDS in stages of 256 K,
@@ -431,63 +447,153 @@ __device__ __forceinline__ void up_tile(const uint4 (&w)[2], uint4 h, v4f (&acc)
   for (int j = 0; j < 4; ++j) acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf(a[j]), as_bf(h), acc[j], 0, 0, 0);
 }
 
-// Token form, grid (T, output blocks / 4), 4 waves, a block of 64 outputs each. What does not depend
-// on h is asked for before h is put together: thread (entry e, share s) adds the parts s, s + shares, ... of four ranks,
-// and the shares are added in order.
+// Few tokens, grid (T, output blocks / 4), 4 waves, a block of 64 outputs each for up to 16 tokens of an adapter. What does
+// not depend on h is asked for before h is put together: thread (entry e, share s) adds the parts s, s + shares, ... of
+// four ranks of a token, and the shares are added in order.
 template <bool kF32>
-__global__ __launch_bounds__(256) void adapter_token_up_kernel(Call c) {
+__global__ __launch_bounds__(256) void adapter_few_up_kernel(Call c) {
   constexpr int RT = 4;   // rank tiles in registers at once
   __shared__ v4f sums[256];
-  __shared__ uint4 h_lds[kMaxRank / 4];
-  const Tile t = one_token(c, blockIdx.x);
+  __shared__ uint4 h_lds[kMaxRank / 16 * 64];
+  const Few f = few_tokens(c, blockIdx.x);
+  if (f.rows == 0) return;
   const Bank& b = c.bank;
   const int tid = threadIdx.x, lane = tid & 63, q = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  // all 16 columns are the token: column 0 finishes the block's first half, column 1 the second
-  const int half = lane & 1;
-  const bool live = (lane & 15) < 2;
-  const int64_t at_base = t.row * c.base_stride, at_y = t.row * c.y_stride;
-  const uint8_t* up = b.up + (t.slot >= 0 ? t.slot : 0) * b.up_bytes() + 16 * lane;
-  const int block = 4 * blockIdx.y + wave, n = 64 * block + 32 * half + 8 * q;   // past the last block: no one's
+  const int block = 4 * blockIdx.y + wave, n = 64 * block + 8 * q;   // past the last block: no output is a lane's
+  const uint8_t* up = b.up + max(f.slot, 0) * b.up_bytes() + (int64_t)min(block, b.blocks - 1) * b.rank_tiles * 2048 + 16 * lane;
   uint4 w[RT][2];
-  Eight<kF32> base = {};
   auto load_up = [&](int r0, int count) {
-    const uint8_t* p = up + ((int64_t)min(block, b.blocks - 1) * b.rank_tiles + r0) * 2048;
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
-      const int at = min(r, count - 1);
-      w[r][0] = ldg128(p + 2048 * at), w[r][1] = ldg128(p + 2048 * at + 1024);
+      const int at = r0 + min(r, count - 1);
+      w[r][0] = ldg128(up + 2048 * at), w[r][1] = ldg128(up + 2048 * at + 1024);
     }
   };
-  if (live && n < b.n) base.load(c, at_base + n);
+  Eight<kF32> base[2];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) base[k].load(c, f.token * c.base_stride + (n + 32 * k < b.n ? n + 32 * k : 0));
   load_up(0, min(RT, b.rank_tiles));   // of the largest rank: the slot's own is still on its way
-  const AdapterSlot slot = t.slot >= 0 ? b.table[t.slot] : AdapterSlot{0, 0.f};
+  const AdapterSlot slot = f.slot >= 0 ? b.table[f.slot] : AdapterSlot{0, 0.f};
   const int tiles = (slot.rank + 15) >> 4;
-  const int entries = 4 * tiles, shares = entries ? 256 / entries : 0;
+  // entry e: ranks 4 (e / rows) .. of column e % rows
+  const int entries = 4 * tiles * f.rows, shares = entries ? max(256 / entries, 1) : 0;
   const int64_t part_stride = (int64_t)c.tokens * 16 * b.rank_tiles;
-  if (tid < entries * shares) {
-    const float* p = c.low + (int64_t)t.row * 16 * b.rank_tiles + 4 * (tid % entries);
+  for (int e0 = 0; e0 < entries; e0 += 256) {
+    const int e = e0 + (shares > 1 ? tid % entries : tid), share = shares > 1 ? tid / entries : 0;
+    const int column = e % f.rows, token = __shfl(f.token, column, 64);
+    const bool in = e < entries && share < shares;
     v4f sum = v4f{0.f, 0.f, 0.f, 0.f};
-    for (int n = tid / entries; n < c.parts; n += shares) sum = sum + *(const v4f*)(p + n * part_stride);
-    sums[tid] = sum;
+    if (in) {
+      const float* p = c.low + (int64_t)token * 16 * b.rank_tiles + 4 * (e / f.rows);
+#pragma unroll 8
+      for (int m = share; m < c.parts; m += shares) sum = sum + *(const v4f*)(p + m * part_stride);
+    }
+    if (shares > 1) {
+      sums[tid] = sum;
+      __syncthreads();
+      if (tid < entries)
+        for (int m = 1; m < min(shares, c.parts); ++m) sum = sum + sums[m * entries + tid];
+    }
+    if (in && share == 0) h_lds[e / f.rows * 16 + column] = h_operand(slot, 4 * (e / f.rows), sum);
   }
   __syncthreads();
-  if (tid < entries) {
-    v4f sum = sums[tid];
-    for (int s = 1; s < min(shares, c.parts); ++s) sum = sum + sums[s * entries + tid];
-    h_lds[tid] = h_operand(slot, 4 * tid, sum);
-  }
-  __syncthreads();
-  // the sums start from base, in the half of the block that the lane finishes
-  const v4f zero = v4f{0.f, 0.f, 0.f, 0.f}, v0 = base.four(0), v1 = base.four(1);
-  v4f acc[4] = {half ? zero : v0, half ? zero : v1, half ? v0 : zero, half ? v1 : zero};
+  v4f acc[4] = {base[0].four(0), base[0].four(1), base[1].four(0), base[1].four(1)};
   for (int r0 = 0; r0 < tiles; r0 += RT) {
     if (r0) load_up(r0, min(RT, tiles - r0));
 #pragma unroll
     for (int r = 0; r < RT; ++r)
-      if (r0 + r < tiles) up_tile(w[r], h_lds[4 * (r0 + r) + q], acc);
+      if (r0 + r < tiles) up_tile(w[r], h_lds[64 * (r0 + r) + lane], acc);
   }
-  if (live && n < b.n) *(uint4*)(c.y + at_y + n) = eight_bf16(half ? acc[2] : acc[0], half ? acc[3] : acc[1]);
+#pragma unroll
+  for (int k = 0; k < 2; ++k)
+    if ((lane & 15) < f.rows && n + 32 * k < b.n)
+      *(uint4*)(c.y + f.token * c.y_stride + n + 32 * k) = eight_bf16(acc[2 * k], acc[2 * k + 1]);
+}
+
+// Few tokens in one launch, for a down that every workgroup can read for itself: grid (T, output blocks / 16), 16 waves.
+// The waves take the K units of 64 in turn, two of them in flight, h is put together through LDS, and each wave finishes
+// a block of 64 outputs whose up and base were asked for at the start.
+template <int RT, bool kF32>
+__global__ __launch_bounds__(1024) void adapter_few_kernel(Call c) {
+  __shared__ v4f sums[16][RT][64];
+  __shared__ uint4 h_lds[RT][64];
+  const int tid = threadIdx.x, lane = tid & 63, q = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const Bank& b = c.bank;
+  const Few f = few_tokens(c, blockIdx.x);
+  if (f.rows == 0) return;
+  const int block = 16 * blockIdx.y + wave, n = 64 * block + 8 * q;
+  const int units = b.chunks / 2, last = b.rank_tiles - 1;
+  const int64_t tile_bytes = (int64_t)b.chunks * 1024;
+  const uint8_t* x = (const uint8_t*)(c.x + f.token * c.x_stride) + 16 * q;
+  const uint8_t* down = b.down + max(f.slot, 0) * b.down_bytes() + 16 * lane;
+  const uint8_t* up = b.up + max(f.slot, 0) * b.up_bytes() + (int64_t)min(block, b.blocks - 1) * b.rank_tiles * 2048 + 16 * lane;
+  struct Unit {
+    uint4 x[2], w[2][RT];
+  } unit[2];
+  auto load = [&](Unit& m, int at) {   // a unit past the last repeats it; what lies past the end of x is zero
+    at = min(at, units - 1);
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const bool in = 64 * at + 32 * s + 8 * q < b.k;
+      const uint4 v = ldg128(in ? x + 128 * at + 64 * s : x - 16 * q);
+      m.x[s] = in ? v : make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int r = 0; r < RT; ++r) m.w[s][r] = ldg128(down + min(r, last) * tile_bytes + 2048 * (int64_t)at + 1024 * s);
+    }
+  };
+  Eight<kF32> base[2];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) base[k].load(c, f.token * c.base_stride + (n + 32 * k < b.n ? n + 32 * k : 0));
+  uint4 w[RT][2];
+  v4f acc[RT];
+#pragma unroll
+  for (int r = 0; r < RT; ++r) acc[r] = v4f{0.f, 0.f, 0.f, 0.f};
+  auto multiply = [&](const Unit& m) {
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int r = 0; r < RT; ++r)
+        acc[r] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf(m.w[s][r]), as_bf(m.x[s]), acc[r], 0, 0, 0);
+  };
+  if (f.slot >= 0) {
+    load(unit[0], wave);
+    load(unit[1], wave + 16);
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+      w[r][0] = ldg128(up + 2048 * min(r, last));
+      w[r][1] = ldg128(up + 2048 * min(r, last) + 1024);
+    }
+    for (int u = wave; u < units; u += 32) {
+      multiply(unit[0]);
+      if (u + 32 < units) load(unit[0], u + 32);
+      if (u + 16 < units) {
+        multiply(unit[1]);
+        if (u + 48 < units) load(unit[1], u + 48);
+      }
+    }
+  }
+  const AdapterSlot slot = f.slot >= 0 ? b.table[f.slot] : AdapterSlot{0, 0.f};
+  const int tiles = (slot.rank + 15) >> 4;
+#pragma unroll
+  for (int r = 0; r < RT; ++r) sums[wave][r][lane] = acc[r];
+  __syncthreads();
+  if (wave < RT) {   // wave r puts rank tile r together
+    v4f sum = sums[0][wave][lane];
+#pragma unroll
+    for (int v = 1; v < 16; ++v) sum = sum + sums[v][wave][lane];
+    h_lds[wave][lane] = h_operand(slot, 16 * wave + 4 * q, sum);
+  }
+  __syncthreads();
+  v4f out[4] = {base[0].four(0), base[0].four(1), base[1].four(0), base[1].four(1)};
+#pragma unroll
+  for (int r = 0; r < RT; ++r)
+    if (r < tiles) up_tile(w[r], h_lds[r][lane], out);
+#pragma unroll
+  for (int k = 0; k < 2; ++k)
+    if ((lane & 15) < f.rows && n + 32 * k < b.n)
+      *(uint4*)(c.y + f.token * c.y_stride + n + 32 * k) = eight_bf16(out[2 * k], out[2 * k + 1]);
 }
 
 // Grouped form: a tile of 64 tokens and four blocks of 64 outputs, one a wave, its weights of all ranks in registers for
@@ -567,12 +673,12 @@ int tiles_of(const Bank& b, int tokens) {
   return (int)(((int64_t)tokens + (int64_t)groups * (kTileTokens - 1)) / kTileTokens);
 }
 
-// Parts of K. Token form: enough workgroups for the chip, at least one unit of 64 a wave. Grouped form: as many as are
-// resident together (two a CU) and no more, since a few beyond would run alone after the rest; at least two stages each.
-// In both, parts T is at most kWantGroups kTileTokens + T.
+// Parts of K. Few tokens: enough workgroups for the chip if the tokens' adapters differ, at least one unit of 64 a wave.
+// Grouped form: as many as are resident together (two a CU) and no more, since a few beyond would run alone after the
+// rest; at least two stages each. In both, parts T is at most kWantGroups kTileTokens + T.
 int parts_of(const Bank& b, int tokens) {
-  if (tokens <= kTokenForm)
-    return std::max(1, std::min({kMaxParts, b.chunks / 8, (kWantGroups + tokens - 1) / tokens}));
+  if (tokens <= kFewTokens)
+    return std::max(1, std::min({kMaxParts, b.chunks / 8, (2 * kWantGroups + tokens - 1) / tokens}));
   return std::max(1, std::min({kMaxParts, b.k / (2 * kStageK), kWantGroups / tiles_of(b, tokens)}));
 }
 
@@ -606,15 +712,26 @@ Workspace workspace_of(const Bank& b, int32_t tokens) {
   return w;
 }
 
-int launch_tokens(const Call& c, bool f32, hipStream_t st) {
+template <int RT>
+int launch_fused(const Call& c, bool f32, hipStream_t st) {
+  const dim3 grid(c.tokens, (c.bank.blocks + 15) / 16);
+  hipLaunchKernelGGL((f32 ? adapter_few_kernel<RT, true> : adapter_few_kernel<RT, false>), grid, dim3(1024), 0, st, c);
+  MX_LAUNCH_CHECK("adapter_few_kernel");
+  return MX_OK;
+}
+
+int launch_few(const Call& c, bool f32, hipStream_t st) {
   const int rt = c.bank.rank_tiles;
-  hipLaunchKernelGGL((rt == 1 ? adapter_token_down_kernel<1> : rt == 2 ? adapter_token_down_kernel<2>
-                                                                       : adapter_token_down_kernel<4>),
+  if (rt <= 2 && rt * c.bank.chunks <= kFusedChunks)
+    return rt == 1 ? launch_fused<1>(c, f32, st) : launch_fused<2>(c, f32, st);
+  hipLaunchKernelGGL((rt == 1   ? adapter_few_down_kernel<1>
+                      : rt == 2 ? adapter_few_down_kernel<2>
+                                : adapter_few_down_kernel<4>),
                      dim3(c.tokens, c.parts), dim3(256), 0, st, c);
-  MX_LAUNCH_CHECK("adapter_token_down_kernel");
+  MX_LAUNCH_CHECK("adapter_few_down_kernel");
   const dim3 grid(c.tokens, (c.bank.blocks + 3) / 4);
-  hipLaunchKernelGGL((f32 ? adapter_token_up_kernel<true> : adapter_token_up_kernel<false>), grid, dim3(256), 0, st, c);
-  MX_LAUNCH_CHECK("adapter_token_up_kernel");
+  hipLaunchKernelGGL((f32 ? adapter_few_up_kernel<true> : adapter_few_up_kernel<false>), grid, dim3(256), 0, st, c);
+  MX_LAUNCH_CHECK("adapter_few_up_kernel");
   return MX_OK;
 }
 
@@ -754,7 +871,7 @@ int mx_adapters_apply(mx_adapters* a, const uint16_t* x, int64_t x_stride, const
   uint8_t* ws = (uint8_t*)workspace;
   Call c{b, x, x_stride, ids, nullptr, nullptr, tokens, parts_of(b, tokens), (float*)(ws + w.low),
          base, base_stride, y, y_stride, 0};
-  if (tokens <= kTokenForm) return launch_tokens(c, f32, st);
+  if (tokens <= kFewTokens) return launch_few(c, f32, st);
   mx_row_plan own{(int32_t*)ws, (int32_t*)(ws + w.pair_row), (int32_t*)(ws + w.row_pair)};
   if (!plan) {
     if (int s = mxi::row_plan(ids, tokens, b.slots, own, st)) return s;
