@@ -36,7 +36,8 @@ constexpr int kTileTokens = 64;    // tokens of a workgroup in the grouped form
 constexpr int kColumns = kTileTokens / 16;
 constexpr int kMaxParts = 32;      // parts of K
 constexpr int kFusedChunks = 256;  // KB of down up to which a call of few tokens is one launch
-constexpr int64_t kStreamBytes = 96 << 20;   // an x of more than this is read past the caches
+// An x of more than this is read, and the y of a base and y of more than this written, past the caches.
+constexpr int64_t kStreamBytes = 96 << 20;
 constexpr int kWantGroups = 512;   // workgroups that the split of K aims at
 
 struct AdapterSlot {
@@ -102,6 +103,7 @@ struct Call {
   uint16_t* y;
   int64_t y_stride;
   int32_t tiles;             // grouped form: the most tiles that there can be
+  bool stream;               // grouped form: y is written past the caches
 };
 
 struct Tile {
@@ -424,19 +426,41 @@ struct Eight<true> {
   __device__ __forceinline__ v4f four(int j) const { return v4f{v[j].x, v[j].y, v[j].z, v[j].w}; }
 };
 
+// Four of the eight BF16 values, the second four with `second`.
+__device__ __forceinline__ v4f four_of(uint4 v, int second) {
+  const uint32_t a = second ? v.z : v.x, b = second ? v.w : v.y;
+  return v4f{mx::u2f(a << 16), mx::u2f(a & 0xFFFF0000u), mx::u2f(b << 16), mx::u2f(b & 0xFFFF0000u)};
+}
+
 template <>
 struct Eight<false> {
   uint4 v;
   __device__ __forceinline__ void load(const Call& c, int64_t at) { v = *(const uint4*)((const uint16_t*)c.base + at); }
-  __device__ __forceinline__ v4f four(int j) const {
-    const uint32_t a = j ? v.z : v.x, b = j ? v.w : v.y;
-    return v4f{mx::u2f(a << 16), mx::u2f(a & 0xFFFF0000u), mx::u2f(b << 16), mx::u2f(b & 0xFFFF0000u)};
-  }
+  __device__ __forceinline__ v4f four(int j) const { return four_of(v, j); }
 };
 
 __device__ __forceinline__ uint4 eight_bf16(v4f a, v4f b) {
   return make_uint4(mxd::bf16_pair(a[0], a[1]), mxd::bf16_pair(a[2], a[3]), mxd::bf16_pair(b[0], b[1]),
                     mxd::bf16_pair(b[2], b[3]));
+}
+
+// Two 16-byte pieces a lane between operand order and memory order. In operand order lane (column, q) holds pieces q of
+// the first and of the second 64 bytes of its column's token, so an access takes 64 bytes of 16 rows; in memory order
+// the lanes of columns 0-7 hold first pieces and those of 8-15 second ones, of column % 8 and then of 8 + column % 8:
+// 128 bytes, a whole line, of 8 rows. The lanes eight apart swap one piece; the same swap leads back.
+// (A plain copy of 4096 rows of 7168 in these orders: 26 and 18 us.)
+__device__ __forceinline__ void swap8(uint4& first, uint4& second, bool low) {
+  const uint32_t a[4] = {first.x, first.y, first.z, first.w}, b[4] = {second.x, second.y, second.z, second.w};
+  uint32_t u[4], v[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {   // in numbers: a choice between structures would go through memory
+    const uint32_t give = low ? b[i] : a[i];
+    const uint32_t got = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)give, 0x128, 0xF, 0xF, false);   // row_ror:8
+    u[i] = low ? a[i] : got;
+    v[i] = low ? got : b[i];
+  }
+  first = make_uint4(u[0], u[1], u[2], u[3]);
+  second = make_uint4(v[0], v[1], v[2], v[3]);
 }
 
 // 16 rows (of two tiles of a half each) against the 16 ranks of `h`: acc[0..3] are the tiles of the block.
@@ -602,10 +626,8 @@ template <int RT, bool kF32>
 __global__ __launch_bounds__(256) void adapter_up_kernel(Call c) {
   __shared__ uint4 h_lds[kColumns * RT * 64];
   const Bank& b = c.bank;
-  const int groups = (b.blocks + 3) / 4;
-  const int work = on_xcd(blockIdx.x, groups * c.tiles), group = work / c.tiles;
-  if (group >= groups) return;
-  const Tile t = find_tile(c, work % c.tiles);
+  const int groups = (b.blocks + 3) / 4, group = blockIdx.x % groups;
+  const Tile t = find_tile(c, blockIdx.x / groups);
   if (t.rows == 0) return;
   const AdapterSlot slot = t.slot >= 0 ? b.table[t.slot] : AdapterSlot{0, 0.f};
   const int tiles = (slot.rank + 15) >> 4;
@@ -630,15 +652,26 @@ __global__ __launch_bounds__(256) void adapter_up_kernel(Call c) {
       w[r][0] = ldg128(p + 2048 * at), w[r][1] = ldg128(p + 2048 * at + 1024);
     }
   }
-  Eight<kF32> base[kColumns][2];
-  uint16_t* y[kColumns];
+  // in memory order (see swap8): this lane's pieces are of two tokens of each column tile, eight columns apart
+  const bool low = (lane & 15) < 8;
+  uint4 base[kColumns][kF32 ? 4 : 2];
+  int64_t token[kColumns][2];
 #pragma unroll
-  for (int i = 0; i < kColumns; ++i) {
-    const int64_t token = __shfl(tokens, 16 * i + (lane & 15), 64);
-    y[i] = c.y + token * c.y_stride + n;
+  for (int i = 0; i < kColumns; ++i)
 #pragma unroll
-    for (int k = 0; k < 2; ++k) base[i][k].load(c, token * c.base_stride + (n + 32 * k < b.n ? n + 32 * k : 0));
-  }
+    for (int k = 0; k < 2; ++k) {
+      token[i][k] = __shfl(tokens, 16 * i + 8 * k + (lane & 7), 64);
+      if constexpr (kF32) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int at = n + 32 * h < b.n ? n + 32 * h + (low ? 0 : 4) : 0;
+          base[i][2 * h + k] = ldg128((const uint8_t*)((const float*)c.base + token[i][k] * c.base_stride + at));
+        }
+      } else {
+        const int at = n + (low ? 0 : 32) < b.n ? n + (low ? 0 : 32) : 0;
+        base[i][k] = ldg128((const uint8_t*)((const uint16_t*)c.base + token[i][k] * c.base_stride + at));
+      }
+    }
 #pragma unroll
   for (int r = 0; r < RT; ++r) {
     const int ranks = slot.rank - 16 * r - 4 * q;   // the sums past the slot's rank are not its own
@@ -646,10 +679,23 @@ __global__ __launch_bounds__(256) void adapter_up_kernel(Call c) {
     h_lds[(wave * RT + r) * 64 + lane] = h[r];
   }
   mxd::lds_barrier();
+  const int at_y = n + (low ? 0 : 32);
 #pragma unroll
   for (int i = 0; i < kColumns; ++i) {
     if (16 * i >= t.rows) break;
-    v4f acc[4] = {base[i][0].four(0), base[i][0].four(1), base[i][1].four(0), base[i][1].four(1)};
+    v4f acc[4];
+    if constexpr (kF32) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        swap8(base[i][2 * h], base[i][2 * h + 1], low);
+        acc[2 * h] = __builtin_bit_cast(v4f, base[i][2 * h]);
+        acc[2 * h + 1] = __builtin_bit_cast(v4f, base[i][2 * h + 1]);
+      }
+    } else {
+      swap8(base[i][0], base[i][1], low);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) acc[k] = four_of(base[i][k >> 1], k & 1);
+    }
     if (tiles == RT) {
 #pragma unroll
       for (int r = 0; r < RT; ++r) up_tile(w[r], h_lds[(i * RT + r) * 64 + lane], acc);
@@ -658,9 +704,15 @@ __global__ __launch_bounds__(256) void adapter_up_kernel(Call c) {
       for (int r = 0; r < RT; ++r)
         if (r < tiles) up_tile(w[r], h_lds[(i * RT + r) * 64 + lane], acc);
     }
+    uint4 out[2] = {eight_bf16(acc[0], acc[1]), eight_bf16(acc[2], acc[3])};
+    swap8(out[0], out[1], low);
 #pragma unroll
     for (int k = 0; k < 2; ++k)
-      if (16 * i + (lane & 15) < t.rows && n + 32 * k < b.n) *(uint4*)(y[i] + 32 * k) = eight_bf16(acc[2 * k], acc[2 * k + 1]);
+      if (16 * i + 8 * k + (lane & 7) < t.rows && at_y < b.n) {
+        mxd::u32x4_t* y = (mxd::u32x4_t*)(c.y + token[i][k] * c.y_stride + at_y);
+        if (c.stream) __builtin_nontemporal_store(__builtin_bit_cast(mxd::u32x4_t, out[k]), y);
+        else *y = __builtin_bit_cast(mxd::u32x4_t, out[k]);
+      }
   }
 }
 
@@ -751,7 +803,7 @@ template <int RT>
 int launch_up(const Call& c, bool f32, hipStream_t st) {
   const int groups = (c.bank.blocks + 3) / 4;
   hipLaunchKernelGGL((f32 ? adapter_up_kernel<RT, true> : adapter_up_kernel<RT, false>),
-                     dim3(round8((int64_t)groups * c.tiles)), dim3(256), 0, st, c);
+                     dim3((unsigned)(groups * c.tiles)), dim3(256), 0, st, c);
   MX_LAUNCH_CHECK("adapter_up_kernel");
   return MX_OK;
 }
@@ -870,7 +922,7 @@ int mx_adapters_apply(mx_adapters* a, const uint16_t* x, int64_t x_stride, const
   hipStream_t st = as_stream(stream);
   uint8_t* ws = (uint8_t*)workspace;
   Call c{b, x, x_stride, ids, nullptr, nullptr, tokens, parts_of(b, tokens), (float*)(ws + w.low),
-         base, base_stride, y, y_stride, 0};
+         base, base_stride, y, y_stride, 0, false};
   if (tokens <= kFewTokens) return launch_few(c, f32, st);
   mx_row_plan own{(int32_t*)ws, (int32_t*)(ws + w.pair_row), (int32_t*)(ws + w.row_pair)};
   if (!plan) {
@@ -880,6 +932,7 @@ int mx_adapters_apply(mx_adapters* a, const uint16_t* x, int64_t x_stride, const
   c.first = plan->first;
   c.row_pair = plan->row_pair;
   c.tiles = tiles_of(b, tokens);
+  c.stream = (int64_t)tokens * b.n * (f32 ? 6 : 4) > kStreamBytes;
   return launch_groups(c, f32, st);
 }
 
