@@ -923,6 +923,8 @@ int mx_adapters_apply(mx_adapters* a, const uint16_t* x, int64_t x_stride, const
   uint8_t* ws = (uint8_t*)workspace;
   Call c{b, x, x_stride, ids, nullptr, nullptr, tokens, parts_of(b, tokens), (float*)(ws + w.low),
          base, base_stride, y, y_stride, 0, false};
+  if (w.low + (uint64_t)c.parts * tokens * 64 * b.rank_tiles > w.bytes)   // parts_of and workspace_of belong together
+    return mxi::fail(MX_ERR_STATE, "%s: %d parts of %d tokens exceed the workspace", who, c.parts, tokens);
   if (tokens <= kFewTokens) return launch_few(c, f32, st);
   mx_row_plan own{(int32_t*)ws, (int32_t*)(ws + w.pair_row), (int32_t*)(ws + w.row_pair)};
   if (!plan) {

@@ -20,7 +20,6 @@ namespace {
 constexpr int kMaxTokens = 1 << 18;   // keeps every grid below 2^32 threads
 constexpr int kMaxTopK = 32, kMaxGroups = 1024;
 constexpr int64_t kMaxWidth = 1 << 24;
-constexpr int kFusedPairs = 1024;   // up to this many pairs the plan is made within the dispatch launch
 // Calls that move more than this go past the caches with what they touch once. The sum of a token counts only with all
 // its pairs here: an expert-parallel rank moves a fraction of what the host can tell.
 constexpr int64_t kStreamBytes = 96 << 20;
@@ -155,58 +154,40 @@ struct DispatchArgs {
   float* row_weights;
 };
 
-// The rows of the plan for one token by counting, for each of its pairs, the pairs before it: wave w counts over a
-// quarter of the ids, which it holds in registers. dst[j] is the row (past first[G] for a pair without a group).
-__device__ __forceinline__ void count_rows(const DispatchArgs& a, int t, int* dst, int (*part)[kMaxTopK]) {
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int quarter = (a.plan.pairs + 255) / 256 * 64, p0 = wave * quarter, p1 = min(p0 + quarter, a.plan.pairs);
-  int key[kFusedPairs / 256];
+// With the plan made in the same launch every workgroup counts for itself: a pair's key and index as one number,
+// key << 11 | p, orders the pairs, so row(p) is the count of smaller numbers and first[g] that of numbers below g << 11.
+constexpr int kIndexBits = 11, kFusedPairs = 1 << kIndexBits, kTargets = 8;
+
+// count[n] = how many pairs come before target[n], for up to kTargets targets at once (the others' are not used): a thread
+// holds P / 256 pairs, two counts share a register, and the waves' sums meet in LDS. `order` is this thread's pairs.
+__device__ __forceinline__ void count_before(const uint32_t* order, int pairs, const uint32_t* target, int (*part)[kTargets],
+                                             int* count) {
+  const int tid = threadIdx.x;
+  int low[kTargets / 2], high[kTargets / 2];
+#pragma unroll
+  for (int n = 0; n < kTargets / 2; ++n) low[n] = high[n] = 0;
 #pragma unroll
   for (int i = 0; i < kFusedPairs / 256; ++i)
-    if (p0 + 64 * i < p1) key[i] = p0 + 64 * i + lane < p1 ? pair_key(a.plan, p0 + 64 * i + lane) : kMaxGroups + 1;
-  for (int j = 0; j < a.k; ++j) {
-    const int p = t * a.k + j, own = pair_key(a.plan, p);
-    int n = 0;
+    if (256 * i < pairs) {
 #pragma unroll
-    for (int i = 0; i < kFusedPairs / 256; ++i)
-      if (p0 + 64 * i < p1) n += __popcll(__ballot(key[i] < own || (key[i] == own && p0 + 64 * i + lane < p)));
-    if (lane == 0) part[wave][j] = n;
-  }
-  __syncthreads();
-  if (tid < a.k) dst[tid] = part[0][tid] + part[1][tid] + part[2][tid] + part[3][tid];
-}
-
-// first[0..G] by one workgroup: the keys counted in LDS (integer additions: any order gives the same counts), then
-// summed.
-__device__ __forceinline__ void count_groups(const PlanArgs& a, int* count) {
-  __shared__ int wave_sum[4];
-  const int tid = threadIdx.x, lane = tid & 63;
-  for (int g = tid; g < kMaxGroups; g += 256) count[g] = 0;
-  __syncthreads();
-  for (int p = tid; p < a.pairs; p += 256) {
-    const int key = pair_key(a, p);
-    if (key < a.groups) atomicAdd(&count[key], 1);
-  }
-  __syncthreads();
-  int own = 0;
+      for (int n = 0; n < kTargets / 2; ++n) {
+        low[n] += order[i] < target[2 * n];
+        high[n] += order[i] < target[2 * n + 1];
+      }
+    }
 #pragma unroll
-  for (int i = 0; i < kMaxGroups / 256; ++i) own += count[tid * (kMaxGroups / 256) + i];
-  int upto = own;
+  for (int n = 0; n < kTargets / 2; ++n) {
+    int both = low[n] | high[n] << 16;   // at most 512 a wave
 #pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int o = __shfl_up(upto, d, 64);
-    if (lane >= d) upto += o;
+    for (int m = 32; m >= 1; m >>= 1) both += __shfl_xor(both, m, 64);
+    if ((tid & 63) == 0) {
+      part[tid >> 6][2 * n] = both & 0xFFFF;
+      part[tid >> 6][2 * n + 1] = both >> 16;
+    }
   }
-  if (lane == 63) wave_sum[tid >> 6] = upto;
   __syncthreads();
-  int base = upto - own;
-  for (int w = 0; w < (tid >> 6); ++w) base += wave_sum[w];
-  for (int i = 0; i < kMaxGroups / 256; ++i) {
-    const int g = tid * (kMaxGroups / 256) + i;
-    if (g <= a.groups) a.first[g] = base;
-    base += count[g];
-  }
-  if (tid == 255 && a.groups == kMaxGroups) a.first[kMaxGroups] = base;
+  if (tid < kTargets) count[tid] = part[0][tid] + part[1][tid] + part[2][tid] + part[3][tid];
+  __syncthreads();
 }
 
 // The token's row is read once and written to each of its rows. U is the widest unit that the row's bytes and the
@@ -230,28 +211,53 @@ __global__ __launch_bounds__(64) void move_rows_kernel(DispatchArgs a, int chunk
   }
 }
 
-// With the plan, in one launch for few pairs: grid (T + 1, chunks); every workgroup finds its own token's rows, the
-// first chunk's writes them, and the last column the groups' first rows.
-template <typename U>
+// With the plan, in one launch for few pairs: grid (T + workgroups of kTargets groups, chunks); every workgroup finds its
+// own token's rows, the first chunk's writes them, and the workgroups past the tokens the groups' first rows.
+template <typename U, bool kStream>
 __global__ __launch_bounds__(256) void dispatch_kernel(DispatchArgs a) {
   __shared__ int dst[kMaxTopK];
-  __shared__ int part[4][kMaxTopK];
-  __shared__ int count[kMaxGroups];
-  const int t = blockIdx.x, tid = threadIdx.x, k = a.k;
-  if (t == a.tokens) {
-    if (blockIdx.y == 0) count_groups(a.plan, count);
+  __shared__ int part[4][kTargets];
+  __shared__ int count[kTargets];
+  const int t = blockIdx.x, tid = threadIdx.x, k = a.k, pairs = a.plan.pairs;
+  if (t >= a.tokens && blockIdx.y > 0) return;
+  uint32_t order[kFusedPairs / 256];
+#pragma unroll
+  for (int i = 0; i < kFusedPairs / 256; ++i)
+    if (256 * i < pairs) order[i] = (uint32_t)a.plan.ids[min(256 * i + tid, pairs - 1)];
+#pragma unroll
+  for (int i = 0; i < kFusedPairs / 256; ++i)
+    if (256 * i < pairs) {
+      const int p = 256 * i + tid;
+      const uint32_t key = min(order[i], (uint32_t)a.plan.groups);   // ids below zero are large as unsigned numbers
+      order[i] = p < pairs ? key << kIndexBits | p : ~0u;
+    }
+  uint32_t target[kTargets];
+  if (t >= a.tokens) {
+    const int g0 = (t - a.tokens) * kTargets;
+#pragma unroll
+    for (int n = 0; n < kTargets; ++n) target[n] = (uint32_t)(g0 + n) << kIndexBits;
+    count_before(order, pairs, target, part, count);
+    if (tid < kTargets && g0 + tid <= a.plan.groups) a.plan.first[g0 + tid] = count[tid];
     return;
   }
-  count_rows(a, t, dst, part);
-  if (tid < k) {
-    const int p = t * k + tid, r = dst[tid];
-    const bool absent = pair_key(a.plan, p) == a.plan.groups;
-    if (blockIdx.y == 0) {
-      a.plan.row_pair[r] = p;
-      a.plan.pair_row[p] = absent ? -1 : r;
-      if (!absent && a.row_weights) a.row_weights[r] = a.weights[p];
+  for (int j0 = 0; j0 < k; j0 += kTargets) {
+#pragma unroll
+    for (int n = 0; n < kTargets; ++n) {
+      const int p = t * k + min(j0 + n, k - 1);
+      target[n] = min((uint32_t)a.plan.ids[p], (uint32_t)a.plan.groups) << kIndexBits | p;
     }
-    dst[tid] = absent ? -1 : r;
+    count_before(order, pairs, target, part, count);
+    const int j = j0 + tid;
+    if (tid < kTargets && j < k) {
+      const int p = t * k + j, r = count[tid];
+      const bool absent = (uint32_t)a.plan.ids[p] >= (uint32_t)a.plan.groups;
+      if (blockIdx.y == 0) {
+        a.plan.row_pair[r] = p;
+        a.plan.pair_row[p] = absent ? -1 : r;
+        if (!absent && a.row_weights) a.row_weights[r] = a.weights[p];
+      }
+      dst[j] = absent ? -1 : r;
+    }
   }
   __syncthreads();
   const U* x = (const U*)a.x + (int64_t)t * a.units;
@@ -259,7 +265,7 @@ __global__ __launch_bounds__(256) void dispatch_kernel(DispatchArgs a) {
     const U v = x[c];
     for (int j = 0; j < k; ++j) {
       const int r = __builtin_amdgcn_readfirstlane(dst[j]);
-      if (r >= 0) ((U*)a.rows)[(int64_t)r * a.units + c] = v;
+      if (r >= 0) store_once<kStream>((U*)a.rows + (int64_t)r * a.units + c, v);
     }
   }
 }
@@ -527,12 +533,14 @@ bool streams(int tokens, int k, int64_t row_bytes, int moves) {
 template <typename U>
 int launch_dispatch(DispatchArgs a, int64_t row_bytes, bool fused, hipStream_t st) {
   a.units = row_bytes / (int64_t)sizeof(U);
+  const bool stream = streams(a.tokens, a.k, row_bytes, 1);
   if (fused) {
-    const unsigned chunks = (unsigned)std::min<int64_t>((a.units + 255) / 256, 64);
-    hipLaunchKernelGGL((dispatch_kernel<U>), dim3(a.tokens + 1, chunks), dim3(256), 0, st, a);
+    // a row in pieces only where the tokens leave room: each piece's workgroup counts anew
+    const unsigned chunks = (unsigned)std::min<int64_t>((a.units + 255) / 256, std::max(1, 1024 / std::max(a.tokens, 1)));
+    const dim3 grid(a.tokens + (a.plan.groups + kTargets) / kTargets, chunks);
+    hipLaunchKernelGGL((stream ? dispatch_kernel<U, true> : dispatch_kernel<U, false>), grid, dim3(256), 0, st, a);
   } else {
     const int chunks = chunks_of(a.tokens, a.units);
-    const bool stream = streams(a.tokens, a.k, row_bytes, 1);
     hipLaunchKernelGGL((stream ? move_rows_kernel<U, true> : move_rows_kernel<U, false>), dim3(a.tokens * chunks),
                        dim3(64), 0, st, a, chunks);
   }
