@@ -383,8 +383,11 @@ __device__ __forceinline__ void combine_units(const CombineArgs& a, int t, int64
 // One wave per token and piece of 64 units (chunks pieces a row; more units, more rounds), a unit of 16 bytes (or one
 // value) a lane, up to eight rows in flight. Lane j holds the token's pair j; each counts the rows before its own and
 // sends it to the lane of that number.
+//
+// At most five waves a SIMD: 4096 x 8 rows of 7168 (529 MB read, 59 written) take 107 us with six or eight, 99 with five,
+// 101 with four and 104 with three, the unweighted sum 98 / 91 / 95 / 99.
 template <int kType, int V>
-__global__ __launch_bounds__(64) void combine_kernel(CombineArgs a, int chunks) {
+__global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(1, 5))) void combine_kernel(CombineArgs a, int chunks) {
   const int t = blockIdx.x / chunks, chunk = blockIdx.x % chunks, lane = threadIdx.x, k = a.k, pairs = a.tokens * k;
   int r = -1;
   float w = 1.f;
@@ -469,7 +472,7 @@ __device__ __forceinline__ float backward_units(const CombineBwdArgs& a, int t, 
 // A token's pairs run on one XCD (workgroups go round the eight of them), so its dy comes from HBM once and from that L2
 // after.
 template <int kType, int V>
-__global__ __launch_bounds__(256) void combine_backward_kernel(CombineBwdArgs a) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 5))) void combine_backward_kernel(CombineBwdArgs a) {
   __shared__ float part[4];
   const int tid = threadIdx.x, lane = tid & 63, k = a.k, pairs = a.tokens * k;
   const int i = blockIdx.x >> 3;
