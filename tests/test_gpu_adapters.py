@@ -69,7 +69,8 @@ def check(got, x, ids, base, adapters, exact):
 # (tokens, rows, width, slots, max_rank): either form and its border, ragged tiles, one value more than a chunk or block
 SHAPES = [(1, 8, 8, 1, 1), (1, 64, 32, 1, 16), (1, 2112, 1536, 3, 64), (2, 72, 40, 2, 7), (5, 24, 520, 8, 256),
           (31, 576, 128, 5, 17), (32, 136, 1600, 4, 33), (33, 64, 72, 3, 16), (40, 1032, 2048, 2, 32), (47, 200, 264, 8, 256), (60, 24, 104, 1, 128),
-          (64, 1024, 96, 70, 64), (65, 8, 1536, 1, 100), (100, 320, 8, 90, 8), (257, 88, 160, 6, 64),
+          (64, 1024, 96, 70, 64), (65, 8, 1536, 1, 100), (100, 320, 8, 90, 8), (127, 72, 1032, 3, 40), (128, 136, 328, 40, 16), (129, 64, 96, 5, 64),
+          (257, 88, 160, 6, 64),
           (1000, 264, 520, 8, 128)]
 
 
@@ -90,7 +91,7 @@ def test_apply(gpu_ctx, tokens, rows, width, slots, max_rank, dtype, exact):
         check(bank.apply(x, ids, base), x, ids, base, adapters, exact)
 
 
-@pytest.mark.parametrize("tokens", [4, 17, 64, 90])
+@pytest.mark.parametrize("tokens", [4, 17, 64, 90, 128, 150])
 def test_all_or_no_tokens_of_one_adapter(gpu_ctx, tokens):
     rng = np.random.default_rng(tokens)
     rows, width = 72, 136
@@ -110,7 +111,7 @@ def test_all_or_no_tokens_of_one_adapter(gpu_ctx, tokens):
         assert bank.apply(x[:0], ids[:0], base[:0]).shape == (0, rows)
 
 
-@pytest.mark.parametrize("tokens", [3, 70])
+@pytest.mark.parametrize("tokens", [3, 70, 170])
 def test_strided_rows_in_place_with_and_without_a_plan(gpu_ctx, tokens):
     """The columns of a stacked output (two projections of one input), in place; what lies beside them stays."""
     rng = np.random.default_rng(tokens)
@@ -140,7 +141,7 @@ def test_strided_rows_in_place_with_and_without_a_plan(gpu_ctx, tokens):
 def test_infinite_and_nan_inputs_stay_with_their_token(gpu_ctx):
     rng = np.random.default_rng(0)
     rows, width = 64, 64
-    for tokens in (3, 40):
+    for tokens in (3, 40, 140):
         adapters = {0: adapter(rng, rows, width, 5, True)}
         with AdapterBank(gpu_ctx, rows, width, 1, 16, tokens) as bank:
             fill(bank, rng, adapters)
@@ -160,7 +161,7 @@ def test_infinite_and_nan_inputs_stay_with_their_token(gpu_ctx):
 
 def test_slots_are_replaced_and_emptied(gpu_ctx):
     rng = np.random.default_rng(6)
-    rows, width, tokens = 40, 72, 50
+    rows, width, tokens = 40, 72, 150
     x, base = inputs(rng, tokens, rows, width, True, "f32")
     ids = rng.integers(0, 2, tokens).astype(np.int32)
     with AdapterBank(gpu_ctx, rows, width, 2, 40, tokens) as bank:
@@ -179,7 +180,7 @@ def test_the_result_does_not_depend_on_a_calls_other_tokens(gpu_ctx):
     """The same tokens in any order, with any neighbours of the same form, give the same bits."""
     rng = np.random.default_rng(14)
     rows, width = 200, 1024
-    for tokens in (20, 300):
+    for tokens in (20, 100, 300):
         with AdapterBank(gpu_ctx, rows, width, 5, 32, tokens) as bank:
             fill(bank, rng, {s: adapter(rng, rows, width, 32 - 3 * s, False) for s in range(5)})
             x, base = inputs(rng, tokens, rows, width, False, "bf16")
@@ -190,7 +191,7 @@ def test_the_result_does_not_depend_on_a_calls_other_tokens(gpu_ctx):
             np.testing.assert_array_equal(bank.apply(x, ids, base), y)
 
 
-@pytest.mark.parametrize("tokens,seed", [(6, 0), (120, 1)])
+@pytest.mark.parametrize("tokens,seed", [(6, 0), (120, 1), (200, 2)])
 def test_captured_calls_replay_on_new_inputs(tokens, seed):
     rows, width, slots = 136, 96, 3
     rng = np.random.default_rng(seed)
@@ -268,12 +269,12 @@ def test_adapters_beside_fp8_projections(block):
         with pytest.raises(ValueError):
             proj.fp8("q_a", np.zeros((2, 256), np.uint16), np.zeros(2, np.int32))   # no bank yet
         for name, (rows, width) in layout.items():
-            bank = proj.open_adapters(name, 3, 12, 64)
+            bank = proj.open_adapters(name, 3, 12, 160)
             with pytest.raises(RuntimeError):
                 proj.open_adapters(name, 3, 12)
             adapters = {s: adapter(rng, rows, width, 4 * (s + 1), False) for s in range(2)}
             fill(bank, rng, adapters)
-            for tokens in (1, 5, 50):
+            for tokens in (1, 5, 50, 150):
                 x = bf16_bits(rng.standard_normal((tokens, width)).astype(np.float32))
                 ids = rng.integers(-1, 3, tokens).astype(np.int32)
                 plain, got = proj.fp8(name, x), proj.fp8(name, x, ids)
@@ -291,9 +292,9 @@ def test_adapters_beside_fp8_projections(block):
                 with pytest.raises(ValueError):
                     proj.fp8(name, np.zeros((2, width), np.uint16), bad)
             with pytest.raises(ValueError):
-                proj.fp8(name, np.zeros((65, width), np.uint16), np.zeros(65, np.int32))
-            batched = proj.fp8(name, x.reshape(5, 10, width), ids.reshape(5, 10))["output_bf16"]
-            np.testing.assert_array_equal(batched.reshape(50, rows), got["output_bf16"])
+                proj.fp8(name, np.zeros((161, width), np.uint16), np.zeros(161, np.int32))
+            batched = proj.fp8(name, x.reshape(5, 30, width), ids.reshape(5, 30))["output_bf16"]
+            np.testing.assert_array_equal(batched.reshape(150, rows), got["output_bf16"])
         proj.banks["o"].close()
         proj.open_adapters("o", 1, 4, 8)
     assert not proj.banks and proj.ctx is None

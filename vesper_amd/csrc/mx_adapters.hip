@@ -31,7 +31,7 @@ typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 
 constexpr int kMaxTokens = 1 << 18, kMaxSlots = 1024, kMaxRank = 256;
 constexpr int kMaxWidth = 1 << 20;
-constexpr int kFewTokens = 64;     // calls of up to this many tokens need no plan: a wave holds their ids
+constexpr int kFewTokens = 128;    // a wave holds the ids of this many tokens, in two registers
 constexpr int kTileTokens = 64;    // tokens of a workgroup in the grouped form
 constexpr int kColumns = kTileTokens / 16;
 constexpr int kMaxParts = 32;      // parts of K
@@ -144,7 +144,8 @@ __device__ __forceinline__ Tile find_tile(const Call& c, int index) {
 }
 
 // Few tokens: the workgroups of token t take the tokens of t's adapter, up to 16 a workgroup. The first of each 16 does
-// it; rows = 0 for the others.
+// it; rows = 0 for the others. (Tokens are the grid's slow dimension: as its fast one, a count of them that eight divides
+// puts all the workgroups of a token on one XCD, and 64 tokens of 16 adapters take 27 us where 65 take 17.)
 struct Few {
   int slot, rows;
   int token;   // of this lane's column, lane % 16; columns past the last repeat it
@@ -152,15 +153,30 @@ struct Few {
 
 __device__ __forceinline__ Few few_tokens(const Call& c, int t) {
   const int lane = threadIdx.x & 63;
-  int id = c.ids[min(lane, c.tokens - 1)];
-  id = lane >= c.tokens ? -2 : id >= 0 && id < c.bank.slots ? id : -1;
-  const int slot = __builtin_amdgcn_readlane(id, t);
-  const uint64_t mask = __ballot(id == slot);
-  const int before = __popcll(mask & ((1ull << t) - 1)), rows = before & 15 ? 0 : min(16, (int)__popcll(mask) - before);
-  const int place = __popcll(mask & ((1ull << lane) - 1)) - before;
-  const bool mine = id == slot && place >= 0 && place < 16;
-  const int tokens = __builtin_amdgcn_ds_permute(4 * (mine ? place : 63), lane);   // lane 63 is no column's
-  return Few{slot, rows, __shfl(tokens, min(lane & 15, max(rows, 1) - 1), 64)};
+  int id[2], place[2];
+  uint64_t mask[2];   // the tokens of t's adapter, 64 tokens each
+#pragma unroll
+  for (int i = 0; i < 2; ++i) id[i] = c.ids[min(64 * i + lane, c.tokens - 1)];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    id[i] = 64 * i + lane >= c.tokens ? -2 : id[i] >= 0 && id[i] < c.bank.slots ? id[i] : -1;
+  const int slot = __builtin_amdgcn_readlane(t < 64 ? id[0] : id[1], t & 63);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) mask[i] = __ballot(id[i] == slot);
+  const int first = __popcll(mask[0]), total = first + __popcll(mask[1]);
+  const uint64_t below = (1ull << (t & 63)) - 1, under = (1ull << lane) - 1;
+  const int before = t < 64 ? __popcll(mask[0] & below) : first + __popcll(mask[1] & below);
+  const int rows = before & 15 ? 0 : min(16, total - before);
+  place[0] = __popcll(mask[0] & under) - before;
+  place[1] = first + __popcll(mask[1] & under) - before;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {   // column n's token goes to lane n; lane 63 is no column's
+    const bool mine = id[i] == slot && place[i] >= 0 && place[i] < 16;
+    id[i] = __builtin_amdgcn_ds_permute(4 * (mine ? place[i] : 63), 64 * i + lane);
+  }
+  const int column = min(lane & 15, max(rows, 1) - 1);
+  const int low = __shfl(id[0], column, 64), high = __shfl(id[1], column, 64);
+  return Few{slot, rows, before + column < first ? low : high};
 }
 
 // The tokens of the tile's 64 columns, one a lane; columns past the last repeat it.
@@ -193,7 +209,7 @@ __device__ __forceinline__ uint4 h_operand(const AdapterSlot& slot, int r0, v4f 
 
 // ---- down: partial sums of h ----
 
-// Few tokens, grid (T, parts), 4 waves: a part of K for up to 16 tokens of an adapter, RT rank tiles at a time (those past
+// Few tokens, grid (parts, T), 4 waves: a part of K for up to 16 tokens of an adapter, RT rank tiles at a time (those past
 // the last repeat it). The waves take the K units (of 64: two chunks) in turn, the next one's loads in
 // flight while one is multiplied, and their sums are added in wave order.
 template <int RT>
@@ -203,8 +219,8 @@ __device__ __forceinline__ void few_down(const Call& c, const Few& f, int r0, in
   const int tid = threadIdx.x, lane = tid & 63, q = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int units = b.chunks / 2, whole = b.k / 64;
-  const int u1 = (int)((int64_t)units * (blockIdx.y + 1) / c.parts);
-  int u = (int)((int64_t)units * blockIdx.y / c.parts) + wave;
+  const int u1 = (int)((int64_t)units * (blockIdx.x + 1) / c.parts);
+  int u = (int)((int64_t)units * blockIdx.x / c.parts) + wave;
   const uint8_t* x = (const uint8_t*)(c.x + f.token * c.x_stride) + 16 * q;
   const int64_t tile_bytes = (int64_t)b.chunks * 1024;
   const uint8_t* w = b.down + f.slot * b.down_bytes() + r0 * tile_bytes + 16 * lane;
@@ -261,7 +277,7 @@ __device__ __forceinline__ void few_down(const Call& c, const Few& f, int r0, in
   for (int r = wave; r < RT; r += 4)
     if (r0 + r < tiles && (lane & 15) < f.rows) {
       const v4f s = ((red[0][r][lane] + red[1][r][lane]) + red[2][r][lane]) + red[3][r][lane];
-      *(v4f*)(c.low + ((int64_t)blockIdx.y * c.tokens + f.token) * (16 * b.rank_tiles) + 16 * (r0 + r) + 4 * q) = s;
+      *(v4f*)(c.low + ((int64_t)blockIdx.x * c.tokens + f.token) * (16 * b.rank_tiles) + 16 * (r0 + r) + 4 * q) = s;
     }
   __syncthreads();
 }
@@ -270,7 +286,7 @@ __device__ __forceinline__ void few_down(const Call& c, const Few& f, int r0, in
 template <int RT>
 __global__ __launch_bounds__(256) void adapter_few_down_kernel(Call c) {
   __shared__ v4f red[4][RT][64];
-  const Few f = few_tokens(c, blockIdx.x);
+  const Few f = few_tokens(c, blockIdx.y);
   if (f.rows == 0 || f.slot < 0) return;
   const int tiles = (c.bank.table[f.slot].rank + 15) >> 4;
   few_down<RT>(c, f, 0, tiles, min(RT, c.bank.rank_tiles), red);
@@ -471,7 +487,7 @@ __device__ __forceinline__ void up_tile(const uint4 (&w)[2], uint4 h, v4f (&acc)
   for (int j = 0; j < 4; ++j) acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf(a[j]), as_bf(h), acc[j], 0, 0, 0);
 }
 
-// Few tokens, grid (T, output blocks / 4), 4 waves, a block of 64 outputs each for up to 16 tokens of an adapter. What does
+// Few tokens, grid (output blocks / 4, T), 4 waves, a block of 64 outputs each for up to 16 tokens of an adapter. What does
 // not depend on h is asked for before h is put together: thread (entry e, share s) adds the parts s, s + shares, ... of
 // four ranks of a token, and the shares are added in order.
 template <bool kF32>
@@ -479,12 +495,12 @@ __global__ __launch_bounds__(256) void adapter_few_up_kernel(Call c) {
   constexpr int RT = 4;   // rank tiles in registers at once
   __shared__ v4f sums[256];
   __shared__ uint4 h_lds[kMaxRank / 16 * 64];
-  const Few f = few_tokens(c, blockIdx.x);
+  const Few f = few_tokens(c, blockIdx.y);
   if (f.rows == 0) return;
   const Bank& b = c.bank;
   const int tid = threadIdx.x, lane = tid & 63, q = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int block = 4 * blockIdx.y + wave, n = 64 * block + 8 * q;   // past the last block: no output is a lane's
+  const int block = 4 * blockIdx.x + wave, n = 64 * block + 8 * q;   // past the last block: no output is a lane's
   const uint8_t* up = b.up + max(f.slot, 0) * b.up_bytes() + (int64_t)min(block, b.blocks - 1) * b.rank_tiles * 2048 + 16 * lane;
   uint4 w[RT][2];
   auto load_up = [&](int r0, int count) {
@@ -535,7 +551,7 @@ __global__ __launch_bounds__(256) void adapter_few_up_kernel(Call c) {
       *(uint4*)(c.y + f.token * c.y_stride + n + 32 * k) = eight_bf16(acc[2 * k], acc[2 * k + 1]);
 }
 
-// Few tokens in one launch, for a down that every workgroup can read for itself: grid (T, output blocks / 16), 16 waves.
+// Few tokens in one launch, for a down that every workgroup can read for itself: grid (output blocks / 16, T), 16 waves.
 // The waves take the K units of 64 in turn, two of them in flight, h is put together through LDS, and each wave finishes
 // a block of 64 outputs whose up and base were asked for at the start.
 template <int RT, bool kF32>
@@ -545,9 +561,9 @@ __global__ __launch_bounds__(1024) void adapter_few_kernel(Call c) {
   const int tid = threadIdx.x, lane = tid & 63, q = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const Bank& b = c.bank;
-  const Few f = few_tokens(c, blockIdx.x);
+  const Few f = few_tokens(c, blockIdx.y);
   if (f.rows == 0) return;
-  const int block = 16 * blockIdx.y + wave, n = 64 * block + 8 * q;
+  const int block = 16 * blockIdx.x + wave, n = 64 * block + 8 * q;
   const int units = b.chunks / 2, last = b.rank_tiles - 1;
   const int64_t tile_bytes = (int64_t)b.chunks * 1024;
   const uint8_t* x = (const uint8_t*)(c.x + f.token * c.x_stride) + 16 * q;
@@ -725,12 +741,16 @@ int tiles_of(const Bank& b, int tokens) {
   return (int)(((int64_t)tokens + (int64_t)groups * (kTileTokens - 1)) / kTileTokens);
 }
 
-// Parts of K. Few tokens: enough workgroups for the chip if the tokens' adapters differ, at least one unit of 64 a wave.
-// Grouped form: as many as are resident together (two a CU) and no more, since a few beyond would run alone after the
-// rest; at least two stages each. In both, parts T is at most kWantGroups kTileTokens + T.
+// Calls of few tokens need no plan and two launches. Up to 64 they are always the faster form, and to the 128 that a wave
+// can hold with at most 64 ranks (the output projection, 16 adapters, 100 and 128 tokens: 21.0 and 22.3 us, grouped
+// 23.0; of rank 128 37.7 and 39.2, grouped 30.8 and 31.9).
+bool is_few(const Bank& b, int tokens) { return tokens <= (b.rank_tiles <= 4 ? kFewTokens : kFewTokens / 2); }
+
+// Parts of K. Few tokens: as many as give each wave a unit of 64, since how many adapters the tokens share is not known
+// here. Grouped form: as many as are resident together (two a CU) and no more, since a few beyond would run alone after
+// the rest; at least two stages each. In both, parts T is at most kWantGroups kTileTokens + T.
 int parts_of(const Bank& b, int tokens) {
-  if (tokens <= kFewTokens)
-    return std::max(1, std::min({kMaxParts, b.chunks / 8, (2 * kWantGroups + tokens - 1) / tokens}));
+  if (is_few(b, tokens)) return std::max(1, std::min(kMaxParts, b.chunks / 8));
   return std::max(1, std::min({kMaxParts, b.k / (2 * kStageK), kWantGroups / tiles_of(b, tokens)}));
 }
 
@@ -766,7 +786,7 @@ Workspace workspace_of(const Bank& b, int32_t tokens) {
 
 template <int RT>
 int launch_fused(const Call& c, bool f32, hipStream_t st) {
-  const dim3 grid(c.tokens, (c.bank.blocks + 15) / 16);
+  const dim3 grid((c.bank.blocks + 15) / 16, c.tokens);
   hipLaunchKernelGGL((f32 ? adapter_few_kernel<RT, true> : adapter_few_kernel<RT, false>), grid, dim3(1024), 0, st, c);
   MX_LAUNCH_CHECK("adapter_few_kernel");
   return MX_OK;
@@ -779,9 +799,9 @@ int launch_few(const Call& c, bool f32, hipStream_t st) {
   hipLaunchKernelGGL((rt == 1   ? adapter_few_down_kernel<1>
                       : rt == 2 ? adapter_few_down_kernel<2>
                                 : adapter_few_down_kernel<4>),
-                     dim3(c.tokens, c.parts), dim3(256), 0, st, c);
+                     dim3(c.parts, c.tokens), dim3(256), 0, st, c);
   MX_LAUNCH_CHECK("adapter_few_down_kernel");
-  const dim3 grid(c.tokens, (c.bank.blocks + 3) / 4);
+  const dim3 grid((c.bank.blocks + 3) / 4, c.tokens);
   hipLaunchKernelGGL((f32 ? adapter_few_up_kernel<true> : adapter_few_up_kernel<false>), grid, dim3(256), 0, st, c);
   MX_LAUNCH_CHECK("adapter_few_up_kernel");
   return MX_OK;
@@ -925,7 +945,7 @@ int mx_adapters_apply(mx_adapters* a, const uint16_t* x, int64_t x_stride, const
          base, base_stride, y, y_stride, 0, false};
   if (w.low + (uint64_t)c.parts * tokens * 64 * b.rank_tiles > w.bytes)   // parts_of and workspace_of belong together
     return mxi::fail(MX_ERR_STATE, "%s: %d parts of %d tokens exceed the workspace", who, c.parts, tokens);
-  if (tokens <= kFewTokens) return launch_few(c, f32, st);
+  if (is_few(b, tokens)) return launch_few(c, f32, st);
   mx_row_plan own{(int32_t*)ws, (int32_t*)(ws + w.pair_row), (int32_t*)(ws + w.row_pair)};
   if (!plan) {
     if (int s = mxi::row_plan(ids, tokens, b.slots, own, st)) return s;
