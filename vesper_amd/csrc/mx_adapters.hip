@@ -207,6 +207,20 @@ __device__ __forceinline__ uint4 h_operand(const AdapterSlot& slot, int r0, v4f 
   return make_uint4(hi[0], hi[1], lo[0], lo[1]);
 }
 
+// The parts first, first + step, ... of four ranks added in that order, eight of them in flight.
+__device__ __forceinline__ v4f sum_parts(const float* p, int64_t stride, int first, int step, int parts) {
+  v4f sum = v4f{0.f, 0.f, 0.f, 0.f};
+  for (int n = first; n < parts; n += 8 * step) {
+    uint4 v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = ldg128((const uint8_t*)(p + min(n + i * step, parts - 1) * stride));
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (n + i * step < parts) sum = sum + __builtin_bit_cast(v4f, v[i]);
+  }
+  return sum;
+}
+
 // ---- down: partial sums of h ----
 
 // Few tokens, grid (parts, T), 4 waves: a part of K for up to 16 tokens of an adapter, RT rank tiles at a time (those past
@@ -417,11 +431,8 @@ __global__ __launch_bounds__(256) void adapter_sum_kernel(Call c) {
   const int per = 4 * b.rank_tiles;   // entries of a token
   const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (e >= (int64_t)c.tokens * per) return;
-  v4f* p = (v4f*)c.low + e;
-  const int64_t stride = (int64_t)c.tokens * per;
-  v4f s = p[0];
-#pragma unroll 8
-  for (int n = 1; n < c.parts; ++n) s = s + p[n * stride];
+  float* p = c.low + 4 * e;
+  const v4f s = sum_parts(p, (int64_t)c.tokens * 4 * per, 0, 1, c.parts);
   const int id = c.ids[e / per], r0 = 4 * (int)(e % per);
   if (id < 0 || id >= b.slots) return;   // the sums of a token without an adapter, or past a slot's rank, are no one's
   *(uint4*)p = h_operand(b.table[id], r0, s);
@@ -524,11 +535,8 @@ __global__ __launch_bounds__(256) void adapter_few_up_kernel(Call c) {
     const int column = e % f.rows, token = __shfl(f.token, column, 64);
     const bool in = e < entries && share < shares;
     v4f sum = v4f{0.f, 0.f, 0.f, 0.f};
-    if (in) {
-      const float* p = c.low + (int64_t)token * 16 * b.rank_tiles + 4 * (e / f.rows);
-#pragma unroll 8
-      for (int m = share; m < c.parts; m += shares) sum = sum + *(const v4f*)(p + m * part_stride);
-    }
+    if (in)
+      sum = sum_parts(c.low + (int64_t)token * 16 * b.rank_tiles + 4 * (e / f.rows), part_stride, share, shares, c.parts);
     if (shares > 1) {
       sums[tid] = sum;
       __syncthreads();
