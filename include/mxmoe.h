@@ -354,7 +354,7 @@ typedef struct mx_row_plan {
 /* ids [T][top_k] -> plan, and rows[pair_row[p]] = x[t] for every pair with a row, with row_weights[pair_row[p]] =
  * weights[p] (both or neither; the route_w that the expert calls take). x = rows = NULL: the plan alone. ids = NULL:
  * rows by the plan of an earlier call with the same tokens, top_k and groups (a second tensor of the same tokens).
- * The outputs overlap no input. */
+ * Here and below outputs overlap no input but where it says so. */
 int mx_dispatch(mx_ctx* ctx, const int32_t* ids, int32_t tokens, int32_t top_k, int32_t groups, const mx_row_plan* plan,
                 const void* x, int32_t dtype, int64_t width, const float* weights, void* rows, float* row_weights,
                 void* stream);

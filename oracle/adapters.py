@@ -14,9 +14,10 @@ def apply(x, ids, base, adapters):
     magnitude = |base| + |scale| |up| (|down| |x|): the sum of all the products' magnitudes."""
     x, y = np.asarray(x, np.float64), np.asarray(base, np.float64).copy()
     size = np.abs(y)
-    for t, slot in enumerate(ids):
-        if slot in adapters:
-            down, up, scale = (np.asarray(a, np.float64) for a in adapters[slot])
-            y[t] += scale * (up @ (down @ x[t]))
-            size[t] += np.abs(scale) * (np.abs(up) @ (np.abs(down) @ np.abs(x[t])))
+    ids = np.asarray(ids)
+    for slot, values in adapters.items():
+        down, up, scale = (np.asarray(a, np.float64) for a in values)
+        own = np.flatnonzero(ids == slot)
+        y[own] += scale * (x[own] @ down.T @ up.T)
+        size[own] += np.abs(scale) * (np.abs(x[own]) @ np.abs(down).T @ np.abs(up).T)
     return y, size

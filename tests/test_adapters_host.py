@@ -120,3 +120,15 @@ def test_apply_refusals(bank):
     for call in (lambda: bank.apply(x, ids, base), lambda: bank.apply_device(A, A, 3, A, A), lambda: bank.clear(0)):
         with pytest.raises(RuntimeError):
             call()
+
+
+def test_a_closed_context_has_taken_the_bank(bank):
+    """No call hands the library a bank whose context is gone."""
+    def closed():
+        raise RuntimeError("device context is closed")
+    bank.ctx._h = closed
+    for call in (lambda: bank.apply_device(A, A, 3, A, A), lambda: bank.load_device(0, A, A, 8), lambda: bank.clear(0),
+                 bank.close):
+        with pytest.raises(RuntimeError):
+            call()
+    assert not bank.ctx.lib.calls

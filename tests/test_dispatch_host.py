@@ -50,7 +50,7 @@ def test_gradients_of_the_oracle_against_differences():
             assert abs((up - down) / (2 * step) - grad[index]) < 1e-7
 
 
-A = 0x10000   # addresses that no check follows
+A, B = 0x10000, 0x20000   # addresses that no check follows
 
 
 def plan_at(first=A, pair_row=A, row_pair=A):
@@ -74,7 +74,7 @@ def dispatch_args(**changed):
     {"plan": plan_at(row_pair=A + 2)}, {"x": None}, {"rows": None}, {"ids": None, "x": None, "rows": None},
     {"weights": A}, {"row_weights": A}, {"x": None, "rows": None, "weights": A, "row_weights": A},
     {"dtype": 3}, {"dtype": -1}, {"width": 0}, {"width": -5}, {"width": (1 << 24) + 1}, {"x": A + 1},
-    {"rows": A + 1}, {"dtype": 1, "x": A + 2}, {"ids": A + 2}, {"weights": A + 1, "row_weights": A},
+    {"rows": A + 1}, {"rows": A}, {"dtype": 1, "x": A + 2}, {"ids": A + 2}, {"weights": A + 1, "row_weights": A},
 ])
 def test_dispatch_refusals(changed):
     assert status("dispatch", *dispatch_args(**changed)) == _lib.MX_ERR_INVALID
@@ -85,34 +85,41 @@ def test_valid_arguments_reach_the_context_check():
     for changed in ({}, {"tokens": 0}, {"x": None, "rows": None}, {"ids": None}, {"dtype": 2, "x": A + 1},
                     {"weights": A, "row_weights": A}):
         assert status("dispatch", *dispatch_args(**changed)) == _lib.MX_ERR_STATE
-    assert status("combine", None, A, 0, A, None, None, 4, 2, 64, A, None) == _lib.MX_ERR_STATE
-    assert status("combine_backward", None, A, A, 0, A, None, 4, 2, 64, A, A, None) == _lib.MX_ERR_STATE
-    assert status("dispatch_backward", None, A, 0, A, None, 4, 2, 64, A, None, None) == _lib.MX_ERR_STATE
+    assert status("combine", None, A, 0, A, None, 2 * A, 4, 2, 64, 2 * A, None) == _lib.MX_ERR_STATE
+    assert status("combine_backward", None, 2 * A, A, 0, A, None, 4, 2, 64, A, A, None) == _lib.MX_ERR_STATE
+    assert status("dispatch_backward", None, A, 0, A, None, 4, 2, 64, 2 * A, None, None) == _lib.MX_ERR_STATE
+
+
+def test_outputs_that_are_an_input_are_refused():
+    """Rows change places between these: what is read would be another row's result."""
+    assert status("combine", None, A, 0, A, None, None, 4, 2, 64, A, None) == _lib.MX_ERR_INVALID
+    assert status("combine_backward", None, A, 2 * A, 0, A, None, 4, 1, 64, A, A, None) == _lib.MX_ERR_INVALID
+    assert status("dispatch_backward", None, A, 0, A, None, 4, 2, 64, A, None, None) == _lib.MX_ERR_INVALID
 
 
 @pytest.mark.parametrize("args", [
-    (None, 0, A, None, None, 4, 2, 64, A), (A, 0, None, None, None, 4, 2, 64, A), (A, 0, A, None, None, 4, 2, 64, None),
-    (A, 2, A, None, None, 4, 2, 64, A), (A, 0, A, None, None, -1, 2, 64, A), (A, 0, A, None, None, 4, 40, 64, A),
-    (A, 0, A, None, None, 4, 2, 0, A), (A + 1, 0, A, None, None, 4, 2, 64, A), (A, 1, A, None, A + 2, 4, 2, 64, A),
-    (A, 0, A + 2, None, None, 4, 2, 64, A), (A, 0, A, A + 1, None, 4, 2, 64, A),
+    (None, 0, A, None, None, 4, 2, 64, B), (A, 0, None, None, None, 4, 2, 64, B), (A, 0, A, None, None, 4, 2, 64, None),
+    (A, 2, A, None, None, 4, 2, 64, B), (A, 0, A, None, None, -1, 2, 64, B), (A, 0, A, None, None, 4, 40, 64, B),
+    (A, 0, A, None, None, 4, 2, 0, B), (A + 1, 0, A, None, None, 4, 2, 64, B), (A, 1, A, None, A + 2, 4, 2, 64, B),
+    (A, 0, A + 2, None, None, 4, 2, 64, B), (A, 0, A, A + 1, None, 4, 2, 64, B),
 ])
 def test_combine_refusals(args):
     assert status("combine", None, *args, None) == _lib.MX_ERR_INVALID
 
 
 @pytest.mark.parametrize("args", [
-    (None, A, 0, A, None, 4, 2, 64, A, A), (A, None, 0, A, None, 4, 2, 64, A, A), (A, A, 0, None, None, 4, 2, 64, A, A),
-    (A, A, 0, A, None, 4, 2, 64, None, None), (A, A, 2, A, None, 4, 2, 64, A, A), (A, A, 0, A, None, 4, 0, 64, A, A),
-    (A, A, 0, A, None, 4, 2, -1, A, A), (A, A, 1, A, None, 4, 2, 64, A + 2, A), (A, A, 0, A, None, 4, 2, 64, A, A + 2),
+    (None, A, 0, A, None, 4, 2, 64, B, A), (A, None, 0, A, None, 4, 2, 64, B, A), (A, A, 0, None, None, 4, 2, 64, B, A),
+    (A, A, 0, A, None, 4, 2, 64, None, None), (A, A, 2, A, None, 4, 2, 64, B, A), (A, A, 0, A, None, 4, 0, 64, B, A),
+    (A, A, 0, A, None, 4, 2, -1, B, A), (A, A, 1, A, None, 4, 2, 64, A + 2, A), (A, A, 0, A, None, 4, 2, 64, B, A + 2),
 ])
 def test_combine_backward_refusals(args):
     assert status("combine_backward", None, *args, None) == _lib.MX_ERR_INVALID
 
 
 @pytest.mark.parametrize("args", [
-    (None, 0, A, None, 4, 2, 64, A, None), (A, 0, None, None, 4, 2, 64, A, None), (A, 0, A, None, 4, 2, 64, None, None),
-    (A, 0, A, A, 4, 2, 64, A, None), (A, 0, A, None, 4, 2, 64, A, A), (A, 2, A, None, 4, 2, 64, A, None),
-    (A, 0, A, None, 1 << 20, 2, 64, A, None), (A + 1, 0, A, None, 4, 2, 64, A, None),
+    (None, 0, A, None, 4, 2, 64, B, None), (A, 0, None, None, 4, 2, 64, B, None), (A, 0, A, None, 4, 2, 64, None, None),
+    (A, 0, A, A, 4, 2, 64, B, None), (A, 0, A, None, 4, 2, 64, B, A), (A, 2, A, None, 4, 2, 64, B, None),
+    (A, 0, A, None, 1 << 20, 2, 64, B, None), (A + 1, 0, A, None, 4, 2, 64, B, None),
 ])
 def test_dispatch_backward_refusals(args):
     assert status("dispatch_backward", None, *args, None) == _lib.MX_ERR_INVALID

@@ -217,6 +217,85 @@ def test_captured_calls_replay_on_new_inputs(tokens, seed):
         ctx.destroy_stream(stream)
 
 
+@pytest.mark.parametrize("tokens", [100, 300])
+def test_rows_past_32_bits(gpu_ctx, tokens):
+    """Strides that put the last rows more than 2^31 values (and for the grouped form 2^32) from the first."""
+    rng = np.random.default_rng(tokens)
+    rows, width, stride = 72, 104, 1 << 25
+    adapters = {s: adapter(rng, rows, width, 9 + s, True) for s in range(2)}
+    ids = rng.integers(-1, 2, tokens).astype(np.int32)
+    x, base = inputs(rng, tokens, rows, width, True, "bf16")
+    with AdapterBank(gpu_ctx, rows, width, 2, 16, tokens) as bank:
+        fill(bank, rng, adapters)
+        at = gpu_ctx.malloc(2 * stride * tokens)   # a row's x, and 256 bytes on its base, which y replaces
+        idd = gpu_ctx.upload(ids)
+        for t in range(tokens):
+            gpu_ctx.copy_h2d(at + 2 * stride * t, x[t])
+            gpu_ctx.copy_h2d(at + 2 * stride * t + 256, base[t])
+        bank.apply_device(at, idd, tokens, at + 256, at + 256, x_stride=stride, base_stride=stride, y_stride=stride)
+        got = np.stack([gpu_ctx.download(at + 2 * stride * t + 256, (rows,), np.uint16) for t in range(tokens)])
+        check(got, x, ids, base, adapters, True)
+        idd.free()
+        gpu_ctx.free(at)
+
+
+def test_calls_larger_than_the_caches(gpu_ctx):
+    """x and y of more than 96 MiB; 1600 of the columns of x are not zero, which keeps every sum exact."""
+    rng = np.random.default_rng(9)
+    tokens, rows, width, slots = 7100, 3592, 7176, 3
+    adapters = {s: adapter(rng, rows, width, 16 - 5 * s, True) for s in range(slots)}
+    ids = rng.integers(-1, slots, tokens).astype(np.int32)
+    x, base = inputs(rng, tokens, rows, width, True, "bf16")
+    x[:, rng.permutation(width)[1600:]] = 0
+    with AdapterBank(gpu_ctx, rows, width, slots, 16, tokens) as bank:
+        fill(bank, rng, adapters)
+        check(bank.apply(x, ids, base), x, ids, base, adapters, True)
+
+
+def test_two_banks_on_two_streams_by_one_plan(gpu_ctx):
+    """A step's projections side by side: a bank and a stream each, the plan of the step's ids for both."""
+    rng = np.random.default_rng(5)
+    tokens, width, slots = 700, 264, 5
+    ids = rng.integers(-1, slots, tokens).astype(np.int32)
+    streams = [gpu_ctx.stream() for _ in range(2)]
+    with ExpertDispatch(gpu_ctx, slots, 1, tokens) as d:
+        idd, sides = gpu_ctx.upload(ids), []
+        d.plan_device(idd, tokens)
+        for rows, on in zip((200, 1032), streams):
+            bank = AdapterBank(gpu_ctx, rows, width, slots, 32, tokens)
+            adapters = {s: adapter(rng, rows, width, 32 - 5 * s, True) for s in range(slots)}
+            fill(bank, rng, adapters)
+            x, base = inputs(rng, tokens, rows, width, True, "f32")
+            dev = [gpu_ctx.upload(a) for a in (x, base, np.zeros((tokens, rows), np.uint16))]
+            sides.append((bank, adapters, x, base, dev, on))
+        gpu_ctx.sync()
+        for _ in range(5):
+            for bank, _, _, _, (xd, bd, yd), on in sides:
+                bank.apply_device(xd, idd, tokens, bd, yd, "f32", plan=d.plan, stream=on)
+        gpu_ctx.sync()
+        for bank, adapters, x, base, dev, on in sides:
+            check(dev[2].download(), x, ids, base, adapters, True)
+            for a in dev:
+                a.free()
+            bank.close()
+            gpu_ctx.destroy_stream(on)
+        idd.free()
+
+
+def test_most_slots(gpu_ctx):
+    """1024 slots of which the last is used, by many tokens and by few; tiles of two tokens each."""
+    rng = np.random.default_rng(8)
+    rows, width, slots = 40, 72, 1024
+    with AdapterBank(gpu_ctx, rows, width, slots, 4, 2100) as bank:
+        adapters = {s: adapter(rng, rows, width, 4, True) for s in range(0, slots, 31)}
+        fill(bank, rng, adapters)
+        for tokens in (20, 2100):
+            ids = (np.arange(tokens) % slots).astype(np.int32)
+            ids[::3] = slots - 1
+            x, base = inputs(rng, tokens, rows, width, True, "bf16")
+            check(bank.apply(x, ids, base), x, ids, base, adapters, True)
+
+
 def test_call_refusals(gpu_ctx):
     rows, width, tokens = 64, 32, 4
     with AdapterBank(gpu_ctx, rows, width, 2, 8, tokens) as bank:
@@ -229,11 +308,13 @@ def test_call_refusals(gpu_ctx):
                         {"base_stride": rows - 8}, {"base_stride": rows + 4}, {"base_type": 1, "base_stride": rows + 2},
                         {"y_stride": rows + 4}, {"y_stride": 8}, {"x": a + 8}, {"base": a + 8}, {"y": a + 2},
                         {"ids": a + 2}, {"workspace": bank.workspace + 16}, {"workspace_bytes": bank.workspace_bytes - 1},
-                        {"y": 2 * a, "y_stride": rows + 8}, {"y": 2 * a, "base_type": 1}, {"x_stride": 1 << 32},
+                        {"y": a}, {"y": 2 * a, "y_stride": rows + 8}, {"y": 2 * a, "base_type": 1}, {"x_stride": 1 << 32},
                         {"plan": C.byref(plan(None, a, a))}, {"plan": C.byref(plan(a, a, None))},
                         {"plan": C.byref(plan(a + 2, a, a))}):
             args = dict(good, **changed)
             assert gpu_ctx.lib.cdll.mx_adapters_apply(bank.handle, *args.values(), None) == _lib.MX_ERR_INVALID, changed
+        with pytest.raises(ValueError):   # a stride of zero is no default
+            bank.apply_device(a, a, tokens, 2 * a, 3 * a, x_stride=0)
         for args in ((2, a, a, 8), (-1, a, a, 8), (0, a, a, 9), (0, a, a, -1), (0, None, a, 8), (0, a, None, 8),
                      (0, a + 1, a, 8)):
             assert gpu_ctx.lib.cdll.mx_adapters_load(bank.handle, *args, 1.0, None) == _lib.MX_ERR_INVALID, args

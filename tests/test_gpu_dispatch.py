@@ -399,3 +399,88 @@ def test_two_dispatches_on_two_streams(gpu_ctx):
             a.free()
     for on in streams:
         gpu_ctx.destroy_stream(on)
+
+
+def test_rows_past_32_bits(gpu_ctx):
+    """More than 2^31 values in the rows: the first and last tokens' are the ones looked at."""
+    rng = np.random.default_rng(6)
+    t, k, width = 600, 2, 1 << 21
+    ids = np.stack([np.arange(t) % 7, 7 + np.arange(t) % 5], 1).astype(np.int32)   # two groups each, all held
+    w = rng.uniform(0.5, 1, (t, k)).astype(np.float32)
+    looked = (0, 1, t // 2, t - 2, t - 1)
+    xs = {i: make_rows(rng, 1, width, "bf16")[0] for i in looked}
+    first, pair_row, row_pair = oracle.plan(ids, 12)
+    assert int(pair_row.max()) * width > 1 << 31
+    with ExpertDispatch(gpu_ctx, 12, k, t) as d:
+        row = 2 * width
+        xd, yd, rd = gpu_ctx.malloc(t * row), gpu_ctx.malloc(t * row), gpu_ctx.malloc(t * k * row)
+        idd, wd, dwd = gpu_ctx.upload(ids), gpu_ctx.upload(w), gpu_ctx.upload(np.zeros((t, k), np.float32))
+        for i, x in xs.items():
+            gpu_ctx.copy_h2d(xd + i * row, x)
+        d.dispatch_device(idd, t, xd, width, rd)
+        for i, x in xs.items():
+            for j in range(k):
+                np.testing.assert_array_equal(gpu_ctx.download(rd + int(pair_row[i, j]) * row, (width,), np.uint16), x)
+        d.combine_device(rd, width, yd, weights_ptr=wd)
+        for i, x in xs.items():
+            want = np.stack([np.float64(w[i, j]) * values(x) for j in range(k)])
+            check(gpu_ctx.download(yd + i * row, (width,), np.uint16), want.sum(0), np.abs(want).sum(0), k + 1, "bf16")
+        d.combine_backward_device(xd, rd, width, rd, dwd, weights_ptr=wd)
+        dw = dwd.download()
+        for i, x in xs.items():
+            v = values(x).astype(np.float64)
+            for j in range(k):
+                got = gpu_ctx.download(rd + int(pair_row[i, j]) * row, (width,), np.uint16)
+                check(got, w[i, j] * v, np.abs(w[i, j] * v), 1, "bf16")
+                assert abs(dw[i, j] - v @ v) <= (width / 256 + 32 + 10) * U * (v @ v)
+        d.dispatch_backward_device(rd, width, yd)
+        for i in xs:
+            terms = [values(gpu_ctx.download(rd + int(r) * row, (width,), np.uint16)).astype(np.float64) for r in pair_row[i]]
+            check(gpu_ctx.download(yd + i * row, (width,), np.uint16), sum(terms), sum(map(np.abs, terms)), k, "bf16")
+        for a in (idd, wd, dwd):
+            a.free()
+        for p in (xd, yd, rd):
+            gpu_ctx.free(p)
+
+
+def test_most_pairs(gpu_ctx):
+    """The largest routing: 2^18 tokens of 32 of 1024 experts, rows of one byte."""
+    rng = np.random.default_rng(7)
+    t, k, e = 1 << 18, 32, 1024
+    ids, x = routing(rng, t, k, e), make_rows(rng, t, 1, "u8")
+    key = np.where((ids >= 0) & (ids < e), ids, e).reshape(-1)
+    row_pair = np.argsort(key, kind="stable")
+    first = np.searchsorted(key[row_pair], np.arange(e + 1))
+    pair_row = np.full(t * k, -1)
+    pair_row[row_pair[:first[e]]] = np.arange(first[e])
+    with ExpertDispatch(gpu_ctx, e, k, t) as d:
+        out = d.dispatch(ids, x)
+    for name, want in (("first", first), ("pair_row", pair_row.reshape(t, k)), ("row_pair", row_pair)):
+        np.testing.assert_array_equal(out[name], want)
+    np.testing.assert_array_equal(out["rows"][:first[-1]], x[row_pair[:first[-1]] // k])
+
+
+@pytest.mark.parametrize("dtype,width", [("bf16", 7168), ("f32", 3584), ("bf16", 7161)])
+def test_calls_larger_than_the_caches(gpu_ctx, dtype, width):
+    """Calls that move more than 96 MiB take their rows past the caches; tokens with all their pairs and without some."""
+    rng = np.random.default_rng(width)
+    t, k, e = 900, 8, 64
+    ids = routing(rng, t, k, e, absent=False)
+    ids[::5] = routing(rng, len(ids[::5]), k, e)
+    x, w = make_rows(rng, t, width, dtype), rng.standard_normal((t, k)).astype(np.float32)
+    with ExpertDispatch(gpu_ctx, e, k, t) as d:
+        out = d.dispatch(ids, x)
+        first, pair_row, row_pair = oracle.plan(ids, e)
+        np.testing.assert_array_equal(out["rows"][:first[-1]], x[row_pair[:first[-1]] // k])
+        rows = make_rows(rng, t * k, width, dtype)
+        want, size = oracle.combine(values(rows), pair_row, w, values(x))
+        check(d.combine(rows, w, x), want, size, k + 2, dtype)
+        got = d.combine_backward(x, rows, w)
+        v, held = values(x).astype(np.float64), pair_row >= 0
+        want = w.reshape(-1, 1)[row_pair[:first[-1]]] * v[row_pair[:first[-1]] // k]
+        check(got["drows"][:first[-1]], want, np.abs(want), 1, dtype)
+        r = values(rows).astype(np.float64)[np.where(held, pair_row, 0)]   # [T, k, width]
+        dot, size = np.einsum("tjw,tw->tj", r, v), np.einsum("tjw,tw->tj", np.abs(r), np.abs(v))
+        assert np.all(np.abs(got["dweights"] - np.where(held, dot, 0)) <= np.where(held, (width / 256 + 42) * U * size, 0))
+        want, size = oracle.combine(values(rows), pair_row)
+        check(d.dispatch_backward(rows)["dx"], want, size, k, dtype)

@@ -50,6 +50,7 @@ class AdapterBank:
 
     def close(self):
         if self.handle:
+            self.ctx._h()   # a closed context has taken the bank with it
             handle, self.handle = self.handle, C.c_void_p()
             self.ctx.lib.adapters_destroy(handle)
         if self.workspace:
@@ -65,6 +66,7 @@ class AdapterBank:
     def _open(self):
         if not self.handle:
             raise RuntimeError("the adapter bank is closed")
+        self.ctx._h()
 
     def _slot(self, slot, rank, scale):
         self._open()
@@ -114,10 +116,13 @@ class AdapterBank:
         if base_dtype not in ("bf16", "f32"):
             raise ValueError("base type must be bf16 or f32")
         ptr = _lib.ptr
-        self.ctx.lib.adapters_apply(self.handle, ptr(x_ptr), x_stride or self.width, ptr(ids_ptr),
+        x_stride = self.width if x_stride is None else x_stride
+        base_stride = self.rows if base_stride is None else base_stride
+        y_stride = self.rows if y_stride is None else y_stride
+        self.ctx.lib.adapters_apply(self.handle, ptr(x_ptr), x_stride, ptr(ids_ptr),
                                     None if plan is None else C.byref(plan), tokens, ptr(base_ptr),
-                                    _lib.MX_ROWS[base_dtype], base_stride or self.rows, ptr(y_ptr),
-                                    y_stride or self.rows, self.workspace, self.workspace_bytes, stream)
+                                    _lib.MX_ROWS[base_dtype], base_stride, ptr(y_ptr), y_stride, self.workspace,
+                                    self.workspace_bytes, None if stream is None else int(stream))
 
     def check_ids(self, ids, tokens: int) -> np.ndarray:
         """Host slot ids [tokens] as int32: each a slot of the bank, or -1 for none."""

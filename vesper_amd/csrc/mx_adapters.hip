@@ -938,6 +938,7 @@ int mx_adapters_apply(mx_adapters* a, const uint16_t* x, int64_t x_stride, const
              "%s: x, base and y must be 16-byte and ids 4-byte aligned", who);
   MX_REQUIRE((const void*)y != base || (!f32 && y_stride == base_stride),
              "%s: y may be base only with the same type and stride", who);
+  MX_REQUIRE(y != x, "%s: y may not be x", who);
   const Workspace w = workspace_of(b, tokens);
   MX_REQUIRE(is_aligned(workspace, 256) && workspace_bytes >= w.bytes,
              "%s: workspace must be 256-byte aligned and hold %llu bytes", who, (unsigned long long)w.bytes);

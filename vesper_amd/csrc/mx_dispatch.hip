@@ -36,11 +36,6 @@ struct PlanArgs {
   int32_t* row_pair;
 };
 
-__device__ __forceinline__ int pair_key(const PlanArgs& a, int p) {
-  const int id = a.ids[p];
-  return id >= 0 && id < a.groups ? id : a.groups;
-}
-
 // Workgroup g places the pairs of key g (kAbsent: g = G, the pairs without a group). Each wave takes a contiguous section
 // of the pairs, 64 at a time: every lane counts the smaller keys and its own key among its pairs (as unsigned numbers,
 // ids below zero are no smaller key; pairs past the section count as ids past the last), and the second walk places the
@@ -614,6 +609,7 @@ int mx_dispatch(mx_ctx* ctx, const int32_t* ids, int32_t tokens, int32_t top_k, 
     if (int s = check_rows(who, dtype, width, true)) return s;
     MX_REQUIRE(is_aligned(x, element_bytes(dtype)) && is_aligned(rows, element_bytes(dtype)),
                "%s: x and rows must be aligned to their elements", who);
+    MX_REQUIRE(rows != x, "%s: rows may not be x", who);
   }
   if (int s = use(ctx)) return s;
   hipStream_t st = as_stream(stream);
@@ -642,6 +638,7 @@ int mx_combine(mx_ctx* ctx, const void* rows, int32_t dtype, const int32_t* pair
   MX_REQUIRE(is_aligned(rows, size) && is_aligned(y, size) && is_aligned(shared, size) && is_aligned(pair_row, 4) &&
                  is_aligned(weights, 4),
              "%s: pointers must be aligned to their elements", who);
+  MX_REQUIRE(y != rows, "%s: y may not be rows", who);
   if (int s = use(ctx)) return s;
   if (!tokens) return MX_OK;
   const CombineArgs a{rows, pair_row, weights, shared, y, tokens, top_k, 0, nullptr, nullptr, false};
@@ -661,6 +658,7 @@ int mx_combine_backward(mx_ctx* ctx, const void* dy, const void* rows, int32_t d
   MX_REQUIRE(is_aligned(dy, size) && is_aligned(rows, size) && is_aligned(drows, size) && is_aligned(pair_row, 4) &&
                  is_aligned(weights, 4) && is_aligned(dweights, 4),
              "%s: pointers must be aligned to their elements", who);
+  MX_REQUIRE(drows != dy, "%s: drows may not be dy", who);
   if (int s = use(ctx)) return s;
   if (!tokens) return MX_OK;
   const CombineBwdArgs a{dy, rows, pair_row, weights, drows, dweights, tokens, top_k, 0, false};
@@ -687,6 +685,7 @@ int mx_dispatch_backward(mx_ctx* ctx, const void* drows, int32_t dtype, const in
   MX_REQUIRE(is_aligned(drows, size) && is_aligned(dx, size) && is_aligned(pair_row, 4) &&
                  is_aligned(drow_weights, 4) && is_aligned(dweights, 4),
              "%s: pointers must be aligned to their elements", who);
+  MX_REQUIRE(dx != drows, "%s: dx may not be drows", who);
   if (int s = use(ctx)) return s;
   if (!tokens) return MX_OK;
   const CombineArgs a{drows, pair_row, nullptr, nullptr, dx, tokens, top_k, 0, drow_weights, dweights, false};
