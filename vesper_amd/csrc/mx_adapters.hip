@@ -89,13 +89,19 @@ __global__ __launch_bounds__(128) void adapter_store_up_kernel(Bank b, uint8_t* 
 
 // ---- the tokens of a workgroup ----
 
+struct Tile {
+  int slot, rows;   // slot -1: tokens without an adapter; rows 0: no tile of this number
+};
+
 struct Call {
   Bank bank;
   const uint16_t* x;
   int64_t x_stride;
   const int32_t* ids;
-  const int32_t* first;      // grouped form: the plan of ids (slots groups)
+  const int32_t* first;      // grouped form: the plan of ids (slots groups), or null: every workgroup counts for itself
   const int32_t* row_pair;
+  Tile* tile;                // grouped form: what down found, for up: the tiles
+  int32_t* tile_token;       // and the tokens of their 64 columns
   int32_t tokens, parts;
   float* low;                // [parts][T][16 rank_tiles]: partial sums of down x
   const void* base;
@@ -106,24 +112,20 @@ struct Call {
   bool stream;               // grouped form: y is written past the caches
 };
 
-struct Tile {
-  int slot;        // -1: tokens without an adapter
-  int row, rows;   // sorted rows
+// Which of the groups' tiles is number `index`: kTileTokens tokens of a group each (a group's last one short), the tokens
+// without an adapter last as group `slots`. count(g) gives the tokens of a group; 64 groups at a time.
+struct Place {
+  int group, skip, rows;   // rows = 0 past the last tile; else tokens kTileTokens skip .. of the group
 };
 
-// Tile `index` of the plan's groups, kTileTokens sorted rows each (a group's last one short), the tokens without an
-// adapter last; rows = 0 past the end. Every wave searches for itself, 64 groups at a time.
-__device__ __forceinline__ Tile find_tile(const Call& c, int index) {
-  const int lane = threadIdx.x & 63, slots = c.bank.slots;
+template <typename Count>
+__device__ __forceinline__ Place find_tile(int slots, int index, Count count) {
+  const int lane = threadIdx.x & 63;
   int before = 0;
-  Tile t{-1, 0, 0};
+  Place t{0, 0, 0};
   for (int g0 = 0; g0 <= slots; g0 += 64) {
-    const int g = g0 + lane;
-    int lo = c.first[min(g, slots)], hi = c.first[min(g + 1, slots)];
-    lo = g <= slots ? min(max(lo, 0), c.tokens) : c.tokens;
-    hi = g < slots ? min(max(hi, lo), c.tokens) : c.tokens;
-    const int count = (hi - lo + kTileTokens - 1) / kTileTokens;
-    int upto = count;
+    const int n = g0 + lane <= slots ? count(g0 + lane) : 0, tiles = (n + kTileTokens - 1) / kTileTokens;
+    int upto = tiles;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
       const int o = __shfl_up(upto, d, 64);
@@ -132,15 +134,86 @@ __device__ __forceinline__ Tile find_tile(const Call& c, int index) {
     const int total = __shfl(upto, 63, 64);
     if (index < before + total) {
       const int at = __ffsll((unsigned long long)__ballot(upto > index - before)) - 1;
-      const int skip = index - before - (__shfl(upto, at, 64) - __shfl(count, at, 64));
-      const int l = __shfl(lo, at, 64) + skip * kTileTokens, h = __shfl(hi, at, 64);
-      t = Tile{g0 + at < slots ? g0 + at : -1, l, min(kTileTokens, h - l)};
+      const int skip = index - before - (__shfl(upto, at, 64) - __shfl(tiles, at, 64));
+      t = Place{g0 + at, skip, min(kTileTokens, __shfl(n, at, 64) - skip * kTileTokens)};
       break;
     }
     before += total;
   }
-  return Tile{__builtin_amdgcn_readfirstlane(t.slot), __builtin_amdgcn_readfirstlane(t.row),
-              __builtin_amdgcn_readfirstlane(t.rows)};
+  return Place{__builtin_amdgcn_readfirstlane(t.group), __builtin_amdgcn_readfirstlane(t.skip),
+               __builtin_amdgcn_readfirstlane(t.rows)};
+}
+
+// Tile `index` by the plan of ids; `token` is that of this lane's column (those past the last repeat it).
+__device__ __forceinline__ Tile plan_tile(const Call& c, int index, int& token) {
+  const int slots = c.bank.slots;
+  auto begin = [&](int g) { return min(max(c.first[g], 0), c.tokens); };
+  const Place t = find_tile(slots, index, [&](int g) {
+    const int lo = begin(g);
+    return (g < slots ? max(begin(g + 1), lo) : c.tokens) - lo;
+  });
+  if (t.rows > 0) {
+    const int row = begin(t.group) + t.skip * kTileTokens + min((int)(threadIdx.x & 63), t.rows - 1);
+    token = c.row_pair[min(row, c.tokens - 1)];
+    token = token >= 0 && token < c.tokens ? token : 0;
+  }
+  return Tile{t.group < slots ? t.group : -1, t.rows};
+}
+
+// The same from the ids themselves, by a workgroup of four waves for itself: it counts the groups in `lds`, finds its
+// tile and picks out the tile's tokens in ascending order. The waves hold the ids, a contiguous section each.
+constexpr int kOwnIds = 16, kOwnTokens = 4 * 64 * kOwnIds;
+constexpr int kCopies = 8;   // of each count, by lane: neighbours of one group take few turns at one of them
+constexpr int kOwnLds = (kMaxSlots + 1) * kCopies + 4 + kTileTokens;   // numbers
+
+__device__ __forceinline__ Tile own_tile(const Call& c, int index, int* lds, int& token) {
+  const int tid = threadIdx.x, lane = tid & 63, slots = c.bank.slots;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  int* count = lds;
+  int* part = lds + (kMaxSlots + 1) * kCopies;
+  int* list = part + 4;
+  const int section = (c.tokens + 255) / 256 * 64, p0 = wave * section + lane;
+  int id[kOwnIds];   // -1: past the last token; tokens without an adapter are group `slots`
+#pragma unroll
+  for (int i = 0; i < kOwnIds; ++i)
+    if (64 * i < section) id[i] = c.ids[min(p0 + 64 * i, c.tokens - 1)];
+  for (int n = tid; n < (slots + 1) * (kCopies / 4); n += 256) ((uint4*)count)[n] = make_uint4(0, 0, 0, 0);
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kOwnIds; ++i)
+    if (64 * i < section) {
+      id[i] = p0 + 64 * i >= c.tokens ? -1 : id[i] >= 0 && id[i] < slots ? id[i] : slots;
+      if (id[i] >= 0) atomicAdd(&count[id[i] * kCopies + lane % kCopies], 1);
+    }
+  __syncthreads();
+  const Place t = find_tile(slots, index, [&](int g) {
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < kCopies; ++i) n += count[g * kCopies + i];
+    return n;
+  });
+  if (t.rows > 0) {
+    int own = 0;
+#pragma unroll
+    for (int i = 0; i < kOwnIds; ++i)
+      if (64 * i < section) own += __popcll(__ballot(id[i] == t.group));
+    if (lane == 0) part[wave] = own;
+    __syncthreads();
+    int at = -t.skip * kTileTokens;
+    for (int w = 0; w < wave; ++w) at += part[w];
+#pragma unroll
+    for (int i = 0; i < kOwnIds; ++i)
+      if (64 * i < section) {
+        const uint64_t mask = __ballot(id[i] == t.group);
+        const int place = at + __popcll(mask & ((1ull << lane) - 1));
+        if (id[i] == t.group && place >= 0 && place < kTileTokens) list[place] = p0 + 64 * i;
+        at += __popcll(mask);
+      }
+    __syncthreads();
+    token = list[min(lane, t.rows - 1)];
+    __syncthreads();
+  }
+  return Tile{t.group < slots ? t.group : -1, t.rows};
 }
 
 // Few tokens: the workgroups of token t take the tokens of t's adapter, up to 16 a workgroup. The first of each 16 does
@@ -177,12 +250,6 @@ __device__ __forceinline__ Few few_tokens(const Call& c, int t) {
   const int column = min(lane & 15, max(rows, 1) - 1);
   const int low = __shfl(id[0], column, 64), high = __shfl(id[1], column, 64);
   return Few{slot, rows, before + column < first ? low : high};
-}
-
-// The tokens of the tile's 64 columns, one a lane; columns past the last repeat it.
-__device__ __forceinline__ int tile_tokens(const Call& c, const Tile& t) {
-  const int p = c.row_pair[t.row + min((int)(threadIdx.x & 63), t.rows - 1)];
-  return p >= 0 && p < c.tokens ? p : 0;
 }
 
 // Workgroups go round the eight XCDs; this numbers them so that each XCD takes a contiguous range of `count`.
@@ -320,9 +387,14 @@ __global__ __launch_bounds__(256, 2) void adapter_down_kernel(Call c, int rank_g
   extern __shared__ uint4 stage_lds[];   // two stages; then the waves' sums [4][kColumns][RT][64]
   const Bank& b = c.bank;
   const int work = on_xcd(blockIdx.x, c.parts * c.tiles * rank_groups);
-  const int part = work / (c.tiles * rank_groups), r0 = RT * (work % rank_groups);
+  const int part = work / (c.tiles * rank_groups), r0 = RT * (work % rank_groups), index = work / rank_groups % c.tiles;
   if (part >= c.parts) return;
-  const Tile t = find_tile(c, work / rank_groups % c.tiles);
+  int tokens = 0;
+  const Tile t = c.first ? plan_tile(c, index, tokens) : own_tile(c, index, (int*)stage_lds, tokens);
+  if (part == 0 && r0 == 0) {
+    if (threadIdx.x < 64) c.tile_token[index * kTileTokens + threadIdx.x] = tokens;
+    if (threadIdx.x == 0) c.tile[index] = t;
+  }
   if (t.rows == 0 || t.slot < 0) return;
   const AdapterSlot slot = b.table[t.slot];
   const int tiles = (slot.rank + 15) >> 4;
@@ -333,7 +405,6 @@ __global__ __launch_bounds__(256, 2) void adapter_down_kernel(Call c, int rank_g
   const int s0 = (int)((int64_t)stages * part / c.parts), s1 = (int)((int64_t)stages * (part + 1) / c.parts);
   const uint32_t lds = mxd::lds_addr(stage_lds);
   const int piece = (lane & 31) ^ (lane >> 5 << 3);   // of its row that this lane copies
-  const int tokens = tile_tokens(c, t);
   const uint8_t* src[kColumns * 2];
 #pragma unroll
   for (int j = 0; j < kColumns * 2; ++j)
@@ -651,21 +722,22 @@ __global__ __launch_bounds__(256) void adapter_up_kernel(Call c) {
   __shared__ uint4 h_lds[kColumns * RT * 64];
   const Bank& b = c.bank;
   const int groups = (b.blocks + 3) / 4, group = blockIdx.x % groups;
-  const Tile t = find_tile(c, blockIdx.x / groups);
+  const int index = blockIdx.x / groups;
+  const Tile t = c.tile[index];
   if (t.rows == 0) return;
+  const int tokens = c.tile_token[index * kTileTokens + (threadIdx.x & 63)];
   const AdapterSlot slot = t.slot >= 0 ? b.table[t.slot] : AdapterSlot{0, 0.f};
   const int tiles = (slot.rank + 15) >> 4;
   const int tid = threadIdx.x, lane = tid & 63, q = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int block = 4 * group + wave, n = 64 * block + 8 * q;   // past the last block: no output is a lane's
   // every load below goes out before the first of them is waited for; lanes without an output repeat another's address
-  const int tokens = tile_tokens(c, t);
   const int64_t rank_stride = 16 * b.rank_tiles;
+  const float* low_h = c.low + __shfl(tokens, 16 * wave + (lane & 15), 64) * rank_stride + 4 * q;
   uint4 h[RT];   // of the wave's column tile
-  {
-    const float* p = c.low + __shfl(tokens, 16 * wave + (lane & 15), 64) * rank_stride + 4 * q;
+  if (RT > 1 || c.parts == 1) {
 #pragma unroll
-    for (int r = 0; r < RT; ++r) h[r] = ldg128((const uint8_t*)(p + 16 * max(min(r, tiles - 1), 0)));
+    for (int r = 0; r < RT; ++r) h[r] = ldg128((const uint8_t*)(low_h + 16 * max(min(r, tiles - 1), 0)));
   }
   uint4 w[RT][2];
   {
@@ -696,6 +768,8 @@ __global__ __launch_bounds__(256) void adapter_up_kernel(Call c) {
         base[i][k] = ldg128((const uint8_t*)((const uint16_t*)c.base + token[i][k] * c.base_stride + at));
       }
     }
+  if constexpr (RT == 1)
+    if (c.parts > 1 && tiles) h[0] = h_operand(slot, 4 * q, sum_parts(low_h, c.tokens * rank_stride, 0, 1, c.parts));
 #pragma unroll
   for (int r = 0; r < RT; ++r) {
     const int ranks = slot.rank - 16 * r - 4 * q;   // the sums past the slot's rank are not its own
@@ -779,7 +853,7 @@ using mxi::use;
 namespace {
 
 struct Workspace {
-  uint64_t pair_row, row_pair, low, bytes;   // offsets; the plan's first at 0
+  uint64_t pair_row, row_pair, tile, tile_token, low, bytes;   // offsets; the plan's first at 0
 };
 
 Workspace workspace_of(const Bank& b, int32_t tokens) {
@@ -787,7 +861,9 @@ Workspace workspace_of(const Bank& b, int32_t tokens) {
   Workspace w;
   w.pair_row = round256(4 * ((uint64_t)b.slots + 1));
   w.row_pair = w.pair_row + round256(4 * (uint64_t)tokens);
-  w.low = w.row_pair + round256(4 * (uint64_t)tokens);
+  w.tile = w.row_pair + round256(4 * (uint64_t)tokens);
+  w.tile_token = w.tile + round256(sizeof(Tile) * (uint64_t)tiles_of(b, tokens));
+  w.low = w.tile_token + round256(4 * kTileTokens * (uint64_t)tiles_of(b, tokens));
   w.bytes = w.low + round256(rows * 64 * b.rank_tiles);
   return w;
 }
@@ -843,7 +919,7 @@ int launch_groups(const Call& c, bool f32, hipStream_t st) {
               : rt == 2 ? (stream ? launch_down<2, true>(c, st) : launch_down<2, false>(c, st))
                         : (stream ? launch_down<4, true>(c, st) : launch_down<4, false>(c, st)))
     return s;
-  if (c.parts > 1) {
+  if (c.parts > 1 && rt > 1) {
     const int64_t entries = (int64_t)c.tokens * 4 * rt;
     hipLaunchKernelGGL(adapter_sum_kernel, dim3((unsigned)((entries + 255) / 256)), dim3(256), 0, st, c);
     MX_LAUNCH_CHECK("adapter_sum_kernel");
@@ -950,18 +1026,17 @@ int mx_adapters_apply(mx_adapters* a, const uint16_t* x, int64_t x_stride, const
   if (int s = use(a->ctx)) return s;
   hipStream_t st = as_stream(stream);
   uint8_t* ws = (uint8_t*)workspace;
-  Call c{b, x, x_stride, ids, nullptr, nullptr, tokens, parts_of(b, tokens), (float*)(ws + w.low),
-         base, base_stride, y, y_stride, 0, false};
+  Call c{b, x, x_stride, ids, nullptr, nullptr, (Tile*)(ws + w.tile), (int32_t*)(ws + w.tile_token), tokens,
+         parts_of(b, tokens), (float*)(ws + w.low), base, base_stride, y, y_stride, 0, false};
   if (w.low + (uint64_t)c.parts * tokens * 64 * b.rank_tiles > w.bytes)   // parts_of and workspace_of belong together
     return mxi::fail(MX_ERR_STATE, "%s: %d parts of %d tokens exceed the workspace", who, c.parts, tokens);
   if (is_few(b, tokens)) return launch_few(c, f32, st);
   mx_row_plan own{(int32_t*)ws, (int32_t*)(ws + w.pair_row), (int32_t*)(ws + w.row_pair)};
-  if (!plan) {
+  if (!plan && tokens > kOwnTokens) {
     if (int s = mxi::row_plan(ids, tokens, b.slots, own, st)) return s;
     plan = &own;
   }
-  c.first = plan->first;
-  c.row_pair = plan->row_pair;
+  if (plan) c.first = plan->first, c.row_pair = plan->row_pair;
   c.tiles = tiles_of(b, tokens);
   c.stream = (int64_t)tokens * b.n * (f32 ? 6 : 4) > kStreamBytes;
   return launch_groups(c, f32, st);
