@@ -157,6 +157,32 @@ def test_gradients_against_differences(gpu_ctx):
             assert abs(loss(rows, weights + step) - loss(rows, weights) - got["dweights"][index]) < limit
 
 
+# pairs around the sizes where another form of the plan takes over (8192, 16384, 49152 over the rounds of 512 groups), and
+# routings that put all pairs in one group or in none
+@pytest.mark.parametrize("tokens,k,experts", [(1025, 8, 30), (2049, 8, 30), (6143, 8, 256), (6145, 8, 256), (49153, 1, 17),
+                                              (70001, 1, 1), (1537, 16, 512), (2051, 8, 1024), (40000, 32, 1023)])
+@pytest.mark.parametrize("kind", ["random", "one", "none"])
+def test_plans_of_many_pairs(gpu_ctx, tokens, k, experts, kind):
+    rng = np.random.default_rng(tokens)
+    ids = routing(rng, tokens, k, experts)
+    if kind != "random":
+        ids[:] = experts - 1 if kind == "one" else experts
+        ids[tokens // 2] = 0
+    key = np.where((ids >= 0) & (ids < experts), ids, experts).reshape(-1)
+    row_pair = np.argsort(key, kind="stable")
+    first = np.searchsorted(key[row_pair], np.arange(experts + 1))
+    pair_row = np.full(tokens * k, -1)
+    pair_row[row_pair[:first[-1]]] = np.arange(first[-1])
+    idd = gpu_ctx.upload(ids)
+    with ExpertDispatch(gpu_ctx, experts, k, tokens) as d:
+        for _ in range(2):   # the second over the first's plan
+            d.plan_device(idd, tokens)
+        got = d.read_plan()
+    idd.free()
+    for name, want in (("first", first), ("pair_row", pair_row.reshape(tokens, k)), ("row_pair", row_pair)):
+        np.testing.assert_array_equal(got[name], want)
+
+
 def test_no_token_and_no_row(gpu_ctx):
     with ExpertDispatch(gpu_ctx, 6, 2, 8) as d:
         got = d.dispatch(np.zeros((0, 2), np.int32), np.zeros((0, 64), np.uint16))

@@ -117,6 +117,158 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanArgs a) {
   else place_key<false, kBatch>(a, g, sums);
 }
 
+// Many pairs: the pairs in up to kMaxChunks contiguous chunks and three launches, work in proportion to the pairs and to
+// chunks x groups: count each chunk's keys; each chunk's first row of each group; place each chunk's pairs. There is no
+// workspace: a chunk's counts lie in its own part of row_pair and its first rows in its own part of pair_row, which its
+// workgroup has read before anyone writes there, so a chunk has at least G + 1 pairs.
+//
+// One launch against three, random ids, 8 a token: of 256 groups 32768 pairs 8.9 and 13.7 us, 131072 28 and 14, 2^21 383
+// and 31; of 1024 groups, whose workgroups are not all resident at once, 16384 pairs 12.7 and 17.7, 32768 20.7 and 18.1,
+// 2^23 3961 and 128.
+constexpr int kMaxChunks = 256, kChunkPairs = 2048;   // at least
+constexpr int kChunkedPairs = 3 << 14;                // above this over the walk's rounds (512 workgroups each)
+static_assert(kChunkPairs > kMaxGroups, "a chunk's part holds a number for every key");
+
+struct ChunkArgs {
+  PlanArgs plan;
+  int32_t chunks;
+  __device__ __forceinline__ int begin(int c) const { return (int)((int64_t)plan.pairs * c / chunks); }
+};
+
+__global__ __launch_bounds__(kPlanThreads) void plan_count_kernel(ChunkArgs a) {
+  __shared__ int count[kMaxGroups + 1];
+  const int tid = threadIdx.x, groups = a.plan.groups, p0 = a.begin(blockIdx.x), p1 = a.begin(blockIdx.x + 1);
+  for (int g = tid; g <= groups; g += kPlanThreads) count[g] = 0;
+  __syncthreads();
+  constexpr int kBatch = 8;
+  for (int at = p0 + tid; at < p1; at += kBatch * kPlanThreads) {
+    uint32_t id[kBatch];
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) id[i] = (uint32_t)a.plan.ids[min(at + i * kPlanThreads, p1 - 1)];
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i)
+      if (at + i * kPlanThreads < p1) atomicAdd(&count[min(id[i], (uint32_t)groups)], 1);
+  }
+  __syncthreads();
+  for (int g = tid; g <= groups; g += kPlanThreads) a.plan.row_pair[p0 + g] = count[g];
+}
+
+// A workgroup 16 keys: thread (key, share of four chunks). What comes before its keys it counts for itself.
+constexpr int kBaseKeys = 16, kShares = kPlanThreads / kBaseKeys, kPerShare = kMaxChunks / kShares;
+
+__global__ __launch_bounds__(kPlanThreads) void plan_base_kernel(ChunkArgs a) {
+  __shared__ int before[kPlanWaves], waves[kPlanWaves][kBaseKeys];
+  const int tid = threadIdx.x, lane = tid & 63, groups = a.plan.groups, g0 = kBaseKeys * blockIdx.x;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int key = g0 + tid % kBaseKeys, c0 = tid / kBaseKeys * kPerShare;
+  int count[kPerShare], sum = 0;
+#pragma unroll
+  for (int i = 0; i < kPerShare; ++i) {
+    const int v = a.plan.row_pair[a.begin(min(c0 + i, a.chunks - 1)) + min(key, groups)];
+    count[i] = c0 + i < a.chunks && key <= groups ? v : 0;
+    sum += count[i];
+  }
+  int below = 0;   // the smaller keys of chunks wave, wave + 16, ...
+  for (int c = wave; c < a.chunks; c += 4 * kPlanWaves)
+    for (int g = lane; g < g0; g += 64) {
+      int v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = a.plan.row_pair[a.begin(min(c + i * kPlanWaves, a.chunks - 1)) + g];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) below += c + i * kPlanWaves < a.chunks ? v[i] : 0;
+    }
+#pragma unroll
+  for (int m = 32; m >= 1; m >>= 1) below += __shfl_xor(below, m, 64);
+  int upto = sum;   // of the wave's shares of this key up to this one
+#pragma unroll
+  for (int d = kBaseKeys; d < 64; d <<= 1) {
+    const int o = __shfl_up(upto, d, 64);
+    if (lane >= d) upto += o;
+  }
+  if (lane == 0) before[wave] = below;
+  if (lane >= 64 - kBaseKeys) waves[wave][lane % kBaseKeys] = upto;
+  __syncthreads();
+  int row = upto - sum, total = 0;
+#pragma unroll
+  for (int w = 0; w < kPlanWaves; ++w) {
+    row += before[w] + (w < wave ? waves[w][tid % kBaseKeys] : 0);
+    total += waves[w][tid % kBaseKeys];
+  }
+  int smaller = total;
+#pragma unroll
+  for (int d = 1; d < kBaseKeys; d <<= 1) {
+    const int o = __shfl_up(smaller, d, kBaseKeys);
+    if (tid % kBaseKeys >= d) smaller += o;
+  }
+  row += smaller - total;
+  if (key > groups) return;
+  if (tid < kBaseKeys) a.plan.first[key] = row;
+#pragma unroll
+  for (int i = 0; i < kPerShare; ++i)
+    if (c0 + i < a.chunks) {
+      a.plan.pair_row[a.begin(c0 + i) + key] = row;
+      row += count[i];
+    }
+}
+
+// A chunk's waves take a contiguous section each and count its keys; the next row of each key and wave then stands in LDS,
+// and 64 pairs at a time find their place among those of their key by a ballot for each bit of the key.
+__global__ __launch_bounds__(kPlanThreads) void plan_place_kernel(ChunkArgs a, int bits) {
+  extern __shared__ int next[];   // [kPlanWaves][groups + 1]
+  const int tid = threadIdx.x, lane = tid & 63, groups = a.plan.groups;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int begin = a.begin(blockIdx.x), end = a.begin(blockIdx.x + 1);
+  const int section = (end - begin + kPlanThreads - 1) / kPlanThreads * 64;
+  const int p0 = min(begin + wave * section, end), p1 = min(p0 + section, end);
+  int* own = next + wave * (groups + 1);
+  for (int g = lane; g <= groups; g += 64) own[g] = 0;
+  __syncthreads();
+  constexpr int kBatch = 8;
+  uint32_t key[kBatch];
+  auto load = [&](int at) {
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) key[i] = min((uint32_t)a.plan.ids[min(at + 64 * i + lane, p1 - 1)], (uint32_t)groups);
+  };
+  for (int at = p0; at < p1; at += 64 * kBatch) {
+    load(at);
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i)
+      if (at + 64 * i + lane < p1) atomicAdd(&own[key[i]], 1);
+  }
+  __syncthreads();
+  for (int g = tid; g <= groups; g += kPlanThreads) {
+    int row = a.plan.pair_row[begin + g];
+#pragma unroll
+    for (int w = 0; w < kPlanWaves; ++w) {
+      const int count = next[w * (groups + 1) + g];
+      next[w * (groups + 1) + g] = row;
+      row += count;
+    }
+  }
+  __syncthreads();   // the chunk's part of pair_row has been read
+  for (int at = p0; at < p1; at += 64 * kBatch) {
+    if (section > 64 * kBatch) load(at);
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      const int p = at + 64 * i + lane;
+      if (at + 64 * i >= p1) break;
+      uint64_t mask = __ballot(p < p1);   // the lanes with this lane's key
+      for (int b = 0; b < bits; ++b) {
+        const bool set = key[i] >> b & 1;
+        const uint64_t with = __ballot(set);
+        mask &= set ? with : ~with;
+      }
+      if (p < p1) {
+        const int place = __popcll(mask & ((1ull << lane) - 1)), r = own[key[i]] + place;
+        a.plan.row_pair[r] = p;
+        a.plan.pair_row[p] = key[i] == (uint32_t)groups ? -1 : r;
+        __builtin_amdgcn_wave_barrier();   // every lane has read its key's row before the first of the key moves it on
+        if (place == 0) own[key[i]] = r + __popcll(mask);
+      }
+    }
+  }
+}
+
 // Access to rows that the call touches once: past the caches where the call moves more than they hold (kStream).
 template <bool kStream, typename R>
 __device__ __forceinline__ R load_once(const R* p) {
@@ -584,7 +736,21 @@ using mxi::use;
 
 int mxi::row_plan(const int32_t* ids, int32_t pairs, int32_t groups, const mx_row_plan& plan, hipStream_t st) {
   const PlanArgs a{ids, pairs, groups, plan.first, plan.pair_row, plan.row_pair};
+  if (pairs > kChunkedPairs / (groups / 512 + 1)) {
+    const ChunkArgs c{a, std::min(kMaxChunks, pairs / kChunkPairs)};
+    hipLaunchKernelGGL(plan_count_kernel, dim3(c.chunks), dim3(kPlanThreads), 0, st, c);
+    MX_LAUNCH_CHECK("plan_count_kernel");
+    hipLaunchKernelGGL(plan_base_kernel, dim3(groups / kBaseKeys + 1), dim3(kPlanThreads), 0, st, c);
+    MX_LAUNCH_CHECK("plan_base_kernel");
+    int bits = 1;
+    while (groups >> bits) ++bits;
+    hipLaunchKernelGGL(plan_place_kernel, dim3(c.chunks), dim3(kPlanThreads), kPlanWaves * (groups + 1) * sizeof(int), st, c,
+                       bits);
+    MX_LAUNCH_CHECK("plan_place_kernel");
+    return MX_OK;
+  }
   if (pairs <= 8 * kPlanThreads) hipLaunchKernelGGL(plan_kernel<8>, dim3(groups + 1), dim3(kPlanThreads), 0, st, a);
+  else if (pairs <= 16 * kPlanThreads) hipLaunchKernelGGL(plan_kernel<16>, dim3(groups + 1), dim3(kPlanThreads), 0, st, a);
   else hipLaunchKernelGGL(plan_kernel<32>, dim3(groups + 1), dim3(kPlanThreads), 0, st, a);
   MX_LAUNCH_CHECK("plan_kernel");
   return MX_OK;
