@@ -1,8 +1,9 @@
 // Low-rank adapters of many requests beside a projection: y[t] = base[t] + scale_a up_a (down_a x[t]), a = ids[t].
 //
 // The quantized base weights cannot take an adapter in, so each token's pair of thin matrices runs beside them: down
-// [rank][K] then up [N][rank], both BF16, with the projection's output (BF16, or its FP32 sums) as base and one rounding.
-// Both products run on V_MFMA_F32_16X16X32_BF16 with the weights as operand A and tokens as operand B's columns:
+// [rank][K] then up [N][rank], both BF16, with the projection's output (BF16, or its FP32 sums) as base and one
+// rounding. Both products run on V_MFMA_F32_16X16X32_BF16 with the weights as operand A and tokens as operand B's
+// columns:
 //   A lane l = row l % 16, K 8 (l / 16) + 0..7; B lane l = column l % 16, same K; D lane l register i = row 4 (l / 16)
 //   + i, column l % 16.
 // So down's D gives lane (token, q) the ranks 4q..4q+3 of a 16-rank tile, which is what up's operand B wants of that
@@ -15,6 +16,10 @@
 //   up: [block of 64 outputs][rank tile][half][lane] 16 bytes: two tiles j = 0, 1 of four ranks each; row m of tile j of
 //   a half is output 64 b + 32 half + 8 (m / 4) + 4 j + m % 4, so a lane's D registers of a half's two tiles are 8
 //   consecutive outputs of its token and the four lanes of a token 32 (64 bytes of y).
+//
+// Three forms. Calls of few tokens are bound by the weights of the adapters they name and by their launches, so each
+// token's workgroups find the tokens that share its adapter by a ballot, one launch or two. Larger calls sort the
+// tokens by adapter into tiles of 64 and read each weight once a tile; x, base and y, once each, then bound them.
 #include <algorithm>
 #include <new>
 
@@ -35,9 +40,15 @@ constexpr int kFewTokens = 128;    // a wave holds the ids of this many tokens, 
 constexpr int kTileTokens = 64;    // tokens of a workgroup in the grouped form
 constexpr int kColumns = kTileTokens / 16;
 constexpr int kMaxParts = 32;      // parts of K
-constexpr int kFusedChunks = 256;  // KB of down up to which a call of few tokens is one launch
-// An x of more than this is read, and the y of a base and y of more than this written, past the caches.
-constexpr int64_t kStreamBytes = 96 << 20;
+// KB of down up to which a call of few tokens is one launch (each of its workgroups reads all of down). One launch and
+// two, one token: 1536 columns of rank 16 (48 KB) 5.0 and 7.4 us, 7168 of rank 16 (224 KB) 6.0 and 7.0, 7168 of rank 32
+// (448 KB) 7.8 and 7.0, 16384 of rank 16 (512 KB) 10.3 and 7.0. Four rank tiles take too many registers: 10.2 and 7.1.
+constexpr int kFusedChunks = 256;
+// Calls whose x, base and y exceed this read x past the caches, which leaves them to the weights, base and y. Past them
+// and through, three sets in turn, 8 adapters of rank 64 or 32: 1000 tokens of 16384 to 7168 (62 MB) 30.6 and 31.0 us,
+// 1500 (92 MB) 33.8 and 37.7, 2000 (123 MB) 43.3 and 48.5, 4096 (252 MB) 72.9 and 72.3; 2500 of 7168 to 1536 (51 MB)
+// 23.4 and 22.5, 4000 (82 MB) 28.5 and 28.1. (For y it makes no difference.)
+constexpr int64_t kStreamBytes = 80 << 20;
 constexpr int kWantGroups = 512;   // workgroups that the split of K aims at
 
 struct AdapterSlot {
@@ -53,13 +64,18 @@ struct Bank {
   int32_t rank_tiles, chunks, blocks;   // of the largest rank; K chunks of 32 (an even count); blocks of 64 outputs
   __host__ __device__ int64_t down_bytes() const { return (int64_t)rank_tiles * chunks * 1024; }
   __host__ __device__ int64_t up_bytes() const { return (int64_t)blocks * rank_tiles * 2048; }
+  // a block of a slot; what is past the bank repeats its last block, and no slot is the first
+  __device__ __forceinline__ const uint8_t* up_at(int slot, int block) const {
+    return up + max(slot, 0) * up_bytes() + (int64_t)min(block, blocks - 1) * rank_tiles * 2048;
+  }
 };
 
 __device__ __forceinline__ v8bf as_bf(uint4 v) { return __builtin_bit_cast(v8bf, v); }
 
 // ---- loading a slot ----
 
-__global__ __launch_bounds__(64) void adapter_store_down_kernel(Bank b, uint8_t* bank, int slot, const uint16_t* src, int rank) {
+__global__ __launch_bounds__(64) void adapter_store_down_kernel(Bank b, uint8_t* bank, int slot, const uint16_t* src,
+                                                                int rank) {
   const int lane = threadIdx.x, c = blockIdx.x, rt = blockIdx.y;
   const int r = 16 * rt + (lane & 15), k0 = 32 * c + 8 * (lane >> 4);
   uint32_t w[4] = {0, 0, 0, 0};
@@ -109,11 +125,10 @@ struct Call {
   uint16_t* y;
   int64_t y_stride;
   int32_t tiles;             // grouped form: the most tiles that there can be
-  bool stream;               // grouped form: y is written past the caches
 };
 
-// Which of the groups' tiles is number `index`: kTileTokens tokens of a group each (a group's last one short), the tokens
-// without an adapter last as group `slots`. count(g) gives the tokens of a group; 64 groups at a time.
+// Which of the groups' tiles is number `index`: kTileTokens tokens of a group each (a group's last one short), the
+// tokens without an adapter last as group `slots`. count(g) gives the tokens of a group; 64 groups at a time.
 struct Place {
   int group, skip, rows;   // rows = 0 past the last tile; else tokens kTileTokens skip .. of the group
 };
@@ -161,7 +176,9 @@ __device__ __forceinline__ Tile plan_tile(const Call& c, int index, int& token) 
 }
 
 // The same from the ids themselves, by a workgroup of four waves for itself: it counts the groups in `lds`, finds its
-// tile and picks out the tile's tokens in ascending order. The waves hold the ids, a contiguous section each.
+// tile and picks out the tile's tokens in ascending order. The waves hold the ids, a contiguous section each. About 2
+// us in each round of workgroups, where the plan is a launch of 5: 1000 tokens of 8 adapters of rank 32 17.8 us, by a
+// plan 20.0; 4096 of rank 64 72.9 and 73.9; 4000 of rank 256, in four rank groups, 157 and 156.
 constexpr int kOwnIds = 16, kOwnTokens = 4 * 64 * kOwnIds;
 constexpr int kCopies = 8;   // of each count, by lane: neighbours of one group take few turns at one of them
 constexpr int kOwnLds = (kMaxSlots + 1) * kCopies + 4 + kTileTokens;   // numbers
@@ -217,8 +234,8 @@ __device__ __forceinline__ Tile own_tile(const Call& c, int index, int* lds, int
 }
 
 // Few tokens: the workgroups of token t take the tokens of t's adapter, up to 16 a workgroup. The first of each 16 does
-// it; rows = 0 for the others. (Tokens are the grid's slow dimension: as its fast one, a count of them that eight divides
-// puts all the workgroups of a token on one XCD, and 64 tokens of 16 adapters take 27 us where 65 take 17.)
+// it; rows = 0 for the others. (Tokens are the grid's slow dimension: as its fast one, a count of them that eight
+// divides puts all the workgroups of a token on one XCD, and 64 tokens of 16 adapters take 27 us where 65 take 17.)
 struct Few {
   int slot, rows;
   int token;   // of this lane's column, lane % 16; columns past the last repeat it
@@ -290,9 +307,10 @@ __device__ __forceinline__ v4f sum_parts(const float* p, int64_t stride, int fir
 
 // ---- down: partial sums of h ----
 
-// Few tokens, grid (parts, T), 4 waves: a part of K for up to 16 tokens of an adapter, RT rank tiles at a time (those past
-// the last repeat it). The waves take the K units (of 64: two chunks) in turn, the next one's loads in
-// flight while one is multiplied, and their sums are added in wave order.
+// Few tokens, grid (parts, T), 4 waves: a part of K for up to 16 tokens of an adapter, RT rank tiles at a time (those
+// past the last repeat it). Bound by down's bytes: 24 tokens of 16 adapters of rank 64 by 16384 (33 MB) 8.0 us. The
+// waves take the K units (of 64: two chunks) in turn, the next one's loads in flight while one is multiplied, and their
+// sums are added in wave order.
 template <int RT>
 __device__ __forceinline__ void few_down(const Call& c, const Few& f, int r0, int tiles, int first_tiles,
                                          v4f (*red)[RT][64]) {
@@ -376,10 +394,12 @@ __global__ __launch_bounds__(256) void adapter_few_down_kernel(Call c) {
 
 // Grouped form: a part of K for a tile of 64 tokens and RT rank tiles, 4 waves. x comes through LDS in stages of 256 K,
 // so that rows are read 512 bytes at a time (in operand order a load takes 64 bytes of each of 16 rows: with rows a
-// power of two apart those meet in the same memory channels); each wave multiplies its K unit of 64 of every stage,
-// its weights straight from the L2 of its XCD, which holds one part's. Two stages: one in flight while one is
-// multiplied. The rows of a pair lie 512 bytes apart and the pairs 1040, and a second row's 16-byte pieces are swapped
-// in halves of 128 bytes, so that the 16 rows of an operand read lie in different banks.
+// power of two apart those meet in the same memory channels); each wave multiplies its K unit of 64 of every stage, its
+// weights straight from the L2 of its XCD, which holds one part's. Two stages: one in flight while one is multiplied.
+// 4096 tokens of 8 adapters of rank 64 by 16384, by a plan: 35 us, of which x (134 MB) alone, read so, takes 25;
+// without LDS 46; tiles of 128 tokens 34, but 62 against 55 with two rank groups. The rows of a pair lie 512 bytes
+// apart and the pairs 1040, and a second row's 16-byte pieces are swapped in halves of 128 bytes, so that the 16 rows
+// of an operand read lie in different banks.
 constexpr int kStageK = 256, kPairBytes = 1040, kStageBytes = kTileTokens / 2 * kPairBytes;
 
 template <int RT, bool kStream>
@@ -496,7 +516,10 @@ __global__ __launch_bounds__(256, 2) void adapter_down_kernel(Call c, int rank_g
   }
 }
 
-// Grouped form: the parts of four ranks of a token added in order, as operand B in the first part's place.
+// Grouped form of more than 16 ranks: the parts of four ranks of a token added in order, as operand B in the first
+// part's place. A launch of its own, 3 to 5 us: in up every workgroup of a tile would add them anew, which 4096 tokens
+// of rank 64 pay with 18 us and 3056 beside 24576 rows with 41, and even rank 32 with 1. Of up to 16 ranks up does it:
+// 1010 tokens of rank 8 12.1 us in all, with this launch 14.0.
 __global__ __launch_bounds__(256) void adapter_sum_kernel(Call c) {
   const Bank& b = c.bank;
   const int per = 4 * b.rank_tiles;   // entries of a token
@@ -569,9 +592,10 @@ __device__ __forceinline__ void up_tile(const uint4 (&w)[2], uint4 h, v4f (&acc)
   for (int j = 0; j < 4; ++j) acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf(a[j]), as_bf(h), acc[j], 0, 0, 0);
 }
 
-// Few tokens, grid (output blocks / 4, T), 4 waves, a block of 64 outputs each for up to 16 tokens of an adapter. What does
-// not depend on h is asked for before h is put together: thread (entry e, share s) adds the parts s, s + shares, ... of
-// four ranks of a token, and the shares are added in order.
+// Few tokens, grid (output blocks / 4, T), 4 waves, a block of 64 outputs each for up to 16 tokens of an adapter (24
+// tokens of 16 adapters of rank 64, 7168 outputs, 15 MB of up: 6.2 us). What does not depend on h is asked for before h
+// is put together: thread (entry e, share s) adds the parts s, s + shares, ... of four ranks of a token, and the shares
+// are added in order.
 template <bool kF32>
 __global__ __launch_bounds__(256) void adapter_few_up_kernel(Call c) {
   constexpr int RT = 4;   // rank tiles in registers at once
@@ -583,7 +607,7 @@ __global__ __launch_bounds__(256) void adapter_few_up_kernel(Call c) {
   const int tid = threadIdx.x, lane = tid & 63, q = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int block = 4 * blockIdx.x + wave, n = 64 * block + 8 * q;   // past the last block: no output is a lane's
-  const uint8_t* up = b.up + max(f.slot, 0) * b.up_bytes() + (int64_t)min(block, b.blocks - 1) * b.rank_tiles * 2048 + 16 * lane;
+  const uint8_t* up = b.up_at(f.slot, block) + 16 * lane;
   uint4 w[RT][2];
   auto load_up = [&](int r0, int count) {
 #pragma unroll
@@ -630,9 +654,10 @@ __global__ __launch_bounds__(256) void adapter_few_up_kernel(Call c) {
       *(uint4*)(c.y + f.token * c.y_stride + n + 32 * k) = eight_bf16(acc[2 * k], acc[2 * k + 1]);
 }
 
-// Few tokens in one launch, for a down that every workgroup can read for itself: grid (output blocks / 16, T), 16 waves.
-// The waves take the K units of 64 in turn, two of them in flight, h is put together through LDS, and each wave finishes
-// a block of 64 outputs whose up and base were asked for at the start.
+// Few tokens in one launch, for a down that every workgroup can read for itself: grid (output blocks / 16, T), 16
+// waves. A chain of two loads' latencies and a launch: one token 4.8 us. The waves take the K units of 64 in turn, two
+// of them in flight, h is put together through LDS, and each wave finishes a block of 64 outputs whose up and base were
+// asked for at the start.
 template <int RT, bool kF32>
 __global__ __launch_bounds__(1024) void adapter_few_kernel(Call c) {
   __shared__ v4f sums[16][RT][64];
@@ -647,7 +672,7 @@ __global__ __launch_bounds__(1024) void adapter_few_kernel(Call c) {
   const int64_t tile_bytes = (int64_t)b.chunks * 1024;
   const uint8_t* x = (const uint8_t*)(c.x + f.token * c.x_stride) + 16 * q;
   const uint8_t* down = b.down + max(f.slot, 0) * b.down_bytes() + 16 * lane;
-  const uint8_t* up = b.up + max(f.slot, 0) * b.up_bytes() + (int64_t)min(block, b.blocks - 1) * b.rank_tiles * 2048 + 16 * lane;
+  const uint8_t* up = b.up_at(f.slot, block) + 16 * lane;
   struct Unit {
     uint4 x[2], w[2][RT];
   } unit[2];
@@ -715,8 +740,10 @@ __global__ __launch_bounds__(1024) void adapter_few_kernel(Call c) {
       *(uint4*)(c.y + f.token * c.y_stride + n + 32 * k) = eight_bf16(out[2 * k], out[2 * k + 1]);
 }
 
-// Grouped form: a tile of 64 tokens and four blocks of 64 outputs, one a wave, its weights of all ranks in registers for
-// the tile's columns, 16 tokens at a time. What does not depend on h is asked for before h goes to LDS.
+// Grouped form: a tile of 64 tokens and four blocks of 64 outputs, one a wave, its weights of all ranks in registers
+// for the tile's columns, 16 tokens at a time. What does not depend on h is asked for before h goes to LDS. Bound by
+// base and y: 4096 tokens of 7168 outputs (117 MB) 30 us, 3056 of 24576 (300 MB) 69; with accesses of 64 bytes the
+// first 37.
 template <int RT, bool kF32>
 __global__ __launch_bounds__(256) void adapter_up_kernel(Call c) {
   __shared__ uint4 h_lds[kColumns * RT * 64];
@@ -741,7 +768,7 @@ __global__ __launch_bounds__(256) void adapter_up_kernel(Call c) {
   }
   uint4 w[RT][2];
   {
-    const uint8_t* p = b.up + max(t.slot, 0) * b.up_bytes() + (int64_t)min(block, b.blocks - 1) * b.rank_tiles * 2048 + 16 * lane;
+    const uint8_t* p = b.up_at(t.slot, block) + 16 * lane;
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
       const int at = max(min(r, tiles - 1), 0);
@@ -807,9 +834,7 @@ __global__ __launch_bounds__(256) void adapter_up_kernel(Call c) {
 #pragma unroll
     for (int k = 0; k < 2; ++k)
       if (16 * i + 8 * k + (lane & 7) < t.rows && at_y < b.n) {
-        mxd::u32x4_t* y = (mxd::u32x4_t*)(c.y + token[i][k] * c.y_stride + at_y);
-        if (c.stream) __builtin_nontemporal_store(__builtin_bit_cast(mxd::u32x4_t, out[k]), y);
-        else *y = __builtin_bit_cast(mxd::u32x4_t, out[k]);
+        *(uint4*)(c.y + token[i][k] * c.y_stride + at_y) = out[k];
       }
   }
 }
@@ -823,9 +848,10 @@ int tiles_of(const Bank& b, int tokens) {
   return (int)(((int64_t)tokens + (int64_t)groups * (kTileTokens - 1)) / kTileTokens);
 }
 
-// Calls of few tokens need no plan and two launches. Up to 64 they are always the faster form, and to the 128 that a wave
-// can hold with at most 64 ranks (the output projection, 16 adapters, 100 and 128 tokens: 21.0 and 22.3 us, grouped
-// 23.0; of rank 128 37.7 and 39.2, grouped 30.8 and 31.9).
+// Which calls are of few tokens: up to 64, and with at most 64 ranks to the 128 that a wave can hold. Few and grouped,
+// 16384 columns and 7168 rows: 16 adapters of rank 64, 64 tokens 17.1 and 21.4 us, 128 22.7 and 21.2; 2 of rank 16, 128
+// tokens 11.7 and 13.3; 16 of rank 128, 64 tokens 31.6 and 34.2, 128 39.2 and 31.9. 1536 columns and 24576 rows, 16 of
+// rank 32: 64 tokens 14.2 and 17.2, 128 19.5 and 17.4; 7168 and 576, 4 of rank 64: 120 tokens 13.7 and 16.5.
 bool is_few(const Bank& b, int tokens) { return tokens <= (b.rank_tiles <= 4 ? kFewTokens : kFewTokens / 2); }
 
 // Parts of K. Few tokens: as many as give each wave a unit of 64, since how many adapters the tokens share is not known
@@ -897,8 +923,8 @@ template <int RT, bool kStream>
 int launch_down(const Call& c, hipStream_t st) {
   const int rank_groups = (c.bank.rank_tiles + RT - 1) / RT;
   constexpr size_t lds = std::max(2 * kStageBytes, 4 * kColumns * RT * 1024);
-  hipLaunchKernelGGL((adapter_down_kernel<RT, kStream>), dim3(round8((int64_t)c.parts * c.tiles * rank_groups)), dim3(256), lds,
-                     st, c, rank_groups);
+  hipLaunchKernelGGL((adapter_down_kernel<RT, kStream>), dim3(round8((int64_t)c.parts * c.tiles * rank_groups)), dim3(256),
+                     lds, st, c, rank_groups);
   MX_LAUNCH_CHECK("adapter_down_kernel");
   return MX_OK;
 }
@@ -914,7 +940,8 @@ int launch_up(const Call& c, bool f32, hipStream_t st) {
 
 int launch_groups(const Call& c, bool f32, hipStream_t st) {
   const int rt = c.bank.rank_tiles;
-  const bool stream = rt <= 4 && 2 * (int64_t)c.tokens * c.bank.k > kStreamBytes;   // more rank tiles read x again
+  const bool stream = rt <= 4 &&   // with more rank tiles x is read again
+                      (int64_t)c.tokens * (2 * (int64_t)c.bank.k + (f32 ? 6 : 4) * (int64_t)c.bank.n) > kStreamBytes;
   if (int s = rt == 1   ? (stream ? launch_down<1, true>(c, st) : launch_down<1, false>(c, st))
               : rt == 2 ? (stream ? launch_down<2, true>(c, st) : launch_down<2, false>(c, st))
                         : (stream ? launch_down<4, true>(c, st) : launch_down<4, false>(c, st)))
@@ -1027,7 +1054,7 @@ int mx_adapters_apply(mx_adapters* a, const uint16_t* x, int64_t x_stride, const
   hipStream_t st = as_stream(stream);
   uint8_t* ws = (uint8_t*)workspace;
   Call c{b, x, x_stride, ids, nullptr, nullptr, (Tile*)(ws + w.tile), (int32_t*)(ws + w.tile_token), tokens,
-         parts_of(b, tokens), (float*)(ws + w.low), base, base_stride, y, y_stride, 0, false};
+         parts_of(b, tokens), (float*)(ws + w.low), base, base_stride, y, y_stride, 0};
   if (w.low + (uint64_t)c.parts * tokens * 64 * b.rank_tiles > w.bytes)   // parts_of and workspace_of belong together
     return mxi::fail(MX_ERR_STATE, "%s: %d parts of %d tokens exceed the workspace", who, c.parts, tokens);
   if (is_few(b, tokens)) return launch_few(c, f32, st);
@@ -1038,7 +1065,6 @@ int mx_adapters_apply(mx_adapters* a, const uint16_t* x, int64_t x_stride, const
   }
   if (plan) c.first = plan->first, c.row_pair = plan->row_pair;
   c.tiles = tiles_of(b, tokens);
-  c.stream = (int64_t)tokens * b.n * (f32 ? 6 : 4) > kStreamBytes;
   return launch_groups(c, f32, st);
 }
 

@@ -4,11 +4,15 @@
 // P = T k pairs p = t k + j; key(p) = ids[p] where that is in [0, G), else G. The plan is the stable order by key:
 //   row(p) = #{q: key(q) < key(p)} + #{q < p: key(q) = key(p)},   first[g] = #{q: key(q) < g}
 // so a group's rows are in ascending token order, as the reference's participation orders them
-// (src/vesper/moe.py:18-30), and pairs without a group come last. Everything is counted with ballots over the ids: no
-// atomics, the same plan on every run.
+// (src/vesper/moe.py:18-30), and pairs without a group come last. A pair's place comes from counts and ballots over the
+// ids (the only atomics add up counts), so the plan is the same on every run.
 //
 // combine adds a token's rows in ascending row (so ascending expert) order in FP32 from zero, the shared row last, and
 // rounds once: without weights the sums of MoEAccumulator (src/vesper/moe.py:42-148), bit for bit.
+//
+// All of it is memory traffic: each row is read once and written once, and the calls reach 5.4 to 5.9 TB/s of a plain
+// copy's 5.0 and a read's 6.9 on 4096 tokens of 8 rows of 7168 BF16 values. Small calls are one launch, 4 to 5 us from
+// the host.
 #include <algorithm>
 
 #include "mx_device.h"
@@ -21,7 +25,10 @@ constexpr int kMaxTokens = 1 << 18;   // keeps every grid below 2^32 threads
 constexpr int kMaxTopK = 32, kMaxGroups = 1024;
 constexpr int64_t kMaxWidth = 1 << 24;
 // Calls that move more than this go past the caches with what they touch once. The sum of a token counts only with all
-// its pairs here: an expert-parallel rank moves a fraction of what the host can tell.
+// its pairs here: an expert-parallel rank moves a fraction of what the host can tell. Through the caches and past them,
+// rows of 7168 BF16 values, 8 a token, three sets of buffers in turn: combine of 600 tokens 19.4 and 21.3 us, of 800
+// 26.2 and 25.2, of 4096 118 and 107; its gradient 400: 20.3 and 20.3, 600: 32.9 and 29.2; dispatch 600: 16.8 and 17.8,
+// 800: 25.0 and 22.5. 600 tokens are 77 MB (the gradient 146), 800 are 103.
 constexpr int64_t kStreamBytes = 96 << 20;
 
 // ---- plan ----
@@ -36,11 +43,13 @@ struct PlanArgs {
   int32_t* row_pair;
 };
 
-// Workgroup g places the pairs of key g (kAbsent: g = G, the pairs without a group). Each wave takes a contiguous section
-// of the pairs, 64 at a time: every lane counts the smaller keys and its own key among its pairs (as unsigned numbers,
-// ids below zero are no smaller key; pairs past the section count as ids past the last), and the second walk places the
-// key's pairs in order. kBatch loads are in flight together, and a section of one batch stays in registers for the
-// second walk. Every workgroup reads all the ids, from the L2s: what counts is the instructions per 64 of them.
+// Workgroup g places the pairs of key g (kAbsent: g = G, the pairs without a group). Each wave takes a contiguous
+// section of the pairs, 64 at a time: every lane counts the smaller keys and its own key among its pairs (as unsigned
+// numbers, ids below zero are no smaller key; pairs past the section count as ids past the last), and the second walk
+// places the key's pairs in order. kBatch loads are in flight together, and a section of one batch stays in registers
+// for the second walk: 8, 16 or 32 by the pairs (16384 pairs of 256 groups: 5.8 us with 16, 9.8 with 32). Every
+// workgroup reads all the ids, from the L2s: what counts is the instructions per 64 of them and the loads' latency
+// (32768 pairs: 8.9 us; with the ids counted by scalar code from ballots 17, with fewer loads in flight 21).
 template <bool kAbsent, int kBatch>
 __device__ __forceinline__ void place_key(const PlanArgs& a, int g, int (*sums)[2]) {
   const int tid = threadIdx.x, lane = tid & 63;
@@ -117,14 +126,14 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanArgs a) {
   else place_key<false, kBatch>(a, g, sums);
 }
 
-// Many pairs: the pairs in up to kMaxChunks contiguous chunks and three launches, work in proportion to the pairs and to
-// chunks x groups: count each chunk's keys; each chunk's first row of each group; place each chunk's pairs. There is no
-// workspace: a chunk's counts lie in its own part of row_pair and its first rows in its own part of pair_row, which its
-// workgroup has read before anyone writes there, so a chunk has at least G + 1 pairs.
+// Many pairs: the pairs in up to kMaxChunks contiguous chunks and three launches, work in proportion to the pairs and
+// to chunks x groups: count each chunk's keys; each chunk's first row of each group; place each chunk's pairs. There is
+// no workspace: a chunk's counts lie in its own part of row_pair and its first rows in its own part of pair_row, which
+// its workgroup has read before anyone writes there, so a chunk has at least G + 1 pairs.
 //
-// One launch against three, random ids, 8 a token: of 256 groups 32768 pairs 8.9 and 13.7 us, 131072 28 and 14, 2^21 383
-// and 31; of 1024 groups, whose workgroups are not all resident at once, 16384 pairs 12.7 and 17.7, 32768 20.7 and 18.1,
-// 2^23 3961 and 128.
+// One launch against three, random ids, 8 a token: of 256 groups 32768 pairs 8.9 and 13.7 us, 131072 28 and 14, 2^21
+// 383 and 31; of 1024 groups, whose workgroups are not all resident at once, 16384 pairs 12.7 and 17.7, 32768 20.7 and
+// 18.1, 2^23 3961 and 128.
 constexpr int kMaxChunks = 256, kChunkPairs = 2048;   // at least
 constexpr int kChunkedPairs = 3 << 14;                // above this over the walk's rounds (512 workgroups each)
 static_assert(kChunkPairs > kMaxGroups, "a chunk's part holds a number for every key");
@@ -211,8 +220,8 @@ __global__ __launch_bounds__(kPlanThreads) void plan_base_kernel(ChunkArgs a) {
     }
 }
 
-// A chunk's waves take a contiguous section each and count its keys; the next row of each key and wave then stands in LDS,
-// and 64 pairs at a time find their place among those of their key by a ballot for each bit of the key.
+// A chunk's waves take a contiguous section each and count its keys; the next row of each key and wave then stands in
+// LDS, and 64 pairs at a time find their place among those of their key by a ballot for each bit of the key.
 __global__ __launch_bounds__(kPlanThreads) void plan_place_kernel(ChunkArgs a, int bits) {
   extern __shared__ int next[];   // [kPlanWaves][groups + 1]
   const int tid = threadIdx.x, lane = tid & 63, groups = a.plan.groups;
@@ -301,12 +310,15 @@ struct DispatchArgs {
   float* row_weights;
 };
 
-// With the plan made in the same launch every workgroup counts for itself: a pair's key and index as one number,
-// key << 11 | p, orders the pairs, so row(p) is the count of smaller numbers and first[g] that of numbers below g << 11.
+// With the plan made in the same launch every workgroup counts for itself: a pair's key and index as one number, key <<
+// 11 | p, orders the pairs, so row(p) is the count of smaller numbers and first[g] that of numbers below g << 11. One
+// launch against the plan and the rows by it, 8 a token: 64 tokens 6.5 and 8.4 us, 128 8.1 and 9.1, 256 10.7 and 10.7,
+// 512 16.0 and 14.9; one token 5.3.
 constexpr int kIndexBits = 11, kFusedPairs = 1 << kIndexBits, kTargets = 8;
 
-// count[n] = how many pairs come before target[n], for up to kTargets targets at once (the others' are not used): a thread
-// holds P / 256 pairs, two counts share a register, and the waves' sums meet in LDS. `order` is this thread's pairs.
+// count[n] = how many pairs come before target[n], for up to kTargets targets at once (the others' are not used): a
+// thread holds P / 256 pairs, two counts share a register, and the waves' sums meet in LDS. `order` is this thread's
+// pairs.
 __device__ __forceinline__ void count_before(const uint32_t* order, int pairs, const uint32_t* target, int (*part)[kTargets],
                                              int* count) {
   const int tid = threadIdx.x;
@@ -340,7 +352,9 @@ __device__ __forceinline__ void count_before(const uint32_t* order, int pairs, c
 // The token's row is read once and written to each of its rows. U is the widest unit that the row's bytes and the
 // pointers allow.
 //
-// By a plan: one wave per token and piece of 64 units (chunks pieces a row; more units, more rounds).
+// By a plan: one wave per token and piece of 64 units (chunks pieces a row; more units, more rounds). 4096 tokens to 8
+// rows of 7168 BF16 values each: 90 us, 5.9 TB/s, against 72 for a fill of the same rows; with plain stores 104, with
+// loads past the caches too 108, a row's workgroup fetching its token 128, workgroups of 448 threads 93.
 template <typename U, bool kStream>
 __global__ __launch_bounds__(64) void move_rows_kernel(DispatchArgs a, int chunks) {
   const int t = blockIdx.x / chunks, chunk = blockIdx.x % chunks, lane = threadIdx.x, k = a.k, pairs = a.tokens * k;
@@ -358,8 +372,8 @@ __global__ __launch_bounds__(64) void move_rows_kernel(DispatchArgs a, int chunk
   }
 }
 
-// With the plan, in one launch for few pairs: grid (T + workgroups of kTargets groups, chunks); every workgroup finds its
-// own token's rows, the first chunk's writes them, and the workgroups past the tokens the groups' first rows.
+// With the plan, in one launch for few pairs: grid (T + workgroups of kTargets groups, chunks); every workgroup finds
+// its own token's rows, the first chunk's writes them, and the workgroups past the tokens the groups' first rows.
 template <typename U, bool kStream>
 __global__ __launch_bounds__(256) void dispatch_kernel(DispatchArgs a) {
   __shared__ int dst[kMaxTopK];
@@ -531,8 +545,9 @@ __device__ __forceinline__ void combine_units(const CombineArgs& a, int t, int64
 // value) a lane, up to eight rows in flight. Lane j holds the token's pair j; each counts the rows before its own and
 // sends it to the lane of that number.
 //
-// At most five waves a SIMD: 4096 x 8 rows of 7168 (529 MB read, 59 written) take 107 us with six or eight, 99 with five,
-// 101 with four and 104 with three, the unweighted sum 98 / 91 / 95 / 99.
+// Bound by HBM reads: 4096 x 8 rows of 7168 (529 MB read, 59 written) take 99 us, 5.9 TB/s. At most five waves a SIMD,
+// so that the rows in flight fit what the memory takes in order: six or eight 107, four 101, three 104; the unweighted
+// sum 98 / 91 / 95 / 99.
 template <int kType, int V>
 __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(1, 5))) void combine_kernel(CombineArgs a, int chunks) {
   const int t = blockIdx.x / chunks, chunk = blockIdx.x % chunks, lane = threadIdx.x, k = a.k, pairs = a.tokens * k;
@@ -614,10 +629,11 @@ __device__ __forceinline__ float backward_units(const CombineBwdArgs& a, int t, 
   return dot;
 }
 
-// One workgroup a pair: drows[row] = w dy[t] and dw = <rows[row], dy[t]>, both from one read of dy and of the row.
-// Each thread adds its products in order, the lanes are added as a tree and the waves in order.
-// A token's pairs run on one XCD (workgroups go round the eight of them), so its dy comes from HBM once and from that L2
-// after.
+// One workgroup a pair: drows[row] = w dy[t] and dw = <rows[row], dy[t]>, both from one read of dy and of the row. Each
+// thread adds its products in order, the lanes are added as a tree and the waves in order. A token's pairs run on one
+// XCD (workgroups go round the eight of them), so its dy comes from HBM once and from that L2 after. 4096 x 8 rows of
+// 7168 BF16 values (998 MB): 178 us, 5.6 TB/s; pairs in plain order 195, rows read through the caches 189, gradients
+// written through them 195; two units a thread of 512 instead of four of 256: 181.
 template <int kType, int V>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 5))) void combine_backward_kernel(CombineBwdArgs a) {
   __shared__ float part[4];
