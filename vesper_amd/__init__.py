@@ -17,6 +17,9 @@ reference's interface for this path:
   integrity.DeviceIntegrity                   src/vesper/integrity.py
   conformance.compare + format hooks          src/vesper/conformance.py
   layer.ExpertBank / MoELayer                 batched decode entry (T <= 16 tokens per call)
+  dispatch.ExpertDispatch                     tokens sorted by expert and back, with gradients (batched moe.py)
+  adapters.AdapterBank                        low-rank adapters of many requests beside a projection
+                                              (projections.NativeProjections.open_adapters)
 """
 
 from .config import BASELINE, REFERENCE, MoEConfig

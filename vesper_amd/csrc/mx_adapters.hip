@@ -516,20 +516,27 @@ __global__ __launch_bounds__(256, 2) void adapter_down_kernel(Call c, int rank_g
   }
 }
 
-// Grouped form of more than 16 ranks: the parts of four ranks of a token added in order, as operand B in the first
-// part's place. A launch of its own, 3 to 5 us: in up every workgroup of a tile would add them anew, which 4096 tokens
-// of rank 64 pay with 18 us and 3056 beside 24576 rows with 41, and even rank 32 with 1. Of up to 16 ranks up does it:
-// 1010 tokens of rank 8 12.1 us in all, with this launch 14.0.
+// Grouped form of more than 16 ranks: the parts of four ranks of a token added, as operand B in the first part's place;
+// more than eight of them, which a thread has in flight at once, by four lanes whose sums are added as a tree. A launch
+// of its own, 3 to 5 us: in up every workgroup of a tile would add them anew, which 4096 tokens of rank 64 pay with 18
+// us and 3056 beside 24576 rows with 41, and even rank 32 with 1. Of up to 16 ranks up does it: 1010 tokens of rank 8
+// 12.1 us in all, with this launch 14.0.
+template <int kShares>
 __global__ __launch_bounds__(256) void adapter_sum_kernel(Call c) {
   const Bank& b = c.bank;
-  const int per = 4 * b.rank_tiles;   // entries of a token
-  const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (e >= (int64_t)c.tokens * per) return;
-  float* p = c.low + 4 * e;
-  const v4f s = sum_parts(p, (int64_t)c.tokens * 4 * per, 0, 1, c.parts);
-  const int id = c.ids[e / per], r0 = 4 * (int)(e % per);
-  if (id < 0 || id >= b.slots) return;   // the sums of a token without an adapter, or past a slot's rank, are no one's
-  *(uint4*)p = h_operand(b.table[id], r0, s);
+  const int per = 4 * b.rank_tiles, share = (threadIdx.x & 63) / (64 / kShares);   // entries of a token
+  const int e = (blockIdx.x * 256 + (threadIdx.x & ~63)) / kShares + threadIdx.x % (64 / kShares);
+  if (e >= c.tokens * per) return;
+  const int id = c.ids[e / per];
+  const bool held = id >= 0 && id < b.slots;   // the sums of a token without an adapter, or past a slot's rank, are no one's
+  const AdapterSlot slot = b.table[held ? id : 0];
+  float* p = c.low + 4 * (int64_t)e;
+  v4f s = sum_parts(p, (int64_t)c.tokens * 4 * per, share, kShares, c.parts);
+#pragma unroll
+  for (int d = 64 / kShares; d < 64; d <<= 1)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s[i] = s[i] + __shfl_xor(s[i], d, 64);
+  if (held && share == 0) *(uint4*)p = h_operand(slot, 4 * (e % per), s);
 }
 
 // ---- up: y = base + up h ----
@@ -947,8 +954,9 @@ int launch_groups(const Call& c, bool f32, hipStream_t st) {
                         : (stream ? launch_down<4, true>(c, st) : launch_down<4, false>(c, st)))
     return s;
   if (c.parts > 1 && rt > 1) {
-    const int64_t entries = (int64_t)c.tokens * 4 * rt;
-    hipLaunchKernelGGL(adapter_sum_kernel, dim3((unsigned)((entries + 255) / 256)), dim3(256), 0, st, c);
+    const int entries = c.tokens * 4 * rt;
+    if (c.parts > 8) hipLaunchKernelGGL(adapter_sum_kernel<4>, dim3((entries + 63) / 64), dim3(256), 0, st, c);
+    else hipLaunchKernelGGL(adapter_sum_kernel<1>, dim3((entries + 255) / 256), dim3(256), 0, st, c);
     MX_LAUNCH_CHECK("adapter_sum_kernel");
   }
   if (rt == 1) return launch_up<1>(c, f32, st);
