@@ -40,10 +40,13 @@ constexpr int kFewTokens = 128;    // a wave holds the ids of this many tokens, 
 constexpr int kTileTokens = 64;    // tokens of a workgroup in the grouped form
 constexpr int kColumns = kTileTokens / 16;
 constexpr int kMaxParts = 32;      // parts of K
-// KB of down up to which a call of few tokens is one launch (each of its workgroups reads all of down). One launch and
-// two, one token: 1536 columns of rank 16 (48 KB) 5.0 and 7.4 us, 7168 of rank 16 (224 KB) 6.0 and 7.0, 7168 of rank 32
-// (448 KB) 7.8 and 7.0, 16384 of rank 16 (512 KB) 10.3 and 7.0. Four rank tiles take too many registers: 10.2 and 7.1.
-constexpr int kFusedChunks = 256;
+// A call of few tokens is one launch if down and the x of its tokens (of 64 at most, since the tokens of a workgroup are 16
+// of one adapter) are no more than this: each of its workgroups reads all of down. One launch and two, rank 12 (one rank
+// tile) of K columns, tokens of adapters: K = 1536, 1 of 1 5.0 and 7.4 us, 16 of 16 7.1 and 9.4, 120 of 2 13.4 and 15.4;
+// 5120, 1 of 1 5.5 and 7.4, 16 of 4 6.6 and 7.7, 40 of 9 7.4 and 8.1, 64 of 3 10.0 and 8.2; 7168, 4 of 4 6.7 and 7.6, 16
+// of 1 9.7 and 7.6, of 16 7.2 and 7.8, 64 of 3 12.2 and 8.2; 16384, 1 of 1 10.3 and 7.0. Rank 32: 1536, 120 of 2 16.3 and
+// 17.2; 7168, 1 of 1 7.8 and 7.0. Four rank tiles take too many registers: 10.2 and 7.1.
+constexpr int kFusedBytes = 320 << 10;
 // Calls whose x, base and y exceed this read x past the caches, which leaves them to the weights, base and y. Past them
 // and through, three sets in turn, 8 adapters of rank 64 or 32: 1000 tokens of 16384 to 7168 (62 MB) 30.6 and 31.0 us,
 // 1500 (92 MB) 33.8 and 37.7, 2000 (123 MB) 43.3 and 48.5, 4096 (252 MB) 72.9 and 72.3; 2500 of 7168 to 1536 (51 MB)
@@ -911,7 +914,7 @@ int launch_fused(const Call& c, bool f32, hipStream_t st) {
 
 int launch_few(const Call& c, bool f32, hipStream_t st) {
   const int rt = c.bank.rank_tiles;
-  if (rt <= 2 && rt * c.bank.chunks <= kFusedChunks)
+  if (rt <= 2 && (16 * rt + std::min(c.tokens, 64)) * c.bank.chunks <= kFusedBytes / 64)
     return rt == 1 ? launch_fused<1>(c, f32, st) : launch_fused<2>(c, f32, st);
   hipLaunchKernelGGL((rt == 1   ? adapter_few_down_kernel<1>
                       : rt == 2 ? adapter_few_down_kernel<2>
