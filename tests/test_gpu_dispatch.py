@@ -361,7 +361,7 @@ def test_experts_between_dispatch_and_combine_are_the_layer(gpu_ctx):
     bank.free()
 
 
-@pytest.mark.parametrize("tokens", [3, 400])
+@pytest.mark.parametrize("tokens", [3, 400, 7000])
 def test_captured_passes_replay_on_new_inputs(gpu_ctx, tokens):
     """Forward and backward captured once on a stream of their own; each replay reads what the buffers then hold."""
     k, e, width = 8, 20, 136

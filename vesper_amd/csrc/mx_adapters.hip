@@ -404,6 +404,7 @@ __global__ __launch_bounds__(256) void adapter_few_down_kernel(Call c) {
 // apart and the pairs 1040, and a second row's 16-byte pieces are swapped in halves of 128 bytes, so that the 16 rows
 // of an operand read lie in different banks.
 constexpr int kStageK = 256, kPairBytes = 1040, kStageBytes = kTileTokens / 2 * kPairBytes;
+static_assert(4 * kOwnLds <= 2 * kStageBytes, "the counts lie where the stages come after them");
 
 template <int RT, bool kStream>
 __global__ __launch_bounds__(256, 2) void adapter_down_kernel(Call c, int rank_groups) {
