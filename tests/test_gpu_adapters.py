@@ -176,8 +176,8 @@ def test_slots_are_replaced_and_emptied(gpu_ctx):
         check(bank.apply(x, ids, base), x, ids, base, adapters, True)
 
 
-def test_the_result_does_not_depend_on_a_calls_other_tokens(gpu_ctx):
-    """The same tokens in any order, with any neighbours of the same form, give the same bits."""
+def test_the_result_does_not_depend_on_the_tokens_order(gpu_ctx):
+    """A call's tokens in any order, and the same call again, give the same bits."""
     rng = np.random.default_rng(14)
     rows, width = 200, 1024
     for tokens in (20, 100, 300):
@@ -282,18 +282,21 @@ def test_two_banks_on_two_streams_by_one_plan(gpu_ctx):
         idd.free()
 
 
-def test_most_slots(gpu_ctx):
-    """1024 slots of which the last is used, by many tokens and by few; tiles of two tokens each."""
-    rng = np.random.default_rng(8)
-    rows, width, slots = 40, 72, 1024
-    with AdapterBank(gpu_ctx, rows, width, slots, 4, 2100) as bank:
-        adapters = {s: adapter(rng, rows, width, 4, True) for s in range(0, slots, 31)}
+@pytest.mark.parametrize("max_rank,dtype", [(4, "bf16"), (24, "f32"), (50, "bf16"), (100, "f32"), (200, "bf16")])
+def test_most_slots(gpu_ctx, max_rank, dtype):
+    """1024 slots. Many groups of two tokens, which make more tiles than the tokens would full ones; and all tokens of
+    the last slot and one other, where nearly all groups that there could be make none."""
+    rng = np.random.default_rng(max_rank)
+    rows, width, slots = 8200, 72, 1024
+    with AdapterBank(gpu_ctx, rows, width, slots, max_rank, 2100) as bank:
+        adapters = {s: adapter(rng, rows, width, max_rank, True) for s in (*range(0, slots, 93), slots - 1)}
         fill(bank, rng, adapters)
         for tokens in (20, 2100):
-            ids = (np.arange(tokens) % slots).astype(np.int32)
-            ids[::3] = slots - 1
-            x, base = inputs(rng, tokens, rows, width, True, "bf16")
-            check(bank.apply(x, ids, base), x, ids, base, adapters, True)
+            x, base = inputs(rng, tokens, rows, width, True, dtype)
+            many = (np.arange(tokens) % slots).astype(np.int32)
+            many[::3] = slots - 1
+            for ids in (many, np.where(np.arange(tokens) % 5, slots - 1, 93).astype(np.int32)):
+                check(bank.apply(x, ids, base), x, ids, base, adapters, True)
 
 
 def test_call_refusals(gpu_ctx):

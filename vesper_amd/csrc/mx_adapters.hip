@@ -40,12 +40,12 @@ constexpr int kFewTokens = 128;    // a wave holds the ids of this many tokens, 
 constexpr int kTileTokens = 64;    // tokens of a workgroup in the grouped form
 constexpr int kColumns = kTileTokens / 16;
 constexpr int kMaxParts = 32;      // parts of K
-// A call of few tokens is one launch if down and the x of its tokens (of 64 at most, since the tokens of a workgroup are 16
-// of one adapter) are no more than this: each of its workgroups reads all of down. One launch and two, rank 12 (one rank
-// tile) of K columns, tokens of adapters: K = 1536, 1 of 1 5.0 and 7.4 us, 16 of 16 7.1 and 9.4, 120 of 2 13.4 and 15.4;
-// 5120, 1 of 1 5.5 and 7.4, 16 of 4 6.6 and 7.7, 40 of 9 7.4 and 8.1, 64 of 3 10.0 and 8.2; 7168, 4 of 4 6.7 and 7.6, 16
-// of 1 9.7 and 7.6, of 16 7.2 and 7.8, 64 of 3 12.2 and 8.2; 16384, 1 of 1 10.3 and 7.0. Rank 32: 1536, 120 of 2 16.3 and
-// 17.2; 7168, 1 of 1 7.8 and 7.0. Four rank tiles take too many registers: 10.2 and 7.1.
+// A call of few tokens is one launch if down and the x of its tokens (of 64 at most, since the tokens of a workgroup
+// are 16 of one adapter) are no more than this: each of its workgroups reads all of down. One launch and two, rank 12
+// (one rank tile) of K columns, tokens of adapters: K = 1536, 1 of 1 5.0 and 7.4 us, 16 of 16 7.1 and 9.4, 120 of 2
+// 13.4 and 15.4; 5120, 1 of 1 5.5 and 7.4, 16 of 4 6.6 and 7.7, 40 of 9 7.4 and 8.1, 64 of 3 10.0 and 8.2; 7168, 4 of 4
+// 6.7 and 7.6, 16 of 1 9.7 and 7.6, of 16 7.2 and 7.8, 64 of 3 12.2 and 8.2; 16384, 1 of 1 10.3 and 7.0. Rank 32: 1536,
+// 120 of 2 16.3 and 17.2; 7168, 1 of 1 7.8 and 7.0. Four rank tiles take too many registers: 10.2 and 7.1.
 constexpr int kFusedBytes = 320 << 10;
 // Calls whose x, base and y exceed this read x past the caches, which leaves them to the weights, base and y. Past them
 // and through, three sets in turn, 8 adapters of rank 64 or 32: 1000 tokens of 16384 to 7168 (62 MB) 30.6 and 31.0 us,
@@ -106,6 +106,14 @@ __global__ __launch_bounds__(128) void adapter_store_up_kernel(Bank b, uint8_t* 
   *(uint4*)dst = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+// threadIdx.x, of which the compiler keeps nothing from one turn of a workgroup's loop to the next: the addresses of a
+// second turn, which few calls have, would take 30 registers of the first.
+__device__ __forceinline__ int thread_here() {
+  int tid = threadIdx.x;
+  asm volatile("" : "+v"(tid));
+  return tid;
+}
+
 // ---- the tokens of a workgroup ----
 
 struct Tile {
@@ -119,7 +127,7 @@ struct Call {
   const int32_t* ids;
   const int32_t* first;      // grouped form: the plan of ids (slots groups), or null: every workgroup counts for itself
   const int32_t* row_pair;
-  Tile* tile;                // grouped form: what down found, for up: the tiles
+  Tile* tile;                // grouped form: what down found, for up: the tiles, then {parts, tiles},
   int32_t* tile_token;       // and the tokens of their 64 columns
   int32_t tokens, parts;
   float* low;                // [parts][T][16 rank_tiles]: partial sums of down x
@@ -127,113 +135,166 @@ struct Call {
   int64_t base_stride;
   uint16_t* y;
   int64_t y_stride;
-  int32_t tiles;             // grouped form: the most tiles that there can be
+  int32_t tiles;             // grouped form: the most tiles that there can be; parts: the most parts
 };
 
-// Which of the groups' tiles is number `index`: kTileTokens tokens of a group each (a group's last one short), the
-// tokens without an adapter last as group `slots`. count(g) gives the tokens of a group; 64 groups at a time.
-struct Place {
-  int group, skip, rows;   // rows = 0 past the last tile; else tokens kTileTokens skip .. of the group
+// Workgroups go round the eight XCDs; this numbers them so that each XCD takes a contiguous range of `count`.
+__device__ __forceinline__ int on_xcd(int id, int count) { return (id & 7) * ((count + 7) >> 3) + (id >> 3); }
+
+// What a workgroup of down does: a part of K and a group of rank tiles for a tile. The split of K follows the tiles
+// that there are, which only the device knows: the slots that no token names make none (600 tokens of 8 adapters of
+// rank 64 by 16384 in a bank of 1024 slots 27 us, split by the tiles that there could be 78).
+struct Work {
+  Tile tile;
+  int index, part, rank_group;   // index -1: nothing
+  int tiles, parts;
 };
 
-template <typename Count>
-__device__ __forceinline__ Place find_tile(int slots, int index, Count count) {
-  const int lane = threadIdx.x & 63;
-  int before = 0;
-  Place t{0, 0, 0};
-  for (int g0 = 0; g0 <= slots; g0 += 64) {
-    const int n = g0 + lane <= slots ? count(g0 + lane) : 0, tiles = (n + kTileTokens - 1) / kTileTokens;
-    int upto = tiles;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int o = __shfl_up(upto, d, 64);
-      if (lane >= d) upto += o;
-    }
-    const int total = __shfl(upto, 63, 64);
-    if (index < before + total) {
-      const int at = __ffsll((unsigned long long)__ballot(upto > index - before)) - 1;
-      const int skip = index - before - (__shfl(upto, at, 64) - __shfl(tiles, at, 64));
-      t = Place{g0 + at, skip, min(kTileTokens, __shfl(n, at, 64) - skip * kTileTokens)};
-      break;
-    }
-    before += total;
-  }
-  return Place{__builtin_amdgcn_readfirstlane(t.group), __builtin_amdgcn_readfirstlane(t.skip),
-               __builtin_amdgcn_readfirstlane(t.rows)};
+// Piece `id` of down's work over `tiles` tiles; each XCD has a contiguous range of it, part by part.
+__device__ __forceinline__ Work split(const Call& c, int id, int tiles, int rank_groups) {
+  Work w;
+  w.tile = Tile{-1, 0};
+  w.tiles = min(tiles, c.tiles);
+  w.parts = min(c.parts, max(kWantGroups / max(w.tiles, 1), 1));
+  const int count = w.parts * w.tiles * rank_groups, piece = on_xcd(id, count);
+  w.index = -1;
+  w.part = w.rank_group = 0;
+  if (id >= (count + 7) / 8 * 8 || piece >= count) return w;
+  const int tile = rank_groups == 1 ? piece : piece / rank_groups;
+  w.rank_group = piece - tile * rank_groups;
+  w.part = tile / w.tiles;
+  w.index = tile - w.part * w.tiles;
+  return w;
 }
 
-// Tile `index` by the plan of ids; `token` is that of this lane's column (those past the last repeat it).
-__device__ __forceinline__ Tile plan_tile(const Call& c, int index, int& token) {
+// Piece `id` of the groups' tiles: kTileTokens tokens of a group each (a group's last one short), the tokens without an
+// adapter last as group `slots`; count(g) gives the tokens of a group. Thread i of the workgroup has the groups from
+// i `per` on. place: the tile's group and the place in it of its first token.
+constexpr int kThreadGroups = kMaxSlots / 256 + 1;
+
+template <typename Count>
+__device__ __forceinline__ Work locate(const Call& c, int id, int rank_groups, Count count, int (&found)[8], int2& place) {
+  const int tid = threadIdx.x, lane = tid & 63, slots = c.bank.slots, per = (slots + 256) / 256, first = tid * per;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  int n[kThreadGroups], mine = 0;
+#pragma unroll
+  for (int i = 0; i < kThreadGroups; ++i)
+    if (i < per) {
+      n[i] = first + i <= slots ? count(first + i) : 0;
+      mine += (n[i] + kTileTokens - 1) / kTileTokens;
+    }
+  int upto = mine;   // of the wave's threads up to this one
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int o = __shfl_up(upto, d, 64);
+    if (lane >= d) upto += o;
+  }
+  if (lane == 63) found[4 + wave] = upto;
+  __syncthreads();
+  int total = 0, before = upto - mine;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    before += w < wave ? found[4 + w] : 0;
+    total += found[4 + w];
+  }
+  Work work = split(c, id, __builtin_amdgcn_readfirstlane(total), rank_groups);
+  if (work.index < 0) return work;
+  if (work.index >= before && work.index < before + mine) {
+    int skip = work.index - before;
+#pragma unroll
+    for (int i = 0; i < kThreadGroups; ++i)
+      if (i < per) {
+        const int tiles = (n[i] + kTileTokens - 1) / kTileTokens;
+        if (skip >= 0 && skip < tiles) {
+          found[0] = first + i;
+          found[1] = skip * kTileTokens;
+          found[2] = min(kTileTokens, n[i] - skip * kTileTokens);
+        }
+        skip -= tiles;
+      }
+  }
+  __syncthreads();
+  place.x = __builtin_amdgcn_readfirstlane(found[0]);
+  place.y = __builtin_amdgcn_readfirstlane(found[1]);
+  work.tile = Tile{place.x < slots ? place.x : -1, __builtin_amdgcn_readfirstlane(found[2])};
+  return work;
+}
+
+// Piece `id` by the plan of ids; `token` is that of this lane's column (those past the last repeat it).
+__device__ __forceinline__ Work plan_work(const Call& c, int id, int rank_groups, int (&found)[8], int& token) {
   const int slots = c.bank.slots;
   auto begin = [&](int g) { return min(max(c.first[g], 0), c.tokens); };
-  const Place t = find_tile(slots, index, [&](int g) {
+  int2 place;
+  const Work work = locate(c, id, rank_groups, [&](int g) {
     const int lo = begin(g);
     return (g < slots ? max(begin(g + 1), lo) : c.tokens) - lo;
-  });
-  if (t.rows > 0) {
-    const int row = begin(t.group) + t.skip * kTileTokens + min((int)(threadIdx.x & 63), t.rows - 1);
+  }, found, place);
+  if (work.index >= 0) {
+    const int row = begin(place.x) + place.y + min((int)(threadIdx.x & 63), work.tile.rows - 1);
     token = c.row_pair[min(row, c.tokens - 1)];
     token = token >= 0 && token < c.tokens ? token : 0;
   }
-  return Tile{t.group < slots ? t.group : -1, t.rows};
+  return work;
 }
 
 // The same from the ids themselves, by a workgroup of four waves for itself: it counts the groups in `lds`, finds its
 // tile and picks out the tile's tokens in ascending order. The waves hold the ids, a contiguous section each. About 2
-// us in each round of workgroups, where the plan is a launch of 5: 1000 tokens of 8 adapters of rank 32 17.8 us, by a
-// plan 20.0; 4096 of rank 64 72.9 and 73.9; 4000 of rank 256, in four rank groups, 157 and 156.
+// us in each round of workgroups, where the plan is a launch of 5 and 1 more to read it: 1000 tokens of 8 adapters of
+// rank 32 17.8 us, by a plan made for the call 20.0; 4096 of rank 64 72.9 and 73.9; 4000 of rank 256, in four rank
+// groups, 157 and 156.
 constexpr int kOwnIds = 16, kOwnTokens = 4 * 64 * kOwnIds;
 constexpr int kCopies = 8;   // of each count, by lane: neighbours of one group take few turns at one of them
 constexpr int kOwnLds = (kMaxSlots + 1) * kCopies + 4 + kTileTokens;   // numbers
 
-__device__ __forceinline__ Tile own_tile(const Call& c, int index, int* lds, int& token) {
+__device__ __forceinline__ Work own_work(const Call& c, int id, int rank_groups, int (&found)[8], int* lds,
+                                         int& token) {
   const int tid = threadIdx.x, lane = tid & 63, slots = c.bank.slots;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   int* count = lds;
   int* part = lds + (kMaxSlots + 1) * kCopies;
   int* list = part + 4;
   const int section = (c.tokens + 255) / 256 * 64, p0 = wave * section + lane;
-  int id[kOwnIds];   // -1: past the last token; tokens without an adapter are group `slots`
+  int key[kOwnIds];   // -1: past the last token; tokens without an adapter are group `slots`
 #pragma unroll
   for (int i = 0; i < kOwnIds; ++i)
-    if (64 * i < section) id[i] = c.ids[min(p0 + 64 * i, c.tokens - 1)];
+    if (64 * i < section) key[i] = c.ids[min(p0 + 64 * i, c.tokens - 1)];
   for (int n = tid; n < (slots + 1) * (kCopies / 4); n += 256) ((uint4*)count)[n] = make_uint4(0, 0, 0, 0);
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < kOwnIds; ++i)
     if (64 * i < section) {
-      id[i] = p0 + 64 * i >= c.tokens ? -1 : id[i] >= 0 && id[i] < slots ? id[i] : slots;
-      if (id[i] >= 0) atomicAdd(&count[id[i] * kCopies + lane % kCopies], 1);
+      key[i] = p0 + 64 * i >= c.tokens ? -1 : key[i] >= 0 && key[i] < slots ? key[i] : slots;
+      if (key[i] >= 0) atomicAdd(&count[key[i] * kCopies + lane % kCopies], 1);
     }
   __syncthreads();
-  const Place t = find_tile(slots, index, [&](int g) {
+  int2 place;
+  const Work work = locate(c, id, rank_groups, [&](int g) {
     int n = 0;
 #pragma unroll
     for (int i = 0; i < kCopies; ++i) n += count[g * kCopies + i];
     return n;
-  });
-  if (t.rows > 0) {
-    int own = 0;
+  }, found, place);
+  if (work.index < 0) return work;
+  int own = 0;
 #pragma unroll
-    for (int i = 0; i < kOwnIds; ++i)
-      if (64 * i < section) own += __popcll(__ballot(id[i] == t.group));
-    if (lane == 0) part[wave] = own;
-    __syncthreads();
-    int at = -t.skip * kTileTokens;
-    for (int w = 0; w < wave; ++w) at += part[w];
+  for (int i = 0; i < kOwnIds; ++i)
+    if (64 * i < section) own += __popcll(__ballot(key[i] == place.x));
+  if (lane == 0) part[wave] = own;
+  __syncthreads();
+  int at = -place.y;
+  for (int w = 0; w < wave; ++w) at += part[w];
 #pragma unroll
-    for (int i = 0; i < kOwnIds; ++i)
-      if (64 * i < section) {
-        const uint64_t mask = __ballot(id[i] == t.group);
-        const int place = at + __popcll(mask & ((1ull << lane) - 1));
-        if (id[i] == t.group && place >= 0 && place < kTileTokens) list[place] = p0 + 64 * i;
-        at += __popcll(mask);
-      }
-    __syncthreads();
-    token = list[min(lane, t.rows - 1)];
-    __syncthreads();
-  }
-  return Tile{t.group < slots ? t.group : -1, t.rows};
+  for (int i = 0; i < kOwnIds; ++i)
+    if (64 * i < section) {
+      const uint64_t mask = __ballot(key[i] == place.x);
+      const int column = at + __popcll(mask & ((1ull << lane) - 1));
+      if (key[i] == place.x && column >= 0 && column < kTileTokens) list[column] = p0 + 64 * i;
+      at += __popcll(mask);
+    }
+  __syncthreads();
+  token = list[min(lane, work.tile.rows - 1)];
+  __syncthreads();   // before the stages
+  return work;
 }
 
 // Few tokens: the workgroups of token t take the tokens of t's adapter, up to 16 a workgroup. The first of each 16 does
@@ -271,9 +332,6 @@ __device__ __forceinline__ Few few_tokens(const Call& c, int t) {
   const int low = __shfl(id[0], column, 64), high = __shfl(id[1], column, 64);
   return Few{slot, rows, before + column < first ? low : high};
 }
-
-// Workgroups go round the eight XCDs; this numbers them so that each XCD takes a contiguous range of `count`.
-__device__ __forceinline__ int on_xcd(int id, int count) { return (id & 7) * ((count + 7) >> 3) + (id >> 3); }
 
 // Four ranks of h, from r0 on, as operand B's K slots: bf16(scale s), then bf16 of what that leaves.
 __device__ __forceinline__ uint4 h_operand(const AdapterSlot& slot, int r0, v4f s) {
@@ -407,26 +465,17 @@ constexpr int kStageK = 256, kPairBytes = 1040, kStageBytes = kTileTokens / 2 * 
 static_assert(4 * kOwnLds <= 2 * kStageBytes, "the counts lie where the stages come after them");
 
 template <int RT, bool kStream>
-__global__ __launch_bounds__(256, 2) void adapter_down_kernel(Call c, int rank_groups) {
-  extern __shared__ uint4 stage_lds[];   // two stages; then the waves' sums [4][kColumns][RT][64]
+__device__ __forceinline__ void down_piece(const Call& c, const Work& work, int tokens, uint4* stage_lds) {
   const Bank& b = c.bank;
-  const int work = on_xcd(blockIdx.x, c.parts * c.tiles * rank_groups);
-  const int part = work / (c.tiles * rank_groups), r0 = RT * (work % rank_groups), index = work / rank_groups % c.tiles;
-  if (part >= c.parts) return;
-  int tokens = 0;
-  const Tile t = c.first ? plan_tile(c, index, tokens) : own_tile(c, index, (int*)stage_lds, tokens);
-  if (part == 0 && r0 == 0) {
-    if (threadIdx.x < 64) c.tile_token[index * kTileTokens + threadIdx.x] = tokens;
-    if (threadIdx.x == 0) c.tile[index] = t;
-  }
-  if (t.rows == 0 || t.slot < 0) return;
+  const Tile t = work.tile;
+  const int part = work.part, r0 = RT * work.rank_group;
   const AdapterSlot slot = b.table[t.slot];
   const int tiles = (slot.rank + 15) >> 4;
   if (r0 >= tiles) return;
   const int tid = threadIdx.x, lane = tid & 63, q = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int stages = (b.k + kStageK - 1) / kStageK, units = b.chunks / 2;
-  const int s0 = (int)((int64_t)stages * part / c.parts), s1 = (int)((int64_t)stages * (part + 1) / c.parts);
+  const int s0 = (int)((int64_t)stages * part / work.parts), s1 = (int)((int64_t)stages * (part + 1) / work.parts);
   const uint32_t lds = mxd::lds_addr(stage_lds);
   const int piece = (lane & 31) ^ (lane >> 5 << 3);   // of its row that this lane copies
   const uint8_t* src[kColumns * 2];
@@ -520,6 +569,25 @@ __global__ __launch_bounds__(256, 2) void adapter_down_kernel(Call c, int rank_g
   }
 }
 
+template <int RT, bool kStream>
+__global__ __launch_bounds__(256, 2) void adapter_down_kernel(Call c, int rank_groups) {
+  extern __shared__ uint4 stage_lds[];   // two stages; then the waves' sums [4][kColumns][RT][64]
+  __shared__ int found[8];   // the tile's group, its first token's place in it, its tokens; then the waves' tiles
+  int tokens = 0;
+  const Work work = c.first ? plan_work(c, blockIdx.x, rank_groups, found, tokens)
+                            : own_work(c, blockIdx.x, rank_groups, found, (int*)stage_lds, tokens);
+  if (blockIdx.x == 0) {
+    if (threadIdx.x == 0) c.tile[c.tiles] = Tile{work.parts, work.tiles};
+    for (int i = work.tiles + threadIdx.x; i < c.tiles; i += 256) c.tile[i] = Tile{-1, 0};
+  }
+  if (work.index < 0) return;
+  if (work.part == 0 && work.rank_group == 0) {
+    if (threadIdx.x < 64) c.tile_token[work.index * kTileTokens + threadIdx.x] = tokens;
+    if (threadIdx.x == 0) c.tile[work.index] = work.tile;
+  }
+  if (work.tile.rows > 0 && work.tile.slot >= 0) down_piece<RT, kStream>(c, work, tokens, stage_lds);
+}
+
 // Grouped form of more than 16 ranks: the parts of four ranks of a token added, as operand B in the first part's place;
 // more than eight of them, which a thread has in flight at once, by four lanes whose sums are added as a tree. A launch
 // of its own, 3 to 5 us: in up every workgroup of a tile would add them anew, which 4096 tokens of rank 64 pay with 18
@@ -535,7 +603,7 @@ __global__ __launch_bounds__(256) void adapter_sum_kernel(Call c) {
   const bool held = id >= 0 && id < b.slots;   // the sums of a token without an adapter, or past a slot's rank, are no one's
   const AdapterSlot slot = b.table[held ? id : 0];
   float* p = c.low + 4 * (int64_t)e;
-  v4f s = sum_parts(p, (int64_t)c.tokens * 4 * per, share, kShares, c.parts);
+  v4f s = sum_parts(p, (int64_t)c.tokens * 4 * per, share, kShares, min(c.tile[c.tiles].slot, c.parts));
 #pragma unroll
   for (int d = 64 / kShares; d < 64; d <<= 1)
 #pragma unroll
@@ -756,17 +824,12 @@ __global__ __launch_bounds__(1024) void adapter_few_kernel(Call c) {
 // base and y: 4096 tokens of 7168 outputs (117 MB) 30 us, 3056 of 24576 (300 MB) 69; with accesses of 64 bytes the
 // first 37.
 template <int RT, bool kF32>
-__global__ __launch_bounds__(256) void adapter_up_kernel(Call c) {
-  __shared__ uint4 h_lds[kColumns * RT * 64];
+__device__ __forceinline__ void up_blocks(const Call& c, int index, const Tile& t, int group, int parts, int tid, uint4* h_lds) {
   const Bank& b = c.bank;
-  const int groups = (b.blocks + 3) / 4, group = blockIdx.x % groups;
-  const int index = blockIdx.x / groups;
-  const Tile t = c.tile[index];
-  if (t.rows == 0) return;
-  const int tokens = c.tile_token[index * kTileTokens + (threadIdx.x & 63)];
+  const int tokens = c.tile_token[index * kTileTokens + (tid & 63)];
   const AdapterSlot slot = t.slot >= 0 ? b.table[t.slot] : AdapterSlot{0, 0.f};
   const int tiles = (slot.rank + 15) >> 4;
-  const int tid = threadIdx.x, lane = tid & 63, q = lane >> 4;
+  const int lane = tid & 63, q = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int block = 4 * group + wave, n = 64 * block + 8 * q;   // past the last block: no output is a lane's
   // every load below goes out before the first of them is waited for; lanes without an output repeat another's address
@@ -807,7 +870,7 @@ __global__ __launch_bounds__(256) void adapter_up_kernel(Call c) {
       }
     }
   if constexpr (RT == 1)
-    if (c.parts > 1 && tiles) h[0] = h_operand(slot, 4 * q, sum_parts(low_h, c.tokens * rank_stride, 0, 1, c.parts));
+    if (c.parts > 1 && tiles) h[0] = h_operand(slot, 4 * q, sum_parts(low_h, c.tokens * rank_stride, 0, 1, parts));
 #pragma unroll
   for (int r = 0; r < RT; ++r) {
     const int ranks = slot.rank - 16 * r - 4 * q;   // the sums past the slot's rank are not its own
@@ -850,6 +913,23 @@ __global__ __launch_bounds__(256) void adapter_up_kernel(Call c) {
   }
 }
 
+// kTurns: for fewer workgroups than there can be tiles.
+template <int RT, bool kF32, bool kTurns>
+__global__ __launch_bounds__(256) void adapter_up_kernel(Call c) {
+  __shared__ uint4 h_lds[kColumns * RT * 64];
+  const int groups = (c.bank.blocks + 3) / 4, group = blockIdx.x % groups;
+  int index = blockIdx.x / groups;
+  Tile t = c.tile[index];
+  const Tile all = c.tile[c.tiles];
+  if (t.rows == 0) return;
+  up_blocks<RT, kF32>(c, index, t, group, all.slot, threadIdx.x, h_lds);
+  if constexpr (kTurns)
+    for (index += gridDim.x / groups; index < all.rows; index += gridDim.x / groups) {
+      __syncthreads();   // before the next tile's h
+      up_blocks<RT, kF32>(c, index, c.tile[index], group, all.slot, thread_here(), h_lds);
+    }
+}
+
 bool is_aligned(const void* p, uintptr_t a) { return ((uintptr_t)p & (a - 1)) == 0; }
 uint64_t round256(uint64_t n) { return (n + 255) & ~(uint64_t)255; }
 
@@ -866,11 +946,12 @@ int tiles_of(const Bank& b, int tokens) {
 bool is_few(const Bank& b, int tokens) { return tokens <= (b.rank_tiles <= 4 ? kFewTokens : kFewTokens / 2); }
 
 // Parts of K. Few tokens: as many as give each wave a unit of 64, since how many adapters the tokens share is not known
-// here. Grouped form: as many as are resident together (two a CU) and no more, since a few beyond would run alone after
-// the rest; at least two stages each. In both, parts T is at most kWantGroups kTileTokens + T.
+// here. Grouped form: the most that `split` may take: as many as are resident together (two a CU) and no more, since a
+// few beyond would run alone after the rest, if every tile is full; at least two stages each. In both, parts T is at
+// most kWantGroups kTileTokens + T.
 int parts_of(const Bank& b, int tokens) {
   if (is_few(b, tokens)) return std::max(1, std::min(kMaxParts, b.chunks / 8));
-  return std::max(1, std::min({kMaxParts, b.k / (2 * kStageK), kWantGroups / tiles_of(b, tokens)}));
+  return std::max(1, std::min({kMaxParts, b.k / (2 * kStageK), kWantGroups * kTileTokens / tokens}));
 }
 
 }  // namespace
@@ -899,7 +980,7 @@ Workspace workspace_of(const Bank& b, int32_t tokens) {
   w.pair_row = round256(4 * ((uint64_t)b.slots + 1));
   w.row_pair = w.pair_row + round256(4 * (uint64_t)tokens);
   w.tile = w.row_pair + round256(4 * (uint64_t)tokens);
-  w.tile_token = w.tile + round256(sizeof(Tile) * (uint64_t)tiles_of(b, tokens));
+  w.tile_token = w.tile + round256(sizeof(Tile) * ((uint64_t)tiles_of(b, tokens) + 1));
   w.low = w.tile_token + round256(4 * kTileTokens * (uint64_t)tiles_of(b, tokens));
   w.bytes = w.low + round256(rows * 64 * b.rank_tiles);
   return w;
@@ -934,19 +1015,29 @@ template <int RT, bool kStream>
 int launch_down(const Call& c, hipStream_t st) {
   const int rank_groups = (c.bank.rank_tiles + RT - 1) / RT;
   constexpr size_t lds = std::max(2 * kStageBytes, 4 * kColumns * RT * 1024);
-  hipLaunchKernelGGL((adapter_down_kernel<RT, kStream>), dim3(round8((int64_t)c.parts * c.tiles * rank_groups)), dim3(256),
-                     lds, st, c, rank_groups);
+  const int64_t pieces = std::max(std::min(c.parts * c.tiles, kWantGroups), c.tiles) * (int64_t)rank_groups;
+  hipLaunchKernelGGL((adapter_down_kernel<RT, kStream>), dim3(round8(pieces)), dim3(256), lds, st, c, rank_groups);
   MX_LAUNCH_CHECK("adapter_down_kernel");
   return MX_OK;
 }
 
-template <int RT>
-int launch_up(const Call& c, bool f32, hipStream_t st) {
+template <int RT, bool kTurns>
+int launch_up(const Call& c, int tiles, bool f32, hipStream_t st) {
   const int groups = (c.bank.blocks + 3) / 4;
-  hipLaunchKernelGGL((f32 ? adapter_up_kernel<RT, true> : adapter_up_kernel<RT, false>),
-                     dim3((unsigned)(groups * c.tiles)), dim3(256), 0, st, c);
+  hipLaunchKernelGGL((f32 ? adapter_up_kernel<RT, true, kTurns> : adapter_up_kernel<RT, false, kTurns>),
+                     dim3((unsigned)(groups * tiles)), dim3(256), 0, st, c);
   MX_LAUNCH_CHECK("adapter_up_kernel");
   return MX_OK;
+}
+
+// How many tiles the tokens make only the device knows; a bank of many slots could make far more than they do. Up has
+// workgroups for the full ones and 32 more, or as many as are resident together, and takes the rest in turns: 24576
+// rows, rank 16, 200 tokens of 8 of 64 adapters 13.6 us, with 64 more 15.3; 1536 rows, 600 tokens of 64 of 1024
+// adapters 15.1 us with 64 more, 17.0 with 32 and 19.5 with 16.
+template <int RT>
+int launch_up(const Call& c, bool f32, hipStream_t st) {
+  const int tiles = c.tokens / kTileTokens + std::max(32, 1024 / ((c.bank.blocks + 3) / 4));
+  return tiles < c.tiles ? launch_up<RT, true>(c, tiles, f32, st) : launch_up<RT, false>(c, c.tiles, f32, st);
 }
 
 int launch_groups(const Call& c, bool f32, hipStream_t st) {
