@@ -39,6 +39,8 @@ constexpr int kMaxWidth = 1 << 20;
 constexpr int kFewTokens = 128;    // a wave holds the ids of this many tokens, in two registers
 constexpr int kTileTokens = 64;    // tokens of a workgroup in the grouped form
 constexpr int kColumns = kTileTokens / 16;
+constexpr int kMostTiles = 8;      // rank tiles that up's waves hold at once; of more, kTurnTiles in turn
+constexpr int kTurnTiles = 4;
 constexpr int kMaxParts = 32;      // parts of K
 // A call of few tokens is one launch if down and the x of its tokens (of 64 at most, since the tokens of a workgroup
 // are 16 of one adapter) are no more than this: each of its workgroups reads all of down. One launch and two, rank 12
@@ -147,41 +149,28 @@ __device__ __forceinline__ int on_xcd(int id, int count) { return (id & 7) * ((c
 struct Work {
   Tile tile;
   int index, part, rank_group;   // index -1: nothing
-  int tiles, parts;
+  int tiles, pieces, parts;      // in all; pieces: groups of rank tiles that the tiles have together
 };
 
-// Piece `id` of down's work over `tiles` tiles; each XCD has a contiguous range of it, part by part.
-__device__ __forceinline__ Work split(const Call& c, int id, int tiles, int rank_groups) {
-  Work w;
-  w.tile = Tile{-1, 0};
-  w.tiles = min(tiles, c.tiles);
-  w.parts = min(c.parts, max(kWantGroups / max(w.tiles, 1), 1));
-  const int count = w.parts * w.tiles * rank_groups, piece = on_xcd(id, count);
-  w.index = -1;
-  w.part = w.rank_group = 0;
-  if (id >= (count + 7) / 8 * 8 || piece >= count) return w;
-  const int tile = rank_groups == 1 ? piece : piece / rank_groups;
-  w.rank_group = piece - tile * rank_groups;
-  w.part = tile / w.tiles;
-  w.index = tile - w.part * w.tiles;
-  return w;
-}
-
-// Piece `id` of the groups' tiles: kTileTokens tokens of a group each (a group's last one short), the tokens without an
-// adapter last as group `slots`; count(g) gives the tokens of a group. Thread i of the workgroup has the groups from
-// i `per` on. place: the tile's group and the place in it of its first token.
+// Piece `id` of down's work: the groups' tiles, kTileTokens tokens of a group each (a group's last one short), the
+// tokens without an adapter last as group `slots`, each for every RT rank tiles that its slot has, then the next part
+// of K; each XCD has a contiguous range of it. count(g) gives the tokens of a group. Thread i of the workgroup has the
+// groups from i `per` on. place: the tile's group and the place in it of its first token.
 constexpr int kThreadGroups = kMaxSlots / 256 + 1;
+constexpr int kPieceShift = 13;   // tiles and pieces are counted in one number: up to 5120 and 20480
+static_assert(kMaxTokens / kTileTokens + kMaxSlots + 1 < 1 << kPieceShift, "a count of tiles has 13 bits");
 
-template <typename Count>
-__device__ __forceinline__ Work locate(const Call& c, int id, int rank_groups, Count count, int (&found)[8], int2& place) {
+template <int RT, typename Count>
+__device__ __forceinline__ Work locate(const Call& c, int id, Count count, int (&found)[8], int2& place) {
   const int tid = threadIdx.x, lane = tid & 63, slots = c.bank.slots, per = (slots + 256) / 256, first = tid * per;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  int n[kThreadGroups], mine = 0;
+  int n[kThreadGroups], each[kThreadGroups], mine = 0;   // each: pieces of a tile
 #pragma unroll
   for (int i = 0; i < kThreadGroups; ++i)
     if (i < per) {
       n[i] = first + i <= slots ? count(first + i) : 0;
-      mine += (n[i] + kTileTokens - 1) / kTileTokens;
+      each[i] = c.bank.rank_tiles > RT && first + i < slots ? max((c.bank.table[first + i].rank + 16 * RT - 1) / (16 * RT), 1) : 1;
+      mine += (n[i] + kTileTokens - 1) / kTileTokens * (1 + (each[i] << kPieceShift));
     }
   int upto = mine;   // of the wave's threads up to this one
 #pragma unroll
@@ -197,41 +186,59 @@ __device__ __forceinline__ Work locate(const Call& c, int id, int rank_groups, C
     before += w < wave ? found[4 + w] : 0;
     total += found[4 + w];
   }
-  Work work = split(c, id, __builtin_amdgcn_readfirstlane(total), rank_groups);
-  if (work.index < 0) return work;
-  if (work.index >= before && work.index < before + mine) {
-    int skip = work.index - before;
+  total = __builtin_amdgcn_readfirstlane(total);
+  Work w;
+  w.tile = Tile{-1, 0};
+  w.tiles = min(total & ((1 << kPieceShift) - 1), c.tiles);
+  w.pieces = min(total >> kPieceShift, c.tiles * ((c.bank.rank_tiles + RT - 1) / RT));
+  w.parts = min(c.parts, max(kWantGroups / max(w.pieces, 1), 1));
+  w.index = -1;
+  w.part = w.rank_group = 0;
+  const int all = w.parts * w.pieces, piece = on_xcd(id, all);
+  if (id >= (all + 7) / 8 * 8 || piece >= all) return w;
+  w.part = piece / w.pieces;
+  int skip = piece - w.part * w.pieces - (before >> kPieceShift);   // pieces from this thread's first on
+  if (skip >= 0 && skip < mine >> kPieceShift) {
+    int index = before & ((1 << kPieceShift) - 1);
 #pragma unroll
     for (int i = 0; i < kThreadGroups; ++i)
       if (i < per) {
-        const int tiles = (n[i] + kTileTokens - 1) / kTileTokens;
-        if (skip >= 0 && skip < tiles) {
+        const int tiles = (n[i] + kTileTokens - 1) / kTileTokens, tile = each[i] == 1 ? skip : skip / each[i];
+        if (skip >= 0 && tile < tiles) {
           found[0] = first + i;
-          found[1] = skip * kTileTokens;
-          found[2] = min(kTileTokens, n[i] - skip * kTileTokens);
+          found[1] = tile * kTileTokens;
+          found[2] = min(kTileTokens, n[i] - tile * kTileTokens);
+          found[3] = (index + tile) << 4 | (skip - tile * each[i]);
         }
-        skip -= tiles;
+        skip -= tiles * each[i];
+        index += tiles;
       }
   }
   __syncthreads();
-  place.x = __builtin_amdgcn_readfirstlane(found[0]);
+  // (a plan that is none may leave all this unwritten: nothing below goes out of range)
+  place.x = min(max(__builtin_amdgcn_readfirstlane(found[0]), 0), slots);
   place.y = __builtin_amdgcn_readfirstlane(found[1]);
-  work.tile = Tile{place.x < slots ? place.x : -1, __builtin_amdgcn_readfirstlane(found[2])};
-  return work;
+  const int rows = min(max(__builtin_amdgcn_readfirstlane(found[2]), 0), kTileTokens);
+  const int at = __builtin_amdgcn_readfirstlane(found[3]);
+  w.index = at >> 4 >= 0 && at >> 4 < w.tiles ? at >> 4 : -1;
+  w.rank_group = at & 15;
+  w.tile = Tile{place.x < slots ? place.x : -1, rows};
+  return w;
 }
 
 // Piece `id` by the plan of ids; `token` is that of this lane's column (those past the last repeat it).
-__device__ __forceinline__ Work plan_work(const Call& c, int id, int rank_groups, int (&found)[8], int& token) {
+template <int RT>
+__device__ __forceinline__ Work plan_work(const Call& c, int id, int (&found)[8], int& token) {
   const int slots = c.bank.slots;
   auto begin = [&](int g) { return min(max(c.first[g], 0), c.tokens); };
   int2 place;
-  const Work work = locate(c, id, rank_groups, [&](int g) {
+  const Work work = locate<RT>(c, id, [&](int g) {
     const int lo = begin(g);
     return (g < slots ? max(begin(g + 1), lo) : c.tokens) - lo;
   }, found, place);
   if (work.index >= 0) {
     const int row = begin(place.x) + place.y + min((int)(threadIdx.x & 63), work.tile.rows - 1);
-    token = c.row_pair[min(row, c.tokens - 1)];
+    token = c.row_pair[min(max(row, 0), c.tokens - 1)];
     token = token >= 0 && token < c.tokens ? token : 0;
   }
   return work;
@@ -246,8 +253,8 @@ constexpr int kOwnIds = 16, kOwnTokens = 4 * 64 * kOwnIds;
 constexpr int kCopies = 8;   // of each count, by lane: neighbours of one group take few turns at one of them
 constexpr int kOwnLds = (kMaxSlots + 1) * kCopies + 4 + kTileTokens;   // numbers
 
-__device__ __forceinline__ Work own_work(const Call& c, int id, int rank_groups, int (&found)[8], int* lds,
-                                         int& token) {
+template <int RT>
+__device__ __forceinline__ Work own_work(const Call& c, int id, int (&found)[8], int* lds, int& token) {
   const int tid = threadIdx.x, lane = tid & 63, slots = c.bank.slots;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   int* count = lds;
@@ -268,7 +275,7 @@ __device__ __forceinline__ Work own_work(const Call& c, int id, int rank_groups,
     }
   __syncthreads();
   int2 place;
-  const Work work = locate(c, id, rank_groups, [&](int g) {
+  const Work work = locate<RT>(c, id, [&](int g) {
     int n = 0;
 #pragma unroll
     for (int i = 0; i < kCopies; ++i) n += count[g * kCopies + i];
@@ -570,12 +577,12 @@ __device__ __forceinline__ void down_piece(const Call& c, const Work& work, int 
 }
 
 template <int RT, bool kStream>
-__global__ __launch_bounds__(256, 2) void adapter_down_kernel(Call c, int rank_groups) {
+__global__ __launch_bounds__(256, 2) void adapter_down_kernel(Call c) {
   extern __shared__ uint4 stage_lds[];   // two stages; then the waves' sums [4][kColumns][RT][64]
-  __shared__ int found[8];   // the tile's group, its first token's place in it, its tokens; then the waves' tiles
+  __shared__ int found[8];   // of the tile: group, first token's place in it, tokens, number and rank group; then sums
   int tokens = 0;
-  const Work work = c.first ? plan_work(c, blockIdx.x, rank_groups, found, tokens)
-                            : own_work(c, blockIdx.x, rank_groups, found, (int*)stage_lds, tokens);
+  const Work work = c.first ? plan_work<RT>(c, blockIdx.x, found, tokens)
+                            : own_work<RT>(c, blockIdx.x, found, (int*)stage_lds, tokens);
   if (blockIdx.x == 0) {
     if (threadIdx.x == 0) c.tile[c.tiles] = Tile{work.parts, work.tiles};
     for (int i = work.tiles + threadIdx.x; i < c.tiles; i += 256) c.tile[i] = Tile{-1, 0};
@@ -819,6 +826,57 @@ __global__ __launch_bounds__(1024) void adapter_few_kernel(Call c) {
       *(uint4*)(c.y + f.token * c.y_stride + n + 32 * k) = eight_bf16(out[2 * k], out[2 * k + 1]);
 }
 
+// Base of the tile's tokens at a block, in memory order (see swap8): this lane's pieces are of two tokens of each
+// column tile, eight columns apart. Lanes without an output repeat another's address.
+template <bool kF32>
+__device__ __forceinline__ void load_base(const Call& c, int tokens, int n, int lane, uint4 (&base)[kColumns][kF32 ? 4 : 2],
+                                          int64_t (&token)[kColumns][2]) {
+  const bool low = (lane & 15) < 8;
+#pragma unroll
+  for (int i = 0; i < kColumns; ++i)
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      token[i][k] = __shfl(tokens, 16 * i + 8 * k + (lane & 7), 64);
+      if constexpr (kF32) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int at = n + 32 * h < c.bank.n ? n + 32 * h + (low ? 0 : 4) : 0;
+          base[i][2 * h + k] = ldg128((const uint8_t*)((const float*)c.base + token[i][k] * c.base_stride + at));
+        }
+      } else {
+        const int at = n + (low ? 0 : 32) < c.bank.n ? n + (low ? 0 : 32) : 0;
+        base[i][k] = ldg128((const uint8_t*)((const uint16_t*)c.base + token[i][k] * c.base_stride + at));
+      }
+    }
+}
+
+// A column tile's base as what its sums start from.
+template <bool kF32>
+__device__ __forceinline__ void from_base(uint4 (&base)[kF32 ? 4 : 2], bool low, v4f (&acc)[4]) {
+  if constexpr (kF32) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      swap8(base[2 * h], base[2 * h + 1], low);
+      acc[2 * h] = __builtin_bit_cast(v4f, base[2 * h]);
+      acc[2 * h + 1] = __builtin_bit_cast(v4f, base[2 * h + 1]);
+    }
+  } else {
+    swap8(base[0], base[1], low);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) acc[k] = four_of(base[k >> 1], k & 1);
+  }
+}
+
+// Column tile i of y, of `rows` tokens in all; `at` is this lane's output in memory order.
+__device__ __forceinline__ void store_y(const Call& c, int rows, int i, int at, int lane, bool low,
+                                        const int64_t (&token)[2], const v4f (&acc)[4]) {
+  uint4 out[2] = {eight_bf16(acc[0], acc[1]), eight_bf16(acc[2], acc[3])};
+  swap8(out[0], out[1], low);
+#pragma unroll
+  for (int k = 0; k < 2; ++k)
+    if (16 * i + 8 * k + (lane & 7) < rows && at < c.bank.n) *(uint4*)(c.y + token[k] * c.y_stride + at) = out[k];
+}
+
 // Grouped form: a tile of 64 tokens and four blocks of 64 outputs, one a wave, its weights of all ranks in registers
 // for the tile's columns, 16 tokens at a time. What does not depend on h is asked for before h goes to LDS. Bound by
 // base and y: 4096 tokens of 7168 outputs (117 MB) 30 us, 3056 of 24576 (300 MB) 69; with accesses of 64 bytes the
@@ -849,26 +907,10 @@ __device__ __forceinline__ void up_blocks(const Call& c, int index, const Tile& 
       w[r][0] = ldg128(p + 2048 * at), w[r][1] = ldg128(p + 2048 * at + 1024);
     }
   }
-  // in memory order (see swap8): this lane's pieces are of two tokens of each column tile, eight columns apart
   const bool low = (lane & 15) < 8;
   uint4 base[kColumns][kF32 ? 4 : 2];
   int64_t token[kColumns][2];
-#pragma unroll
-  for (int i = 0; i < kColumns; ++i)
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      token[i][k] = __shfl(tokens, 16 * i + 8 * k + (lane & 7), 64);
-      if constexpr (kF32) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int at = n + 32 * h < b.n ? n + 32 * h + (low ? 0 : 4) : 0;
-          base[i][2 * h + k] = ldg128((const uint8_t*)((const float*)c.base + token[i][k] * c.base_stride + at));
-        }
-      } else {
-        const int at = n + (low ? 0 : 32) < b.n ? n + (low ? 0 : 32) : 0;
-        base[i][k] = ldg128((const uint8_t*)((const uint16_t*)c.base + token[i][k] * c.base_stride + at));
-      }
-    }
+  load_base<kF32>(c, tokens, n, lane, base, token);
   if constexpr (RT == 1)
     if (c.parts > 1 && tiles) h[0] = h_operand(slot, 4 * q, sum_parts(low_h, c.tokens * rank_stride, 0, 1, parts));
 #pragma unroll
@@ -883,18 +925,7 @@ __device__ __forceinline__ void up_blocks(const Call& c, int index, const Tile& 
   for (int i = 0; i < kColumns; ++i) {
     if (16 * i >= t.rows) break;
     v4f acc[4];
-    if constexpr (kF32) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        swap8(base[i][2 * h], base[i][2 * h + 1], low);
-        acc[2 * h] = __builtin_bit_cast(v4f, base[i][2 * h]);
-        acc[2 * h + 1] = __builtin_bit_cast(v4f, base[i][2 * h + 1]);
-      }
-    } else {
-      swap8(base[i][0], base[i][1], low);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) acc[k] = four_of(base[i][k >> 1], k & 1);
-    }
+    from_base<kF32>(base[i], low, acc);
     if (tiles == RT) {
 #pragma unroll
       for (int r = 0; r < RT; ++r) up_tile(w[r], h_lds[(i * RT + r) * 64 + lane], acc);
@@ -903,30 +934,78 @@ __device__ __forceinline__ void up_blocks(const Call& c, int index, const Tile& 
       for (int r = 0; r < RT; ++r)
         if (r < tiles) up_tile(w[r], h_lds[(i * RT + r) * 64 + lane], acc);
     }
-    uint4 out[2] = {eight_bf16(acc[0], acc[1]), eight_bf16(acc[2], acc[3])};
-    swap8(out[0], out[1], low);
-#pragma unroll
-    for (int k = 0; k < 2; ++k)
-      if (16 * i + 8 * k + (lane & 7) < t.rows && at_y < b.n) {
-        *(uint4*)(c.y + token[i][k] * c.y_stride + at_y) = out[k];
-      }
+    store_y(c, t.rows, i, at_y, lane, low, token[i], acc);
   }
 }
 
-// kTurns: for fewer workgroups than there can be tiles.
+// The same in a bank of more than 128 ranks: the blocks' sums of all 64 tokens stay in registers, and the ranks go
+// through 64 at a time, only the slot's own. 4096 tokens of adapters of rank 256, 64 and 16 in a bank of 256, 24576
+// outputs: 218, 122 and 100 us in all; all 16 rank tiles at once 277, 218 and 186. (In a bank of 128 ranks eight at
+// once are the faster: rank 64 97 us and 107.)
+template <bool kF32>
+__device__ __forceinline__ void up_blocks_many(const Call& c, int index, const Tile& t, int group, int tid, uint4* h_lds) {
+  constexpr int RT = kTurnTiles;
+  const Bank& b = c.bank;
+  const int tokens = c.tile_token[index * kTileTokens + (tid & 63)];
+  const AdapterSlot slot = t.slot >= 0 ? b.table[t.slot] : AdapterSlot{0, 0.f};
+  const int tiles = (slot.rank + 15) >> 4;
+  const int lane = tid & 63, q = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int block = 4 * group + wave, n = 64 * block + 8 * q;   // past the last block: no output is a lane's
+  const float* low_h = c.low + __shfl(tokens, 16 * wave + (lane & 15), 64) * (int64_t)(16 * b.rank_tiles) + 4 * q;
+  const uint8_t* up = b.up_at(t.slot, block) + 16 * lane;
+  const bool low = (lane & 15) < 8;
+  uint4 base[kColumns][kF32 ? 4 : 2];
+  int64_t token[kColumns][2];
+  load_base<kF32>(c, tokens, n, lane, base, token);
+  v4f acc[kColumns][4];
+#pragma unroll
+  for (int i = 0; i < kColumns; ++i) from_base<kF32>(base[i], low, acc[i]);
+  for (int r0 = 0; r0 < tiles; r0 += RT) {
+    uint4 h[RT], w[RT][2];
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+      const int at = min(r0 + r, tiles - 1);
+      h[r] = ldg128((const uint8_t*)(low_h + 16 * at));
+      w[r][0] = ldg128(up + 2048 * at), w[r][1] = ldg128(up + 2048 * at + 1024);
+    }
+    if (r0) __syncthreads();   // the h before this has been read
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+      const int ranks = slot.rank - 16 * (r0 + r) - 4 * q;
+      if (ranks <= 0) h[r] = make_uint4(0, 0, 0, 0);
+      h_lds[(wave * RT + r) * 64 + lane] = h[r];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kColumns; ++i)
+#pragma unroll
+      for (int r = 0; r < RT; ++r)
+        if (16 * i < t.rows && r0 + r < tiles) up_tile(w[r], h_lds[(i * RT + r) * 64 + lane], acc[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < kColumns; ++i)
+    if (16 * i < t.rows) store_y(c, t.rows, i, n + (low ? 0 : 32), lane, low, token[i], acc[i]);
+}
+
+// RT rank tiles, or in turns if there are more. kTurns: for fewer workgroups than there can be tiles.
 template <int RT, bool kF32, bool kTurns>
 __global__ __launch_bounds__(256) void adapter_up_kernel(Call c) {
-  __shared__ uint4 h_lds[kColumns * RT * 64];
+  __shared__ uint4 h_lds[kColumns * (RT > kMostTiles ? kTurnTiles : RT) * 64];
   const int groups = (c.bank.blocks + 3) / 4, group = blockIdx.x % groups;
   int index = blockIdx.x / groups;
   Tile t = c.tile[index];
   const Tile all = c.tile[c.tiles];
   if (t.rows == 0) return;
-  up_blocks<RT, kF32>(c, index, t, group, all.slot, threadIdx.x, h_lds);
+  auto blocks = [&](const Tile& tile, int tid) {
+    if constexpr (RT <= kMostTiles) up_blocks<RT, kF32>(c, index, tile, group, all.slot, tid, h_lds);
+    else up_blocks_many<kF32>(c, index, tile, group, tid, h_lds);
+  };
+  blocks(t, threadIdx.x);
   if constexpr (kTurns)
     for (index += gridDim.x / groups; index < all.rows; index += gridDim.x / groups) {
       __syncthreads();   // before the next tile's h
-      up_blocks<RT, kF32>(c, index, c.tile[index], group, all.slot, thread_here(), h_lds);
+      blocks(c.tile[index], thread_here());
     }
 }
 
@@ -1013,10 +1092,10 @@ unsigned round8(int64_t n) { return (unsigned)((n + 7) / 8 * 8); }
 
 template <int RT, bool kStream>
 int launch_down(const Call& c, hipStream_t st) {
-  const int rank_groups = (c.bank.rank_tiles + RT - 1) / RT;
+  const int most = c.tiles * ((c.bank.rank_tiles + RT - 1) / RT);
   constexpr size_t lds = std::max(2 * kStageBytes, 4 * kColumns * RT * 1024);
-  const int64_t pieces = std::max(std::min(c.parts * c.tiles, kWantGroups), c.tiles) * (int64_t)rank_groups;
-  hipLaunchKernelGGL((adapter_down_kernel<RT, kStream>), dim3(round8(pieces)), dim3(256), lds, st, c, rank_groups);
+  hipLaunchKernelGGL((adapter_down_kernel<RT, kStream>), dim3(round8(std::max(std::min(c.parts * most, kWantGroups), most))),
+                     dim3(256), lds, st, c);
   MX_LAUNCH_CHECK("adapter_down_kernel");
   return MX_OK;
 }
@@ -1057,7 +1136,7 @@ int launch_groups(const Call& c, bool f32, hipStream_t st) {
   if (rt == 1) return launch_up<1>(c, f32, st);
   if (rt == 2) return launch_up<2>(c, f32, st);
   if (rt <= 4) return launch_up<4>(c, f32, st);
-  return rt <= 8 ? launch_up<8>(c, f32, st) : launch_up<16>(c, f32, st);
+  return rt <= kMostTiles ? launch_up<kMostTiles>(c, f32, st) : launch_up<kMaxRank / 16>(c, f32, st);
 }
 
 }  // namespace
