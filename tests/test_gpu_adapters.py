@@ -71,7 +71,7 @@ SHAPES = [(1, 8, 8, 1, 1), (1, 64, 32, 1, 16), (1, 2112, 1536, 3, 64), (2, 72, 4
           (31, 576, 128, 5, 17), (32, 136, 1600, 4, 33), (33, 64, 72, 3, 16), (40, 1032, 2048, 2, 32), (47, 200, 264, 8, 256), (60, 24, 104, 1, 128),
           (64, 1024, 96, 70, 64), (65, 8, 1536, 1, 100), (100, 320, 8, 90, 8), (127, 72, 1032, 3, 40), (128, 136, 328, 40, 16), (129, 64, 96, 5, 64),
           (257, 88, 160, 6, 64),
-          (1000, 264, 520, 8, 128)]
+          (150, 136, 600, 8, 256), (1000, 264, 520, 8, 128)]
 
 
 @pytest.mark.parametrize("tokens,rows,width,slots,max_rank", SHAPES)
@@ -252,8 +252,10 @@ def test_calls_larger_than_the_caches(gpu_ctx):
         check(bank.apply(x, ids, base), x, ids, base, adapters, True)
 
 
-def test_two_banks_on_two_streams_by_one_plan(gpu_ctx):
-    """A step's projections side by side: a bank and a stream each, the plan of the step's ids for both."""
+@pytest.mark.parametrize("max_rank", [32, 256])
+def test_two_banks_on_two_streams_by_one_plan(gpu_ctx, max_rank):
+    """A step's projections side by side: a bank and a stream each, the plan of the step's ids for both; adapters of the
+    banks' largest rank and of small ones."""
     rng = np.random.default_rng(5)
     tokens, width, slots = 700, 264, 5
     ids = rng.integers(-1, slots, tokens).astype(np.int32)
@@ -262,8 +264,8 @@ def test_two_banks_on_two_streams_by_one_plan(gpu_ctx):
         idd, sides = gpu_ctx.upload(ids), []
         d.plan_device(idd, tokens)
         for rows, on in zip((200, 1032), streams):
-            bank = AdapterBank(gpu_ctx, rows, width, slots, 32, tokens)
-            adapters = {s: adapter(rng, rows, width, 32 - 5 * s, True) for s in range(slots)}
+            bank = AdapterBank(gpu_ctx, rows, width, slots, max_rank, tokens)
+            adapters = {s: adapter(rng, rows, width, max_rank >> s, True) for s in range(slots)}
             fill(bank, rng, adapters)
             x, base = inputs(rng, tokens, rows, width, True, "f32")
             dev = [gpu_ctx.upload(a) for a in (x, base, np.zeros((tokens, rows), np.uint16))]
