@@ -608,16 +608,17 @@ __global__ __launch_bounds__(256) void adapter_sum_kernel(Call c) {
   const int per = 4 * b.rank_tiles, share = (threadIdx.x & 63) / (64 / kShares);   // entries of a token
   const int e = (blockIdx.x * 256 + (threadIdx.x & ~63)) / kShares + threadIdx.x % (64 / kShares);
   if (e >= c.tokens * per) return;
-  const int id = c.ids[e / per];
-  const bool held = id >= 0 && id < b.slots;   // the sums of a token without an adapter, or past a slot's rank, are no one's
-  const AdapterSlot slot = b.table[held ? id : 0];
+  const int id = c.ids[e / per], r0 = 4 * (e % per);
+  if (id < 0 || id >= b.slots) return;
+  const AdapterSlot slot = b.table[id];
+  if (r0 >= slot.rank) return;   // what lies past a slot's rank no one has written, and up takes as zero
   float* p = c.low + 4 * (int64_t)e;
   v4f s = sum_parts(p, (int64_t)c.tokens * 4 * per, share, kShares, min(c.tile[c.tiles].slot, c.parts));
 #pragma unroll
-  for (int d = 64 / kShares; d < 64; d <<= 1)
+  for (int d = 64 / kShares; d < 64; d <<= 1)   // the lanes of an entry are here or gone together
 #pragma unroll
     for (int i = 0; i < 4; ++i) s[i] = s[i] + __shfl_xor(s[i], d, 64);
-  if (held && share == 0) *(uint4*)p = h_operand(slot, 4 * (e % per), s);
+  if (share == 0) *(uint4*)p = h_operand(slot, r0, s);
 }
 
 // ---- up: y = base + up h ----
