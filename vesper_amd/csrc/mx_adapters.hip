@@ -146,7 +146,7 @@ __device__ __forceinline__ int on_xcd(int id, int count) { return (id & 7) * ((c
 // What a workgroup of down does: a part of K and a group of rank tiles for a tile. The split of K follows the tiles
 // that there are, which only the device knows: the slots that no token names make none (600 tokens of 8 adapters of
 // rank 64 by 16384 in a bank of 1024 slots 27 us, split by the tiles that there could be 78), and a slot of fewer ranks
-// than the bank's largest has fewer pieces (4096 tokens of rank 16 by 16384 in a bank of 256 ranks 65 us, with idle
+// than the bank's largest has fewer pieces (4096 tokens of rank 16 by 16384 in a bank of 256 ranks 61 us, with idle
 // workgroups for the other ranks 111).
 struct Work {
   Tile tile;
