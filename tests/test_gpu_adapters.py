@@ -252,6 +252,30 @@ def test_calls_larger_than_the_caches(gpu_ctx):
         check(bank.apply(x, ids, base), x, ids, base, adapters, True)
 
 
+@pytest.mark.parametrize("first", [[0, 60, 40, 170], [0, 30, 60, 171], [0, -1, 60, 170], [1, 30, 60, 170], [170] * 4,
+                                   [0, 1 << 30, 1 << 30, 170]])
+def test_a_plan_that_is_none_does_nothing(gpu_ctx, first):
+    """Groups that do not cover the tokens in order: y is left as it was, and nothing out of range is touched. The same
+    call by a right plan follows."""
+    rng = np.random.default_rng(1)
+    tokens, rows, width, slots = 170, 72, 104, 3
+    adapters = {s: adapter(rng, rows, width, 16, True) for s in range(slots)}
+    ids = np.sort(rng.integers(-1, slots, tokens)).astype(np.int32)
+    x, base = inputs(rng, tokens, rows, width, True, "bf16")
+    with AdapterBank(gpu_ctx, rows, width, slots, 16, tokens) as bank, ExpertDispatch(gpu_ctx, slots, 1, tokens) as d:
+        fill(bank, rng, adapters)
+        xd, idd, bd, yd = (gpu_ctx.upload(a) for a in (x, ids, base, np.full((tokens, rows), 0x1234, np.uint16)))
+        d.plan_device(idd, tokens)
+        gpu_ctx.copy_h2d(d.first, np.array(first, np.int32))
+        bank.apply_device(xd, idd, tokens, bd, yd, plan=d.plan)
+        assert (yd.download() == 0x1234).all()
+        d.plan_device(idd, tokens)
+        bank.apply_device(xd, idd, tokens, bd, yd, plan=d.plan)
+        check(yd.download(), x, ids, base, adapters, True)
+        for a in (xd, idd, bd, yd):
+            a.free()
+
+
 @pytest.mark.parametrize("max_rank", [32, 256])
 def test_two_banks_on_two_streams_by_one_plan(gpu_ctx, max_rank):
     """A step's projections side by side: a bank and a stream each, the plan of the step's ids for both; adapters of the

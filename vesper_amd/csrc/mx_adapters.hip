@@ -156,8 +156,9 @@ struct Work {
 
 // Piece `id` of down's work: the groups' tiles, kTileTokens tokens of a group each (a group's last one short), the
 // tokens without an adapter last as group `slots`, each for every RT rank tiles that its slot has, then the next part
-// of K; each XCD has a contiguous range of it. count(g) gives the tokens of a group. Thread i of the workgroup has the
-// groups from i `per` on. place: the tile's group and the place in it of its first token.
+// of K; each XCD has a contiguous range of it. count(g) gives the tokens of a group, -1 if the plan is none: then there
+// is nothing to do. Thread i of the workgroup has the groups from i `per` on. place: the tile's group and the place in
+// it of its first token.
 constexpr int kThreadGroups = kMaxSlots / 256 + 1;
 constexpr int kPieceShift = 13;   // tiles and pieces are counted in one number: up to 5120 and 20480
 static_assert(kMaxTokens / kTileTokens + kMaxSlots + 1 < 1 << kPieceShift, "a count of tiles has 13 bits");
@@ -180,19 +181,25 @@ __device__ __forceinline__ Work locate(const Call& c, int id, Count count, int (
     const int o = __shfl_up(upto, d, 64);
     if (lane >= d) upto += o;
   }
-  if (lane == 63) found[4 + wave] = upto;
+  bool none = false;
+#pragma unroll
+  for (int i = 0; i < kThreadGroups; ++i) none |= i < per && n[i] < 0;
+  none = __any(none);
+  if (lane == 63) found[4 + wave] = none ? -1 : upto;
   __syncthreads();
   int total = 0, before = upto - mine;
+  none = false;
 #pragma unroll
   for (int w = 0; w < 4; ++w) {
+    none |= found[4 + w] < 0;
     before += w < wave ? found[4 + w] : 0;
     total += found[4 + w];
   }
-  total = __builtin_amdgcn_readfirstlane(total);
+  total = __builtin_amdgcn_readfirstlane(none ? 0 : total);
   Work w;
   w.tile = Tile{-1, 0};
-  w.tiles = min(total & ((1 << kPieceShift) - 1), c.tiles);
-  w.pieces = min(total >> kPieceShift, c.tiles * ((c.bank.rank_tiles + RT - 1) / RT));
+  w.tiles = total & ((1 << kPieceShift) - 1);
+  w.pieces = total >> kPieceShift;
   w.parts = min(c.parts, max(kWantGroups / max(w.pieces, 1), 1));
   w.index = -1;
   w.part = w.rank_group = 0;
@@ -217,14 +224,12 @@ __device__ __forceinline__ Work locate(const Call& c, int id, Count count, int (
       }
   }
   __syncthreads();
-  // (a plan that is none may leave all this unwritten: nothing below goes out of range)
-  place.x = min(max(__builtin_amdgcn_readfirstlane(found[0]), 0), slots);
+  place.x = __builtin_amdgcn_readfirstlane(found[0]);
   place.y = __builtin_amdgcn_readfirstlane(found[1]);
-  const int rows = min(max(__builtin_amdgcn_readfirstlane(found[2]), 0), kTileTokens);
   const int at = __builtin_amdgcn_readfirstlane(found[3]);
-  w.index = at >> 4 >= 0 && at >> 4 < w.tiles ? at >> 4 : -1;
+  w.index = at >> 4;
   w.rank_group = at & 15;
-  w.tile = Tile{place.x < slots ? place.x : -1, rows};
+  w.tile = Tile{place.x < slots ? place.x : -1, __builtin_amdgcn_readfirstlane(found[2])};
   return w;
 }
 
@@ -232,15 +237,13 @@ __device__ __forceinline__ Work locate(const Call& c, int id, Count count, int (
 template <int RT>
 __device__ __forceinline__ Work plan_work(const Call& c, int id, int (&found)[8], int& token) {
   const int slots = c.bank.slots;
-  auto begin = [&](int g) { return min(max(c.first[g], 0), c.tokens); };
   int2 place;
   const Work work = locate<RT>(c, id, [&](int g) {
-    const int lo = begin(g);
-    return (g < slots ? max(begin(g + 1), lo) : c.tokens) - lo;
+    const int lo = c.first[g], hi = g < slots ? c.first[g + 1] : c.tokens;
+    return lo >= 0 && (g || !lo) && lo <= hi && hi <= c.tokens ? hi - lo : -1;
   }, found, place);
   if (work.index >= 0) {
-    const int row = begin(place.x) + place.y + min((int)(threadIdx.x & 63), work.tile.rows - 1);
-    token = c.row_pair[min(max(row, 0), c.tokens - 1)];
+    token = c.row_pair[c.first[place.x] + place.y + min((int)(threadIdx.x & 63), work.tile.rows - 1)];
     token = token >= 0 && token < c.tokens ? token : 0;
   }
   return work;
