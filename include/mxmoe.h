@@ -391,9 +391,8 @@ int mx_adapters_load(mx_adapters* a, int32_t slot, const uint16_t* down, const u
                      void* stream);
 /* Bytes of workspace (256-byte aligned device memory) for calls of up to `tokens` tokens. */
 uint64_t mx_adapters_workspace_bytes(const mx_adapters* a, int32_t tokens);
-/* y[t] = BF16(base[t] + scale up (down x[t])) with the adapter of slot ids[t] (device int32), in FP32 and rounded once
- * (down x is taken into the second product as two BF16 terms, about 16 significant bits); BF16(base[t]) where ids[t] is
- * outside [0, slots) or its slot empty. x BF16 [T][k], base [T][n] BF16 or FP32 (base_type MX_ROWS_BF16 / _F32: a
+/* y[t] = BF16(base[t] + scale up (down x[t])) with the adapter of slot ids[t] (device int32), in FP32 and rounded once;
+ * BF16(base[t]) where ids[t] is outside [0, slots) or its slot empty. x BF16 [T][k], base [T][n] BF16 or FP32 (base_type MX_ROWS_BF16 / _F32: a
  * projection's output, or its trace), y BF16 [T][n]; rows `stride` values apart (a multiple of 8; 4 for an FP32 base),
  * all 16-byte aligned. y may be base (BF16, one stride); other overlaps are not supported. tokens in [0, 2^18].
  * plan NULL, or mx_dispatch's plan of ids with top_k 1 and groups = slots (made once for all projections of a step);

@@ -7,9 +7,10 @@
 //   A lane l = row l % 16, K 8 (l / 16) + 0..7; B lane l = column l % 16, same K; D lane l register i = row 4 (l / 16)
 //   + i, column l % 16.
 // So down's D gives lane (token, q) the ranks 4q..4q+3 of a 16-rank tile, which is what up's operand B wants of that
-// lane: up takes the 16 ranks of a tile in one MFMA of 32, K slots 0..3 of a lane holding its ranks of bf16(h) and 4..7
-// those of bf16(h - bf16(h)) against up's values given twice. h = scale * (down x) keeps about 16 significant bits that
-// way, for no further load of up.
+// lane. h = scale * (down x) is FP32 up to there and loses nothing: its 24 bits are three BF16 terms of 8 (the top half
+// of its bits, the top half of what that leaves, and the rest, as far as BF16's smallest numbers reach). A tile's 16
+// ranks take one MFMA, K slots 0..3 of a lane holding its ranks' first terms and 4..7 their second against up's values
+// given twice, and a second one, or half of one that two tiles share, for the third. No load of up is repeated.
 //
 // The bank stores each slot in operand order, padded with zeros to whole tiles:
 //   down: [rank tile][K chunk of 32][lane] 16 bytes: rank 16 rt + l % 16, K 32 c + 8 (l / 16) + 0..7
@@ -22,6 +23,7 @@
 // tokens by adapter into tiles of 64 and read each weight once a tile; x, base and y, once each, then bound them.
 #include <algorithm>
 #include <new>
+#include <type_traits>
 
 #include "mx_device.h"
 #include "mx_internal.h"
@@ -345,24 +347,39 @@ __device__ __forceinline__ Few few_tokens(const Call& c, int t) {
   return Few{slot, rows, before + column < first ? low : high};
 }
 
-// Four ranks of h, from r0 on, as operand B's K slots: bf16(scale s), then bf16 of what that leaves.
-__device__ __forceinline__ uint4 h_operand(const AdapterSlot& slot, int r0, v4f s) {
-  uint32_t hi[2], lo[2];
+// Four ranks of h, from r0 on; past the slot's rank zero.
+__device__ __forceinline__ v4f h_of(const AdapterSlot& slot, int r0, v4f s) {
+  v4f h;
 #pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    float h[2], rest[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) h[i] = r0 + 2 * k + i < slot.rank ? slot.scale * s[2 * k + i] : 0.f;
-    hi[k] = mxd::bf16_pair(h[0], h[1]);
-    rest[0] = h[0] - mx::u2f(hi[k] << 16);
-    rest[1] = h[1] - mx::u2f(hi[k] & 0xFFFF0000u);
-#pragma unroll
-    for (int i = 0; i < 2; ++i)   // an infinite term has no second one
-      if ((hi[k] >> (16 * i) & 0x7F80u) == 0x7F80u) rest[i] = 0.f;
-    lo[k] = mxd::bf16_pair(rest[0], rest[1]);
-  }
-  return make_uint4(hi[0], hi[1], lo[0], lo[1]);
+  for (int i = 0; i < 4; ++i) h[i] = r0 + i < slot.rank ? slot.scale * s[i] : 0.f;
+  return h;
 }
+
+// Four ranks of h as up's operand B: the first two terms of each, and the third.
+struct Terms {
+  uint4 two;
+  uint2 third;
+};
+
+__device__ __forceinline__ Terms split(v4f h) {
+  uint32_t t[3][4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    t[0][i] = mx::f2u(h[i]);
+    const bool finite = (t[0][i] & 0x7F800000u) != 0x7F800000u;   // infinities and NaN are their first term
+    const float rest = finite ? h[i] - mx::u2f(t[0][i] & 0xFFFF0000u) : 0.f;
+    t[1][i] = mx::f2u(rest);
+    t[2][i] = mx::f2u(rest - mx::u2f(t[1][i] & 0xFFFF0000u));
+  }
+  uint32_t w[3][2];   // the upper halves of two
+#pragma unroll
+  for (int n = 0; n < 3; ++n)
+#pragma unroll
+    for (int k = 0; k < 2; ++k) w[n][k] = __builtin_amdgcn_perm(t[n][2 * k + 1], t[n][2 * k], 0x07060302u);
+  return Terms{make_uint4(w[0][0], w[0][1], w[1][0], w[1][1]), make_uint2(w[2][0], w[2][1])};
+}
+
+__device__ __forceinline__ v4f load_h(const float* p) { return __builtin_bit_cast(v4f, ldg128((const uint8_t*)p)); }
 
 // The parts first, first + step, ... of four ranks added in that order, eight of them in flight.
 __device__ __forceinline__ v4f sum_parts(const float* p, int64_t stride, int first, int step, int parts) {
@@ -576,8 +593,7 @@ __device__ __forceinline__ void down_piece(const Call& c, const Work& work, int 
     v4f s = red[(wave * RT + r) * 64 + lane];
 #pragma unroll
     for (int v = 1; v < 4; ++v) s = s + red[((v * kColumns + wave) * RT + r) * 64 + lane];
-    if (c.parts == 1) *(uint4*)(low + 16 * r) = h_operand(slot, 16 * (r0 + r) + 4 * q, s);
-    else *(v4f*)(low + 16 * r) = s;
+    *(v4f*)(low + 16 * r) = c.parts == 1 ? h_of(slot, 16 * (r0 + r) + 4 * q, s) : s;
   }
 }
 
@@ -600,7 +616,7 @@ __global__ __launch_bounds__(256, 2) void adapter_down_kernel(Call c) {
   if (work.tile.rows > 0 && work.tile.slot >= 0) down_piece<RT, kStream>(c, work, tokens, stage_lds);
 }
 
-// Grouped form of more than 16 ranks: the parts of four ranks of a token added, as operand B in the first part's place;
+// Grouped form of more than 16 ranks: the parts of four ranks of a token added, as h in the first part's place;
 // more than eight of them, which a thread has in flight at once, by four lanes whose sums are added as a tree. A launch
 // of its own, 3 to 5 us: in up every workgroup of a tile would add them anew, which 4096 tokens of rank 64 pay with 18
 // us and 3056 beside 24576 rows with 41, and even rank 32 with 1. Of up to 16 ranks up does it: 1010 tokens of rank 8
@@ -621,7 +637,7 @@ __global__ __launch_bounds__(256) void adapter_sum_kernel(Call c) {
   for (int d = 64 / kShares; d < 64; d <<= 1)   // the lanes of an entry are here or gone together
 #pragma unroll
     for (int i = 0; i < 4; ++i) s[i] = s[i] + __shfl_xor(s[i], d, 64);
-  if (share == 0) *(uint4*)p = h_operand(slot, r0, s);
+  if (share == 0) *(v4f*)p = h_of(slot, r0, s);
 }
 
 // ---- up: y = base + up h ----
@@ -676,12 +692,42 @@ __device__ __forceinline__ void swap8(uint4& first, uint4& second, bool low) {
   second = make_uint4(v[0], v[1], v[2], v[3]);
 }
 
-// 16 rows (of two tiles of a half each) against the 16 ranks of `h`: acc[0..3] are the tiles of the block.
-__device__ __forceinline__ void up_tile(const uint4 (&w)[2], uint4 h, v4f (&acc)[4]) {
-  const uint4 a[4] = {make_uint4(w[0].x, w[0].y, w[0].x, w[0].y), make_uint4(w[0].z, w[0].w, w[0].z, w[0].w),
-                      make_uint4(w[1].x, w[1].y, w[1].x, w[1].y), make_uint4(w[1].z, w[1].w, w[1].z, w[1].w)};
+// 16 rows (of two tiles of a half each) against operand B `h`: K slots 0..3 are the ranks of up's tile a, 4..7 those of b
+// (their two halves). acc[0..3] are the tiles of the block.
+__device__ __forceinline__ void up_mfma(uint4 a0, uint4 a1, uint4 b0, uint4 b1, uint4 h, v4f (&acc)[4]) {
+  const v8bf v = as_bf(h);
+  acc[0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf(make_uint4(a0.x, a0.y, b0.x, b0.y)), v, acc[0], 0, 0, 0);
+  acc[1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf(make_uint4(a0.z, a0.w, b0.z, b0.w)), v, acc[1], 0, 0, 0);
+  acc[2] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf(make_uint4(a1.x, a1.y, b1.x, b1.y)), v, acc[2], 0, 0, 0);
+  acc[3] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf(make_uint4(a1.z, a1.w, b1.z, b1.w)), v, acc[3], 0, 0, 0);
+}
+
+// Up of RT rank tiles at most, `count` of them the slot's. This lane's terms of tile r of a column tile lie at two[64 r];
+// the third terms either of two tiles together, at third[64 (r / 2)], in one MFMA, or of each alone, at third[64 r], in
+// one of its own. Together is the fewer MFMAs, alone the fewer moves between registers: 4096 tokens of 8 adapters, 1536
+// columns and 24576 rows, rank 64 (FP32 base) 141 us together and 136 alone, 128 (BF16 base) 136 and 147, 256 210 and 220.
+template <int RT>
+__device__ __forceinline__ void up_tiles(const uint4 (&w)[RT][2], const uint4* two, const uint4* third, int count,
+                                         v4f (&acc)[4]) {
 #pragma unroll
-  for (int j = 0; j < 4; ++j) acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf(a[j]), as_bf(h), acc[j], 0, 0, 0);
+  for (int r = 0; r < RT; ++r) {
+    if (r >= count) continue;
+    up_mfma(w[r][0], w[r][1], w[r][0], w[r][1], two[64 * r], acc);
+    const uint4 rest = third[64 * (r / 2)];
+    if (r % 2) up_mfma(w[r - 1][0], w[r - 1][1], w[r][0], w[r][1], rest, acc);
+    else if (r + 1 >= count) up_mfma(w[r][0], w[r][1], w[r][0], w[r][1], make_uint4(rest.x, rest.y, 0, 0), acc);
+  }
+}
+template <int RT>
+__device__ __forceinline__ void up_tiles(const uint4 (&w)[RT][2], const uint4* two, const uint2* third, int count,
+                                         v4f (&acc)[4]) {
+#pragma unroll
+  for (int r = 0; r < RT; ++r)
+    if (r < count) {
+      const uint2 rest = third[64 * r];
+      up_mfma(w[r][0], w[r][1], w[r][0], w[r][1], two[64 * r], acc);
+      up_mfma(w[r][0], w[r][1], w[r][0], w[r][1], make_uint4(rest.x, rest.y, 0, 0), acc);
+    }
 }
 
 // Few tokens, grid (output blocks / 4, T), 4 waves, a block of 64 outputs each for up to 16 tokens of an adapter (24
@@ -689,10 +735,11 @@ __device__ __forceinline__ void up_tile(const uint4 (&w)[2], uint4 h, v4f (&acc)
 // is put together: thread (entry e, share s) adds the parts s, s + shares, ... of four ranks of a token, and the shares
 // are added in order.
 template <bool kF32>
-__global__ __launch_bounds__(256) void adapter_few_up_kernel(Call c) {
+__global__ __launch_bounds__(256, 2) void adapter_few_up_kernel(Call c) {
   constexpr int RT = 4;   // rank tiles in registers at once
   __shared__ v4f sums[256];
   __shared__ uint4 h_lds[kMaxRank / 16 * 64];
+  __shared__ uint4 third_lds[kMaxRank / 32 * 64];
   const Few f = few_tokens(c, blockIdx.y);
   if (f.rows == 0) return;
   const Bank& b = c.bank;
@@ -730,15 +777,18 @@ __global__ __launch_bounds__(256) void adapter_few_up_kernel(Call c) {
       if (tid < entries)
         for (int m = 1; m < min(shares, c.parts); ++m) sum = sum + sums[m * entries + tid];
     }
-    if (in && share == 0) h_lds[e / f.rows * 16 + column] = h_operand(slot, 4 * (e / f.rows), sum);
+    if (in && share == 0) {
+      const Terms h = split(h_of(slot, 4 * (e / f.rows), sum));
+      const int four = e / f.rows, at = four % 4 * 16 + column;
+      h_lds[four / 4 * 64 + at] = h.two;
+      ((uint2*)third_lds)[2 * (four / 8 * 64 + at) + four / 4 % 2] = h.third;
+    }
   }
   __syncthreads();
   v4f acc[4] = {base[0].four(0), base[0].four(1), base[1].four(0), base[1].four(1)};
   for (int r0 = 0; r0 < tiles; r0 += RT) {
     if (r0) load_up(r0, min(RT, tiles - r0));
-#pragma unroll
-    for (int r = 0; r < RT; ++r)
-      if (r0 + r < tiles) up_tile(w[r], h_lds[64 * (r0 + r) + lane], acc);
+    up_tiles<RT>(w, h_lds + 64 * r0 + lane, third_lds + 32 * r0 + lane, tiles - r0, acc);
   }
 #pragma unroll
   for (int k = 0; k < 2; ++k)
@@ -754,6 +804,7 @@ template <int RT, bool kF32>
 __global__ __launch_bounds__(1024) void adapter_few_kernel(Call c) {
   __shared__ v4f sums[16][RT][64];
   __shared__ uint4 h_lds[RT][64];
+  __shared__ uint4 third_lds[64];
   const int tid = threadIdx.x, lane = tid & 63, q = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const Bank& b = c.bank;
@@ -819,13 +870,13 @@ __global__ __launch_bounds__(1024) void adapter_few_kernel(Call c) {
     v4f sum = sums[0][wave][lane];
 #pragma unroll
     for (int v = 1; v < 16; ++v) sum = sum + sums[v][wave][lane];
-    h_lds[wave][lane] = h_operand(slot, 16 * wave + 4 * q, sum);
+    const Terms h = split(h_of(slot, 16 * wave + 4 * q, sum));
+    h_lds[wave][lane] = h.two;
+    ((uint2*)third_lds)[2 * lane + wave] = h.third;
   }
   __syncthreads();
   v4f out[4] = {base[0].four(0), base[0].four(1), base[1].four(0), base[1].four(1)};
-#pragma unroll
-  for (int r = 0; r < RT; ++r)
-    if (r < tiles) up_tile(w[r], h_lds[r][lane], out);
+  up_tiles<RT>(w, h_lds[0] + lane, third_lds + lane, tiles, out);
 #pragma unroll
   for (int k = 0; k < 2; ++k)
     if ((lane & 15) < f.rows && n + 32 * k < b.n)
@@ -883,12 +934,32 @@ __device__ __forceinline__ void store_y(const Call& c, int rows, int i, int at, 
     if (16 * i + 8 * k + (lane & 7) < rows && at < c.bank.n) *(uint4*)(c.y + token[k] * c.y_stride + at) = out[k];
 }
 
+// A column tile's terms into LDS for up_tiles; `ranks` is how many ranks the slot has from this lane's first on: the sums
+// past them are not its own.
+template <int RT, typename Third>
+__device__ __forceinline__ void put_h(const v4f (&h)[RT], int ranks, uint4* two, Third* third) {
+  Terms t[RT];
+#pragma unroll
+  for (int r = 0; r < RT; ++r) {
+    t[r] = split(ranks > 16 * r ? h[r] : v4f{0.f, 0.f, 0.f, 0.f});
+    two[64 * r] = t[r].two;
+    if constexpr (sizeof(Third) == 8) third[64 * r] = t[r].third;
+    else if (r % 2) third[64 * (r / 2)] = make_uint4(t[r - 1].third.x, t[r - 1].third.y, t[r].third.x, t[r].third.y);
+  }
+}
+// How the workgroups of RT rank tiles hold the third terms, and how many of them a column tile has.
+template <int RT>
+using Third = std::conditional_t<(RT > 4), uint4, uint2>;
+template <int RT>
+constexpr int kThirds = RT > 4 ? RT / 2 : RT;
+
 // Grouped form: a tile of 64 tokens and four blocks of 64 outputs, one a wave, its weights of all ranks in registers
 // for the tile's columns, 16 tokens at a time. What does not depend on h is asked for before h goes to LDS. Bound by
 // base and y: 4096 tokens of 7168 outputs (117 MB) 30 us, 3056 of 24576 (300 MB) 69; with accesses of 64 bytes the
 // first 37.
 template <int RT, bool kF32>
-__device__ __forceinline__ void up_blocks(const Call& c, int index, const Tile& t, int group, int parts, int tid, uint4* h_lds) {
+__device__ __forceinline__ void up_blocks(const Call& c, int index, const Tile& t, int group, int parts, int tid, uint4* h_lds,
+                                          Third<RT>* third_lds) {
   const Bank& b = c.bank;
   const int tokens = c.tile_token[index * kTileTokens + (tid & 63)];
   const AdapterSlot slot = t.slot >= 0 ? b.table[t.slot] : AdapterSlot{0, 0.f};
@@ -899,10 +970,10 @@ __device__ __forceinline__ void up_blocks(const Call& c, int index, const Tile& 
   // every load below goes out before the first of them is waited for; lanes without an output repeat another's address
   const int64_t rank_stride = 16 * b.rank_tiles;
   const float* low_h = c.low + __shfl(tokens, 16 * wave + (lane & 15), 64) * rank_stride + 4 * q;
-  uint4 h[RT];   // of the wave's column tile
+  v4f h[RT];   // of the wave's column tile
   if (RT > 1 || c.parts == 1) {
 #pragma unroll
-    for (int r = 0; r < RT; ++r) h[r] = ldg128((const uint8_t*)(low_h + 16 * max(min(r, tiles - 1), 0)));
+    for (int r = 0; r < RT; ++r) h[r] = load_h(low_h + 16 * max(min(r, tiles - 1), 0));
   }
   uint4 w[RT][2];
   {
@@ -918,13 +989,8 @@ __device__ __forceinline__ void up_blocks(const Call& c, int index, const Tile& 
   int64_t token[kColumns][2];
   load_base<kF32>(c, tokens, n, lane, base, token);
   if constexpr (RT == 1)
-    if (c.parts > 1 && tiles) h[0] = h_operand(slot, 4 * q, sum_parts(low_h, c.tokens * rank_stride, 0, 1, parts));
-#pragma unroll
-  for (int r = 0; r < RT; ++r) {
-    const int ranks = slot.rank - 16 * r - 4 * q;   // the sums past the slot's rank are not its own
-    if (ranks <= 0) h[r] = make_uint4(0, 0, 0, 0);
-    h_lds[(wave * RT + r) * 64 + lane] = h[r];
-  }
+    if (c.parts > 1 && tiles) h[0] = h_of(slot, 4 * q, sum_parts(low_h, c.tokens * rank_stride, 0, 1, parts));
+  put_h(h, slot.rank - 4 * q, h_lds + wave * RT * 64 + lane, third_lds + wave * kThirds<RT> * 64 + lane);
   mxd::lds_barrier();
   const int at_y = n + (low ? 0 : 32);
 #pragma unroll
@@ -932,14 +998,10 @@ __device__ __forceinline__ void up_blocks(const Call& c, int index, const Tile& 
     if (16 * i >= t.rows) break;
     v4f acc[4];
     from_base<kF32>(base[i], low, acc);
-    if (tiles == RT) {
-#pragma unroll
-      for (int r = 0; r < RT; ++r) up_tile(w[r], h_lds[(i * RT + r) * 64 + lane], acc);
-    } else {
-#pragma unroll
-      for (int r = 0; r < RT; ++r)
-        if (r < tiles) up_tile(w[r], h_lds[(i * RT + r) * 64 + lane], acc);
-    }
+    const uint4* two = h_lds + i * RT * 64 + lane;
+    const Third<RT>* third = third_lds + i * kThirds<RT> * 64 + lane;
+    if (tiles == RT) up_tiles<RT>(w, two, third, RT, acc);
+    else up_tiles<RT>(w, two, third, tiles, acc);
     store_y(c, t.rows, i, at_y, lane, low, token[i], acc);
   }
 }
@@ -949,8 +1011,9 @@ __device__ __forceinline__ void up_blocks(const Call& c, int index, const Tile& 
 // outputs: 218, 122 and 100 us in all; all 16 rank tiles at once 277, 218 and 186. (In a bank of 128 ranks eight at
 // once are the faster: rank 64 97 us and 107.)
 template <bool kF32>
-__device__ __forceinline__ void up_blocks_many(const Call& c, int index, const Tile& t, int group, int tid, uint4* h_lds) {
-  constexpr int RT = kTurnTiles;
+__device__ __forceinline__ void up_blocks_many(const Call& c, int index, const Tile& t, int group, int tid, uint4* h_lds,
+                                               uint4* third_lds) {
+  constexpr int RT = kTurnTiles, kPairs = RT / 2;   // third terms together
   const Bank& b = c.bank;
   const int tokens = c.tile_token[index * kTileTokens + (tid & 63)];
   const AdapterSlot slot = t.slot >= 0 ? b.table[t.slot] : AdapterSlot{0, 0.f};
@@ -968,44 +1031,43 @@ __device__ __forceinline__ void up_blocks_many(const Call& c, int index, const T
 #pragma unroll
   for (int i = 0; i < kColumns; ++i) from_base<kF32>(base[i], low, acc[i]);
   for (int r0 = 0; r0 < tiles; r0 += RT) {
-    uint4 h[RT], w[RT][2];
+    v4f h[RT];
+    uint4 w[RT][2];
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
       const int at = min(r0 + r, tiles - 1);
-      h[r] = ldg128((const uint8_t*)(low_h + 16 * at));
+      h[r] = load_h(low_h + 16 * at);
       w[r][0] = ldg128(up + 2048 * at), w[r][1] = ldg128(up + 2048 * at + 1024);
     }
     if (r0) __syncthreads();   // the h before this has been read
-#pragma unroll
-    for (int r = 0; r < RT; ++r) {
-      const int ranks = slot.rank - 16 * (r0 + r) - 4 * q;
-      if (ranks <= 0) h[r] = make_uint4(0, 0, 0, 0);
-      h_lds[(wave * RT + r) * 64 + lane] = h[r];
-    }
+    put_h(h, slot.rank - 16 * r0 - 4 * q, h_lds + wave * RT * 64 + lane, third_lds + wave * kPairs * 64 + lane);
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < kColumns; ++i)
-#pragma unroll
-      for (int r = 0; r < RT; ++r)
-        if (16 * i < t.rows && r0 + r < tiles) up_tile(w[r], h_lds[(i * RT + r) * 64 + lane], acc[i]);
+      if (16 * i < t.rows)
+        up_tiles<RT>(w, h_lds + i * RT * 64 + lane, third_lds + i * kPairs * 64 + lane, tiles - r0, acc[i]);
   }
 #pragma unroll
   for (int i = 0; i < kColumns; ++i)
     if (16 * i < t.rows) store_y(c, t.rows, i, n + (low ? 0 : 32), lane, low, token[i], acc[i]);
 }
 
-// RT rank tiles, or in turns if there are more. kTurns: for fewer workgroups than there can be tiles.
+// RT rank tiles, or in turns if there are more. kTurns: for fewer workgroups than there can be tiles. With room for two
+// waves a SIMD or more the compiler keeps the sums in VGPRs. It must: where it had them in AGPRs, its copy of a base that
+// no rank tile adds to (a tile without an adapter) held the first of four values four times.
 template <int RT, bool kF32, bool kTurns>
-__global__ __launch_bounds__(256) void adapter_up_kernel(Call c) {
-  __shared__ uint4 h_lds[kColumns * (RT > kMostTiles ? kTurnTiles : RT) * 64];
+__global__ __launch_bounds__(256, RT > 4 && RT <= kMostTiles && !kF32 ? 3 : 2) void adapter_up_kernel(Call c) {
+  constexpr int kHeld = RT > kMostTiles ? kTurnTiles : RT;
+  __shared__ uint4 h_lds[kColumns * kHeld * 64];
+  __shared__ Third<RT> third_lds[kColumns * (RT > kMostTiles ? kTurnTiles / 2 : kThirds<RT>) * 64];
   const int groups = (c.bank.blocks + 3) / 4, group = blockIdx.x % groups;
   int index = blockIdx.x / groups;
   Tile t = c.tile[index];
   const Tile all = c.tile[c.tiles];
   if (t.rows == 0) return;
   auto blocks = [&](const Tile& tile, int tid) {
-    if constexpr (RT <= kMostTiles) up_blocks<RT, kF32>(c, index, tile, group, all.slot, tid, h_lds);
-    else up_blocks_many<kF32>(c, index, tile, group, tid, h_lds);
+    if constexpr (RT <= kMostTiles) up_blocks<RT, kF32>(c, index, tile, group, all.slot, tid, h_lds, third_lds);
+    else up_blocks_many<kF32>(c, index, tile, group, tid, h_lds, third_lds);
   };
   blocks(t, threadIdx.x);
   if constexpr (kTurns)
