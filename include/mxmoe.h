@@ -395,9 +395,10 @@ uint64_t mx_adapters_workspace_bytes(const mx_adapters* a, int32_t tokens);
  * BF16(base[t]) where ids[t] is outside [0, slots) or its slot empty. x BF16 [T][k], base [T][n] BF16 or FP32 (base_type MX_ROWS_BF16 / _F32: a
  * projection's output, or its trace), y BF16 [T][n]; rows `stride` values apart (a multiple of 8; 4 for an FP32 base),
  * all 16-byte aligned. y may be base (BF16, one stride); other overlaps are not supported. tokens in [0, 2^18].
- * plan NULL, or mx_dispatch's plan of ids with top_k 1 and groups = slots (made once for all projections of a step);
- * calls of few tokens do not use it, and by one whose groups do not cover the tokens in order y stays as it was. Calls
- * that share a workspace must not overlap. The order of the sums follows the number of tokens and of each slot's. */
+ * plan NULL, or mx_dispatch's plan of ids with top_k 1 and groups = slots (made once for all projections of a step; its
+ * first must hold slots + 1 numbers). Calls of up to 128 tokens (64 if max_rank is above 64) do not read it; by one whose
+ * groups do not cover the tokens in order y stays as it was. Calls that share a workspace must not overlap. The order of
+ * the sums follows the number of tokens and of each slot's. */
 int mx_adapters_apply(mx_adapters* a, const uint16_t* x, int64_t x_stride, const int32_t* ids, const mx_row_plan* plan,
                       int32_t tokens, const void* base, int32_t base_type, int64_t base_stride, uint16_t* y,
                       int64_t y_stride, void* workspace, uint64_t workspace_bytes, void* stream);

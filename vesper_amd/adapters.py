@@ -18,6 +18,7 @@ import math
 import numpy as np
 
 from . import _lib
+from .dispatch import ExpertDispatch, RowPlan
 
 MAX_SLOTS, MAX_RANK, MAX_TOKENS, MAX_SIZE = 1024, 256, 1 << 18, 1 << 20
 
@@ -38,6 +39,7 @@ class AdapterBank:
                              f"[1, {MAX_TOKENS}] required")
         self.ctx, self.rows, self.width = ctx, int(rows), int(width)
         self.slots, self.max_rank, self.max_tokens = int(slots), int(max_rank), int(max_tokens)
+        self.few_tokens = 128 if self.max_rank <= 64 else 64   # calls of up to so many find each adapter's tokens anew
         handle = C.c_void_p()
         ctx.lib.adapters_create(ctx._h(), self.rows, self.width, self.slots, self.max_rank, C.byref(handle))
         self.handle, self.workspace = handle, 0
@@ -108,13 +110,15 @@ class AdapterBank:
     def apply_device(self, x_ptr, ids_ptr, tokens: int, base_ptr, y_ptr, base_dtype: str = "bf16", x_stride=None,
                      base_stride=None, y_stride=None, plan=None, stream=None):
         """y [tokens, rows] BF16 of x [tokens, width] BF16, base [tokens, rows] and int32 ids [tokens]; strides in
-        values (None: contiguous). plan: the MxRowPlan of ids (ExpertDispatch(ctx, slots, 1, tokens).plan after
-        plan_device), made once for all projections of a step; None makes it within the call. No synchronisation."""
+        values (None: contiguous). plan: ExpertDispatch(ctx, slots, 1, tokens) after plan_device(ids, tokens), or its
+        .plan, made once for all projections of a step whose banks have as many slots; None makes it within the call,
+        and up to few_tokens no plan is read. (An MxRowPlan of a caller's own is taken as it is.) No synchronisation."""
         self._open()
         if not 0 <= tokens <= self.max_tokens:
             raise ValueError(f"token count outside [0, {self.max_tokens}]")
         if base_dtype not in ("bf16", "f32"):
             raise ValueError("base type must be bf16 or f32")
+        plan = self.check_plan(plan, tokens)
         ptr = _lib.ptr
         x_stride = self.width if x_stride is None else x_stride
         base_stride = self.rows if base_stride is None else base_stride
@@ -123,6 +127,24 @@ class AdapterBank:
                                     None if plan is None else C.byref(plan), tokens, ptr(base_ptr),
                                     _lib.MX_ROWS[base_dtype], base_stride, ptr(y_ptr), y_stride, self.workspace,
                                     self.workspace_bytes, None if stream is None else int(stream))
+
+    def check_plan(self, plan, tokens: int) -> _lib.MxRowPlan | None:
+        """The plan that a call of `tokens` tokens reads, None if it reads none."""
+        if plan is None:
+            return None
+        if not isinstance(plan, (ExpertDispatch, _lib.MxRowPlan)):
+            raise TypeError("plan must be an ExpertDispatch or its plan")
+        if tokens <= self.few_tokens:
+            return None
+        if isinstance(plan, RowPlan):
+            plan = plan.dispatch
+        if not isinstance(plan, ExpertDispatch):
+            return plan
+        made = plan._open()
+        if (plan.experts, plan.top_k, made, plan.ctx.ordinal) != (self.slots, 1, tokens, self.ctx.ordinal):
+            raise ValueError(f"the plan is of {made} tokens with {plan.top_k} of {plan.experts} groups on device "
+                             f"{plan.ctx.ordinal}; this call takes {tokens} with 1 of {self.slots} on {self.ctx.ordinal}")
+        return plan.plan
 
     def check_ids(self, ids, tokens: int) -> np.ndarray:
         """Host slot ids [tokens] as int32: each a slot of the bank, or -1 for none."""

@@ -45,6 +45,14 @@ def host_rows(array, rows: int | None = None, bytes_too: bool = False):
     return np.ascontiguousarray(array), name
 
 
+class RowPlan(_lib.MxRowPlan):
+    """The device addresses of an ExpertDispatch's plan, and the object that knows what it was made for."""
+
+    def __init__(self, dispatch: ExpertDispatch):
+        super().__init__(dispatch.first, dispatch.pair_row, dispatch.row_pair)
+        self.dispatch = dispatch
+
+
 class ExpertDispatch:
     def __init__(self, ctx: _lib.Context, experts: int, top_k: int, max_tokens: int):
         if not 1 <= experts <= MAX_EXPERTS or not 1 <= top_k <= MAX_TOP_K or not 1 <= max_tokens <= MAX_TOKENS:
@@ -60,8 +68,8 @@ class ExpertDispatch:
             self.close()
             raise
         self.first, self.pair_row, self.row_pair = (d.ptr for d in self._owned)
-        self.plan = _lib.MxRowPlan(self.first, self.pair_row, self.row_pair)
         self.tokens = None   # of the plan in the buffers
+        self.plan = RowPlan(self)
 
     def close(self):
         for d in self._owned:

@@ -168,10 +168,12 @@ class NativeProjections:
 
         adapters_ptr (device int32 [T], the slots of open_adapters, -1 for none) adds each row's adapter: to the FP32
         sums where trace_ptr keeps them, else to y. x must then outlive the projection (y and trace apart from x);
-        plan as in AdapterBank.apply_device."""
+        plan as in AdapterBank.apply_device, refused before the projection runs."""
         self._ready()
         rows, width = self.layout[name]
         bank = None if adapters_ptr is None else self._bank(name, int(tokens))
+        if bank is not None:   # what cannot be is refused before the projection has run
+            plan = bank.check_plan(plan, int(tokens))
         self.ctx.lib.fp8_projection(self.ctx._h(), C.c_void_p(self.tiled[name]), rows, width, self.block,
                                     C.c_void_p(int(x_ptr)), int(tokens), C.c_void_p(int(y_ptr)),
                                     _lib.vp(trace_ptr), _lib.vp(q_ptr), _lib.vp(s_ptr), _lib._stream(stream))
