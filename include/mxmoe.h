@@ -386,7 +386,8 @@ typedef struct mx_adapters mx_adapters;
 int mx_adapters_create(mx_ctx* ctx, int32_t n, int32_t k, int32_t slots, int32_t max_rank, mx_adapters** out);
 int mx_adapters_destroy(mx_adapters* a);
 /* Fill `slot` from device memory, ordered on `stream` (rank 0, with NULL weights: empty it). Calls of
- * mx_adapters_apply ordered after it see the new adapter. */
+ * mx_adapters_apply ordered after it see the new adapter. The scale is finite, and so must down and up be: an infinite up
+ * gives NaN, since the parts that h goes into the product in may be zero beside it. */
 int mx_adapters_load(mx_adapters* a, int32_t slot, const uint16_t* down, const uint16_t* up, int32_t rank, float scale,
                      void* stream);
 /* Bytes of workspace (256-byte aligned device memory) for calls of up to `tokens` tokens. */

@@ -76,12 +76,13 @@ class AdapterBank:
             raise ValueError(f"slot outside [0, {self.slots})")
         if not 1 <= rank <= self.max_rank:
             raise ValueError(f"adapter rank outside [1, {self.max_rank}]")
-        if not math.isfinite(scale):
-            raise ValueError("adapter scale must be finite")
+        if not math.isfinite(C.c_float(scale).value):
+            raise ValueError("adapter scale must be a finite FP32 value")
 
     # -- loading ----------------------------------------------------------------------------------
     def load_device(self, slot: int, down_ptr, up_ptr, rank: int, scale: float = 1.0, stream=None):
-        """Slot <- device BF16 down [rank, width] and up [rows, rank], ordered on `stream`."""
+        """Slot <- device BF16 down [rank, width] and up [rows, rank], ordered on `stream`. The weights must be finite
+        (load checks it)."""
         self._slot(slot, rank, scale)
         self.ctx.lib.adapters_load(self.handle, slot, _lib.vp(down_ptr), _lib.vp(up_ptr), int(rank), float(scale),
                                    _lib._stream(stream))

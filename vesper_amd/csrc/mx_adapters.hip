@@ -22,6 +22,7 @@
 // token's workgroups find the tokens that share its adapter by a ballot, one launch or two. Larger calls sort the
 // tokens by adapter into tiles of 64 and read each weight once a tile; x, base and y, once each, then bound them.
 #include <algorithm>
+#include <cmath>
 #include <new>
 #include <type_traits>
 
@@ -1254,6 +1255,7 @@ int mx_adapters_load(mx_adapters* a, int32_t slot, const uint16_t* down, const u
   MX_REQUIRE(rank >= 0 && rank <= a->max_rank, "%s: rank %d outside [0, %d]", who, rank, a->max_rank);
   MX_REQUIRE(rank == 0 || (down && up), "%s: null pointer", who);
   MX_REQUIRE(is_aligned(down, 2) && is_aligned(up, 2), "%s: weights must be 2-byte aligned", who);
+  MX_REQUIRE(std::isfinite(scale), "%s: the scale must be finite", who);
   if (int s = use(a->ctx)) return s;
   const Bank& b = a->bank;
   hipStream_t st = as_stream(stream);
