@@ -198,13 +198,18 @@ class NativeProjections:
                     raise ValueError("adapters must name one slot per row of values")
                 ids = self._bank(name, tokens).check_ids(ids.reshape(tokens), tokens)
             sdt, sw = (np.uint8, width // 32) if self.block == 32 else (np.float32, width // 128)
-            x = self.ctx.upload(np.ascontiguousarray(values).reshape(tokens, width))
-            q = self.ctx.empty((tokens, width), np.uint8)
-            s = self.ctx.empty((tokens, sw), sdt)
-            trace = self.ctx.empty((tokens, rows), np.float32)
-            out = self.ctx.empty((tokens, rows), np.uint16)
-            slots = None if ids is None else self.ctx.upload(ids)
+            dev = []
+
+            def on_device(make, *args):
+                dev.append(make(*args))
+                return dev[-1]
             try:
+                x = on_device(self.ctx.upload, np.ascontiguousarray(values).reshape(tokens, width))
+                q = on_device(self.ctx.empty, (tokens, width), np.uint8)
+                s = on_device(self.ctx.empty, (tokens, sw), sdt)
+                trace = on_device(self.ctx.empty, (tokens, rows), np.float32)
+                out = on_device(self.ctx.empty, (tokens, rows), np.uint16)
+                slots = None if ids is None else on_device(self.ctx.upload, ids)
                 self.project_device(name, x.ptr, tokens, out.ptr, trace_ptr=trace, q_ptr=q, s_ptr=s, adapters_ptr=slots)
                 scale_key = "scale_e8m0" if self.block == 32 else "scale_f32"
                 return {"input_fp8": q.download().reshape(*lead, width),
@@ -212,7 +217,7 @@ class NativeProjections:
                         "output_fp32": trace.download().reshape(*lead, rows),
                         "output_bf16": out.download().reshape(*lead, rows)}
             finally:
-                for d in (x, q, s, trace, out) + (() if slots is None else (slots,)):
+                for d in dev:
                     d.free()
 
     def grouped(self, values):
