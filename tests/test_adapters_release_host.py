@@ -1,4 +1,4 @@
-"""What a failing call leaves behind: nothing that is allocated."""
+"""What a failing call and a failing close leave behind: nothing that is allocated, and no open context."""
 
 import numpy as np
 import pytest
@@ -11,13 +11,17 @@ from vesper_amd.resources import MemoryBudget
 
 class Lib:
     def __init__(self):
-        self.cdll = self
+        self.cdll, self.fail_destroy = self, False
 
     def mx_adapters_workspace_bytes(self, *_):
         return 256
 
     def adapters_create(self, *args):
         args[-1]._obj.value = 0x10000
+
+    def adapters_destroy(self, *_):
+        if self.fail_destroy:
+            raise _lib.HipError("destroy")
 
     def __getattr__(self, name):
         return lambda *args: None
@@ -29,7 +33,7 @@ class Context:
     ordinal = 0
 
     def __init__(self):
-        self.lib, self.live, self.next, self.left = Lib(), set(), 0x1000, None
+        self.lib, self.live, self.next, self.left, self.closed = Lib(), set(), 0x1000, None, False
 
     def _h(self):
         return None
@@ -58,6 +62,9 @@ class Context:
     def owned_bytes(self):
         return len(self.live), len(self.live)
 
+    def close(self):
+        self.closed = True
+
 
 @pytest.fixture
 def proj():
@@ -84,3 +91,13 @@ def test_fp8_frees_what_it_allocated_when_an_allocation_fails(proj, with_adapter
     proj.ctx.left = None
     assert proj.fp8("o", values, ids)["output_bf16"].shape == (3, 64)
     assert proj.ctx.live == before
+
+
+def test_the_context_closes_although_a_bank_does_not(proj):
+    ctx = proj.ctx
+    proj.open_adapters("o", 2, 4, 8)
+    ctx.lib.fail_destroy = True
+    with pytest.raises(_lib.HipError):
+        proj.__exit__(None, None, None)
+    assert ctx.closed and proj.ctx is None and not proj.banks and not proj.opened and not proj.tiled
+    assert proj.budget.reserved == 0

@@ -18,6 +18,7 @@ of the output.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import math
 import threading
@@ -118,12 +119,13 @@ class NativeProjections:
                 raise
 
     def _close_context(self):
-        while self.banks:
-            self.banks.popitem()[1].close()
-        self._device_peak = max(self._device_peak, self.ctx.owned_bytes()[1])
-        self.ctx.close()
-        self.ctx = None
-        self.budget.release(HOST_ALLOWANCE)
+        with contextlib.ExitStack() as steps:   # from the last to the first, each whether or not the others fail
+            steps.callback(self.budget.release, HOST_ALLOWANCE)
+            ctx, self.ctx = self.ctx, None
+            steps.callback(ctx.close)
+            self._device_peak = max(self._device_peak, ctx.owned_bytes()[1])
+            while self.banks:
+                steps.callback(self.banks.popitem()[1].close)
 
     def _ready(self):
         if not self.opened:
@@ -274,6 +276,6 @@ class NativeProjections:
     def __exit__(self, *_):
         with self.lock:
             self.opened = False
+            self.tiled.clear()
             if self.ctx is not None:
                 self._close_context()
-            self.tiled.clear()
