@@ -127,6 +127,9 @@ int mx_read_kernel(mx_ctx* ctx, const void* src, uint64_t bytes, uint32_t* out, 
  * prefill epilogue with the bit-exact software encoder on every FP32 bit pattern (clamped to +-448 as the
  * activation quantizers clamp); *mismatches receives the count, 0 when they agree. Synchronous. */
 int mx_check_e4m3_pack(mx_ctx* ctx, uint64_t* mismatches);
+/* The same for the hardware rounding of two FP32 values to BF16, which combine and the adapters use, against the software
+ * rounding on every FP32 bit pattern (NaN included), in either half. */
+int mx_check_bf16_pair(mx_ctx* ctx, uint64_t* mismatches);
 
 /* out[r][k] = E2M1(packed[r][k/2] nibble, low first) * E8M0(scales[r][k/32]); bit-exact. */
 int mx_dequant_mxfp4(mx_ctx* ctx, const uint8_t* packed, const uint8_t* scales, float* out,

@@ -157,6 +157,7 @@ SIGNATURES = {
     "mx_audit_gate": ([_P, _P, _I32, _P, _I32, _P, _U64, _P], C.c_int),
     "mx_owned_size": ([_P, _P, C.POINTER(_U64)], C.c_int),
     "mx_check_e4m3_pack": ([_P, C.POINTER(_U64)], C.c_int),
+    "mx_check_bf16_pair": ([_P, C.POINTER(_U64)], C.c_int),
 }
 
 _lock = threading.Lock()

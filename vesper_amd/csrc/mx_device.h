@@ -148,7 +148,7 @@ __device__ __forceinline__ float bf16_round_sel(float f) {
 }
 
 // mx::bf16_bits of two values, the first in the low half: one V_CVT_PK_BF16_F32, equal to the software rounding on
-// every FP32 bit pattern (NaN included; checked on gfx950 over all 2^32).
+// every FP32 bit pattern (NaN included): mx_check_bf16_pair.
 __device__ __forceinline__ uint32_t bf16_pair(float lo, float hi) {
   typedef float f2 __attribute__((ext_vector_type(2)));
   typedef __bf16 b2 __attribute__((ext_vector_type(2)));

@@ -135,6 +135,38 @@ __global__ __launch_bounds__(256) void e4m3_pack_check_kernel(uint32_t* counts) 
   counts[tid] = bad;
 }
 
+// mxd::bf16_pair in both halves, against the software rounding on every FP32 bit pattern: per-thread mismatch counts.
+__global__ __launch_bounds__(256) void bf16_pair_check_kernel(uint32_t* counts) {
+  const uint32_t tid = blockIdx.x * blockDim.x + threadIdx.x, threads = gridDim.x * blockDim.x;
+  uint32_t bad = 0;
+  for (uint64_t m = tid; m < (1ull << 32); m += threads) {
+    const uint32_t other = (uint32_t)m * 0x9E3779B1u + 1;
+    const float v = mx::u2f((uint32_t)m), o = mx::u2f(other);
+    bad += mxd::bf16_pair(v, o) != (mx::bf16_bits(v) | mx::bf16_bits(o) << 16);
+    bad += mxd::bf16_pair(o, v) != (mx::bf16_bits(o) | mx::bf16_bits(v) << 16);
+  }
+  counts[tid] = bad;
+}
+
+// The sum of what the threads of a check kernel counted.
+static int count_mismatches(mx_ctx* ctx, const char* who, void (*kernel)(uint32_t*), uint64_t* mismatches) {
+  if (int st = use(ctx)) return st;
+  MX_REQUIRE(mismatches != nullptr, "%s: null output", who);
+  constexpr int kBlocks = 4096, kThreads = 256;
+  uint32_t* d = nullptr;
+  MX_HIP(hipMalloc(&d, sizeof(uint32_t) * kBlocks * kThreads));
+  std::vector<uint32_t> h(kBlocks * kThreads);
+  hipLaunchKernelGGL(kernel, dim3(kBlocks), dim3(kThreads), 0, nullptr, d);
+  hipError_t e = hipGetLastError();
+  if (e == hipSuccess) e = hipMemcpy(h.data(), d, sizeof(uint32_t) * h.size(), hipMemcpyDeviceToHost);
+  (void)hipFree(d);
+  if (e != hipSuccess) return hip_fail(e, who);
+  uint64_t total = 0;
+  for (uint32_t c : h) total += c;
+  *mismatches = total;
+  return MX_OK;
+}
+
 namespace mxi {
 
 int act_quant32_scaled(mx_ctx* ctx, const uint16_t* x, uint8_t* q, uint8_t* scales, uint16_t* scaled, int64_t rows,
@@ -158,21 +190,11 @@ int act_quant32_scaled(mx_ctx* ctx, const uint16_t* x, uint8_t* q, uint8_t* scal
 extern "C" {
 
 int mx_check_e4m3_pack(mx_ctx* ctx, uint64_t* mismatches) {
-  if (int st = use(ctx)) return st;
-  MX_REQUIRE(mismatches != nullptr, "mx_check_e4m3_pack: null output");
-  constexpr int kBlocks = 4096, kThreads = 256;
-  uint32_t* d = nullptr;
-  MX_HIP(hipMalloc(&d, sizeof(uint32_t) * kBlocks * kThreads));
-  std::vector<uint32_t> h(kBlocks * kThreads);
-  hipLaunchKernelGGL(e4m3_pack_check_kernel, dim3(kBlocks), dim3(kThreads), 0, nullptr, d);
-  hipError_t e = hipGetLastError();
-  if (e == hipSuccess) e = hipMemcpy(h.data(), d, sizeof(uint32_t) * h.size(), hipMemcpyDeviceToHost);
-  (void)hipFree(d);
-  if (e != hipSuccess) return hip_fail(e, "mx_check_e4m3_pack");
-  uint64_t total = 0;
-  for (uint32_t c : h) total += c;
-  *mismatches = total;
-  return MX_OK;
+  return count_mismatches(ctx, "mx_check_e4m3_pack", e4m3_pack_check_kernel, mismatches);
+}
+
+int mx_check_bf16_pair(mx_ctx* ctx, uint64_t* mismatches) {
+  return count_mismatches(ctx, "mx_check_bf16_pair", bf16_pair_check_kernel, mismatches);
 }
 
 int mx_dequant_mxfp4(mx_ctx* ctx, const uint8_t* packed, const uint8_t* scales, float* out, int64_t rows,
