@@ -24,7 +24,6 @@
 #include <algorithm>
 #include <cmath>
 #include <new>
-#include <type_traits>
 
 #include "mx_device.h"
 #include "mx_internal.h"
@@ -703,10 +702,10 @@ __device__ __forceinline__ void up_mfma(uint4 a0, uint4 a1, uint4 b0, uint4 b1, 
   acc[3] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf(make_uint4(a1.z, a1.w, b1.z, b1.w)), v, acc[3], 0, 0, 0);
 }
 
-// Up of RT rank tiles at most, `count` of them the slot's. This lane's terms of tile r of a column tile lie at two[64 r];
-// the third terms either of two tiles together, at third[64 (r / 2)], in one MFMA, or of each alone, at third[64 r], in
-// one of its own. Together is the fewer MFMAs, alone the fewer moves between registers: 4096 tokens of 8 adapters, 1536
-// columns and 24576 rows, rank 64 (FP32 base) 141 us together and 136 alone, 128 (BF16 base) 136 and 147, 256 210 and 220.
+// Up of RT rank tiles at most, `count` of them the slot's (up's others may hold anything). This lane's terms of tile r of
+// a column tile lie at two[64 r] and, the third ones of two tiles together, at third[64 (r / 2)]. 4096 tokens of 8 adapters
+// of rank 128 and 256 (BF16 base), 1536 columns and 24576 rows: 136 and 210 us, with an MFMA for the third terms of each
+// tile 147 and 220; of rank 64 no different.
 template <int RT>
 __device__ __forceinline__ void up_tiles(const uint4 (&w)[RT][2], const uint4* two, const uint4* third, int count,
                                          v4f (&acc)[4]) {
@@ -718,17 +717,6 @@ __device__ __forceinline__ void up_tiles(const uint4 (&w)[RT][2], const uint4* t
     if (r % 2) up_mfma(w[r - 1][0], w[r - 1][1], w[r][0], w[r][1], rest, acc);
     else if (r + 1 >= count) up_mfma(w[r][0], w[r][1], w[r][0], w[r][1], make_uint4(rest.x, rest.y, 0, 0), acc);
   }
-}
-template <int RT>
-__device__ __forceinline__ void up_tiles(const uint4 (&w)[RT][2], const uint4* two, const uint2* third, int count,
-                                         v4f (&acc)[4]) {
-#pragma unroll
-  for (int r = 0; r < RT; ++r)
-    if (r < count) {
-      const uint2 rest = third[64 * r];
-      up_mfma(w[r][0], w[r][1], w[r][0], w[r][1], two[64 * r], acc);
-      up_mfma(w[r][0], w[r][1], w[r][0], w[r][1], make_uint4(rest.x, rest.y, 0, 0), acc);
-    }
 }
 
 // Few tokens, grid (output blocks / 4, T), 4 waves, a block of 64 outputs each for up to 16 tokens of an adapter (24
@@ -937,22 +925,17 @@ __device__ __forceinline__ void store_y(const Call& c, int rows, int i, int at, 
 
 // A column tile's terms into LDS for up_tiles; `ranks` is how many ranks the slot has from this lane's first on: the sums
 // past them are not its own.
-template <int RT, typename Third>
-__device__ __forceinline__ void put_h(const v4f (&h)[RT], int ranks, uint4* two, Third* third) {
+template <int RT>
+__device__ __forceinline__ void put_h(const v4f (&h)[RT], int ranks, uint4* two, uint4* third) {
   Terms t[RT];
 #pragma unroll
   for (int r = 0; r < RT; ++r) {
     t[r] = split(ranks > 16 * r ? h[r] : v4f{0.f, 0.f, 0.f, 0.f});
     two[64 * r] = t[r].two;
-    if constexpr (sizeof(Third) == 8) third[64 * r] = t[r].third;
-    else if (r % 2) third[64 * (r / 2)] = make_uint4(t[r - 1].third.x, t[r - 1].third.y, t[r].third.x, t[r].third.y);
+    if (r % 2) third[64 * (r / 2)] = make_uint4(t[r - 1].third.x, t[r - 1].third.y, t[r].third.x, t[r].third.y);
+    else if (r + 1 == RT) third[64 * (r / 2)] = make_uint4(t[r].third.x, t[r].third.y, 0, 0);
   }
 }
-// How the workgroups of RT rank tiles hold the third terms, and how many of them a column tile has.
-template <int RT>
-using Third = std::conditional_t<(RT > 4), uint4, uint2>;
-template <int RT>
-constexpr int kThirds = RT > 4 ? RT / 2 : RT;
 
 // Grouped form: a tile of 64 tokens and four blocks of 64 outputs, one a wave, its weights of all ranks in registers
 // for the tile's columns, 16 tokens at a time. What does not depend on h is asked for before h goes to LDS. Bound by
@@ -960,7 +943,8 @@ constexpr int kThirds = RT > 4 ? RT / 2 : RT;
 // first 37.
 template <int RT, bool kF32>
 __device__ __forceinline__ void up_blocks(const Call& c, int index, const Tile& t, int group, int parts, int tid, uint4* h_lds,
-                                          Third<RT>* third_lds) {
+                                          uint4* third_lds) {
+  constexpr int kPairs = (RT + 1) / 2;
   const Bank& b = c.bank;
   const int tokens = c.tile_token[index * kTileTokens + (tid & 63)];
   const AdapterSlot slot = t.slot >= 0 ? b.table[t.slot] : AdapterSlot{0, 0.f};
@@ -991,7 +975,7 @@ __device__ __forceinline__ void up_blocks(const Call& c, int index, const Tile& 
   load_base<kF32>(c, tokens, n, lane, base, token);
   if constexpr (RT == 1)
     if (c.parts > 1 && tiles) h[0] = h_of(slot, 4 * q, sum_parts(low_h, c.tokens * rank_stride, 0, 1, parts));
-  put_h(h, slot.rank - 4 * q, h_lds + wave * RT * 64 + lane, third_lds + wave * kThirds<RT> * 64 + lane);
+  put_h(h, slot.rank - 4 * q, h_lds + wave * RT * 64 + lane, third_lds + wave * kPairs * 64 + lane);
   mxd::lds_barrier();
   const int at_y = n + (low ? 0 : 32);
 #pragma unroll
@@ -999,8 +983,7 @@ __device__ __forceinline__ void up_blocks(const Call& c, int index, const Tile& 
     if (16 * i >= t.rows) break;
     v4f acc[4];
     from_base<kF32>(base[i], low, acc);
-    const uint4* two = h_lds + i * RT * 64 + lane;
-    const Third<RT>* third = third_lds + i * kThirds<RT> * 64 + lane;
+    const uint4 *two = h_lds + i * RT * 64 + lane, *third = third_lds + i * kPairs * 64 + lane;
     if (tiles == RT) up_tiles<RT>(w, two, third, RT, acc);
     else up_tiles<RT>(w, two, third, tiles, acc);
     store_y(c, t.rows, i, at_y, lane, low, token[i], acc);
@@ -1014,7 +997,7 @@ __device__ __forceinline__ void up_blocks(const Call& c, int index, const Tile& 
 template <bool kF32>
 __device__ __forceinline__ void up_blocks_many(const Call& c, int index, const Tile& t, int group, int tid, uint4* h_lds,
                                                uint4* third_lds) {
-  constexpr int RT = kTurnTiles, kPairs = RT / 2;   // third terms together
+  constexpr int RT = kTurnTiles, kPairs = RT / 2;
   const Bank& b = c.bank;
   const int tokens = c.tile_token[index * kTileTokens + (tid & 63)];
   const AdapterSlot slot = t.slot >= 0 ? b.table[t.slot] : AdapterSlot{0, 0.f};
@@ -1055,12 +1038,13 @@ __device__ __forceinline__ void up_blocks_many(const Call& c, int index, const T
 
 // RT rank tiles, or in turns if there are more. kTurns: for fewer workgroups than there can be tiles. With room for two
 // waves a SIMD or more the compiler keeps the sums in VGPRs. It must: where it had them in AGPRs, its copy of a base that
-// no rank tile adds to (a tile without an adapter) held the first of four values four times.
+// no rank tile adds to (a tile without an adapter) held the first of four values four times. At most three waves: rank 64,
+// 8 adapters, 4096 tokens, 1536 columns and 24576 rows take 106 us (FP32 base 131), with no such limit 112 (137).
 template <int RT, bool kF32, bool kTurns>
-__global__ __launch_bounds__(256, RT > 4 && RT <= kMostTiles && !kF32 ? 3 : 2) void adapter_up_kernel(Call c) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 3))) void adapter_up_kernel(Call c) {
   constexpr int kHeld = RT > kMostTiles ? kTurnTiles : RT;
   __shared__ uint4 h_lds[kColumns * kHeld * 64];
-  __shared__ Third<RT> third_lds[kColumns * (RT > kMostTiles ? kTurnTiles / 2 : kThirds<RT>) * 64];
+  __shared__ uint4 third_lds[kColumns * ((kHeld + 1) / 2) * 64];
   const int groups = (c.bank.blocks + 3) / 4, group = blockIdx.x % groups;
   int index = blockIdx.x / groups;
   Tile t = c.tile[index];
@@ -1094,9 +1078,9 @@ int tiles_of(const Bank& b, int tokens) {
 bool is_few(const Bank& b, int tokens) { return tokens <= (b.rank_tiles <= 4 ? kFewTokens : kFewTokens / 2); }
 
 // Parts of K. Few tokens: as many as give each wave a unit of 64, since how many adapters the tokens share is not known
-// here. Grouped form: the most that `split` may take: as many as are resident together (two a CU) and no more, since a
-// few beyond would run alone after the rest, if every tile is full; at least two stages each. In both, parts T is at
-// most kWantGroups kTileTokens + T.
+// here. Grouped form: the most that down may take (locate): as many as are resident together (two a CU) and no more,
+// since a few beyond would run alone after the rest, if every tile is full; at least two stages each. In both, parts T is
+// at most kWantGroups kTileTokens + T.
 int parts_of(const Bank& b, int tokens) {
   if (is_few(b, tokens)) return std::max(1, std::min(kMaxParts, b.chunks / 8));
   return std::max(1, std::min({kMaxParts, b.k / (2 * kStageK), kWantGroups * kTileTokens / tokens}));

@@ -60,7 +60,8 @@ inline hipStream_t as_stream(void* s) { return reinterpret_cast<hipStream_t>(s);
 int act_quant32_scaled(mx_ctx* ctx, const uint16_t* x, uint8_t* q, uint8_t* scales, uint16_t* scaled, int64_t rows,
                        int64_t width, hipStream_t stream);
 
-// The plan of mx_dispatch (mx_dispatch.hip): pairs ids -> plan, one launch; the caller has checked the arguments.
+// The plan of mx_dispatch (mx_dispatch.hip): pairs ids -> plan; the caller has checked the arguments. One launch, or for
+// many pairs three, which keep their counts in row_pair and pair_row meanwhile.
 int row_plan(const int32_t* ids, int32_t pairs, int32_t groups, const mx_row_plan& plan, hipStream_t stream);
 
 // What other translation units need of a decode layer (defined with the layer in mx_moe.hip).
