@@ -46,15 +46,16 @@ constexpr int kTurnTiles = 4;
 constexpr int kMaxParts = 32;      // parts of K
 // A call of few tokens is one launch if down and the x of its tokens (of 64 at most, since the tokens of a workgroup
 // are 16 of one adapter) are no more than this: each of its workgroups reads all of down. One launch and two, rank 12
-// (one rank tile) of K columns, tokens of adapters: K = 1536, 1 of 1 5.0 and 7.4 us, 16 of 16 7.1 and 9.4, 120 of 2
-// 13.4 and 15.4; 5120, 1 of 1 5.5 and 7.4, 16 of 4 6.6 and 7.7, 40 of 9 7.4 and 8.1, 64 of 3 10.0 and 8.2; 7168, 4 of 4
-// 6.7 and 7.6, 16 of 1 9.7 and 7.6, of 16 7.2 and 7.8, 64 of 3 12.2 and 8.2; 16384, 1 of 1 10.3 and 7.0. Rank 32: 1536,
-// 120 of 2 16.3 and 17.2; 7168, 1 of 1 7.8 and 7.0. Four rank tiles take too many registers: 10.2 and 7.1.
+// (one rank tile), BF16 base, tokens of adapters: 1536 columns and 24576 rows, 1 of 1 4.5 and 7.1 us, 16 of 16 7.2 and
+// 9.8, 120 of 2 13.0 and 14.9; 5120 and 1280, 1 of 1 5.7 and 8.4, 16 of 4 6.9 and 8.6, 40 of 9 7.2 and 8.8, 64 of 3 10.3
+// and 9.0; 7168 and 1536, 4 of 4 6.8 and 8.4, 16 of 1 9.8 and 8.5, of 16 7.4 and 8.5, 64 of 3 12.4 and 9.1; 16384 and
+// 7168, 1 of 1 10.9 and 8.6. Rank 32: 1536 and 24576, 120 of 2 15.9 and 16.6; 7168 and 1536, 1 of 1 8.6 and 8.4. Four
+// rank tiles take too many registers: 10.2 and 7.1.
 constexpr int kFusedBytes = 320 << 10;
 // Calls whose x, base and y exceed this read x past the caches, which leaves them to the weights, base and y. Past them
-// and through, three sets in turn, 8 adapters of rank 64 or 32: 1000 tokens of 16384 to 7168 (62 MB) 30.6 and 31.0 us,
-// 1500 (92 MB) 33.8 and 37.7, 2000 (123 MB) 43.3 and 48.5, 4096 (252 MB) 72.9 and 72.3; 2500 of 7168 to 1536 (51 MB)
-// 23.4 and 22.5, 4000 (82 MB) 28.5 and 28.1. (For y it makes no difference.)
+// and through, three sets in turn, BF16 base, 8 adapters: of rank 64, 1000 tokens of 16384 to 7168 (62 MB) 30.9 and 31.0
+// us, 1500 (92 MB) 34.8 and 38.5, 2000 (123 MB) 41.7 and 46.9, 4096 (252 MB) 74.0 and 73.9; of rank 32, 2500 of 7168 to
+// 1536 (51 MB) 24.2 and 22.7, 4000 (82 MB) 29.8 and 28.8. (For y it makes no difference.)
 constexpr int64_t kStreamBytes = 80 << 20;
 constexpr int kWantGroups = 512;   // workgroups that the split of K aims at
 
@@ -148,8 +149,8 @@ __device__ __forceinline__ int on_xcd(int id, int count) { return (id & 7) * ((c
 // What a workgroup of down does: a part of K and a group of rank tiles for a tile. The split of K follows the tiles
 // that there are, which only the device knows: the slots that no token names make none (600 tokens of 8 adapters of
 // rank 64 by 16384 in a bank of 1024 slots 27 us, split by the tiles that there could be 78), and a slot of fewer ranks
-// than the bank's largest has fewer pieces (4096 tokens of rank 16 by 16384 in a bank of 256 ranks 61 us, with idle
-// workgroups for the other ranks 111).
+// than the bank's largest has fewer pieces (4096 tokens of rank 16 by 16384 in a bank of 256 ranks 73 us, with idle
+// workgroups for the other ranks some 50 more; in a bank of 16 ranks 60).
 struct Work {
   Tile tile;
   int index, part, rank_group;   // index -1: nothing
@@ -254,8 +255,8 @@ __device__ __forceinline__ Work plan_work(const Call& c, int id, int (&found)[8]
 // The same from the ids themselves, by a workgroup of four waves for itself: it counts the groups in `lds`, finds its
 // tile and picks out the tile's tokens in ascending order. The waves hold the ids, a contiguous section each. About 2
 // us in each round of workgroups, where the plan is a launch of 5 and 1 more to read it: 1000 tokens of 8 adapters of
-// rank 32 17.8 us, by a plan made for the call 20.0; 4096 of rank 64 72.9 and 73.9; 4000 of rank 256, in four rank
-// groups, 157 and 156.
+// rank 32, 7168 columns and 1536 rows, 17.9 us, by a plan made for the call 20.4; 16384 columns and 7168 rows, 4096 of
+// rank 64 74.1 and 74.4, 4000 of 4 of rank 256, in four rank groups, 151 and 152.
 constexpr int kOwnIds = 16, kOwnTokens = 4 * 64 * kOwnIds;
 constexpr int kCopies = 8;   // of each count, by lane: neighbours of one group take few turns at one of them
 constexpr int kOwnLds = (kMaxSlots + 1) * kCopies + 4 + kTileTokens;   // numbers
@@ -486,7 +487,7 @@ __global__ __launch_bounds__(256) void adapter_few_down_kernel(Call c) {
 // so that rows are read 512 bytes at a time (in operand order a load takes 64 bytes of each of 16 rows: with rows a
 // power of two apart those meet in the same memory channels); each wave multiplies its K unit of 64 of every stage, its
 // weights straight from the L2 of its XCD, which holds one part's. Two stages: one in flight while one is multiplied.
-// 4096 tokens of 8 adapters of rank 64 by 16384, by a plan: 35 us, of which x (134 MB) alone, read so, takes 25;
+// 4096 tokens of 8 adapters of rank 64 by 16384: 36 to 39 us, by a plan 35, of which x (134 MB) alone, read so, takes 25;
 // without LDS 46; tiles of 128 tokens 34, but 62 against 55 with two rank groups. The rows of a pair lie 512 bytes
 // apart and the pairs 1040, and a second row's 16-byte pieces are swapped in halves of 128 bytes, so that the 16 rows
 // of an operand read lie in different banks.
@@ -619,8 +620,8 @@ __global__ __launch_bounds__(256, 2) void adapter_down_kernel(Call c) {
 // Grouped form of more than 16 ranks: the parts of four ranks of a token added, as h in the first part's place;
 // more than eight of them, which a thread has in flight at once, by four lanes whose sums are added as a tree. A launch
 // of its own, 3 to 5 us: in up every workgroup of a tile would add them anew, which 4096 tokens of rank 64 pay with 18
-// us and 3056 beside 24576 rows with 41, and even rank 32 with 1. Of up to 16 ranks up does it: 1010 tokens of rank 8
-// 12.1 us in all, with this launch 14.0.
+// us and 3056 beside 24576 rows with 41, and even rank 32 with 1. Of up to 16 ranks up does it: 1010 tokens of rank 8,
+// 7168 columns and 576 rows, 12.4 us in all, with this launch 1.9 more.
 template <int kShares>
 __global__ __launch_bounds__(256) void adapter_sum_kernel(Call c) {
   const Bank& b = c.bank;
@@ -720,7 +721,7 @@ __device__ __forceinline__ void up_tiles(const uint4 (&w)[RT][2], const uint4* t
 }
 
 // Few tokens, grid (output blocks / 4, T), 4 waves, a block of 64 outputs each for up to 16 tokens of an adapter (24
-// tokens of 16 adapters of rank 64, 7168 outputs, 15 MB of up: 6.2 us). What does not depend on h is asked for before h
+// tokens of 16 adapters of rank 64, 7168 outputs, 15 MB of up: 5.8 to 7.1 us). What does not depend on h is asked for before h
 // is put together: thread (entry e, share s) adds the parts s, s + shares, ... of four ranks of a token, and the shares
 // are added in order.
 template <bool kF32>
@@ -786,7 +787,7 @@ __global__ __launch_bounds__(256, 2) void adapter_few_up_kernel(Call c) {
 }
 
 // Few tokens in one launch, for a down that every workgroup can read for itself: grid (output blocks / 16, T), 16
-// waves. A chain of two loads' latencies and a launch: one token 4.8 us. The waves take the K units of 64 in turn, two
+// waves. A chain of two loads' latencies and a launch: one token of 24576 outputs 4.5 to 5.5 us. The waves take the K units of 64 in turn, two
 // of them in flight, h is put together through LDS, and each wave finishes a block of 64 outputs whose up and base were
 // asked for at the start.
 template <int RT, bool kF32>
@@ -939,8 +940,7 @@ __device__ __forceinline__ void put_h(const v4f (&h)[RT], int ranks, uint4* two,
 
 // Grouped form: a tile of 64 tokens and four blocks of 64 outputs, one a wave, its weights of all ranks in registers
 // for the tile's columns, 16 tokens at a time. What does not depend on h is asked for before h goes to LDS. Bound by
-// base and y: 4096 tokens of 7168 outputs (117 MB) 30 us, 3056 of 24576 (300 MB) 69; with accesses of 64 bytes the
-// first 37.
+// base and y: 4096 tokens of 7168 outputs (117 MB) 30 to 32 us; with accesses of 64 bytes 7 more.
 template <int RT, bool kF32>
 __device__ __forceinline__ void up_blocks(const Call& c, int index, const Tile& t, int group, int parts, int tid, uint4* h_lds,
                                           uint4* third_lds) {
@@ -991,9 +991,9 @@ __device__ __forceinline__ void up_blocks(const Call& c, int index, const Tile& 
 }
 
 // The same in a bank of more than 128 ranks: the blocks' sums of all 64 tokens stay in registers, and the ranks go
-// through 64 at a time, only the slot's own. 4096 tokens of adapters of rank 256, 64 and 16 in a bank of 256, 24576
-// outputs: 218, 122 and 100 us in all; all 16 rank tiles at once 277, 218 and 186. (In a bank of 128 ranks eight at
-// once are the faster: rank 64 97 us and 107.)
+// through 64 at a time, only the slot's own. 4096 tokens of 8 adapters of rank 256, 64 and 16 in a bank of 256, 1536
+// columns and 24576 outputs, BF16 base: 202, 114 and 105 us in all; all 16 rank tiles at once 340, 248 and 211. (In a bank
+// of 128 ranks eight at once and four in turn: rank 128 127 and 144 us, rank 64 115 and 113.)
 template <bool kF32>
 __device__ __forceinline__ void up_blocks_many(const Call& c, int index, const Tile& t, int group, int tid, uint4* h_lds,
                                                uint4* third_lds) {
@@ -1072,9 +1072,10 @@ int tiles_of(const Bank& b, int tokens) {
 }
 
 // Which calls are of few tokens: up to 64, and with at most 64 ranks to the 128 that a wave can hold. Few and grouped,
-// 16384 columns and 7168 rows: 16 adapters of rank 64, 64 tokens 17.1 and 21.4 us, 128 22.7 and 21.2; 2 of rank 16, 128
-// tokens 11.7 and 13.3; 16 of rank 128, 64 tokens 31.6 and 34.2, 128 39.2 and 31.9. 1536 columns and 24576 rows, 16 of
-// rank 32: 64 tokens 14.2 and 17.2, 128 19.5 and 17.4; 7168 and 576, 4 of rank 64: 120 tokens 13.7 and 16.5.
+// BF16 base, 16384 columns and 7168 rows: 16 adapters of rank 64, 64 tokens 17.2 and 20.4 us, 128 22.6 and 20.5; 2 of rank
+// 16, 128 tokens 10.8 and 13.3; 16 of rank 128, 32 tokens 25.4 and 27.5, 64 31.8 and 29.1, 128 41.3 and 28.6. 16 of rank
+// 128, 64 tokens, 1536 columns and 24576 rows 32.0 and 33.3, 7168 and 1536 16.6 and 19.3. 1536 and 24576, 16 of rank 32:
+// 64 tokens 14.3 and 18.0, 128 19.9 and 18.0; 7168 and 576, 4 of rank 64: 120 tokens 14.0 and 16.8.
 bool is_few(const Bank& b, int tokens) { return tokens <= (b.rank_tiles <= 4 ? kFewTokens : kFewTokens / 2); }
 
 // Parts of K. Few tokens: as many as give each wave a unit of 64, since how many adapters the tokens share is not known
@@ -1163,9 +1164,9 @@ int launch_up(const Call& c, int tiles, bool f32, hipStream_t st) {
 }
 
 // How many tiles the tokens make only the device knows; a bank of many slots could make far more than they do. Up has
-// workgroups for the full ones and 32 more, or as many as are resident together, and takes the rest in turns: 24576
-// rows, rank 16, 200 tokens of 8 of 64 adapters 13.6 us, with 64 more 15.3; 1536 rows, 600 tokens of 64 of 1024
-// adapters 15.1 us with 64 more, 17.0 with 32 and 19.5 with 16.
+// workgroups for the full ones and 32 more, or as many as are resident together, and takes the rest in turns: 1536
+// columns, 24576 rows, rank 16, 200 tokens of 8 of 64 slots in any order 15.4 us, with 64 more 16.7; 7168 columns, 1536
+// rows (of which 170 tiles are resident), 600 tokens of 64 of 1024 slots 16.7, with 32 and 16 more some 2 and 4 above.
 template <int RT>
 int launch_up(const Call& c, bool f32, hipStream_t st) {
   const int tiles = c.tokens / kTileTokens + std::max(32, 1024 / ((c.bank.blocks + 3) / 4));

@@ -28,7 +28,8 @@ constexpr int64_t kMaxWidth = 1 << 24;
 // its pairs here: an expert-parallel rank moves a fraction of what the host can tell. Through the caches and past them,
 // rows of 7168 BF16 values, 8 a token, three sets of buffers in turn: combine of 600 tokens 19.4 and 21.3 us, of 800
 // 26.2 and 25.2, of 4096 118 and 107; its gradient 400: 20.3 and 20.3, 600: 32.9 and 29.2; dispatch 600: 16.8 and 17.8,
-// 800: 25.0 and 22.5. 600 tokens are 77 MB (the gradient 146), 800 are 103.
+// 800: 25.0 and 22.5. 600 tokens are 77 MB (the gradient 146), 800 are 103. Dispatch, which writes each row once, goes by
+// all the pairs that the host knows of: on a rank that holds a part of them it may write past the caches what would fit.
 constexpr int64_t kStreamBytes = 96 << 20;
 
 // ---- plan ----
@@ -547,7 +548,8 @@ __device__ __forceinline__ void combine_units(const CombineArgs& a, int t, int64
 //
 // Bound by HBM reads: 4096 x 8 rows of 7168 (529 MB read, 59 written) take 99 us, 5.9 TB/s. At most five waves a SIMD,
 // so that the rows in flight fit what the memory takes in order: six or eight 107, four 101, three 104; the unweighted
-// sum 98 / 91 / 95 / 99.
+// sum 98 / 91 / 95 / 99. Calls of rows from the caches neither gain nor lose by it: 16 tokens 5.1 us, 333 of 6 FP32 rows
+// of 5120 unweighted 9.7 (9.8 without).
 template <int kType, int V>
 __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(1, 5))) void combine_kernel(CombineArgs a, int chunks) {
   const int t = blockIdx.x / chunks, chunk = blockIdx.x % chunks, lane = threadIdx.x, k = a.k, pairs = a.tokens * k;
@@ -633,7 +635,8 @@ __device__ __forceinline__ float backward_units(const CombineBwdArgs& a, int t, 
 // thread adds its products in order, the lanes are added as a tree and the waves in order. A token's pairs run on one
 // XCD (workgroups go round the eight of them), so its dy comes from HBM once and from that L2 after. 4096 x 8 rows of
 // 7168 BF16 values (998 MB): 178 us, 5.6 TB/s; pairs in plain order 195, rows read through the caches 189, gradients
-// written through them 195; two units a thread of 512 instead of four of 256: 181.
+// written through them 195; two units a thread of 512 instead of four of 256: 181. At most five waves a SIMD: 179 without
+// that, and 1500 tokens of FP32 rows of 5120, an eighth of their six held, 12.8 in place of 13.2, which it costs.
 template <int kType, int V>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 5))) void combine_backward_kernel(CombineBwdArgs a) {
   __shared__ float part[4];
