@@ -723,7 +723,7 @@ __device__ __forceinline__ void up_tiles(const uint4 (&w)[RT][2], const uint4* t
 // Few tokens, grid (output blocks / 4, T), 4 waves, a block of 64 outputs each for up to 16 tokens of an adapter (24
 // tokens of 16 adapters of rank 64, 7168 outputs, 15 MB of up: 5.8 to 7.1 us). What does not depend on h is asked for before h
 // is put together: thread (entry e, share s) adds the parts s, s + shares, ... of four ranks of a token, and the shares
-// are added in order.
+// are added in order. (Two waves a SIMD at least, as adapter_up_kernel and for the same reason.)
 template <bool kF32>
 __global__ __launch_bounds__(256, 2) void adapter_few_up_kernel(Call c) {
   constexpr int RT = 4;   // rank tiles in registers at once
