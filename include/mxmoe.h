@@ -407,6 +407,120 @@ int mx_adapters_apply(mx_adapters* a, const uint16_t* x, int64_t x_stride, const
                       int32_t tokens, const void* base, int32_t base_type, int64_t base_stride, uint16_t* y,
                       int64_t y_stride, void* workspace, uint64_t workspace_bytes, void* stream);
 
+/* ---- heads normalized and rotated, a paged key/value cache in 4 bits, and the attention that reads it: what stands
+ *      between the attention projections (mx_fp8_projection) and the output projection ----
+ *
+ * A head is `width` consecutive values: the first `norm` of them are divided by their root mean square and multiplied by
+ * weight (n = weight * x / sqrt(mean(x^2) + eps), weight NULL = 1), and the `dims` values from `first` on are turned in
+ * pairs by the token's position: (a, b) -> (a c - b s, b c + a s). MX_ROTATE_PAIRS pairs neighbours (2 i, 2 i + 1),
+ * MX_ROTATE_HALVES i with i + dims / 2. norm = 0 and dims = 0 leave a step out. width, norm, first and dims are multiples
+ * of 8 (dims of 16 for halves), width at most 4096.
+ *
+ * The mean square is summed in 64 bits and its root rounded to FP32 once; every product and sum after it is one FP32
+ * operation, so results do not depend on how a call is divided among the device's units. */
+#define MX_ROTATE_PAIRS 0
+#define MX_ROTATE_HALVES 1
+typedef struct mx_rotation {
+  const float* table;        /* [table_positions][dims] (16-byte aligned): dims / 2 cosines, then their sines  */
+  int32_t table_positions;
+  const int32_t* positions;  /* [T]; a token whose position is outside [0, table_positions) is no token: below */
+  int32_t width, norm, first, dims;
+  int32_t style;             /* MX_ROTATE_*                                                                     */
+  int32_t inverse;           /* 1: by the negative angles                                                      */
+  float eps;
+} mx_rotation;
+/* `heads` heads of every token: head h of token t at x + t * x_stride + h * width (strides in values). */
+typedef struct mx_heads {
+  const void* x;
+  int64_t x_stride;
+  int32_t heads;
+  const float* weight;       /* [norm] or NULL                                                                 */
+  void* y;                   /* may be x with one stride and type                                              */
+  int64_t y_stride;
+} mx_heads;
+typedef struct mx_heads_grad {
+  const void* x;             /* the forward call's input; NULL where norm = 0                                  */
+  int64_t x_stride;
+  int32_t heads;
+  const float* weight;
+  const void* dy;
+  int64_t dy_stride;
+  void* dx;                  /* may be x or dy, with its stride                                                */
+  int64_t dx_stride;
+  float* dweight;            /* [norm]: the sum over all tokens and heads; NULL = not asked for                */
+} mx_heads_grad;
+/* One or two sets of heads (queries, and keys with weights of their own) in one launch, x_type and y_type MX_ROWS_BF16 or
+ * _F32. positions may be NULL where dims = 0. Rows that are no token keep the y they had. tokens in [0, 2^20], tokens *
+ * heads below 2^31 in all. The values need no more than their own alignment (16 bytes are faster). */
+int mx_rotate_heads(mx_ctx* ctx, const mx_heads* sets, int32_t n_sets, int32_t tokens, const mx_rotation* rotation,
+                    int32_t x_type, int32_t y_type, void* stream);
+/* Bytes of workspace (16-byte aligned device memory) for gradients of weights of `norm` values. */
+uint64_t mx_rotate_heads_workspace_bytes(int32_t norm);
+/* The gradients: dx for dy, all of one type, and dweight in FP32, summed in a fixed order. Rows that are no token get a
+ * zero dx and add nothing. workspace may be NULL where no dweight is asked for. */
+int mx_rotate_heads_backward(mx_ctx* ctx, const mx_heads_grad* sets, int32_t n_sets, int32_t tokens,
+                             const mx_rotation* rotation, int32_t type, void* workspace, uint64_t workspace_bytes,
+                             void* stream);
+
+/* Keys and values of tokens in pages of `page` tokens (a power of two in [16, 1024]) for each of `heads` key heads: E2M1
+ * codes, the even value in the low nibble, and one E8M0 scale per 32 values of a token: the smallest power of two (at
+ * most 2^125) that keeps the block's largest magnitude, at least 1e-4, within 6; a block that holds an infinity or NaN
+ * has scale 255 and stands for NaN. All arrays are 16-byte aligned device memory of the caller's. Values apart from the
+ * keys: width = value_width, 64, 128 or 256. Latent caches, whose values are the first value_width of the key:
+ * v_codes = v_scales = NULL, (width, value_width) = (512, 512) or (576, 512). */
+typedef struct mx_kv4 {
+  uint8_t* k_codes;          /* [pages][heads][page][width / 2]                                                */
+  uint8_t* k_scales;         /* [pages][heads][page][4 ceil(width / 128)], width / 32 of them in use           */
+  uint8_t* v_codes;          /* [pages][heads][page][value_width / 2] or NULL                                  */
+  uint8_t* v_scales;
+  int32_t pages, page, heads, width, value_width;
+} mx_kv4;
+typedef struct mx_kv4_rows {
+  const void* k;             /* [T][heads][width], tokens k_stride values apart                                */
+  int64_t k_stride;
+  const void* v;             /* [T][heads][value_width]; NULL for latents                                      */
+  int64_t v_stride;
+  int32_t type;              /* MX_ROWS_BF16 or _F32, of both                                                  */
+  int32_t tokens;            /* [0, 2^20]                                                                      */
+  const int64_t* slots;      /* [T] page * cache.page + place in the page                                      */
+  const float* weight;       /* [rotation.norm] or NULL                                                        */
+  uint16_t* k_rounded;       /* [T][heads][width] BF16 values that the stored codes stand for; or NULL         */
+  uint16_t* v_rounded;
+} mx_kv4_rows;
+/* Keys normalized and rotated on the way (rotation NULL: as they are), rounded to BF16, then to codes, into their slots;
+ * values rounded to BF16 and to codes. A token whose slot is outside the cache, or whose position is outside the table, is
+ * not stored and its rounded rows stay as they were. Slots of one call must differ: of two tokens with one slot, either's
+ * codes may stay beside either's scales. */
+int mx_kv4_append(mx_ctx* ctx, const mx_kv4* cache, const mx_kv4_rows* rows, const mx_rotation* rotation, void* stream);
+
+typedef struct mx_kv4_query {
+  const uint16_t* q;         /* [T][heads][cache.width] BF16, tokens q_stride values apart (a multiple of 8)   */
+  int64_t q_stride;
+  int32_t heads;             /* a multiple of cache.heads                                                      */
+  int32_t tokens;            /* T, [0, 2^20]                                                                   */
+  int32_t batch;             /* sequences, [0, 2^16]                                                           */
+  const int32_t* q_first;    /* [batch + 1] first query row of each sequence, ascending from 0 to at most T; NULL: T / batch rows each */
+  const int32_t* table;      /* [batch][columns] page numbers                                                  */
+  int32_t columns;
+  const int32_t* lengths;    /* [batch] tokens in the cache, the queries' own among them                       */
+  float scale;
+  int32_t window;            /* 0, or: a query sees the last `window` positions, its own among them            */
+  const float* sinks;        /* [heads] a logit that takes part in the sum and has no value; or NULL           */
+  uint16_t* out;             /* [T][heads][cache.value_width] BF16, tokens out_stride values apart (of 8)      */
+  int64_t out_stride;
+  float* lse;                /* [T][heads] log of the sum of exp(logit) without the sink; or NULL              */
+} mx_kv4_query;
+/* Bytes of workspace (16-byte aligned device memory) of mx_kv4_attend for this cache's shape, so many query heads, up to
+ * `tokens` tokens and `batch` sequences; 0 with an error text for what attend refuses. */
+uint64_t mx_kv4_workspace_bytes(mx_ctx* ctx, const mx_kv4* cache, int32_t heads, int32_t tokens, int32_t batch);
+/* out = softmax(scale q K^T) V for every query row: the n query rows of a sequence are its last n positions, and a row sees
+ * the positions up to its own (the last `window`). Softmax statistics, sums and products are FP32, of BF16 probabilities
+ * and the exact values of the codes. A row that sees nothing gets zero and lse -infinity. Page numbers outside the cache
+ * and lengths past columns * page hide their tokens; a token one of whose blocks is NaN makes the rows that see it NaN and
+ * no others. Rows behind q_first[batch] stay as they were. Calls that share a workspace must not overlap. */
+int mx_kv4_attend(mx_ctx* ctx, const mx_kv4* cache, const mx_kv4_query* query, void* workspace, uint64_t workspace_bytes,
+                  void* stream);
+
 /* ---- routed MoE layer (replaces ConnectedMoE.forward, src/vesper/connected.py:125-186) ---- */
 
 typedef struct mx_moe_config {

@@ -20,6 +20,7 @@ LIB_PATH = PKG / "libmxmoe.so"
 MX_OK, MX_ERR_INVALID, MX_ERR_MEMORY, MX_ERR_STATE, MX_ERR_HIP = 0, -1, -2, -3, -4
 MX_FMT_MXFP4, MX_FMT_FP8_BLOCK32 = 0, 1
 MX_ROWS = {"bf16": 0, "f32": 1, "u8": 2}
+MX_ROTATE = {"pairs": 0, "halves": 1}
 MX_SCORE = {"sigmoid": 0, "sqrtsoftplus": 1}
 BUFFERS = {"logits": 0, "scores": 1, "selection": 2, "indices": 3, "weights": 4, "xq": 5, "xs": 6, "plan": 7,
            "w1": 8, "w3": 9, "down_input": 10, "down_q": 11, "down_s": 12, "expert_out": 13, "trace": 14,
@@ -59,6 +60,38 @@ class MxRowPlan(C.Structure):
 
 
 _P, _I32, _I64, _U64, _F = C.c_void_p, C.c_int32, C.c_int64, C.c_uint64, C.c_float
+
+
+class MxRotation(C.Structure):
+    _fields_ = [("table", _P), ("table_positions", _I32), ("positions", _P), ("width", _I32), ("norm", _I32),
+                ("first", _I32), ("dims", _I32), ("style", _I32), ("inverse", _I32), ("eps", _F)]
+
+
+class MxHeads(C.Structure):
+    _fields_ = [("x", _P), ("x_stride", _I64), ("heads", _I32), ("weight", _P), ("y", _P), ("y_stride", _I64)]
+
+
+class MxHeadsGrad(C.Structure):
+    _fields_ = [("x", _P), ("x_stride", _I64), ("heads", _I32), ("weight", _P), ("dy", _P), ("dy_stride", _I64),
+                ("dx", _P), ("dx_stride", _I64), ("dweight", _P)]
+
+
+class MxKv4(C.Structure):
+    _fields_ = [("k_codes", _P), ("k_scales", _P), ("v_codes", _P), ("v_scales", _P), ("pages", _I32), ("page", _I32),
+                ("heads", _I32), ("width", _I32), ("value_width", _I32)]
+
+
+class MxKv4Append(C.Structure):
+    _fields_ = [("k", _P), ("k_stride", _I64), ("v", _P), ("v_stride", _I64), ("type", _I32), ("tokens", _I32),
+                ("slots", _P), ("weight", _P), ("k_rounded", _P), ("v_rounded", _P)]
+
+
+class MxKv4Attend(C.Structure):
+    _fields_ = [("q", _P), ("q_stride", _I64), ("heads", _I32), ("tokens", _I32), ("batch", _I32), ("q_first", _P),
+                ("table", _P), ("columns", _I32), ("lengths", _P), ("scale", _F), ("window", _I32), ("sinks", _P),
+                ("out", _P), ("out_stride", _I64), ("lse", _P)]
+
+
 SIGNATURES = {
     "mx_last_error": ([], C.c_char_p),
     "mx_device_count": ([], C.c_int),
@@ -110,6 +143,13 @@ SIGNATURES = {
     "mx_adapters_workspace_bytes": ([_P, _I32], _U64),
     "mx_adapters_apply": ([_P, _P, _I64, _P, C.POINTER(MxRowPlan), _I32, _P, _I32, _I64, _P, _I64, _P, _U64, _P],
                           C.c_int),
+    "mx_rotate_heads": ([_P, C.POINTER(MxHeads), _I32, _I32, C.POINTER(MxRotation), _I32, _I32, _P], C.c_int),
+    "mx_rotate_heads_workspace_bytes": ([_I32], _U64),
+    "mx_rotate_heads_backward": ([_P, C.POINTER(MxHeadsGrad), _I32, _I32, C.POINTER(MxRotation), _I32, _P, _U64, _P],
+                                 C.c_int),
+    "mx_kv4_append": ([_P, C.POINTER(MxKv4), C.POINTER(MxKv4Append), C.POINTER(MxRotation), _P], C.c_int),
+    "mx_kv4_workspace_bytes": ([_P, C.POINTER(MxKv4), _I32, _I32, _I32], _U64),
+    "mx_kv4_attend": ([_P, C.POINTER(MxKv4), C.POINTER(MxKv4Attend), _P, _U64, _P], C.c_int),
     "mx_tiled_expert_bytes": ([_I32, _I32], _U64),
     "mx_tile_expert": ([_P, C.POINTER(MxExpertPtrs), _I32, _I32, _P, _P], C.c_int),
     "mx_untile_expert": ([_P, _P, _I32, _I32, C.POINTER(MxExpertPtrs), _P], C.c_int),

@@ -1,0 +1,271 @@
+// A paged key/value cache in 4 bits: appending to it, and the attention that reads it.
+#include <algorithm>
+#include <type_traits>
+
+#include "mx_heads.h"
+
+namespace {
+
+using namespace mxh;
+
+constexpr int kMaxTokens = 1 << 20, kMaxBatch = 1 << 16;
+
+__host__ __device__ __forceinline__ int scale_pitch(int width) { return (width + 127) / 128 * 4; }
+
+// ---- append ----
+
+struct AppendArgs {
+  mx_kv4 cache;
+  mx_kv4_rows rows;
+  mx_rotation rot;
+  int64_t total;   // key rows, then value rows
+  bool wide;
+};
+
+// A row on L lanes: normalized, rotated and rounded to BF16; then each quad of lanes holds a block of 32 values, whose
+// largest magnitude (as integers, so that an infinity or NaN is the largest) gives the scale.
+template <int L, int NI>
+__global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
+  const int g = threadIdx.x % L;
+  const int64_t r = (int64_t)blockIdx.x * (256 / L) + threadIdx.x / L;
+  if (r >= a.total) return;
+  const int heads = a.cache.heads;
+  const int64_t key_rows = (int64_t)a.rows.tokens * heads;
+  const bool value = r >= key_rows;
+  const uint32_t row = (uint32_t)(value ? r - key_rows : r), t = row / (uint32_t)heads, h = row - t * (uint32_t)heads;
+  const int64_t slot = a.rows.slots[t];
+  const int64_t page = slot / a.cache.page;
+  const float* angles = nullptr;
+  if (slot < 0 || page >= a.cache.pages || !place_of(a.rot, t, angles)) return;
+  const int width = value ? a.cache.value_width : a.cache.width;
+  const int64_t size = a.rows.type == MX_ROWS_F32 ? 4 : 2;
+  const void* x = value ? (const uint8_t*)a.rows.v + (t * a.rows.v_stride + (int64_t)h * width) * size
+                        : (const uint8_t*)a.rows.k + (t * a.rows.k_stride + (int64_t)h * width) * size;
+  mx_rotation rot = a.rot;
+  if (value) rot.norm = rot.dims = 0;
+  float v[NI][8];
+  normalized_row<L, NI>(x, a.rows.type, a.wide, rot, angles, a.rows.weight, 0, width, g, v);
+  const int64_t at = (page * heads + h) * a.cache.page + slot % a.cache.page;
+  uint8_t* codes = (value ? a.cache.v_codes : a.cache.k_codes) + at * (width / 2);
+  uint8_t* scales = (value ? a.cache.v_scales : a.cache.k_scales) + at * scale_pitch(width);
+  uint16_t* rounded = value ? a.rows.v_rounded : a.rows.k_rounded;
+#pragma unroll
+  for (int i = 0; i < NI; ++i) {
+    const int c = 8 * (i * L + g);
+    uint32_t top = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      v[i][j] = mxd::bf16_round_sel(v[i][j]);
+      top = max(top, mx::f2u(v[i][j]) & 0x7FFFFFFFu);
+    }
+    top = max(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, 0xB1, 0xF, 0xF, false));
+    top = max(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, 0x4E, 0xF, 0xF, false));
+    if (c >= width) continue;
+    // amax = m 2^k: 6 2^e >= amax from e = k - 2 on where m <= 1.5, else from k - 1
+    const bool finite = top < 0x7F800000u;
+    const uint32_t amax = max(top, mx::kAmaxFloorBits);
+    uint32_t e8 = (amax >> 23) - ((amax & 0x7FFFFFu) <= 0x400000u ? 2 : 1);
+    e8 = finite ? min(e8, 252u) : 255u;
+    const float scale = mx::u2f(e8 << 23);
+    uint32_t w = 0;
+    if (finite) {
+      w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[i][0], v[i][1], scale, 0);
+      w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[i][2], v[i][3], scale, 1);
+      w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[i][4], v[i][5], scale, 2);
+      w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[i][6], v[i][7], scale, 3);
+    }
+    *(uint32_t*)(codes + c / 2) = w;
+    if ((g & 3) == 0) scales[c / 32] = (uint8_t)e8;
+    if (rounded) {
+      uint4 o;
+      o.x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 0));
+      o.y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 1));
+      o.z = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 2));
+      o.w = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 3));
+      *(uint4*)(rounded + ((int64_t)t * heads + h) * width + c) = o;
+    }
+  }
+}
+
+// ---- attend ----
+
+struct AttendArgs {
+  mx_kv4 cache;
+  mx_kv4_query query;
+};
+
+// One wave a query row and head, one cached token at a time; a lane holds 8 values of a row and step.
+__global__ __launch_bounds__(256) void attend_kernel(AttendArgs a) {
+  const mx_kv4& kv = a.cache;
+  const mx_kv4_query& q = a.query;
+  const int lane = threadIdx.x & 63;
+  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (row >= (int64_t)q.tokens * q.heads) return;
+  const int t = (int)(row / q.heads), head = (int)(row % q.heads), h = head / (q.heads / kv.heads);
+  int b, first, n;
+  if (q.q_first) {
+    int lo = 0, hi = q.batch;   // the last sequence that begins at or before t
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) / 2;
+      if (q.q_first[mid] <= t) lo = mid; else hi = mid;
+    }
+    b = lo, first = q.q_first[b], n = q.q_first[b + 1] - first;
+    if (t >= first + n || t < first) return;
+  } else {
+    n = q.tokens / q.batch, b = t / n, first = b * n;
+  }
+  const int64_t held = min((int64_t)q.lengths[b], (int64_t)q.columns * kv.page);
+  const int64_t end = min(held, (int64_t)q.lengths[b] - n + (t - first) + 1);
+  const int64_t begin = q.window ? max<int64_t>(0, (int64_t)q.lengths[b] - n + (t - first) + 1 - q.window) : 0;
+  const int words = kv.width / 8, value_words = kv.value_width / 8, pitch = scale_pitch(kv.width), value_pitch = scale_pitch(kv.value_width);
+  const uint16_t* qr = q.q + t * q.q_stride + (int64_t)head * kv.width;
+  float qv[2][8] = {}, o[2][8] = {};
+  for (int i = 0; i < 2; ++i)
+    if (lane + 64 * i < words)
+      for (int j = 0; j < 8; ++j) qv[i][j] = mx::bf16_value(qr[8 * (lane + 64 * i) + j]);
+  float m = -INFINITY, l = 0.f;
+  for (int64_t p = begin; p < end; ++p) {
+    const int page = q.table[b * (int64_t)q.columns + p / kv.page];
+    if (page < 0 || page >= kv.pages) continue;
+    const int64_t at = ((int64_t)page * kv.heads + h) * kv.page + p % kv.page;
+    float s = 0.f, kd[2][8];
+    for (int i = 0; i < 2; ++i)
+      if (lane + 64 * i < words) {
+        const uint32_t w = ((const uint32_t*)(kv.k_codes + at * (kv.width / 2)))[lane + 64 * i];
+        const float e = mx::e8m0_value(kv.k_scales[at * pitch + (lane + 64 * i) / 4]);
+        for (int j = 0; j < 8; ++j) kd[i][j] = mx::fp4_value(w >> (4 * j) & 15) * e, s += qv[i][j] * kd[i][j];
+      }
+    if (kv.v_codes)
+      for (int i = 0; i < 2; ++i)
+        if (lane + 64 * i < value_words) {
+          const uint32_t w = ((const uint32_t*)(kv.v_codes + at * (kv.value_width / 2)))[lane + 64 * i];
+          const float e = mx::e8m0_value(kv.v_scales[at * value_pitch + (lane + 64 * i) / 4]);
+          for (int j = 0; j < 8; ++j) kd[i][j] = mx::fp4_value(w >> (4 * j) & 15) * e;
+          if (e != e) s = e;   // the whole token is NaN
+        }
+    s = group_sum<64>(s) * q.scale;
+    if (s == -INFINITY) continue;
+    const float top = s != s ? s : fmaxf(m, s), shrink = m == -INFINITY ? 0.f : expf(m - top), w = expf(s - top);
+    m = top, l = l * shrink + w;
+    for (int i = 0; i < 2; ++i)
+      for (int j = 0; j < 8; ++j) o[i][j] = o[i][j] * shrink + w * kd[i][j];
+  }
+  const float total = q.sinks ? l + (m == -INFINITY ? 0.f : expf(q.sinks[head] - m)) : l;
+  const float inv = l == 0.f ? 0.f : 1.f / total;
+  uint16_t* out = q.out + t * q.out_stride + (int64_t)head * kv.value_width;
+  for (int i = 0; i < 2; ++i)
+    if (lane + 64 * i < value_words)
+      for (int j = 0; j < 8; ++j) out[8 * (lane + 64 * i) + j] = (uint16_t)mx::bf16_bits(o[i][j] * inv);
+  if (q.lse && lane == 0) q.lse[(int64_t)t * q.heads + head] = l == 0.f ? -INFINITY : m + logf(l);
+}
+
+int check_cache(const char* who, const mx_kv4* c) {
+  MX_REQUIRE(c, "%s: null cache", who);
+  MX_REQUIRE(c->page >= 16 && c->page <= 1024 && (c->page & (c->page - 1)) == 0, "%s: page of %d tokens not a power of two in [16, 1024]",
+             who, c->page);
+  MX_REQUIRE(c->heads >= 1 && c->heads <= 1024, "%s: %d key heads outside [1, 1024]", who, c->heads);
+  MX_REQUIRE(c->pages >= 1 && (int64_t)c->pages * c->heads * c->page <= (1ll << 40), "%s: %d pages", who, c->pages);
+  const bool apart = c->v_codes || c->v_scales;
+  if (apart)
+    MX_REQUIRE((c->width == 64 || c->width == 128 || c->width == 256) && c->value_width == c->width,
+               "%s: keys of %d and values of %d; 64, 128 or 256 of both are supported", who, c->width, c->value_width);
+  else
+    MX_REQUIRE((c->width == 512 || c->width == 576) && c->value_width == 512,
+               "%s: latents of %d with values of %d; 512 or 576 with 512 are supported", who, c->width, c->value_width);
+  MX_REQUIRE(c->k_codes && c->k_scales && (!apart || (c->v_codes && c->v_scales)), "%s: null cache array", who);
+  MX_REQUIRE(aligned(c->k_codes, 16) && aligned(c->k_scales, 16) && aligned(c->v_codes, 16) && aligned(c->v_scales, 16),
+             "%s: cache arrays must be 16-byte aligned", who);
+  return MX_OK;
+}
+
+int check_attend(const char* who, const mx_kv4* c, int32_t heads, int32_t tokens, int32_t batch) {
+  if (int s = check_cache(who, c)) return s;
+  MX_REQUIRE(heads >= 1 && heads <= (1 << 16) && heads % c->heads == 0, "%s: %d query heads for %d key heads", who, heads, c->heads);
+  MX_REQUIRE(tokens >= 0 && tokens <= kMaxTokens, "%s: token count %d outside [0, %d]", who, tokens, kMaxTokens);
+  MX_REQUIRE(batch >= 0 && batch <= kMaxBatch, "%s: %d sequences outside [0, %d]", who, batch, kMaxBatch);
+  MX_REQUIRE((int64_t)tokens * heads < (1ll << 31), "%s: 2^31 query rows or more in all", who);
+  return MX_OK;
+}
+
+}  // namespace
+
+using mxi::as_stream;
+using mxi::use;
+
+extern "C" {
+
+int mx_kv4_append(mx_ctx* ctx, const mx_kv4* cache, const mx_kv4_rows* rows, const mx_rotation* rotation, void* stream) {
+  const char* who = "mx_kv4_append";
+  if (int s = check_cache(who, cache)) return s;
+  MX_REQUIRE(rows, "%s: null rows", who);
+  MX_REQUIRE(rows->tokens >= 0 && rows->tokens <= kMaxTokens, "%s: token count %d outside [0, %d]", who, rows->tokens, kMaxTokens);
+  MX_REQUIRE((int64_t)rows->tokens * cache->heads < (1ll << 30), "%s: 2^30 rows or more in all", who);
+  MX_REQUIRE(rows->type == MX_ROWS_BF16 || rows->type == MX_ROWS_F32, "%s: row type %d", who, rows->type);
+  const bool apart = cache->v_codes != nullptr;
+  MX_REQUIRE(rows->k && rows->slots && (rows->v != nullptr) == apart, "%s: keys, slots and, where the cache holds them, values", who);
+  MX_REQUIRE(apart || !rows->v_rounded, "%s: latents have no values of their own", who);
+  const int64_t size = rows->type == MX_ROWS_F32 ? 4 : 2;
+  MX_REQUIRE(rows->k_stride >= (int64_t)cache->heads * cache->width && rows->k_stride < (1ll << 40) &&
+                 (!apart || (rows->v_stride >= (int64_t)cache->heads * cache->value_width && rows->v_stride < (1ll << 40))),
+             "%s: token strides below the tokens' values", who);
+  MX_REQUIRE(aligned(rows->k, size) && aligned(rows->v, size) && aligned(rows->weight, 4) && aligned(rows->slots, 8),
+             "%s: pointers must be aligned to their elements", who);
+  MX_REQUIRE(aligned(rows->k_rounded, 16) && aligned(rows->v_rounded, 16), "%s: rounded rows must be 16-byte aligned", who);
+  AppendArgs a{};
+  a.cache = *cache, a.rows = *rows;
+  if (rotation) {
+    if (int s = check_rotation(who, rotation)) return s;
+    MX_REQUIRE(rotation->width == cache->width, "%s: a rotation of %d values for keys of %d", who, rotation->width, cache->width);
+    a.rot = *rotation;
+  }
+  a.total = (int64_t)rows->tokens * cache->heads * (apart ? 2 : 1);
+  a.wide = aligned(rows->k, 16) && aligned(rows->v, 16) && rows->k_stride * size % 16 == 0 && rows->v_stride * size % 16 == 0;
+  if (int s = use(ctx)) return s;
+  if (!rows->tokens) return MX_OK;
+  return by_lanes(cache->width, [&](auto l, auto n) {
+    constexpr int L = decltype(l)::value, NI = decltype(n)::value;
+    hipLaunchKernelGGL((append_kernel<L, NI>), dim3((unsigned)((a.total + 256 / L - 1) / (256 / L))), dim3(256), 0, as_stream(stream), a);
+    MX_LAUNCH_CHECK("append_kernel");
+    return MX_OK;
+  });
+}
+
+uint64_t mx_kv4_workspace_bytes(mx_ctx* ctx, const mx_kv4* cache, int32_t heads, int32_t tokens, int32_t batch) {
+  if (check_attend("mx_kv4_workspace_bytes", cache, heads, tokens, batch)) return 0;
+  return 16;
+}
+
+int mx_kv4_attend(mx_ctx* ctx, const mx_kv4* cache, const mx_kv4_query* query, void* workspace, uint64_t workspace_bytes,
+                  void* stream) {
+  const char* who = "mx_kv4_attend";
+  MX_REQUIRE(query, "%s: null query", who);
+  const mx_kv4_query& q = *query;
+  if (int s = check_attend(who, cache, q.heads, q.tokens, q.batch)) return s;
+  MX_REQUIRE(q.columns >= 1 && (int64_t)q.columns * cache->page < (1ll << 31), "%s: %d columns of pages of %d tokens", who, q.columns,
+             cache->page);
+  MX_REQUIRE(q.q_first || (q.batch ? q.tokens % q.batch == 0 : q.tokens == 0), "%s: %d rows do not divide among %d sequences", who,
+             q.tokens, q.batch);
+  MX_REQUIRE(q.window >= 0, "%s: window %d", who, q.window);
+  MX_REQUIRE(q.scale > 0.f && q.scale <= 3.4e38f, "%s: scale must be finite and positive", who);
+  MX_REQUIRE(q.q_stride >= (int64_t)q.heads * cache->width && q.q_stride % 8 == 0 && q.q_stride < (1ll << 40) &&
+                 q.out_stride >= (int64_t)q.heads * cache->value_width && q.out_stride % 8 == 0 && q.out_stride < (1ll << 40),
+             "%s: token strides must be multiples of 8 that hold the heads", who);
+  if (q.tokens && q.batch) {
+    MX_REQUIRE(q.q && q.out && q.table && q.lengths, "%s: null pointer", who);
+    MX_REQUIRE(aligned(q.q, 16) && aligned(q.out, 16) && aligned(q.q_first, 4) && aligned(q.table, 4) && aligned(q.lengths, 4) &&
+                   aligned(q.sinks, 4) && aligned(q.lse, 4),
+               "%s: q and out must be 16-byte aligned, the others to their elements", who);
+  }
+  const uint64_t need = mx_kv4_workspace_bytes(ctx, cache, q.heads, q.tokens, q.batch);
+  MX_REQUIRE(workspace && aligned(workspace, 16) && workspace_bytes >= need, "%s: %llu bytes of workspace, 16-byte aligned, needed", who,
+             (unsigned long long)need);
+  if (int s = use(ctx)) return s;
+  if (!q.tokens || !q.batch) return MX_OK;
+  const AttendArgs a{*cache, q};
+  const int64_t rows = (int64_t)q.tokens * q.heads;
+  hipLaunchKernelGGL(attend_kernel, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, as_stream(stream), a);
+  MX_LAUNCH_CHECK("attend_kernel");
+  return MX_OK;
+}
+
+}  // extern "C"
