@@ -497,11 +497,11 @@ typedef struct mx_kv4_query {
   const uint16_t* q;         /* [T][heads][cache.width] BF16, tokens q_stride values apart (a multiple of 8)   */
   int64_t q_stride;
   int32_t heads;             /* a multiple of cache.heads                                                      */
-  int32_t tokens;            /* T, [0, 2^20]                                                                   */
+  int32_t tokens;            /* T, [0, 2^20]; tokens * heads at most 2^30                                      */
   int32_t batch;             /* sequences, [0, 2^16]                                                           */
   const int32_t* q_first;    /* [batch + 1] first query row of each sequence, ascending from 0 to at most T; NULL: T / batch rows each */
   const int32_t* table;      /* [batch][columns] page numbers                                                  */
-  int32_t columns;
+  int32_t columns;           /* columns * page at most 2^30                                                    */
   const int32_t* lengths;    /* [batch] tokens in the cache, the queries' own among them                       */
   float scale;
   int32_t window;            /* 0, or: a query sees the last `window` positions, its own among them            */

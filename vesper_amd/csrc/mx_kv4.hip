@@ -1,16 +1,13 @@
-// A paged key/value cache in 4 bits: appending to it, and the attention that reads it.
+// Appending to a paged key/value cache in 4 bits.
 #include <algorithm>
 #include <type_traits>
 
-#include "mx_heads.h"
+#include "mx_kv4.h"
 
 namespace {
 
 using namespace mxh;
-
-constexpr int kMaxTokens = 1 << 20, kMaxBatch = 1 << 16;
-
-__host__ __device__ __forceinline__ int scale_pitch(int width) { return (width + 127) / 128 * 4; }
+using namespace mxk;
 
 // ---- append ----
 
@@ -87,79 +84,9 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
   }
 }
 
-// ---- attend ----
+}  // namespace
 
-struct AttendArgs {
-  mx_kv4 cache;
-  mx_kv4_query query;
-};
-
-// One wave a query row and head, one cached token at a time; a lane holds 8 values of a row and step.
-__global__ __launch_bounds__(256) void attend_kernel(AttendArgs a) {
-  const mx_kv4& kv = a.cache;
-  const mx_kv4_query& q = a.query;
-  const int lane = threadIdx.x & 63;
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (row >= (int64_t)q.tokens * q.heads) return;
-  const int t = (int)(row / q.heads), head = (int)(row % q.heads), h = head / (q.heads / kv.heads);
-  int b, first, n;
-  if (q.q_first) {
-    int lo = 0, hi = q.batch;   // the last sequence that begins at or before t
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) / 2;
-      if (q.q_first[mid] <= t) lo = mid; else hi = mid;
-    }
-    b = lo, first = q.q_first[b], n = q.q_first[b + 1] - first;
-    if (t >= first + n || t < first) return;
-  } else {
-    n = q.tokens / q.batch, b = t / n, first = b * n;
-  }
-  const int64_t held = min((int64_t)q.lengths[b], (int64_t)q.columns * kv.page);
-  const int64_t end = min(held, (int64_t)q.lengths[b] - n + (t - first) + 1);
-  const int64_t begin = q.window ? max<int64_t>(0, (int64_t)q.lengths[b] - n + (t - first) + 1 - q.window) : 0;
-  const int words = kv.width / 8, value_words = kv.value_width / 8, pitch = scale_pitch(kv.width), value_pitch = scale_pitch(kv.value_width);
-  const uint16_t* qr = q.q + t * q.q_stride + (int64_t)head * kv.width;
-  float qv[2][8] = {}, o[2][8] = {};
-  for (int i = 0; i < 2; ++i)
-    if (lane + 64 * i < words)
-      for (int j = 0; j < 8; ++j) qv[i][j] = mx::bf16_value(qr[8 * (lane + 64 * i) + j]);
-  float m = -INFINITY, l = 0.f;
-  for (int64_t p = begin; p < end; ++p) {
-    const int page = q.table[b * (int64_t)q.columns + p / kv.page];
-    if (page < 0 || page >= kv.pages) continue;
-    const int64_t at = ((int64_t)page * kv.heads + h) * kv.page + p % kv.page;
-    float s = 0.f, kd[2][8];
-    for (int i = 0; i < 2; ++i)
-      if (lane + 64 * i < words) {
-        const uint32_t w = ((const uint32_t*)(kv.k_codes + at * (kv.width / 2)))[lane + 64 * i];
-        const float e = mx::e8m0_value(kv.k_scales[at * pitch + (lane + 64 * i) / 4]);
-        for (int j = 0; j < 8; ++j) kd[i][j] = mx::fp4_value(w >> (4 * j) & 15) * e, s += qv[i][j] * kd[i][j];
-      }
-    if (kv.v_codes)
-      for (int i = 0; i < 2; ++i)
-        if (lane + 64 * i < value_words) {
-          const uint32_t w = ((const uint32_t*)(kv.v_codes + at * (kv.value_width / 2)))[lane + 64 * i];
-          const float e = mx::e8m0_value(kv.v_scales[at * value_pitch + (lane + 64 * i) / 4]);
-          for (int j = 0; j < 8; ++j) kd[i][j] = mx::fp4_value(w >> (4 * j) & 15) * e;
-          if (e != e) s = e;   // the whole token is NaN
-        }
-    s = group_sum<64>(s) * q.scale;
-    if (s == -INFINITY) continue;
-    const float top = s != s ? s : fmaxf(m, s), shrink = m == -INFINITY ? 0.f : expf(m - top), w = expf(s - top);
-    m = top, l = l * shrink + w;
-    for (int i = 0; i < 2; ++i)
-      for (int j = 0; j < 8; ++j) o[i][j] = o[i][j] * shrink + w * kd[i][j];
-  }
-  const float total = q.sinks ? l + (m == -INFINITY ? 0.f : expf(q.sinks[head] - m)) : l;
-  const float inv = l == 0.f ? 0.f : 1.f / total;
-  uint16_t* out = q.out + t * q.out_stride + (int64_t)head * kv.value_width;
-  for (int i = 0; i < 2; ++i)
-    if (lane + 64 * i < value_words)
-      for (int j = 0; j < 8; ++j) out[8 * (lane + 64 * i) + j] = (uint16_t)mx::bf16_bits(o[i][j] * inv);
-  if (q.lse && lane == 0) q.lse[(int64_t)t * q.heads + head] = l == 0.f ? -INFINITY : m + logf(l);
-}
-
-int check_cache(const char* who, const mx_kv4* c) {
+int mxk::check_cache(const char* who, const mx_kv4* c) {
   MX_REQUIRE(c, "%s: null cache", who);
   MX_REQUIRE(c->page >= 16 && c->page <= 1024 && (c->page & (c->page - 1)) == 0, "%s: page of %d tokens not a power of two in [16, 1024]",
              who, c->page);
@@ -177,17 +104,6 @@ int check_cache(const char* who, const mx_kv4* c) {
              "%s: cache arrays must be 16-byte aligned", who);
   return MX_OK;
 }
-
-int check_attend(const char* who, const mx_kv4* c, int32_t heads, int32_t tokens, int32_t batch) {
-  if (int s = check_cache(who, c)) return s;
-  MX_REQUIRE(heads >= 1 && heads <= (1 << 16) && heads % c->heads == 0, "%s: %d query heads for %d key heads", who, heads, c->heads);
-  MX_REQUIRE(tokens >= 0 && tokens <= kMaxTokens, "%s: token count %d outside [0, %d]", who, tokens, kMaxTokens);
-  MX_REQUIRE(batch >= 0 && batch <= kMaxBatch, "%s: %d sequences outside [0, %d]", who, batch, kMaxBatch);
-  MX_REQUIRE((int64_t)tokens * heads < (1ll << 31), "%s: 2^31 query rows or more in all", who);
-  return MX_OK;
-}
-
-}  // namespace
 
 using mxi::as_stream;
 using mxi::use;
@@ -228,44 +144,6 @@ int mx_kv4_append(mx_ctx* ctx, const mx_kv4* cache, const mx_kv4_rows* rows, con
     MX_LAUNCH_CHECK("append_kernel");
     return MX_OK;
   });
-}
-
-uint64_t mx_kv4_workspace_bytes(mx_ctx* ctx, const mx_kv4* cache, int32_t heads, int32_t tokens, int32_t batch) {
-  if (check_attend("mx_kv4_workspace_bytes", cache, heads, tokens, batch)) return 0;
-  return 16;
-}
-
-int mx_kv4_attend(mx_ctx* ctx, const mx_kv4* cache, const mx_kv4_query* query, void* workspace, uint64_t workspace_bytes,
-                  void* stream) {
-  const char* who = "mx_kv4_attend";
-  MX_REQUIRE(query, "%s: null query", who);
-  const mx_kv4_query& q = *query;
-  if (int s = check_attend(who, cache, q.heads, q.tokens, q.batch)) return s;
-  MX_REQUIRE(q.columns >= 1 && (int64_t)q.columns * cache->page < (1ll << 31), "%s: %d columns of pages of %d tokens", who, q.columns,
-             cache->page);
-  MX_REQUIRE(q.q_first || (q.batch ? q.tokens % q.batch == 0 : q.tokens == 0), "%s: %d rows do not divide among %d sequences", who,
-             q.tokens, q.batch);
-  MX_REQUIRE(q.window >= 0, "%s: window %d", who, q.window);
-  MX_REQUIRE(q.scale > 0.f && q.scale <= 3.4e38f, "%s: scale must be finite and positive", who);
-  MX_REQUIRE(q.q_stride >= (int64_t)q.heads * cache->width && q.q_stride % 8 == 0 && q.q_stride < (1ll << 40) &&
-                 q.out_stride >= (int64_t)q.heads * cache->value_width && q.out_stride % 8 == 0 && q.out_stride < (1ll << 40),
-             "%s: token strides must be multiples of 8 that hold the heads", who);
-  if (q.tokens && q.batch) {
-    MX_REQUIRE(q.q && q.out && q.table && q.lengths, "%s: null pointer", who);
-    MX_REQUIRE(aligned(q.q, 16) && aligned(q.out, 16) && aligned(q.q_first, 4) && aligned(q.table, 4) && aligned(q.lengths, 4) &&
-                   aligned(q.sinks, 4) && aligned(q.lse, 4),
-               "%s: q and out must be 16-byte aligned, the others to their elements", who);
-  }
-  const uint64_t need = mx_kv4_workspace_bytes(ctx, cache, q.heads, q.tokens, q.batch);
-  MX_REQUIRE(workspace && aligned(workspace, 16) && workspace_bytes >= need, "%s: %llu bytes of workspace, 16-byte aligned, needed", who,
-             (unsigned long long)need);
-  if (int s = use(ctx)) return s;
-  if (!q.tokens || !q.batch) return MX_OK;
-  const AttendArgs a{*cache, q};
-  const int64_t rows = (int64_t)q.tokens * q.heads;
-  hipLaunchKernelGGL(attend_kernel, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, as_stream(stream), a);
-  MX_LAUNCH_CHECK("attend_kernel");
-  return MX_OK;
 }
 
 }  // extern "C"
