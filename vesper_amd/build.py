@@ -33,6 +33,9 @@ HIP_FLAGS = [
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
     "-Wall", "-Wno-unused-function", "-Wno-unused-variable",
 ]
+# Attention: products sum up in ordinary registers, so that rescaling a sum moves nothing; the queries take the
+# accumulation registers.
+FILE_FLAGS = {"mx_attend": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
 
 
 def hipcc() -> str:
@@ -58,7 +61,7 @@ def build(jobs: int | None = None, verbose: bool = False) -> Path:
     objects = [BUILD / (src.stem + ".o") for src in sources]
     jobs = jobs or min(len(sources), os.cpu_count() or 4, 8)
     with cf.ThreadPoolExecutor(max_workers=jobs) as pool:
-        futures = [pool.submit(_run, [compiler, *HIP_FLAGS, "-c", str(src), "-o", str(obj)])
+        futures = [pool.submit(_run, [compiler, *HIP_FLAGS, *FILE_FLAGS.get(src.stem, []), "-c", str(src), "-o", str(obj)])
                    for src, obj in zip(sources, objects)]
         for f in futures:
             out = f.result()

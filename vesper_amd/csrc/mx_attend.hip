@@ -171,27 +171,38 @@ __global__ __launch_bounds__(1024) void plan_kernel(AttendArgs a, int rows, int 
   make_plan<1024>(a, {(int32_t*)(a.space + a.at.base), (int64_t*)(a.space + a.at.prefix)}, sums, rows, step);
 }
 
-// Two E4M3 terms of 16 query values under one scale: y = v 2^-e in [-256, 256], its nearest code, and of what is left the
-// nearest code under 2^-4 of the scale.
-__device__ __forceinline__ void split16(const float (&v)[16], uint32_t exponent, uint32_t* high, uint32_t* low) {
-  const float inv = mx::u2f((254u - exponent) << 23);
+// Two E4M3 terms of 16 query values (BF16 pairs w) under the scale 2^(exponent - 127), which takes them into [-256, 256]:
+// the nearest code, and of what is left the nearest code under 2^-4 of the scale.
+__device__ __forceinline__ void split16(const uint32_t (&w)[8], uint32_t exponent, uint32_t* high, uint32_t* low) {
+  typedef short v2s __attribute__((ext_vector_type(2)));
+  typedef __bf16 v2b __attribute__((ext_vector_type(2)));
+  const float scale = mx::u2f(exponent << 23), fine = mx::u2f((exponent - 4u) << 23);
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    int h = 0, l = 0;
-    h = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * j] * inv, v[4 * j + 1] * inv, h, false);
-    h = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * j + 2] * inv, v[4 * j + 3] * inv, h, true);
-    const auto a = __builtin_amdgcn_cvt_pk_f32_fp8(h, false), b = __builtin_amdgcn_cvt_pk_f32_fp8(h, true);
-    l = __builtin_amdgcn_cvt_pk_fp8_f32((v[4 * j] * inv - a[0]) * 16.f, (v[4 * j + 1] * inv - a[1]) * 16.f, l, false);
-    l = __builtin_amdgcn_cvt_pk_fp8_f32((v[4 * j + 2] * inv - b[0]) * 16.f, (v[4 * j + 3] * inv - b[1]) * 16.f, l, true);
-    high[j] = h, low[j] = l;
+    v2s h = {0, 0}, l = {0, 0};
+    h = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(h, __builtin_bit_cast(v2b, w[2 * j]), scale, false);
+    h = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(h, __builtin_bit_cast(v2b, w[2 * j + 1]), scale, true);
+    high[j] = __builtin_bit_cast(uint32_t, h);
+    const auto a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(high[j], scale, false), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(high[j], scale, true);
+    l = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(l, mx::u2f(w[2 * j] << 16) - a[0], mx::u2f(w[2 * j] & 0xFFFF0000u) - a[1], fine, false);
+    l = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(l, mx::u2f(w[2 * j + 1] << 16) - b[0], mx::u2f(w[2 * j + 1] & 0xFFFF0000u) - b[1], fine, true);
+    low[j] = __builtin_bit_cast(uint32_t, l);
   }
 }
 
-// The scale exponent of a block of 32 query values whose magnitudes' largest (as bits) is top: [128, 256) 2^e. 255 (NaN)
-// where a value is not finite; blocks below 2^-107 lose their last bits.
+// The scale exponent of a block of 32 query values whose magnitudes' largest (as BF16 bits) is top: [128, 256) 2^e. 255
+// (NaN) where a value is not finite; blocks below 2^-107 lose their last bits.
 __device__ __forceinline__ uint32_t query_exponent(uint32_t top) {
-  return top >= 0x7F800000u ? 255u : max(top >> 23, 20u) - 7u;
+  return top >= 0x7F80u ? 255u : max(top >> 7, 20u) - 7u;
 }
+__device__ __forceinline__ uint32_t pair_max(uint32_t a, uint32_t b) {   // of two 16-bit numbers each
+  typedef unsigned short v2u __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(v2u, a), __builtin_bit_cast(v2u, b)));
+}
+
+// Into the accumulation registers: where a wave has all 512 registers of a lane, the queries, which only products read,
+// stay in the half that other instructions cannot use.
+__device__ __forceinline__ void keep(v8i& v) { asm volatile("" : "+a"(v)); }
 
 template <int kA, int kB>
 __device__ __forceinline__ v16f scores(uint4 k, const v8i& q, v16f c, uint32_t ks, uint32_t qs) {
@@ -214,6 +225,9 @@ __device__ __forceinline__ float halves_sum(float v) {
   return __int_as_float(p[0]) + __int_as_float(p[1]);
 }
 
+// Waves that a SIMD holds (so workgroups a CU), by what their registers allow.
+__host__ __device__ constexpr int waves(int value_width) { return value_width <= 64 ? 3 : value_width <= 128 ? 2 : 1; }
+
 // WK, WV: widths of a key and of a value; kApart: values have codes of their own; RG: the workgroup's row groups of 32. A
 // step is 4 / RG tiles of 32 tokens, each of which RG waves (one a row group) score and, in parts, convert.
 //
@@ -234,10 +248,15 @@ struct Attend {
   static constexpr int CB = WV < 64 ? WV : 64;             // columns that go out at a time
   static constexpr int kOut = 32 * (CB + 4) * 4;           // bytes of a wave's
   static constexpr int kLds = TG * kBuffers * kTile > 4 * kOut ? TG * kBuffers * kTile : 4 * kOut;
-  static constexpr int kWaves = WV <= 64 ? 3 : WV <= 128 ? 2 : 1;   // a SIMD
+  static constexpr int kWaves = waves(WV), kGroups = kCus * kWaves;
 };
 
-// A row's result: out, and lse with its first column.
+// Where a row of a unit goes (in values; -1: nowhere), and its factor.
+struct Place {
+  int64_t at;
+  float by;
+};
+
 struct RowOut {
   float inv, lse;
 };
@@ -259,6 +278,7 @@ __global__ __launch_bounds__(256, (Attend<WK, WV, kApart, RG>::kWaves)) void att
   __shared__ __attribute__((aligned(16))) uint8_t exchange[A::kExchange];
   __shared__ float tops[2][4][32];
   __shared__ float stats[4][32][2];
+  __shared__ Place places[A::kRows];
   __shared__ int64_t plan_prefix[kInlineTiles + 1];
   __shared__ int32_t plan_base[kInlineTiles + 1];
   __shared__ int64_t sums[4];
@@ -272,10 +292,10 @@ __global__ __launch_bounds__(256, (Attend<WK, WV, kApart, RG>::kWaves)) void att
     make_plan<256>(a, plan, sums, A::kRows, A::kStep);
   }
   const int64_t all = plan.prefix[plan.base[a.q.batch]] * a.cache.heads;
-  const int groups = gridDim.x;
+  constexpr int groups = A::kGroups;
   const int64_t per = max<int64_t>((all + groups - 1) / groups, 1);
   // workgroups go round the XCDs: neighbours in the work, which share keys, to one L2
-  const int g = groups % kXcds ? (int)blockIdx.x : (int)(blockIdx.x % kXcds) * (groups / kXcds) + (int)blockIdx.x / kXcds;
+  const int g = (int)(blockIdx.x % kXcds) * (groups / kXcds) + (int)blockIdx.x / kXcds;
   int64_t x = min(g * per, all);
   const int64_t end = min(x + per, all);
   Shared* shared = (Shared*)(a.space + a.at.units) + g;
@@ -304,7 +324,7 @@ __global__ __launch_bounds__(256, (Attend<WK, WV, kApart, RG>::kWaves)) void att
     const int t0 = plan.base[b], t1 = plan.base[b + 1];
     const int64_t p0 = plan.prefix[t0], span = plan.prefix[t1] - p0;
     const int64_t in = x - p0 * a.cache.heads;
-    const int h = (int)(in / span);
+    const int h = (in | span) >> 32 ? (int)(in / span) : (int)((uint32_t)in / (uint32_t)span);
     const int64_t rest = in - h * span;
     int tile;
     {
@@ -332,45 +352,13 @@ __global__ __launch_bounds__(256, (Attend<WK, WV, kApart, RG>::kWaves)) void att
     seen(a, s, min(row0, rows - 1) / a.group, unused, all_hi);
     seen(a, s, min(row0 + 31, rows - 1) / a.group, all_lo, unused);
 
-    v8i qh[KS], ql[KS];
-    uint32_t qs[(KS + 1) / 2] = {};
-    {
-      const uint16_t* q = a.q.q + (s.first + i) * a.q.q_stride + (int64_t)(h * a.group + row % a.group) * WK;
-#pragma unroll
-      for (int k = 0; k < KS; ++k) {
-        float v[2][16];
-        uint32_t top[2] = {0, 0};
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const uint4 w = mxd::ldg128((const uint8_t*)(q + 64 * k + 32 * e + 16 * half + 8 * j));
-            const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-            for (int n = 0; n < 4; ++n) {
-              v[e][8 * j + 2 * n] = mx::u2f(u[n] << 16), v[e][8 * j + 2 * n + 1] = mx::u2f(u[n] & 0xFFFF0000u);
-              top[e] = max(top[e], max((u[n] << 16) & 0x7FFFFFFFu, u[n] & 0x7FFF0000u));
-            }
-          }
-          top[e] = max(top[e], (uint32_t)__shfl_xor((int)top[e], 32, 64));
-        }
-        const uint32_t e0 = query_exponent(top[0]), e1 = query_exponent(top[1]);
-        uint32_t hi16[8], lo16[8];
-        split16(v[0], min(e0, 247u), hi16, lo16);
-        split16(v[1], min(e1, 247u), hi16 + 4, lo16 + 4);
-#pragma unroll
-        for (int n = 0; n < 8; ++n) qh[k][n] = (int)hi16[n], ql[k][n] = (int)lo16[n];
-        const uint32_t own = half ? e1 : e0;
-        qs[k / 2] |= (own | (own == 255u ? 255u : own - 4u) << 8) << (16 * (k & 1));
-      }
-    }
-
     float m = kLowest, l = 0.f;   // the maximum is a whole number: every rescaling is exact
     v16f o[DB];
 #pragma unroll
-    for (int d = 0; d < DB; ++d)
+    for (int d = 0; d < DB; ++d) {
 #pragma unroll
       for (int n = 0; n < 16; ++n) o[d][n] = 0.f;
+    }
 
     // -- loads: the lane's token of a step, its page a step ahead --
     const int32_t* table = a.q.table + (int64_t)b * a.q.columns;
@@ -401,6 +389,65 @@ __global__ __launch_bounds__(256, (Attend<WK, WV, kApart, RG>::kWaves)) void att
     };
     load(it0, page_of(it0));
     int page_next = page_of(it0 + 1);
+
+    v8i qh[KS], ql[KS];
+    uint32_t qs[(KS + 1) / 2] = {};
+    {
+      // 64 values of a step, 2 x 16 a lane; the waves of a row group take turns and exchange what they made
+      const uint16_t* q = a.q.q + (s.first + i) * a.q.q_stride + (int64_t)(h * a.group + row % a.group) * WK;
+      uint4* made = (uint4*)lds + rg * (KS * 256) + lane;
+      uint32_t* made_scales = (uint32_t*)(lds + RG * KS * 4096) + rg * (KS * 64) + lane;
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        if (TG > 1 && k % TG != tg) continue;
+        uint32_t w[2][8], top[2], high[8], low[8];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const uint4 v = mxd::ldg128((const uint8_t*)(q + 64 * k + 32 * e + 16 * half + 8 * j));
+            w[e][4 * j] = v.x, w[e][4 * j + 1] = v.y, w[e][4 * j + 2] = v.z, w[e][4 * j + 3] = v.w;
+          }
+          top[e] = w[e][0] & 0x7FFF7FFFu;
+#pragma unroll
+          for (int j = 1; j < 8; ++j) top[e] = pair_max(top[e], w[e][j] & 0x7FFF7FFFu);
+          top[e] = max(top[e] & 0xFFFFu, top[e] >> 16);
+          top[e] = max(top[e], (uint32_t)__shfl_xor((int)top[e], 32, 64));
+        }
+        const uint32_t e0 = query_exponent(top[0]), e1 = query_exponent(top[1]), own = half ? e1 : e0;
+        split16(w[0], min(e0, 247u), high, low);
+        split16(w[1], min(e1, 247u), high + 4, low + 4);
+        const uint32_t scales = own | (own == 255u ? 255u : own - 4u) << 8;
+        if constexpr (TG > 1) {
+          made[k * 256] = make_uint4(high[0], high[1], high[2], high[3]), made[k * 256 + 64] = make_uint4(high[4], high[5], high[6], high[7]);
+          made[k * 256 + 128] = make_uint4(low[0], low[1], low[2], low[3]), made[k * 256 + 192] = make_uint4(low[4], low[5], low[6], low[7]);
+          made_scales[k * 64] = scales;
+        } else {
+#pragma unroll
+          for (int n = 0; n < 8; ++n) qh[k][n] = (int)high[n], ql[k][n] = (int)low[n];
+          qs[k / 2] |= scales << (16 * (k & 1));
+        }
+      }
+      if constexpr (TG > 1) {
+        mxd::lds_barrier();
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const uint4 u = made[k * 256 + 64 * j], v = made[k * 256 + 128 + 64 * j];
+            qh[k][4 * j] = (int)u.x, qh[k][4 * j + 1] = (int)u.y, qh[k][4 * j + 2] = (int)u.z, qh[k][4 * j + 3] = (int)u.w;
+            ql[k][4 * j] = (int)v.x, ql[k][4 * j + 1] = (int)v.y, ql[k][4 * j + 2] = (int)v.z, ql[k][4 * j + 3] = (int)v.w;
+          }
+          qs[k / 2] |= made_scales[k * 64] << (16 * (k & 1));
+        }
+        mxd::lds_barrier();   // before the values come where they were
+      }
+      if constexpr (A::kWaves == 1) {
+#pragma unroll
+        for (int k = 0; k < KS; ++k) keep(qh[k]), keep(ql[k]);
+      }
+    }
+
 
     for (int it = it0; it < it1; ++it) {
       // -- scores --
@@ -481,9 +528,10 @@ __global__ __launch_bounds__(256, (Attend<WK, WV, kApart, RG>::kWaves)) void att
         const float by = power(m, next);
         m = next, l *= by;
 #pragma unroll
-        for (int d = 0; d < DB; ++d)
+        for (int d = 0; d < DB; ++d) {
 #pragma unroll
           for (int n = 0; n < 16; ++n) o[d][n] *= by;
+        }
       };
       if constexpr (!kSplit)
         if (__any(own != m)) rescale(own);
@@ -549,36 +597,42 @@ __global__ __launch_bounds__(256, (Attend<WK, WV, kApart, RG>::kWaves)) void att
     __syncthreads();   // and everybody has read its values
     const bool alone = x == unit0 && unit1 <= end;
     const int64_t slot = 2 * g + (g * per < unit0 ? 1 : 0);
-    float* part = (float*)(a.space + a.at.rows) + slot * A::kRows * WV;
-    auto whole = [&](int group, int r, float& most, float& all_l) {
-      most = kLowest, all_l = 0.f;
+    float most = kLowest, all_l = 0.f;
 #pragma unroll
-      for (int t = 0; t < TG; ++t) most = fmaxf(most, stats[t * RG + group][r][0]);
+    for (int t = 0; t < TG; ++t) most = fmaxf(most, stats[t * RG + rg][col][0]);
 #pragma unroll
-      for (int t = 0; t < TG; ++t) all_l += stats[t * RG + group][r][1] * power(stats[t * RG + group][r][0], most);
-    };
-    // four columns c of a row of row group `group`
-    auto put_out = [&](int group, int r, int c, float4 v) {
-      const int out_row = tile * A::kRows + group * 32 + r;
-      if (out_row >= rows) return;
-      float most, all_l;
-      whole(group, r, most, all_l);
+    for (int t = 0; t < TG; ++t) all_l += stats[t * RG + rg][col][1] * power(stats[t * RG + rg][col][0], most);
+    if (tg == 0 && half == 0) {
+      const int r = rg * 32 + col;
+      Place to{-1, 1.f};
+      if (row0 + col < rows) {
+        if (alone) {
+          const int head = h * a.group + row % a.group;
+          const int64_t token = s.first + i;
+          const RowOut f = row_out(a, head, most, all_l);
+          to = {token * a.q.out_stride + (int64_t)head * WV, f.inv};
+          if (a.q.lse) a.q.lse[token * a.q.heads + head] = f.lse;
+        } else {
+          to.at = (slot * A::kRows + r) * WV;
+          ((float2*)(a.space + a.at.stats))[slot * A::kRows + r] = make_float2(most, all_l);
+        }
+      }
+      places[r] = to;
+    }
+    __syncthreads();
+    float* part = (float*)(a.space + a.at.rows);
+    auto put_out = [&](int r, int c, float4 v) {   // four columns of a row
+      const Place to = places[r];
+      if (to.at < 0) return;
       if (alone) {
-        const int head = h * a.group + out_row % a.group;
-        const int64_t token = s.first + out_row / a.group;
-        const RowOut f = row_out(a, head, most, all_l);
         uint2 w;
-        w.x = mxd::bf16_pair(v.x * f.inv, v.y * f.inv), w.y = mxd::bf16_pair(v.z * f.inv, v.w * f.inv);
-        *(uint2*)(a.q.out + token * a.q.out_stride + (int64_t)head * WV + c) = w;
-        if (a.q.lse && c == 0) a.q.lse[token * a.q.heads + head] = f.lse;
+        w.x = mxd::bf16_pair(v.x * to.by, v.y * to.by), w.y = mxd::bf16_pair(v.z * to.by, v.w * to.by);
+        *(uint2*)(a.q.out + to.at + c) = w;
       } else {
-        *(float4*)(part + (int64_t)(group * 32 + r) * WV + c) = v;
-        if (c == 0) ((float2*)(a.space + a.at.stats))[slot * A::kRows + group * 32 + r] = make_float2(most, all_l);
+        *(float4*)(part + to.at + c) = v;
       }
     };
     float* own_out = (float*)(lds + wave * A::kOut);
-    float most, all_l;
-    whole(rg, col, most, all_l);
     const float by = power(m, most);
 #pragma unroll
     for (int d0 = 0; d0 < DB; d0 += CB / 32) {
@@ -592,23 +646,22 @@ __global__ __launch_bounds__(256, (Attend<WK, WV, kApart, RG>::kWaves)) void att
         }
       constexpr int L = CB / 4;   // lanes a row
       if constexpr (kSplit || TG == 1) {
-#pragma unroll
-        for (int r = 0; r < 32; r += 64 / L) {
-          const int at = r + lane / L, c = lane % L * 4;
-          put_out(rg, at, (kSplit ? tg * DB * 32 : 0) + d0 * 32 + c, *(const float4*)(own_out + at * (CB + 4) + c));
-        }
+        const int c = lane % L * 4;
+#pragma unroll 4
+        for (int r = lane / L; r < 32; r += 64 / L)
+          put_out(rg * 32 + r, (kSplit ? tg * DB * 32 : 0) + d0 * 32 + c, *(const float4*)(own_out + r * (CB + 4) + c));
       } else {
         __syncthreads();
-#pragma unroll
+#pragma unroll 1
         for (int e = tid; e < A::kRows * L; e += 256) {
-          const int r = e / L, c = e % L * 4, group = r / 32, at = r % 32;
+          const int r = e / L, c = e % L * 4;
           float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
           for (int t = 0; t < TG; ++t) {
-            const float4 w = *(const float4*)((const float*)(lds + (t * RG + group) * A::kOut) + at * (CB + 4) + c);
+            const float4 w = *(const float4*)((const float*)(lds + (t * RG + r / 32) * A::kOut) + r % 32 * (CB + 4) + c);
             v.x += w.x, v.y += w.y, v.z += w.z, v.w += w.w;
           }
-          put_out(group, at, d0 * 32 + c, v);
+          put_out(r, d0 * 32 + c, v);
         }
         __syncthreads();
       }
@@ -638,13 +691,15 @@ __global__ __launch_bounds__(256) void join_kernel(AttendArgs a, int tile_rows) 
   // the others' first pieces of work
   auto slot = [&](int i) { return (int64_t)2 * (blockIdx.x + i) + (i ? 0 : s.slot); };
   float most = kLowest;
+#pragma unroll 8
   for (int i = 0; i < s.parts; ++i) most = fmaxf(most, stats[slot(i) * tile_rows + r].x);
   float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
   float sum = 0.f;
+#pragma unroll 8
   for (int i = 0; i < s.parts; ++i) {
     const float2 st = stats[slot(i) * tile_rows + r];
-    const float by = power(st.x, most);
     const float4 p = *(const float4*)(parts + (slot(i) * tile_rows + r) * WV + c);
+    const float by = power(st.x, most);
     sum += st.y * by;
     v.x += p.x * by, v.y += p.y * by, v.z += p.z * by, v.w += p.w * by;
   }
@@ -677,7 +732,7 @@ auto by_widths(const mx_kv4* c, F fn) {
   return fn(integral_constant<int, 256>(), integral_constant<int, 256>(), std::true_type());
 }
 
-int workgroups(int value_width) { return kCus * (value_width <= 64 ? 3 : value_width <= 128 ? 2 : 1); }
+int workgroups(int value_width) { return kCus * waves(value_width); }
 
 // Row tiles of all sequences at most: each sequence's last one may be partly full.
 int64_t most_tiles(int64_t rows, int batch, int tile_rows) { return rows / tile_rows + batch; }
