@@ -33,7 +33,7 @@ typedef __bf16 v8b __attribute__((ext_vector_type(8)));
 typedef mxd::v8i v8i;
 
 constexpr int kCus = 256, kXcds = 8;
-constexpr int kInlineTiles = 1024;   // sequences, and row tiles of all of them, that every workgroup counts for itself
+constexpr int kInlineTiles = 1024;   // row tiles of all sequences that every workgroup counts for itself
 constexpr float kLowest = -3e38f;    // the maximum of a row that has seen nothing yet
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
@@ -103,13 +103,14 @@ struct Plan {
   int64_t* prefix;
 };
 
+// Sum of v over the threads before this one, and over all N; v below 2^26.
 template <int N>
-__device__ __forceinline__ int64_t scan(int64_t v, int64_t* sums, int64_t& all) {
+__device__ __forceinline__ int64_t scan(uint32_t v, uint32_t* sums, int64_t& all) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int64_t s = v;
+  uint32_t s = v;
 #pragma unroll
   for (int m = 1; m < 64; m <<= 1) {
-    const int64_t o = __shfl_up(s, m, 64);
+    const uint32_t o = __shfl_up(s, m, 64);
     s += lane >= m ? o : 0;
   }
   __syncthreads();
@@ -125,38 +126,45 @@ __device__ __forceinline__ int64_t scan(int64_t v, int64_t* sums, int64_t& all) 
   return before + s - v;
 }
 
-__device__ __forceinline__ int find(const int32_t* base, int n, int i) {   // the last b with base[b] <= i
+template <typename T>
+__device__ __forceinline__ int find(int n, T at_most) {   // the last i in [0, n) for which at_most(i), which 0 is
   int lo = 0, hi = n;
   while (hi - lo > 1) {
     const int mid = (lo + hi) / 2;
-    if (base[mid] <= i) lo = mid; else hi = mid;
+    if (at_most(mid)) lo = mid; else hi = mid;
   }
   return lo;
 }
 
 template <int N>
-__device__ __forceinline__ void make_plan(const AttendArgs& a, Plan p, int64_t* sums, int rows, int step) {
+__device__ __forceinline__ void make_plan(const AttendArgs& a, Plan p, uint32_t* sums, int rows, int step) {
   int64_t tiles = 0, all;
-  for (int b0 = 0; b0 < a.q.batch; b0 += N) {
-    const int b = b0 + threadIdx.x;
-    int64_t n = 0;
-    if (b < a.q.batch) n = ((int64_t)sequence(a, b).n * a.group + rows - 1) / rows;
-    const int64_t before = scan<N>(n, sums, all);
-    // (no more than there is room for: a q_first that does not ascend could name more rows than there are)
-    if (b < a.q.batch) p.base[b] = (int)min<int64_t>(tiles + before, a.tiles);
-    tiles += all;
+  const int each = a.q.q_first ? 0 : (a.q.tokens / a.q.batch * a.group + rows - 1) / rows;   // row tiles of a sequence
+  if (each) {
+    for (int b = threadIdx.x; b <= a.q.batch; b += N) p.base[b] = b * each;
+    tiles = (int64_t)a.q.batch * each;
+  } else {
+    for (int b0 = 0; b0 < a.q.batch; b0 += N) {
+      const int b = b0 + threadIdx.x;
+      uint32_t n = 0;
+      if (b < a.q.batch) n = (uint32_t)(((int64_t)sequence(a, b).n * a.group + rows - 1) / rows);
+      const int64_t before = scan<N>(n, sums, all);
+      // (no more than there is room for: a q_first that does not ascend could name more rows than there are)
+      if (b < a.q.batch) p.base[b] = (int)min<int64_t>(tiles + before, a.tiles);
+      tiles += all;
+    }
+    tiles = min<int64_t>(tiles, a.tiles);
+    if (threadIdx.x == 0) p.base[a.q.batch] = (int)tiles;
+    __syncthreads();
   }
-  tiles = min<int64_t>(tiles, a.tiles);
-  if (threadIdx.x == 0) p.base[a.q.batch] = (int)tiles;
-  __syncthreads();
   int64_t sum = 0;
   for (int i0 = 0; i0 < tiles; i0 += N) {
     const int i = i0 + threadIdx.x;
-    int64_t n = 0;
+    uint32_t n = 0;
     if (i < tiles) {
-      const int b = find(p.base, a.q.batch, i);
+      const int b = each ? i / each : find(a.q.batch, [&](int k) { return p.base[k] <= i; });
       int lo, hi;
-      n = tile_iterations(a, sequence(a, b), i - p.base[b], rows, step, lo, hi);
+      n = tile_iterations(a, sequence(a, b), each ? i - b * each : i - p.base[b], rows, step, lo, hi);
     }
     const int64_t before = scan<N>(n, sums, all);
     if (i < tiles) p.prefix[i] = sum + before;
@@ -167,8 +175,83 @@ __device__ __forceinline__ void make_plan(const AttendArgs& a, Plan p, int64_t* 
 }
 
 __global__ __launch_bounds__(1024) void plan_kernel(AttendArgs a, int rows, int step) {
-  __shared__ int64_t sums[16];
+  __shared__ uint32_t sums[16];
   make_plan<1024>(a, {(int32_t*)(a.space + a.at.base), (int64_t*)(a.space + a.at.prefix)}, sums, rows, step);
+}
+
+// What every lane holds, in scalar registers.
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ int64_t uniform(int64_t v) {
+  return (int64_t)((uint64_t)(uint32_t)uniform((int)(v >> 32)) << 32 | (uint32_t)uniform((int)v));
+}
+__device__ __forceinline__ Sequence uniform(Sequence s) {
+  s.first = uniform(s.first), s.n = uniform(s.n), s.held = uniform(s.held), s.end = uniform(s.end);
+  return s;
+}
+
+// A workgroup's way through the units: iterations in the order sequence, key head, row tile.
+struct Units {
+  int b, h, tile, tiles;    // the unit, and row tiles of its sequence
+  Sequence s;
+  int lo, hi;               // the tokens that its rows see
+  int64_t unit0, unit1;     // its iterations
+};
+
+__device__ __forceinline__ void enter(const AttendArgs& a, Units& u, int rows, int step) {
+  u.unit1 = u.unit0 + uniform(tile_iterations(a, u.s, u.tile, rows, step, u.lo, u.hi));
+  u.lo = uniform(u.lo), u.hi = uniform(u.hi);
+}
+
+__device__ __forceinline__ int tiles_of(const AttendArgs& a, const Sequence& s, int rows) {
+  return (int)(((int64_t)s.n * a.group + rows - 1) / rows);
+}
+
+__device__ __forceinline__ void next_unit(const AttendArgs& a, Units& u, int rows, int step) {
+  u.unit0 = u.unit1;
+  if (++u.tile == u.tiles) {
+    u.tile = 0;
+    if (++u.h == a.cache.heads) {
+      u.h = 0;
+      do {
+        if (++u.b == a.q.batch) return;   // no iterations are left
+        u.s = uniform(sequence(a, u.b));
+        u.tiles = tiles_of(a, u.s, rows);
+      } while (u.tiles == 0);
+    }
+  }
+  enter(a, u, rows, step);
+}
+
+// The unit of iteration x of `all`: by each thread of N its share of an LDS plan (found: two words), else by halving.
+template <int N>
+__device__ __forceinline__ void first_unit(const AttendArgs& a, const Plan& p, bool in_lds, int64_t x, int32_t* found, Units& u, int rows,
+                                           int step) {
+  const int64_t heads = a.cache.heads;
+  if (in_lds) {
+    for (int b = threadIdx.x; b < a.q.batch; b += N)
+      if (p.prefix[p.base[b]] * heads <= x && x < p.prefix[p.base[b + 1]] * heads) found[0] = b;
+    __syncthreads();
+    u.b = uniform(found[0]);
+  } else {
+    u.b = uniform(find(a.q.batch, [&](int b) { return p.prefix[p.base[b]] * heads <= x; }));
+  }
+  const int t0 = uniform(p.base[u.b]), t1 = uniform(p.base[u.b + 1]);
+  const int64_t p0 = uniform(p.prefix[t0]), span = uniform(p.prefix[t1]) - p0, in = x - p0 * heads;
+  u.h = (in | span) >> 32 ? (int)(in / span) : (int)((uint32_t)in / (uint32_t)span);
+  const int64_t rest = in - u.h * span + p0;
+  if (in_lds) {
+    for (int t = t0 + threadIdx.x; t < t1; t += N)
+      if (p.prefix[t] <= rest && rest < p.prefix[t + 1]) found[1] = t;
+    __syncthreads();
+    u.tile = uniform(found[1]) - t0;
+  } else {
+    u.tile = uniform(find(t1 - t0, [&](int t) { return p.prefix[t0 + t] <= rest; }));
+  }
+  u.h = uniform(u.h);
+  u.unit0 = x - (rest - uniform(p.prefix[t0 + u.tile]));
+  u.s = uniform(sequence(a, u.b));
+  u.tiles = tiles_of(a, u.s, rows);
+  enter(a, u, rows, step);
 }
 
 // Two E4M3 terms of 16 query values (BF16 pairs w) under the scale 2^(exponent - 127), which takes them into [-256, 256]:
@@ -225,31 +308,44 @@ __device__ __forceinline__ float halves_sum(float v) {
   return __int_as_float(p[0]) + __int_as_float(p[1]);
 }
 
-// Waves that a SIMD holds (so workgroups a CU), by what their registers allow.
-__host__ __device__ constexpr int waves(int value_width) { return value_width <= 64 ? 3 : value_width <= 128 ? 2 : 1; }
-
-// WK, WV: widths of a key and of a value; kApart: values have codes of their own; RG: the workgroup's row groups of 32. A
-// step is 4 / RG tiles of 32 tokens, each of which RG waves (one a row group) score and, in parts, convert.
-//
-// kSplit (latents): 32 rows of 512 columns and their queries would be 390 registers of a lane's 512 before anything else,
-// so a wave multiplies all of the step's tiles by WV RG / 4 columns of the values, and the waves of a row group exchange
-// their probabilities through LDS. Otherwise a wave keeps to its tile, and the waves' sums are added at the end.
-template <int WK, int WV, bool kApart, int RG>
-struct Attend {
-  static constexpr bool kSplit = WV >= 512;
-  static constexpr int TG = 4 / RG, kRows = 32 * RG, kStep = 32 * TG;
-  static constexpr int KS = WK / 64, VS = WV / 64, DB = WV / 32 / (kSplit ? TG : 1);
-  static constexpr int KW = scale_pitch(WK) / 4, VW = scale_pitch(WV) / 4;
-  static constexpr int VO = (VS + RG - 1) / RG;            // 64-column pieces of the values that a wave converts
-  static constexpr int kTile = 64 * WV;                    // bytes of 32 tokens' values in BF16
-  // of the values, where others read what a wave has written: two, so that one barrier a step is enough, if they fit
-  static constexpr int kBuffers = (RG > 1 || kSplit) && 2 * TG * kTile <= 131072 ? 2 : 1;
-  static constexpr int kExchange = kSplit ? 2 * 4 * 64 * 32 : 16;   // probabilities
-  static constexpr int CB = WV < 64 ? WV : 64;             // columns that go out at a time
-  static constexpr int kOut = 32 * (CB + 4) * 4;           // bytes of a wave's
-  static constexpr int kLds = TG * kBuffers * kTile > 4 * kOut ? TG * kBuffers * kTile : 4 * kOut;
-  static constexpr int kWaves = waves(WV), kGroups = kCus * kWaves;
+// 64 query values of a row from column c on as the right operand of a step: the lane's 2 x 16 (half: which of each 32) in two
+// terms, and their scale bytes.
+struct QueryStep {
+  uint32_t high[8], low[8], scales;
 };
+struct QueryWords {
+  uint32_t w[2][8];
+};
+
+__device__ __forceinline__ QueryWords query_words(const uint16_t* q, int c, int half) {
+  QueryWords r;
+#pragma unroll
+  for (int e = 0; e < 2; ++e)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const uint4 v = mxd::ldg128((const uint8_t*)(q + c + 32 * e + 16 * half + 8 * j));
+      r.w[e][4 * j] = v.x, r.w[e][4 * j + 1] = v.y, r.w[e][4 * j + 2] = v.z, r.w[e][4 * j + 3] = v.w;
+    }
+  return r;
+}
+
+__device__ __forceinline__ QueryStep query_step(const QueryWords& q, int half) {
+  QueryStep r;
+  uint32_t e[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    uint32_t top = q.w[i][0] & 0x7FFF7FFFu;
+#pragma unroll
+    for (int j = 1; j < 8; ++j) top = pair_max(top, q.w[i][j] & 0x7FFF7FFFu);
+    top = max(top & 0xFFFFu, top >> 16);
+    const auto both = __builtin_amdgcn_permlane32_swap(top, top, false, false);
+    e[i] = query_exponent(max((uint32_t)both[0], (uint32_t)both[1]));
+    split16(q.w[i], min(e[i], 247u), r.high + 4 * i, r.low + 4 * i);
+  }
+  const uint32_t own = half ? e[1] : e[0];
+  r.scales = own | (own == 255u ? 255u : own - 4u) << 8;
+  return r;
+}
 
 // Where a row of a unit goes (in values; -1: nowhere), and its factor.
 struct Place {
@@ -269,29 +365,391 @@ __device__ __forceinline__ float power(float from, float to) {   // 2^(from - to
   return from == to ? 1.f : __builtin_amdgcn_exp2f(from - to);
 }
 
-template <int WK, int WV, bool kApart, int RG>
-__global__ __launch_bounds__(256, (Attend<WK, WV, kApart, RG>::kWaves)) void attend_kernel(AttendArgs a, int inline_plan) {
-  using A = Attend<WK, WV, kApart, RG>;
-  constexpr bool kSplit = A::kSplit;
-  constexpr int TG = A::TG, KS = A::KS, VS = A::VS, DB = A::DB, KW = A::KW, VW = A::VW, VO = A::VO, CB = A::CB;
+// Latents. 64 (or 32) rows of 512 columns with their queries are 64 (32) + 66 registers of each of the workgroup's eight
+// waves, two a SIMD: with one, of 512 registers, every other instruction slot stays empty (7.5 clocks an instruction).
+//
+// A step is TG tiles of 32 tokens. The waves of a row group and tile split the width: each scores its half, they exchange
+// half of the sums, and each goes on with 16 of the tile's tokens. Wave kh takes its tokens rotated by 16, so that what it
+// keeps is in the first registers. For the values each wave has WV RG / 8 columns of all of the step's tokens.
+template <int WK, int RG>
+struct Latent {
+  static constexpr int WV = 512, TG = 4 / RG, kRows = 32 * RG, kStep = 32 * TG, CG = 8 / RG;
+  static constexpr int KS = WK / 64, KH = (KS + 1) / 2;    // 64-column steps of a key, and of a wave: kh's 4 and the last
+  static constexpr int DB = WV / 32 / CG;                  // 32-column blocks of a wave
+  static constexpr int VO = 4 / RG;                        // 64-column pieces of the values that a wave converts
+  static constexpr int kTile = 64 * WV;                    // bytes of 32 tokens' values in BF16
+  static constexpr int kBuffers = RG > 1 ? 2 : 1;
+  static constexpr int kValues = kBuffers * TG * kTile;
+  static constexpr int kSums = 8 * 2048, kWeights = 8 * 1024;   // what waves exchange: half sums, probabilities
+  static constexpr int CB = 64, kOut = 32 * (CB + 4) * 4;  // columns that go out at a time, and a wave's bytes of them
+};
+
+template <int WK, int RG>
+__global__ __launch_bounds__(512, 2) void latent_kernel(AttendArgs a, int inline_plan) {
+  using A = Latent<WK, RG>;
+  constexpr int WV = A::WV, TG = A::TG, CG = A::CG, KS = A::KS, KH = A::KH, DB = A::DB, VO = A::VO, CB = A::CB;
+  __shared__ __attribute__((aligned(16))) uint8_t lds[A::kValues + A::kSums + A::kWeights];
+  __shared__ __attribute__((aligned(16))) float tops[RG][32][CG];
+  __shared__ float stats[8][32];
+  __shared__ Place places[A::kRows];
+  __shared__ uint32_t sums[8];
+  __shared__ int32_t found[2];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int rg = wave % RG, cg = wave / RG, kh = cg & 1, tile = cg >> 1;
+  const int col = lane & 31, half = lane >> 5;   // the lane's query row of the products
+  const int mine = col ^ (16 * kh);              // as a loader, its token of the tile
+  uint8_t *half_sums = lds + A::kValues, *weights = half_sums + A::kSums;
+
+  Plan plan{(int32_t*)(a.space + a.at.base), (int64_t*)(a.space + a.at.prefix)};
+  if (inline_plan) {
+    plan = {(int32_t*)(lds + 8 * (kInlineTiles + 1)), (int64_t*)lds};
+    make_plan<512>(a, plan, sums, A::kRows, A::kStep);
+  }
+  const int64_t all = uniform(plan.prefix[plan.base[a.q.batch]]) * a.cache.heads;
+  const int64_t per = max<int64_t>((all + kCus - 1) / kCus, 1);
+  // workgroups go round the XCDs: neighbours in the work, which share keys, to one L2
+  const int g = (int)(blockIdx.x % kXcds) * (kCus / kXcds) + (int)blockIdx.x / kXcds;
+  int64_t x = min(g * per, all);
+  const int64_t end = min(x + per, all);
+  Shared* shared = (Shared*)(a.space + a.at.units) + g;
+  if (x >= end) {
+    if (tid == 0) shared->parts = 0;
+    return;
+  }
+  Units u;
+  first_unit<512>(a, plan, inline_plan, x, found, u, A::kRows, A::kStep);
+
+  // LDS places of the values: a loader's 16-byte pieces of its token, and a reader's 8 bytes; pieces of neighbouring tokens
+  // lie apart
+  const int spread = 2 * (mine & 3) + ((mine >> 2) & 1);
+  uint32_t put[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) put[i] = tile * A::kTile + mine * (2 * WV) + ((4 * half + i) ^ spread) * 16;
+  const int rt = (lane & 15) >> 2, rc = lane & 3, rs = 2 * rt + half;
+  const uint32_t get0 = cg * (DB * 64) + (4 * half + rt) * (2 * WV) + ((2 * ((lane >> 4) & 1) + rc / 2) ^ rs) * 16 + (rc & 1) * 8;
+  const uint32_t get1 = get0 ^ 64;
+
+  for (;;) {
+    const int it0 = (int)(x - u.unit0), it1 = (int)(min(u.unit1, end) - u.unit0);
+    // -- the wave's query rows --
+    const int rows = u.s.n * a.group;   // at most 2^30
+    const int row0 = u.tile * A::kRows + rg * 32, row = min(row0 + col, rows - 1);
+    const int i = row / a.group;
+    int row_lo, row_hi;
+    seen(a, u.s, i, row_lo, row_hi);
+    // tokens [all_lo, all_hi) are seen by all of the wave's rows
+    int all_lo, all_hi, unused;
+    seen(a, u.s, min(row0, rows - 1) / a.group, unused, all_hi);
+    seen(a, u.s, min(row0 + 31, rows - 1) / a.group, all_lo, unused);
+    all_lo = uniform(all_lo), all_hi = uniform(all_hi);
+
+    // -- loads: the lane's token of a step, its page a step ahead --
+    const int32_t* table = a.q.table + (int64_t)u.b * a.q.columns;
+    const int lo = u.lo, hi = u.hi, h = u.h;
+    auto token_of = [&](int it) { return lo + (it * TG + tile) * 32 + mine; };
+    auto page_of = [&](int it) {
+      const int t = token_of(it);
+      return it < it1 && t < hi ? table[t >> a.page_shift] : -1;
+    };
+    uint4 kreg[KH];
+    uint32_t kscale[(KH + 1) / 2];
+    bool valid = false;
+    auto load = [&](int it, int page) {
+      valid = page >= 0 && page < a.cache.pages;
+      const int64_t at = ((int64_t)(valid ? page : 0) * a.cache.heads + h << a.page_shift) + (token_of(it) & ((1 << a.page_shift) - 1));
+      const uint8_t* p = a.cache.k_codes + at * (WK / 2) + 128 * kh + 16 * half;
+      const uint8_t* ps = a.cache.k_scales + at * scale_pitch(WK) + 8 * kh;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) kreg[k] = mxd::ldg128(p + 32 * k);
+      kscale[0] = mxd::ldg32(ps), kscale[1] = mxd::ldg32(ps + 4);
+      if constexpr (KS > 8) {
+        if (kh == 0) kreg[4] = mxd::ldg128(p + 256), kscale[2] = mxd::ldg32(ps + 16);
+      }
+    };
+    load(it0, page_of(it0));
+    int page_next = page_of(it0 + 1);
+
+    // -- the queries: the row group's waves convert KS / CG steps of 64 values each and exchange them --
+    v8i qh[KH], ql[KH];
+    uint32_t qs[(KH + 1) / 2] = {};
+    {
+      const uint16_t* q = a.q.q + (u.s.first + i) * a.q.q_stride + (int64_t)(h * a.group + row % a.group) * WK;
+      constexpr int kEach = (KS + CG - 1) / CG;
+      QueryWords words[kEach];
+#pragma unroll
+      for (int e = 0; e < kEach; ++e)
+        if (KS % CG == 0 || e * CG + cg < KS) words[e] = query_words(q, 64 * (e * CG + cg), half);
+      uint4* made = (uint4*)lds + rg * (KS * 256) + lane;
+      uint32_t* made_scales = (uint32_t*)(lds + RG * KS * 4096) + rg * (KS * 64) + lane;
+      __syncthreads();   // the plan, or the last unit's rows, have been read
+#pragma unroll
+      for (int e = 0; e < kEach; ++e) {
+        const int k = e * CG + cg;
+        if (KS % CG && k >= KS) break;
+        const QueryStep s = query_step(words[e], half);
+        made[k * 256] = make_uint4(s.high[0], s.high[1], s.high[2], s.high[3]), made[k * 256 + 64] = make_uint4(s.high[4], s.high[5], s.high[6], s.high[7]);
+        made[k * 256 + 128] = make_uint4(s.low[0], s.low[1], s.low[2], s.low[3]), made[k * 256 + 192] = make_uint4(s.low[4], s.low[5], s.low[6], s.low[7]);
+        made_scales[k * 64] = s.scales;
+      }
+      mxd::lds_barrier();
+#pragma unroll
+      for (int e = 0; e < KH; ++e) {
+        const int k = e < 4 ? 4 * kh + e : 8;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const uint4 w = made[k * 256 + 64 * j], v = made[k * 256 + 128 + 64 * j];
+          qh[e][4 * j] = (int)w.x, qh[e][4 * j + 1] = (int)w.y, qh[e][4 * j + 2] = (int)w.z, qh[e][4 * j + 3] = (int)w.w;
+          ql[e][4 * j] = (int)v.x, ql[e][4 * j + 1] = (int)v.y, ql[e][4 * j + 2] = (int)v.z, ql[e][4 * j + 3] = (int)v.w;
+        }
+        qs[e / 2] |= made_scales[k * 64] << (16 * (e & 1));
+      }
+      mxd::lds_barrier();   // before the values come where they were
+    }
+
+    float m = kLowest, l = 0.f;   // the maximum is a whole number: every rescaling is exact
+    v16f o[DB];
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int n = 0; n < 16; ++n) o[d][n] = 0.f;
+
+    for (int it = it0; it < it1; ++it) {
+      // -- scores of the wave's half of the width --
+      uint32_t ks[(KH + 1) / 2];
+#pragma unroll
+      for (int w = 0; w < (KH + 1) / 2; ++w) ks[w] = kscale[w] >> (8 * half);
+      v16f sc;
+#pragma unroll
+      for (int n = 0; n < 16; ++n) sc[n] = 0.f;
+#pragma unroll
+      for (int k = 0; k < KH; ++k) {
+        if (k == 4 && kh) break;
+        if (k & 1) {
+          sc = scores<2, 2>(kreg[k], qh[k], sc, ks[k / 2], qs[k / 2]);
+          sc = scores<2, 3>(kreg[k], ql[k], sc, ks[k / 2], qs[k / 2]);
+        } else {
+          sc = scores<0, 0>(kreg[k], qh[k], sc, ks[k / 2], qs[k / 2]);
+          sc = scores<0, 1>(kreg[k], ql[k], sc, ks[k / 2], qs[k / 2]);
+        }
+      }
+      // -- values to BF16: pieces rg, rg + RG, ... of the wave's four --
+      uint8_t* buffer = lds + (A::kBuffers > 1 ? (it & 1) * (TG * A::kTile) : 0);
+      auto convert = [&] {
+#pragma unroll
+        for (int k = 0; k < VO; ++k) {
+          uint4 w = kreg[k * RG];
+          uint32_t word = ks[k * RG / 2] >> (16 * (k * RG & 1));
+#pragma unroll
+          for (int r = 1; r < RG; ++r)
+            if (rg == r) w = kreg[k * RG + r], word = ks[(k * RG + r) / 2] >> (16 * ((k * RG + r) & 1));
+          const uint32_t e = word & 255u;
+          const bool hide = e == 255u || !valid;   // counts as zero: who sees a NaN token sees it in the score
+          const float scale = mx::u2f((hide ? 127u : e) << 23);
+          const uint32_t c[4] = {hide ? 0u : w.x, hide ? 0u : w.y, hide ? 0u : w.z, hide ? 0u : w.w};
+#pragma unroll
+          for (int n = 0; n < 4; ++n) {
+            uint4 v;
+            v.x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c[n], scale, 0));
+            v.y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c[n], scale, 1));
+            v.z = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c[n], scale, 2));
+            v.w = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c[n], scale, 3));
+            *(uint4*)(buffer + put[n] + 128 * (4 * kh + k * RG + rg)) = v;
+          }
+        }
+      };
+      if (A::kBuffers > 1) convert();
+      // -- the other half's sums of the tokens that stay here (registers 0 to 7) --
+      {
+        float4* to = (float4*)(half_sums + wave * 2048) + lane;
+        to[0] = make_float4(sc[8], sc[9], sc[10], sc[11]), to[64] = make_float4(sc[12], sc[13], sc[14], sc[15]);
+      }
+      mxd::lds_barrier();
+      float s[8];
+      {
+        const float4* from = (const float4*)(half_sums + (wave ^ RG) * 2048) + lane;
+        const float4 u0 = from[0], u1 = from[64];
+        s[0] = sc[0] + u0.x, s[1] = sc[1] + u0.y, s[2] = sc[2] + u0.z, s[3] = sc[3] + u0.w;
+        s[4] = sc[4] + u1.x, s[5] = sc[5] + u1.y, s[6] = sc[6] + u1.z, s[7] = sc[7] + u1.w;
+      }
+      if (A::kBuffers == 1) convert();   // nobody reads the last step's any more
+      const uint32_t shown = (uint32_t)__ballot(valid) & 0xFFFFu;
+      const int first = lo + (it * TG + tile) * 32 + 16 * kh;
+      load(it + 1, page_next);
+      page_next = page_of(it + 2);
+      // -- softmax --
+      if (shown != 0xFFFFu || first < all_lo || first + 16 > all_hi) {
+#pragma unroll
+        for (int n = 0; n < 8; ++n) {
+          const int t = 8 * (n / 4) + 4 * half + (n & 3);
+          s[n] = (shown >> t & 1) && first + t >= row_lo && first + t < row_hi ? s[n] : -INFINITY;
+        }
+      }
+      float top = fmaxf(s[0], s[1]);
+#pragma unroll
+      for (int n = 2; n < 8; ++n) top = fmaxf(top, s[n]);
+      top = other_half_max(top) * a.c;
+      // the maximum stays until it is 2^8 too low: probabilities up to 2^8 lose nothing
+      const float own = top > m + 8.f ? ceilf(top) : m;
+      uint32_t p[4];
+      float sum = 0.f;
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        const float p0 = __builtin_amdgcn_exp2f(fmaf(s[2 * n], a.c, -own)), p1 = __builtin_amdgcn_exp2f(fmaf(s[2 * n + 1], a.c, -own));
+        sum += p0 + p1;
+        p[n] = mxd::bf16_pair(p0, p1);
+      }
+      ((uint4*)(weights + wave * 1024))[lane] = make_uint4(p[0], p[1], p[2], p[3]);
+      if (half == 0) tops[rg][col][cg] = own;
+      mxd::lds_barrier();
+      float theirs[CG], next = kLowest;
+      {
+        const float4* from = (const float4*)tops[rg][col];
+#pragma unroll
+        for (int t = 0; t < CG / 4; ++t) {
+          const float4 v = from[t];
+          theirs[4 * t] = v.x, theirs[4 * t + 1] = v.y, theirs[4 * t + 2] = v.z, theirs[4 * t + 3] = v.w;
+          next = fmaxf(next, fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)));
+        }
+      }
+      const bool moved = __any(next != m);   // else everybody's is m
+      if (moved) {
+        const float by = power(m, next);
+        m = next, l *= by;
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+          for (int n = 0; n < 16; ++n) o[d][n] *= by;
+        sum *= power(own, next);
+      }
+      l += sum;
+      // -- O^T += V^T P^T --
+#pragma unroll
+      for (int t = 0; t < CG; ++t) {   // 16 tokens, of the wave that weighed them
+        const uint4 w = ((const uint4*)(weights + (t * RG + rg) * 1024))[lane];
+        uint32_t pw[4] = {w.x, w.y, w.z, w.w};
+        if (moved) {   // whole powers of two: exact
+          const float by = power(theirs[t], m);
+#pragma unroll
+          for (int n = 0; n < 4; ++n) pw[n] = mxd::bf16_pair(mx::u2f(pw[n] << 16) * by, mx::u2f(pw[n] & 0xFFFF0000u) * by);
+        }
+        const v8b pv = __builtin_bit_cast(v8b, make_uint4(pw[0], pw[1], pw[2], pw[3]));
+#pragma unroll
+        for (int d = 0; d < DB; ++d) {
+          const uint8_t* at = buffer + (d & 1 ? get1 : get0) + 128 * (d / 2) + (t >> 1) * A::kTile + 16 * (t & 1) * (2 * WV);
+          typedef __attribute__((address_space(3))) v4s lds_v4s;
+          v4s w2[2];
+          w2[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)at);
+          w2[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(at + 8 * (2 * WV)));
+          const v8b vv = __builtin_bit_cast(v8b, w2);
+          o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vv, pv, o[d], 0, 0, 0);
+        }
+      }
+    }
+
+    // -- the row's sum over the waves, and out --
+    l = halves_sum(l);
+    if (half == 0) stats[wave][col] = l;
+    __syncthreads();   // and everybody has read its values
+    const bool alone = x == u.unit0 && u.unit1 <= end;
+    const int64_t slot = 2 * g + (g * per < u.unit0 ? 1 : 0);
+    if (cg == 0 && half == 0) {
+      float all_l = 0.f;
+#pragma unroll
+      for (int t = 0; t < CG; ++t) all_l += stats[t * RG + rg][col];
+      Place to{-1, 1.f};
+      if (row0 + col < rows) {
+        if (alone) {
+          const int head = h * a.group + row % a.group;
+          const int64_t token = u.s.first + i;
+          const RowOut f = row_out(a, head, m, all_l);
+          to = {token * a.q.out_stride + (int64_t)head * WV, f.inv};
+          if (a.q.lse) a.q.lse[token * a.q.heads + head] = f.lse;
+        } else {
+          ((float2*)(a.space + a.at.stats))[slot * A::kRows + rg * 32 + col] = make_float2(m, all_l);
+        }
+      }
+      places[rg * 32 + col] = to;
+    }
+    if (alone) {
+      __syncthreads();
+      float* own_out = (float*)(lds + wave * A::kOut);
+#pragma unroll
+      for (int d0 = 0; d0 < DB; d0 += 2) {
+#pragma unroll
+        for (int d = 0; d < 2; ++d)
+#pragma unroll
+          for (int n = 0; n < 4; ++n) {
+            const v16f& v = o[d0 + d];
+            *(float4*)(own_out + col * (CB + 4) + 32 * d + 8 * n + 4 * half) = make_float4(v[4 * n], v[4 * n + 1], v[4 * n + 2], v[4 * n + 3]);
+          }
+#pragma unroll 2
+        for (int r = lane / 8; r < 32; r += 8) {
+          const int c = lane % 8 * 8;
+          const Place to = places[rg * 32 + r];
+          const float4 v0 = *(const float4*)(own_out + r * (CB + 4) + c), v1 = *(const float4*)(own_out + r * (CB + 4) + c + 4);
+          if (to.at < 0) continue;
+          uint4 w;
+          w.x = mxd::bf16_pair(v0.x * to.by, v0.y * to.by), w.y = mxd::bf16_pair(v0.z * to.by, v0.w * to.by);
+          w.z = mxd::bf16_pair(v1.x * to.by, v1.y * to.by), w.w = mxd::bf16_pair(v1.z * to.by, v1.w * to.by);
+          *(uint4*)(a.q.out + to.at + cg * (DB * 32) + d0 * 32 + c) = w;
+        }
+      }
+    } else {   // parts as the registers have them: [wave][block][4 registers][lane]
+      float4* part = (float4*)(a.space + a.at.rows) + (slot * 8 + wave) * (DB * 4 * 64) + lane;
+#pragma unroll
+      for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int n = 0; n < 4; ++n) part[(d * 4 + n) * 64] = make_float4(o[d][4 * n], o[d][4 * n + 1], o[d][4 * n + 2], o[d][4 * n + 3]);
+    }
+    if (u.unit1 >= end) {   // the workgroup's last: it joins the unit if it began it and does not end it
+      if (tid == 0) {
+        Shared v{u.b, h, u.tile, 0, (int)(slot & 1)};
+        if (!alone && x == u.unit0) v.parts = (int)((u.unit1 - 1) / per - g + 1);
+        *shared = v;
+      }
+      return;
+    }
+    x = u.unit1;
+    next_unit(a, u, A::kRows, A::kStep);
+  }
+}
+
+// Waves of the grouped kernel that a SIMD holds (so workgroups a CU), by what their registers allow.
+__host__ __device__ constexpr int waves(int width) { return width <= 64 ? 3 : width <= 128 ? 2 : 1; }
+
+// Values apart from their keys. A step is TG = 4 / RG tiles of 32 tokens, a tile the work of RG waves, one a row group, which
+// share its values; a wave keeps to its tile, and the token groups' sums are added at the end.
+template <int W, int RG>
+struct Grouped {
+  static constexpr int TG = 4 / RG, kRows = 32 * RG, kStep = 32 * TG;
+  static constexpr int KS = W / 64, DB = W / 32, KW = scale_pitch(W) / 4;
+  static constexpr int VO = (KS + RG - 1) / RG;            // 64-column pieces of the values that a wave converts
+  static constexpr int kTile = 64 * W;                     // bytes of 32 tokens' values in BF16
+  static constexpr int kBuffers = RG > 1 ? 2 : 1;          // others read what a wave has written: with two, one barrier a step
+  static constexpr int CB = 64, kOut = 32 * (CB + 4) * 4;  // columns that go out at a time, and a wave's bytes of them
+  static constexpr int kValues = TG * kBuffers * kTile, kLds = kValues > 4 * kOut ? kValues : 4 * kOut;
+  static constexpr int kWaves = waves(W), kGroups = kCus * kWaves;
+};
+
+template <int W, int RG>
+__global__ __launch_bounds__(256, (Grouped<W, RG>::kWaves)) void grouped_kernel(AttendArgs a, int inline_plan) {
+  using A = Grouped<W, RG>;
+  constexpr int TG = A::TG, KS = A::KS, DB = A::DB, KW = A::KW, VO = A::VO, CB = A::CB;
   __shared__ __attribute__((aligned(16))) uint8_t lds[A::kLds];
-  __shared__ __attribute__((aligned(16))) uint8_t exchange[A::kExchange];
-  __shared__ float tops[2][4][32];
   __shared__ float stats[4][32][2];
   __shared__ Place places[A::kRows];
-  __shared__ int64_t plan_prefix[kInlineTiles + 1];
-  __shared__ int32_t plan_base[kInlineTiles + 1];
-  __shared__ int64_t sums[4];
+  __shared__ uint32_t sums[4];
+  __shared__ int32_t found[2];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int rg = wave % RG, tg = wave / RG;
   const int col = lane & 31, half = lane >> 5;   // the lane's query row of the products; as a loader, its token
 
   Plan plan{(int32_t*)(a.space + a.at.base), (int64_t*)(a.space + a.at.prefix)};
   if (inline_plan) {
-    plan = {plan_base, plan_prefix};
+    plan = {(int32_t*)(lds + 8 * (kInlineTiles + 1)), (int64_t*)lds};
     make_plan<256>(a, plan, sums, A::kRows, A::kStep);
   }
-  const int64_t all = plan.prefix[plan.base[a.q.batch]] * a.cache.heads;
+  const int64_t all = uniform(plan.prefix[plan.base[a.q.batch]]) * a.cache.heads;
   constexpr int groups = A::kGroups;
   const int64_t per = max<int64_t>((all + groups - 1) / groups, 1);
   // workgroups go round the XCDs: neighbours in the work, which share keys, to one L2
@@ -299,133 +757,92 @@ __global__ __launch_bounds__(256, (Attend<WK, WV, kApart, RG>::kWaves)) void att
   int64_t x = min(g * per, all);
   const int64_t end = min(x + per, all);
   Shared* shared = (Shared*)(a.space + a.at.units) + g;
-  if (tid == 0 && x >= end) shared->parts = 0;
+  if (x >= end) {
+    if (tid == 0) shared->parts = 0;
+    return;
+  }
+  Units u;
+  first_unit<256>(a, plan, inline_plan, x, found, u, A::kRows, A::kStep);
 
   // LDS places: a loader's 16-byte pieces of its token, and a reader's 8 bytes; pieces of neighbouring tokens lie apart
   const int spread = 2 * (col & 3) + ((col >> 2) & 1);
   uint32_t put[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) put[i] = col * (2 * WV) + ((4 * half + i) ^ spread) * 16;
+  for (int i = 0; i < 4; ++i) put[i] = tg * A::kTile + col * (2 * W) + ((4 * half + i) ^ spread) * 16;
   const int rt = (lane & 15) >> 2, rc = lane & 3, rs = 2 * rt + half;
-  const uint32_t get0 = (4 * half + rt) * (2 * WV) + ((2 * ((lane >> 4) & 1) + rc / 2) ^ rs) * 16 + (rc & 1) * 8;
+  const uint32_t get0 = tg * A::kTile + (4 * half + rt) * (2 * W) + ((2 * ((lane >> 4) & 1) + rc / 2) ^ rs) * 16 + (rc & 1) * 8;
   const uint32_t get1 = get0 ^ 64;
 
-  while (x < end) {
-    // -- the unit of iteration x --
-    int b;
-    {
-      int lo = 0, hi = a.q.batch;
-      while (hi - lo > 1) {
-        const int mid = (lo + hi) / 2;
-        if (plan.prefix[plan.base[mid]] * a.cache.heads <= x) lo = mid; else hi = mid;
-      }
-      b = lo;
-    }
-    const int t0 = plan.base[b], t1 = plan.base[b + 1];
-    const int64_t p0 = plan.prefix[t0], span = plan.prefix[t1] - p0;
-    const int64_t in = x - p0 * a.cache.heads;
-    const int h = (in | span) >> 32 ? (int)(in / span) : (int)((uint32_t)in / (uint32_t)span);
-    const int64_t rest = in - h * span;
-    int tile;
-    {
-      int lo = t0, hi = t1;
-      while (hi - lo > 1) {
-        const int mid = (lo + hi) / 2;
-        if (plan.prefix[mid] - p0 <= rest) lo = mid; else hi = mid;
-      }
-      tile = lo - t0;
-    }
-    const int64_t unit0 = x - (rest - (plan.prefix[t0 + tile] - p0)), unit1 = unit0 + plan.prefix[t0 + tile + 1] - plan.prefix[t0 + tile];
-    const Sequence s = sequence(a, b);
-    int lo, hi;
-    tile_iterations(a, s, tile, A::kRows, A::kStep, lo, hi);
-    const int it0 = (int)(x - unit0), it1 = (int)(min(unit1, end) - unit0);
-
+  for (;;) {
+    const int it0 = (int)(x - u.unit0), it1 = (int)(min(u.unit1, end) - u.unit0);
     // -- the wave's query rows --
-    const int rows = s.n * a.group;   // at most 2^30
-    const int row0 = tile * A::kRows + rg * 32, row = min(row0 + col, rows - 1);
+    const int rows = u.s.n * a.group;   // at most 2^30
+    const int row0 = u.tile * A::kRows + rg * 32, row = min(row0 + col, rows - 1);
     const int i = row / a.group;
     int row_lo, row_hi;
-    seen(a, s, i, row_lo, row_hi);
+    seen(a, u.s, i, row_lo, row_hi);
     // tokens [all_lo, all_hi) are seen by all of the wave's rows
     int all_lo, all_hi, unused;
-    seen(a, s, min(row0, rows - 1) / a.group, unused, all_hi);
-    seen(a, s, min(row0 + 31, rows - 1) / a.group, all_lo, unused);
-
-    float m = kLowest, l = 0.f;   // the maximum is a whole number: every rescaling is exact
-    v16f o[DB];
-#pragma unroll
-    for (int d = 0; d < DB; ++d) {
-#pragma unroll
-      for (int n = 0; n < 16; ++n) o[d][n] = 0.f;
-    }
+    seen(a, u.s, min(row0, rows - 1) / a.group, unused, all_hi);
+    seen(a, u.s, min(row0 + 31, rows - 1) / a.group, all_lo, unused);
+    all_lo = uniform(all_lo), all_hi = uniform(all_hi);
 
     // -- loads: the lane's token of a step, its page a step ahead --
-    const int32_t* table = a.q.table + (int64_t)b * a.q.columns;
+    const int32_t* table = a.q.table + (int64_t)u.b * a.q.columns;
+    const int lo = u.lo, hi = u.hi, h = u.h;
     auto token_of = [&](int it) { return lo + (it * TG + tg) * 32 + col; };
     auto page_of = [&](int it) {
       const int t = token_of(it);
       return it < it1 && t < hi ? table[t >> a.page_shift] : -1;
     };
     uint4 kreg[KS], vreg[VO];
-    uint32_t kscale[KW], vscale[VW];
+    uint32_t kscale[KW], vscale[KW];
     bool valid = false;
     auto load = [&](int it, int page) {
       valid = page >= 0 && page < a.cache.pages;
       const int64_t at = ((int64_t)(valid ? page : 0) * a.cache.heads + h << a.page_shift) + (token_of(it) & ((1 << a.page_shift) - 1));
-      const uint8_t* p = a.cache.k_codes + at * (WK / 2) + 16 * half;
+      const uint8_t* p = a.cache.k_codes + at * (W / 2) + 16 * half;
+      const uint8_t* pv = a.cache.v_codes + at * (W / 2) + 16 * half;
 #pragma unroll
       for (int k = 0; k < KS; ++k) kreg[k] = mxd::ldg128(p + 32 * k);
 #pragma unroll
-      for (int w = 0; w < KW; ++w) kscale[w] = mxd::ldg32(a.cache.k_scales + at * scale_pitch(WK) + 4 * w);
-      if constexpr (kApart) {
-#pragma unroll
-        for (int w = 0; w < VW; ++w) vscale[w] = mxd::ldg32(a.cache.v_scales + at * scale_pitch(WV) + 4 * w);
-        const uint8_t* pv = a.cache.v_codes + at * (WV / 2) + 16 * half;
-#pragma unroll
-        for (int k = 0; k < VO; ++k)
-          if (k * RG + rg < VS) vreg[k] = mxd::ldg128(pv + 32 * (k * RG + rg));
+      for (int w = 0; w < KW; ++w) {
+        kscale[w] = mxd::ldg32(a.cache.k_scales + at * scale_pitch(W) + 4 * w);
+        vscale[w] = mxd::ldg32(a.cache.v_scales + at * scale_pitch(W) + 4 * w);
       }
+#pragma unroll
+      for (int k = 0; k < VO; ++k)
+        if (k * RG + rg < KS) vreg[k] = mxd::ldg128(pv + 32 * (k * RG + rg));
     };
     load(it0, page_of(it0));
     int page_next = page_of(it0 + 1);
 
+    // -- the queries: a row group's waves convert KS / TG steps of 64 values each and exchange them --
     v8i qh[KS], ql[KS];
     uint32_t qs[(KS + 1) / 2] = {};
     {
-      // 64 values of a step, 2 x 16 a lane; the waves of a row group take turns and exchange what they made
-      const uint16_t* q = a.q.q + (s.first + i) * a.q.q_stride + (int64_t)(h * a.group + row % a.group) * WK;
+      const uint16_t* q = a.q.q + (u.s.first + i) * a.q.q_stride + (int64_t)(h * a.group + row % a.group) * W;
+      constexpr int kEach = (KS + TG - 1) / TG;
+      QueryWords words[kEach];
+#pragma unroll
+      for (int e = 0; e < kEach; ++e)
+        if (e * TG + tg < KS) words[e] = query_words(q, 64 * (e * TG + tg), half);
       uint4* made = (uint4*)lds + rg * (KS * 256) + lane;
       uint32_t* made_scales = (uint32_t*)(lds + RG * KS * 4096) + rg * (KS * 64) + lane;
+      __syncthreads();   // the plan, or the last unit's rows, have been read
 #pragma unroll
-      for (int k = 0; k < KS; ++k) {
-        if (TG > 1 && k % TG != tg) continue;
-        uint32_t w[2][8], top[2], high[8], low[8];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const uint4 v = mxd::ldg128((const uint8_t*)(q + 64 * k + 32 * e + 16 * half + 8 * j));
-            w[e][4 * j] = v.x, w[e][4 * j + 1] = v.y, w[e][4 * j + 2] = v.z, w[e][4 * j + 3] = v.w;
-          }
-          top[e] = w[e][0] & 0x7FFF7FFFu;
-#pragma unroll
-          for (int j = 1; j < 8; ++j) top[e] = pair_max(top[e], w[e][j] & 0x7FFF7FFFu);
-          top[e] = max(top[e] & 0xFFFFu, top[e] >> 16);
-          top[e] = max(top[e], (uint32_t)__shfl_xor((int)top[e], 32, 64));
-        }
-        const uint32_t e0 = query_exponent(top[0]), e1 = query_exponent(top[1]), own = half ? e1 : e0;
-        split16(w[0], min(e0, 247u), high, low);
-        split16(w[1], min(e1, 247u), high + 4, low + 4);
-        const uint32_t scales = own | (own == 255u ? 255u : own - 4u) << 8;
+      for (int e = 0; e < kEach; ++e) {
+        const int k = e * TG + tg;
+        if (k >= KS) break;
+        const QueryStep s = query_step(words[e], half);
         if constexpr (TG > 1) {
-          made[k * 256] = make_uint4(high[0], high[1], high[2], high[3]), made[k * 256 + 64] = make_uint4(high[4], high[5], high[6], high[7]);
-          made[k * 256 + 128] = make_uint4(low[0], low[1], low[2], low[3]), made[k * 256 + 192] = make_uint4(low[4], low[5], low[6], low[7]);
-          made_scales[k * 64] = scales;
+          made[k * 256] = make_uint4(s.high[0], s.high[1], s.high[2], s.high[3]), made[k * 256 + 64] = make_uint4(s.high[4], s.high[5], s.high[6], s.high[7]);
+          made[k * 256 + 128] = make_uint4(s.low[0], s.low[1], s.low[2], s.low[3]), made[k * 256 + 192] = make_uint4(s.low[4], s.low[5], s.low[6], s.low[7]);
+          made_scales[k * 64] = s.scales;
         } else {
 #pragma unroll
-          for (int n = 0; n < 8; ++n) qh[k][n] = (int)high[n], ql[k][n] = (int)low[n];
-          qs[k / 2] |= scales << (16 * (k & 1));
+          for (int n = 0; n < 8; ++n) qh[e][n] = (int)s.high[n], ql[e][n] = (int)s.low[n];
+          qs[e / 2] |= s.scales << (16 * (e & 1));
         }
       }
       if constexpr (TG > 1) {
@@ -434,8 +851,8 @@ __global__ __launch_bounds__(256, (Attend<WK, WV, kApart, RG>::kWaves)) void att
         for (int k = 0; k < KS; ++k) {
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            const uint4 u = made[k * 256 + 64 * j], v = made[k * 256 + 128 + 64 * j];
-            qh[k][4 * j] = (int)u.x, qh[k][4 * j + 1] = (int)u.y, qh[k][4 * j + 2] = (int)u.z, qh[k][4 * j + 3] = (int)u.w;
+            const uint4 w = made[k * 256 + 64 * j], v = made[k * 256 + 128 + 64 * j];
+            qh[k][4 * j] = (int)w.x, qh[k][4 * j + 1] = (int)w.y, qh[k][4 * j + 2] = (int)w.z, qh[k][4 * j + 3] = (int)w.w;
             ql[k][4 * j] = (int)v.x, ql[k][4 * j + 1] = (int)v.y, ql[k][4 * j + 2] = (int)v.z, ql[k][4 * j + 3] = (int)v.w;
           }
           qs[k / 2] |= made_scales[k * 64] << (16 * (k & 1));
@@ -448,20 +865,25 @@ __global__ __launch_bounds__(256, (Attend<WK, WV, kApart, RG>::kWaves)) void att
       }
     }
 
+    float m = kLowest, l = 0.f;   // the maximum is a whole number: every rescaling is exact
+    v16f o[DB];
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int n = 0; n < 16; ++n) o[d][n] = 0.f;
 
     for (int it = it0; it < it1; ++it) {
       // -- scores --
       uint32_t bad = 0;
 #pragma unroll
-      for (int w = 0; w < (kApart ? VW : KW); ++w) {
-        const uint32_t word = kApart ? vscale[w] : kscale[w];
-        constexpr int used = (kApart ? WV : WK) / 32;
-        bad |= marks(4 * w + 4 <= used ? word : word & ((1u << 8 * (used & 3)) - 1u));
+      for (int w = 0; w < KW; ++w) {
+        constexpr int used = W / 32;
+        bad |= marks(4 * w + 4 <= used ? vscale[w] : vscale[w] & ((1u << 8 * (used & 3)) - 1u));
       }
       const bool hide = bad || !valid;   // its values count as zero; who sees a NaN token sees it in the score
       uint32_t ks[KW];
 #pragma unroll
-      for (int w = 0; w < KW; ++w) ks[w] = kApart && bad ? ~0u : kscale[w] >> (8 * half);
+      for (int w = 0; w < KW; ++w) ks[w] = bad ? ~0u : kscale[w] >> (8 * half);
       v16f sc;
 #pragma unroll
       for (int n = 0; n < 16; ++n) sc[n] = 0.f;
@@ -476,34 +898,23 @@ __global__ __launch_bounds__(256, (Attend<WK, WV, kApart, RG>::kWaves)) void att
         }
       }
       // -- values to BF16 --
-      const int turn = A::kBuffers > 1 ? it & 1 : 0;
-      uint8_t* buffer = lds + turn * (TG * A::kTile);
+      uint8_t* buffer = lds + (A::kBuffers > 1 ? (it & 1) * (TG * A::kTile) : 0);
 #pragma unroll
       for (int k = 0; k < VO; ++k) {
         const int piece = k * RG + rg;   // columns [64 piece, + 64), the lane's half of them
-        if (VO * RG > VS && piece >= VS) break;
-        uint4 w;
-        uint32_t word;
-        if constexpr (kApart) {
-          w = vreg[k];
-          word = VW == 1 ? vscale[0] : vscale[piece / 2];
-        } else {
-          w = kreg[k * RG], word = kscale[k * RG / 2];
-#pragma unroll
-          for (int r = 1; r < RG; ++r)
-            if (rg == r) w = kreg[k * RG + r], word = kscale[(k * RG + r) / 2];
-        }
+        if (VO * RG > KS && piece >= KS) break;
+        const uint32_t word = KW == 1 || piece < 2 ? vscale[0] : vscale[KW - 1];
         const uint32_t e = word >> (8 * half + 16 * (piece & 1)) & 255u;
         const float scale = mx::u2f((hide ? 127u : e) << 23);
-        const uint32_t u[4] = {hide ? 0u : w.x, hide ? 0u : w.y, hide ? 0u : w.z, hide ? 0u : w.w};
+        const uint32_t c[4] = {hide ? 0u : vreg[k].x, hide ? 0u : vreg[k].y, hide ? 0u : vreg[k].z, hide ? 0u : vreg[k].w};
 #pragma unroll
         for (int n = 0; n < 4; ++n) {
           uint4 v;
-          v.x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(u[n], scale, 0));
-          v.y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(u[n], scale, 1));
-          v.z = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(u[n], scale, 2));
-          v.w = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(u[n], scale, 3));
-          *(uint4*)(buffer + tg * A::kTile + put[n] + 128 * piece) = v;
+          v.x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c[n], scale, 0));
+          v.y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c[n], scale, 1));
+          v.z = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c[n], scale, 2));
+          v.w = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c[n], scale, 3));
+          *(uint4*)(buffer + put[n] + 128 * piece) = v;
         }
       }
       const uint32_t shown = (uint32_t)__ballot(valid);
@@ -515,7 +926,7 @@ __global__ __launch_bounds__(256, (Attend<WK, WV, kApart, RG>::kWaves)) void att
 #pragma unroll
         for (int n = 0; n < 16; ++n) {
           const int t = 8 * (n / 4) + 4 * half + (n & 3);
-          if (!(shown >> t & 1) || first + t < row_lo || first + t >= row_hi) sc[n] = -INFINITY;
+          sc[n] = (shown >> t & 1) && first + t >= row_lo && first + t < row_hi ? sc[n] : -INFINITY;
         }
       }
       float top = fmaxf(sc[0], sc[1]);
@@ -523,80 +934,46 @@ __global__ __launch_bounds__(256, (Attend<WK, WV, kApart, RG>::kWaves)) void att
       for (int n = 2; n < 16; ++n) top = fmaxf(top, sc[n]);
       top = other_half_max(top) * a.c;
       // the maximum stays until it is 2^8 too low: probabilities up to 2^8 lose nothing
-      float own = top > m + 8.f ? ceilf(top) : m;
-      auto rescale = [&](float next) {
-        const float by = power(m, next);
-        m = next, l *= by;
+      const float own = top > m + 8.f ? ceilf(top) : m;
+      if (__any(own != m)) {
+        const float by = power(m, own);
+        m = own, l *= by;
 #pragma unroll
-        for (int d = 0; d < DB; ++d) {
+        for (int d = 0; d < DB; ++d)
 #pragma unroll
           for (int n = 0; n < 16; ++n) o[d][n] *= by;
-        }
-      };
-      if constexpr (!kSplit)
-        if (__any(own != m)) rescale(own);
+      }
       uint32_t p[8];
-      float sum = 0.f;
 #pragma unroll
       for (int n = 0; n < 8; ++n) {
-        const float p0_ = __builtin_amdgcn_exp2f(fmaf(sc[2 * n], a.c, -own)), p1_ = __builtin_amdgcn_exp2f(fmaf(sc[2 * n + 1], a.c, -own));
-        sum += p0_ + p1_;
-        p[n] = mxd::bf16_pair(p0_, p1_);
+        const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[2 * n], a.c, -m)), p1 = __builtin_amdgcn_exp2f(fmaf(sc[2 * n + 1], a.c, -m));
+        l += p0 + p1;
+        p[n] = mxd::bf16_pair(p0, p1);
       }
-      if constexpr (kSplit) {
-        uint4* to = (uint4*)(exchange + ((it & 1) * 4 + wave) * 2048) + lane;
-        to[0] = make_uint4(p[0], p[1], p[2], p[3]), to[64] = make_uint4(p[4], p[5], p[6], p[7]);
-        if (half == 0) tops[it & 1][wave][col] = own;
-      } else {
-        l += sum;
-      }
-      if (RG > 1 || kSplit) mxd::lds_barrier();
-      if constexpr (kSplit) {
-        float next = own;
-#pragma unroll
-        for (int t = 1; t < TG; ++t) next = fmaxf(next, tops[it & 1][(tg + t) % TG * RG + rg][col]);
-        if (__any(next != m)) rescale(next);
-        l += sum * power(own, next);
-      }
+      if (RG > 1) mxd::lds_barrier();
       // -- O^T += V^T P^T --
 #pragma unroll
-      for (int t = 0; t < (kSplit ? TG : 1); ++t) {
-        if constexpr (kSplit) {
-          const uint4* from = (const uint4*)(exchange + ((it & 1) * 4 + t * RG + rg) * 2048) + lane;
-          const uint4 p0_ = from[0], p1_ = from[64];
-          p[0] = p0_.x, p[1] = p0_.y, p[2] = p0_.z, p[3] = p0_.w, p[4] = p1_.x, p[5] = p1_.y, p[6] = p1_.z, p[7] = p1_.w;
-          const float theirs = tops[it & 1][t * RG + rg][col];
-          if (__any(theirs != m)) {   // whole powers of two: exact
-            const float by = power(theirs, m);
+      for (int k = 0; k < 2; ++k) {
+        const v8b pv = __builtin_bit_cast(v8b, make_uint4(p[4 * k], p[4 * k + 1], p[4 * k + 2], p[4 * k + 3]));
 #pragma unroll
-            for (int n = 0; n < 8; ++n) p[n] = mxd::bf16_pair(mx::u2f(p[n] << 16) * by, mx::u2f(p[n] & 0xFFFF0000u) * by);
-          }
-        }
-        const uint8_t* from = buffer + (kSplit ? t : tg) * A::kTile + (kSplit ? tg * (DB * 64) : 0);
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const v8b pv = __builtin_bit_cast(v8b, make_uint4(p[4 * k], p[4 * k + 1], p[4 * k + 2], p[4 * k + 3]));
-#pragma unroll
-          for (int d = 0; d < DB; ++d) {
-            const uint8_t* at = from + (d & 1 ? get1 : get0) + 128 * (d / 2) + 16 * k * (2 * WV);
-            typedef __attribute__((address_space(3))) v4s lds_v4s;
-            v4s w[2];
-            w[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)at);
-            w[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(at + 8 * (2 * WV)));
-            const v8b vv = __builtin_bit_cast(v8b, w);
-            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vv, pv, o[d], 0, 0, 0);
-          }
+        for (int d = 0; d < DB; ++d) {
+          const uint8_t* at = buffer + (d & 1 ? get1 : get0) + 128 * (d / 2) + 16 * k * (2 * W);
+          typedef __attribute__((address_space(3))) v4s lds_v4s;
+          v4s w[2];
+          w[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)at);
+          w[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(at + 8 * (2 * W)));
+          const v8b vv = __builtin_bit_cast(v8b, w);
+          o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vv, pv, o[d], 0, 0, 0);
         }
       }
-      if (kSplit && A::kBuffers == 1) mxd::lds_barrier();
     }
 
     // -- the token groups' sums together, and out --
     l = halves_sum(l);
     if (half == 0) stats[wave][col][0] = m, stats[wave][col][1] = l;
     __syncthreads();   // and everybody has read its values
-    const bool alone = x == unit0 && unit1 <= end;
-    const int64_t slot = 2 * g + (g * per < unit0 ? 1 : 0);
+    const bool alone = x == u.unit0 && u.unit1 <= end;
+    const int64_t slot = 2 * g + (g * per < u.unit0 ? 1 : 0);
     float most = kLowest, all_l = 0.f;
 #pragma unroll
     for (int t = 0; t < TG; ++t) most = fmaxf(most, stats[t * RG + rg][col][0]);
@@ -608,12 +985,12 @@ __global__ __launch_bounds__(256, (Attend<WK, WV, kApart, RG>::kWaves)) void att
       if (row0 + col < rows) {
         if (alone) {
           const int head = h * a.group + row % a.group;
-          const int64_t token = s.first + i;
+          const int64_t token = u.s.first + i;
           const RowOut f = row_out(a, head, most, all_l);
-          to = {token * a.q.out_stride + (int64_t)head * WV, f.inv};
+          to = {token * a.q.out_stride + (int64_t)head * W, f.inv};
           if (a.q.lse) a.q.lse[token * a.q.heads + head] = f.lse;
         } else {
-          to.at = (slot * A::kRows + r) * WV;
+          to.at = (slot * A::kRows + r) * W;
           ((float2*)(a.space + a.at.stats))[slot * A::kRows + r] = make_float2(most, all_l);
         }
       }
@@ -645,14 +1022,13 @@ __global__ __launch_bounds__(256, (Attend<WK, WV, kApart, RG>::kWaves)) void att
               make_float4(v[4 * n] * by, v[4 * n + 1] * by, v[4 * n + 2] * by, v[4 * n + 3] * by);
         }
       constexpr int L = CB / 4;   // lanes a row
-      if constexpr (kSplit || TG == 1) {
+      if constexpr (TG == 1) {
         const int c = lane % L * 4;
 #pragma unroll 4
-        for (int r = lane / L; r < 32; r += 64 / L)
-          put_out(rg * 32 + r, (kSplit ? tg * DB * 32 : 0) + d0 * 32 + c, *(const float4*)(own_out + r * (CB + 4) + c));
+        for (int r = lane / L; r < 32; r += 64 / L) put_out(rg * 32 + r, d0 * 32 + c, *(const float4*)(own_out + r * (CB + 4) + c));
       } else {
         __syncthreads();
-#pragma unroll 1
+#pragma unroll 2
         for (int e = tid; e < A::kRows * L; e += 256) {
           const int r = e / L, c = e % L * 4;
           float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -666,50 +1042,81 @@ __global__ __launch_bounds__(256, (Attend<WK, WV, kApart, RG>::kWaves)) void att
         __syncthreads();
       }
     }
-    __syncthreads();
-    if (tid == 0 && unit1 >= end) {   // the workgroup's last: it joins the unit if it began it and does not end it
-      Shared v{b, h, tile, 0};
-      if (!alone && x == unit0) v.parts = (int)((unit1 - 1) / per - g + 1);
-      v.slot = (int)(slot & 1);
-      *shared = v;
+    if (u.unit1 >= end) {   // the workgroup's last: it joins the unit if it began it and does not end it
+      if (tid == 0) {
+        Shared v{u.b, h, u.tile, 0, (int)(slot & 1)};
+        if (!alone && x == u.unit0) v.parts = (int)((u.unit1 - 1) / per - g + 1);
+        *shared = v;
+      }
+      return;
     }
-    x = min(unit1, end);
+    x = u.unit1;
+    next_unit(a, u, A::kRows, A::kStep);
   }
 }
 
-// A unit that several workgroups had, four columns a thread: blockIdx.x the workgroup that began it.
-template <int WV>
-__global__ __launch_bounds__(256) void join_kernel(AttendArgs a, int tile_rows) {
-  const Shared s = ((const Shared*)(a.space + a.at.units))[blockIdx.x];
-  if (s.parts < 2) return;
-  const int e = blockIdx.y * 256 + threadIdx.x, r = e / (WV / 4), c = e % (WV / 4) * 4;
-  const Sequence q = sequence(a, s.b);
-  const int row = s.tile * tile_rows + r;
-  if (row >= q.n * a.group) return;
-  const float2* stats = (const float2*)(a.space + a.at.stats);
-  const float* parts = (const float*)(a.space + a.at.rows);
-  // the others' first pieces of work
+// The parts of four values of a row: the first workgroup's lies in slot 2 g + slot, the others' in their first.
+struct Joined {
+  float4 v;
+  float most, sum;
+};
+template <typename Part>
+__device__ __forceinline__ Joined join_parts(const AttendArgs& a, const Shared& s, int tile_rows, int r, Part part) {
+  const float2* stats = (const float2*)(a.space + a.at.stats) + r;
   auto slot = [&](int i) { return (int64_t)2 * (blockIdx.x + i) + (i ? 0 : s.slot); };
-  float most = kLowest;
+  Joined j{make_float4(0.f, 0.f, 0.f, 0.f), kLowest, 0.f};
 #pragma unroll 8
-  for (int i = 0; i < s.parts; ++i) most = fmaxf(most, stats[slot(i) * tile_rows + r].x);
-  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-  float sum = 0.f;
+  for (int i = 0; i < s.parts; ++i) j.most = fmaxf(j.most, stats[slot(i) * tile_rows].x);
 #pragma unroll 8
   for (int i = 0; i < s.parts; ++i) {
-    const float2 st = stats[slot(i) * tile_rows + r];
-    const float4 p = *(const float4*)(parts + (slot(i) * tile_rows + r) * WV + c);
-    const float by = power(st.x, most);
-    sum += st.y * by;
-    v.x += p.x * by, v.y += p.y * by, v.z += p.z * by, v.w += p.w * by;
+    const float2 st = stats[slot(i) * tile_rows];
+    const float4 p = part(slot(i));
+    const float by = power(st.x, j.most);
+    j.sum += st.y * by;
+    j.v.x += p.x * by, j.v.y += p.y * by, j.v.z += p.z * by, j.v.w += p.w * by;
   }
+  return j;
+}
+
+__device__ __forceinline__ void put_joined(const AttendArgs& a, const Shared& s, const Sequence& q, int row, int c, int width, const Joined& j) {
   const int head = s.h * a.group + row % a.group;
   const int64_t token = q.first + row / a.group;
-  const RowOut f = row_out(a, head, most, sum);
+  const RowOut f = row_out(a, head, j.most, j.sum);
   uint2 w;
-  w.x = mxd::bf16_pair(v.x * f.inv, v.y * f.inv), w.y = mxd::bf16_pair(v.z * f.inv, v.w * f.inv);
-  *(uint2*)(a.q.out + token * a.q.out_stride + (int64_t)head * WV + c) = w;
+  w.x = mxd::bf16_pair(j.v.x * f.inv, j.v.y * f.inv), w.y = mxd::bf16_pair(j.v.z * f.inv, j.v.w * f.inv);
+  *(uint2*)(a.q.out + token * a.q.out_stride + (int64_t)head * width + c) = w;
   if (a.q.lse && c == 0) a.q.lse[token * a.q.heads + head] = f.lse;
+}
+
+// A unit of latents that several workgroups had, four values a thread: blockIdx.x the workgroup that began it.
+template <int RG>
+__global__ __launch_bounds__(256) void join_latent_kernel(AttendArgs a) {
+  using A = Latent<512, RG>;
+  const Shared s = ((const Shared*)(a.space + a.at.units))[blockIdx.x];
+  if (s.parts < 2) return;
+  const int e = blockIdx.y * 256 + threadIdx.x, lane = e & 63, n = e >> 6 & 3, d = e >> 8 & (A::DB - 1), wave = e / (256 * A::DB);
+  const int rg = wave % RG, cg = wave / RG, r = rg * 32 + (lane & 31), c = cg * (A::DB * 32) + 32 * d + 8 * n + 4 * (lane >> 5);
+  const Sequence q = sequence(a, s.b);
+  const int row = s.tile * A::kRows + r;
+  if (row >= q.n * a.group) return;
+  const float4* parts = (const float4*)(a.space + a.at.rows) + e;
+  const Joined j = join_parts(a, s, A::kRows, r, [&](int64_t slot) { return parts[slot * (A::kRows * A::WV / 4)]; });
+  put_joined(a, s, q, row, c, A::WV, j);
+}
+
+// A unit that several workgroups had, four values a thread: blockIdx.x the workgroup that began it.
+template <int W, int RG>
+__global__ __launch_bounds__(256) void join_grouped_kernel(AttendArgs a) {
+  using A = Grouped<W, RG>;
+  const Shared s = ((const Shared*)(a.space + a.at.units))[blockIdx.x];
+  if (s.parts < 2) return;
+  const int e = blockIdx.y * 256 + threadIdx.x, r = e / (W / 4), c = e % (W / 4) * 4;
+  const Sequence q = sequence(a, s.b);
+  const int row = s.tile * A::kRows + r;
+  if (row >= q.n * a.group) return;
+  const float4* parts = (const float4*)(a.space + a.at.rows) + e;
+  const Joined j = join_parts(a, s, A::kRows, r, [&](int64_t slot) { return parts[slot * (A::kRows * W / 4)]; });
+  put_joined(a, s, q, row, c, W, j);
 }
 
 int check_attend(const char* who, const mx_kv4* c, int32_t heads, int32_t tokens, int32_t batch) {
@@ -721,24 +1128,13 @@ int check_attend(const char* who, const mx_kv4* c, int32_t heads, int32_t tokens
   return MX_OK;
 }
 
-// fn(WK, WV, apart) of a checked cache.
-template <typename F>
-auto by_widths(const mx_kv4* c, F fn) {
-  using std::integral_constant;
-  if (c->width == 512) return fn(integral_constant<int, 512>(), integral_constant<int, 512>(), std::false_type());
-  if (c->width == 576) return fn(integral_constant<int, 576>(), integral_constant<int, 512>(), std::false_type());
-  if (c->width == 64) return fn(integral_constant<int, 64>(), integral_constant<int, 64>(), std::true_type());
-  if (c->width == 128) return fn(integral_constant<int, 128>(), integral_constant<int, 128>(), std::true_type());
-  return fn(integral_constant<int, 256>(), integral_constant<int, 256>(), std::true_type());
-}
-
-int workgroups(int value_width) { return kCus * waves(value_width); }
+int workgroups(const mx_kv4* c) { return kCus * (c->v_codes ? waves(c->width) : 1); }
 
 // Row tiles of all sequences at most: each sequence's last one may be partly full.
 int64_t most_tiles(int64_t rows, int batch, int tile_rows) { return rows / tile_rows + batch; }
 
 Space space_of(const mx_kv4* c, int group, int tokens, int batch, int tile_rows) {
-  const int64_t n = workgroups(c->value_width), tiles = most_tiles((int64_t)tokens * group, batch, tile_rows);
+  const int64_t n = workgroups(c), tiles = most_tiles((int64_t)tokens * group, batch, tile_rows);
   auto up = [](int64_t v) { return (v + 255) / 256 * 256; };
   Space s;
   s.units = 0;
@@ -806,20 +1202,37 @@ int mx_kv4_attend(mx_ctx* ctx, const mx_kv4* cache, const mx_kv4_query* query, v
     hipLaunchKernelGGL(plan_kernel, dim3(1), dim3(1024), 0, st, a, tile_rows, step);
     MX_LAUNCH_CHECK("plan_kernel");
   }
-  return by_widths(cache, [&](auto wk, auto wv, auto apart) {
-    constexpr int WK = decltype(wk)::value, WV = decltype(wv)::value;
-    constexpr bool kApart = decltype(apart)::value;
-    const int n = workgroups(WV);
-    const dim3 grid(n), threads(256);
-    if (rg == 1) hipLaunchKernelGGL((attend_kernel<WK, WV, kApart, 1>), grid, threads, 0, st, a, (int)inline_plan);
-    else if (rg == 2) hipLaunchKernelGGL((attend_kernel<WK, WV, kApart, 2>), grid, threads, 0, st, a, (int)inline_plan);
-    if constexpr (kApart)
-      if (rg == 4) hipLaunchKernelGGL((attend_kernel<WK, WV, kApart, 4>), grid, threads, 0, st, a, (int)inline_plan);
-    MX_LAUNCH_CHECK("attend_kernel");
-    hipLaunchKernelGGL(join_kernel<WV>, dim3(n, tile_rows * WV / 1024), threads, 0, st, a, tile_rows);
-    MX_LAUNCH_CHECK("join_kernel");
+  const int n = workgroups(cache);
+  auto latent = [&](auto wk, auto groups) {
+    constexpr int WK = decltype(wk)::value, RG = decltype(groups)::value;
+    hipLaunchKernelGGL((latent_kernel<WK, RG>), dim3(n), dim3(512), 0, st, a, (int)inline_plan);
+    MX_LAUNCH_CHECK("latent_kernel");
+    hipLaunchKernelGGL(join_latent_kernel<RG>, dim3(n, 16 * RG), dim3(256), 0, st, a);
+    MX_LAUNCH_CHECK("join_latent_kernel");
     return MX_OK;
-  });
+  };
+  auto grouped = [&](auto w, auto groups) {
+    constexpr int W = decltype(w)::value, RG = decltype(groups)::value;
+    hipLaunchKernelGGL((grouped_kernel<W, RG>), dim3(n), dim3(256), 0, st, a, (int)inline_plan);
+    MX_LAUNCH_CHECK("grouped_kernel");
+    hipLaunchKernelGGL((join_grouped_kernel<W, RG>), dim3(n, RG * W / 32), dim3(256), 0, st, a);
+    MX_LAUNCH_CHECK("join_grouped_kernel");
+    return MX_OK;
+  };
+  using std::integral_constant;
+  auto by_rows = [&](auto launch, auto w) {
+    if (rg == 1) return launch(w, integral_constant<int, 1>());
+    if (rg == 2) return launch(w, integral_constant<int, 2>());
+    return launch(w, integral_constant<int, 4>());
+  };
+  auto two = [&](auto w) { return rg == 1 ? latent(w, integral_constant<int, 1>()) : latent(w, integral_constant<int, 2>()); };
+  switch (cache->width) {
+    case 64: return by_rows(grouped, integral_constant<int, 64>());
+    case 128: return by_rows(grouped, integral_constant<int, 128>());
+    case 256: return by_rows(grouped, integral_constant<int, 256>());
+    case 512: return two(integral_constant<int, 512>());
+    default: return two(integral_constant<int, 576>());
+  }
 }
 
 }  // extern "C"
