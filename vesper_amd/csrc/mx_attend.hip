@@ -58,6 +58,10 @@ struct Shared {
   int32_t b, h, tile, parts, slot;
 };
 
+// (the library's minimum and maximum of 64-bit integers go through doubles)
+__device__ __forceinline__ int64_t lesser(int64_t a, int64_t b) { return a < b ? a : b; }
+__device__ __forceinline__ int64_t larger(int64_t a, int64_t b) { return a > b ? a : b; }
+
 struct Sequence {
   int first, n;        // query rows in tokens
   int held;            // cached tokens
@@ -74,15 +78,15 @@ __device__ __forceinline__ Sequence sequence(const AttendArgs& a, int b) {
   }
   const int length = a.q.lengths[b];
   s.end = length;
-  s.held = (int)min<int64_t>(max(length, 0), (int64_t)a.q.columns << a.page_shift);
+  s.held = (int)lesser(max(length, 0), (int64_t)a.q.columns << a.page_shift);
   return s;
 }
 
 // The tokens that query token i of the sequence sees.
 __device__ __forceinline__ void seen(const AttendArgs& a, const Sequence& s, int i, int& lo, int& hi) {
   const int64_t end = s.end - s.n + i + 1;
-  hi = (int)min<int64_t>(max<int64_t>(end, 0), s.held);
-  lo = a.q.window ? (int)min<int64_t>(max<int64_t>(end - a.q.window, 0), hi) : 0;
+  hi = (int)lesser(larger(end, 0), s.held);
+  lo = a.q.window ? (int)lesser(larger(end - a.q.window, 0), hi) : 0;
 }
 
 // Tokens [lo, hi) that some row of row tile `tile` sees (lo at a whole step), and its iterations of `step` tokens: one at
@@ -91,7 +95,7 @@ __device__ __forceinline__ int tile_iterations(const AttendArgs& a, const Sequen
   const int64_t row0 = (int64_t)tile * rows, all = (int64_t)s.n * a.group;
   int l1, h0;
   seen(a, s, (int)(row0 / a.group), lo, h0);
-  seen(a, s, (int)((min<int64_t>(row0 + rows, all) - 1) / a.group), l1, hi);
+  seen(a, s, (int)((lesser(row0 + rows, all) - 1) / a.group), l1, hi);
   lo &= ~31;
   return max(1, (hi - lo + step - 1) / step);
 }
@@ -150,10 +154,10 @@ __device__ __forceinline__ void make_plan(const AttendArgs& a, Plan p, uint32_t*
       if (b < a.q.batch) n = (uint32_t)(((int64_t)sequence(a, b).n * a.group + rows - 1) / rows);
       const int64_t before = scan<N>(n, sums, all);
       // (no more than there is room for: a q_first that does not ascend could name more rows than there are)
-      if (b < a.q.batch) p.base[b] = (int)min<int64_t>(tiles + before, a.tiles);
+      if (b < a.q.batch) p.base[b] = (int)lesser(tiles + before, a.tiles);
       tiles += all;
     }
-    tiles = min<int64_t>(tiles, a.tiles);
+    tiles = lesser(tiles, a.tiles);
     if (threadIdx.x == 0) p.base[a.q.batch] = (int)tiles;
     __syncthreads();
   }
@@ -308,8 +312,9 @@ __device__ __forceinline__ float halves_sum(float v) {
   return __int_as_float(p[0]) + __int_as_float(p[1]);
 }
 
-// 64 query values of a row from column c on as the right operand of a step: the lane's 2 x 16 (half: which of each 32) in two
-// terms, and their scale bytes.
+// Query values of a step as the right operand of the scores' products: a lane's 2 x 16 in two terms, and their scale bytes.
+// 32x32x64: the lane's row is lane % 32, the 16s from 16 half and 32 + 16 half on; 16x16x128: lane % 16, from 16 quad and
+// 64 + 16 quad on. A lane gives the scales of block half (quad) of 32, not those of the values it holds.
 struct QueryStep {
   uint32_t high[8], low[8], scales;
 };
@@ -317,34 +322,63 @@ struct QueryWords {
   uint32_t w[2][8];
 };
 
-__device__ __forceinline__ QueryWords query_words(const uint16_t* q, int c, int half) {
+template <int kApart = 64>
+__device__ __forceinline__ QueryWords query_words(const uint16_t* q, bool first_only = false) {
   QueryWords r;
 #pragma unroll
   for (int e = 0; e < 2; ++e)
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      const uint4 v = mxd::ldg128((const uint8_t*)(q + c + 32 * e + 16 * half + 8 * j));
+      uint4 v = make_uint4(0u, 0u, 0u, 0u);
+      if (e == 0 || !first_only) v = mxd::ldg128((const uint8_t*)(q + kApart * e + 8 * j));
       r.w[e][4 * j] = v.x, r.w[e][4 * j + 1] = v.y, r.w[e][4 * j + 2] = v.z, r.w[e][4 * j + 3] = v.w;
     }
   return r;
 }
+
+__device__ __forceinline__ uint32_t largest(const uint32_t (&w)[8]) {
+  uint32_t top = w[0] & 0x7FFF7FFFu;
+#pragma unroll
+  for (int j = 1; j < 8; ++j) top = pair_max(top, w[j] & 0x7FFF7FFFu);
+  return max(top & 0xFFFFu, top >> 16);
+}
+__device__ __forceinline__ uint32_t scale_bytes(uint32_t e) { return e | (e == 255u ? 255u : e - 4u) << 8; }
 
 __device__ __forceinline__ QueryStep query_step(const QueryWords& q, int half) {
   QueryStep r;
   uint32_t e[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    uint32_t top = q.w[i][0] & 0x7FFF7FFFu;
-#pragma unroll
-    for (int j = 1; j < 8; ++j) top = pair_max(top, q.w[i][j] & 0x7FFF7FFFu);
-    top = max(top & 0xFFFFu, top >> 16);
+    const uint32_t top = largest(q.w[i]);
     const auto both = __builtin_amdgcn_permlane32_swap(top, top, false, false);
     e[i] = query_exponent(max((uint32_t)both[0], (uint32_t)both[1]));
     split16(q.w[i], min(e[i], 247u), r.high + 4 * i, r.low + 4 * i);
   }
-  const uint32_t own = half ? e[1] : e[0];
-  r.scales = own | (own == 255u ? 255u : own - 4u) << 8;
+  r.scales = scale_bytes(half ? e[1] : e[0]);
   return r;
+}
+
+__device__ __forceinline__ QueryStep query_step16(const QueryWords& q, int l16, int quad) {
+  QueryStep r;
+  uint32_t e[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {   // blocks quad / 2 and 2 + quad / 2, halved between quads
+    const uint32_t top = largest(q.w[i]);
+    const auto both = __builtin_amdgcn_permlane16_swap(top, top, false, false);
+    e[i] = query_exponent(max((uint32_t)both[0], (uint32_t)both[1]));
+    split16(q.w[i], min(e[i], 247u), r.high + 4 * i, r.low + 4 * i);
+  }
+  const int from = (quad & 1) * 32 + l16;   // a lane of block `quad`
+  const uint32_t e0 = (uint32_t)__shfl((int)e[0], from, 64), e1 = (uint32_t)__shfl((int)e[1], from, 64);
+  r.scales = scale_bytes(quad < 2 ? e0 : e1);
+  return r;
+}
+
+// 16 bytes at any multiple of 4.
+__device__ __forceinline__ uint4 words4(const uint8_t* p) {
+  typedef mxd::u32x4_t words __attribute__((aligned(4)));
+  const words v = *(const __attribute__((address_space(1))) words*)p;
+  return make_uint4(v.x, v.y, v.z, v.w);
 }
 
 // Where a row of a unit goes (in values; -1: nowhere), and its factor.
@@ -365,40 +399,74 @@ __device__ __forceinline__ float power(float from, float to) {   // 2^(from - to
   return from == to ? 1.f : __builtin_amdgcn_exp2f(from - to);
 }
 
-// Latents. 64 (or 32) rows of 512 columns with their queries are 64 (32) + 66 registers of each of the workgroup's eight
-// waves, two a SIMD: with one, of 512 registers, every other instruction slot stays empty (7.5 clocks an instruction).
-//
-// A step is TG tiles of 32 tokens. The waves of a row group and tile split the width: each scores its half, they exchange
-// half of the sums, and each goes on with 16 of the tile's tokens. Wave kh takes its tokens rotated by 16, so that what it
-// keeps is in the first registers. For the values each wave has WV RG / 8 columns of all of the step's tokens.
+// Latents. A step is 64 tokens, for 64 (RG = 2) or 32 rows, of eight waves, two a SIMD:
+//   four score waves: 16 rows and 64 (32) tokens each, by V_MFMA_SCALE_F32_16X16X128_F8F6F4 with the rows' queries in 64
+//     registers; then the softmax of these, and the probabilities to LDS;
+//   four value waves: 128 columns and all rows each. Each converts its columns of the step's tokens into an LDS tile of its
+//     own, between the products of the last step's values with the last step's probabilities.
+// So the matrix units have a score wave's and a value wave's products to choose from, and each wave's other instructions go
+// on under the other's products; one barrier a step. Codes and scales come to LDS by copies that nobody waits for, kStages -
+// 1 steps ahead, once for all waves.
 template <int WK, int RG>
 struct Latent {
-  static constexpr int WV = 512, TG = 4 / RG, kRows = 32 * RG, kStep = 32 * TG, CG = 8 / RG;
-  static constexpr int KS = WK / 64, KH = (KS + 1) / 2;    // 64-column steps of a key, and of a wave: kh's 4 and the last
-  static constexpr int DB = WV / 32 / CG;                  // 32-column blocks of a wave
-  static constexpr int VO = 4 / RG;                        // 64-column pieces of the values that a wave converts
-  static constexpr int kTile = 64 * WV;                    // bytes of 32 tokens' values in BF16
-  static constexpr int kBuffers = RG > 1 ? 2 : 1;
-  static constexpr int kValues = kBuffers * TG * kTile;
-  static constexpr int kSums = 8 * 2048, kWeights = 8 * 1024;   // what waves exchange: half sums, probabilities
+  static constexpr int WV = 512, RQ = 2 * RG, TT = 4 / RQ, T2 = 4 / TT, kRows = 32 * RG, kStep = 64;
+  static constexpr bool kPart = WK % 128 != 0;             // a last step of 64 columns of the keys
+  static constexpr int KS = (WK + 127) / 128;
+  static constexpr int kStages = kPart ? 3 : 4;
+  // LDS: the values' tiles [4 waves][64 tokens][128 columns], the step's probabilities by 16 tokens, twice, and the stages:
+  // codes [64][256 B], scales [64][16 B], and of a last step codes [64][32 B] and scales [64][4 B]
+  static constexpr int kTile = 64 * 256, kValues = 4 * kTile;
+  static constexpr int kWeights = 4 * kRows * 32;
+  static constexpr int kScales = 64 * 256, kTail = kScales + 64 * 16, kTailScales = kTail + 64 * 32;
+  static constexpr int kStage = kPart ? kTailScales + 64 * 4 : kTail;
+  static constexpr int kRing = kValues + 2 * kWeights, kLds = kRing + kStages * kStage;
+  static constexpr int kCopies = kPart ? 7 : 5;            // of a value wave and step
+  // the queries' exchange, over the tiles and probabilities
+  static constexpr int kMade = 4 * 256 + (kPart ? 128 : 0);
+  static_assert(RQ * (kMade * 16 + KS * 256) <= kRing, "the queries lie before the stages");
+  static_assert(8 * (kInlineTiles + 1) + 4 * (kInlineTiles + 2) <= kRing, "and so does the plan");
   static constexpr int CB = 64, kOut = 32 * (CB + 4) * 4;  // columns that go out at a time, and a wave's bytes of them
+  static_assert(4 * kOut <= kRing, "and what goes out");
 };
+
+template <int kA, int kB>
+__device__ __forceinline__ mxd::v4f scores16(uint4 k, const v8i& q, mxd::v4f c, uint32_t ks, uint32_t qs) {
+  const v8i av = {(int)k.x, (int)k.y, (int)k.z, (int)k.w, 0, 0, 0, 0};
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av, q, c, 4, 0, kA, (int)ks, kB, (int)qs);
+}
+// Step K of the scores, both terms.
+template <int K>
+__device__ __forceinline__ mxd::v4f score_step(uint4 k, const v8i& high, const v8i& low, mxd::v4f c, uint32_t ks, uint32_t qs) {
+  c = scores16<K & 3, 2 * (K & 1)>(k, high, c, ks, qs);
+  return scores16<K & 3, 2 * (K & 1) + 1>(k, low, c, ks, qs);
+}
+
+// Over the four lanes of a row (lane % 16).
+__device__ __forceinline__ float row_max4(float v) {
+  const auto p = __builtin_amdgcn_permlane16_swap(__float_as_int(v), __float_as_int(v), false, false);
+  return other_half_max(fmaxf(__int_as_float(p[0]), __int_as_float(p[1])));
+}
+__device__ __forceinline__ float row_sum4(float v) {
+  const auto p = __builtin_amdgcn_permlane16_swap(__float_as_int(v), __float_as_int(v), false, false);
+  return halves_sum(__int_as_float(p[0]) + __int_as_float(p[1]));
+}
 
 template <int WK, int RG>
 __global__ __launch_bounds__(512, 2) void latent_kernel(AttendArgs a, int inline_plan) {
   using A = Latent<WK, RG>;
-  constexpr int WV = A::WV, TG = A::TG, CG = A::CG, KS = A::KS, KH = A::KH, DB = A::DB, VO = A::VO, CB = A::CB;
-  __shared__ __attribute__((aligned(16))) uint8_t lds[A::kValues + A::kSums + A::kWeights];
-  __shared__ __attribute__((aligned(16))) float tops[RG][32][CG];
-  __shared__ float stats[8][32];
+  constexpr int WV = A::WV, RQ = A::RQ, TT = A::TT, T2 = A::T2, KS = A::KS, CB = A::CB;
+  constexpr bool kPart = A::kPart;
+  __shared__ __attribute__((aligned(16))) uint8_t lds[A::kLds];
+  __shared__ float tops[2][A::kRows][TT];
+  __shared__ float stats[A::kRows][TT][2];
   __shared__ Place places[A::kRows];
   __shared__ uint32_t sums[8];
   __shared__ int32_t found[2];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int rg = wave % RG, cg = wave / RG, kh = cg & 1, tile = cg >> 1;
-  const int col = lane & 31, half = lane >> 5;   // the lane's query row of the products
-  const int mine = col ^ (16 * kh);              // as a loader, its token of the tile
-  uint8_t *half_sums = lds + A::kValues, *weights = half_sums + A::kSums;
+  const int l16 = lane & 15, quad = lane >> 4, col = lane & 31, half = lane >> 5;
+  const int rq = wave % RQ, tt = wave % 4 / RQ;   // a score wave's 16 rows and tokens
+  const int cg = wave - 4;                        // a value wave's columns
+  uint8_t* weights = lds + A::kValues;
 
   Plan plan{(int32_t*)(a.space + a.at.base), (int64_t*)(a.space + a.at.prefix)};
   if (inline_plan) {
@@ -406,11 +474,11 @@ __global__ __launch_bounds__(512, 2) void latent_kernel(AttendArgs a, int inline
     make_plan<512>(a, plan, sums, A::kRows, A::kStep);
   }
   const int64_t all = uniform(plan.prefix[plan.base[a.q.batch]]) * a.cache.heads;
-  const int64_t per = max<int64_t>((all + kCus - 1) / kCus, 1);
+  const int64_t per = larger((all + kCus - 1) / kCus, 1);
   // workgroups go round the XCDs: neighbours in the work, which share keys, to one L2
   const int g = (int)(blockIdx.x % kXcds) * (kCus / kXcds) + (int)blockIdx.x / kXcds;
-  int64_t x = min(g * per, all);
-  const int64_t end = min(x + per, all);
+  int64_t x = lesser(g * per, all);
+  const int64_t end = lesser(x + per, all);
   Shared* shared = (Shared*)(a.space + a.at.units) + g;
   if (x >= end) {
     if (tid == 0) shared->parts = 0;
@@ -419,287 +487,369 @@ __global__ __launch_bounds__(512, 2) void latent_kernel(AttendArgs a, int inline
   Units u;
   first_unit<512>(a, plan, inline_plan, x, found, u, A::kRows, A::kStep);
 
-  // LDS places of the values: a loader's 16-byte pieces of its token, and a reader's 8 bytes; pieces of neighbouring tokens
-  // lie apart
-  const int spread = 2 * (mine & 3) + ((mine >> 2) & 1);
-  uint32_t put[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) put[i] = tile * A::kTile + mine * (2 * WV) + ((4 * half + i) ^ spread) * 16;
-  const int rt = (lane & 15) >> 2, rc = lane & 3, rs = 2 * rt + half;
-  const uint32_t get0 = cg * (DB * 64) + (4 * half + rt) * (2 * WV) + ((2 * ((lane >> 4) & 1) + rc / 2) ^ rs) * 16 + (rc & 1) * 8;
-  const uint32_t get1 = get0 ^ 64;
-
+  const int spread = 2 * (l16 & 3) + ((l16 >> 2) & 1);   // pieces of 16 bytes of neighbouring tokens' values lie apart
   for (;;) {
-    const int it0 = (int)(x - u.unit0), it1 = (int)(min(u.unit1, end) - u.unit0);
-    // -- the wave's query rows --
-    const int rows = u.s.n * a.group;   // at most 2^30
-    const int row0 = u.tile * A::kRows + rg * 32, row = min(row0 + col, rows - 1);
-    const int i = row / a.group;
-    int row_lo, row_hi;
-    seen(a, u.s, i, row_lo, row_hi);
-    // tokens [all_lo, all_hi) are seen by all of the wave's rows
-    int all_lo, all_hi, unused;
-    seen(a, u.s, min(row0, rows - 1) / a.group, unused, all_hi);
-    seen(a, u.s, min(row0 + 31, rows - 1) / a.group, all_lo, unused);
-    all_lo = uniform(all_lo), all_hi = uniform(all_hi);
-
-    // -- loads: the lane's token of a step, its page a step ahead --
-    const int32_t* table = a.q.table + (int64_t)u.b * a.q.columns;
+    const int it0 = (int)(x - u.unit0), it1 = (int)(lesser(u.unit1, end) - u.unit0);
     const int lo = u.lo, hi = u.hi, h = u.h;
-    auto token_of = [&](int it) { return lo + (it * TG + tile) * 32 + mine; };
-    auto page_of = [&](int it) {
-      const int t = token_of(it);
-      return it < it1 && t < hi ? table[t >> a.page_shift] : -1;
-    };
-    uint4 kreg[KH];
-    uint32_t kscale[(KH + 1) / 2];
-    bool valid = false;
-    auto load = [&](int it, int page) {
-      valid = page >= 0 && page < a.cache.pages;
-      const int64_t at = ((int64_t)(valid ? page : 0) * a.cache.heads + h << a.page_shift) + (token_of(it) & ((1 << a.page_shift) - 1));
-      const uint8_t* p = a.cache.k_codes + at * (WK / 2) + 128 * kh + 16 * half;
-      const uint8_t* ps = a.cache.k_scales + at * scale_pitch(WK) + 8 * kh;
+    const int rows = u.s.n * a.group;   // at most 2^30
+    const int row0 = u.tile * A::kRows, row = min(row0 + rq * 16 + l16, rows - 1);
+    const int i = row / a.group;
+    // -- the queries' loads: KS steps of 128 values of the wave's 16 rows, divided among their 8 / RQ waves --
+    constexpr int kSharers = 8 / RQ, kEach = (KS + kSharers - 1) / kSharers;
+    const int sharer = wave / RQ;
+    const uint16_t* q = a.q.q + (u.s.first + i) * a.q.q_stride + (int64_t)(h * a.group + row % a.group) * WK;
+    QueryWords words[kEach];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) kreg[k] = mxd::ldg128(p + 32 * k);
-      kscale[0] = mxd::ldg32(ps), kscale[1] = mxd::ldg32(ps + 4);
-      if constexpr (KS > 8) {
-        if (kh == 0) kreg[4] = mxd::ldg128(p + 256), kscale[2] = mxd::ldg32(ps + 16);
-      }
-    };
-    load(it0, page_of(it0));
-    int page_next = page_of(it0 + 1);
-
-    // -- the queries: the row group's waves convert KS / CG steps of 64 values each and exchange them --
-    v8i qh[KH], ql[KH];
-    uint32_t qs[(KH + 1) / 2] = {};
-    {
-      const uint16_t* q = a.q.q + (u.s.first + i) * a.q.q_stride + (int64_t)(h * a.group + row % a.group) * WK;
-      constexpr int kEach = (KS + CG - 1) / CG;
-      QueryWords words[kEach];
-#pragma unroll
-      for (int e = 0; e < kEach; ++e)
-        if (KS % CG == 0 || e * CG + cg < KS) words[e] = query_words(q, 64 * (e * CG + cg), half);
-      uint4* made = (uint4*)lds + rg * (KS * 256) + lane;
-      uint32_t* made_scales = (uint32_t*)(lds + RG * KS * 4096) + rg * (KS * 64) + lane;
-      __syncthreads();   // the plan, or the last unit's rows, have been read
-#pragma unroll
-      for (int e = 0; e < kEach; ++e) {
-        const int k = e * CG + cg;
-        if (KS % CG && k >= KS) break;
-        const QueryStep s = query_step(words[e], half);
-        made[k * 256] = make_uint4(s.high[0], s.high[1], s.high[2], s.high[3]), made[k * 256 + 64] = make_uint4(s.high[4], s.high[5], s.high[6], s.high[7]);
-        made[k * 256 + 128] = make_uint4(s.low[0], s.low[1], s.low[2], s.low[3]), made[k * 256 + 192] = make_uint4(s.low[4], s.low[5], s.low[6], s.low[7]);
-        made_scales[k * 64] = s.scales;
-      }
-      mxd::lds_barrier();
-#pragma unroll
-      for (int e = 0; e < KH; ++e) {
-        const int k = e < 4 ? 4 * kh + e : 8;
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const uint4 w = made[k * 256 + 64 * j], v = made[k * 256 + 128 + 64 * j];
-          qh[e][4 * j] = (int)w.x, qh[e][4 * j + 1] = (int)w.y, qh[e][4 * j + 2] = (int)w.z, qh[e][4 * j + 3] = (int)w.w;
-          ql[e][4 * j] = (int)v.x, ql[e][4 * j + 1] = (int)v.y, ql[e][4 * j + 2] = (int)v.z, ql[e][4 * j + 3] = (int)v.w;
-        }
-        qs[e / 2] |= made_scales[k * 64] << (16 * (e & 1));
-      }
-      mxd::lds_barrier();   // before the values come where they were
+    for (int e = 0; e < kEach; ++e) {
+      const int k = e * kSharers + sharer;
+      if (KS % kSharers == 0 || k < KS) words[e] = query_words(q + 128 * k + 16 * quad, kPart && k == KS - 1);
     }
-
-    float m = kLowest, l = 0.f;   // the maximum is a whole number: every rescaling is exact
-    v16f o[DB];
+    // -- pages: 16 tokens have one --
+    const __attribute__((address_space(4))) int32_t* table =
+        (const __attribute__((address_space(4))) int32_t*)(a.q.table + (int64_t)u.b * a.q.columns);
+    auto page_of = [&](int t) {   // -1: none
+      const int page = table[min(t, max(hi - 1, 0)) >> a.page_shift];
+      return t < hi && (uint32_t)page < (uint32_t)a.cache.pages ? page : -1;
+    };
+    // -- a value wave's copies of step `it`: its 16 tokens --
+    auto copy = [&](int it) {
+      const int t = lo + it * A::kStep + 16 * cg, page = max(page_of(t), 0);
+      const int64_t at = (((int64_t)page * a.cache.heads + h) << a.page_shift) + (t & ((1 << a.page_shift) - 1));
+      const uint8_t* codes = a.cache.k_codes + at * (WK / 2);
+      const uint8_t* scales = a.cache.k_scales + at * scale_pitch(WK);
+      const uint32_t stage = (uint32_t)uniform((int)(mxd::lds_addr(lds) + A::kRing + (it % A::kStages) * A::kStage));
 #pragma unroll
-    for (int d = 0; d < DB; ++d)
-#pragma unroll
-      for (int n = 0; n < 16; ++n) o[d][n] = 0.f;
-
-    for (int it = it0; it < it1; ++it) {
-      // -- scores of the wave's half of the width --
-      uint32_t ks[(KH + 1) / 2];
-#pragma unroll
-      for (int w = 0; w < (KH + 1) / 2; ++w) ks[w] = kscale[w] >> (8 * half);
-      v16f sc;
-#pragma unroll
-      for (int n = 0; n < 16; ++n) sc[n] = 0.f;
-#pragma unroll
-      for (int k = 0; k < KH; ++k) {
-        if (k == 4 && kh) break;
-        if (k & 1) {
-          sc = scores<2, 2>(kreg[k], qh[k], sc, ks[k / 2], qs[k / 2]);
-          sc = scores<2, 3>(kreg[k], ql[k], sc, ks[k / 2], qs[k / 2]);
-        } else {
-          sc = scores<0, 0>(kreg[k], qh[k], sc, ks[k / 2], qs[k / 2]);
-          sc = scores<0, 1>(kreg[k], ql[k], sc, ks[k / 2], qs[k / 2]);
-        }
+      for (int j = 0; j < 4; ++j) {   // four tokens, their pieces changed about by the token
+        const uint32_t token = 4 * j + quad, piece = l16 ^ (token & 7);
+        mxd::global_to_lds16(codes + (token * (WK / 2) + piece * 16), stage + (16 * cg + 4 * j) * 256);
       }
-      // -- values to BF16: pieces rg, rg + RG, ... of the wave's four --
-      uint8_t* buffer = lds + (A::kBuffers > 1 ? (it & 1) * (TG * A::kTile) : 0);
-      auto convert = [&] {
+      if (lane < 16) mxd::global_to_lds16(scales + lane * scale_pitch(WK), stage + A::kScales + 256 * cg);
+      if constexpr (kPart) {
+        if (lane < 32) mxd::global_to_lds16(codes + ((lane >> 1) * (WK / 2) + 256 + (lane & 1) * 16), stage + A::kTail + 512 * cg);
+        if (lane < 16) mxd::global_to_lds4(scales + lane * scale_pitch(WK) + 16, stage + A::kTailScales + 64 * cg);
+      }
+    };
+    if (wave >= 4) {
 #pragma unroll
-        for (int k = 0; k < VO; ++k) {
-          uint4 w = kreg[k * RG];
-          uint32_t word = ks[k * RG / 2] >> (16 * (k * RG & 1));
+      for (int k = 0; k < A::kStages - 1; ++k)
+        if (it0 + k < it1) copy(it0 + k);
+    }
+    // -- the queries, converted and exchanged --
+    uint4* made = (uint4*)lds + rq * A::kMade + lane;
+    uint32_t* made_scales = (uint32_t*)(lds + RQ * A::kMade * 16) + rq * (KS * 64) + lane;
+    __syncthreads();   // the plan, or the last unit's rows, have been read
 #pragma unroll
-          for (int r = 1; r < RG; ++r)
-            if (rg == r) w = kreg[k * RG + r], word = ks[(k * RG + r) / 2] >> (16 * ((k * RG + r) & 1));
-          const uint32_t e = word & 255u;
-          const bool hide = e == 255u || !valid;   // counts as zero: who sees a NaN token sees it in the score
-          const float scale = mx::u2f((hide ? 127u : e) << 23);
-          const uint32_t c[4] = {hide ? 0u : w.x, hide ? 0u : w.y, hide ? 0u : w.z, hide ? 0u : w.w};
+    for (int e = 0; e < kEach; ++e) {
+      const int k = e * kSharers + sharer;
+      if (KS % kSharers && k >= KS) break;
+      const QueryStep s = query_step16(words[e], l16, quad);
+      made[k * 256] = make_uint4(s.high[0], s.high[1], s.high[2], s.high[3]);
+      const int low = kPart && k == 4 ? 64 : 128;   // a last step has nothing in its second halves
+      made[k * 256 + low] = make_uint4(s.low[0], s.low[1], s.low[2], s.low[3]);
+      if (!kPart || k < 4) {
+        made[k * 256 + 64] = make_uint4(s.high[4], s.high[5], s.high[6], s.high[7]);
+        made[k * 256 + 192] = make_uint4(s.low[4], s.low[5], s.low[6], s.low[7]);
+      }
+      made_scales[k * 64] = s.scales;
+    }
+    const bool alone = x == u.unit0 && u.unit1 <= end;
+    const int64_t slot = 2 * g + (g * per < u.unit0 ? 1 : 0);
+
+    if (wave < 4) {
+      mxd::lds_barrier();
+      v8i qh[KS], ql[KS];
+      uint32_t qs[(KS + 1) / 2] = {};
 #pragma unroll
-          for (int n = 0; n < 4; ++n) {
-            uint4 v;
-            v.x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c[n], scale, 0));
-            v.y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c[n], scale, 1));
-            v.z = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c[n], scale, 2));
-            v.w = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c[n], scale, 3));
-            *(uint4*)(buffer + put[n] + 128 * (4 * kh + k * RG + rg)) = v;
+      for (int k = 0; k < KS; ++k) {
+        const bool last = kPart && k == 4;
+        const uint4 h0 = made[k * 256], l0 = made[k * 256 + (last ? 64 : 128)];
+        const uint4 h1 = last ? make_uint4(0u, 0u, 0u, 0u) : made[k * 256 + 64], l1 = last ? make_uint4(0u, 0u, 0u, 0u) : made[k * 256 + 192];
+        qh[k] = {(int)h0.x, (int)h0.y, (int)h0.z, (int)h0.w, (int)h1.x, (int)h1.y, (int)h1.z, (int)h1.w};
+        ql[k] = {(int)l0.x, (int)l0.y, (int)l0.z, (int)l0.w, (int)l1.x, (int)l1.y, (int)l1.z, (int)l1.w};
+        qs[k / 2] |= made_scales[k * 64] << (16 * (k & 1));
+      }
+      int row_lo, row_hi;
+      seen(a, u.s, i, row_lo, row_hi);
+      // tokens [all_lo, all_hi) are seen by all of the wave's rows
+      int all_lo, all_hi, unused;
+      seen(a, u.s, min(row0 + rq * 16, rows - 1) / a.group, unused, all_hi);
+      seen(a, u.s, min(row0 + rq * 16 + 15, rows - 1) / a.group, all_lo, unused);
+      all_lo = uniform(all_lo), all_hi = uniform(all_hi);
+      const uint32_t get_k = tt * T2 * 4096 + l16 * 256 + ((quad ^ (l16 & 7)) * 16);
+      // probabilities: [16 tokens][row][half][8 tokens of it], as the products take them
+      uint8_t* const put_w = weights + (tt * T2 * A::kRows + rq * 16 + l16) * 32 + (quad & 1) * 16 + (quad >> 1) * 8;
+      float m = kLowest, l = 0.f;   // the maximum is a whole number: every rescaling is exact
+      float own = kLowest, sum = 0.f;
+      mxd::copy_barrier();   // the first step is there, and the queries have been read
+      for (int it = it0; it < it1; ++it) {
+        const uint8_t* stage = lds + A::kRing + (it % A::kStages) * A::kStage;
+        const int first = lo + it * A::kStep + tt * T2 * 16;
+        uint32_t shown = 0;
+#pragma unroll
+        for (int t = 0; t < T2; ++t) shown |= page_of(first + 16 * t) >= 0 ? 1u << t : 0u;
+        mxd::v4f sc[T2];
+        uint32_t ks[T2], klast[T2];
+#pragma unroll
+        for (int t = 0; t < T2; ++t) {
+          const uint4 w = *(const uint4*)(stage + A::kScales + (tt * T2 + t) * 256 + l16 * 16);
+          const uint32_t pick = 0x0C0C0400u + 0x0101u * quad;   // byte `quad` of the four words
+          ks[t] = __builtin_amdgcn_perm(w.y, w.x, pick) | __builtin_amdgcn_perm(w.w, w.z, pick) << 16;
+          sc[t] = {0.f, 0.f, 0.f, 0.f};
+          if constexpr (kPart) {
+            const uint32_t v = *(const uint32_t*)(stage + A::kTailScales + ((tt * T2 + t) * 16 + l16) * 4);
+            klast[t] = quad > 1 ? 127u : v >> (8 * quad);
+          }
+        }
+        auto codes = [&](int k, int t) { return *(const uint4*)(stage + (get_k ^ (k & 1 ? 64 : 0)) + 128 * (k >> 1) + 4096 * t); };
+#pragma unroll
+        for (int t = 0; t < T2; ++t) sc[t] = score_step<0>(codes(0, t), qh[0], ql[0], sc[t], ks[t], qs[0]);
+#pragma unroll
+        for (int t = 0; t < T2; ++t) sc[t] = score_step<1>(codes(1, t), qh[1], ql[1], sc[t], ks[t], qs[0]);
+#pragma unroll
+        for (int t = 0; t < T2; ++t) sc[t] = score_step<2>(codes(2, t), qh[2], ql[2], sc[t], ks[t], qs[1]);
+#pragma unroll
+        for (int t = 0; t < T2; ++t) sc[t] = score_step<3>(codes(3, t), qh[3], ql[3], sc[t], ks[t], qs[1]);
+        if constexpr (kPart) {
+#pragma unroll
+          for (int t = 0; t < T2; ++t) {
+            uint4 w = *(const uint4*)(stage + A::kTail + ((tt * T2 + t) * 16 + l16) * 32 + (quad & 1) * 16);
+            w = quad > 1 ? make_uint4(0u, 0u, 0u, 0u) : w;
+            sc[t] = score_step<4>(w, qh[KS - 1], ql[KS - 1], sc[t], klast[t], qs[2]);
+          }
+        }
+        if (shown != (1u << T2) - 1 || first < all_lo || first + 16 * T2 > all_hi) {
+#pragma unroll
+          for (int t = 0; t < T2; ++t)
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+              const int at = first + 16 * t + 4 * quad + n;
+              sc[t][n] = (shown >> t & 1) && at >= row_lo && at < row_hi ? sc[t][n] : -INFINITY;
+            }
+        }
+        if constexpr (TT > 1) {
+          if (it > it0) {   // the maximum with the last step's of the row's other waves
+            float next = kLowest;
+#pragma unroll
+            for (int t = 0; t < TT; ++t) next = fmaxf(next, tops[(it - 1) & 1][rq * 16 + l16][t]);
+            l = l * power(m, next) + sum * power(own, next);
+            m = next;
+          }
+        }
+        float top = fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3]));
+#pragma unroll
+        for (int t = 1; t < T2; ++t) top = fmaxf(top, fmaxf(fmaxf(sc[t][0], sc[t][1]), fmaxf(sc[t][2], sc[t][3])));
+        top = row_max4(top) * a.c;
+        // the maximum stays until it is 2^8 too low: probabilities up to 2^8 lose nothing
+        own = top > m + 8.f ? ceilf(top) : m;
+        sum = 0.f;
+#pragma unroll
+        for (int t = 0; t < T2; ++t) {
+          float p[4];
+#pragma unroll
+          for (int n = 0; n < 4; ++n) p[n] = __builtin_amdgcn_exp2f(fmaf(sc[t][n], a.c, -own));
+          sum += (p[0] + p[1]) + (p[2] + p[3]);
+          *(uint2*)(put_w + (it & 1) * A::kWeights + t * (A::kRows * 32)) = make_uint2(mxd::bf16_pair(p[0], p[1]), mxd::bf16_pair(p[2], p[3]));
+        }
+        if (quad == 0) tops[it & 1][rq * 16 + l16][tt] = own;
+        if constexpr (TT == 1) {
+          l = l * power(m, own) + sum;
+          m = own;
+        }
+        mxd::copy_barrier();
+      }
+      if constexpr (TT > 1) {
+        float next = kLowest;
+#pragma unroll
+        for (int t = 0; t < TT; ++t) next = fmaxf(next, tops[(it1 - 1) & 1][rq * 16 + l16][t]);
+        l = l * power(m, next) + sum * power(own, next);
+        m = next;
+      }
+      l = row_sum4(l);
+      if (quad == 0) stats[rq * 16 + l16][tt][0] = m, stats[rq * 16 + l16][tt][1] = l;
+      __syncthreads();
+      // where the rows go
+      if (tid < A::kRows) {
+        const int r = tid;
+        float all_l = 0.f;
+#pragma unroll
+        for (int t = 0; t < TT; ++t) all_l += stats[r][t][1];
+        Place to{-1, 1.f};
+        if (row0 + r < rows) {
+          if (alone) {
+            const int head = h * a.group + (row0 + r) % a.group;
+            const int64_t token = u.s.first + (row0 + r) / a.group;
+            const RowOut f = row_out(a, head, stats[r][0][0], all_l);
+            to = {token * a.q.out_stride + (int64_t)head * WV, f.inv};
+            if (a.q.lse) a.q.lse[token * a.q.heads + head] = f.lse;
+          } else {
+            ((float2*)(a.space + a.at.stats))[slot * A::kRows + r] = make_float2(stats[r][0][0], all_l);
+          }
+        }
+        places[r] = to;
+      }
+      __syncthreads();
+    } else {
+      // LDS places of the wave's values: a converter's 16-byte pieces of its token, and a reader's 8 bytes
+      uint8_t* tile = lds + cg * A::kTile;
+      uint32_t put[4];
+#pragma unroll
+      for (int n = 0; n < 4; ++n) put[n] = l16 * 256 + 128 * (quad >> 1) + ((4 * (quad & 1) + n) ^ spread) * 16;
+      const int rt = l16 >> 2, rc = lane & 3, rs = 2 * rt + half;
+      const uint32_t get0 = (4 * half + rt) * 256 + ((2 * (quad & 1) + rc / 2) ^ rs) * 16 + (rc & 1) * 8, get1 = get0 ^ 64;
+      const uint32_t get_c = l16 * 256 + (((4 * (cg & 1) + quad) ^ (l16 & 7)) * 16) + 128 * (cg >> 1);   // the columns' codes
+      const uint32_t get_s = A::kScales + l16 * 16 + 4 * cg;
+      float m[RG];
+      v16f o[RG][4];
+#pragma unroll
+      for (int r = 0; r < RG; ++r) {
+        m[r] = kLowest;
+#pragma unroll
+        for (int d = 0; d < 4; ++d)
+#pragma unroll
+          for (int n = 0; n < 16; ++n) o[r][d][n] = 0.f;
+      }
+      // 16 tokens' columns of step `it` to BF16
+      auto convert = [&](int it, int t) {
+        const uint8_t* stage = lds + A::kRing + (it % A::kStages) * A::kStage;
+        const uint4 w = *(const uint4*)(stage + get_c + 4096 * t);
+        const uint32_t e = *(const uint32_t*)(stage + get_s + 256 * t) >> (8 * quad) & 255u;
+        // NaN blocks count as tiny here, as what no token of the sequence has left: who sees a NaN token has NaN from its
+        // score, and for the others 0 times this is 0
+        const int first = lo + it * A::kStep + 16 * t;
+        const bool valid = l16 < (page_of(first) >= 0 ? hi - first : 0);
+        const float scale = mx::u2f((e != 255u && valid ? e : 0u) << 23);
+        const uint32_t c[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+          uint4 v;
+          v.x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c[n], scale, 0));
+          v.y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c[n], scale, 1));
+          v.z = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c[n], scale, 2));
+          v.w = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c[n], scale, 3));
+          *(uint4*)(tile + put[n] + 4096 * t) = v;
+        }
+      };
+      bool moved = false;
+      float theirs[RG][TT];
+      auto settle = [&](int it) {   // the maxima with step `it`'s
+        bool any = false;
+        float next[RG];
+#pragma unroll
+        for (int r = 0; r < RG; ++r) {
+          next[r] = kLowest;
+#pragma unroll
+          for (int t = 0; t < TT; ++t) {
+            theirs[r][t] = tops[it & 1][r * 32 + col][t];
+            next[r] = fmaxf(next[r], theirs[r][t]);
+          }
+          any |= next[r] != m[r];
+        }
+        moved = __any(any);
+        if (moved) {
+#pragma unroll
+          for (int r = 0; r < RG; ++r) {
+            const float by = power(m[r], next[r]);
+            m[r] = next[r];
+#pragma unroll
+            for (int d = 0; d < 4; ++d)
+#pragma unroll
+              for (int n = 0; n < 16; ++n) o[r][d][n] *= by;
           }
         }
       };
-      if (A::kBuffers > 1) convert();
-      // -- the other half's sums of the tokens that stay here (registers 0 to 7) --
-      {
-        float4* to = (float4*)(half_sums + wave * 2048) + lane;
-        to[0] = make_float4(sc[8], sc[9], sc[10], sc[11]), to[64] = make_float4(sc[12], sc[13], sc[14], sc[15]);
-      }
-      mxd::lds_barrier();
-      float s[8];
-      {
-        const float4* from = (const float4*)(half_sums + (wave ^ RG) * 2048) + lane;
-        const float4 u0 = from[0], u1 = from[64];
-        s[0] = sc[0] + u0.x, s[1] = sc[1] + u0.y, s[2] = sc[2] + u0.z, s[3] = sc[3] + u0.w;
-        s[4] = sc[4] + u1.x, s[5] = sc[5] + u1.y, s[6] = sc[6] + u1.z, s[7] = sc[7] + u1.w;
-      }
-      if (A::kBuffers == 1) convert();   // nobody reads the last step's any more
-      const uint32_t shown = (uint32_t)__ballot(valid) & 0xFFFFu;
-      const int first = lo + (it * TG + tile) * 32 + 16 * kh;
-      load(it + 1, page_next);
-      page_next = page_of(it + 2);
-      // -- softmax --
-      if (shown != 0xFFFFu || first < all_lo || first + 16 > all_hi) {
+      // O^T += V^T P^T of step `it`, 16 tokens
+      auto multiply = [&](int it, int t) {
+        v8b pv[RG];
 #pragma unroll
-        for (int n = 0; n < 8; ++n) {
-          const int t = 8 * (n / 4) + 4 * half + (n & 3);
-          s[n] = (shown >> t & 1) && first + t >= row_lo && first + t < row_hi ? s[n] : -INFINITY;
+        for (int r = 0; r < RG; ++r) {
+          uint4 w = *(const uint4*)(weights + (it & 1) * A::kWeights + (t * A::kRows + r * 32 + col) * 32 + half * 16);
+          if (TT > 1 && moved) {   // whole powers of two: exact
+            const float f = power(theirs[r][t / T2], m[r]);
+            auto scaled = [&](uint32_t v) { return mxd::bf16_pair(mx::u2f(v << 16) * f, mx::u2f(v & 0xFFFF0000u) * f); };
+            w = make_uint4(scaled(w.x), scaled(w.y), scaled(w.z), scaled(w.w));
+          }
+          pv[r] = __builtin_bit_cast(v8b, w);
         }
-      }
-      float top = fmaxf(s[0], s[1]);
 #pragma unroll
-      for (int n = 2; n < 8; ++n) top = fmaxf(top, s[n]);
-      top = other_half_max(top) * a.c;
-      // the maximum stays until it is 2^8 too low: probabilities up to 2^8 lose nothing
-      const float own = top > m + 8.f ? ceilf(top) : m;
-      uint32_t p[4];
-      float sum = 0.f;
-#pragma unroll
-      for (int n = 0; n < 4; ++n) {
-        const float p0 = __builtin_amdgcn_exp2f(fmaf(s[2 * n], a.c, -own)), p1 = __builtin_amdgcn_exp2f(fmaf(s[2 * n + 1], a.c, -own));
-        sum += p0 + p1;
-        p[n] = mxd::bf16_pair(p0, p1);
-      }
-      ((uint4*)(weights + wave * 1024))[lane] = make_uint4(p[0], p[1], p[2], p[3]);
-      if (half == 0) tops[rg][col][cg] = own;
-      mxd::lds_barrier();
-      float theirs[CG], next = kLowest;
-      {
-        const float4* from = (const float4*)tops[rg][col];
-#pragma unroll
-        for (int t = 0; t < CG / 4; ++t) {
-          const float4 v = from[t];
-          theirs[4 * t] = v.x, theirs[4 * t + 1] = v.y, theirs[4 * t + 2] = v.z, theirs[4 * t + 3] = v.w;
-          next = fmaxf(next, fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)));
-        }
-      }
-      const bool moved = __any(next != m);   // else everybody's is m
-      if (moved) {
-        const float by = power(m, next);
-        m = next, l *= by;
-#pragma unroll
-        for (int d = 0; d < DB; ++d)
-#pragma unroll
-          for (int n = 0; n < 16; ++n) o[d][n] *= by;
-        sum *= power(own, next);
-      }
-      l += sum;
-      // -- O^T += V^T P^T --
-#pragma unroll
-      for (int t = 0; t < CG; ++t) {   // 16 tokens, of the wave that weighed them
-        const uint4 w = ((const uint4*)(weights + (t * RG + rg) * 1024))[lane];
-        uint32_t pw[4] = {w.x, w.y, w.z, w.w};
-        if (moved) {   // whole powers of two: exact
-          const float by = power(theirs[t], m);
-#pragma unroll
-          for (int n = 0; n < 4; ++n) pw[n] = mxd::bf16_pair(mx::u2f(pw[n] << 16) * by, mx::u2f(pw[n] & 0xFFFF0000u) * by);
-        }
-        const v8b pv = __builtin_bit_cast(v8b, make_uint4(pw[0], pw[1], pw[2], pw[3]));
-#pragma unroll
-        for (int d = 0; d < DB; ++d) {
-          const uint8_t* at = buffer + (d & 1 ? get1 : get0) + 128 * (d / 2) + (t >> 1) * A::kTile + 16 * (t & 1) * (2 * WV);
+        for (int d = 0; d < 4; ++d) {
+          const uint8_t* at = tile + (d & 1 ? get1 : get0) + 128 * (d / 2) + 4096 * t;
           typedef __attribute__((address_space(3))) v4s lds_v4s;
           v4s w2[2];
           w2[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)at);
-          w2[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(at + 8 * (2 * WV)));
+          w2[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(at + 2048));
           const v8b vv = __builtin_bit_cast(v8b, w2);
-          o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vv, pv, o[d], 0, 0, 0);
-        }
-      }
-    }
-
-    // -- the row's sum over the waves, and out --
-    l = halves_sum(l);
-    if (half == 0) stats[wave][col] = l;
-    __syncthreads();   // and everybody has read its values
-    const bool alone = x == u.unit0 && u.unit1 <= end;
-    const int64_t slot = 2 * g + (g * per < u.unit0 ? 1 : 0);
-    if (cg == 0 && half == 0) {
-      float all_l = 0.f;
 #pragma unroll
-      for (int t = 0; t < CG; ++t) all_l += stats[t * RG + rg][col];
-      Place to{-1, 1.f};
-      if (row0 + col < rows) {
-        if (alone) {
-          const int head = h * a.group + row % a.group;
-          const int64_t token = u.s.first + i;
-          const RowOut f = row_out(a, head, m, all_l);
-          to = {token * a.q.out_stride + (int64_t)head * WV, f.inv};
-          if (a.q.lse) a.q.lse[token * a.q.heads + head] = f.lse;
+          for (int r = 0; r < RG; ++r) o[r][d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vv, pv[r], o[r][d], 0, 0, 0);
+        }
+      };
+      // this wave's copies of the step after `it` have landed; those of later steps may be on their way
+      auto landed = [&](int it) {
+        if (it + A::kStages - 1 < it1) {
+          copy(it + A::kStages - 1);
+          __builtin_amdgcn_s_waitcnt(mxd::vm_wait_imm(A::kCopies * (A::kStages - 2)));
         } else {
-          ((float2*)(a.space + a.at.stats))[slot * A::kRows + rg * 32 + col] = make_float2(m, all_l);
+          __builtin_amdgcn_s_waitcnt(mxd::vm_wait_imm(0));
         }
+        asm volatile("" ::: "memory");
+      };
+      mxd::lds_barrier();   // (the queries)
+      __builtin_amdgcn_s_waitcnt(mxd::vm_wait_imm(0));
+      mxd::copy_barrier();
+#pragma unroll
+      for (int t = 0; t < 4; ++t) convert(it0, t);
+      landed(it0);
+      mxd::copy_barrier();
+      for (int it = it0 + 1; it < it1; ++it) {
+        settle(it - 1);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          multiply(it - 1, t);
+          if (t > 0) convert(it, t - 1);
+        }
+        convert(it, 3);
+        landed(it);
+        mxd::copy_barrier();
       }
-      places[rg * 32 + col] = to;
-    }
-    if (alone) {
+      settle(it1 - 1);
+#pragma unroll
+      for (int t = 0; t < 4; ++t) multiply(it1 - 1, t);
       __syncthreads();
-      float* own_out = (float*)(lds + wave * A::kOut);
+      __syncthreads();
+      if (alone) {
+        float* own_out = (float*)(lds + cg * A::kOut);
 #pragma unroll
-      for (int d0 = 0; d0 < DB; d0 += 2) {
+        for (int r = 0; r < RG; ++r)
 #pragma unroll
-        for (int d = 0; d < 2; ++d)
+          for (int d0 = 0; d0 < 4; d0 += 2) {
 #pragma unroll
-          for (int n = 0; n < 4; ++n) {
-            const v16f& v = o[d0 + d];
-            *(float4*)(own_out + col * (CB + 4) + 32 * d + 8 * n + 4 * half) = make_float4(v[4 * n], v[4 * n + 1], v[4 * n + 2], v[4 * n + 3]);
-          }
+            for (int d = 0; d < 2; ++d)
+#pragma unroll
+              for (int n = 0; n < 4; ++n) {
+                const v16f& v = o[r][d0 + d];
+                *(float4*)(own_out + col * (CB + 4) + 32 * d + 8 * n + 4 * half) = make_float4(v[4 * n], v[4 * n + 1], v[4 * n + 2], v[4 * n + 3]);
+              }
 #pragma unroll 2
-        for (int r = lane / 8; r < 32; r += 8) {
-          const int c = lane % 8 * 8;
-          const Place to = places[rg * 32 + r];
-          const float4 v0 = *(const float4*)(own_out + r * (CB + 4) + c), v1 = *(const float4*)(own_out + r * (CB + 4) + c + 4);
-          if (to.at < 0) continue;
-          uint4 w;
-          w.x = mxd::bf16_pair(v0.x * to.by, v0.y * to.by), w.y = mxd::bf16_pair(v0.z * to.by, v0.w * to.by);
-          w.z = mxd::bf16_pair(v1.x * to.by, v1.y * to.by), w.w = mxd::bf16_pair(v1.z * to.by, v1.w * to.by);
-          *(uint4*)(a.q.out + to.at + cg * (DB * 32) + d0 * 32 + c) = w;
-        }
+            for (int at = lane / 8; at < 32; at += 8) {
+              const int c = lane % 8 * 8;
+              const Place to = places[r * 32 + at];
+              const float4 v0 = *(const float4*)(own_out + at * (CB + 4) + c), v1 = *(const float4*)(own_out + at * (CB + 4) + c + 4);
+              if (to.at < 0) continue;
+              uint4 w;
+              w.x = mxd::bf16_pair(v0.x * to.by, v0.y * to.by), w.y = mxd::bf16_pair(v0.z * to.by, v0.w * to.by);
+              w.z = mxd::bf16_pair(v1.x * to.by, v1.y * to.by), w.w = mxd::bf16_pair(v1.z * to.by, v1.w * to.by);
+              *(uint4*)(a.q.out + to.at + cg * 128 + d0 * 32 + c) = w;
+            }
+          }
+      } else {   // parts as the registers have them: [wave][row group][block][4 registers][lane]
+        float4* part = (float4*)(a.space + a.at.rows) + (slot * 4 + cg) * (RG * 4 * 4 * 64) + lane;
+#pragma unroll
+        for (int r = 0; r < RG; ++r)
+#pragma unroll
+          for (int d = 0; d < 4; ++d)
+#pragma unroll
+            for (int n = 0; n < 4; ++n)
+              part[((r * 4 + d) * 4 + n) * 64] = make_float4(o[r][d][4 * n], o[r][d][4 * n + 1], o[r][d][4 * n + 2], o[r][d][4 * n + 3]);
       }
-    } else {   // parts as the registers have them: [wave][block][4 registers][lane]
-      float4* part = (float4*)(a.space + a.at.rows) + (slot * 8 + wave) * (DB * 4 * 64) + lane;
-#pragma unroll
-      for (int d = 0; d < DB; ++d)
-#pragma unroll
-        for (int n = 0; n < 4; ++n) part[(d * 4 + n) * 64] = make_float4(o[d][4 * n], o[d][4 * n + 1], o[d][4 * n + 2], o[d][4 * n + 3]);
     }
     if (u.unit1 >= end) {   // the workgroup's last: it joins the unit if it began it and does not end it
       if (tid == 0) {
@@ -711,6 +861,7 @@ __global__ __launch_bounds__(512, 2) void latent_kernel(AttendArgs a, int inline
     }
     x = u.unit1;
     next_unit(a, u, A::kRows, A::kStep);
+    __syncthreads();   // what went out has been read before the next unit's copies and queries come
   }
 }
 
@@ -751,11 +902,11 @@ __global__ __launch_bounds__(256, (Grouped<W, RG>::kWaves)) void grouped_kernel(
   }
   const int64_t all = uniform(plan.prefix[plan.base[a.q.batch]]) * a.cache.heads;
   constexpr int groups = A::kGroups;
-  const int64_t per = max<int64_t>((all + groups - 1) / groups, 1);
+  const int64_t per = larger((all + groups - 1) / groups, 1);
   // workgroups go round the XCDs: neighbours in the work, which share keys, to one L2
   const int g = (int)(blockIdx.x % kXcds) * (groups / kXcds) + (int)blockIdx.x / kXcds;
-  int64_t x = min(g * per, all);
-  const int64_t end = min(x + per, all);
+  int64_t x = lesser(g * per, all);
+  const int64_t end = lesser(x + per, all);
   Shared* shared = (Shared*)(a.space + a.at.units) + g;
   if (x >= end) {
     if (tid == 0) shared->parts = 0;
@@ -774,7 +925,7 @@ __global__ __launch_bounds__(256, (Grouped<W, RG>::kWaves)) void grouped_kernel(
   const uint32_t get1 = get0 ^ 64;
 
   for (;;) {
-    const int it0 = (int)(x - u.unit0), it1 = (int)(min(u.unit1, end) - u.unit0);
+    const int it0 = (int)(x - u.unit0), it1 = (int)(lesser(u.unit1, end) - u.unit0);
     // -- the wave's query rows --
     const int rows = u.s.n * a.group;   // at most 2^30
     const int row0 = u.tile * A::kRows + rg * 32, row = min(row0 + col, rows - 1);
@@ -800,7 +951,7 @@ __global__ __launch_bounds__(256, (Grouped<W, RG>::kWaves)) void grouped_kernel(
     bool valid = false;
     auto load = [&](int it, int page) {
       valid = page >= 0 && page < a.cache.pages;
-      const int64_t at = ((int64_t)(valid ? page : 0) * a.cache.heads + h << a.page_shift) + (token_of(it) & ((1 << a.page_shift) - 1));
+      const int64_t at = (((int64_t)(valid ? page : 0) * a.cache.heads + h) << a.page_shift) + (token_of(it) & ((1 << a.page_shift) - 1));
       const uint8_t* p = a.cache.k_codes + at * (W / 2) + 16 * half;
       const uint8_t* pv = a.cache.v_codes + at * (W / 2) + 16 * half;
 #pragma unroll
@@ -826,7 +977,7 @@ __global__ __launch_bounds__(256, (Grouped<W, RG>::kWaves)) void grouped_kernel(
       QueryWords words[kEach];
 #pragma unroll
       for (int e = 0; e < kEach; ++e)
-        if (e * TG + tg < KS) words[e] = query_words(q, 64 * (e * TG + tg), half);
+        if (e * TG + tg < KS) words[e] = query_words<32>(q + 64 * (e * TG + tg) + 16 * half);
       uint4* made = (uint4*)lds + rg * (KS * 256) + lane;
       uint32_t* made_scales = (uint32_t*)(lds + RG * KS * 4096) + rg * (KS * 64) + lane;
       __syncthreads();   // the plan, or the last unit's rows, have been read
@@ -1055,68 +1206,109 @@ __global__ __launch_bounds__(256, (Grouped<W, RG>::kWaves)) void grouped_kernel(
   }
 }
 
-// The parts of four values of a row: the first workgroup's lies in slot 2 g + slot, the others' in their first.
-struct Joined {
-  float4 v;
-  float most, sum;
-};
-template <typename Part>
-__device__ __forceinline__ Joined join_parts(const AttendArgs& a, const Shared& s, int tile_rows, int r, Part part) {
-  const float2* stats = (const float2*)(a.space + a.at.stats) + r;
-  auto slot = [&](int i) { return (int64_t)2 * (blockIdx.x + i) + (i ? 0 : s.slot); };
-  Joined j{make_float4(0.f, 0.f, 0.f, 0.f), kLowest, 0.f};
-#pragma unroll 8
-  for (int i = 0; i < s.parts; ++i) j.most = fmaxf(j.most, stats[slot(i) * tile_rows].x);
-#pragma unroll 8
-  for (int i = 0; i < s.parts; ++i) {
-    const float2 st = stats[slot(i) * tile_rows];
-    const float4 p = part(slot(i));
-    const float by = power(st.x, j.most);
-    j.sum += st.y * by;
-    j.v.x += p.x * by, j.v.y += p.y * by, j.v.z += p.z * by, j.v.w += p.w * by;
+// The units that several workgroups had. A workgroup takes pieces of 64 times four values, of all units in turn: its waves
+// add up every fourth part each. Which units there are it finds in the workgroups' last units, all of them at once.
+//
+// piece(e, r, c): the row and first column of the e-th four values of a unit, as its parts have them.
+template <int kGroups, int kRows, int WV, typename Piece>
+__device__ __forceinline__ void join(const AttendArgs& a, Piece piece) {
+  __shared__ Shared list[kGroups];
+  __shared__ int32_t from[kGroups];
+  __shared__ uint32_t counts[4];
+  __shared__ float4 sums[4][64];
+  __shared__ float2 tops[4][64];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  int n = 0;
+  for (int g0 = 0; g0 < kGroups; g0 += 256) {
+    const Shared s = ((const Shared*)(a.space + a.at.units))[g0 + tid];
+    const uint64_t mask = __ballot(s.parts > 1);
+    if (lane == 0) counts[wave] = __popcll(mask);
+    __syncthreads();
+    int at = n + __popcll(mask & ((1ull << lane) - 1));
+    for (int w = 0; w < 4; ++w) {
+      at += w < wave ? counts[w] : 0;
+      n += counts[w];
+    }
+    if (s.parts > 1) list[at] = s, from[at] = g0 + tid;
+    __syncthreads();
   }
-  return j;
+  constexpr int kPieces = kRows * WV / 256;
+  const float4* parts = (const float4*)(a.space + a.at.rows);
+  for (int k = blockIdx.x; k < n * kPieces; k += gridDim.x) {
+    const Shared s = list[k / kPieces];
+    const int g = from[k / kPieces], e = k % kPieces * 64 + lane;
+    int r, c;
+    piece(e, r, c);
+    const float2* stats = (const float2*)(a.space + a.at.stats) + r;
+    // the first workgroup's part lies in its slot s.slot, the others' in their first
+    auto slot = [&](int i) { return (int64_t)2 * (g + i) + (i ? 0 : s.slot); };
+    float most = kLowest, sum = 0.f;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int i0 = wave; i0 < s.parts; i0 += 16) {   // four at a time
+      float2 st[4];
+      float4 p[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int64_t at = slot(min(i0 + 4 * j, s.parts - 1));
+        st[j] = stats[at * kRows];
+        p[j] = parts[at * (kRows * WV / 4) + e];
+      }
+      float next = most;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) next = fmaxf(next, st[j].x);
+      const float by = power(most, next);
+      most = next, sum *= by;
+      v.x *= by, v.y *= by, v.z *= by, v.w *= by;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (i0 + 4 * j >= s.parts) break;
+        const float f = power(st[j].x, most);
+        sum += st[j].y * f;
+        v.x += p[j].x * f, v.y += p[j].y * f, v.z += p[j].z * f, v.w += p[j].w * f;
+      }
+    }
+    sums[wave][lane] = v, tops[wave][lane] = make_float2(most, sum);
+    __syncthreads();
+    if (wave == 0) {
+#pragma unroll
+      for (int w = 1; w < 4; ++w) most = fmaxf(most, tops[w][lane].x);
+      sum = 0.f, v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const float f = power(tops[w][lane].x, most);
+        const float4 p = sums[w][lane];
+        sum += tops[w][lane].y * f;
+        v.x += p.x * f, v.y += p.y * f, v.z += p.z * f, v.w += p.w * f;
+      }
+      const Sequence q = sequence(a, s.b);
+      const int row = s.tile * kRows + r;
+      if (row < q.n * a.group) {
+        const int head = s.h * a.group + row % a.group;
+        const int64_t token = q.first + row / a.group;
+        const RowOut f = row_out(a, head, most, sum);
+        uint2 w;
+        w.x = mxd::bf16_pair(v.x * f.inv, v.y * f.inv), w.y = mxd::bf16_pair(v.z * f.inv, v.w * f.inv);
+        *(uint2*)(a.q.out + token * a.q.out_stride + (int64_t)head * WV + c) = w;
+        if (a.q.lse && c == 0) a.q.lse[token * a.q.heads + head] = f.lse;
+      }
+    }
+    __syncthreads();
+  }
 }
 
-__device__ __forceinline__ void put_joined(const AttendArgs& a, const Shared& s, const Sequence& q, int row, int c, int width, const Joined& j) {
-  const int head = s.h * a.group + row % a.group;
-  const int64_t token = q.first + row / a.group;
-  const RowOut f = row_out(a, head, j.most, j.sum);
-  uint2 w;
-  w.x = mxd::bf16_pair(j.v.x * f.inv, j.v.y * f.inv), w.y = mxd::bf16_pair(j.v.z * f.inv, j.v.w * f.inv);
-  *(uint2*)(a.q.out + token * a.q.out_stride + (int64_t)head * width + c) = w;
-  if (a.q.lse && c == 0) a.q.lse[token * a.q.heads + head] = f.lse;
-}
-
-// A unit of latents that several workgroups had, four values a thread: blockIdx.x the workgroup that began it.
 template <int RG>
 __global__ __launch_bounds__(256) void join_latent_kernel(AttendArgs a) {
   using A = Latent<512, RG>;
-  const Shared s = ((const Shared*)(a.space + a.at.units))[blockIdx.x];
-  if (s.parts < 2) return;
-  const int e = blockIdx.y * 256 + threadIdx.x, lane = e & 63, n = e >> 6 & 3, d = e >> 8 & (A::DB - 1), wave = e / (256 * A::DB);
-  const int rg = wave % RG, cg = wave / RG, r = rg * 32 + (lane & 31), c = cg * (A::DB * 32) + 32 * d + 8 * n + 4 * (lane >> 5);
-  const Sequence q = sequence(a, s.b);
-  const int row = s.tile * A::kRows + r;
-  if (row >= q.n * a.group) return;
-  const float4* parts = (const float4*)(a.space + a.at.rows) + e;
-  const Joined j = join_parts(a, s, A::kRows, r, [&](int64_t slot) { return parts[slot * (A::kRows * A::WV / 4)]; });
-  put_joined(a, s, q, row, c, A::WV, j);
+  join<kCus, A::kRows, A::WV>(a, [](int e, int& r, int& c) {
+    const int lane = e & 63, n = e >> 6 & 3, d = e >> 8 & 3, rg = e >> 10 & (RG - 1), wave = e / (1024 * RG);
+    r = rg * 32 + (lane & 31), c = wave * 128 + 32 * d + 8 * n + 4 * (lane >> 5);
+  });
 }
 
-// A unit that several workgroups had, four values a thread: blockIdx.x the workgroup that began it.
 template <int W, int RG>
 __global__ __launch_bounds__(256) void join_grouped_kernel(AttendArgs a) {
   using A = Grouped<W, RG>;
-  const Shared s = ((const Shared*)(a.space + a.at.units))[blockIdx.x];
-  if (s.parts < 2) return;
-  const int e = blockIdx.y * 256 + threadIdx.x, r = e / (W / 4), c = e % (W / 4) * 4;
-  const Sequence q = sequence(a, s.b);
-  const int row = s.tile * A::kRows + r;
-  if (row >= q.n * a.group) return;
-  const float4* parts = (const float4*)(a.space + a.at.rows) + e;
-  const Joined j = join_parts(a, s, A::kRows, r, [&](int64_t slot) { return parts[slot * (A::kRows * W / 4)]; });
-  put_joined(a, s, q, row, c, W, j);
+  join<A::kGroups, A::kRows, W>(a, [](int e, int& r, int& c) { r = e / (W / 4), c = e % (W / 4) * 4; });
 }
 
 int check_attend(const char* who, const mx_kv4* c, int32_t heads, int32_t tokens, int32_t batch) {
@@ -1202,12 +1394,12 @@ int mx_kv4_attend(mx_ctx* ctx, const mx_kv4* cache, const mx_kv4_query* query, v
     hipLaunchKernelGGL(plan_kernel, dim3(1), dim3(1024), 0, st, a, tile_rows, step);
     MX_LAUNCH_CHECK("plan_kernel");
   }
-  const int n = workgroups(cache);
+  const int n = workgroups(cache), joiners = 8 * kCus;
   auto latent = [&](auto wk, auto groups) {
     constexpr int WK = decltype(wk)::value, RG = decltype(groups)::value;
     hipLaunchKernelGGL((latent_kernel<WK, RG>), dim3(n), dim3(512), 0, st, a, (int)inline_plan);
     MX_LAUNCH_CHECK("latent_kernel");
-    hipLaunchKernelGGL(join_latent_kernel<RG>, dim3(n, 16 * RG), dim3(256), 0, st, a);
+    hipLaunchKernelGGL(join_latent_kernel<RG>, dim3(joiners), dim3(256), 0, st, a);
     MX_LAUNCH_CHECK("join_latent_kernel");
     return MX_OK;
   };
@@ -1215,7 +1407,7 @@ int mx_kv4_attend(mx_ctx* ctx, const mx_kv4* cache, const mx_kv4_query* query, v
     constexpr int W = decltype(w)::value, RG = decltype(groups)::value;
     hipLaunchKernelGGL((grouped_kernel<W, RG>), dim3(n), dim3(256), 0, st, a, (int)inline_plan);
     MX_LAUNCH_CHECK("grouped_kernel");
-    hipLaunchKernelGGL((join_grouped_kernel<W, RG>), dim3(n, RG * W / 32), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((join_grouped_kernel<W, RG>), dim3(joiners), dim3(256), 0, st, a);
     MX_LAUNCH_CHECK("join_grouped_kernel");
     return MX_OK;
   };
