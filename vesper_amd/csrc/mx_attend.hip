@@ -507,13 +507,23 @@ __global__ __launch_bounds__(512, 2) void latent_kernel(AttendArgs a, int inline
     // -- pages: 16 tokens have one --
     const __attribute__((address_space(4))) int32_t* table =
         (const __attribute__((address_space(4))) int32_t*)(a.q.table + (int64_t)u.b * a.q.columns);
-    auto page_of = [&](int t) {   // -1: none
-      const int page = table[min(t, max(hi - 1, 0)) >> a.page_shift];
-      return t < hi && (uint32_t)page < (uint32_t)a.cache.pages ? page : -1;
+    auto entry_of = [&](int t) { return table[min(t, max(hi - 1, 0)) >> a.page_shift]; };
+    auto is_there = [&](int t, int entry) { return t < hi && (uint32_t)entry < (uint32_t)a.cache.pages; };
+    // a step's four entries are asked for a step before they are looked at, so that nobody waits for them; bit t: 16 tokens
+    int entries[4];
+    auto ask = [&](int it) {
+#pragma unroll
+      for (int t = 0; t < 4; ++t) entries[t] = entry_of(lo + it * A::kStep + 16 * t);
     };
-    // -- a value wave's copies of step `it`: its 16 tokens --
-    auto copy = [&](int it) {
-      const int t = lo + it * A::kStep + 16 * cg, page = max(page_of(t), 0);
+    auto shown_of = [&](int it) {
+      uint32_t shown = 0;
+#pragma unroll
+      for (int t = 0; t < 4; ++t) shown |= is_there(lo + it * A::kStep + 16 * t, entries[t]) ? 1u << t : 0u;
+      return shown;
+    };
+    // -- a value wave's copies of step `it`: its 16 tokens, on page `entry` --
+    auto copy = [&](int it, int entry) {
+      const int t = lo + it * A::kStep + 16 * cg, page = is_there(t, entry) ? entry : 0;
       const int64_t at = (((int64_t)page * a.cache.heads + h) << a.page_shift) + (t & ((1 << a.page_shift) - 1));
       const uint8_t* codes = a.cache.k_codes + at * (WK / 2);
       const uint8_t* scales = a.cache.k_scales + at * scale_pitch(WK);
@@ -532,8 +542,10 @@ __global__ __launch_bounds__(512, 2) void latent_kernel(AttendArgs a, int inline
     if (wave >= 4) {
 #pragma unroll
       for (int k = 0; k < A::kStages - 1; ++k)
-        if (it0 + k < it1) copy(it0 + k);
+        if (it0 + k < it1) copy(it0 + k, entry_of(lo + (it0 + k) * A::kStep + 16 * cg));
     }
+    ask(it0);
+    uint32_t shown = shown_of(it0);
     // -- the queries, converted and exchanged --
     uint4* made = (uint4*)lds + rq * A::kMade + lane;
     uint32_t* made_scales = (uint32_t*)(lds + RQ * A::kMade * 16) + rq * (KS * 64) + lane;
@@ -584,9 +596,7 @@ __global__ __launch_bounds__(512, 2) void latent_kernel(AttendArgs a, int inline
       for (int it = it0; it < it1; ++it) {
         const uint8_t* stage = lds + A::kRing + (it % A::kStages) * A::kStage;
         const int first = lo + it * A::kStep + tt * T2 * 16;
-        uint32_t shown = 0;
-#pragma unroll
-        for (int t = 0; t < T2; ++t) shown |= page_of(first + 16 * t) >= 0 ? 1u << t : 0u;
+        ask(it + 1);
         mxd::v4f sc[T2];
         uint32_t ks[T2], klast[T2];
 #pragma unroll
@@ -617,13 +627,13 @@ __global__ __launch_bounds__(512, 2) void latent_kernel(AttendArgs a, int inline
             sc[t] = score_step<4>(w, qh[KS - 1], ql[KS - 1], sc[t], klast[t], qs[2]);
           }
         }
-        if (shown != (1u << T2) - 1 || first < all_lo || first + 16 * T2 > all_hi) {
+        if (shown != 15u || first < all_lo || first + 16 * T2 > all_hi) {
 #pragma unroll
           for (int t = 0; t < T2; ++t)
 #pragma unroll
             for (int n = 0; n < 4; ++n) {
               const int at = first + 16 * t + 4 * quad + n;
-              sc[t][n] = (shown >> t & 1) && at >= row_lo && at < row_hi ? sc[t][n] : -INFINITY;
+              sc[t][n] = (shown >> (tt * T2 + t) & 1) && at >= row_lo && at < row_hi ? sc[t][n] : -INFINITY;
             }
         }
         if constexpr (TT > 1) {
@@ -655,6 +665,7 @@ __global__ __launch_bounds__(512, 2) void latent_kernel(AttendArgs a, int inline
           l = l * power(m, own) + sum;
           m = own;
         }
+        shown = shown_of(it + 1);
         mxd::copy_barrier();
       }
       if constexpr (TT > 1) {
@@ -708,25 +719,31 @@ __global__ __launch_bounds__(512, 2) void latent_kernel(AttendArgs a, int inline
 #pragma unroll
           for (int n = 0; n < 16; ++n) o[r][d][n] = 0.f;
       }
-      // 16 tokens' columns of step `it` to BF16
-      auto convert = [&](int it, int t) {
+      // 16 tokens' columns of a step: their codes, and to BF16
+      struct Codes {
+        uint4 w;
+        uint32_t scales;
+        bool valid;
+      };
+      auto codes_of = [&](int it, int t) {
         const uint8_t* stage = lds + A::kRing + (it % A::kStages) * A::kStage;
-        const uint4 w = *(const uint4*)(stage + get_c + 4096 * t);
-        const uint32_t e = *(const uint32_t*)(stage + get_s + 256 * t) >> (8 * quad) & 255u;
+        return Codes{*(const uint4*)(stage + get_c + 4096 * t), *(const uint32_t*)(stage + get_s + 256 * t),
+                     l16 < (shown >> t & 1 ? hi - (lo + it * A::kStep + 16 * t) : 0)};
+      };
+      auto convert = [&](const Codes& v, int t) {
         // NaN blocks count as tiny here, as what no token of the sequence has left: who sees a NaN token has NaN from its
         // score, and for the others 0 times this is 0
-        const int first = lo + it * A::kStep + 16 * t;
-        const bool valid = l16 < (page_of(first) >= 0 ? hi - first : 0);
-        const float scale = mx::u2f((e != 255u && valid ? e : 0u) << 23);
-        const uint32_t c[4] = {w.x, w.y, w.z, w.w};
+        const uint32_t e = v.scales >> (8 * quad) & 255u;
+        const float scale = mx::u2f((e != 255u && v.valid ? e : 0u) << 23);
+        const uint32_t c[4] = {v.w.x, v.w.y, v.w.z, v.w.w};
 #pragma unroll
         for (int n = 0; n < 4; ++n) {
-          uint4 v;
-          v.x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c[n], scale, 0));
-          v.y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c[n], scale, 1));
-          v.z = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c[n], scale, 2));
-          v.w = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c[n], scale, 3));
-          *(uint4*)(tile + put[n] + 4096 * t) = v;
+          uint4 w;
+          w.x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c[n], scale, 0));
+          w.y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c[n], scale, 1));
+          w.z = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c[n], scale, 2));
+          w.w = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c[n], scale, 3));
+          *(uint4*)(tile + put[n] + 4096 * t) = w;
         }
       };
       bool moved = false;
@@ -757,35 +774,47 @@ __global__ __launch_bounds__(512, 2) void latent_kernel(AttendArgs a, int inline
           }
         }
       };
-      // O^T += V^T P^T of step `it`, 16 tokens
-      auto multiply = [&](int it, int t) {
-        v8b pv[RG];
+      // 16 tokens' values and probabilities of step `it`, and O^T += V^T P^T of them
+      struct Operands {
+        v8b v[4], p[RG];
+      };
+      auto operands = [&](int it, int t) {
+        Operands r;
 #pragma unroll
-        for (int r = 0; r < RG; ++r) {
-          uint4 w = *(const uint4*)(weights + (it & 1) * A::kWeights + (t * A::kRows + r * 32 + col) * 32 + half * 16);
-          if (TT > 1 && moved) {   // whole powers of two: exact
-            const float f = power(theirs[r][t / T2], m[r]);
-            auto scaled = [&](uint32_t v) { return mxd::bf16_pair(mx::u2f(v << 16) * f, mx::u2f(v & 0xFFFF0000u) * f); };
-            w = make_uint4(scaled(w.x), scaled(w.y), scaled(w.z), scaled(w.w));
-          }
-          pv[r] = __builtin_bit_cast(v8b, w);
-        }
+        for (int i = 0; i < RG; ++i)
+          r.p[i] = __builtin_bit_cast(v8b, *(const uint4*)(weights + (it & 1) * A::kWeights + (t * A::kRows + i * 32 + col) * 32 + half * 16));
 #pragma unroll
         for (int d = 0; d < 4; ++d) {
           const uint8_t* at = tile + (d & 1 ? get1 : get0) + 128 * (d / 2) + 4096 * t;
           typedef __attribute__((address_space(3))) v4s lds_v4s;
-          v4s w2[2];
-          w2[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)at);
-          w2[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(at + 2048));
-          const v8b vv = __builtin_bit_cast(v8b, w2);
-#pragma unroll
-          for (int r = 0; r < RG; ++r) o[r][d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vv, pv[r], o[r][d], 0, 0, 0);
+          v4s w[2];
+          w[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)at);
+          w[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(at + 2048));
+          r.v[d] = __builtin_bit_cast(v8b, w);
         }
+        return r;
       };
+      auto multiply = [&](Operands& r, int t) {
+        if (TT > 1 && moved) {   // whole powers of two: exact
+#pragma unroll
+          for (int i = 0; i < RG; ++i) {
+            const float f = power(theirs[i][t / T2], m[i]);
+            auto scaled = [&](uint32_t v) { return mxd::bf16_pair(mx::u2f(v << 16) * f, mx::u2f(v & 0xFFFF0000u) * f); };
+            const uint4 w = __builtin_bit_cast(uint4, r.p[i]);
+            r.p[i] = __builtin_bit_cast(v8b, make_uint4(scaled(w.x), scaled(w.y), scaled(w.z), scaled(w.w)));
+          }
+        }
+#pragma unroll
+        for (int d = 0; d < 4; ++d)
+#pragma unroll
+          for (int i = 0; i < RG; ++i) o[i][d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(r.v[d], r.p[i], o[i][d], 0, 0, 0);
+      };
+      int entry = entry_of(lo + (it0 + A::kStages - 1) * A::kStep + 16 * cg);   // of the next copies
+      auto next_entry = [&](int it) { return entry_of(lo + (it + A::kStages) * A::kStep + 16 * cg); };
       // this wave's copies of the step after `it` have landed; those of later steps may be on their way
       auto landed = [&](int it) {
         if (it + A::kStages - 1 < it1) {
-          copy(it + A::kStages - 1);
+          copy(it + A::kStages - 1, entry);
           __builtin_amdgcn_s_waitcnt(mxd::vm_wait_imm(A::kCopies * (A::kStages - 2)));
         } else {
           __builtin_amdgcn_s_waitcnt(mxd::vm_wait_imm(0));
@@ -796,23 +825,42 @@ __global__ __launch_bounds__(512, 2) void latent_kernel(AttendArgs a, int inline
       __builtin_amdgcn_s_waitcnt(mxd::vm_wait_imm(0));
       mxd::copy_barrier();
 #pragma unroll
-      for (int t = 0; t < 4; ++t) convert(it0, t);
+      for (int t = 0; t < 4; ++t) convert(codes_of(it0, t), t);
+      ask(it0 + 1);
+      int asked = next_entry(it0);
       landed(it0);
+      entry = asked;
+      shown = shown_of(it0 + 1);
       mxd::copy_barrier();
       for (int it = it0 + 1; it < it1; ++it) {
+        // everything is read from LDS a turn before it is used: 16 tokens' products, under which the next ones' operands come
+        // and this step's take the place of those just read
+        asked = next_entry(it);
+        Codes next[4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) next[t] = codes_of(it, t);
+        ask(it + 1);
+        Operands now = operands(it - 1, 0);
         settle(it - 1);
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
-          multiply(it - 1, t);
-          if (t > 0) convert(it, t - 1);
+          Operands after;
+          if (t < 3) after = operands(it - 1, t + 1);
+          multiply(now, t);
+          convert(next[t], t);
+          if (t < 3) now = after;
         }
-        convert(it, 3);
         landed(it);
+        entry = asked;
+        shown = shown_of(it + 1);
         mxd::copy_barrier();
       }
       settle(it1 - 1);
 #pragma unroll
-      for (int t = 0; t < 4; ++t) multiply(it1 - 1, t);
+      for (int t = 0; t < 4; ++t) {
+        Operands now = operands(it1 - 1, t);
+        multiply(now, t);
+      }
       __syncthreads();
       __syncthreads();
       if (alone) {
