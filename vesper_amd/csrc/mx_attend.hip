@@ -14,9 +14,10 @@
 //        the values become BF16 (exactly: two significant bits and a power of two) by V_CVT_SCALEF32_PK_BF16_FP4, in the
 //        row order in which they lie, and go through LDS, whose transposing reads give each lane its column's tokens.
 //
-// Work is divided evenly over the device: a unit is the row tile of one sequence and key head, an iteration one step of all
-// the workgroup's token groups, and workgroup g takes the iterations [g per, (g + 1) per) of all units in a row. Units that
-// a workgroup has alone go straight to out; the others' parts go to the workspace and join_kernel adds them up.
+// Work is divided evenly over the device. A unit is the row tile of one sequence and key head; it costs its iterations (a step
+// of all the workgroup's token groups each) and kBegin more for its queries and its way out. Workgroup g takes the costs
+// [g per, (g + 1) per) of all units in a row. Units that a workgroup has alone go straight to out; the others' parts go to
+// the workspace and a second kernel adds them up.
 #include <algorithm>
 #include <type_traits>
 
@@ -34,6 +35,7 @@ typedef mxd::v8i v8i;
 
 constexpr int kCus = 256, kXcds = 8;
 constexpr int kInlineTiles = 1024;   // row tiles of all sequences that every workgroup counts for itself
+constexpr int kBegin = 4;            // what a unit's beginning and end cost, in iterations
 constexpr float kLowest = -3e38f;    // the maximum of a row that has seen nothing yet
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
@@ -100,8 +102,8 @@ __device__ __forceinline__ int tile_iterations(const AttendArgs& a, const Sequen
   return max(1, (hi - lo + step - 1) / step);
 }
 
-// The plan: base[b] = row tiles of the sequences before b, prefix[i] = iterations (of one key head) of the row tiles before
-// i. Made by a workgroup of N threads in its LDS, or by plan_kernel in the workspace.
+// The plan: base[b] = row tiles of the sequences before b, prefix[i] = costs (of one key head) of the row tiles before i.
+// Made by a workgroup of N threads in its LDS, or by plan_kernel in the workspace.
 struct Plan {
   int32_t* base;
   int64_t* prefix;
@@ -168,7 +170,7 @@ __device__ __forceinline__ void make_plan(const AttendArgs& a, Plan p, uint32_t*
     if (i < tiles) {
       const int b = each ? i / each : find(a.q.batch, [&](int k) { return p.base[k] <= i; });
       int lo, hi;
-      n = tile_iterations(a, sequence(a, b), each ? i - b * each : i - p.base[b], rows, step, lo, hi);
+      n = kBegin + tile_iterations(a, sequence(a, b), each ? i - b * each : i - p.base[b], rows, step, lo, hi);
     }
     const int64_t before = scan<N>(n, sums, all);
     if (i < tiles) p.prefix[i] = sum + before;
@@ -193,17 +195,21 @@ __device__ __forceinline__ Sequence uniform(Sequence s) {
   return s;
 }
 
-// A workgroup's way through the units: iterations in the order sequence, key head, row tile.
+// A workgroup's way through the units, in the order sequence, key head, row tile.
 struct Units {
+  int64_t x, end;           // the costs that are the workgroup's, from x on
   int b, h, tile, tiles;    // the unit, and row tiles of its sequence
   Sequence s;
   int lo, hi;               // the tokens that its rows see
-  int64_t unit0, unit1;     // its iterations
+  int64_t unit0;            // its costs begin here
+  int n, it0, it1;          // its iterations, and the workgroup's of them
+  bool first;               // nothing came before it in this workgroup
 };
 
 __device__ __forceinline__ void enter(const AttendArgs& a, Units& u, int rows, int step) {
-  u.unit1 = u.unit0 + uniform(tile_iterations(a, u.s, u.tile, rows, step, u.lo, u.hi));
+  u.n = uniform(tile_iterations(a, u.s, u.tile, rows, step, u.lo, u.hi));
   u.lo = uniform(u.lo), u.hi = uniform(u.hi);
+  u.it0 = (int)larger(u.x - u.unit0 - kBegin, 0), u.it1 = (int)lesser(u.end - u.unit0 - kBegin, u.n);
 }
 
 __device__ __forceinline__ int tiles_of(const AttendArgs& a, const Sequence& s, int rows) {
@@ -211,13 +217,15 @@ __device__ __forceinline__ int tiles_of(const AttendArgs& a, const Sequence& s, 
 }
 
 __device__ __forceinline__ void next_unit(const AttendArgs& a, Units& u, int rows, int step) {
-  u.unit0 = u.unit1;
+  u.first &= u.it1 <= u.it0;
+  u.x = u.unit0 = u.unit0 + kBegin + u.n;
+  if (u.x >= u.end) return;
   if (++u.tile == u.tiles) {
     u.tile = 0;
     if (++u.h == a.cache.heads) {
       u.h = 0;
       do {
-        if (++u.b == a.q.batch) return;   // no iterations are left
+        ++u.b;
         u.s = uniform(sequence(a, u.b));
         u.tiles = tiles_of(a, u.s, rows);
       } while (u.tiles == 0);
@@ -226,36 +234,61 @@ __device__ __forceinline__ void next_unit(const AttendArgs& a, Units& u, int row
   enter(a, u, rows, step);
 }
 
-// The unit of iteration x of `all`: by each thread of N its share of an LDS plan (found: two words), else by halving.
+// in / span, which is below 2^16: the quotient in FP32 is within 1 of it.
+__device__ __forceinline__ int few(int64_t in, int64_t span) {
+  int q = (int)((float)in / (float)span);
+  q -= q * span > in;
+  q += (q + 1) * span <= in;
+  return q;
+}
+
+// Workgroup g's share of the units: where it begins. By each thread of N its share of an LDS plan (found: two words), else
+// by halving. Whether there is anything.
 template <int N>
-__device__ __forceinline__ void first_unit(const AttendArgs& a, const Plan& p, bool in_lds, int64_t x, int32_t* found, Units& u, int rows,
-                                           int step) {
-  const int64_t heads = a.cache.heads;
+__device__ __forceinline__ bool first_unit(const AttendArgs& a, const Plan& p, bool in_lds, int g, int64_t& per, int groups, int32_t* found,
+                                           Units& u, int rows, int step) {
+  const int heads = a.cache.heads;
+  const int64_t all = uniform(p.prefix[uniform(p.base[a.q.batch])]) * heads;
+  per = larger((all + groups - 1) / groups, 1);
+  u.x = lesser(g * per, all), u.end = lesser(u.x + per, all), u.first = true;
+  if (u.x >= u.end) return false;
   if (in_lds) {
     for (int b = threadIdx.x; b < a.q.batch; b += N)
-      if (p.prefix[p.base[b]] * heads <= x && x < p.prefix[p.base[b + 1]] * heads) found[0] = b;
+      if (p.prefix[p.base[b]] * heads <= u.x && u.x < p.prefix[p.base[b + 1]] * heads) found[0] = b;
     __syncthreads();
     u.b = uniform(found[0]);
   } else {
-    u.b = uniform(find(a.q.batch, [&](int b) { return p.prefix[p.base[b]] * heads <= x; }));
+    u.b = uniform(find(a.q.batch, [&](int b) { return p.prefix[p.base[b]] * heads <= u.x; }));
   }
-  const int t0 = uniform(p.base[u.b]), t1 = uniform(p.base[u.b + 1]);
-  const int64_t p0 = uniform(p.prefix[t0]), span = uniform(p.prefix[t1]) - p0, in = x - p0 * heads;
-  u.h = (in | span) >> 32 ? (int)(in / span) : (int)((uint32_t)in / (uint32_t)span);
-  const int64_t rest = in - u.h * span + p0;
-  if (in_lds) {
-    for (int t = t0 + threadIdx.x; t < t1; t += N)
-      if (p.prefix[t] <= rest && rest < p.prefix[t + 1]) found[1] = t;
-    __syncthreads();
-    u.tile = uniform(found[1]) - t0;
-  } else {
-    u.tile = uniform(find(t1 - t0, [&](int t) { return p.prefix[t0 + t] <= rest; }));
-  }
-  u.h = uniform(u.h);
-  u.unit0 = x - (rest - uniform(p.prefix[t0 + u.tile]));
   u.s = uniform(sequence(a, u.b));
-  u.tiles = tiles_of(a, u.s, rows);
+  const int t0 = uniform(p.base[u.b]), t1 = uniform(p.base[u.b + 1]);
+  const int64_t p0 = uniform(p.prefix[t0]), span = uniform(p.prefix[t1]) - p0, in = u.x - p0 * heads;
+  u.h = uniform(few(in, span));
+  const int64_t rest = in - u.h * span + p0;
+  u.tile = 0, u.tiles = t1 - t0;
+  if (u.tiles > 1) {
+    if (in_lds) {
+      for (int t = t0 + threadIdx.x; t < t1; t += N)
+        if (p.prefix[t] <= rest && rest < p.prefix[t + 1]) found[1] = t;
+      __syncthreads();
+      u.tile = uniform(found[1]) - t0;
+    } else {
+      u.tile = uniform(find(t1 - t0, [&](int t) { return p.prefix[t0 + t] <= rest; }));
+    }
+  }
+  u.unit0 = u.x - (rest - uniform(p.prefix[t0 + u.tile]));
   enter(a, u, rows, step);
+  return true;
+}
+
+// The unit's end in this workgroup: `alone` it has all of it. The workgroup's last unit, if it began it and does not end it,
+// is joined from there on.
+__device__ __forceinline__ bool is_alone(const Units& u) { return u.it0 == 0 && u.it1 == u.n; }
+__device__ __forceinline__ void note(const Units& u, int64_t per, int g, Shared* shared) {
+  Shared v{u.b, u.h, u.tile, 0, u.first ? 0 : 1};
+  const int64_t end = u.unit0 + kBegin + u.n;
+  if (u.it0 == 0 && u.it1 > 0 && u.it1 < u.n) v.parts = few(end - 1, per) - g + 1;
+  *shared = v;
 }
 
 // Two E4M3 terms of 16 query values (BF16 pairs w) under the scale 2^(exponent - 127), which takes them into [-256, 256]:
@@ -473,23 +506,28 @@ __global__ __launch_bounds__(512, 2) void latent_kernel(AttendArgs a, int inline
     plan = {(int32_t*)(lds + 8 * (kInlineTiles + 1)), (int64_t*)lds};
     make_plan<512>(a, plan, sums, A::kRows, A::kStep);
   }
-  const int64_t all = uniform(plan.prefix[plan.base[a.q.batch]]) * a.cache.heads;
-  const int64_t per = larger((all + kCus - 1) / kCus, 1);
   // workgroups go round the XCDs: neighbours in the work, which share keys, to one L2
   const int g = (int)(blockIdx.x % kXcds) * (kCus / kXcds) + (int)blockIdx.x / kXcds;
-  int64_t x = lesser(g * per, all);
-  const int64_t end = lesser(x + per, all);
   Shared* shared = (Shared*)(a.space + a.at.units) + g;
-  if (x >= end) {
+  int64_t per;
+  Units u;
+  if (!first_unit<512>(a, plan, inline_plan, g, per, kCus, found, u, A::kRows, A::kStep)) {
     if (tid == 0) shared->parts = 0;
     return;
   }
-  Units u;
-  first_unit<512>(a, plan, inline_plan, x, found, u, A::kRows, A::kStep);
 
   const int spread = 2 * (l16 & 3) + ((l16 >> 2) & 1);   // pieces of 16 bytes of neighbouring tokens' values lie apart
+  auto go_on = [&] {   // to the next unit, if there is one
+    if (u.end <= u.unit0 + kBegin + u.n && tid == 0) note(u, per, g, shared);
+    next_unit(a, u, A::kRows, A::kStep);
+    return u.x < u.end;
+  };
   for (;;) {
-    const int it0 = (int)(x - u.unit0), it1 = (int)(lesser(u.unit1, end) - u.unit0);
+    if (u.it1 <= u.it0) {   // only what the unit's beginning costs is this workgroup's
+      if (!go_on()) return;
+      continue;
+    }
+    const int it0 = u.it0, it1 = u.it1;
     const int lo = u.lo, hi = u.hi, h = u.h;
     const int rows = u.s.n * a.group;   // at most 2^30
     const int row0 = u.tile * A::kRows, row = min(row0 + rq * 16 + l16, rows - 1);
@@ -539,12 +577,15 @@ __global__ __launch_bounds__(512, 2) void latent_kernel(AttendArgs a, int inline
         if (lane < 16) mxd::global_to_lds4(scales + lane * scale_pitch(WK) + 16, stage + A::kTailScales + 64 * cg);
       }
     };
+    ask(it0);
     if (wave >= 4) {
+      int first_entries[A::kStages - 1];
+#pragma unroll
+      for (int k = 0; k < A::kStages - 1; ++k) first_entries[k] = entry_of(lo + (it0 + k) * A::kStep + 16 * cg);
 #pragma unroll
       for (int k = 0; k < A::kStages - 1; ++k)
-        if (it0 + k < it1) copy(it0 + k, entry_of(lo + (it0 + k) * A::kStep + 16 * cg));
+        if (it0 + k < it1) copy(it0 + k, first_entries[k]);
     }
-    ask(it0);
     uint32_t shown = shown_of(it0);
     // -- the queries, converted and exchanged --
     uint4* made = (uint4*)lds + rq * A::kMade + lane;
@@ -564,8 +605,8 @@ __global__ __launch_bounds__(512, 2) void latent_kernel(AttendArgs a, int inline
       }
       made_scales[k * 64] = s.scales;
     }
-    const bool alone = x == u.unit0 && u.unit1 <= end;
-    const int64_t slot = 2 * g + (g * per < u.unit0 ? 1 : 0);
+    const bool alone = is_alone(u);
+    const int64_t slot = 2 * g + (u.first ? 0 : 1);
 
     if (wave < 4) {
       mxd::lds_barrier();
@@ -899,16 +940,7 @@ __global__ __launch_bounds__(512, 2) void latent_kernel(AttendArgs a, int inline
               part[((r * 4 + d) * 4 + n) * 64] = make_float4(o[r][d][4 * n], o[r][d][4 * n + 1], o[r][d][4 * n + 2], o[r][d][4 * n + 3]);
       }
     }
-    if (u.unit1 >= end) {   // the workgroup's last: it joins the unit if it began it and does not end it
-      if (tid == 0) {
-        Shared v{u.b, h, u.tile, 0, (int)(slot & 1)};
-        if (!alone && x == u.unit0) v.parts = (int)((u.unit1 - 1) / per - g + 1);
-        *shared = v;
-      }
-      return;
-    }
-    x = u.unit1;
-    next_unit(a, u, A::kRows, A::kStep);
+    if (!go_on()) return;
     __syncthreads();   // what went out has been read before the next unit's copies and queries come
   }
 }
@@ -948,20 +980,16 @@ __global__ __launch_bounds__(256, (Grouped<W, RG>::kWaves)) void grouped_kernel(
     plan = {(int32_t*)(lds + 8 * (kInlineTiles + 1)), (int64_t*)lds};
     make_plan<256>(a, plan, sums, A::kRows, A::kStep);
   }
-  const int64_t all = uniform(plan.prefix[plan.base[a.q.batch]]) * a.cache.heads;
   constexpr int groups = A::kGroups;
-  const int64_t per = larger((all + groups - 1) / groups, 1);
   // workgroups go round the XCDs: neighbours in the work, which share keys, to one L2
   const int g = (int)(blockIdx.x % kXcds) * (groups / kXcds) + (int)blockIdx.x / kXcds;
-  int64_t x = lesser(g * per, all);
-  const int64_t end = lesser(x + per, all);
   Shared* shared = (Shared*)(a.space + a.at.units) + g;
-  if (x >= end) {
+  int64_t per;
+  Units u;
+  if (!first_unit<256>(a, plan, inline_plan, g, per, groups, found, u, A::kRows, A::kStep)) {
     if (tid == 0) shared->parts = 0;
     return;
   }
-  Units u;
-  first_unit<256>(a, plan, inline_plan, x, found, u, A::kRows, A::kStep);
 
   // LDS places: a loader's 16-byte pieces of its token, and a reader's 8 bytes; pieces of neighbouring tokens lie apart
   const int spread = 2 * (col & 3) + ((col >> 2) & 1);
@@ -972,8 +1000,17 @@ __global__ __launch_bounds__(256, (Grouped<W, RG>::kWaves)) void grouped_kernel(
   const uint32_t get0 = tg * A::kTile + (4 * half + rt) * (2 * W) + ((2 * ((lane >> 4) & 1) + rc / 2) ^ rs) * 16 + (rc & 1) * 8;
   const uint32_t get1 = get0 ^ 64;
 
+  auto go_on = [&] {   // to the next unit, if there is one
+    if (u.end <= u.unit0 + kBegin + u.n && tid == 0) note(u, per, g, shared);
+    next_unit(a, u, A::kRows, A::kStep);
+    return u.x < u.end;
+  };
   for (;;) {
-    const int it0 = (int)(x - u.unit0), it1 = (int)(lesser(u.unit1, end) - u.unit0);
+    if (u.it1 <= u.it0) {   // only what the unit's beginning costs is this workgroup's
+      if (!go_on()) return;
+      continue;
+    }
+    const int it0 = u.it0, it1 = u.it1;
     // -- the wave's query rows --
     const int rows = u.s.n * a.group;   // at most 2^30
     const int row0 = u.tile * A::kRows + rg * 32, row = min(row0 + col, rows - 1);
@@ -1171,8 +1208,8 @@ __global__ __launch_bounds__(256, (Grouped<W, RG>::kWaves)) void grouped_kernel(
     l = halves_sum(l);
     if (half == 0) stats[wave][col][0] = m, stats[wave][col][1] = l;
     __syncthreads();   // and everybody has read its values
-    const bool alone = x == u.unit0 && u.unit1 <= end;
-    const int64_t slot = 2 * g + (g * per < u.unit0 ? 1 : 0);
+    const bool alone = is_alone(u);
+    const int64_t slot = 2 * g + (u.first ? 0 : 1);
     float most = kLowest, all_l = 0.f;
 #pragma unroll
     for (int t = 0; t < TG; ++t) most = fmaxf(most, stats[t * RG + rg][col][0]);
@@ -1241,50 +1278,46 @@ __global__ __launch_bounds__(256, (Grouped<W, RG>::kWaves)) void grouped_kernel(
         __syncthreads();
       }
     }
-    if (u.unit1 >= end) {   // the workgroup's last: it joins the unit if it began it and does not end it
-      if (tid == 0) {
-        Shared v{u.b, h, u.tile, 0, (int)(slot & 1)};
-        if (!alone && x == u.unit0) v.parts = (int)((u.unit1 - 1) / per - g + 1);
-        *shared = v;
-      }
-      return;
-    }
-    x = u.unit1;
-    next_unit(a, u, A::kRows, A::kStep);
+    if (!go_on()) return;
   }
 }
 
-// The units that several workgroups had. A workgroup takes pieces of 64 times four values, of all units in turn: its waves
-// add up every fourth part each. Which units there are it finds in the workgroups' last units, all of them at once.
+// The units that several workgroups had, in pieces of 64 times four values. Where there are more waves than pieces a
+// workgroup's waves share a piece's parts; else each takes a piece. Every wave finds the units for itself, in the
+// workgroups' last ones, all of them at once.
 //
 // piece(e, r, c): the row and first column of the e-th four values of a unit, as its parts have them.
 template <int kGroups, int kRows, int WV, typename Piece>
 __device__ __forceinline__ void join(const AttendArgs& a, Piece piece) {
-  __shared__ Shared list[kGroups];
-  __shared__ int32_t from[kGroups];
-  __shared__ uint32_t counts[4];
   __shared__ float4 sums[4][64];
   __shared__ float2 tops[4][64];
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  constexpr int kLook = kGroups / 64, kPieces = kRows * WV / 256;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const Shared* units = (const Shared*)(a.space + a.at.units);
+  uint64_t masks[kLook];
   int n = 0;
-  for (int g0 = 0; g0 < kGroups; g0 += 256) {
-    const Shared s = ((const Shared*)(a.space + a.at.units))[g0 + tid];
-    const uint64_t mask = __ballot(s.parts > 1);
-    if (lane == 0) counts[wave] = __popcll(mask);
-    __syncthreads();
-    int at = n + __popcll(mask & ((1ull << lane) - 1));
-    for (int w = 0; w < 4; ++w) {
-      at += w < wave ? counts[w] : 0;
-      n += counts[w];
-    }
-    if (s.parts > 1) list[at] = s, from[at] = g0 + tid;
-    __syncthreads();
-  }
-  constexpr int kPieces = kRows * WV / 256;
+#pragma unroll
+  for (int j = 0; j < kLook; ++j) masks[j] = __ballot(units[64 * j + lane].parts > 1);
+#pragma unroll
+  for (int j = 0; j < kLook; ++j) n += __popcll(masks[j]);
+  const bool together = n * kPieces < (int)gridDim.x * 2;
+  const int stride = together ? (int)gridDim.x : 4 * (int)gridDim.x;
   const float4* parts = (const float4*)(a.space + a.at.rows);
-  for (int k = blockIdx.x; k < n * kPieces; k += gridDim.x) {
-    const Shared s = list[k / kPieces];
-    const int g = from[k / kPieces], e = k % kPieces * 64 + lane;
+  for (int k = together ? (int)blockIdx.x : (int)blockIdx.x * 4 + wave; k < n * kPieces; k += stride) {
+    int nth = k / kPieces, g = 0;   // the nth set bit
+#pragma unroll
+    for (int j = 0; j < kLook; ++j) {
+      const int here = __popcll(masks[j]);
+      if (nth >= 0 && nth < here) {
+        uint64_t m = masks[j];
+        for (; nth > 0; --nth) m &= m - 1;
+        g = 64 * j + __builtin_ctzll(m);
+        nth = -1;
+      }
+      nth -= nth >= 0 ? here : 0;
+    }
+    const Shared s = units[g];
+    const int e = k % kPieces * 64 + lane;
     int r, c;
     piece(e, r, c);
     const float2* stats = (const float2*)(a.space + a.at.stats) + r;
@@ -1292,32 +1325,35 @@ __device__ __forceinline__ void join(const AttendArgs& a, Piece piece) {
     auto slot = [&](int i) { return (int64_t)2 * (g + i) + (i ? 0 : s.slot); };
     float most = kLowest, sum = 0.f;
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int i0 = wave; i0 < s.parts; i0 += 16) {   // four at a time
-      float2 st[4];
-      float4 p[4];
+    auto add = [&](int i0, int step) {   // eight parts at a time
+      float2 st[8];
+      float4 p[8];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int64_t at = slot(min(i0 + 4 * j, s.parts - 1));
+      for (int j = 0; j < 8; ++j) {
+        const int64_t at = slot(min(i0 + step * j, s.parts - 1));
         st[j] = stats[at * kRows];
         p[j] = parts[at * (kRows * WV / 4) + e];
       }
       float next = most;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) next = fmaxf(next, st[j].x);
+      for (int j = 0; j < 8; ++j) next = fmaxf(next, st[j].x);
       const float by = power(most, next);
       most = next, sum *= by;
       v.x *= by, v.y *= by, v.z *= by, v.w *= by;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (i0 + 4 * j >= s.parts) break;
-        const float f = power(st[j].x, most);
-        sum += st[j].y * f;
-        v.x += p[j].x * f, v.y += p[j].y * f, v.z += p[j].z * f, v.w += p[j].w * f;
+      for (int j = 0; j < 8; ++j) {
+        const float f = i0 + step * j < s.parts ? power(st[j].x, most) : 0.f;
+        const bool use = i0 + step * j < s.parts;   // (not by a factor of zero: a part may hold NaN)
+        sum += use ? st[j].y * f : 0.f;
+        v.x += use ? p[j].x * f : 0.f, v.y += use ? p[j].y * f : 0.f, v.z += use ? p[j].z * f : 0.f, v.w += use ? p[j].w * f : 0.f;
       }
-    }
-    sums[wave][lane] = v, tops[wave][lane] = make_float2(most, sum);
-    __syncthreads();
-    if (wave == 0) {
+    };
+    if (together) {
+      for (int i0 = wave; i0 < s.parts; i0 += 32) add(i0, 4);
+      __syncthreads();
+      sums[wave][lane] = v, tops[wave][lane] = make_float2(most, sum);
+      __syncthreads();
+      if (wave) continue;
 #pragma unroll
       for (int w = 1; w < 4; ++w) most = fmaxf(most, tops[w][lane].x);
       sum = 0.f, v = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -1328,19 +1364,19 @@ __device__ __forceinline__ void join(const AttendArgs& a, Piece piece) {
         sum += tops[w][lane].y * f;
         v.x += p.x * f, v.y += p.y * f, v.z += p.z * f, v.w += p.w * f;
       }
-      const Sequence q = sequence(a, s.b);
-      const int row = s.tile * kRows + r;
-      if (row < q.n * a.group) {
-        const int head = s.h * a.group + row % a.group;
-        const int64_t token = q.first + row / a.group;
-        const RowOut f = row_out(a, head, most, sum);
-        uint2 w;
-        w.x = mxd::bf16_pair(v.x * f.inv, v.y * f.inv), w.y = mxd::bf16_pair(v.z * f.inv, v.w * f.inv);
-        *(uint2*)(a.q.out + token * a.q.out_stride + (int64_t)head * WV + c) = w;
-        if (a.q.lse && c == 0) a.q.lse[token * a.q.heads + head] = f.lse;
-      }
+    } else {
+      for (int i0 = 0; i0 < s.parts; i0 += 8) add(i0, 1);
     }
-    __syncthreads();
+    const Sequence q = sequence(a, s.b);
+    const int row = s.tile * kRows + r;
+    if (row >= q.n * a.group) continue;
+    const int head = s.h * a.group + row % a.group;
+    const int64_t token = q.first + row / a.group;
+    const RowOut f = row_out(a, head, most, sum);
+    uint2 w;
+    w.x = mxd::bf16_pair(v.x * f.inv, v.y * f.inv), w.y = mxd::bf16_pair(v.z * f.inv, v.w * f.inv);
+    *(uint2*)(a.q.out + token * a.q.out_stride + (int64_t)head * WV + c) = w;
+    if (a.q.lse && c == 0) a.q.lse[token * a.q.heads + head] = f.lse;
   }
 }
 
