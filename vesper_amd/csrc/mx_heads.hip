@@ -14,116 +14,153 @@ namespace {
 using namespace mxh;
 
 constexpr int kMaxTokens = 1 << 20, kMaxWidth = 4096;
-constexpr int kGradBlocks = 512;   // workgroups of one set of heads that add up dweight
+constexpr int kGradBlocks = 1024;   // workgroups that add up dweight, of both sets together
+
+// A piece is K heads of one token and set on a group of L lanes: its rows are asked for at once, its angles and weights once.
+struct Pieces {
+  int of[2];   // of a token, by set
+  __host__ __device__ int per_token() const { return of[0] + of[1]; }
+};
 
 struct HeadsArgs {
   mx_heads set[2];
-  int heads;           // of both sets
-  int64_t rows;        // tokens * heads
+  Pieces n;
+  int tokens;
   mx_rotation rot;
-  int x_type, y_type;
+  int y_type;
   bool wide;
-  int from, to;        // the columns that the call touches
+  int from, to;   // the columns that the call touches
 };
 
-template <int L, int NI>
+template <int L, int NI, int K, bool F32>
 __global__ __launch_bounds__(256) void rotate_kernel(HeadsArgs a) {
   const int g = threadIdx.x % L;
-  const int64_t step = (int64_t)gridDim.x * (256 / L);
-  for (int64_t r = (int64_t)blockIdx.x * (256 / L) + threadIdx.x / L; r < a.rows; r += step) {
-    const uint32_t t = (uint32_t)r / (uint32_t)a.heads;
-    int h = (uint32_t)r - t * (uint32_t)a.heads;
-    const float* angles = nullptr;
-    if (!place_of(a.rot, t, angles)) continue;
-    const int second = h >= a.set[0].heads;
+  const uint32_t each = a.n.per_token(), pieces = (uint32_t)a.tokens * each;
+  for (uint32_t first = blockIdx.x * (256 / L); first < pieces; first += gridDim.x * (256 / L)) {
+    const uint32_t mine = first + threadIdx.x / L, p = min(mine, pieces - 1), t = p / each;
+    const int j = p - t * each;
+    const bool second = j >= a.n.of[0];
     const mx_heads& s = a.set[second];
-    h -= second ? a.set[0].heads : 0;
-    const int64_t xe = a.x_type == MX_ROWS_F32 ? 4 : 2, ye = a.y_type == MX_ROWS_F32 ? 4 : 2;
-    const void* x = (const uint8_t*)s.x + (t * s.x_stride + (int64_t)h * a.rot.width) * xe;
-    void* y = (uint8_t*)s.y + (t * s.y_stride + (int64_t)h * a.rot.width) * ye;
-    float v[NI][8];
-    normalized_row<L, NI>(x, a.x_type, a.wide, a.rot, angles, s.weight, a.from, a.to, g, v);
+    const int h = (second ? j - a.n.of[0] : j) * K;
+    const int64_t xe = F32 ? 4 : 2, ye = a.y_type == MX_ROWS_F32 ? 4 : 2;
+    const uint8_t* x = (const uint8_t*)s.x + (t * s.x_stride + (int64_t)h * a.rot.width) * xe;
+    uint8_t* y = (uint8_t*)s.y + (t * s.y_stride + (int64_t)h * a.rot.width) * ye;
+    const int heads = s.heads - h;   // of the piece, if below K
+    Raw8<F32> raw[K][NI];
 #pragma unroll
-    for (int i = 0; i < NI; ++i) {
-      const int c = a.from + 8 * (i * L + g);
-      if (c < a.to) store8(y, a.y_type, a.wide, c, v[i]);
+    for (int k = 0; k < K; ++k) load_row<L, NI>(x + (int64_t)min(k, heads - 1) * a.rot.width * xe, a.wide, a.from, a.to, g, raw[k]);
+    Columns<NI> cols;
+    const float* angles = nullptr;
+    const bool live = place_of(a.rot, t, angles) && mine < pieces;
+    weights_of<L>(a.rot, s.weight, a.from, g, cols);
+    angles_of<L>(a.rot, angles, a.from, a.to, g, cols);
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      float v[NI][8];
+      finish_row<L, NI>(x + (int64_t)min(k, heads - 1) * a.rot.width * xe, a.wide, a.rot, cols, a.from, g, raw[k], v);
+      if (!live || k >= heads) continue;
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+        const int c = a.from + 8 * (i * L + g);
+        if (c < a.to) store8(y + (int64_t)k * a.rot.width * ye, a.y_type, a.wide, c, v[i]);
+      }
     }
   }
 }
 
 struct GradArgs {
   mx_heads_grad set[2];
+  Pieces n;
   int tokens;
   mx_rotation rot;
-  int type;
   bool wide;
-  float* parts;   // [2][kGradBlocks][norm]
+  int blocks[2];   // workgroups of each set
+  float* parts;    // [blocks[0] + blocks[1]][norm]
 };
 
-// blockIdx.y: the set. A lane keeps its columns' sums for dweight over its rows; the workgroup's go to parts.
-template <int L, int NI>
+// The first blocks[0] workgroups have the first set. A lane keeps its columns' sums for dweight over its rows; the
+// workgroup's go to parts.
+template <int L, int NI, int K, bool F32>
 __global__ __launch_bounds__(256) void rotate_backward_kernel(GradArgs a) {
   extern __shared__ float sums[];   // [256 / L][8 L NI] where dweight is asked for
-  const mx_heads_grad& s = a.set[blockIdx.y];
+  const bool second = (int)blockIdx.x >= a.blocks[0];
+  const mx_heads_grad& s = a.set[second];
   const int g = threadIdx.x % L, norm = a.rot.norm, width = a.rot.width;
-  const int64_t size = a.type == MX_ROWS_F32 ? 4 : 2;
+  constexpr int64_t size = F32 ? 4 : 2;
+  constexpr int type = F32 ? MX_ROWS_F32 : MX_ROWS_BF16;
   const float sign = a.rot.inverse ? 1.f : -1.f;   // R^T turns back
+  Columns<NI> cols;
+  weights_of<L>(a.rot, s.weight, 0, g, cols);
   float dw[NI][8] = {};
-  const int64_t rows = (int64_t)a.tokens * s.heads, step = (int64_t)gridDim.x * (256 / L);
-  for (int64_t r = (int64_t)blockIdx.x * (256 / L) + threadIdx.x / L; r < rows; r += step) {
-    const uint32_t t = (uint32_t)r / (uint32_t)s.heads;
-    const int64_t head = (int64_t)((uint32_t)r - t * (uint32_t)s.heads) * width;
-    const uint8_t* dy = (const uint8_t*)s.dy + (t * s.dy_stride + head) * size;
-    const uint8_t* x = (const uint8_t*)s.x + (t * s.x_stride + head) * size;
-    uint8_t* dx = (uint8_t*)s.dx + (t * s.dx_stride + head) * size;
+  const uint32_t each = a.n.of[second], pieces = (uint32_t)a.tokens * each, block = blockIdx.x - (second ? a.blocks[0] : 0);
+  for (uint32_t first = block * (256 / L); first < pieces; first += a.blocks[second] * (256 / L)) {
+    const uint32_t mine = first + threadIdx.x / L, p = min(mine, pieces - 1), t = p / each;
+    const int h = (p - t * each) * K, heads = s.heads - h;
+    const uint8_t* dy = (const uint8_t*)s.dy + (t * s.dy_stride + (int64_t)h * width) * size;
+    const uint8_t* x = (const uint8_t*)s.x + (t * s.x_stride + (int64_t)h * width) * size;
+    uint8_t* dx = (uint8_t*)s.dx + (t * s.dx_stride + (int64_t)h * width) * size;
+    Raw8<F32> raw_d[K][NI], raw_x[K][NI];
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int64_t at = (int64_t)min(k, heads - 1) * width * size;
+      load_row<L, NI>(dy + at, a.wide, 0, width, g, raw_d[k]);
+      load_row<L, NI>(x + at, a.wide, 0, norm, g, raw_x[k]);
+    }
     const float* angles = nullptr;
-    const bool live = place_of(a.rot, t, angles);
-    float d[NI][8], u[NI][8];
-    double sum = 0;
+    const bool there = mine < pieces, live = place_of(a.rot, t, angles) && there;
+    angles_of<L>(a.rot, angles, 0, width, g, cols);
 #pragma unroll
-    for (int i = 0; i < NI; ++i) {
-      const int c = 8 * (i * L + g);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) d[i][j] = u[i][j] = 0.f;
-      if (c >= width || !live) continue;
-      load8(dy, a.type, a.wide, c, d[i]);
-      if (c < norm) load8(x, a.type, a.wide, c, u[i]);
-    }
-#pragma unroll
-    for (int i = 0; i < NI; ++i) {
-      const int c = 8 * (i * L + g);
-      if (c < width && live) turn8(a.rot, angles, sign, c, d[i], [&](int at, float (&p)[8]) { load8(dy, a.type, a.wide, at, p); });
-#pragma unroll
-      for (int j = 0; j < 8; ++j) sum = fma((double)u[i][j], (double)u[i][j], sum);
-    }
-    if (norm) {
-      const float r = root(group_sum<L>(sum), norm, a.rot.eps);
-      float dot = 0.f;
+    for (int k = 0; k < K; ++k) {
+      const bool counts = live && k < heads;   // (a select, not a factor: what does not count may hold NaN)
+      float d[NI][8], u[NI][8];
+      double sum = 0;
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
-        const int c = 8 * (i * L + g);
-        if (c >= norm) continue;
-        float w[8];
-        weights8(s.weight, c, w);
+        values(raw_d[k][i], d[i]), values(raw_x[k][i], u[i]);
+        if (__all(counts)) continue;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          u[i][j] *= r;
-          dw[i][j] += d[i][j] * u[i][j];
-          d[i][j] *= w[j];
-          dot += d[i][j] * u[i][j];
+        for (int j = 0; j < 8; ++j) d[i][j] = counts ? d[i][j] : 0.f, u[i][j] = counts ? u[i][j] : 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+        turn8(a.rot, cols.a[i], sign, d[i], [&](float (&q)[8]) {
+          if constexpr (NI == 1) {
+            partner_lane<L>(a.rot, cols.a[0], g, d[0], q);
+          } else if (cols.a[i].on) {   // (from memory once more)
+            values(load_raw<F32>(dy, a.wide, 8 * (i * L + g) + (cols.a[i].low ? a.rot.dims / 2 : -(a.rot.dims / 2))), q);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) q[j] = counts ? q[j] : 0.f;
+          }
+        });
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sum = fma((double)u[i][j], (double)u[i][j], sum);
+      }
+      if (norm) {
+        const float r = root(group_sum<L>(sum), norm, a.rot.eps);
+        float dot = 0.f;
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+          if (!cols.normed[i]) continue;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            u[i][j] *= r;
+            dw[i][j] += d[i][j] * u[i][j];
+            d[i][j] *= cols.w[i][j];
+            dot += d[i][j] * u[i][j];
+          }
         }
-      }
-      const float mean = group_sum<L>(dot) / norm;
+        const float mean = group_sum<L>(dot) / norm;
 #pragma unroll
-      for (int i = 0; i < NI; ++i) {
-        if (8 * (i * L + g) >= norm) continue;
+        for (int i = 0; i < NI; ++i)
+          if (cols.normed[i])
 #pragma unroll
-        for (int j = 0; j < 8; ++j) d[i][j] = r * (d[i][j] - u[i][j] * mean);
+            for (int j = 0; j < 8; ++j) d[i][j] = r * (d[i][j] - u[i][j] * mean);
       }
+      if (!there || k >= heads) continue;
+#pragma unroll
+      for (int i = 0; i < NI; ++i)
+        if (8 * (i * L + g) < width) store8(dx + (int64_t)k * width * size, type, a.wide, 8 * (i * L + g), d[i]);
     }
-#pragma unroll
-    for (int i = 0; i < NI; ++i)
-      if (8 * (i * L + g) < width) store8(dx, a.type, a.wide, 8 * (i * L + g), d[i]);
   }
   if (!s.dweight) return;
 #pragma unroll
@@ -131,7 +168,7 @@ __global__ __launch_bounds__(256) void rotate_backward_kernel(GradArgs a) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) sums[threadIdx.x / L * (8 * L * NI) + 8 * (i * L + g) + j] = dw[i][j];
   __syncthreads();
-  float* part = a.parts + ((int64_t)blockIdx.y * kGradBlocks + blockIdx.x) * norm;
+  float* part = a.parts + (int64_t)blockIdx.x * norm;
   for (int c = threadIdx.x; c < norm; c += 256) {
     float v = 0.f;
 #pragma unroll 4
@@ -140,23 +177,43 @@ __global__ __launch_bounds__(256) void rotate_backward_kernel(GradArgs a) {
   }
 }
 
-// dweight from the workgroups' parts: 16 rows of 64 columns add up every 16th part.
-__global__ __launch_bounds__(1024) void dweight_kernel(GradArgs a, int blocks) {
-  __shared__ float sums[16][64];
-  float* out = a.set[blockIdx.y].dweight;
+// dweight from the workgroups' parts, 32 columns a workgroup: 128 rows of eight lanes, eight parts in flight each.
+__global__ __launch_bounds__(1024) void dweight_kernel(GradArgs a) {
+  __shared__ float4 sums[16][8];
+  const int set = blockIdx.y, norm = a.rot.norm;
+  float* out = a.set[set].dweight;
   if (!out) return;
-  const int c = blockIdx.x * 64 + threadIdx.x % 64, k = threadIdx.x / 64;
-  const float* part = a.parts + (int64_t)blockIdx.y * kGradBlocks * a.rot.norm;
-  float v = 0.f;
-  if (c < a.rot.norm)
-    for (int b = k; b < blocks; b += 16) v += part[(int64_t)b * a.rot.norm + c];
-  sums[k][threadIdx.x % 64] = v;
-  __syncthreads();
-  if (k == 0 && c < a.rot.norm) {
+  const int lane = threadIdx.x & 7, c = blockIdx.x * 32 + 4 * lane, blocks = a.blocks[set];
+  const float* part = a.parts + (int64_t)(set ? a.blocks[0] : 0) * norm + min(c, norm - 4);
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int b0 = threadIdx.x / 8; b0 < blocks; b0 += 1024) {
+    float4 p[8];
 #pragma unroll
-    for (int i = 1; i < 16; ++i) v += sums[i][threadIdx.x];
-    out[c] = v;
+    for (int i = 0; i < 8; ++i) p[i] = *(const float4*)(part + (int64_t)min(b0 + 128 * i, blocks - 1) * norm);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (b0 + 128 * i < blocks) v.x += p[i].x, v.y += p[i].y, v.z += p[i].z, v.w += p[i].w;
   }
+#pragma unroll
+  for (int m = 8; m < 64; m <<= 1)
+    v.x += __shfl_xor(v.x, m, 64), v.y += __shfl_xor(v.y, m, 64), v.z += __shfl_xor(v.z, m, 64), v.w += __shfl_xor(v.w, m, 64);
+  if ((threadIdx.x & 63) < 8) sums[threadIdx.x / 64][lane] = v;
+  __syncthreads();
+  if (threadIdx.x >= 8 || c >= norm) return;
+#pragma unroll
+  for (int i = 1; i < 16; ++i) v.x += sums[i][lane].x, v.y += sums[i][lane].y, v.z += sums[i][lane].z, v.w += sums[i][lane].w;
+  out[c] = v.x, out[c + 1] = v.y, out[c + 2] = v.z, out[c + 3] = v.w;
+}
+
+// fn(K, F32) for a call's rows: four heads a piece where that still leaves every SIMD four waves.
+template <int L, int NI, typename F>
+int by_piece(int64_t rows, bool f32, F fn) {
+  using std::integral_constant;
+  using std::bool_constant;
+  if constexpr (NI == 1) {
+    if (rows * L / 64 >= 4 * 16 * 256) return f32 ? fn(integral_constant<int, 4>(), bool_constant<true>()) : fn(integral_constant<int, 4>(), bool_constant<false>());
+  }
+  return f32 ? fn(integral_constant<int, 1>(), bool_constant<true>()) : fn(integral_constant<int, 1>(), bool_constant<false>());
 }
 
 int check_type(const char* who, int32_t type) {
@@ -212,7 +269,7 @@ int mx_rotate_heads(mx_ctx* ctx, const mx_heads* sets, int32_t n_sets, int32_t t
   if (int s = check_type(who, x_type)) return s;
   if (int s = check_type(who, y_type)) return s;
   HeadsArgs a{};
-  a.heads = (int)heads, a.rows = tokens * heads, a.rot = *rotation, a.x_type = x_type, a.y_type = y_type;
+  a.tokens = tokens, a.rot = *rotation, a.y_type = y_type;
   a.to = rotation->width;
   const int64_t xe = x_type == MX_ROWS_F32 ? 4 : 2, ye = y_type == MX_ROWS_F32 ? 4 : 2;
   bool wide = true, in_place = true;
@@ -234,29 +291,34 @@ int mx_rotate_heads(mx_ctx* ctx, const mx_heads* sets, int32_t n_sets, int32_t t
   if (!tokens || a.to == a.from) return MX_OK;
   return mxh::by_lanes(a.to - a.from, [&](auto l, auto n) {
     constexpr int L = decltype(l)::value, NI = decltype(n)::value;
-    const unsigned grid = (unsigned)std::min<int64_t>((a.rows + 256 / L - 1) / (256 / L), 1 << 14);
-    hipLaunchKernelGGL((rotate_kernel<L, NI>), dim3(grid), dim3(256), 0, as_stream(stream), a);
-    MX_LAUNCH_CHECK("rotate_kernel");
-    return MX_OK;
+    return by_piece<L, NI>(tokens * heads, x_type == MX_ROWS_F32, [&](auto k, auto f32) {
+      constexpr int K = decltype(k)::value;
+      for (int i = 0; i < n_sets; ++i) a.n.of[i] = (sets[i].heads + K - 1) / K;
+      const int64_t pieces = (int64_t)tokens * a.n.per_token();
+      const unsigned grid = (unsigned)std::min<int64_t>((pieces + 256 / L - 1) / (256 / L), 1 << 16);
+      hipLaunchKernelGGL((rotate_kernel<L, NI, K, decltype(f32)::value>), dim3(grid), dim3(256), 0, as_stream(stream), a);
+      MX_LAUNCH_CHECK("rotate_kernel");
+      return MX_OK;
+    });
   });
 }
 
 uint64_t mx_rotate_heads_workspace_bytes(int32_t norm) {
   if (norm < 0 || norm > kMaxWidth) return 0;
-  return 2ull * kGradBlocks * norm * sizeof(float);
+  return (uint64_t)kGradBlocks * norm * sizeof(float);
 }
 
 int mx_rotate_heads_backward(mx_ctx* ctx, const mx_heads_grad* sets, int32_t n_sets, int32_t tokens, const mx_rotation* rotation,
                              int32_t type, void* workspace, uint64_t workspace_bytes, void* stream) {
   const char* who = "mx_rotate_heads_backward";
   MX_REQUIRE(sets && (n_sets == 1 || n_sets == 2), "%s: one or two sets of heads", who);
-  int64_t heads = 0, most = 1;
-  for (int i = 0; i < n_sets; ++i) heads += std::max(sets[i].heads, 0), most = std::max<int64_t>(most, sets[i].heads);
+  int64_t heads = 0;
+  for (int i = 0; i < n_sets; ++i) heads += std::max(sets[i].heads, 0);
   if (int s = check_sets(who, n_sets, tokens, rotation, heads)) return s;
   if (int s = check_type(who, type)) return s;
   const int64_t size = type == MX_ROWS_F32 ? 4 : 2;
   GradArgs a{};
-  a.tokens = tokens, a.rot = *rotation, a.type = type, a.parts = (float*)workspace;
+  a.tokens = tokens, a.rot = *rotation, a.parts = (float*)workspace;
   bool wide = true, weights = false;
   for (int i = 0; i < n_sets; ++i) {
     const mx_heads_grad& s = sets[i];
@@ -284,16 +346,25 @@ int mx_rotate_heads_backward(mx_ctx* ctx, const mx_heads_grad* sets, int32_t n_s
   if (!tokens && !weights) return MX_OK;
   return mxh::by_lanes(rotation->width, [&](auto l, auto n) {
     constexpr int L = decltype(l)::value, NI = decltype(n)::value;
-    const int64_t steps = std::max<int64_t>((tokens * most + 256 / L - 1) / (256 / L), 1);
-    const unsigned grid = (unsigned)(weights ? std::min<int64_t>((steps + 3) / 4, kGradBlocks) : std::min<int64_t>(steps, 1 << 14));
-    hipLaunchKernelGGL((rotate_backward_kernel<L, NI>), dim3(grid, n_sets), dim3(256), weights ? 256 * NI * 8 * sizeof(float) : 0,
-                       as_stream(stream), a);
-    MX_LAUNCH_CHECK("rotate_backward_kernel");
-    if (weights) {
-      hipLaunchKernelGGL(dweight_kernel, dim3((rotation->norm + 63) / 64, n_sets), dim3(1024), 0, as_stream(stream), a, (int)grid);
-      MX_LAUNCH_CHECK("dweight_kernel");
-    }
-    return MX_OK;
+    return by_piece<L, NI>(tokens * heads, type == MX_ROWS_F32, [&](auto k, auto f32) {
+      constexpr int K = decltype(k)::value;
+      int64_t steps[2] = {0, 0};
+      for (int i = 0; i < n_sets; ++i) {
+        a.n.of[i] = (sets[i].heads + K - 1) / K;
+        steps[i] = ((int64_t)tokens * a.n.of[i] + 256 / L - 1) / (256 / L);
+      }
+      // as many turns for every workgroup, whichever its set
+      const int64_t most = (weights ? kGradBlocks : 1 << 16) - 2, turns = std::max<int64_t>((steps[0] + steps[1] + most - 1) / most, 1);
+      for (int i = 0; i < n_sets; ++i) a.blocks[i] = (int)std::max<int64_t>((steps[i] + turns - 1) / turns, 1);
+      hipLaunchKernelGGL((rotate_backward_kernel<L, NI, K, decltype(f32)::value>), dim3(a.blocks[0] + a.blocks[1]), dim3(256),
+                         weights ? 256 * NI * 8 * sizeof(float) : 0, as_stream(stream), a);
+      MX_LAUNCH_CHECK("rotate_backward_kernel");
+      if (weights) {
+        hipLaunchKernelGGL(dweight_kernel, dim3((rotation->norm + 31) / 32, n_sets), dim3(1024), 0, as_stream(stream), a);
+        MX_LAUNCH_CHECK("dweight_kernel");
+      }
+      return MX_OK;
+    });
   });
 }
 

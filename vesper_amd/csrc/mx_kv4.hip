@@ -21,27 +21,32 @@ struct AppendArgs {
 
 // A row on L lanes: normalized, rotated and rounded to BF16; then each quad of lanes holds a block of 32 values, whose
 // largest magnitude (as integers, so that an infinity or NaN is the largest) gives the scale.
-template <int L, int NI>
+template <int L, int NI, bool F32>
 __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
   const int g = threadIdx.x % L;
-  const int64_t r = (int64_t)blockIdx.x * (256 / L) + threadIdx.x / L;
-  if (r >= a.total) return;
+  const int64_t mine = (int64_t)blockIdx.x * (256 / L) + threadIdx.x / L, r = mine < a.total ? mine : a.total - 1;
   const int heads = a.cache.heads;
   const int64_t key_rows = (int64_t)a.rows.tokens * heads;
   const bool value = r >= key_rows;
   const uint32_t row = (uint32_t)(value ? r - key_rows : r), t = row / (uint32_t)heads, h = row - t * (uint32_t)heads;
   const int64_t slot = a.rows.slots[t];
-  const int64_t page = slot / a.cache.page;
-  const float* angles = nullptr;
-  if (slot < 0 || page >= a.cache.pages || !place_of(a.rot, t, angles)) return;
   const int width = value ? a.cache.value_width : a.cache.width;
-  const int64_t size = a.rows.type == MX_ROWS_F32 ? 4 : 2;
+  const int64_t size = F32 ? 4 : 2;
   const void* x = value ? (const uint8_t*)a.rows.v + (t * a.rows.v_stride + (int64_t)h * width) * size
                         : (const uint8_t*)a.rows.k + (t * a.rows.k_stride + (int64_t)h * width) * size;
+  Raw8<F32> raw[NI];
+  load_row<L, NI>(x, a.wide, 0, width, g, raw);
   mx_rotation rot = a.rot;
-  if (value) rot.norm = rot.dims = 0;
+  const float* angles = nullptr;
+  const bool placed = place_of(rot, t, angles);
+  if (value) rot.norm = 0, angles = nullptr;
+  Columns<NI> cols;
+  weights_of<L>(rot, a.rows.weight, 0, g, cols);
+  angles_of<L>(rot, angles, 0, width, g, cols);
   float v[NI][8];
-  normalized_row<L, NI>(x, a.rows.type, a.wide, rot, angles, a.rows.weight, 0, width, g, v);
+  finish_row<L, NI>(x, a.wide, rot, cols, 0, g, raw, v);
+  const int64_t page = slot / a.cache.page;
+  if (mine >= a.total || slot < 0 || page >= a.cache.pages || !placed) return;
   const int64_t at = (page * heads + h) * a.cache.page + slot % a.cache.page;
   uint8_t* codes = (value ? a.cache.v_codes : a.cache.k_codes) + at * (width / 2);
   uint8_t* scales = (value ? a.cache.v_scales : a.cache.k_scales) + at * scale_pitch(width);
@@ -140,7 +145,8 @@ int mx_kv4_append(mx_ctx* ctx, const mx_kv4* cache, const mx_kv4_rows* rows, con
   if (!rows->tokens) return MX_OK;
   return by_lanes(cache->width, [&](auto l, auto n) {
     constexpr int L = decltype(l)::value, NI = decltype(n)::value;
-    hipLaunchKernelGGL((append_kernel<L, NI>), dim3((unsigned)((a.total + 256 / L - 1) / (256 / L))), dim3(256), 0, as_stream(stream), a);
+    const auto kernel = rows->type == MX_ROWS_F32 ? append_kernel<L, NI, true> : append_kernel<L, NI, false>;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)((a.total + 256 / L - 1) / (256 / L))), dim3(256), 0, as_stream(stream), a);
     MX_LAUNCH_CHECK("append_kernel");
     return MX_OK;
   });
