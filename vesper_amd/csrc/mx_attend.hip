@@ -1133,6 +1133,7 @@ __global__ __launch_bounds__(256, (Grouped<W, RG>::kWaves)) void grouped_kernel(
           sc = scores<0, 1>(kreg[k], ql[k], sc, ks[k / 2], qs[k / 2]);
         }
       }
+      __builtin_amdgcn_sched_barrier(0);   // what follows runs beside the products
       // -- values to BF16 --
       uint8_t* buffer = lds + (A::kBuffers > 1 ? (it & 1) * (TG * A::kTile) : 0);
 #pragma unroll
@@ -1187,20 +1188,24 @@ __global__ __launch_bounds__(256, (Grouped<W, RG>::kWaves)) void grouped_kernel(
         p[n] = mxd::bf16_pair(p0, p1);
       }
       if (RG > 1) mxd::lds_barrier();
-      // -- O^T += V^T P^T --
+      // -- O^T += V^T P^T, the values read two products ahead --
+      v8b vv[3];
+      auto read = [&](int n) {
+        const int k = n / DB, d = n % DB;
+        const uint8_t* at = buffer + (d & 1 ? get1 : get0) + 128 * (d / 2) + 16 * k * (2 * W);
+        typedef __attribute__((address_space(3))) v4s lds_v4s;
+        v4s w[2];
+        w[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)at);
+        w[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(at + 8 * (2 * W)));
+        vv[n % 3] = __builtin_bit_cast(v8b, w);
+      };
+      read(0), read(1);
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const v8b pv = __builtin_bit_cast(v8b, make_uint4(p[4 * k], p[4 * k + 1], p[4 * k + 2], p[4 * k + 3]));
-#pragma unroll
-        for (int d = 0; d < DB; ++d) {
-          const uint8_t* at = buffer + (d & 1 ? get1 : get0) + 128 * (d / 2) + 16 * k * (2 * W);
-          typedef __attribute__((address_space(3))) v4s lds_v4s;
-          v4s w[2];
-          w[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)at);
-          w[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(at + 8 * (2 * W)));
-          const v8b vv = __builtin_bit_cast(v8b, w);
-          o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vv, pv, o[d], 0, 0, 0);
-        }
+      for (int n = 0; n < 2 * DB; ++n) {
+        const int k = n / DB, d = n % DB;
+        if (n + 2 < 2 * DB) read(n + 2);
+        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vv[n % 3], __builtin_bit_cast(v8b, make_uint4(p[4 * k], p[4 * k + 1], p[4 * k + 2], p[4 * k + 3])),
+                                                       o[d], 0, 0, 0);
       }
     }
 
@@ -1325,31 +1330,38 @@ __device__ __forceinline__ void join(const AttendArgs& a, Piece piece) {
     auto slot = [&](int i) { return (int64_t)2 * (g + i) + (i ? 0 : s.slot); };
     float most = kLowest, sum = 0.f;
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    auto add = [&](int i0, int step) {   // eight parts at a time
-      float2 st[8];
-      float4 p[8];
+    auto add = [&](auto count, int i0, int step) {   // so many parts at a time
+      constexpr int N = decltype(count)::value;
+      float2 st[N];
+      float4 p[N];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
+      for (int j = 0; j < N; ++j) {
         const int64_t at = slot(min(i0 + step * j, s.parts - 1));
         st[j] = stats[at * kRows];
         p[j] = parts[at * (kRows * WV / 4) + e];
       }
       float next = most;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) next = fmaxf(next, st[j].x);
+      for (int j = 0; j < N; ++j) next = fmaxf(next, st[j].x);
       const float by = power(most, next);
       most = next, sum *= by;
       v.x *= by, v.y *= by, v.z *= by, v.w *= by;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float f = i0 + step * j < s.parts ? power(st[j].x, most) : 0.f;
+      for (int j = 0; j < N; ++j) {
         const bool use = i0 + step * j < s.parts;   // (not by a factor of zero: a part may hold NaN)
+        const float f = power(st[j].x, most);
         sum += use ? st[j].y * f : 0.f;
         v.x += use ? p[j].x * f : 0.f, v.y += use ? p[j].y * f : 0.f, v.z += use ? p[j].z * f : 0.f, v.w += use ? p[j].w * f : 0.f;
       }
     };
+    constexpr std::integral_constant<int, 2> two{};
+    constexpr std::integral_constant<int, 8> eight{};
     if (together) {
-      for (int i0 = wave; i0 < s.parts; i0 += 32) add(i0, 4);
+      if (s.parts <= 8) {
+        if (wave < s.parts) add(two, wave, 4);
+      } else {
+        for (int i0 = wave; i0 < s.parts; i0 += 32) add(eight, i0, 4);
+      }
       __syncthreads();
       sums[wave][lane] = v, tops[wave][lane] = make_float2(most, sum);
       __syncthreads();
@@ -1365,7 +1377,11 @@ __device__ __forceinline__ void join(const AttendArgs& a, Piece piece) {
         v.x += p.x * f, v.y += p.y * f, v.z += p.z * f, v.w += p.w * f;
       }
     } else {
-      for (int i0 = 0; i0 < s.parts; i0 += 8) add(i0, 1);
+      if (s.parts <= 4) {
+        for (int i0 = 0; i0 < s.parts; i0 += 2) add(two, i0, 1);
+      } else {
+        for (int i0 = 0; i0 < s.parts; i0 += 8) add(eight, i0, 1);
+      }
     }
     const Sequence q = sequence(a, s.b);
     const int row = s.tile * kRows + r;

@@ -14,7 +14,7 @@ namespace {
 using namespace mxh;
 
 constexpr int kMaxTokens = 1 << 20, kMaxWidth = 4096;
-constexpr int kGradBlocks = 1024;   // workgroups that add up dweight, of both sets together
+constexpr int kGradBlocks = 1280;   // workgroups that add up dweight, of both sets together (and one more of each)
 
 // A piece is K heads of one token and set on a group of L lanes: its rows are asked for at once, its angles and weights once.
 struct Pieces {
@@ -70,7 +70,6 @@ __global__ __launch_bounds__(256) void rotate_kernel(HeadsArgs a) {
 
 struct GradArgs {
   mx_heads_grad set[2];
-  Pieces n;
   int tokens;
   mx_rotation rot;
   bool wide;
@@ -80,7 +79,7 @@ struct GradArgs {
 
 // The first blocks[0] workgroups have the first set. A lane keeps its columns' sums for dweight over its rows; the
 // workgroup's go to parts.
-template <int L, int NI, int K, bool F32>
+template <int L, int NI, bool F32>
 __global__ __launch_bounds__(256) void rotate_backward_kernel(GradArgs a) {
   extern __shared__ float sums[];   // [256 / L][8 L NI] where dweight is asked for
   const bool second = (int)blockIdx.x >= a.blocks[0];
@@ -92,75 +91,67 @@ __global__ __launch_bounds__(256) void rotate_backward_kernel(GradArgs a) {
   Columns<NI> cols;
   weights_of<L>(a.rot, s.weight, 0, g, cols);
   float dw[NI][8] = {};
-  const uint32_t each = a.n.of[second], pieces = (uint32_t)a.tokens * each, block = blockIdx.x - (second ? a.blocks[0] : 0);
-  for (uint32_t first = block * (256 / L); first < pieces; first += a.blocks[second] * (256 / L)) {
-    const uint32_t mine = first + threadIdx.x / L, p = min(mine, pieces - 1), t = p / each;
-    const int h = (p - t * each) * K, heads = s.heads - h;
-    const uint8_t* dy = (const uint8_t*)s.dy + (t * s.dy_stride + (int64_t)h * width) * size;
-    const uint8_t* x = (const uint8_t*)s.x + (t * s.x_stride + (int64_t)h * width) * size;
-    uint8_t* dx = (uint8_t*)s.dx + (t * s.dx_stride + (int64_t)h * width) * size;
-    Raw8<F32> raw_d[K][NI], raw_x[K][NI];
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const int64_t at = (int64_t)min(k, heads - 1) * width * size;
-      load_row<L, NI>(dy + at, a.wide, 0, width, g, raw_d[k]);
-      load_row<L, NI>(x + at, a.wide, 0, norm, g, raw_x[k]);
-    }
+  const uint32_t each = s.heads, rows = (uint32_t)a.tokens * each, step = a.blocks[second] * (256 / L);
+  const uint32_t begin = (blockIdx.x - (second ? a.blocks[0] : 0)) * (256 / L);
+  for (uint32_t first = begin; first < rows; first += step) {
+    const uint32_t mine = first + threadIdx.x / L, p = min(mine, rows - 1), t = p / each;
+    const int64_t head = (int64_t)(p - t * each) * width;
+    const uint8_t* dy = (const uint8_t*)s.dy + (t * s.dy_stride + head) * size;
+    uint8_t* dx = (uint8_t*)s.dx + (t * s.dx_stride + head) * size;
+    Raw8<F32> raw_d[NI], raw_x[NI];
+    load_row<L, NI>(dy, a.wide, 0, width, g, raw_d);
+    load_row<L, NI>((const uint8_t*)s.x + (t * s.x_stride + head) * size, a.wide, 0, norm, g, raw_x);
     const float* angles = nullptr;
-    const bool there = mine < pieces, live = place_of(a.rot, t, angles) && there;
+    const bool there = mine < rows, counts = place_of(a.rot, t, angles) && there;
     angles_of<L>(a.rot, angles, 0, width, g, cols);
+    float d[NI][8], u[NI][8];
+    double sum = 0;
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const bool counts = live && k < heads;   // (a select, not a factor: what does not count may hold NaN)
-      float d[NI][8], u[NI][8];
-      double sum = 0;
+    for (int i = 0; i < NI; ++i) {
+      values(raw_d[i], d[i]), values(raw_x[i], u[i]);
+      if (__all(counts)) continue;
 #pragma unroll
-      for (int i = 0; i < NI; ++i) {
-        values(raw_d[k][i], d[i]), values(raw_x[k][i], u[i]);
-        if (__all(counts)) continue;
+      for (int j = 0; j < 8; ++j) d[i][j] = counts ? d[i][j] : 0.f, u[i][j] = counts ? u[i][j] : 0.f;   // (they may hold NaN)
+    }
 #pragma unroll
-        for (int j = 0; j < 8; ++j) d[i][j] = counts ? d[i][j] : 0.f, u[i][j] = counts ? u[i][j] : 0.f;
-      }
+    for (int i = 0; i < NI; ++i) {
+      turn8(a.rot, cols.a[i], sign, d[i], [&](float (&q)[8]) {
+        if constexpr (NI == 1) {
+          partner_lane<L>(a.rot, cols.a[0], g, d[0], q);
+        } else if (cols.a[i].on) {   // (from memory once more)
+          values(load_raw<F32>(dy, a.wide, 8 * (i * L + g) + (cols.a[i].low ? a.rot.dims / 2 : -(a.rot.dims / 2))), q);
 #pragma unroll
-      for (int i = 0; i < NI; ++i) {
-        turn8(a.rot, cols.a[i], sign, d[i], [&](float (&q)[8]) {
-          if constexpr (NI == 1) {
-            partner_lane<L>(a.rot, cols.a[0], g, d[0], q);
-          } else if (cols.a[i].on) {   // (from memory once more)
-            values(load_raw<F32>(dy, a.wide, 8 * (i * L + g) + (cols.a[i].low ? a.rot.dims / 2 : -(a.rot.dims / 2))), q);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) q[j] = counts ? q[j] : 0.f;
-          }
-        });
-#pragma unroll
-        for (int j = 0; j < 8; ++j) sum = fma((double)u[i][j], (double)u[i][j], sum);
-      }
-      if (norm) {
-        const float r = root(group_sum<L>(sum), norm, a.rot.eps);
-        float dot = 0.f;
-#pragma unroll
-        for (int i = 0; i < NI; ++i) {
-          if (!cols.normed[i]) continue;
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            u[i][j] *= r;
-            dw[i][j] += d[i][j] * u[i][j];
-            d[i][j] *= cols.w[i][j];
-            dot += d[i][j] * u[i][j];
-          }
+          for (int j = 0; j < 8; ++j) q[j] = counts ? q[j] : 0.f;
         }
-        const float mean = group_sum<L>(dot) / norm;
+      });
 #pragma unroll
-        for (int i = 0; i < NI; ++i)
-          if (cols.normed[i])
+      for (int j = 0; j < 8; ++j) sum = fma((double)u[i][j], (double)u[i][j], sum);
+    }
+    if (norm) {
+      const float r = root(group_sum<L>(sum), norm, a.rot.eps);
+      float dot = 0.f;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) d[i][j] = r * (d[i][j] - u[i][j] * mean);
+      for (int i = 0; i < NI; ++i) {
+        if (!cols.normed[i]) continue;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          u[i][j] *= r;
+          dw[i][j] += d[i][j] * u[i][j];
+          d[i][j] *= cols.w[i][j];
+          dot += d[i][j] * u[i][j];
+        }
       }
-      if (!there || k >= heads) continue;
+      const float mean = group_sum<L>(dot) / norm;
 #pragma unroll
       for (int i = 0; i < NI; ++i)
-        if (8 * (i * L + g) < width) store8(dx + (int64_t)k * width * size, type, a.wide, 8 * (i * L + g), d[i]);
+        if (cols.normed[i])
+#pragma unroll
+          for (int j = 0; j < 8; ++j) d[i][j] = r * (d[i][j] - u[i][j] * mean);
     }
+    if (!there) continue;
+#pragma unroll
+    for (int i = 0; i < NI; ++i)
+      if (8 * (i * L + g) < width) store8(dx, type, a.wide, 8 * (i * L + g), d[i]);
   }
   if (!s.dweight) return;
 #pragma unroll
@@ -305,7 +296,7 @@ int mx_rotate_heads(mx_ctx* ctx, const mx_heads* sets, int32_t n_sets, int32_t t
 
 uint64_t mx_rotate_heads_workspace_bytes(int32_t norm) {
   if (norm < 0 || norm > kMaxWidth) return 0;
-  return (uint64_t)kGradBlocks * norm * sizeof(float);
+  return (uint64_t)(kGradBlocks + 2) * norm * sizeof(float);
 }
 
 int mx_rotate_heads_backward(mx_ctx* ctx, const mx_heads_grad* sets, int32_t n_sets, int32_t tokens, const mx_rotation* rotation,
@@ -346,25 +337,19 @@ int mx_rotate_heads_backward(mx_ctx* ctx, const mx_heads_grad* sets, int32_t n_s
   if (!tokens && !weights) return MX_OK;
   return mxh::by_lanes(rotation->width, [&](auto l, auto n) {
     constexpr int L = decltype(l)::value, NI = decltype(n)::value;
-    return by_piece<L, NI>(tokens * heads, type == MX_ROWS_F32, [&](auto k, auto f32) {
-      constexpr int K = decltype(k)::value;
-      int64_t steps[2] = {0, 0};
-      for (int i = 0; i < n_sets; ++i) {
-        a.n.of[i] = (sets[i].heads + K - 1) / K;
-        steps[i] = ((int64_t)tokens * a.n.of[i] + 256 / L - 1) / (256 / L);
-      }
-      // as many turns for every workgroup, whichever its set
-      const int64_t most = (weights ? kGradBlocks : 1 << 16) - 2, turns = std::max<int64_t>((steps[0] + steps[1] + most - 1) / most, 1);
-      for (int i = 0; i < n_sets; ++i) a.blocks[i] = (int)std::max<int64_t>((steps[i] + turns - 1) / turns, 1);
-      hipLaunchKernelGGL((rotate_backward_kernel<L, NI, K, decltype(f32)::value>), dim3(a.blocks[0] + a.blocks[1]), dim3(256),
-                         weights ? 256 * NI * 8 * sizeof(float) : 0, as_stream(stream), a);
-      MX_LAUNCH_CHECK("rotate_backward_kernel");
-      if (weights) {
-        hipLaunchKernelGGL(dweight_kernel, dim3((rotation->norm + 31) / 32, n_sets), dim3(1024), 0, as_stream(stream), a);
-        MX_LAUNCH_CHECK("dweight_kernel");
-      }
-      return MX_OK;
-    });
+    int64_t steps[2] = {0, 0};
+    for (int i = 0; i < n_sets; ++i) steps[i] = ((int64_t)tokens * sets[i].heads + 256 / L - 1) / (256 / L);
+    // as many turns for every workgroup, whichever its set
+    const int64_t most = weights ? kGradBlocks : 1 << 16, turns = std::max<int64_t>((steps[0] + steps[1] + most - 1) / most, 1);
+    for (int i = 0; i < n_sets; ++i) a.blocks[i] = (int)std::max<int64_t>((steps[i] + turns - 1) / turns, 1);
+    const auto kernel = type == MX_ROWS_F32 ? rotate_backward_kernel<L, NI, true> : rotate_backward_kernel<L, NI, false>;
+    hipLaunchKernelGGL(kernel, dim3(a.blocks[0] + a.blocks[1]), dim3(256), weights ? 256 * NI * 8 * sizeof(float) : 0, as_stream(stream), a);
+    MX_LAUNCH_CHECK("rotate_backward_kernel");
+    if (weights) {
+      hipLaunchKernelGGL(dweight_kernel, dim3((rotation->norm + 31) / 32, n_sets), dim3(1024), 0, as_stream(stream), a);
+      MX_LAUNCH_CHECK("dweight_kernel");
+    }
+    return MX_OK;
   });
 }
 
