@@ -44,10 +44,28 @@ struct Space {
   int64_t units, stats, rows, base, prefix, total;
 };
 
+// n / d for n below 2^31: with m = floor(2^(31 + s) / d) + 1, s = ceil(log2 d), n m exceeds n 2^(31 + s) / d by less than
+// 2^(31 + s) / d.
+struct Divide {
+  uint32_t m, d;
+  int shift;
+  Divide() = default;
+  explicit Divide(int by) : d(by) {
+    int s = 0;
+    while ((1ll << s) < by) ++s;
+    shift = 31 + s, m = (uint32_t)((1ull << shift) / by + 1);
+  }
+  __device__ __forceinline__ int of(int n) const { return (int)((uint64_t)(uint32_t)n * m >> shift); }
+  __device__ __forceinline__ int rest(int n) const { return n - of(n) * (int)d; }
+};
+
 struct AttendArgs {
   mx_kv4 cache;
   mx_kv4_query q;
   int group;           // query heads of a key head
+  Divide by_group;
+  int rows_each, tiles_each;   // query tokens and row tiles of a sequence, where all have as many
+  Divide by_tiles;             // by the latter
   int page_shift;
   int tiles;           // row tiles of all sequences, at most
   float c;             // scale log2(e)
@@ -76,7 +94,7 @@ __device__ __forceinline__ Sequence sequence(const AttendArgs& a, int b) {
     s.first = min(max(a.q.q_first[b], 0), a.q.tokens);
     s.n = min(max(a.q.q_first[b + 1], s.first), a.q.tokens) - s.first;
   } else {
-    s.n = a.q.tokens / a.q.batch, s.first = b * s.n;
+    s.n = a.rows_each, s.first = b * s.n;
   }
   const int length = a.q.lengths[b];
   s.end = length;
@@ -94,31 +112,32 @@ __device__ __forceinline__ void seen(const AttendArgs& a, const Sequence& s, int
 // Tokens [lo, hi) that some row of row tile `tile` sees (lo at a whole step), and its iterations of `step` tokens: one at
 // least, which writes the rows that see nothing.
 __device__ __forceinline__ int tile_iterations(const AttendArgs& a, const Sequence& s, int tile, int rows, int step, int& lo, int& hi) {
-  const int64_t row0 = (int64_t)tile * rows, all = (int64_t)s.n * a.group;
+  const int row0 = tile * rows, all = s.n * a.group;   // at most 2^30
   int l1, h0;
-  seen(a, s, (int)(row0 / a.group), lo, h0);
-  seen(a, s, (int)((lesser(row0 + rows, all) - 1) / a.group), l1, hi);
+  seen(a, s, a.by_group.of(row0), lo, h0);
+  seen(a, s, a.by_group.of(min(row0 + rows, all) - 1), l1, hi);
   lo &= ~31;
   return max(1, (hi - lo + step - 1) / step);
 }
 
-// The plan: base[b] = row tiles of the sequences before b, prefix[i] = costs (of one key head) of the row tiles before i.
-// Made by a workgroup of N threads in its LDS, or by plan_kernel in the workspace.
+// The plan: base[b] = row tiles of the sequences before b (where they differ), prefix[i] = costs (of one key head) of the
+// row tiles before i. Made by a workgroup of N threads in its LDS, or by plan_kernel in the workspace.
 struct Plan {
   int32_t* base;
   int64_t* prefix;
 };
 
-// Sum of v over the threads before this one, and over all N; v below 2^26.
+// Sum of v over the threads before this one, and over all N; the v below 2^26.
 template <int N>
 __device__ __forceinline__ int64_t scan(uint32_t v, uint32_t* sums, int64_t& all) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   uint32_t s = v;
-#pragma unroll
-  for (int m = 1; m < 64; m <<= 1) {
-    const uint32_t o = __shfl_up(s, m, 64);
-    s += lane >= m ? o : 0;
-  }
+  s += __builtin_amdgcn_update_dpp(0, s, 0x111, 0xF, 0xF, false);   // within 16 lanes, from 1, 2, 4 and 8 before
+  s += __builtin_amdgcn_update_dpp(0, s, 0x112, 0xF, 0xF, false);
+  s += __builtin_amdgcn_update_dpp(0, s, 0x114, 0xF, 0xF, false);
+  s += __builtin_amdgcn_update_dpp(0, s, 0x118, 0xF, 0xF, false);
+  s += __builtin_amdgcn_update_dpp(0, s, 0x142, 0xA, 0xF, false);   // rows 1 and 3 from the last lane before them
+  s += __builtin_amdgcn_update_dpp(0, s, 0x143, 0xC, 0xF, false);   // rows 2 and 3 from lane 31
   __syncthreads();
   if (lane == 63) sums[wave] = s;
   __syncthreads();
@@ -132,8 +151,10 @@ __device__ __forceinline__ int64_t scan(uint32_t v, uint32_t* sums, int64_t& all
   return before + s - v;
 }
 
+// The last i in [0, n) for which at_most(i), which 0 is and none after one that is not: by a thread, and by a wave, which
+// looks at 64 at a time.
 template <typename T>
-__device__ __forceinline__ int find(int n, T at_most) {   // the last i in [0, n) for which at_most(i), which 0 is
+__device__ __forceinline__ int find(int n, T at_most) {
   int lo = 0, hi = n;
   while (hi - lo > 1) {
     const int mid = (lo + hi) / 2;
@@ -141,15 +162,22 @@ __device__ __forceinline__ int find(int n, T at_most) {   // the last i in [0, n
   }
   return lo;
 }
+template <typename T>
+__device__ __forceinline__ int find_by_wave(int n, T at_most) {
+  int lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int step = (hi - lo + 63) / 64, i = lo + (int)(threadIdx.x & 63) * step;
+    lo += (__popcll(__ballot(i < hi && at_most(min(i, n - 1)))) - 1) * step;
+    hi = min(lo + step, hi);
+  }
+  return lo;
+}
 
 template <int N>
 __device__ __forceinline__ void make_plan(const AttendArgs& a, Plan p, uint32_t* sums, int rows, int step) {
-  int64_t tiles = 0, all;
-  const int each = a.q.q_first ? 0 : (a.q.tokens / a.q.batch * a.group + rows - 1) / rows;   // row tiles of a sequence
-  if (each) {
-    for (int b = threadIdx.x; b <= a.q.batch; b += N) p.base[b] = b * each;
-    tiles = (int64_t)a.q.batch * each;
-  } else {
+  int64_t tiles = (int64_t)a.q.batch * a.tiles_each, all;
+  const bool each = !a.q.q_first;
+  if (!each) {
     for (int b0 = 0; b0 < a.q.batch; b0 += N) {
       const int b = b0 + threadIdx.x;
       uint32_t n = 0;
@@ -168,9 +196,9 @@ __device__ __forceinline__ void make_plan(const AttendArgs& a, Plan p, uint32_t*
     const int i = i0 + threadIdx.x;
     uint32_t n = 0;
     if (i < tiles) {
-      const int b = each ? i / each : find(a.q.batch, [&](int k) { return p.base[k] <= i; });
+      const int b = each ? a.by_tiles.of(i) : find(a.q.batch, [&](int k) { return p.base[k] <= i; });
       int lo, hi;
-      n = kBegin + tile_iterations(a, sequence(a, b), each ? i - b * each : i - p.base[b], rows, step, lo, hi);
+      n = kBegin + tile_iterations(a, sequence(a, b), each ? a.by_tiles.rest(i) : i - p.base[b], rows, step, lo, hi);
     }
     const int64_t before = scan<N>(n, sums, all);
     if (i < tiles) p.prefix[i] = sum + before;
@@ -195,7 +223,7 @@ __device__ __forceinline__ Sequence uniform(Sequence s) {
   return s;
 }
 
-// A workgroup's way through the units, in the order sequence, key head, row tile.
+// A workgroup's way through the units, in the order key head, sequence, row tile.
 struct Units {
   int64_t x, end;           // the costs that are the workgroup's, from x on
   int b, h, tile, tiles;    // the unit, and row tiles of its sequence
@@ -222,14 +250,11 @@ __device__ __forceinline__ void next_unit(const AttendArgs& a, Units& u, int row
   if (u.x >= u.end) return;
   if (++u.tile == u.tiles) {
     u.tile = 0;
-    if (++u.h == a.cache.heads) {
-      u.h = 0;
-      do {
-        ++u.b;
-        u.s = uniform(sequence(a, u.b));
-        u.tiles = tiles_of(a, u.s, rows);
-      } while (u.tiles == 0);
-    }
+    do {   // (there is another, since costs are left)
+      if (++u.b == a.q.batch) u.b = 0, ++u.h;
+      u.s = uniform(sequence(a, u.b));
+      u.tiles = tiles_of(a, u.s, rows);
+    } while (u.tiles == 0);
   }
   enter(a, u, rows, step);
 }
@@ -243,40 +268,38 @@ __device__ __forceinline__ int few(int64_t in, int64_t span) {
 }
 
 // Workgroup g's share of the units: where it begins. By each thread of N its share of an LDS plan (found: two words), else
-// by halving. Whether there is anything.
+// by each wave. Whether there is anything.
 template <int N>
 __device__ __forceinline__ bool first_unit(const AttendArgs& a, const Plan& p, bool in_lds, int g, int64_t& per, int groups, int32_t* found,
                                            Units& u, int rows, int step) {
-  const int heads = a.cache.heads;
-  const int64_t all = uniform(p.prefix[uniform(p.base[a.q.batch])]) * heads;
+  const bool each = !a.q.q_first;
+  const int tiles = each ? a.q.batch * a.tiles_each : uniform(p.base[a.q.batch]);
+  const int64_t total = uniform(p.prefix[tiles]), all = total * a.cache.heads;
   per = larger((all + groups - 1) / groups, 1);
   u.x = lesser(g * per, all), u.end = lesser(u.x + per, all), u.first = true;
   if (u.x >= u.end) return false;
+  u.h = a.cache.heads > 1 ? uniform(few(u.x, total)) : 0;
+  const int64_t before = u.h * total, rest = u.x - before;
+  int t;
   if (in_lds) {
-    for (int b = threadIdx.x; b < a.q.batch; b += N)
-      if (p.prefix[p.base[b]] * heads <= u.x && u.x < p.prefix[p.base[b + 1]] * heads) found[0] = b;
+    for (int i = threadIdx.x; i < tiles; i += N)
+      if (p.prefix[i] <= rest && rest < p.prefix[i + 1]) found[0] = i;
     __syncthreads();
-    u.b = uniform(found[0]);
+    t = uniform(found[0]);
+    if (!each) {
+      for (int b = threadIdx.x; b < a.q.batch; b += N)
+        if (p.base[b] <= t && t < p.base[b + 1]) found[1] = b;
+      __syncthreads();
+    }
+    u.b = each ? a.by_tiles.of(t) : uniform(found[1]);
   } else {
-    u.b = uniform(find(a.q.batch, [&](int b) { return p.prefix[p.base[b]] * heads <= u.x; }));
+    t = uniform(find_by_wave(tiles, [&](int i) { return p.prefix[i] <= rest; }));
+    u.b = each ? a.by_tiles.of(t) : uniform(find_by_wave(a.q.batch, [&](int b) { return p.base[b] <= t; }));
   }
   u.s = uniform(sequence(a, u.b));
-  const int t0 = uniform(p.base[u.b]), t1 = uniform(p.base[u.b + 1]);
-  const int64_t p0 = uniform(p.prefix[t0]), span = uniform(p.prefix[t1]) - p0, in = u.x - p0 * heads;
-  u.h = uniform(few(in, span));
-  const int64_t rest = in - u.h * span + p0;
-  u.tile = 0, u.tiles = t1 - t0;
-  if (u.tiles > 1) {
-    if (in_lds) {
-      for (int t = t0 + threadIdx.x; t < t1; t += N)
-        if (p.prefix[t] <= rest && rest < p.prefix[t + 1]) found[1] = t;
-      __syncthreads();
-      u.tile = uniform(found[1]) - t0;
-    } else {
-      u.tile = uniform(find(t1 - t0, [&](int t) { return p.prefix[t0 + t] <= rest; }));
-    }
-  }
-  u.unit0 = u.x - (rest - uniform(p.prefix[t0 + u.tile]));
+  u.tiles = tiles_of(a, u.s, rows);
+  u.tile = t - (each ? u.b * a.tiles_each : uniform(p.base[u.b]));
+  u.unit0 = before + uniform(p.prefix[t]);
   enter(a, u, rows, step);
   return true;
 }
@@ -458,8 +481,6 @@ struct Latent {
   static constexpr int kMade = 4 * 256 + (kPart ? 128 : 0);
   static_assert(RQ * (kMade * 16 + KS * 256) <= kRing, "the queries lie before the stages");
   static_assert(8 * (kInlineTiles + 1) + 4 * (kInlineTiles + 2) <= kRing, "and so does the plan");
-  static constexpr int CB = 64, kOut = 32 * (CB + 4) * 4;  // columns that go out at a time, and a wave's bytes of them
-  static_assert(4 * kOut <= kRing, "and what goes out");
 };
 
 template <int kA, int kB>
@@ -487,7 +508,7 @@ __device__ __forceinline__ float row_sum4(float v) {
 template <int WK, int RG>
 __global__ __launch_bounds__(512, 2) void latent_kernel(AttendArgs a, int inline_plan) {
   using A = Latent<WK, RG>;
-  constexpr int WV = A::WV, RQ = A::RQ, TT = A::TT, T2 = A::T2, KS = A::KS, CB = A::CB;
+  constexpr int WV = A::WV, RQ = A::RQ, TT = A::TT, T2 = A::T2, KS = A::KS;
   constexpr bool kPart = A::kPart;
   __shared__ __attribute__((aligned(16))) uint8_t lds[A::kLds];
   __shared__ float tops[2][A::kRows][TT];
@@ -531,11 +552,11 @@ __global__ __launch_bounds__(512, 2) void latent_kernel(AttendArgs a, int inline
     const int lo = u.lo, hi = u.hi, h = u.h;
     const int rows = u.s.n * a.group;   // at most 2^30
     const int row0 = u.tile * A::kRows, row = min(row0 + rq * 16 + l16, rows - 1);
-    const int i = row / a.group;
+    const int i = a.by_group.of(row);
     // -- the queries' loads: KS steps of 128 values of the wave's 16 rows, divided among their 8 / RQ waves --
     constexpr int kSharers = 8 / RQ, kEach = (KS + kSharers - 1) / kSharers;
     const int sharer = wave / RQ;
-    const uint16_t* q = a.q.q + (u.s.first + i) * a.q.q_stride + (int64_t)(h * a.group + row % a.group) * WK;
+    const uint16_t* q = a.q.q + (u.s.first + i) * a.q.q_stride + (int64_t)(h * a.group + a.by_group.rest(row)) * WK;
     QueryWords words[kEach];
 #pragma unroll
     for (int e = 0; e < kEach; ++e) {
@@ -625,8 +646,8 @@ __global__ __launch_bounds__(512, 2) void latent_kernel(AttendArgs a, int inline
       seen(a, u.s, i, row_lo, row_hi);
       // tokens [all_lo, all_hi) are seen by all of the wave's rows
       int all_lo, all_hi, unused;
-      seen(a, u.s, min(row0 + rq * 16, rows - 1) / a.group, unused, all_hi);
-      seen(a, u.s, min(row0 + rq * 16 + 15, rows - 1) / a.group, all_lo, unused);
+      seen(a, u.s, a.by_group.of(min(row0 + rq * 16, rows - 1)), unused, all_hi);
+      seen(a, u.s, a.by_group.of(min(row0 + rq * 16 + 15, rows - 1)), all_lo, unused);
       all_lo = uniform(all_lo), all_hi = uniform(all_hi);
       const uint32_t get_k = tt * T2 * 4096 + l16 * 256 + ((quad ^ (l16 & 7)) * 16);
       // probabilities: [16 tokens][row][half][8 tokens of it], as the products take them
@@ -728,8 +749,8 @@ __global__ __launch_bounds__(512, 2) void latent_kernel(AttendArgs a, int inline
         Place to{-1, 1.f};
         if (row0 + r < rows) {
           if (alone) {
-            const int head = h * a.group + (row0 + r) % a.group;
-            const int64_t token = u.s.first + (row0 + r) / a.group;
+            const int head = h * a.group + a.by_group.rest(row0 + r);
+            const int64_t token = u.s.first + a.by_group.of(row0 + r);
             const RowOut f = row_out(a, head, stats[r][0][0], all_l);
             to = {token * a.q.out_stride + (int64_t)head * WV, f.inv};
             if (a.q.lse) a.q.lse[token * a.q.heads + head] = f.lse;
@@ -863,7 +884,12 @@ __global__ __launch_bounds__(512, 2) void latent_kernel(AttendArgs a, int inline
         asm volatile("" ::: "memory");
       };
       mxd::lds_barrier();   // (the queries)
-      __builtin_amdgcn_s_waitcnt(mxd::vm_wait_imm(0));
+      if (it0 + A::kStages - 1 <= it1) {   // the first step's copies have landed
+        __builtin_amdgcn_s_waitcnt(mxd::vm_wait_imm(A::kCopies * (A::kStages - 2)));
+      } else {
+        __builtin_amdgcn_s_waitcnt(mxd::vm_wait_imm(0));
+      }
+      asm volatile("" ::: "memory");
       mxd::copy_barrier();
 #pragma unroll
       for (int t = 0; t < 4; ++t) convert(codes_of(it0, t), t);
@@ -905,30 +931,24 @@ __global__ __launch_bounds__(512, 2) void latent_kernel(AttendArgs a, int inline
       __syncthreads();
       __syncthreads();
       if (alone) {
-        float* own_out = (float*)(lds + cg * A::kOut);
+        // a lane has 4 of every 8 columns of its row: the halves exchange fours, and each stores 8 in a row
 #pragma unroll
-        for (int r = 0; r < RG; ++r)
+        for (int r = 0; r < RG; ++r) {
+          const Place to = places[r * 32 + col];
+          if (to.at < 0) continue;
+          uint16_t* out = a.q.out + to.at + cg * 128 + 8 * half;
 #pragma unroll
-          for (int d0 = 0; d0 < 4; d0 += 2) {
+          for (int d = 0; d < 4; ++d)
 #pragma unroll
-            for (int d = 0; d < 2; ++d)
-#pragma unroll
-              for (int n = 0; n < 4; ++n) {
-                const v16f& v = o[r][d0 + d];
-                *(float4*)(own_out + col * (CB + 4) + 32 * d + 8 * n + 4 * half) = make_float4(v[4 * n], v[4 * n + 1], v[4 * n + 2], v[4 * n + 3]);
-              }
-#pragma unroll 2
-            for (int at = lane / 8; at < 32; at += 8) {
-              const int c = lane % 8 * 8;
-              const Place to = places[r * 32 + at];
-              const float4 v0 = *(const float4*)(own_out + at * (CB + 4) + c), v1 = *(const float4*)(own_out + at * (CB + 4) + c + 4);
-              if (to.at < 0) continue;
-              uint4 w;
-              w.x = mxd::bf16_pair(v0.x * to.by, v0.y * to.by), w.y = mxd::bf16_pair(v0.z * to.by, v0.w * to.by);
-              w.z = mxd::bf16_pair(v1.x * to.by, v1.y * to.by), w.w = mxd::bf16_pair(v1.z * to.by, v1.w * to.by);
-              *(uint4*)(a.q.out + to.at + cg * 128 + d0 * 32 + c) = w;
+            for (int n = 0; n < 16; n += 8) {
+              const v16f& v = o[r][d];
+              const auto x = __builtin_amdgcn_permlane32_swap(mxd::bf16_pair(v[n] * to.by, v[n + 1] * to.by),
+                                                              mxd::bf16_pair(v[n + 4] * to.by, v[n + 5] * to.by), false, false);
+              const auto y = __builtin_amdgcn_permlane32_swap(mxd::bf16_pair(v[n + 2] * to.by, v[n + 3] * to.by),
+                                                              mxd::bf16_pair(v[n + 6] * to.by, v[n + 7] * to.by), false, false);
+              *(uint4*)(out + 32 * d + 2 * n) = make_uint4(x[0], y[0], x[1], y[1]);
             }
-          }
+        }
       } else {   // parts as the registers have them: [wave][row group][block][4 registers][lane]
         float4* part = (float4*)(a.space + a.at.rows) + (slot * 4 + cg) * (RG * 4 * 4 * 64) + lane;
 #pragma unroll
@@ -1014,13 +1034,13 @@ __global__ __launch_bounds__(256, (Grouped<W, RG>::kWaves)) void grouped_kernel(
     // -- the wave's query rows --
     const int rows = u.s.n * a.group;   // at most 2^30
     const int row0 = u.tile * A::kRows + rg * 32, row = min(row0 + col, rows - 1);
-    const int i = row / a.group;
+    const int i = a.by_group.of(row);
     int row_lo, row_hi;
     seen(a, u.s, i, row_lo, row_hi);
     // tokens [all_lo, all_hi) are seen by all of the wave's rows
     int all_lo, all_hi, unused;
-    seen(a, u.s, min(row0, rows - 1) / a.group, unused, all_hi);
-    seen(a, u.s, min(row0 + 31, rows - 1) / a.group, all_lo, unused);
+    seen(a, u.s, a.by_group.of(min(row0, rows - 1)), unused, all_hi);
+    seen(a, u.s, a.by_group.of(min(row0 + 31, rows - 1)), all_lo, unused);
     all_lo = uniform(all_lo), all_hi = uniform(all_hi);
 
     // -- loads: the lane's token of a step, its page a step ahead --
@@ -1057,7 +1077,7 @@ __global__ __launch_bounds__(256, (Grouped<W, RG>::kWaves)) void grouped_kernel(
     v8i qh[KS], ql[KS];
     uint32_t qs[(KS + 1) / 2] = {};
     {
-      const uint16_t* q = a.q.q + (u.s.first + i) * a.q.q_stride + (int64_t)(h * a.group + row % a.group) * W;
+      const uint16_t* q = a.q.q + (u.s.first + i) * a.q.q_stride + (int64_t)(h * a.group + a.by_group.rest(row)) * W;
       constexpr int kEach = (KS + TG - 1) / TG;
       QueryWords words[kEach];
 #pragma unroll
@@ -1225,7 +1245,7 @@ __global__ __launch_bounds__(256, (Grouped<W, RG>::kWaves)) void grouped_kernel(
       Place to{-1, 1.f};
       if (row0 + col < rows) {
         if (alone) {
-          const int head = h * a.group + row % a.group;
+          const int head = h * a.group + a.by_group.rest(row);
           const int64_t token = u.s.first + i;
           const RowOut f = row_out(a, head, most, all_l);
           to = {token * a.q.out_stride + (int64_t)head * W, f.inv};
@@ -1386,8 +1406,8 @@ __device__ __forceinline__ void join(const AttendArgs& a, Piece piece) {
     const Sequence q = sequence(a, s.b);
     const int row = s.tile * kRows + r;
     if (row >= q.n * a.group) continue;
-    const int head = s.h * a.group + row % a.group;
-    const int64_t token = q.first + row / a.group;
+    const int head = s.h * a.group + a.by_group.rest(row);
+    const int64_t token = q.first + a.by_group.of(row);
     const RowOut f = row_out(a, head, most, sum);
     uint2 w;
     w.x = mxd::bf16_pair(v.x * f.inv, v.y * f.inv), w.y = mxd::bf16_pair(v.z * f.inv, v.w * f.inv);
@@ -1485,6 +1505,9 @@ int mx_kv4_attend(mx_ctx* ctx, const mx_kv4* cache, const mx_kv4_query* query, v
   // as many row groups as an average sequence's rows fill
   const int64_t rows = ((int64_t)q.tokens + q.batch - 1) / q.batch * a.group;
   const int rg = rows <= 32 ? 1 : rows <= 64 || !cache->v_codes ? 2 : 4, tile_rows = 32 * rg, step = 128 / rg;
+  a.by_group = Divide(a.group);
+  if (!q.q_first) a.rows_each = q.tokens / q.batch, a.tiles_each = (int)(((int64_t)a.rows_each * a.group + tile_rows - 1) / tile_rows);
+  a.by_tiles = Divide(std::max(a.tiles_each, 1));
   a.at = space_of(cache, a.group, q.tokens, q.batch, tile_rows);
   const int64_t tiles = most_tiles((int64_t)q.tokens * a.group, q.batch, tile_rows);
   a.tiles = (int)tiles;
