@@ -4,10 +4,12 @@ query at a time, src/vesper/kernels/normalization_probe.cu:4-86; its cache keeps
 
 HeadRotation   y = rotation(weight * x / rms(x)) of every head, and its gradients
 KVCache4       pages of E2M1 codes with an E8M0 scale per 32 values: append (normalized and rotated on the way), attend
-CachedAttention  one decode step of the block-32 projections over a cache: wq_a, wq_b, heads, append, attend, wo_a, wo_b
+CachedAttention  the block-32 projections' attention over a cache (NativeProjections.open_cache): wq_a and wq_b with their
+               norms, the rotation, wkv into the cache, attention, the rotation back, wo_a, wo_b
 
 The *_device methods take device pointers and do not synchronise; the others take and return host arrays (BF16 as uint16
-bits, or FP32). A KVCache4 has one workspace: its attend calls must not overlap on different streams.
+bits, or FP32). A KVCache4 has one workspace, a CachedAttention one set of buffers: calls of one object must not overlap
+on different streams.
 """
 
 from __future__ import annotations
@@ -19,6 +21,7 @@ import numpy as np
 
 from . import _lib
 from .dispatch import host_rows, row_type
+from .projections import GROUPED_MAX_TOKENS, WO_A, WO_A_GROUPS, validate_values
 
 MAX_TOKENS, MAX_WIDTH, MAX_BATCH = 1 << 20, 4096, 1 << 16
 APART_WIDTHS, LATENT_WIDTHS = (64, 128, 256), ((512, 512), (576, 512))
@@ -289,6 +292,28 @@ class KVCache4:
             raise ValueError("two tokens name one slot")
         return np.ascontiguousarray(slots, np.int64)
 
+    def _sequences(self, table, lengths, counts, t):
+        """The int32 arrays of `t` query rows' sequences: pages, lengths and, with counts, first rows."""
+        table, lengths = np.asarray(table), np.asarray(lengths)
+        b = lengths.shape[0] if lengths.ndim == 1 else -1
+        if (b < 0 or table.ndim != 2 or table.shape[0] != b or table.shape[1] < 1
+                or any(a.dtype not in (np.dtype(np.int32), np.dtype(np.int64)) for a in (table, lengths))):
+            raise ValueError("table must be an integer array [B, columns] and lengths one [B]")
+        if b and (lengths.min() < 0 or lengths.max() > table.shape[1] * self.page):
+            raise ValueError("lengths must fit their pages")
+        used = np.arange(table.shape[1]) * self.page < lengths[:, None]
+        if np.any(used & ((table < 0) | (table >= self.pages))):
+            raise ValueError(f"page numbers in use must be in [0, {self.pages})")
+        first = None
+        if counts is not None:
+            counts = np.asarray(counts)
+            if counts.shape != (b,) or counts.dtype.kind not in "iu" or (b and counts.min() < 0) or counts.sum() > t:
+                raise ValueError(f"counts must be {b} numbers of query rows, {t} in all")
+            first = np.concatenate([[0], np.cumsum(counts)]).astype(np.int32)
+        elif t % max(b, 1) or (t and not b):
+            raise ValueError("query rows do not divide among the sequences")
+        return np.ascontiguousarray(table, np.int32), np.ascontiguousarray(lengths, np.int32), first
+
     def append(self, k, slots, v=None, rotation: HeadRotation | None = None, positions=None, weight=None) -> dict:
         """Stores the tokens; {"k" [T, heads, width], and "v"}: BF16 bits of what the codes stand for (zero where a token
         is not stored)."""
@@ -332,31 +357,15 @@ class KVCache4:
         if dtype != "bf16":
             raise ValueError("q must be BF16 storage bits")
         t = q.shape[0]
-        table, lengths = np.asarray(table), np.asarray(lengths)
-        b = lengths.shape[0] if lengths.ndim == 1 else -1
-        if (b < 0 or table.ndim != 2 or table.shape[0] != b or table.shape[1] < 1
-                or any(a.dtype not in (np.dtype(np.int32), np.dtype(np.int64)) for a in (table, lengths))):
-            raise ValueError("table must be an integer array [B, columns] and lengths one [B]")
-        if b and (lengths.min() < 0 or lengths.max() > table.shape[1] * self.page):
-            raise ValueError("lengths must fit their pages")
-        used = np.arange(table.shape[1]) * self.page < lengths[:, None]
-        if np.any(used & ((table < 0) | (table >= self.pages))):
-            raise ValueError(f"page numbers in use must be in [0, {self.pages})")
-        first = None
-        if counts is not None:
-            counts = np.asarray(counts)
-            if counts.shape != (b,) or counts.dtype.kind not in "iu" or (b and counts.min() < 0) or counts.sum() > t:
-                raise ValueError(f"counts must be {b} numbers of query rows, {t} in all")
-            first = np.concatenate([[0], np.cumsum(counts)]).astype(np.int32)
-        elif t % max(b, 1) or (t and not b):
-            raise ValueError("query rows do not divide among the sequences")
+        table, lengths, first = self._sequences(table, lengths, counts, t)
+        b = lengths.shape[0]
         if sinks is not None:
             sinks = np.ascontiguousarray(sinks, np.float32)
             if sinks.shape != (self.query_heads,):
                 raise ValueError(f"sinks must be [{self.query_heads}]")
         dev = []
         try:
-            for a in (q, np.ascontiguousarray(table, np.int32), np.ascontiguousarray(lengths, np.int32), first, sinks,
+            for a in (q, table, lengths, first, sinks,
                       np.zeros((t, self.query_heads, self.value_width), np.uint16),
                       np.full((t, self.query_heads), -np.inf, np.float32)):
                 dev.append(None if a is None else self.ctx.upload(a))
@@ -380,3 +389,133 @@ class KVCache4:
             out[name] = np.stack([self.ctx.download(d.ptr + p * size, d.shape[1:], np.uint8) for p in pages]) if pages \
                 else np.zeros((0, *d.shape[1:]), np.uint8)
         return out
+
+
+class CachedAttention:
+    """An attention layer of the block-32 projections over a cache of its latents: of 64 heads of 512 values and one key
+    head, the last 64 of them rotated. Opened by NativeProjections.open_cache, with which it closes (or earlier, by its
+    close()). For x [T, 5120]:
+
+      q = heads(wq_b(norm(wq_a(x)) q_norm)), normalized and rotated;  k = wkv(x), normalized with kv_norm and rotated, into
+      the cache;  o = attention(q, cache), rotated back;  y = wo_b(wo_a(o)), wo_a by groups of eight heads."""
+
+    HEADS, WIDTH, DIMS = 64, 512, 64
+
+    def __init__(self, projections, pages: int, page: int, table, *, max_tokens: int, max_batch: int, q_norm=None,
+                 kv_norm=None, sinks=None, scale: float = 512 ** -0.5, window: int = 0, eps: float = 1e-6):
+        ctx, layout = projections.ctx, projections.layout
+        group_rows, group_width = WO_A[0] // WO_A_GROUPS, WO_A[1]
+        if projections.block != 32 or not projections.has_wo_a:
+            raise ValueError("a cache needs block-32 projections with wo_a")
+        if any(layout.get(n, (0, 0))[0] != rows for n, rows in (("wq_b", self.HEADS * self.WIDTH), ("wkv", self.WIDTH))) \
+                or "wq_a" not in layout or "wo_b" not in layout or layout["wq_a"][0] != layout["wq_b"][1] \
+                or layout["wq_a"][1] != layout["wkv"][1] or layout["wo_b"][1] != WO_A[0] \
+                or self.HEADS * self.WIDTH != WO_A_GROUPS * group_width:
+            raise ValueError("the projections are not of 64 heads over latents of 512")
+        if not (math.isfinite(scale) and scale > 0) or window < 0:
+            raise ValueError("scale must be positive and window not negative")
+        if table is None or not 1 <= max_tokens <= MAX_TOKENS // self.HEADS:
+            raise ValueError(f"a cache needs the rotation's table and max_tokens in [1, {MAX_TOKENS // self.HEADS}]")
+        self.hidden, self.rank = layout["wq_a"][1], layout["wq_a"][0]
+        weights = [None if w is None else np.ascontiguousarray(w, np.float32) for w in (q_norm, kv_norm, sinks)]
+        for name, w, n in zip(("q_norm", "kv_norm", "sinks"), weights, (self.rank, self.WIDTH, self.HEADS)):
+            if w is not None and w.shape != (n,):
+                raise ValueError(f"{name} must be [{n}]")
+        self.projections, self.ctx = projections, ctx
+        self.scale, self.window, self.max_tokens = float(scale), int(window), int(max_tokens)
+        self._owned = []
+        try:
+            self.cache = self._own(KVCache4(ctx, pages, page, 1, self.WIDTH, self.WIDTH, query_heads=self.HEADS,
+                                            max_tokens=max_tokens, max_batch=max_batch))
+            self.down = self._own(HeadRotation(ctx, self.rank, norm=self.rank, eps=eps))
+            self.heads = self._own(HeadRotation(ctx, self.WIDTH, norm=self.WIDTH, dims=self.DIMS, eps=eps, table=table))
+            self.back = self._own(HeadRotation(ctx, self.WIDTH, dims=self.DIMS, table=table))
+            self.q_norm, self.kv_norm, self.sinks = (None if w is None else self._own(ctx.upload(w)) for w in weights)
+            wide, tokens = self.HEADS * self.WIDTH, self.max_tokens
+            self.qa, self.q, self.k, self.o, self.codes, self.scales, self.grouped = (
+                self._own(ctx.empty((tokens, n), t)) for n, t in (
+                    (self.rank, np.uint16), (wide, np.uint16), (self.WIDTH, np.uint16), (wide, np.uint16),
+                    (wide, np.uint8), (wide // 32, np.uint8), (WO_A_GROUPS * group_rows, np.uint16)))
+        except BaseException:
+            self.close()
+            raise
+
+    def _own(self, thing):
+        self._owned.append(thing)
+        return thing
+
+    def close(self):
+        while self._owned:
+            held = self._owned.pop()
+            (held.close if hasattr(held, "close") else held.free)()
+
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *_):
+        self.close()
+
+    def _open(self):
+        if not self._owned:
+            raise RuntimeError("the cache is closed")
+        self.projections._ready()
+
+    # -- device pointers in and out, no host synchronisation ---------------------------------------
+    def step_device(self, x_ptr, tokens: int, positions_ptr, slots_ptr, table_ptr, columns: int, lengths_ptr, batch: int,
+                    y_ptr, q_first_ptr=None, stream=None):
+        """y [T, hidden] of x [T, hidden], both BF16: the tokens' latents go into device int64 slots [T] (outside the
+        cache: not stored) at int32 positions [T], then each token attends to its sequence's `lengths` [batch] tokens on
+        pages `table` [batch, columns], its own among them. The tokens are the last of their sequences: as many of each,
+        or those that int32 q_first [batch + 1] gives. Rows of no sequence have nothing to say in y."""
+        self._open()
+        if not 0 <= tokens <= self.max_tokens or not 0 <= batch <= self.cache.max_batch:
+            raise ValueError(f"the cache was opened for {self.max_tokens} tokens of {self.cache.max_batch} sequences a call")
+        if not tokens:
+            return
+        proj, lib, handle, vp = self.projections, self.ctx.lib, self.ctx._h(), _lib.vp
+        rows, width = WO_A[0] // WO_A_GROUPS, WO_A[1]
+        proj.project_device("wkv", x_ptr, tokens, self.k.ptr, stream)
+        self.cache.append_device(self.k.ptr, slots_ptr, tokens, rotation=self.heads, positions_ptr=positions_ptr,
+                                 weight_ptr=self.kv_norm, stream=stream)
+        proj.project_device("wq_a", x_ptr, tokens, self.qa.ptr, stream)
+        self.down.apply_device([self.down.set(self.qa, 1, self.qa, self.q_norm)], tokens, stream=stream)
+        proj.project_device("wq_b", self.qa.ptr, tokens, self.q.ptr, stream)
+        self.heads.apply_device([self.heads.set(self.q, self.HEADS, self.q)], tokens, positions_ptr, stream=stream)
+        self.cache.attend_device(self.q, tokens, table_ptr, columns, lengths_ptr, batch, self.o, self.scale, q_first_ptr,
+                                 self.window, self.sinks, stream=stream)
+        self.back.apply_device([self.back.set(self.o, self.HEADS, self.o)], tokens, positions_ptr, inverse=True,
+                               stream=stream)
+        lib.kv_round32(handle, vp(self.o), tokens * self.HEADS * self.WIDTH, vp(self.q), vp(self.codes), vp(self.scales),
+                       _lib._stream(stream))   # (the rounded values take the queries' place)
+        for t in range(0, tokens, GROUPED_MAX_TOKENS):
+            lib.fp8_grouped_projection(handle, C.c_void_p(proj.tiled["wo_a"]), WO_A_GROUPS, rows, width,
+                                       C.c_void_p(self.codes.ptr + t * WO_A_GROUPS * width),
+                                       C.c_void_p(self.scales.ptr + t * WO_A_GROUPS * width // 32),
+                                       min(GROUPED_MAX_TOKENS, tokens - t),
+                                       C.c_void_p(self.grouped.ptr + t * WO_A_GROUPS * rows * 2), None, _lib._stream(stream))
+        proj.project_device("wo_b", self.grouped.ptr, tokens, y_ptr, stream)
+
+    # -- host arrays -------------------------------------------------------------------------------
+    def step(self, x, positions, slots, table, lengths, counts=None) -> np.ndarray:
+        """y [T, hidden] BF16 bits: x [T, hidden] BF16 bits, positions [T], slots [T], table [B, columns] and lengths [B]
+        with the tokens of this step; counts [B] of them of each sequence (None: as many of each)."""
+        with self.projections.lock:
+            self._open()
+            t = validate_values(x, self.hidden)
+            if x.ndim != 2 or t > self.max_tokens:
+                raise ValueError(f"x must be [T, {self.hidden}] with T of at most {self.max_tokens}")
+            positions = self.heads._positions(positions, t)
+            slots = self.cache._slots(slots, t)
+            table, lengths, first = self.cache._sequences(table, lengths, counts, t)
+            dev = []
+            try:
+                for a in (x, positions, slots, table, lengths, first):
+                    dev.append(None if a is None else self.ctx.upload(a))
+                dev.append(self.ctx.empty((t, self.hidden), np.uint16))
+                ptr = [None if d is None else d.ptr for d in dev]
+                self.step_device(ptr[0], t, ptr[1], ptr[2], ptr[3], table.shape[1], ptr[4], lengths.shape[0], ptr[6], ptr[5])
+                return dev[6].download()
+            finally:
+                for d in dev:
+                    if d is not None:
+                        d.free()

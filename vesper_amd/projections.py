@@ -14,6 +14,9 @@ column group), and `project_device` is the pointer-level fast path.
 `open_adapters(name, ...)` opens a bank of low-rank adapters beside a projection; `fp8(name, values, adapters=ids)` and
 `project_device(..., adapters_ptr=...)` then add each row's adapter to the projection's FP32 sums before the one rounding
 of the output.
+
+`open_cache(...)` (block 32 with wo_a) opens the attention layer that the projections are of over a paged 4-bit cache:
+its `step` takes tokens from the layer's input to wo_b's output.
 """
 
 from __future__ import annotations
@@ -84,6 +87,7 @@ class NativeProjections:
         self.lock, self.opened, self.ctx = threading.Lock(), False, None
         self.tiled = {}
         self.banks = {}          # projection name -> its AdapterBank
+        self.caches = []         # open_cache's
         self.budget = MemoryBudget(cap=HOST_ALLOWANCE, owner="projections")
         self._device_peak = 0   # the context's peak owned bytes, kept past close for stats()
 
@@ -126,6 +130,8 @@ class NativeProjections:
             self._device_peak = max(self._device_peak, ctx.owned_bytes()[1])
             while self.banks:
                 steps.callback(self.banks.popitem()[1].close)
+            while self.caches:
+                steps.callback(self.caches.pop().close)
 
     def _ready(self):
         if not self.opened:
@@ -155,6 +161,15 @@ class NativeProjections:
             rows, width = self.layout[name]
             self.banks[name] = AdapterBank(self.ctx, rows, width, slots, max_rank, min(max_tokens, MAX_ROWS))
             return self.banks[name]
+
+    def open_cache(self, pages, page, table, **options):
+        """attention.CachedAttention(self, pages, page, table, **options); it closes with the runtime."""
+        from .attention import CachedAttention
+        with self.lock:
+            self._ready()
+            self.caches = [c for c in self.caches if c._owned]
+            self.caches.append(CachedAttention(self, pages, page, table, **options))
+            return self.caches[-1]
 
     def _bank(self, name, tokens):
         bank = self.banks.get(name)
