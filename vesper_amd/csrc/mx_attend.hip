@@ -599,13 +599,11 @@ __global__ __launch_bounds__(512, 2) void latent_kernel(AttendArgs a, int inline
       }
     };
     ask(it0);
+    int first_entries[A::kStages - 1];
     if (wave >= 4) {
-      int first_entries[A::kStages - 1];
 #pragma unroll
       for (int k = 0; k < A::kStages - 1; ++k) first_entries[k] = entry_of(lo + (it0 + k) * A::kStep + 16 * cg);
-#pragma unroll
-      for (int k = 0; k < A::kStages - 1; ++k)
-        if (it0 + k < it1) copy(it0 + k, first_entries[k]);
+      copy(it0, first_entries[0]);
     }
     uint32_t shown = shown_of(it0);
     // -- the queries, converted and exchanged --
@@ -625,6 +623,11 @@ __global__ __launch_bounds__(512, 2) void latent_kernel(AttendArgs a, int inline
         made[k * 256 + 192] = make_uint4(s.low[4], s.low[5], s.low[6], s.low[7]);
       }
       made_scales[k * 64] = s.scales;
+    }
+    if (wave >= 4) {   // (the queries come before these)
+#pragma unroll
+      for (int k = 1; k < A::kStages - 1; ++k)
+        if (it0 + k < it1) copy(it0 + k, first_entries[k]);
     }
     const bool alone = is_alone(u);
     const int64_t slot = 2 * g + (u.first ? 0 : 1);
