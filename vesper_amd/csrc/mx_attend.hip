@@ -1505,9 +1505,19 @@ int mx_kv4_attend(mx_ctx* ctx, const mx_kv4* cache, const mx_kv4_query* query, v
   AttendArgs a{};
   a.cache = *cache, a.q = q, a.group = q.heads / cache->heads, a.c = q.scale * kLog2e, a.space = (uint8_t*)workspace;
   while (1 << a.page_shift < cache->page) ++a.page_shift;
-  // as many row groups as an average sequence's rows fill
-  const int64_t rows = ((int64_t)q.tokens + q.batch - 1) / q.batch * a.group;
-  const int rg = rows <= 32 ? 1 : rows <= 64 || !cache->v_codes ? 2 : 4, tile_rows = 32 * rg, step = 128 / rg;
+  // As many row groups as an average sequence's rows fill, and fewer where little is to do: each lengthens every workgroup's
+  // beginning and end, and saves the others' reading and converting. By the steps of 32 rows and 32 tokens that a wave has
+  // when the tables are full. Latents of 64 heads: 128 x 300 tokens (5 steps) 20.9 us with one and 33.2 with two, 1 x 4099
+  // (2) 19.5 and 22.1, 16 x 4000 (4) 32.0 and 33.1, 16 x 16000 (16) 69.6 and 55.9. Values apart, 32 heads of 128 over 8 key
+  // heads: 64 rows of 600 tokens (1 step) 17.3, 20.5 and 21.3 us with one, two and four, 256 of 2000 (8) 28.7, 29.3 and
+  // 33.4, 4 x 64 of 4000 (16) 43.1, 38.9 and 42.9, 2048 of 2048 (64) 72.1, 65.1 and 80.0, 2048 of 8192 (256) 292, 275 and 270.
+  const int n = workgroups(cache);
+  const int64_t tokens_each = ((int64_t)q.tokens + q.batch - 1) / q.batch, rows = tokens_each * a.group;
+  const int64_t held = std::min<int64_t>((int64_t)q.columns * cache->page, q.window ? q.window + tokens_each : INT64_MAX);
+  const double steps = (double)q.batch * cache->heads * ((rows + 31) / 32) * ((held + 31) / 32) / (4. * n);
+  int rg = rows <= 32 ? 1 : rows <= 64 || !cache->v_codes ? 2 : 4;
+  rg = std::min(rg, steps <= (cache->v_codes ? 8 : 5) ? 1 : steps <= 128 ? 2 : 4);
+  const int tile_rows = 32 * rg, step = 128 / rg;
   a.by_group = Divide(a.group);
   if (!q.q_first) a.rows_each = q.tokens / q.batch, a.tiles_each = (int)(((int64_t)a.rows_each * a.group + tile_rows - 1) / tile_rows);
   a.by_tiles = Divide(std::max(a.tiles_each, 1));
@@ -1520,7 +1530,7 @@ int mx_kv4_attend(mx_ctx* ctx, const mx_kv4* cache, const mx_kv4_query* query, v
     hipLaunchKernelGGL(plan_kernel, dim3(1), dim3(1024), 0, st, a, tile_rows, step);
     MX_LAUNCH_CHECK("plan_kernel");
   }
-  const int n = workgroups(cache), joiners = 8 * kCus;
+  const int joiners = 8 * kCus;
   auto latent = [&](auto wk, auto groups) {
     constexpr int WK = decltype(wk)::value, RG = decltype(groups)::value;
     hipLaunchKernelGGL((latent_kernel<WK, RG>), dim3(n), dim3(512), 0, st, a, (int)inline_plan);
