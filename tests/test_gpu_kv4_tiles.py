@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 
 from oracle import attention as oracle
-from oracle.formats import bf16_bits, bf16_round
+from oracle.formats import bf16_bits, bf16_round, bf16_values
 from tests.test_gpu_kv4 import ATTENDS, check, fill, open_cache, pages_for
 
 pytestmark = pytest.mark.gpu
@@ -68,3 +68,18 @@ def test_more_units_than_a_workgroup_counts(gpu_ctx, kind, heads, kv_heads, colu
         q = bf16_round(rng.standard_normal((int(counts.sum()), heads, cache.width)).astype(np.float32))
         want = oracle.attend(q, keys, values, lengths, counts, 0.05)
         check(cache.attend(bf16_bits(q), table, lengths, 0.05, counts), q, keys, lengths, 0.05, *want)
+
+
+@pytest.mark.parametrize("kind,heads,kv_heads", [("512", 64, 1), ("576", 128, 1), ("64", 14, 2), ("128", 32, 8), ("256", 8, 2)])
+@pytest.mark.parametrize("columns", [1, 1 << 18])
+def test_one_token_is_its_values(gpu_ctx, kind, heads, kv_heads, columns):
+    """Its probability is 1 to 2^-20 whatever its logit, and a value has two significant bits: nothing is left to round."""
+    rng = np.random.default_rng(heads)
+    lengths = np.ones(9, int)
+    table, pages = pages_for(rng, lengths, 16, columns=columns)
+    with open_cache(gpu_ctx, kind, pages, 16, kv_heads, heads) as cache:
+        _, values = fill(cache, rng, table, lengths)
+        q = bf16_round((rng.standard_normal((9, heads, cache.width)) * np.exp2(np.arange(9) - 6)[:, None, None]).astype(np.float32))
+        got = bf16_values(cache.attend(bf16_bits(q), table, lengths, cache.width ** -0.5)["out"])
+        for b in range(9):
+            np.testing.assert_array_equal(got[b], values[b][0].repeat(heads // kv_heads, 0))

@@ -8,8 +8,10 @@
 // operand of O^T = V^T P^T as they are.
 //   S^T: V_MFMA_SCALE_F32_32X32X64_F8F6F4 on the codes and scales as they lie in the cache, with the query as two E4M3
 //        terms: a BF16 value has 8 significant bits, the first term takes 4 of them and the second, 2^-4 of its scale, the
-//        rest, so the products are those of the BF16 query (to 2^-20 of a block's largest). At the rate of E4M3, two terms
-//        cost what one BF16 product does, and the keys need no conversion.
+//        rest, so the products are those of the BF16 query (to 2^-21 of a block's largest). At the rate of E4M3, two terms
+//        cost what one BF16 product does, and the keys need no conversion. The instruction adds the products of eight
+//        neighbours without what lies 2^-13 below the largest of them (measured; between eights it keeps 24 bits): on normal
+//        values logits are off by some 2^-19 of the sum of their products' magnitudes.
 //   O^T: V_MFMA_F32_32X32X16_BF16. A scale belongs to a token and 32 columns, but this product runs over the tokens, so
 //        the values become BF16 (exactly: two significant bits and a power of two) by V_CVT_SCALEF32_PK_BF16_FP4, in the
 //        row order in which they lie, and go through LDS, whose transposing reads give each lane its column's tokens.
@@ -443,6 +445,13 @@ struct Place {
   float by;
 };
 
+// The maximum m with a step's largest logit: the logit itself at first, so that one token alone has probability 1. After that
+// it stays until it is 2^8 too low (probabilities up to 2^8 lose nothing) and is raised by whole numbers, which scale
+// what is in BF16 exactly.
+__device__ __forceinline__ float raised(float m, float top) {
+  return top > m + 8.f ? (m == kLowest ? top : m + ceilf(top - m)) : m;
+}
+
 struct RowOut {
   float inv, lse;
 };
@@ -655,7 +664,7 @@ __global__ __launch_bounds__(512, 2) void latent_kernel(AttendArgs a, int inline
       const uint32_t get_k = tt * T2 * 4096 + l16 * 256 + ((quad ^ (l16 & 7)) * 16);
       // probabilities: [16 tokens][row][half][8 tokens of it], as the products take them
       uint8_t* const put_w = weights + (tt * T2 * A::kRows + rq * 16 + l16) * 32 + (quad & 1) * 16 + (quad >> 1) * 8;
-      float m = kLowest, l = 0.f;   // the maximum is a whole number: every rescaling is exact
+      float m = kLowest, l = 0.f;
       float own = kLowest, sum = 0.f;
       mxd::copy_barrier();   // the first step is there, and the queries have been read
       for (int it = it0; it < it1; ++it) {
@@ -714,8 +723,8 @@ __global__ __launch_bounds__(512, 2) void latent_kernel(AttendArgs a, int inline
 #pragma unroll
         for (int t = 1; t < T2; ++t) top = fmaxf(top, fmaxf(fmaxf(sc[t][0], sc[t][1]), fmaxf(sc[t][2], sc[t][3])));
         top = row_max4(top) * a.c;
-        // the maximum stays until it is 2^8 too low: probabilities up to 2^8 lose nothing
-        own = top > m + 8.f ? ceilf(top) : m;
+        own = m;
+        if (__any(top > m + 8.f)) own = raised(m, top);
         sum = 0.f;
 #pragma unroll
         for (int t = 0; t < T2; ++t) {
@@ -860,7 +869,7 @@ __global__ __launch_bounds__(512, 2) void latent_kernel(AttendArgs a, int inline
         return r;
       };
       auto multiply = [&](Operands& r, int t) {
-        if (TT > 1 && moved) {   // whole powers of two: exact
+        if (TT > 1 && moved) {   // by powers of two, but for a unit's first step
 #pragma unroll
           for (int i = 0; i < RG; ++i) {
             const float f = power(theirs[i][t / T2], m[i]);
@@ -1124,7 +1133,7 @@ __global__ __launch_bounds__(256, (Grouped<W, RG>::kWaves)) void grouped_kernel(
       }
     }
 
-    float m = kLowest, l = 0.f;   // the maximum is a whole number: every rescaling is exact
+    float m = kLowest, l = 0.f;
     v16f o[DB];
 #pragma unroll
     for (int d = 0; d < DB; ++d)
@@ -1193,10 +1202,8 @@ __global__ __launch_bounds__(256, (Grouped<W, RG>::kWaves)) void grouped_kernel(
 #pragma unroll
       for (int n = 2; n < 16; ++n) top = fmaxf(top, sc[n]);
       top = other_half_max(top) * a.c;
-      // the maximum stays until it is 2^8 too low: probabilities up to 2^8 lose nothing
-      const float own = top > m + 8.f ? ceilf(top) : m;
-      if (__any(own != m)) {
-        const float by = power(m, own);
+      if (__any(top > m + 8.f)) {
+        const float own = raised(m, top), by = power(m, own);
         m = own, l *= by;
 #pragma unroll
         for (int d = 0; d < DB; ++d)
