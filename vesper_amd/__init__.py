@@ -20,6 +20,9 @@ reference's interface for this path:
   dispatch.ExpertDispatch                     tokens sorted by expert and back, with gradients (batched moe.py)
   adapters.AdapterBank                        low-rank adapters of many requests beside a projection
                                               (projections.NativeProjections.open_adapters)
+  attention.HeadRotation / KVCache4           heads normalized and rotated, a paged 4-bit cache, its attention
+  attention.CachedAttention                   the block-32 projections' attention layer over a cache
+                                              (projections.NativeProjections.open_cache)
 """
 
 from .config import BASELINE, REFERENCE, MoEConfig

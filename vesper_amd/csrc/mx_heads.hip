@@ -4,6 +4,9 @@
 //   dx = r (w g - u mean(w g u)) on those values and g on the others,   dw = sum over tokens and heads of g u.
 //
 // Memory traffic alone: a row is read once into registers, eight values a lane, by as many lanes as it has eights.
+// Measured for 4096 tokens of 32 + 8 heads of 128 in BF16, all of each turned: forward 20.2 us for 86 MB (4.3 TB/s; 27.3 with
+// a row at a time, whose loads waited for the token's position), backward 28.2 us for 128 MB (4.5 TB/s) and 4.6 for the
+// workgroups' parts of dweight (46 and 9.4 with 512 workgroups for either set).
 #include <algorithm>
 #include <type_traits>
 
@@ -77,7 +80,8 @@ struct GradArgs {
   float* parts;    // [blocks[0] + blocks[1]][norm]
 };
 
-// The first blocks[0] workgroups have the first set. A lane keeps its columns' sums for dweight over its rows; the
+// A row at a time here: two or four a lane (37 and 38 us for both kernels in place of 36) or one asked for ahead (41 to 52)
+// take registers that more waves use better. The first blocks[0] workgroups have the first set. A lane keeps its columns' sums for dweight over its rows; the
 // workgroup's go to parts.
 template <int L, int NI, bool F32>
 __global__ __launch_bounds__(256) void rotate_backward_kernel(GradArgs a) {

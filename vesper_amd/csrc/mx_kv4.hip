@@ -19,6 +19,9 @@ struct AppendArgs {
   bool wide;
 };
 
+// Latency: a row's chain of loads, sums and one store. 4096 latents of 576 in 7.0 us (11.8 MB), 16 in 3.4, an empty launch
+// about 2.
+//
 // A row on L lanes: normalized, rotated and rounded to BF16; then each quad of lanes holds a block of 32 values, whose
 // largest magnitude (as integers, so that an infinity or NaN is the largest) gives the scale.
 template <int L, int NI, bool F32>
