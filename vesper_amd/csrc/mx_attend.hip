@@ -18,8 +18,8 @@
 //
 // Work is divided evenly over the device. A unit is the row tile of one sequence and key head; it costs its iterations (a step
 // of all the workgroup's token groups each) and kBegin more for its queries and its way out. Workgroup g takes the costs
-// [g per, (g + 1) per) of all units in a row. Units that a workgroup has alone go straight to out; the others' parts go to
-// the workspace and a second kernel adds them up.
+// [g per, (g + 1) per) of all units in a row, or, where units are short, those whose costs begin there. Units that a workgroup
+// has alone go straight to out; the others' parts go to the workspace and a second kernel adds them up.
 #include <algorithm>
 #include <type_traits>
 
@@ -72,6 +72,7 @@ struct AttendArgs {
   Divide by_tiles;             // by the latter
   int page_shift;
   int tiles;           // row tiles of all sequences, at most
+  bool whole;          // units stay whole: with the workgroup in whose costs they begin
   float c;             // scale log2(e)
   uint8_t* space;
   Space at;
@@ -241,7 +242,11 @@ struct Units {
 __device__ __forceinline__ void enter(const AttendArgs& a, Units& u, int rows, int step) {
   u.n = uniform(tile_iterations(a, u.s, u.tile, rows, step, u.lo, u.hi));
   u.lo = uniform(u.lo), u.hi = uniform(u.hi);
-  u.it0 = (int)larger(u.x - u.unit0 - kBegin, 0), u.it1 = (int)lesser(u.end - u.unit0 - kBegin, u.n);
+  if (a.whole) {
+    u.it0 = u.unit0 < u.x ? u.n : 0, u.it1 = u.n;
+  } else {
+    u.it0 = (int)larger(u.x - u.unit0 - kBegin, 0), u.it1 = (int)lesser(u.end - u.unit0 - kBegin, u.n);
+  }
 }
 
 __device__ __forceinline__ int tiles_of(const AttendArgs& a, const Sequence& s, int rows) {
@@ -1549,6 +1554,13 @@ int mx_kv4_attend(mx_ctx* ctx, const mx_kv4* cache, const mx_kv4_query* query, v
   a.tiles = (int)tiles;
   const bool inline_plan = tiles <= kInlineTiles;   // at least as many as sequences
   hipStream_t st = as_stream(stream);
+  // Units of few iterations stay whole, by what the tables can hold: parts cost another beginning, their way out and the
+  // second launch, some 9 us. One token each, split and whole: latents of 64 heads 128 x 500 tokens (8 iterations) 25.1 and
+  // 22.9 us, 400 x 500 64.1 and 54.3, but 1 x 320 (5) 14.1 and 15.5; 32 heads over 8 key heads 64 x 1000 (8) 22.7 and 19.5,
+  // 1 x 800 (7) 13.4 and 13.1, 1 x 1000 13.1 and 13.9; prompts of 1000 with a window of 128 (2) 36.5 and 27.4.
+  const int64_t span = std::min<int64_t>(held, q.window ? (int64_t)q.window + 31 + (tile_rows + a.group - 1) / a.group : INT64_MAX);
+  const bool few_units = (int64_t)q.batch * cache->heads * ((rows + tile_rows - 1) / tile_rows) < 16;
+  a.whole = span <= (int64_t)step * (!few_units ? 8 : cache->v_codes ? 7 : 4);
   if (!inline_plan) {
     hipLaunchKernelGGL(plan_kernel, dim3(1), dim3(1024), 0, st, a, tile_rows, step);
     MX_LAUNCH_CHECK("plan_kernel");
@@ -1558,6 +1570,7 @@ int mx_kv4_attend(mx_ctx* ctx, const mx_kv4* cache, const mx_kv4_query* query, v
     constexpr int WK = decltype(wk)::value, RG = decltype(groups)::value;
     hipLaunchKernelGGL((latent_kernel<WK, RG>), dim3(n), dim3(512), 0, st, a, (int)inline_plan);
     MX_LAUNCH_CHECK("latent_kernel");
+    if (a.whole) return MX_OK;
     hipLaunchKernelGGL(join_latent_kernel<RG>, dim3(joiners), dim3(256), 0, st, a);
     MX_LAUNCH_CHECK("join_latent_kernel");
     return MX_OK;
@@ -1566,6 +1579,7 @@ int mx_kv4_attend(mx_ctx* ctx, const mx_kv4* cache, const mx_kv4_query* query, v
     constexpr int W = decltype(w)::value, RG = decltype(groups)::value;
     hipLaunchKernelGGL((grouped_kernel<W, RG>), dim3(n), dim3(256), 0, st, a, (int)inline_plan);
     MX_LAUNCH_CHECK("grouped_kernel");
+    if (a.whole) return MX_OK;
     hipLaunchKernelGGL((join_grouped_kernel<W, RG>), dim3(joiners), dim3(256), 0, st, a);
     MX_LAUNCH_CHECK("join_grouped_kernel");
     return MX_OK;
