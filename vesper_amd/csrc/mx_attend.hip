@@ -37,6 +37,9 @@ typedef mxd::v8i v8i;
 
 constexpr int kCus = 256, kXcds = 8;
 constexpr int kInlineTiles = 1024;   // row tiles of all sequences that every workgroup counts for itself
+// Where the plan is made: in the workspace by a launch of its own, in every workgroup's LDS, or, up to 64 tiles, in the
+// registers of every wave.
+constexpr int kInSpace = 0, kInLds = 1, kByWave = 2;
 // What a unit's beginning and end cost, in iterations. With 2, 4, 6 and 8: the 48 sequences below 71, 61, 63 and 63 us, two
 // prompts 365, 361, 360 and 356.
 constexpr int kBegin = 4;
@@ -132,17 +135,21 @@ struct Plan {
   int64_t* prefix;
 };
 
-// Sum of v over the threads before this one, and over all N; the v below 2^26.
-template <int N>
-__device__ __forceinline__ int64_t scan(uint32_t v, uint32_t* sums, int64_t& all) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  uint32_t s = v;
+// Sum of s over the wave's lanes up to this one.
+__device__ __forceinline__ uint32_t wave_scan(uint32_t s) {
   s += __builtin_amdgcn_update_dpp(0, s, 0x111, 0xF, 0xF, false);   // within 16 lanes, from 1, 2, 4 and 8 before
   s += __builtin_amdgcn_update_dpp(0, s, 0x112, 0xF, 0xF, false);
   s += __builtin_amdgcn_update_dpp(0, s, 0x114, 0xF, 0xF, false);
   s += __builtin_amdgcn_update_dpp(0, s, 0x118, 0xF, 0xF, false);
   s += __builtin_amdgcn_update_dpp(0, s, 0x142, 0xA, 0xF, false);   // rows 1 and 3 from the last lane before them
   s += __builtin_amdgcn_update_dpp(0, s, 0x143, 0xC, 0xF, false);   // rows 2 and 3 from lane 31
+  return s;
+}
+// Sum of v over the threads before this one, and over all N; v below 2^26.
+template <int N>
+__device__ __forceinline__ int64_t scan(uint32_t v, uint32_t* sums, int64_t& all) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const uint32_t s = wave_scan(v);
   __syncthreads();
   if (lane == 63) sums[wave] = s;
   __syncthreads();
@@ -239,14 +246,17 @@ struct Units {
   bool first;               // nothing came before it in this workgroup
 };
 
-__device__ __forceinline__ void enter(const AttendArgs& a, Units& u, int rows, int step) {
-  u.n = uniform(tile_iterations(a, u.s, u.tile, rows, step, u.lo, u.hi));
-  u.lo = uniform(u.lo), u.hi = uniform(u.hi);
+__device__ __forceinline__ void share(const AttendArgs& a, Units& u) {
   if (a.whole) {
     u.it0 = u.unit0 < u.x ? u.n : 0, u.it1 = u.n;
   } else {
     u.it0 = (int)larger(u.x - u.unit0 - kBegin, 0), u.it1 = (int)lesser(u.end - u.unit0 - kBegin, u.n);
   }
+}
+__device__ __forceinline__ void enter(const AttendArgs& a, Units& u, int rows, int step) {
+  u.n = uniform(tile_iterations(a, u.s, u.tile, rows, step, u.lo, u.hi));
+  u.lo = uniform(u.lo), u.hi = uniform(u.hi);
+  share(a, u);
 }
 
 __device__ __forceinline__ int tiles_of(const AttendArgs& a, const Sequence& s, int rows) {
@@ -310,6 +320,51 @@ __device__ __forceinline__ bool first_unit(const AttendArgs& a, const Plan& p, b
   u.tile = t - (each ? u.b * a.tiles_each : uniform(p.base[u.b]));
   u.unit0 = before + uniform(p.prefix[t]);
   enter(a, u, rows, step);
+  return true;
+}
+
+// The same for at most 64 row tiles, one a lane, by every wave for itself: without LDS and barriers, which saves 0.8 to 0.9 us
+// of a call (16 x 1000 tokens of 8 key heads 17.9 to 17.0, one session of latents over 4099 19.5 to 18.7).
+__device__ __forceinline__ bool first_of_few(const AttendArgs& a, int g, int64_t& per, int groups, Units& u, int rows, int step) {
+  const int lane = threadIdx.x & 63;
+  int b, tile, tiles;
+  if (!a.q.q_first) {
+    tiles = a.q.batch * a.tiles_each;
+    b = a.by_tiles.of(min(lane, tiles - 1)), tile = a.by_tiles.rest(lane);
+  } else {
+    const uint32_t own = lane < a.q.batch ? tiles_of(a, sequence(a, lane), rows) : 0, upto = wave_scan(own);
+    tiles = (int)min((uint32_t)__builtin_amdgcn_readlane(upto, 63), (uint32_t)a.tiles);
+    b = 0;   // the last sequence that begins at or before the lane's tile
+#pragma unroll
+    for (int s = 32; s > 0; s >>= 1) {
+      const int begin = __shfl((int)(upto - own), min(b + s, 63), 64);
+      b += b + s < a.q.batch && begin <= lane ? s : 0;
+    }
+    tile = lane - __shfl((int)(upto - own), b, 64);
+  }
+  if (tiles == 0) return false;
+  Sequence s{};
+  int lo = 0, hi = 0;
+  uint32_t n = 0;
+  if (lane < tiles) {
+    s = sequence(a, b);
+    n = kBegin + tile_iterations(a, s, tile, rows, step, lo, hi);
+  }
+  const uint32_t upto = wave_scan(n);
+  const int64_t total = (uint32_t)__builtin_amdgcn_readlane(upto, 63), all = total * a.cache.heads;
+  per = larger((all + groups - 1) / groups, 1);
+  u.x = lesser(g * per, all), u.end = lesser(u.x + per, all), u.first = true;
+  if (u.x >= u.end) return false;
+  u.h = a.cache.heads > 1 ? uniform(few(u.x, total)) : 0;
+  const int64_t before = u.h * total, rest = u.x - before;
+  const int at = __builtin_ctzll(__ballot(upto > rest));
+  auto of = [&](int v) { return __builtin_amdgcn_readlane(v, at); };
+  u.b = of(b), u.tile = of(tile), u.n = of((int)n) - kBegin, u.lo = of(lo), u.hi = of(hi);
+  u.s.first = of(s.first), u.s.n = of(s.n), u.s.held = of(s.held);
+  u.s.end = (int64_t)((uint64_t)(uint32_t)of((int)(s.end >> 32)) << 32 | (uint32_t)of((int)s.end));
+  u.tiles = tiles_of(a, u.s, rows);
+  u.unit0 = before + (uint32_t)of((int)upto) - (u.n + kBegin);
+  share(a, u);
   return true;
 }
 
@@ -529,7 +584,7 @@ __device__ __forceinline__ float row_sum4(float v) {
 }
 
 template <int WK, int RG>
-__global__ __launch_bounds__(512, 2) void latent_kernel(AttendArgs a, int inline_plan) {
+__global__ __launch_bounds__(512, 2) void latent_kernel(AttendArgs a, int by) {
   using A = Latent<WK, RG>;
   constexpr int WV = A::WV, RQ = A::RQ, TT = A::TT, T2 = A::T2, KS = A::KS;
   constexpr bool kPart = A::kPart;
@@ -546,7 +601,7 @@ __global__ __launch_bounds__(512, 2) void latent_kernel(AttendArgs a, int inline
   uint8_t* weights = lds + A::kValues;
 
   Plan plan{(int32_t*)(a.space + a.at.base), (int64_t*)(a.space + a.at.prefix)};
-  if (inline_plan) {
+  if (by == kInLds) {
     plan = {(int32_t*)(lds + 8 * (kInlineTiles + 1)), (int64_t*)lds};
     make_plan<512>(a, plan, sums, A::kRows, A::kStep);
   }
@@ -555,7 +610,8 @@ __global__ __launch_bounds__(512, 2) void latent_kernel(AttendArgs a, int inline
   Shared* shared = (Shared*)(a.space + a.at.units) + g;
   int64_t per;
   Units u;
-  if (!first_unit<512>(a, plan, inline_plan, g, per, kCus, found, u, A::kRows, A::kStep)) {
+  if (!(by == kByWave ? first_of_few(a, g, per, kCus, u, A::kRows, A::kStep)
+                      : first_unit<512>(a, plan, by == kInLds, g, per, kCus, found, u, A::kRows, A::kStep))) {
     if (tid == 0) shared->parts = 0;
     return;
   }
@@ -1015,7 +1071,7 @@ struct Grouped {
 };
 
 template <int W, int RG>
-__global__ __launch_bounds__(256, (Grouped<W, RG>::kWaves)) void grouped_kernel(AttendArgs a, int inline_plan) {
+__global__ __launch_bounds__(256, (Grouped<W, RG>::kWaves)) void grouped_kernel(AttendArgs a, int by) {
   using A = Grouped<W, RG>;
   constexpr int TG = A::TG, KS = A::KS, DB = A::DB, KW = A::KW, VO = A::VO, CB = A::CB;
   __shared__ __attribute__((aligned(16))) uint8_t lds[A::kLds];
@@ -1028,7 +1084,7 @@ __global__ __launch_bounds__(256, (Grouped<W, RG>::kWaves)) void grouped_kernel(
   const int col = lane & 31, half = lane >> 5;   // the lane's query row of the products; as a loader, its token
 
   Plan plan{(int32_t*)(a.space + a.at.base), (int64_t*)(a.space + a.at.prefix)};
-  if (inline_plan) {
+  if (by == kInLds) {
     plan = {(int32_t*)(lds + 8 * (kInlineTiles + 1)), (int64_t*)lds};
     make_plan<256>(a, plan, sums, A::kRows, A::kStep);
   }
@@ -1038,7 +1094,8 @@ __global__ __launch_bounds__(256, (Grouped<W, RG>::kWaves)) void grouped_kernel(
   Shared* shared = (Shared*)(a.space + a.at.units) + g;
   int64_t per;
   Units u;
-  if (!first_unit<256>(a, plan, inline_plan, g, per, groups, found, u, A::kRows, A::kStep)) {
+  if (!(by == kByWave ? first_of_few(a, g, per, groups, u, A::kRows, A::kStep)
+                      : first_unit<256>(a, plan, by == kInLds, g, per, groups, found, u, A::kRows, A::kStep))) {
     if (tid == 0) shared->parts = 0;
     return;
   }
@@ -1552,7 +1609,7 @@ int mx_kv4_attend(mx_ctx* ctx, const mx_kv4* cache, const mx_kv4_query* query, v
   a.at = space_of(cache, a.group, q.tokens, q.batch, tile_rows);
   const int64_t tiles = most_tiles((int64_t)q.tokens * a.group, q.batch, tile_rows);
   a.tiles = (int)tiles;
-  const bool inline_plan = tiles <= kInlineTiles;   // at least as many as sequences
+  const int by = tiles <= 64 ? kByWave : tiles <= kInlineTiles ? kInLds : kInSpace;   // (at least as many as sequences)
   hipStream_t st = as_stream(stream);
   // Units of few iterations stay whole, by what the tables can hold: parts cost another beginning, their way out and the
   // second launch, some 9 us. One token each, split and whole: latents of 64 heads 128 x 500 tokens (8 iterations) 25.1 and
@@ -1561,14 +1618,14 @@ int mx_kv4_attend(mx_ctx* ctx, const mx_kv4* cache, const mx_kv4_query* query, v
   const int64_t span = std::min<int64_t>(held, q.window ? (int64_t)q.window + 31 + (tile_rows + a.group - 1) / a.group : INT64_MAX);
   const bool few_units = (int64_t)q.batch * cache->heads * ((rows + tile_rows - 1) / tile_rows) < 16;
   a.whole = span <= (int64_t)step * (!few_units ? 8 : cache->v_codes ? 7 : 4);
-  if (!inline_plan) {
+  if (by == kInSpace) {
     hipLaunchKernelGGL(plan_kernel, dim3(1), dim3(1024), 0, st, a, tile_rows, step);
     MX_LAUNCH_CHECK("plan_kernel");
   }
   const int joiners = 8 * kCus;
   auto latent = [&](auto wk, auto groups) {
     constexpr int WK = decltype(wk)::value, RG = decltype(groups)::value;
-    hipLaunchKernelGGL((latent_kernel<WK, RG>), dim3(n), dim3(512), 0, st, a, (int)inline_plan);
+    hipLaunchKernelGGL((latent_kernel<WK, RG>), dim3(n), dim3(512), 0, st, a, by);
     MX_LAUNCH_CHECK("latent_kernel");
     if (a.whole) return MX_OK;
     hipLaunchKernelGGL(join_latent_kernel<RG>, dim3(joiners), dim3(256), 0, st, a);
@@ -1577,7 +1634,7 @@ int mx_kv4_attend(mx_ctx* ctx, const mx_kv4* cache, const mx_kv4_query* query, v
   };
   auto grouped = [&](auto w, auto groups) {
     constexpr int W = decltype(w)::value, RG = decltype(groups)::value;
-    hipLaunchKernelGGL((grouped_kernel<W, RG>), dim3(n), dim3(256), 0, st, a, (int)inline_plan);
+    hipLaunchKernelGGL((grouped_kernel<W, RG>), dim3(n), dim3(256), 0, st, a, by);
     MX_LAUNCH_CHECK("grouped_kernel");
     if (a.whole) return MX_OK;
     hipLaunchKernelGGL((join_grouped_kernel<W, RG>), dim3(joiners), dim3(256), 0, st, a);
