@@ -555,7 +555,7 @@ struct Latent {
   static constexpr int kStage = kPart ? kTailScales + 64 * 4 : kTail;
   static constexpr int kRing = kValues + 2 * kWeights, kLds = kRing + kStages * kStage;
   static constexpr int kCopies = kPart ? 7 : 5;            // of a value wave and step
-  // the queries' exchange, over the tiles and probabilities
+  // the first queries' exchange, over the tiles and probabilities
   static constexpr int kMade = 4 * 256 + (kPart ? 128 : 0);
   static_assert(RQ * (kMade * 16 + KS * 256) <= kRing, "the queries lie before the stages");
   static_assert(8 * (kInlineTiles + 1) + 4 * (kInlineTiles + 2) <= kRing, "and so does the plan");
@@ -617,78 +617,76 @@ __global__ __launch_bounds__(512, 2) void latent_kernel(AttendArgs a, int by) {
   }
 
   const int spread = 2 * (l16 & 3) + ((l16 >> 2) & 1);   // pieces of 16 bytes of neighbouring tokens' values lie apart
-  auto go_on = [&] {   // to the next unit, if there is one
-    if (u.end <= u.unit0 + kBegin + u.n && tid == 0) note(u, per, g, shared);
-    next_unit(a, u, A::kRows, A::kStep);
-    return u.x < u.end;
-  };
-  for (;;) {
-    if (u.it1 <= u.it0) {   // only what the unit's beginning costs is this workgroup's
-      if (!go_on()) return;
-      continue;
+  // To the next unit of which iterations are this workgroup's, from `ahead` units on: whether there is one. Every wave goes
+  // its own way through the same units.
+  auto go_on = [&](int ahead) {
+    for (;; ahead = 1) {
+      if (ahead) {
+        if (u.end <= u.unit0 + kBegin + u.n && tid == 0) note(u, per, g, shared);
+        next_unit(a, u, A::kRows, A::kStep);
+        if (u.x >= u.end) return false;
+      }
+      if (u.it1 > u.it0) return true;
     }
-    const int it0 = u.it0, it1 = u.it1;
-    const int lo = u.lo, hi = u.hi, h = u.h;
-    const int rows = u.s.n * a.group;   // at most 2^30
-    const int row0 = u.tile * A::kRows, row = min(row0 + rq * 16 + l16, rows - 1);
-    const int i = a.by_group.of(row);
-    // -- the queries' loads: KS steps of 128 values of the wave's 16 rows, divided among their 8 / RQ waves --
+  };
+  if (!go_on(0)) return;
+  // -- pages: 16 tokens have one --
+  typedef const __attribute__((address_space(4))) int32_t Entry;
+  auto table_of = [&] { return (Entry*)(a.q.table + (int64_t)u.b * a.q.columns); };
+  auto entry_of = [&](Entry* table, int hi, int t) { return table[min(t, max(hi - 1, 0)) >> a.page_shift]; };
+  auto is_there = [&](int hi, int t, int entry) { return t < hi && (uint32_t)entry < (uint32_t)a.cache.pages; };
+  // a step's four entries are asked for a step before they are looked at, so that nobody waits for them; bit t: 16 tokens
+  int entries[4];
+  auto ask = [&](Entry* table, int lo, int hi, int it) {
+#pragma unroll
+    for (int t = 0; t < 4; ++t) entries[t] = entry_of(table, hi, lo + it * A::kStep + 16 * t);
+  };
+  auto shown_of = [&](int lo, int hi, int it) {
+    uint32_t shown = 0;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) shown |= is_there(hi, lo + it * A::kStep + 16 * t, entries[t]) ? 1u << t : 0u;
+    return shown;
+  };
+  // -- a value wave's copies of step `it`: its 16 tokens, on page `entry` --
+  auto copy = [&](int h, int lo, int hi, int it, int entry) {
+    const int t = lo + it * A::kStep + 16 * cg, page = is_there(hi, t, entry) ? entry : 0;
+    const int64_t at = (((int64_t)page * a.cache.heads + h) << a.page_shift) + (t & ((1 << a.page_shift) - 1));
+    const uint8_t* codes = a.cache.k_codes + at * (WK / 2);
+    const uint8_t* scales = a.cache.k_scales + at * scale_pitch(WK);
+    auto stage = [&](int at) { return (uint32_t)uniform((int)(mxd::lds_addr(lds) + A::kRing + (it % A::kStages) * A::kStage) + at); };
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {   // four tokens, their pieces changed about by the token
+      const uint32_t token = 4 * j + quad, piece = l16 ^ (token & 7);
+      mxd::global_to_lds16(codes + (token * (WK / 2) + piece * 16), stage((16 * cg + 4 * j) * 256));
+    }
+    if (lane < 16) mxd::global_to_lds16(scales + lane * scale_pitch(WK), stage(A::kScales + 256 * cg));
+    if constexpr (kPart) {
+      if (lane < 32) mxd::global_to_lds16(codes + ((lane >> 1) * (WK / 2) + 256 + (lane & 1) * 16), stage(A::kTail + 512 * cg));
+      if (lane < 16) mxd::global_to_lds4(scales + lane * scale_pitch(WK) + 16, stage(A::kTailScales + 64 * cg));
+    }
+  };
+  auto begin = [&] {   // a unit's first step, asked for while the unit before ends
+    copy(u.h, u.lo, u.hi, u.it0, entry_of(table_of(), u.hi, u.lo + u.it0 * A::kStep + 16 * cg));
+  };
+  auto query_row = [&] {   // a lane's, of the 16 of row quarter rq
+    const int row = min(u.tile * A::kRows + rq * 16 + l16, u.s.n * a.group - 1);
+    return a.q.q + (u.s.first + a.by_group.of(row)) * a.q.q_stride + (int64_t)(u.h * a.group + a.by_group.rest(row)) * WK + 16 * quad;
+  };
+  // -- the first unit's queries, KS steps of 128 values, converted by the rows' 8 / RQ waves together and exchanged --
+  uint4* const made = (uint4*)lds + rq * A::kMade + lane;
+  uint32_t* const made_scales = (uint32_t*)(lds + RQ * A::kMade * 16) + rq * (KS * 64) + lane;
+  {
     constexpr int kSharers = 8 / RQ, kEach = (KS + kSharers - 1) / kSharers;
     const int sharer = wave / RQ;
-    const uint16_t* q = a.q.q + (u.s.first + i) * a.q.q_stride + (int64_t)(h * a.group + a.by_group.rest(row)) * WK;
+    const uint16_t* q = query_row();
     QueryWords words[kEach];
 #pragma unroll
     for (int e = 0; e < kEach; ++e) {
       const int k = e * kSharers + sharer;
-      if (KS % kSharers == 0 || k < KS) words[e] = query_words(q + 128 * k + 16 * quad, kPart && k == KS - 1);
+      if (KS % kSharers == 0 || k < KS) words[e] = query_words(q + 128 * k, kPart && k == KS - 1);
     }
-    // -- pages: 16 tokens have one --
-    const __attribute__((address_space(4))) int32_t* table =
-        (const __attribute__((address_space(4))) int32_t*)(a.q.table + (int64_t)u.b * a.q.columns);
-    auto entry_of = [&](int t) { return table[min(t, max(hi - 1, 0)) >> a.page_shift]; };
-    auto is_there = [&](int t, int entry) { return t < hi && (uint32_t)entry < (uint32_t)a.cache.pages; };
-    // a step's four entries are asked for a step before they are looked at, so that nobody waits for them; bit t: 16 tokens
-    int entries[4];
-    auto ask = [&](int it) {
-#pragma unroll
-      for (int t = 0; t < 4; ++t) entries[t] = entry_of(lo + it * A::kStep + 16 * t);
-    };
-    auto shown_of = [&](int it) {
-      uint32_t shown = 0;
-#pragma unroll
-      for (int t = 0; t < 4; ++t) shown |= is_there(lo + it * A::kStep + 16 * t, entries[t]) ? 1u << t : 0u;
-      return shown;
-    };
-    // -- a value wave's copies of step `it`: its 16 tokens, on page `entry` --
-    auto copy = [&](int it, int entry) {
-      const int t = lo + it * A::kStep + 16 * cg, page = is_there(t, entry) ? entry : 0;
-      const int64_t at = (((int64_t)page * a.cache.heads + h) << a.page_shift) + (t & ((1 << a.page_shift) - 1));
-      const uint8_t* codes = a.cache.k_codes + at * (WK / 2);
-      const uint8_t* scales = a.cache.k_scales + at * scale_pitch(WK);
-      const uint32_t stage = (uint32_t)uniform((int)(mxd::lds_addr(lds) + A::kRing + (it % A::kStages) * A::kStage));
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {   // four tokens, their pieces changed about by the token
-        const uint32_t token = 4 * j + quad, piece = l16 ^ (token & 7);
-        mxd::global_to_lds16(codes + (token * (WK / 2) + piece * 16), stage + (16 * cg + 4 * j) * 256);
-      }
-      if (lane < 16) mxd::global_to_lds16(scales + lane * scale_pitch(WK), stage + A::kScales + 256 * cg);
-      if constexpr (kPart) {
-        if (lane < 32) mxd::global_to_lds16(codes + ((lane >> 1) * (WK / 2) + 256 + (lane & 1) * 16), stage + A::kTail + 512 * cg);
-        if (lane < 16) mxd::global_to_lds4(scales + lane * scale_pitch(WK) + 16, stage + A::kTailScales + 64 * cg);
-      }
-    };
-    ask(it0);
-    int first_entries[A::kStages - 1];
-    if (wave >= 4) {
-#pragma unroll
-      for (int k = 0; k < A::kStages - 1; ++k) first_entries[k] = entry_of(lo + (it0 + k) * A::kStep + 16 * cg);
-      copy(it0, first_entries[0]);
-    }
-    uint32_t shown = shown_of(it0);
-    // -- the queries, converted and exchanged --
-    uint4* made = (uint4*)lds + rq * A::kMade + lane;
-    uint32_t* made_scales = (uint32_t*)(lds + RQ * A::kMade * 16) + rq * (KS * 64) + lane;
-    __syncthreads();   // the plan, or the last unit's rows, have been read
+    if (wave >= 4) begin();
+    if (by == kInLds) __syncthreads();   // the plan has been read
 #pragma unroll
     for (int e = 0; e < kEach; ++e) {
       const int k = e * kSharers + sharer;
@@ -703,29 +701,51 @@ __global__ __launch_bounds__(512, 2) void latent_kernel(AttendArgs a, int by) {
       }
       made_scales[k * 64] = s.scales;
     }
-    if (wave >= 4) {   // (the queries come before these)
+  }
+  if (wave < 4) {
+    // -- further units': by the score waves, asked for while the unit before ends, where the registers hold them --
+    constexpr bool kAhead = !kPart;
+    QueryWords words[KS];
+    auto load = [&] {
+      const uint16_t* q = query_row();
 #pragma unroll
-      for (int k = 1; k < A::kStages - 1; ++k)
-        if (it0 + k < it1) copy(it0 + k, first_entries[k]);
-    }
-    const bool alone = is_alone(u);
-    const int64_t slot = 2 * g + (u.first ? 0 : 1);
-
-    if (wave < 4) {
-      mxd::lds_barrier();
+      for (int k = 0; k < KS; ++k) words[k] = query_words(q + 128 * k, kPart && k == KS - 1);
+    };
+    bool exchanged = true;
+    mxd::lds_barrier();
+    for (;;) {
+      const int it0 = u.it0, it1 = u.it1, lo = u.lo, hi = u.hi;
+      Entry* const table = table_of();
+      const bool alone = is_alone(u);
+      const int64_t slot = 2 * g + (u.first ? 0 : 1);
+      ask(table, lo, hi, it0);
+      uint32_t shown = shown_of(lo, hi, it0);
+      const int h = u.h, first_token = u.s.first, rows = u.s.n * a.group, row0 = u.tile * A::kRows;   // rows at most 2^30
       v8i qh[KS], ql[KS];
       uint32_t qs[(KS + 1) / 2] = {};
+      if (exchanged) {
 #pragma unroll
-      for (int k = 0; k < KS; ++k) {
-        const bool last = kPart && k == 4;
-        const uint4 h0 = made[k * 256], l0 = made[k * 256 + (last ? 64 : 128)];
-        const uint4 h1 = last ? make_uint4(0u, 0u, 0u, 0u) : made[k * 256 + 64], l1 = last ? make_uint4(0u, 0u, 0u, 0u) : made[k * 256 + 192];
-        qh[k] = {(int)h0.x, (int)h0.y, (int)h0.z, (int)h0.w, (int)h1.x, (int)h1.y, (int)h1.z, (int)h1.w};
-        ql[k] = {(int)l0.x, (int)l0.y, (int)l0.z, (int)l0.w, (int)l1.x, (int)l1.y, (int)l1.z, (int)l1.w};
-        qs[k / 2] |= made_scales[k * 64] << (16 * (k & 1));
+        for (int k = 0; k < KS; ++k) {
+          const bool last = kPart && k == 4;
+          const uint4 h0 = made[k * 256], l0 = made[k * 256 + (last ? 64 : 128)];
+          const uint4 h1 = last ? make_uint4(0u, 0u, 0u, 0u) : made[k * 256 + 64], l1 = last ? make_uint4(0u, 0u, 0u, 0u) : made[k * 256 + 192];
+          qh[k] = {(int)h0.x, (int)h0.y, (int)h0.z, (int)h0.w, (int)h1.x, (int)h1.y, (int)h1.z, (int)h1.w};
+          ql[k] = {(int)l0.x, (int)l0.y, (int)l0.z, (int)l0.w, (int)l1.x, (int)l1.y, (int)l1.z, (int)l1.w};
+          qs[k / 2] |= made_scales[k * 64] << (16 * (k & 1));
+        }
+      } else {
+        if (!kAhead) load();
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+          const QueryStep s = query_step16(words[k], l16, quad);
+#pragma unroll
+          for (int n = 0; n < 8; ++n) qh[k][n] = (int)s.high[n], ql[k][n] = (int)s.low[n];
+          qs[k / 2] |= s.scales << (16 * (k & 1));
+        }
       }
+      exchanged = false;
       int row_lo, row_hi;
-      seen(a, u.s, i, row_lo, row_hi);
+      seen(a, u.s, a.by_group.of(min(row0 + rq * 16 + l16, rows - 1)), row_lo, row_hi);
       // tokens [all_lo, all_hi) are seen by all of the wave's rows
       int all_lo, all_hi, unused;
       seen(a, u.s, a.by_group.of(min(row0 + rq * 16, rows - 1)), unused, all_hi);
@@ -736,11 +756,11 @@ __global__ __launch_bounds__(512, 2) void latent_kernel(AttendArgs a, int by) {
       uint8_t* const put_w = weights + (tt * T2 * A::kRows + rq * 16 + l16) * 32 + (quad & 1) * 16 + (quad >> 1) * 8;
       float m = kLowest, l = 0.f;
       float own = kLowest, sum = 0.f;
-      mxd::copy_barrier();   // the first step is there, and the queries have been read
+      mxd::copy_barrier();   // the first step is there, and exchanged queries have been read
       for (int it = it0; it < it1; ++it) {
         const uint8_t* stage = lds + A::kRing + (it % A::kStages) * A::kStage;
         const int first = lo + it * A::kStep + tt * T2 * 16;
-        ask(it + 1);
+        ask(table, lo, hi, it + 1);
         mxd::v4f sc[T2];
         uint32_t ks[T2], klast[T2];
 #pragma unroll
@@ -809,9 +829,11 @@ __global__ __launch_bounds__(512, 2) void latent_kernel(AttendArgs a, int by) {
           l = l * power(m, own) + sum;
           m = own;
         }
-        shown = shown_of(it + 1);
+        shown = shown_of(lo, hi, it + 1);
         mxd::copy_barrier();
       }
+      const bool more = go_on(1);
+      if (kAhead && more) load();
       if constexpr (TT > 1) {
         float next = kLowest;
 #pragma unroll
@@ -832,7 +854,7 @@ __global__ __launch_bounds__(512, 2) void latent_kernel(AttendArgs a, int by) {
         if (row0 + r < rows) {
           if (alone) {
             const int head = h * a.group + a.by_group.rest(row0 + r);
-            const int64_t token = u.s.first + a.by_group.of(row0 + r);
+            const int64_t token = first_token + a.by_group.of(row0 + r);
             const RowOut f = row_out(a, head, stats[r][0][0], all_l);
             to = {token * a.q.out_stride + (int64_t)head * WV, f.inv};
             if (a.q.lse) a.q.lse[token * a.q.heads + head] = f.lse;
@@ -843,16 +865,32 @@ __global__ __launch_bounds__(512, 2) void latent_kernel(AttendArgs a, int by) {
         places[r] = to;
       }
       __syncthreads();
-    } else {
-      // LDS places of the wave's values: a converter's 16-byte pieces of its token, and a reader's 8 bytes
-      uint8_t* tile = lds + cg * A::kTile;
-      uint32_t put[4];
+      if (!more) return;
+    }
+  } else {
+    // LDS places of the wave's values: a converter's 16-byte pieces of its token, and a reader's 8 bytes
+    uint8_t* tile = lds + cg * A::kTile;
+    uint32_t put[4];
 #pragma unroll
-      for (int n = 0; n < 4; ++n) put[n] = l16 * 256 + 128 * (quad >> 1) + ((4 * (quad & 1) + n) ^ spread) * 16;
-      const int rt = l16 >> 2, rc = lane & 3, rs = 2 * rt + half;
-      const uint32_t get0 = (4 * half + rt) * 256 + ((2 * (quad & 1) + rc / 2) ^ rs) * 16 + (rc & 1) * 8, get1 = get0 ^ 64;
-      const uint32_t get_c = l16 * 256 + (((4 * (cg & 1) + quad) ^ (l16 & 7)) * 16) + 128 * (cg >> 1);   // the columns' codes
-      const uint32_t get_s = A::kScales + l16 * 16 + 4 * cg;
+    for (int n = 0; n < 4; ++n) put[n] = l16 * 256 + 128 * (quad >> 1) + ((4 * (quad & 1) + n) ^ spread) * 16;
+    const int rt = l16 >> 2, rc = lane & 3, rs = 2 * rt + half;
+    const uint32_t get0 = (4 * half + rt) * 256 + ((2 * (quad & 1) + rc / 2) ^ rs) * 16 + (rc & 1) * 8, get1 = get0 ^ 64;
+    const uint32_t get_c = l16 * 256 + (((4 * (cg & 1) + quad) ^ (l16 & 7)) * 16) + 128 * (cg >> 1);   // the columns' codes
+    const uint32_t get_s = A::kScales + l16 * 16 + 4 * cg;
+    bool exchanged = true;
+    for (;;) {
+      const int it0 = u.it0, it1 = u.it1, lo = u.lo, hi = u.hi;
+      Entry* const table = table_of();
+      const bool alone = is_alone(u);
+      const int64_t slot = 2 * g + (u.first ? 0 : 1);
+      ask(table, lo, hi, it0);
+      uint32_t shown = shown_of(lo, hi, it0);
+      const int h = u.h;
+#pragma unroll
+      for (int k = 1; k < A::kStages - 1; ++k)
+        if (it0 + k < it1) copy(h, lo, hi, it0 + k, entry_of(table, hi, lo + (it0 + k) * A::kStep + 16 * cg));
+      if (exchanged) mxd::lds_barrier();   // (the queries)
+      exchanged = false;
       float m[RG];
       v16f o[RG][4];
 #pragma unroll
@@ -953,19 +991,18 @@ __global__ __launch_bounds__(512, 2) void latent_kernel(AttendArgs a, int by) {
 #pragma unroll
           for (int i = 0; i < RG; ++i) o[i][d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(r.v[d], r.p[i], o[i][d], 0, 0, 0);
       };
-      int entry = entry_of(lo + (it0 + A::kStages - 1) * A::kStep + 16 * cg);   // of the next copies
-      auto next_entry = [&](int it) { return entry_of(lo + (it + A::kStages) * A::kStep + 16 * cg); };
+      int entry = entry_of(table, hi, lo + (it0 + A::kStages - 1) * A::kStep + 16 * cg);   // of the next copies
+      auto next_entry = [&](int it) { return entry_of(table, hi, lo + (it + A::kStages) * A::kStep + 16 * cg); };
       // this wave's copies of the step after `it` have landed; those of later steps may be on their way
       auto landed = [&](int it) {
         if (it + A::kStages - 1 < it1) {
-          copy(it + A::kStages - 1, entry);
+          copy(h, lo, hi, it + A::kStages - 1, entry);
           __builtin_amdgcn_s_waitcnt(mxd::vm_wait_imm(A::kCopies * (A::kStages - 2)));
         } else {
           __builtin_amdgcn_s_waitcnt(mxd::vm_wait_imm(0));
         }
         asm volatile("" ::: "memory");
       };
-      mxd::lds_barrier();   // (the queries)
       if (it0 + A::kStages - 1 <= it1) {   // the first step's copies have landed
         __builtin_amdgcn_s_waitcnt(mxd::vm_wait_imm(A::kCopies * (A::kStages - 2)));
       } else {
@@ -975,11 +1012,11 @@ __global__ __launch_bounds__(512, 2) void latent_kernel(AttendArgs a, int by) {
       mxd::copy_barrier();
 #pragma unroll
       for (int t = 0; t < 4; ++t) convert(codes_of(it0, t), t);
-      ask(it0 + 1);
+      ask(table, lo, hi, it0 + 1);
       int asked = next_entry(it0);
       landed(it0);
       entry = asked;
-      shown = shown_of(it0 + 1);
+      shown = shown_of(lo, hi, it0 + 1);
       mxd::copy_barrier();
       for (int it = it0 + 1; it < it1; ++it) {
         // everything is read from LDS a turn before it is used: 16 tokens' products, under which the next ones' operands come
@@ -988,7 +1025,7 @@ __global__ __launch_bounds__(512, 2) void latent_kernel(AttendArgs a, int by) {
         Codes next[4];
 #pragma unroll
         for (int t = 0; t < 4; ++t) next[t] = codes_of(it, t);
-        ask(it + 1);
+        ask(table, lo, hi, it + 1);
         Operands now = operands(it - 1, 0);
         settle(it - 1);
 #pragma unroll
@@ -1001,9 +1038,11 @@ __global__ __launch_bounds__(512, 2) void latent_kernel(AttendArgs a, int by) {
         }
         landed(it);
         entry = asked;
-        shown = shown_of(it + 1);
+        shown = shown_of(lo, hi, it + 1);
         mxd::copy_barrier();
       }
+      const bool more = go_on(1);   // (the stages are free, and the values are read last)
+      if (more) begin();
       settle(it1 - 1);
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
@@ -1041,9 +1080,8 @@ __global__ __launch_bounds__(512, 2) void latent_kernel(AttendArgs a, int by) {
             for (int n = 0; n < 4; ++n)
               part[((r * 4 + d) * 4 + n) * 64] = make_float4(o[r][d][4 * n], o[r][d][4 * n + 1], o[r][d][4 * n + 2], o[r][d][4 * n + 3]);
       }
+      if (!more) return;
     }
-    if (!go_on()) return;
-    __syncthreads();   // what went out has been read before the next unit's copies and queries come
   }
 }
 
