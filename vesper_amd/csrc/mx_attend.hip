@@ -40,8 +40,8 @@ constexpr int kInlineTiles = 1024;   // row tiles of all sequences that every wo
 // Where the plan is made: in the workspace by a launch of its own, in every workgroup's LDS, or, up to 64 tiles, in the
 // registers of every wave.
 constexpr int kInSpace = 0, kInLds = 1, kByWave = 2;
-// What a unit's beginning and end cost, in iterations. With 2, 4, 6 and 8: the 48 sequences below 71, 61, 63 and 63 us, two
-// prompts 365, 361, 360 and 356.
+// What a unit's beginning and end cost, in iterations. With 3, 4, 5 and 6: the 48 sequences below 63.7, 62.9, 63.7 and 64.1 us,
+// drafts over 576-wide latents 84.1, 84.1, 86.2 and 85.8.
 constexpr int kBegin = 4;
 constexpr float kLowest = -3e38f;    // the maximum of a row that has seen nothing yet
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
@@ -535,12 +535,15 @@ __device__ __forceinline__ float power(float from, float to) {   // 2^(from - to
 // on under the other's products; one barrier a step. Codes and scales come to LDS by copies that nobody waits for, kStages -
 // 1 steps ahead, once for all waves.
 //
-// Measured at 64 heads of 512 over 48 sequences of 200 to 30,000 tokens (86 MB, 39 GFLOP): 55 us and 10 us for the joining,
-// 650 TFLOP/s in the first. A step takes about 3,400 clocks, its products 2,048 of a SIMD's and its LDS traffic about 1,950;
-// a workgroup's first unit about 17,000 before its first step (the plan 4,000, its place 3,500, the queries from the caches
-// and into their terms 9,000), each further one 9,500, and its way out 4,000 to 5,000. Before the roles were parted, with
-// eight waves that all scored and multiplied: 120 us. What was slower: the next unit's queries and copies asked for before
-// this one's end (72 us in place of 61 for both kernels: 256 registers no longer hold it).
+// A workgroup's first queries are converted by all eight waves, later units' by the score waves while the value waves finish
+// the unit before; its first copies are asked for before its last products.
+//
+// Measured at 64 heads of 512 over 48 sequences of 200 to 30,000 tokens (86 MB, 39 GFLOP): 58 us and 10 us for the joining,
+// 667 TFLOP/s in the first. A step takes about 3,500 clocks, its products 2,048 of a SIMD's and its LDS traffic about 1,950; a
+// workgroup has its first queries after about 17,000 (5,500 for the division, the rest the queries, from the caches beside
+// the first copies), and its way out takes 5,000. Before the roles were parted, with eight waves that all scored and
+// multiplied, both took 120 us. Not faster: priorities for either role (61 to 63 us for both kernels in place of 61), all of a
+// unit's first copies before the rows of the one before go out (windows of 128 over prompts 124 us in place of 122).
 template <int WK, int RG>
 struct Latent {
   static constexpr int WV = 512, RQ = 2 * RG, TT = 4 / RQ, T2 = 4 / TT, kRows = 32 * RG, kStep = 64;
