@@ -83,3 +83,19 @@ def test_one_token_is_its_values(gpu_ctx, kind, heads, kv_heads, columns):
         got = bf16_values(cache.attend(bf16_bits(q), table, lengths, cache.width ** -0.5)["out"])
         for b in range(9):
             np.testing.assert_array_equal(got[b], values[b][0].repeat(heads // kv_heads, 0))
+
+
+@pytest.mark.parametrize("kind,heads,kv_heads", [("512", 40, 1), ("576", 16, 1), ("64", 14, 2), ("128", 32, 8), ("256", 8, 2)])
+@pytest.mark.parametrize("given", [False, True])
+@pytest.mark.parametrize("columns", [None, 1 << 14])
+def test_some_hundred_sequences(gpu_ctx, kind, heads, kv_heads, given, columns):
+    """More row tiles than a wave has lanes, fewer than a workgroup counts, with and without rows of empty sequences."""
+    rng, page = np.random.default_rng(heads + given), 16
+    lengths = np.concatenate([rng.integers(0, 90, 180), [2000, 0, 1]])
+    counts = (rng.integers(0, 3, lengths.size) * (lengths > 2)) if given else np.ones(lengths.size, int)
+    table, pages = pages_for(rng, lengths, page, columns=columns)
+    with open_cache(gpu_ctx, kind, pages, page, kv_heads, heads) as cache:
+        keys, values = fill(cache, rng, table, lengths)
+        q = bf16_round(rng.standard_normal((int(counts.sum()), heads, cache.width)).astype(np.float32))
+        want = oracle.attend(q, keys, values, lengths, counts, 0.05)
+        check(cache.attend(bf16_bits(q), table, lengths, 0.05, counts if given else None), q, keys, lengths, 0.05, *want)
