@@ -269,8 +269,14 @@ __device__ __forceinline__ void next_unit(const AttendArgs& a, Units& u, int row
   if (u.x >= u.end) return;
   if (++u.tile == u.tiles) {
     u.tile = 0;
-    do {   // (there is another, since costs are left)
-      if (++u.b == a.q.batch) u.b = 0, ++u.h;
+    do {   // (there is another, since costs are left, unless somebody changes the sequences meanwhile)
+      if (++u.b == a.q.batch) {
+        u.b = 0;
+        if (++u.h == a.cache.heads) {
+          u.x = u.end;
+          return;
+        }
+      }
       u.s = uniform(sequence(a, u.b));
       u.tiles = tiles_of(a, u.s, rows);
     } while (u.tiles == 0);
@@ -371,10 +377,10 @@ __device__ __forceinline__ bool first_of_few(const AttendArgs& a, int g, int64_t
 // The unit's end in this workgroup: `alone` it has all of it. The workgroup's last unit, if it began it and does not end it,
 // is joined from there on.
 __device__ __forceinline__ bool is_alone(const Units& u) { return u.it0 == 0 && u.it1 == u.n; }
-__device__ __forceinline__ void note(const Units& u, int64_t per, int g, Shared* shared) {
+__device__ __forceinline__ void note(const Units& u, int64_t per, int g, int groups, Shared* shared) {
   Shared v{u.b, u.h, u.tile, 0, u.first ? 0 : 1};
   const int64_t end = u.unit0 + kBegin + u.n;
-  if (u.it0 == 0 && u.it1 > 0 && u.it1 < u.n) v.parts = few(end - 1, per) - g + 1;
+  if (u.it0 == 0 && u.it1 > 0 && u.it1 < u.n) v.parts = min(few(end - 1, per), groups - 1) - g + 1;
   *shared = v;
 }
 
@@ -611,13 +617,12 @@ __global__ __launch_bounds__(512, 2) void latent_kernel(AttendArgs a, int by) {
   // workgroups go round the XCDs: neighbours in the work, which share keys, to one L2
   const int g = (int)(blockIdx.x % kXcds) * (kCus / kXcds) + (int)blockIdx.x / kXcds;
   Shared* shared = (Shared*)(a.space + a.at.units) + g;
+  if (tid == 0) shared->parts = 0;
   int64_t per;
   Units u;
   if (!(by == kByWave ? first_of_few(a, g, per, kCus, u, A::kRows, A::kStep)
-                      : first_unit<512>(a, plan, by == kInLds, g, per, kCus, found, u, A::kRows, A::kStep))) {
-    if (tid == 0) shared->parts = 0;
+                      : first_unit<512>(a, plan, by == kInLds, g, per, kCus, found, u, A::kRows, A::kStep)))
     return;
-  }
 
   const int spread = 2 * (l16 & 3) + ((l16 >> 2) & 1);   // pieces of 16 bytes of neighbouring tokens' values lie apart
   // To the next unit of which iterations are this workgroup's, from `ahead` units on: whether there is one. Every wave goes
@@ -625,7 +630,7 @@ __global__ __launch_bounds__(512, 2) void latent_kernel(AttendArgs a, int by) {
   auto go_on = [&](int ahead) {
     for (;; ahead = 1) {
       if (ahead) {
-        if (u.end <= u.unit0 + kBegin + u.n && tid == 0) note(u, per, g, shared);
+        if (u.end <= u.unit0 + kBegin + u.n && tid == 0) note(u, per, g, kCus, shared);
         next_unit(a, u, A::kRows, A::kStep);
         if (u.x >= u.end) return false;
       }
@@ -1133,13 +1138,12 @@ __global__ __launch_bounds__(256, (Grouped<W, RG>::kWaves)) void grouped_kernel(
   // workgroups go round the XCDs: neighbours in the work, which share keys, to one L2
   const int g = (int)(blockIdx.x % kXcds) * (groups / kXcds) + (int)blockIdx.x / kXcds;
   Shared* shared = (Shared*)(a.space + a.at.units) + g;
+  if (tid == 0) shared->parts = 0;
   int64_t per;
   Units u;
   if (!(by == kByWave ? first_of_few(a, g, per, groups, u, A::kRows, A::kStep)
-                      : first_unit<256>(a, plan, by == kInLds, g, per, groups, found, u, A::kRows, A::kStep))) {
-    if (tid == 0) shared->parts = 0;
+                      : first_unit<256>(a, plan, by == kInLds, g, per, groups, found, u, A::kRows, A::kStep)))
     return;
-  }
 
   // LDS places: a loader's 16-byte pieces of its token, and a reader's 8 bytes; pieces of neighbouring tokens lie apart
   const int spread = 2 * (col & 3) + ((col >> 2) & 1);
@@ -1151,7 +1155,7 @@ __global__ __launch_bounds__(256, (Grouped<W, RG>::kWaves)) void grouped_kernel(
   const uint32_t get1 = get0 ^ 64;
 
   auto go_on = [&] {   // to the next unit, if there is one
-    if (u.end <= u.unit0 + kBegin + u.n && tid == 0) note(u, per, g, shared);
+    if (u.end <= u.unit0 + kBegin + u.n && tid == 0) note(u, per, g, groups, shared);
     next_unit(a, u, A::kRows, A::kStep);
     return u.x < u.end;
   };
