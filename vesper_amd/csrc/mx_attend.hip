@@ -783,31 +783,17 @@ __global__ __launch_bounds__(512, 2) void latent_kernel(AttendArgs a, int by) {
           }
         }
         auto codes = [&](int k, int t) { return *(const uint4*)(stage + (get_k ^ (k & 1 ? 64 : 0)) + 128 * (k >> 1) + 4096 * t); };
-#pragma unroll
-        for (int t = 0; t < T2; ++t) sc[t] = score_step<0>(codes(0, t), qh[0], ql[0], sc[t], ks[t], qs[0]);
-#pragma unroll
-        for (int t = 0; t < T2; ++t) sc[t] = score_step<1>(codes(1, t), qh[1], ql[1], sc[t], ks[t], qs[0]);
-#pragma unroll
-        for (int t = 0; t < T2; ++t) sc[t] = score_step<2>(codes(2, t), qh[2], ql[2], sc[t], ks[t], qs[1]);
-#pragma unroll
-        for (int t = 0; t < T2; ++t) sc[t] = score_step<3>(codes(3, t), qh[3], ql[3], sc[t], ks[t], qs[1]);
-        if constexpr (kPart) {
-#pragma unroll
-          for (int t = 0; t < T2; ++t) {
+        auto score = [&](int t) {
+          sc[t] = score_step<0>(codes(0, t), qh[0], ql[0], sc[t], ks[t], qs[0]);
+          sc[t] = score_step<1>(codes(1, t), qh[1], ql[1], sc[t], ks[t], qs[0]);
+          sc[t] = score_step<2>(codes(2, t), qh[2], ql[2], sc[t], ks[t], qs[1]);
+          sc[t] = score_step<3>(codes(3, t), qh[3], ql[3], sc[t], ks[t], qs[1]);
+          if constexpr (kPart) {
             uint4 w = *(const uint4*)(stage + A::kTail + ((tt * T2 + t) * 16 + l16) * 32 + (quad & 1) * 16);
             w = quad > 1 ? make_uint4(0u, 0u, 0u, 0u) : w;
             sc[t] = score_step<4>(w, qh[KS - 1], ql[KS - 1], sc[t], klast[t], qs[2]);
           }
-        }
-        if (shown != 15u || first < all_lo || first + 16 * T2 > all_hi) {
-#pragma unroll
-          for (int t = 0; t < T2; ++t)
-#pragma unroll
-            for (int n = 0; n < 4; ++n) {
-              const int at = first + 16 * t + 4 * quad + n;
-              sc[t][n] = (shown >> (tt * T2 + t) & 1) && at >= row_lo && at < row_hi ? sc[t][n] : -INFINITY;
-            }
-        }
+        };
         if constexpr (TT > 1) {
           if (it > it0) {   // the maximum with the last step's of the row's other waves
             float next = kLowest;
@@ -817,20 +803,44 @@ __global__ __launch_bounds__(512, 2) void latent_kernel(AttendArgs a, int by) {
             m = next;
           }
         }
-        float top = fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3]));
-#pragma unroll
-        for (int t = 1; t < T2; ++t) top = fmaxf(top, fmaxf(fmaxf(sc[t][0], sc[t][1]), fmaxf(sc[t][2], sc[t][3])));
-        top = row_max4(top) * a.c;
-        own = m;
-        if (__any(top > m + 8.f)) own = raised(m, top);
-        sum = 0.f;
-#pragma unroll
-        for (int t = 0; t < T2; ++t) {
+        own = m, sum = 0.f;
+        float top = -INFINITY;
+        auto weigh = [&](int t) {   // the probabilities of 16 tokens
           float p[4];
 #pragma unroll
           for (int n = 0; n < 4; ++n) p[n] = __builtin_amdgcn_exp2f(fmaf(sc[t][n], a.c, -own));
           sum += (p[0] + p[1]) + (p[2] + p[3]);
           *(uint2*)(put_w + (it & 1) * A::kWeights + t * (A::kRows * 32)) = make_uint2(mxd::bf16_pair(p[0], p[1]), mxd::bf16_pair(p[2], p[3]));
+        };
+        auto look = [&](int t) { top = fmaxf(top, fmaxf(fmaxf(sc[t][0], sc[t][1]), fmaxf(sc[t][2], sc[t][3]))); };
+        const bool plain = shown == 15u && first >= all_lo && first + 16 * T2 <= all_hi;
+        if (plain) {   // under the maximum so far, which seldom rises: 16 tokens' probabilities beside the next ones' scores
+          score(0);
+#pragma unroll
+          for (int t = 0; t < T2; ++t) {
+            if (t + 1 < T2) score(t + 1);
+            look(t), weigh(t);
+          }
+        } else {
+#pragma unroll
+          for (int t = 0; t < T2; ++t) score(t);
+#pragma unroll
+          for (int t = 0; t < T2; ++t) {
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+              const int at = first + 16 * t + 4 * quad + n;
+              sc[t][n] = (shown >> (tt * T2 + t) & 1) && at >= row_lo && at < row_hi ? sc[t][n] : -INFINITY;
+            }
+            look(t);
+          }
+        }
+        top = row_max4(top) * a.c;
+        const bool rises = __any(top > m + 8.f);
+        if (rises) own = raised(m, top);
+        if (!plain || rises) {
+          sum = 0.f;
+#pragma unroll
+          for (int t = 0; t < T2; ++t) weigh(t);
         }
         if (quad == 0) tops[it & 1][rq * 16 + l16][tt] = own;
         if constexpr (TT == 1) {
