@@ -534,7 +534,8 @@ __device__ __forceinline__ float power(float from, float to) {   // 2^(from - to
 
 // Latents. A step is 64 tokens, for 64 (RG = 2) or 32 rows, of eight waves, two a SIMD:
 //   four score waves: 16 rows and 64 (32) tokens each, by V_MFMA_SCALE_F32_16X16X128_F8F6F4 with the rows' queries in 64
-//     registers; then the softmax of these, and the probabilities to LDS;
+//     registers; and the softmax of these, 16 tokens' beside the next ones' scores, under the maximum so far (drafts over
+//     576-wide latents 78.6 us, with all scores first 82.9), and the probabilities to LDS;
 //   four value waves: 128 columns and all rows each. Each converts its columns of the step's tokens into an LDS tile of its
 //     own, between the products of the last step's values with the last step's probabilities.
 // So the matrix units have a score wave's and a value wave's products to choose from, and each wave's other instructions go
@@ -544,8 +545,8 @@ __device__ __forceinline__ float power(float from, float to) {   // 2^(from - to
 // A workgroup's first queries are converted by all eight waves, later units' by the score waves while the value waves finish
 // the unit before; its first copies are asked for before its last products.
 //
-// Measured at 64 heads of 512 over 48 sequences of 200 to 30,000 tokens (86 MB, 39 GFLOP): 58 us and 10 us for the joining,
-// 667 TFLOP/s in the first. A step takes about 3,500 clocks, its products 2,048 of a SIMD's and its LDS traffic about 1,950; a
+// Measured at 64 heads of 512 over 48 sequences of 200 to 30,000 tokens (86 MB, 39 GFLOP): 56 us and 10 us for the joining,
+// 690 TFLOP/s in the first. A step takes about 3,500 clocks, its products 2,048 of a SIMD's and its LDS traffic about 1,950; a
 // workgroup has its first queries after about 17,000 (5,500 for the division, the rest the queries, from the caches beside
 // the first copies), and its way out takes 5,000. Before the roles were parted, with eight waves that all scored and
 // multiplied, both took 120 us. Not faster: priorities for either role (61 to 63 us for both kernels in place of 61), all of a
