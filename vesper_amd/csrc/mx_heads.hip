@@ -132,7 +132,7 @@ __global__ __launch_bounds__(256) void rotate_backward_kernel(GradArgs a) {
       for (int j = 0; j < 8; ++j) sum = fma((double)u[i][j], (double)u[i][j], sum);
     }
     if (norm) {
-      const float r = root(group_sum<L>(sum), norm, a.rot.eps);
+      const float whole = root(group_sum<L>(sum), norm, a.rot.eps), r = counts ? whole : 0.f;   // (infinite where eps is zero)
       float dot = 0.f;
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
@@ -151,6 +151,12 @@ __global__ __launch_bounds__(256) void rotate_backward_kernel(GradArgs a) {
         if (cols.normed[i])
 #pragma unroll
           for (int j = 0; j < 8; ++j) d[i][j] = r * (d[i][j] - u[i][j] * mean);
+    }
+    if (!__all(counts)) {   // zero whatever the weights are
+#pragma unroll
+      for (int i = 0; i < NI; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) d[i][j] = counts ? d[i][j] : 0.f;
     }
     if (!there) continue;
 #pragma unroll
