@@ -466,7 +466,8 @@ class CachedAttention:
         """y [T, hidden] of x [T, hidden], both BF16: the tokens' latents go into device int64 slots [T] (outside the
         cache: not stored) at int32 positions [T], then each token attends to its sequence's `lengths` [batch] tokens on
         pages `table` [batch, columns], its own among them. The tokens are the last of their sequences: as many of each,
-        or those that int32 q_first [batch + 1] gives. Rows of no sequence have nothing to say in y."""
+        or those that int32 q_first [batch + 1] gives. Rows of y behind the last sequence are of no use: what an earlier
+        step left of its attention, projected."""
         self._open()
         if not 0 <= tokens <= self.max_tokens or not 0 <= batch <= self.cache.max_batch:
             raise ValueError(f"the cache was opened for {self.max_tokens} tokens of {self.cache.max_batch} sequences a call")
@@ -498,7 +499,8 @@ class CachedAttention:
     # -- host arrays -------------------------------------------------------------------------------
     def step(self, x, positions, slots, table, lengths, counts=None) -> np.ndarray:
         """y [T, hidden] BF16 bits: x [T, hidden] BF16 bits, positions [T], slots [T], table [B, columns] and lengths [B]
-        with the tokens of this step; counts [B] of them of each sequence (None: as many of each)."""
+        with the tokens of this step; counts [B] of them of each sequence (None: as many of each). Rows behind the last
+        sequence are stored where they have a slot, and zero in y."""
         with self.projections.lock:
             self._open()
             t = validate_values(x, self.hidden)
@@ -514,7 +516,10 @@ class CachedAttention:
                 dev.append(self.ctx.empty((t, self.hidden), np.uint16))
                 ptr = [None if d is None else d.ptr for d in dev]
                 self.step_device(ptr[0], t, ptr[1], ptr[2], ptr[3], table.shape[1], ptr[4], lengths.shape[0], ptr[6], ptr[5])
-                return dev[6].download()
+                y = dev[6].download()
+                if first is not None:
+                    y[first[-1]:] = 0
+                return y
             finally:
                 for d in dev:
                     if d is not None:
