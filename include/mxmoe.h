@@ -11,7 +11,9 @@
  * each declaration below names the reference interface it replaces.
  *
  * A context keeps a reusable device buffer (scratch, 4 MiB from mx_create on,
- * grown by calls that need more), and a layer keeps its per-call buffers: calls on one context, or on one layer, must not
+ * grown by calls that need more, which cannot allocate on a stream under capture:
+ * mx_fp8_reserve before; what a captured call was given stays until mx_destroy,
+ * so that its graph may be replayed after larger calls), and a layer keeps its per-call buffers: calls on one context, or on one layer, must not
  * run concurrently on different streams. Use one context per stream that runs
  * alongside others, as the reference serialises calls per Device
  * (src/vesper/connected.py:131-133).
@@ -308,6 +310,9 @@ int mx_act_quant128(mx_ctx* ctx, const uint16_t* x_bf16, uint8_t* q, float* s, i
  * with x: the call reads x before it writes them. */
 int mx_fp8_projection(mx_ctx* ctx, const void* tiled, int32_t n, int32_t k, int32_t block, const uint16_t* x_bf16,
                       int32_t tokens, uint16_t* y_bf16, float* trace, uint8_t* q_out, void* s_out, void* stream);
+/* Grows the context's scratch to what mx_fp8_projection (and mx_fp8_grouped_projection) of n rows by k needs for any call of
+ * up to `tokens` tokens, which can then be captured whatever ran before. */
+int mx_fp8_reserve(mx_ctx* ctx, int32_t n, int32_t k, int32_t tokens);
 
 /* Grouped block-32 FP8 projection (the attention output projection wo_a): weight rows [g rows, (g + 1)
  * rows) of `tiled` (mx_fp8_tile, block 32, groups x rows by K) multiply activation group g, so

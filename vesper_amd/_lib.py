@@ -184,6 +184,7 @@ SIGNATURES = {
     "mx_fp8_tiled_bytes": ([_I32, _I32, _I32], _U64),
     "mx_fp8_tile": ([_P, _P, _P, _I32, _I32, _I32, _P, _P], C.c_int),
     "mx_act_quant128": ([_P, _P, _P, _P, _I64, _I64, _P], C.c_int),
+    "mx_fp8_reserve": ([_P, _I32, _I32, _I32], C.c_int),
     "mx_fp8_projection": ([_P, _P, _I32, _I32, _I32, _P, _I32, _P, _P, _P, _P, _P], C.c_int),
     "mx_fp8_expert_forward": ([_P, _P, _P, _P, _I32, _I32, _P, _I32, _F, _P, _P, C.POINTER(MxExpertStages), _P],
                               C.c_int),

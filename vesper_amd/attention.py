@@ -431,6 +431,9 @@ class CachedAttention:
             self.heads = self._own(HeadRotation(ctx, self.WIDTH, norm=self.WIDTH, dims=self.DIMS, eps=eps, table=table))
             self.back = self._own(HeadRotation(ctx, self.WIDTH, dims=self.DIMS, table=table))
             self.q_norm, self.kv_norm, self.sinks = (None if w is None else self._own(ctx.upload(w)) for w in weights)
+            for name in ("wq_a", "wq_b", "wkv", "wo_b"):   # so that a first step can be captured
+                ctx.lib.fp8_reserve(ctx._h(), *layout[name], self.max_tokens)
+            ctx.lib.fp8_reserve(ctx._h(), *WO_A, min(self.max_tokens, GROUPED_MAX_TOKENS))
             wide, tokens = self.HEADS * self.WIDTH, self.max_tokens
             self.qa, self.q, self.k, self.o, self.codes, self.scales, self.grouped = (
                 self._own(ctx.empty((tokens, n), t)) for n, t in (

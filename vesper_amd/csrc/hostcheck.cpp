@@ -1,10 +1,12 @@
 // Host build of the device numerics (mx_numerics.h) for exhaustive CPU comparison with the oracle, and of the prefill
-// ring's layout (mx_ring.h). Nothing here runs on the GPU path; libmxmoe.so compiles the same headers for gfx950.
+// ring's layout (mx_ring.h) and a context's scratch (mx_scratch.h). Nothing here runs on the GPU path; libmxmoe.so compiles
+// the same headers for gfx950.
 #include <cmath>
 #include <cstdint>
 
 #include "mx_numerics.h"
 #include "mx_ring.h"
+#include "mx_scratch.h"
 
 extern "C" {
 
@@ -90,6 +92,32 @@ void mxh_prefill_ring(int32_t live, int32_t u, int32_t* out) {
   out[2] = mxring::kXLdsBytes;
   out[3] = mxring::kXStageB;
   out[4] = mxring::xacts_read(live, u);
+}
+
+// A context's scratch over n calls of `bytes` each, captured or not: after each call its status, its buffer (numbered from 1
+// in the order of allocation), that buffer's bytes, and the buffers that are allocated, as bits; then those left at the end.
+// The failing-th allocation fails (0: none does).
+int64_t mxh_scratch(const int64_t* bytes, const int32_t* captured, int32_t n, int32_t failing, int64_t* out) {
+  int64_t made = 0, live = 0;
+  mxs::Scratch s;
+  auto alloc = [&](void** p, uint64_t) {
+    if (++made == failing) return -1;
+    live |= 1ll << made;
+    *p = (void*)(intptr_t)made;
+    return 0;
+  };
+  auto release = [&](void* p) {
+    live &= ~(1ll << (intptr_t)p);
+    return 0;
+  };
+  for (int i = 0; i < n; ++i) {
+    out[4 * i] = mxs::reserve(s, bytes[i], captured[i] != 0, alloc, release, -2);
+    out[4 * i + 1] = (int64_t)(intptr_t)s.p;
+    out[4 * i + 2] = s.bytes;
+    out[4 * i + 3] = live;
+  }
+  mxs::release_all(s, release);
+  return live;
 }
 
 }  // extern "C"

@@ -333,7 +333,7 @@ int mx_expert_forward_bf16(mx_ctx* ctx, const void* tiled, int32_t H, int32_t I,
   MX_REQUIRE(!h || is_aligned(h, 4), "mx_expert_forward_bf16: h must be 4-byte aligned");
   hipStream_t st = as_stream(stream);
   void* base = nullptr;
-  if (int s = mxi::scratch(ctx, bf16_scratch_bytes(I, T), &base)) return s;
+  if (int s = mxi::scratch(ctx, bf16_scratch_bytes(I, T), st, &base)) return s;
   uint16_t* hs = (uint16_t*)base;
   GateUpArgs ga{(const uint8_t*)tiled, x, route_w, h, gu, hs, H, I, T};
   const bool few = T <= kFewTokens;

@@ -811,6 +811,10 @@ uint64_t fp8_partial_bytes(int N, int K, int T) {
   return splits > 1 ? (uint64_t)splits * T * N * sizeof(float) : 0;
 }
 
+// The codes of `rows` rows of a projection's input in the context's scratch, and their scales (4 bytes a chunk).
+uint64_t codes_bytes(uint64_t rows, int K) { return (rows * K + 255) & ~255ull; }
+uint64_t scales_bytes(uint64_t rows, int K) { return (rows * (K / 32) + 255) & ~255ull; }
+
 // Fused quantization passes (4 blocks of 128 each per wave) for a K part's chunks x the tokens, shared by the
 // part's M waves: 1, 2 or 4, or 0 when they exceed the part's LDS rows (the call then quantizes in its own
 // launch).
@@ -997,9 +1001,9 @@ int mx_fp8_projection(mx_ctx* ctx, const void* tiled, int32_t N, int32_t K, int3
   const bool codes = q_out || s_out;
   const bool ordered = T <= kGemvMaxTokens && (!codes || T > kFusedMaxTokens);
   const uint64_t rows = ordered ? (T + kTok - 1) / kTok * kTok : T;
-  const uint64_t q_b = (rows * K + 255) & ~255ull, s_b = (rows * (K / 32) + 255) & ~255ull;   // 4 scale bytes a chunk
+  const uint64_t q_b = codes_bytes(rows, K), s_b = scales_bytes(rows, K);
   void* base = nullptr;
-  if (int s = scratch(ctx, q_b + s_b + fp8_partial_bytes(N, K, T) + 256, &base)) return s;
+  if (int s = scratch(ctx, q_b + s_b + fp8_partial_bytes(N, K, T) + 256, st, &base)) return s;
   uint8_t* q = q_out && !ordered ? q_out : (uint8_t*)base;
   void* sc = s_out && !ordered ? s_out : (void*)((uint8_t*)base + q_b);
   float* partial = (float*)((uint8_t*)base + q_b + s_b);
@@ -1017,6 +1021,22 @@ int mx_fp8_projection(mx_ctx* ctx, const void* tiled, int32_t N, int32_t K, int3
   return launch_fp8_product((const uint8_t*)tiled, N, K, block, q, sc, T, y, trace, partial, st, nullptr, ordered);
 }
 
+int mx_fp8_reserve(mx_ctx* ctx, int32_t N, int32_t K, int32_t tokens) {
+  if (int s = use(ctx)) return s;
+  if (int s = check_fp8_shape(N, K, 32, "mx_fp8_reserve")) return s;
+  MX_REQUIRE(tokens >= 0 && tokens <= (1 << 20), "mx_fp8_reserve: token count %d outside [0, %d]", tokens, 1 << 20);
+  // The splits depend on the tokens: by single tokens below the GEMM's, above by its tiles of tokens, the last of them full
+  // or the call's.
+  uint64_t partial = 0;
+  for (int t = 1; t <= std::min(tokens, kGemvMaxTokens); ++t) partial = std::max(partial, fp8_partial_bytes(N, K, t));
+  if (tokens > kGemvMaxTokens)
+    for (int64_t t = 0; t < tokens; t += kGemmTok)
+      partial = std::max(partial, fp8_partial_bytes(N, K, (int)std::min<int64_t>(t + kGemmTok, tokens)));
+  const uint64_t rows = std::max(tokens, kGemvMaxTokens);   // (whole tiles of 16 for the fewest)
+  void* base = nullptr;
+  return scratch(ctx, codes_bytes(rows, K) + scales_bytes(rows, K) + partial + 256, nullptr, &base);
+}
+
 int mx_fp8_grouped_projection(mx_ctx* ctx, const void* tiled, int32_t groups, int32_t rows, int32_t K,
                               const uint8_t* q, const uint8_t* s, int32_t T, uint16_t* y, float* trace, void* stream) {
   if (int st = use(ctx)) return st;
@@ -1032,7 +1052,7 @@ int mx_fp8_grouped_projection(mx_ctx* ctx, const void* tiled, int32_t groups, in
                  ((uintptr_t)y & 7) == 0 && ((uintptr_t)trace & 15) == 0,
              "mx_fp8_grouped_projection: tiled 256-byte, q 16-byte, s 4-byte, y 8-byte, trace 16-byte alignment");
   void* partial = nullptr;
-  if (int st = scratch(ctx, fp8_partial_bytes(N, K, T), &partial)) return st;
+  if (int st = scratch(ctx, fp8_partial_bytes(N, K, T), as_stream(stream), &partial)) return st;
   return launch_fp8_product((const uint8_t*)tiled, N, K, 32, q, s, T, y, trace, (float*)partial, as_stream(stream),
                             nullptr, false, rows);
 }
@@ -1057,7 +1077,7 @@ int mx_fp8_expert_forward(mx_ctx* ctx, const void* w1, const void* w3, const voi
   uint64_t total = fp8_partial_bytes(H, I, T);
   for (uint64_t b : sizes) total += b;
   void* base = nullptr;
-  if (int s = scratch(ctx, total, &base)) return s;
+  if (int s = scratch(ctx, total, st, &base)) return s;
   uint8_t* cur = (uint8_t*)base;
   uint8_t* buf[5];
   for (int i = 0; i < 5; ++i) {

@@ -9,6 +9,7 @@
 #include <unordered_map>
 
 #include "../../include/mxmoe.h"
+#include "mx_scratch.h"
 
 struct mx_ctx {
   int device = 0;
@@ -18,12 +19,11 @@ struct mx_ctx {
   std::mutex lock;
   std::unordered_map<void*, uint64_t> owned;        // device allocations
   std::unordered_map<void*, uint64_t> pinned;       // host pinned allocations
-  void* scratch = nullptr;                          // reusable device scratch, MX_SCRATCH_START bytes or more
-  uint64_t scratch_bytes = 0;
+  mxs::Scratch scratch;                             // reusable device scratch, MX_SCRATCH_START bytes or more
 };
 
-// The scratch a context starts with. Growing it frees and allocates, which synchronises the device and fails under
-// stream capture; an FP8 call of up to 32 tokens over widths up to 100,000 (codes and scales in whole tiles of 16
+// The scratch a context starts with. Growing it allocates (and frees, unless a capture was given the old one), which
+// synchronises the device and fails under stream capture; an FP8 call of up to 32 tokens over widths up to 100,000 (codes and scales in whole tiles of 16
 // tokens: 32 x width x 33 / 32 bytes) and an FP8 or BF16 expert call fit from the start.
 #define MX_SCRATCH_START (4u << 20)
 
@@ -44,8 +44,9 @@ void clear_error();
 // Make the context's device current for this thread.
 int use(mx_ctx* ctx);
 
-// Context-owned scratch of at least `bytes` (grows; never shrinks until destroy).
-int scratch(mx_ctx* ctx, uint64_t bytes, void** out);
+// Context-owned scratch of at least `bytes` for a call on `stream` (grows; never shrinks until destroy). What a captured call
+// was given stays until destroy, since its graph may be replayed after any other call.
+int scratch(mx_ctx* ctx, uint64_t bytes, hipStream_t stream, void** out);
 
 // The allocation-free tiled expert call's fixed device array (mx_moe.hip): its device address is taken once
 // per device, with the device current (mx_create), and looked up by later calls on that device.

@@ -2232,7 +2232,7 @@ int mx_expert_forward(mx_ctx* ctx, const mx_expert_ptrs* w, int32_t format, int3
   // the reference layout is tiled into scratch (one pass over the expert's bytes) and the tiled call runs on it
   const uint64_t blob_b = (tiled_offsets(H, I).total + 255) & ~255ull;
   void* base = nullptr;
-  if (int s = mxi::scratch(ctx, blob_b + tiled_call_scratch_bytes(H, I, T), &base)) return s;
+  if (int s = mxi::scratch(ctx, blob_b + tiled_call_scratch_bytes(H, I, T), as_stream(stream), &base)) return s;
   uint8_t* b8 = (uint8_t*)base;
   hipLaunchKernelGGL(tile_expert_kernel, dim3(2048), dim3(256), 0, as_stream(stream), *w, b8, H, I, 1);
   MX_LAUNCH_CHECK("tile_expert_kernel");
@@ -2246,7 +2246,7 @@ int mx_expert_forward_tiled(mx_ctx* ctx, const void* tiled, int32_t H, int32_t I
   if (int s = check_tiled_call("mx_expert_forward_tiled", tiled, H, I, x, T, limit, y)) return s;
   if (T == 0) return MX_OK;
   void* base = nullptr;
-  if (int s = mxi::scratch(ctx, tiled_call_scratch_bytes(H, I, T), &base)) return s;
+  if (int s = mxi::scratch(ctx, tiled_call_scratch_bytes(H, I, T), as_stream(stream), &base)) return s;
   return tiled_call_on(ctx, (uint8_t*)base, tiled, H, I, x, T, limit, route_w, y, stages, stream);
 }
 
@@ -2277,7 +2277,7 @@ int mx_gemv_mxfp4(mx_ctx* ctx, const uint8_t* q, const uint8_t* sa, const uint8_
              "mx_gemv_mxfp4: q/w 16-byte, scales 4-byte and y 8-byte alignment required");
   hipStream_t st = as_stream(stream);
   void* base = nullptr;
-  if (int s = mxi::scratch(ctx, sizeof(Plan), &base)) return s;
+  if (int s = mxi::scratch(ctx, sizeof(Plan), as_stream(stream), &base)) return s;
   Plan* plan = (Plan*)base;
   hipLaunchKernelGGL(single_plan_kernel, dim3(1), dim3(64), 0, st, plan, T, (const float*)nullptr);
   MX_LAUNCH_CHECK("single_plan_kernel");
@@ -2355,7 +2355,7 @@ int mx_router(mx_ctx* ctx, const float* W, const float* bias, const uint16_t* x,
   float *scores = out->scores, *selection = out->selection;
   if (!scores || !selection) {
     void* base = nullptr;
-    if (int s = mxi::scratch(ctx, (uint64_t)T * E * 8, &base)) return s;
+    if (int s = mxi::scratch(ctx, (uint64_t)T * E * 8, as_stream(stream), &base)) return s;
     if (!scores) scores = (float*)base;
     if (!selection) selection = (float*)base + (uint64_t)T * E;
   }
@@ -2407,7 +2407,7 @@ int mx_router_postprocess(mx_ctx* ctx, const float* logits, const float* bias, i
   float *scores = out->scores, *selection = out->selection;
   if (!scores || !selection) {
     void* base = nullptr;
-    if (int s = mxi::scratch(ctx, (uint64_t)T * E * 8, &base)) return s;
+    if (int s = mxi::scratch(ctx, (uint64_t)T * E * 8, as_stream(stream), &base)) return s;
     if (!scores) scores = (float*)base;
     if (!selection) selection = (float*)base + (uint64_t)T * E;
   }

@@ -34,16 +34,25 @@ int use(mx_ctx* ctx) {
   return MX_OK;
 }
 
-int scratch(mx_ctx* ctx, uint64_t bytes, void** out) {
-  if (ctx->scratch_bytes < bytes) {
-    if (ctx->scratch) MX_HIP(hipFree(ctx->scratch));
-    ctx->scratch = nullptr;
-    ctx->scratch_bytes = 0;
-    MX_HIP(hipMalloc(&ctx->scratch, bytes));
-    ctx->scratch_bytes = bytes;
+int scratch(mx_ctx* ctx, uint64_t bytes, hipStream_t stream, void** out) {
+  hipStreamCaptureStatus state = hipStreamCaptureStatusNone;
+  if (stream && hipStreamIsCapturing(stream, &state) != hipSuccess) {   // (the default stream is never captured)
+    (void)hipGetLastError();
+    state = hipStreamCaptureStatusNone;
   }
-  *out = ctx->scratch;
-  return MX_OK;
+  const int s = mxs::reserve(
+      ctx->scratch, bytes, state != hipStreamCaptureStatusNone,
+      [](void** p, uint64_t n) {
+        MX_HIP(hipMalloc(p, n));
+        return MX_OK;
+      },
+      [](void* p) {
+        MX_HIP(hipFree(p));
+        return MX_OK;
+      },
+      MX_ERR_MEMORY);
+  if (s == MX_OK) *out = ctx->scratch.p;
+  return s;
 }
 
 }  // namespace mxi
@@ -75,8 +84,8 @@ int mx_create(int device, uint64_t cap_bytes, mx_ctx** out) {
   mx_ctx* ctx = new mx_ctx();
   ctx->device = device;
   ctx->cap = cap_bytes;
-  ctx->scratch = scratch;
-  ctx->scratch_bytes = MX_SCRATCH_START;
+  ctx->scratch.p = scratch;
+  ctx->scratch.bytes = MX_SCRATCH_START;
   *out = ctx;
   return MX_OK;
 }
@@ -88,7 +97,7 @@ int mx_destroy(mx_ctx* ctx) {
     if (hipDeviceSynchronize() != hipSuccess) status = hip_fail(hipGetLastError(), "mx_destroy: synchronize");
     for (auto& kv : ctx->owned) (void)hipFree(kv.first);
     for (auto& kv : ctx->pinned) (void)hipHostFree(kv.first);
-    if (ctx->scratch) (void)hipFree(ctx->scratch);
+    mxs::release_all(ctx->scratch, [](void* p) { (void)hipFree(p); });
   }
   delete ctx;
   return status;
