@@ -520,6 +520,12 @@ __device__ __forceinline__ float raised(float m, float top) {
   return top > m + 8.f ? (m == kLowest ? top : m + ceilf(top - m)) : m;
 }
 
+// A maximum so far from zero that FP32 holds it to whole numbers only: c s - m, rounded once, would not be about zero where s
+// is the largest logit (its power overflows from 2^31 on). There c s is rounded by itself, as m is.
+__device__ __forceinline__ bool far_off(float m) { return fabsf(m) >= 0x1p24f && m != kLowest; }
+// What a step's largest logit has to pass for the maximum to be looked at: anything, where it is far off.
+__device__ __forceinline__ float bar_of(float m) { return far_off(m) ? -INFINITY : m + 8.f; }
+
 struct RowOut {
   float inv, lse;
 };
@@ -765,6 +771,7 @@ __global__ __launch_bounds__(512, 2) void latent_kernel(AttendArgs a, int by) {
       uint8_t* const put_w = weights + (tt * T2 * A::kRows + rq * 16 + l16) * 32 + (quad & 1) * 16 + (quad >> 1) * 8;
       float m = kLowest, l = 0.f;
       float own = kLowest, sum = 0.f;
+      bool far = false;   // one of the wave's maxima is far off
       mxd::copy_barrier();   // the first step is there, and exchanged queries have been read
       for (int it = it0; it < it1; ++it) {
         const uint8_t* stage = lds + A::kRing + (it % A::kStages) * A::kStage;
@@ -801,20 +808,20 @@ __global__ __launch_bounds__(512, 2) void latent_kernel(AttendArgs a, int by) {
 #pragma unroll
             for (int t = 0; t < TT; ++t) next = fmaxf(next, tops[(it - 1) & 1][rq * 16 + l16][t]);
             l = l * power(m, next) + sum * power(own, next);
-            m = next;
+            m = next, far = __any(far_off(m));
           }
         }
         own = m, sum = 0.f;
-        float top = -INFINITY;
+        float top = -INFINITY, c = a.c;
         auto weigh = [&](int t) {   // the probabilities of 16 tokens
           float p[4];
 #pragma unroll
-          for (int n = 0; n < 4; ++n) p[n] = __builtin_amdgcn_exp2f(fmaf(sc[t][n], a.c, -own));
+          for (int n = 0; n < 4; ++n) p[n] = __builtin_amdgcn_exp2f(fmaf(sc[t][n], c, -own));
           sum += (p[0] + p[1]) + (p[2] + p[3]);
           *(uint2*)(put_w + (it & 1) * A::kWeights + t * (A::kRows * 32)) = make_uint2(mxd::bf16_pair(p[0], p[1]), mxd::bf16_pair(p[2], p[3]));
         };
         auto look = [&](int t) { top = fmaxf(top, fmaxf(fmaxf(sc[t][0], sc[t][1]), fmaxf(sc[t][2], sc[t][3]))); };
-        const bool plain = shown == 15u && first >= all_lo && first + 16 * T2 <= all_hi;
+        const bool plain = shown == 15u && first >= all_lo && first + 16 * T2 <= all_hi && !far;
         if (plain) {   // under the maximum so far, which seldom rises: 16 tokens' probabilities beside the next ones' scores
           score(0);
 #pragma unroll
@@ -839,6 +846,14 @@ __global__ __launch_bounds__(512, 2) void latent_kernel(AttendArgs a, int by) {
         const bool rises = __any(top > m + 8.f);
         if (rises) own = raised(m, top);
         if (!plain || rises) {
+          far = __any(far_off(own));
+          if (far) {
+#pragma unroll
+            for (int t = 0; t < T2; ++t)
+#pragma unroll
+              for (int n = 0; n < 4; ++n) sc[t][n] *= a.c;
+            c = 1.f;
+          }
           sum = 0.f;
 #pragma unroll
           for (int t = 0; t < T2; ++t) weigh(t);
@@ -1266,7 +1281,7 @@ __global__ __launch_bounds__(256, (Grouped<W, RG>::kWaves)) void grouped_kernel(
       }
     }
 
-    float m = kLowest, l = 0.f;
+    float m = kLowest, bar = kLowest, l = 0.f;
     v16f o[DB];
 #pragma unroll
     for (int d = 0; d < DB; ++d)
@@ -1335,18 +1350,24 @@ __global__ __launch_bounds__(256, (Grouped<W, RG>::kWaves)) void grouped_kernel(
 #pragma unroll
       for (int n = 2; n < 16; ++n) top = fmaxf(top, sc[n]);
       top = other_half_max(top) * a.c;
-      if (__any(top > m + 8.f)) {
+      float c = a.c;   // far off: 1, and c s in the scores' place (prompts of 128 wide 379 us with this, 374 without)
+      if (__any(top > bar)) {
         const float own = raised(m, top), by = power(m, own);
-        m = own, l *= by;
+        m = own, bar = bar_of(m), l *= by;
 #pragma unroll
         for (int d = 0; d < DB; ++d)
 #pragma unroll
           for (int n = 0; n < 16; ++n) o[d][n] *= by;
+        if (__any(far_off(m))) {
+#pragma unroll
+          for (int n = 0; n < 16; ++n) sc[n] *= a.c;
+          c = 1.f;
+        }
       }
       uint32_t p[8];
 #pragma unroll
       for (int n = 0; n < 8; ++n) {
-        const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[2 * n], a.c, -m)), p1 = __builtin_amdgcn_exp2f(fmaf(sc[2 * n + 1], a.c, -m));
+        const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[2 * n], c, -m)), p1 = __builtin_amdgcn_exp2f(fmaf(sc[2 * n + 1], c, -m));
         l += p0 + p1;
         p[n] = mxd::bf16_pair(p0, p1);
       }
