@@ -9,9 +9,14 @@
 //   S^T: V_MFMA_SCALE_F32_32X32X64_F8F6F4 on the codes and scales as they lie in the cache, with the query as two E4M3
 //        terms: a BF16 value has 8 significant bits, the first term takes 4 of them and the second, 2^-4 of its scale, the
 //        rest, so the products are those of the BF16 query (to 2^-21 of a block's largest). At the rate of E4M3, two terms
-//        cost what one BF16 product does, and the keys need no conversion. The instruction adds the products of eight
-//        neighbours without what lies 2^-13 below the largest of them (measured; between eights it keeps 24 bits): on normal
-//        values logits are off by some 2^-19 of the sum of their products' magnitudes.
+//        cost what one BF16 product does, and the keys need no conversion. The instruction cuts each of eight neighbouring
+//        products towards zero at 2^-13 of the largest power of two that two factors of one make, and adds those up exactly
+//        (measured, bit for bit; a code of 0.5 counts as 1 there, a product of zero not at all; between eights it keeps 24
+//        bits). So seven products lose up to 2^-12 of the largest each, in both terms 7 (1 + 2 2^-4) 2^-12 < 2^-9 of the
+//        eights' largest products: no more than rounding the query's value to BF16 may have changed that product by. On normal
+//        values logits are off by some 2^-19 of the sum of their products' magnitudes; with one channel of the query 100 times
+//        its neighbours by 0.002 at most and 2e-4 on average (2-norm) where they are about 3 and the rounding of the query is
+//        0.004, with it 1000 times by 0.05 and 0.004 of 22 (rounding 0.025).
 //   O^T: V_MFMA_F32_32X32X16_BF16. A scale belongs to a token and 32 columns, but this product runs over the tokens, so
 //        the values become BF16 (exactly: two significant bits and a power of two) by V_CVT_SCALEF32_PK_BF16_FP4, in the
 //        row order in which they lie, and go through LDS, whose transposing reads give each lane its column's tokens.
