@@ -1610,6 +1610,9 @@ int check_attend(const char* who, const mx_kv4* c, int32_t heads, int32_t tokens
   return MX_OK;
 }
 
+// The most row groups of 32 that a workgroup takes.
+int most_groups(const mx_kv4* c) { return c->v_codes ? 4 : 2; }
+
 int workgroups(const mx_kv4* c) { return kCus * (c->v_codes ? waves(c->width) : 1); }
 
 // Row tiles of all sequences at most: each sequence's last one may be partly full.
@@ -1639,7 +1642,7 @@ uint64_t mx_kv4_workspace_bytes(mx_ctx* ctx, const mx_kv4* cache, int32_t heads,
   if (check_attend("mx_kv4_workspace_bytes", cache, heads, tokens, batch)) return 0;
   const int group = heads / cache->heads;
   int64_t most = 0;
-  for (int rg = 1; rg <= 4; rg *= 2) most = std::max(most, space_of(cache, group, tokens, batch, 32 * rg).total);
+  for (int rg = 1; rg <= most_groups(cache); rg *= 2) most = std::max(most, space_of(cache, group, tokens, batch, 32 * rg).total);
   return (uint64_t)most;
 }
 
@@ -1682,8 +1685,8 @@ int mx_kv4_attend(mx_ctx* ctx, const mx_kv4* cache, const mx_kv4_query* query, v
   const int64_t tokens_each = ((int64_t)q.tokens + q.batch - 1) / q.batch, rows = tokens_each * a.group;
   const int64_t held = std::min<int64_t>((int64_t)q.columns * cache->page, q.window ? q.window + tokens_each : INT64_MAX);
   const double steps = (double)q.batch * cache->heads * ((rows + 31) / 32) * ((held + 31) / 32) / (4. * n);
-  int rg = rows <= 32 ? 1 : rows <= 64 || !cache->v_codes ? 2 : 4;
-  rg = std::min(rg, steps <= (cache->v_codes ? 8 : 5) ? 1 : steps <= 128 ? 2 : 4);
+  int rg = rows <= 32 ? 1 : rows <= 64 ? 2 : 4;
+  rg = std::min({rg, most_groups(cache), steps <= (cache->v_codes ? 8 : 5) ? 1 : steps <= 128 ? 2 : 4});
   const int tile_rows = 32 * rg, step = 128 / rg;
   a.by_group = Divide(a.group);
   if (!q.q_first) a.rows_each = q.tokens / q.batch, a.tiles_each = (int)(((int64_t)a.rows_each * a.group + tile_rows - 1) / tile_rows);
