@@ -77,9 +77,13 @@ class HeadRotation:
     def __exit__(self, *_):
         self.close()
 
-    def struct(self, positions_ptr=None, inverse: bool = False) -> _lib.MxRotation:
+    def _open(self):
         if self.ctx is None:
             raise RuntimeError("the rotation is closed")
+        return self.ctx._h()
+
+    def struct(self, positions_ptr=None, inverse: bool = False) -> _lib.MxRotation:
+        self._open()
         return _lib.MxRotation(_lib.ptr(self.table), self.positions, _lib.ptr(positions_ptr), self.width, self.norm,
                                self.first, self.dims, self.style, int(bool(inverse)), self.eps)
 
@@ -108,8 +112,7 @@ class HeadRotation:
     def open_gradients(self):
         """The workspace of the weights' gradients; allocated by the first call that needs it unless opened before (a
         call inside a stream capture cannot allocate)."""
-        if self.ctx is None:
-            raise RuntimeError("the rotation is closed")
+        self._open()
         if self.workspace is None and self.workspace_bytes:
             self.workspace = self.ctx.empty((self.workspace_bytes,), np.uint8)
 
@@ -154,6 +157,7 @@ class HeadRotation:
 
     def apply(self, x, positions=None, weight=None, inverse: bool = False) -> np.ndarray:
         """[T, heads, width] of x, in its type; rows of no token (position -1) as they were."""
+        self._open()
         flat, dtype, (t, heads) = self._host(x, "x")
         dev = []
         try:
@@ -169,6 +173,7 @@ class HeadRotation:
 
     def backward(self, dy, x, positions=None, weight=None, inverse: bool = False) -> dict:
         """{"dx" [T, heads, width], and with norm "dweight" [norm]}."""
+        self._open()
         dy, dtype, (t, heads) = self._host(dy, "dy")
         x, x_dtype, shape = self._host(x, "x")
         if x_dtype != dtype or shape != (t, heads):
