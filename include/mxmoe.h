@@ -462,7 +462,8 @@ int mx_rotate_heads(mx_ctx* ctx, const mx_heads* sets, int32_t n_sets, int32_t t
 /* Bytes of workspace (16-byte aligned device memory) for gradients of weights of `norm` values. */
 uint64_t mx_rotate_heads_workspace_bytes(int32_t norm);
 /* The gradients: dx for dy, all of one type, and dweight in FP32, summed in a fixed order. Rows that are no token get a
- * zero dx and add nothing. workspace may be NULL where no dweight is asked for. */
+ * zero dx and add nothing. workspace may be NULL where no dweight is asked for; calls
+ * that share one must not overlap, nor be made by two threads at once. */
 int mx_rotate_heads_backward(mx_ctx* ctx, const mx_heads_grad* sets, int32_t n_sets, int32_t tokens,
                              const mx_rotation* rotation, int32_t type, void* workspace, uint64_t workspace_bytes,
                              void* stream);
@@ -527,7 +528,8 @@ uint64_t mx_kv4_workspace_bytes(mx_ctx* ctx, const mx_kv4* cache, int32_t heads,
  * its neighbours. How a row's tokens are divided follows the lengths of all sequences of the call, so the last bits of a
  * result can differ with what is beside it; the same call gives the same bits. A row that sees nothing gets zero and lse
  * -infinity. Page numbers outside the cache and lengths past columns * page hide their tokens; a token one of whose blocks is NaN makes the rows that see it NaN and
- * no others. Rows behind q_first[batch] stay as they were. Calls that share a workspace must not overlap. */
+ * no others. Rows behind q_first[batch] stay as they were. Calls that share a workspace must not overlap, and are
+ * several launches each: threads that share a stream too make them one after another. */
 int mx_kv4_attend(mx_ctx* ctx, const mx_kv4* cache, const mx_kv4_query* query, void* workspace, uint64_t workspace_bytes,
                   void* stream);
 

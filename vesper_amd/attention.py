@@ -8,14 +8,16 @@ CachedAttention  the block-32 projections' attention over a cache (NativeProject
                norms, the rotation, wkv into the cache, attention, the rotation back, wo_a, wo_b
 
 The *_device methods take device pointers and do not synchronise; the others take and return host arrays (BF16 as uint16
-bits, or FP32). A KVCache4 has one workspace, a CachedAttention one set of buffers: calls of one object must not overlap
-on different streams.
+bits, or FP32). A HeadRotation and a KVCache4 have one workspace, a CachedAttention one set of buffers: calls of one object
+must not overlap on different streams. Calls from several threads take turns, each with all its launches, and close waits for
+them.
 """
 
 from __future__ import annotations
 
 import ctypes as C
 import math
+import threading
 
 import numpy as np
 
@@ -56,6 +58,7 @@ class HeadRotation:
             table = np.ascontiguousarray(table, np.float32)
             if table.ndim != 2 or table.shape[0] < 1 or table.shape[1] != dims or not np.isfinite(table).all():
                 raise ValueError(f"the rotation's table must be finite FP32 [positions, {dims}]")
+        self.lock = threading.RLock()
         self.ctx, self.width, self.norm, self.first, self.dims = ctx, int(width), int(norm), int(first), int(dims)
         self.style, self.eps = _lib.MX_ROTATE[style], float(eps)
         self.positions = table.shape[0] if dims else 0
@@ -64,12 +67,13 @@ class HeadRotation:
         self.workspace = None
 
     def close(self):
-        for name in ("table", "workspace"):
-            held = getattr(self, name)
-            if held is not None:
-                setattr(self, name, None)
-                held.free()
-        self.ctx = None
+        with self.lock:
+            for name in ("table", "workspace"):
+                held = getattr(self, name)
+                if held is not None:
+                    setattr(self, name, None)
+                    held.free()
+            self.ctx = None
 
     def __enter__(self):
         return self
@@ -104,29 +108,32 @@ class HeadRotation:
     def apply_device(self, sets, tokens: int, positions_ptr=None, x_dtype: str = "bf16", y_dtype: str | None = None,
                      inverse: bool = False, stream=None):
         """One or two `set`s (queries, and keys with weights of their own) in one launch."""
-        rotation = self.struct(positions_ptr, inverse)
-        array = (_lib.MxHeads * len(sets))(*sets)
-        self.ctx.lib.rotate_heads(self.ctx._h(), array, len(sets), int(tokens), C.byref(rotation), row_type(x_dtype),
-                                  row_type(y_dtype or x_dtype), _lib._stream(stream))
+        with self.lock:
+            rotation = self.struct(positions_ptr, inverse)
+            array = (_lib.MxHeads * len(sets))(*sets)
+            self.ctx.lib.rotate_heads(self.ctx._h(), array, len(sets), int(tokens), C.byref(rotation), row_type(x_dtype),
+                                      row_type(y_dtype or x_dtype), _lib._stream(stream))
 
     def open_gradients(self):
         """The workspace of the weights' gradients; allocated by the first call that needs it unless opened before (a
         call inside a stream capture cannot allocate)."""
-        self._open()
-        if self.workspace is None and self.workspace_bytes:
-            self.workspace = self.ctx.empty((self.workspace_bytes,), np.uint8)
+        with self.lock:
+            self._open()
+            if self.workspace is None and self.workspace_bytes:
+                self.workspace = self.ctx.empty((self.workspace_bytes,), np.uint8)
 
     def backward_device(self, grads, tokens: int, positions_ptr=None, dtype: str = "bf16", inverse: bool = False,
                         stream=None):
         """The gradients of apply_device(inverse) for one or two `grad`s. Calls that ask for dweight share a workspace:
         they must not overlap on different streams."""
-        rotation = self.struct(positions_ptr, inverse)
-        if any(g.dweight for g in grads):
-            self.open_gradients()
-        array = (_lib.MxHeadsGrad * len(grads))(*grads)
-        self.ctx.lib.rotate_heads_backward(self.ctx._h(), array, len(grads), int(tokens), C.byref(rotation),
-                                           row_type(dtype), _lib.ptr(self.workspace), self.workspace_bytes,
-                                           _lib._stream(stream))
+        with self.lock:
+            rotation = self.struct(positions_ptr, inverse)
+            if any(g.dweight for g in grads):
+                self.open_gradients()
+            array = (_lib.MxHeadsGrad * len(grads))(*grads)
+            self.ctx.lib.rotate_heads_backward(self.ctx._h(), array, len(grads), int(tokens), C.byref(rotation),
+                                               row_type(dtype), _lib.ptr(self.workspace), self.workspace_bytes,
+                                               _lib._stream(stream))
 
     # -- host arrays -------------------------------------------------------------------------------
     def _host(self, x, what):
@@ -216,7 +223,7 @@ class KVCache4:
         self.width, self.apart = int(width), value_width is None
         self.value_width = self.width if self.apart else int(value_width)
         self.query_heads, self.max_tokens, self.max_batch = int(query_heads), int(max_tokens), int(max_batch)
-        self._owned = []
+        self.lock, self._owned = threading.Lock(), []
         try:
             for w in (self.width, self.value_width) if self.apart else (self.width,):
                 for bytes_ in (w // 2, -(-w // 128) * 4):
@@ -235,8 +242,9 @@ class KVCache4:
             raise
 
     def close(self):
-        while self._owned:
-            self._owned.pop().free()
+        with self.lock:
+            while self._owned:
+                self._owned.pop().free()
 
     def __enter__(self):
         return self
@@ -255,28 +263,30 @@ class KVCache4:
                       k_rounded_ptr=None, v_rounded_ptr=None, stream=None):
         """Keys [T, heads, width] (through `rotation`) and values into device int64 slots [T] (page * self.page + place;
         outside the cache: not stored), and the BF16 values that the codes stand for where asked."""
-        handle, ptr = self._open(), _lib.ptr
-        turned = None if rotation is None else rotation.struct(positions_ptr)
-        rows = _lib.MxKv4Append(ptr(k_ptr), self.heads * self.width if k_stride is None else k_stride, ptr(v_ptr),
-                                self.heads * self.value_width if v_stride is None else v_stride, row_type(dtype), int(tokens),
-                                ptr(slots_ptr), ptr(weight_ptr), ptr(k_rounded_ptr), ptr(v_rounded_ptr))
-        self.ctx.lib.kv4_append(handle, C.byref(self.struct), C.byref(rows), None if turned is None else C.byref(turned),
-                                _lib._stream(stream))
+        with self.lock:
+            handle, ptr = self._open(), _lib.ptr
+            turned = None if rotation is None else rotation.struct(positions_ptr)
+            rows = _lib.MxKv4Append(ptr(k_ptr), self.heads * self.width if k_stride is None else k_stride, ptr(v_ptr),
+                                    self.heads * self.value_width if v_stride is None else v_stride, row_type(dtype), int(tokens),
+                                    ptr(slots_ptr), ptr(weight_ptr), ptr(k_rounded_ptr), ptr(v_rounded_ptr))
+            self.ctx.lib.kv4_append(handle, C.byref(self.struct), C.byref(rows), None if turned is None else C.byref(turned),
+                                    _lib._stream(stream))
 
     def attend_device(self, q_ptr, tokens: int, table_ptr, columns: int, lengths_ptr, batch: int, out_ptr, scale: float,
                       q_first_ptr=None, window: int = 0, sinks_ptr=None, lse_ptr=None, q_stride=None, out_stride=None,
                       stream=None):
         """out [T, query_heads, value_width] BF16 of q [T, query_heads, width] BF16: tokens / batch query rows of each
         sequence, or those that device int32 q_first [batch + 1] gives."""
-        handle, ptr = self._open(), _lib.ptr
-        if not 0 <= tokens <= self.max_tokens or not 0 <= batch <= self.max_batch:
-            raise ValueError(f"the cache was opened for {self.max_tokens} query rows of {self.max_batch} sequences a call")
-        query = _lib.MxKv4Attend(ptr(q_ptr), self.query_heads * self.width if q_stride is None else q_stride,
-                                 self.query_heads, int(tokens), int(batch), ptr(q_first_ptr), ptr(table_ptr), int(columns),
-                                 ptr(lengths_ptr), float(scale), int(window), ptr(sinks_ptr), ptr(out_ptr),
-                                 self.query_heads * self.value_width if out_stride is None else out_stride, ptr(lse_ptr))
-        self.ctx.lib.kv4_attend(handle, C.byref(self.struct), C.byref(query), self.workspace.ptr, self.workspace_bytes,
-                                _lib._stream(stream))
+        with self.lock:
+            handle, ptr = self._open(), _lib.ptr
+            if not 0 <= tokens <= self.max_tokens or not 0 <= batch <= self.max_batch:
+                raise ValueError(f"the cache was opened for {self.max_tokens} query rows of {self.max_batch} sequences a call")
+            query = _lib.MxKv4Attend(ptr(q_ptr), self.query_heads * self.width if q_stride is None else q_stride,
+                                     self.query_heads, int(tokens), int(batch), ptr(q_first_ptr), ptr(table_ptr), int(columns),
+                                     ptr(lengths_ptr), float(scale), int(window), ptr(sinks_ptr), ptr(out_ptr),
+                                     self.query_heads * self.value_width if out_stride is None else out_stride, ptr(lse_ptr))
+            self.ctx.lib.kv4_attend(handle, C.byref(self.struct), C.byref(query), self.workspace.ptr, self.workspace_bytes,
+                                    _lib._stream(stream))
 
     # -- host arrays -------------------------------------------------------------------------------
     def _rows(self, x, width, what, heads):
@@ -428,7 +438,7 @@ class CachedAttention:
                 raise ValueError(f"{name} must be [{n}]")
         self.projections, self.ctx = projections, ctx
         self.scale, self.window, self.max_tokens = float(scale), int(window), int(max_tokens)
-        self._owned = []
+        self.lock, self._owned = threading.Lock(), []
         try:
             self.cache = self._own(KVCache4(ctx, pages, page, 1, self.WIDTH, self.WIDTH, query_heads=self.HEADS,
                                             max_tokens=max_tokens, max_batch=max_batch))
@@ -453,9 +463,10 @@ class CachedAttention:
         return thing
 
     def close(self):
-        while self._owned:
-            held = self._owned.pop()
-            (held.close if hasattr(held, "close") else held.free)()
+        with self.lock:
+            while self._owned:
+                held = self._owned.pop()
+                (held.close if hasattr(held, "close") else held.free)()
 
     def __enter__(self):
         return self
@@ -475,34 +486,36 @@ class CachedAttention:
         cache: not stored) at int32 positions [T], then each token attends to its sequence's `lengths` [batch] tokens on
         pages `table` [batch, columns], its own among them. The tokens are the last of their sequences: as many of each,
         or those that int32 q_first [batch + 1] gives. Rows of y behind the last sequence are of no use: what an earlier
-        step left of its attention, projected."""
-        self._open()
-        if not 0 <= tokens <= self.max_tokens or not 0 <= batch <= self.cache.max_batch:
-            raise ValueError(f"the cache was opened for {self.max_tokens} tokens of {self.cache.max_batch} sequences a call")
-        if not tokens:
-            return
-        proj, lib, handle, vp = self.projections, self.ctx.lib, self.ctx._h(), _lib.vp
-        rows, width = WO_A[0] // WO_A_GROUPS, WO_A[1]
-        proj.project_device("wkv", x_ptr, tokens, self.k.ptr, stream)
-        self.cache.append_device(self.k.ptr, slots_ptr, tokens, rotation=self.heads, positions_ptr=positions_ptr,
-                                 weight_ptr=self.kv_norm, stream=stream)
-        proj.project_device("wq_a", x_ptr, tokens, self.qa.ptr, stream)
-        self.down.apply_device([self.down.set(self.qa, 1, self.qa, self.q_norm)], tokens, stream=stream)
-        proj.project_device("wq_b", self.qa.ptr, tokens, self.q.ptr, stream)
-        self.heads.apply_device([self.heads.set(self.q, self.HEADS, self.q)], tokens, positions_ptr, stream=stream)
-        self.cache.attend_device(self.q, tokens, table_ptr, columns, lengths_ptr, batch, self.o, self.scale, q_first_ptr,
-                                 self.window, self.sinks, stream=stream)
-        self.back.apply_device([self.back.set(self.o, self.HEADS, self.o)], tokens, positions_ptr, inverse=True,
-                               stream=stream)
-        lib.kv_round32(handle, vp(self.o), tokens * self.HEADS * self.WIDTH, vp(self.q), vp(self.codes), vp(self.scales),
-                       _lib._stream(stream))   # (the rounded values take the queries' place)
-        for t in range(0, tokens, GROUPED_MAX_TOKENS):
-            lib.fp8_grouped_projection(handle, C.c_void_p(proj.tiled["wo_a"]), WO_A_GROUPS, rows, width,
-                                       C.c_void_p(self.codes.ptr + t * WO_A_GROUPS * width),
-                                       C.c_void_p(self.scales.ptr + t * WO_A_GROUPS * width // 32),
-                                       min(GROUPED_MAX_TOKENS, tokens - t),
-                                       C.c_void_p(self.grouped.ptr + t * WO_A_GROUPS * rows * 2), None, _lib._stream(stream))
-        proj.project_device("wo_b", self.grouped.ptr, tokens, y_ptr, stream)
+        step left of its attention, projected. Threads take turns on one layer; device calls on the runtime beside it (another
+        layer's step_device, project_device) share the context's scratch and are the caller's to order."""
+        with self.lock:
+            self._open()
+            if not 0 <= tokens <= self.max_tokens or not 0 <= batch <= self.cache.max_batch:
+                raise ValueError(f"the cache was opened for {self.max_tokens} tokens of {self.cache.max_batch} sequences a call")
+            if not tokens:
+                return
+            proj, lib, handle, vp = self.projections, self.ctx.lib, self.ctx._h(), _lib.vp
+            rows, width = WO_A[0] // WO_A_GROUPS, WO_A[1]
+            proj.project_device("wkv", x_ptr, tokens, self.k.ptr, stream)
+            self.cache.append_device(self.k.ptr, slots_ptr, tokens, rotation=self.heads, positions_ptr=positions_ptr,
+                                     weight_ptr=self.kv_norm, stream=stream)
+            proj.project_device("wq_a", x_ptr, tokens, self.qa.ptr, stream)
+            self.down.apply_device([self.down.set(self.qa, 1, self.qa, self.q_norm)], tokens, stream=stream)
+            proj.project_device("wq_b", self.qa.ptr, tokens, self.q.ptr, stream)
+            self.heads.apply_device([self.heads.set(self.q, self.HEADS, self.q)], tokens, positions_ptr, stream=stream)
+            self.cache.attend_device(self.q, tokens, table_ptr, columns, lengths_ptr, batch, self.o, self.scale, q_first_ptr,
+                                     self.window, self.sinks, stream=stream)
+            self.back.apply_device([self.back.set(self.o, self.HEADS, self.o)], tokens, positions_ptr, inverse=True,
+                                   stream=stream)
+            lib.kv_round32(handle, vp(self.o), tokens * self.HEADS * self.WIDTH, vp(self.q), vp(self.codes), vp(self.scales),
+                           _lib._stream(stream))   # (the rounded values take the queries' place)
+            for t in range(0, tokens, GROUPED_MAX_TOKENS):
+                lib.fp8_grouped_projection(handle, C.c_void_p(proj.tiled["wo_a"]), WO_A_GROUPS, rows, width,
+                                           C.c_void_p(self.codes.ptr + t * WO_A_GROUPS * width),
+                                           C.c_void_p(self.scales.ptr + t * WO_A_GROUPS * width // 32),
+                                           min(GROUPED_MAX_TOKENS, tokens - t),
+                                           C.c_void_p(self.grouped.ptr + t * WO_A_GROUPS * rows * 2), None, _lib._stream(stream))
+            proj.project_device("wo_b", self.grouped.ptr, tokens, y_ptr, stream)
 
     # -- host arrays -------------------------------------------------------------------------------
     def step(self, x, positions, slots, table, lengths, counts=None) -> np.ndarray:
