@@ -25,8 +25,15 @@ from . import _lib
 from .dispatch import host_rows, row_type
 from .projections import GROUPED_MAX_TOKENS, WO_A, WO_A_GROUPS, validate_values
 
-MAX_TOKENS, MAX_WIDTH, MAX_BATCH = 1 << 20, 4096, 1 << 16
+MAX_TOKENS, MAX_WIDTH, MAX_BATCH, MAX_HEADS = 1 << 20, 4096, 1 << 16, 1 << 16
 APART_WIDTHS, LATENT_WIDTHS = (64, 128, 256), ((512, 512), (576, 512))
+
+
+def _count(value, most: int, what: str) -> int:
+    """A number that a call hands to the library in 32 bits."""
+    if not 0 <= value <= most:
+        raise ValueError(f"{what} must be in [0, {most}]")
+    return int(value)
 
 
 def rotation_table(positions: int, dims: int, base: float = 10000.0, scaling: float = 1.0) -> np.ndarray:
@@ -36,6 +43,13 @@ def rotation_table(positions: int, dims: int, base: float = 10000.0, scaling: fl
         raise ValueError("a table needs positions, an even number of dims and a positive base")
     angle = np.arange(positions, dtype=np.float64)[:, None] * scaling * base ** (-np.arange(0, dims, 2) / dims)
     return np.concatenate([np.cos(angle), np.sin(angle)], 1).astype(np.float32)
+
+
+def _window(window) -> int:
+    """Of 2^31 positions and more, which are all that a length can have, as 2^31 - 1."""
+    if window < 0:
+        raise ValueError("window must not be negative")
+    return min(int(window), 2 ** 31 - 1)
 
 
 class HeadRotation:
@@ -93,14 +107,16 @@ class HeadRotation:
 
     def set(self, x_ptr, heads, y_ptr, weight_ptr=None, x_stride=None, y_stride=None) -> _lib.MxHeads:
         """`heads` heads of every token at x_ptr, to y_ptr (strides in values between tokens; None: contiguous)."""
-        own, ptr = int(heads) * self.width, _lib.ptr
-        return _lib.MxHeads(ptr(x_ptr), own if x_stride is None else x_stride, int(heads), ptr(weight_ptr), ptr(y_ptr),
+        heads, ptr = _count(heads, MAX_HEADS, "heads"), _lib.ptr
+        own = heads * self.width
+        return _lib.MxHeads(ptr(x_ptr), own if x_stride is None else x_stride, heads, ptr(weight_ptr), ptr(y_ptr),
                             own if y_stride is None else y_stride)
 
     def grad(self, x_ptr, heads, dy_ptr, dx_ptr, weight_ptr=None, dweight_ptr=None, x_stride=None, dy_stride=None,
              dx_stride=None) -> _lib.MxHeadsGrad:
-        own, ptr = int(heads) * self.width, _lib.ptr
-        return _lib.MxHeadsGrad(ptr(x_ptr), own if x_stride is None else x_stride, int(heads), ptr(weight_ptr), ptr(dy_ptr),
+        heads, ptr = _count(heads, MAX_HEADS, "heads"), _lib.ptr
+        own = heads * self.width
+        return _lib.MxHeadsGrad(ptr(x_ptr), own if x_stride is None else x_stride, heads, ptr(weight_ptr), ptr(dy_ptr),
                                 own if dy_stride is None else dy_stride, ptr(dx_ptr), own if dx_stride is None else dx_stride,
                                 ptr(dweight_ptr))
 
@@ -111,8 +127,8 @@ class HeadRotation:
         with self.lock:
             rotation = self.struct(positions_ptr, inverse)
             array = (_lib.MxHeads * len(sets))(*sets)
-            self.ctx.lib.rotate_heads(self.ctx._h(), array, len(sets), int(tokens), C.byref(rotation), row_type(x_dtype),
-                                      row_type(y_dtype or x_dtype), _lib._stream(stream))
+            self.ctx.lib.rotate_heads(self.ctx._h(), array, len(sets), _count(tokens, MAX_TOKENS, "tokens"), C.byref(rotation),
+                                      row_type(x_dtype), row_type(y_dtype or x_dtype), _lib._stream(stream))
 
     def open_gradients(self):
         """The workspace of the weights' gradients; allocated by the first call that needs it unless opened before (a
@@ -131,9 +147,9 @@ class HeadRotation:
             if any(g.dweight for g in grads):
                 self.open_gradients()
             array = (_lib.MxHeadsGrad * len(grads))(*grads)
-            self.ctx.lib.rotate_heads_backward(self.ctx._h(), array, len(grads), int(tokens), C.byref(rotation),
-                                               row_type(dtype), _lib.ptr(self.workspace), self.workspace_bytes,
-                                               _lib._stream(stream))
+            self.ctx.lib.rotate_heads_backward(self.ctx._h(), array, len(grads), _count(tokens, MAX_TOKENS, "tokens"),
+                                               C.byref(rotation), row_type(dtype), _lib.ptr(self.workspace),
+                                               self.workspace_bytes, _lib._stream(stream))
 
     # -- host arrays -------------------------------------------------------------------------------
     def _host(self, x, what):
@@ -215,8 +231,8 @@ class KVCache4:
             raise ValueError(f"latents and their values must be {LATENT_WIDTHS} wide")
         if not 16 <= page <= 1024 or page & (page - 1):
             raise ValueError("a page must be a power of two of tokens in [16, 1024]")
-        if pages < 1 or not 1 <= heads <= 1024 or query_heads < 1 or query_heads % heads:
-            raise ValueError("a cache needs pages, and query heads that are a multiple of its key heads")
+        if pages < 1 or not 1 <= heads <= 1024 or not 1 <= query_heads <= MAX_HEADS or query_heads % heads:
+            raise ValueError(f"a cache needs pages, and query heads that are a multiple of its key heads, {MAX_HEADS} at most")
         if not 1 <= max_tokens <= MAX_TOKENS or not 1 <= max_batch <= MAX_BATCH:
             raise ValueError(f"max_tokens in [1, {MAX_TOKENS}] and max_batch in [1, {MAX_BATCH}] required")
         self.ctx, self.pages, self.page, self.heads = ctx, int(pages), int(page), int(heads)
@@ -267,8 +283,9 @@ class KVCache4:
             handle, ptr = self._open(), _lib.ptr
             turned = None if rotation is None else rotation.struct(positions_ptr)
             rows = _lib.MxKv4Append(ptr(k_ptr), self.heads * self.width if k_stride is None else k_stride, ptr(v_ptr),
-                                    self.heads * self.value_width if v_stride is None else v_stride, row_type(dtype), int(tokens),
-                                    ptr(slots_ptr), ptr(weight_ptr), ptr(k_rounded_ptr), ptr(v_rounded_ptr))
+                                    self.heads * self.value_width if v_stride is None else v_stride, row_type(dtype),
+                                    _count(tokens, MAX_TOKENS, "tokens"), ptr(slots_ptr), ptr(weight_ptr),
+                                    ptr(k_rounded_ptr), ptr(v_rounded_ptr))
             self.ctx.lib.kv4_append(handle, C.byref(self.struct), C.byref(rows), None if turned is None else C.byref(turned),
                                     _lib._stream(stream))
 
@@ -282,8 +299,9 @@ class KVCache4:
             if not 0 <= tokens <= self.max_tokens or not 0 <= batch <= self.max_batch:
                 raise ValueError(f"the cache was opened for {self.max_tokens} query rows of {self.max_batch} sequences a call")
             query = _lib.MxKv4Attend(ptr(q_ptr), self.query_heads * self.width if q_stride is None else q_stride,
-                                     self.query_heads, int(tokens), int(batch), ptr(q_first_ptr), ptr(table_ptr), int(columns),
-                                     ptr(lengths_ptr), float(scale), int(window), ptr(sinks_ptr), ptr(out_ptr),
+                                     self.query_heads, int(tokens), int(batch), ptr(q_first_ptr), ptr(table_ptr),
+                                     _count(columns, (1 << 30) // self.page, "columns"),
+                                     ptr(lengths_ptr), float(scale), _window(window), ptr(sinks_ptr), ptr(out_ptr),
                                      self.query_heads * self.value_width if out_stride is None else out_stride, ptr(lse_ptr))
             self.ctx.lib.kv4_attend(handle, C.byref(self.struct), C.byref(query), self.workspace.ptr, self.workspace_bytes,
                                     _lib._stream(stream))
