@@ -509,7 +509,7 @@ typedef struct mx_kv4_query {
   const int32_t* table;      /* [batch][columns] page numbers                                                  */
   int32_t columns;           /* columns * page at most 2^30                                                    */
   const int32_t* lengths;    /* [batch] tokens in the cache, the queries' own among them                       */
-  float scale;
+  float scale;               /* positive, at most 2.3e38                                                       */
   int32_t window;            /* 0, or: a query sees the last `window` positions, its own among them            */
   const float* sinks;        /* [heads] a logit that takes part in the sum and has no value; or NULL           */
   uint16_t* out;             /* [T][heads][cache.value_width] BF16, tokens out_stride values apart (of 8)      */

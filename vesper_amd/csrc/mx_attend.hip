@@ -1657,7 +1657,7 @@ int mx_kv4_attend(mx_ctx* ctx, const mx_kv4* cache, const mx_kv4_query* query, v
   MX_REQUIRE(q.q_first || (q.batch ? q.tokens % q.batch == 0 : q.tokens == 0), "%s: %d rows do not divide among %d sequences", who,
              q.tokens, q.batch);
   MX_REQUIRE(q.window >= 0, "%s: window %d", who, q.window);
-  MX_REQUIRE(q.scale > 0.f && q.scale <= 3.4e38f, "%s: scale must be finite and positive", who);
+  MX_REQUIRE(q.scale > 0.f && q.scale <= 2.3e38f, "%s: scale must be positive and at most 2.3e38", who);   // (times log2(e))
   MX_REQUIRE(q.q_stride >= (int64_t)q.heads * cache->width && q.q_stride % 8 == 0 && q.q_stride < (1ll << 40) &&
                  q.out_stride >= (int64_t)q.heads * cache->value_width && q.out_stride % 8 == 0 && q.out_stride < (1ll << 40),
              "%s: token strides must be multiples of 8 that hold the heads", who);
