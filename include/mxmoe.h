@@ -452,7 +452,8 @@ typedef struct mx_heads_grad {
   int64_t dy_stride;
   void* dx;                  /* may be x or dy, with its stride                                                */
   int64_t dx_stride;
-  float* dweight;            /* [norm]: the sum over all tokens and heads; NULL = not asked for                */
+  float* dweight;            /* [norm]: the sum over all tokens and heads; NULL = not asked for. Apart from the other set's: */
+                             /* where both have one weight, add the two                                        */
 } mx_heads_grad;
 /* One or two sets of heads (queries, and keys with weights of their own) in one launch, x_type and y_type MX_ROWS_BF16 or
  * _F32. positions may be NULL where dims = 0. Rows that are no token keep the y they had. tokens in [0, 2^20], tokens *

@@ -140,8 +140,9 @@ class HeadRotation:
 
     def backward_device(self, grads, tokens: int, positions_ptr=None, dtype: str = "bf16", inverse: bool = False,
                         stream=None):
-        """The gradients of apply_device(inverse) for one or two `grad`s. Calls that ask for dweight share a workspace:
-        they must not overlap on different streams."""
+        """The gradients of apply_device(inverse) for one or two `grad`s, each with a dweight of its own (the sum of both is
+        the gradient of a weight that they share). Calls that ask for dweight share a workspace: they must not overlap on
+        different streams."""
         with self.lock:
             rotation = self.struct(positions_ptr, inverse)
             if any(g.dweight for g in grads):
