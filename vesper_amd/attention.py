@@ -283,7 +283,7 @@ class KVCache4:
         with self.lock:
             handle, ptr = self._open(), _lib.ptr
             turned = None if rotation is None else rotation.struct(positions_ptr)
-            if rotation is not None and rotation.ctx.ordinal != self.ctx.ordinal:
+            if rotation is not None and rotation.ctx is not self.ctx and rotation.ctx.ordinal != self.ctx.ordinal:
                 raise ValueError(f"the rotation is on device {rotation.ctx.ordinal}, the cache on {self.ctx.ordinal}")
             rows = _lib.MxKv4Append(ptr(k_ptr), self.heads * self.width if k_stride is None else k_stride, ptr(v_ptr),
                                     self.heads * self.value_width if v_stride is None else v_stride, row_type(dtype),
