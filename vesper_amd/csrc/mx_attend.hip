@@ -45,8 +45,8 @@ constexpr int kInlineTiles = 1024;   // row tiles of all sequences that every wo
 // Where the plan is made: in the workspace by a launch of its own, in every workgroup's LDS, or, up to 64 tiles, in the
 // registers of every wave.
 constexpr int kInSpace = 0, kInLds = 1, kByWave = 2;
-// What a unit's beginning and end cost, in iterations. With 3, 4, 5 and 6: the 48 sequences below 63.7, 62.9, 63.7 and 64.1 us,
-// drafts over 576-wide latents 84.1, 84.1, 86.2 and 85.8.
+// What a unit's beginning and end cost, in iterations. With 3, 4, 5 and 6: the 48 sequences below 60.5, 59.8, 60.6 and 60.9 us,
+// drafts over 576-wide latents 78.6, 78.4, 80.4 and 79.7, single tokens of grouped queries 74.8, 73.6, 73.0 and 73.2.
 constexpr int kBegin = 4;
 constexpr float kLowest = -3e38f;    // the maximum of a row that has seen nothing yet
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
@@ -329,6 +329,7 @@ __device__ __forceinline__ bool first_unit(const AttendArgs& a, const Plan& p, b
   u.s = uniform(sequence(a, u.b));
   u.tiles = tiles_of(a, u.s, rows);
   u.tile = t - (each ? u.b * a.tiles_each : uniform(p.base[u.b]));
+  if (u.tile >= u.tiles) return false;   // (somebody has changed the sequences meanwhile: it may have no row left to read)
   u.unit0 = before + uniform(p.prefix[t]);
   enter(a, u, rows, step);
   return true;
@@ -374,6 +375,7 @@ __device__ __forceinline__ bool first_of_few(const AttendArgs& a, int g, int64_t
   u.s.first = of(s.first), u.s.n = of(s.n), u.s.held = of(s.held);
   u.s.end = (int64_t)((uint64_t)(uint32_t)of((int)(s.end >> 32)) << 32 | (uint32_t)of((int)s.end));
   u.tiles = tiles_of(a, u.s, rows);
+  if (u.tile >= u.tiles) return false;   // (as above)
   u.unit0 = before + (uint32_t)of((int)upto) - (u.n + kBegin);
   share(a, u);
   return true;
@@ -556,8 +558,8 @@ __device__ __forceinline__ float power(float from, float to) {   // 2^(from - to
 // A workgroup's first queries are converted by all eight waves, later units' by the score waves while the value waves finish
 // the unit before; its first copies are asked for before its last products.
 //
-// Measured at 64 heads of 512 over 48 sequences of 200 to 30,000 tokens (86 MB, 39 GFLOP): 56 us and 10 us for the joining,
-// 690 TFLOP/s in the first. A step takes about 3,500 clocks, its products 2,048 of a SIMD's and its LDS traffic about 1,950; a
+// Measured at 64 heads of 512 over 48 sequences of 200 to 30,000 tokens (86 MB, 39 GFLOP): 57 us and 10 us for the joining,
+// 680 TFLOP/s in the first. A step takes about 3,500 clocks, its products 2,048 of a SIMD's and its LDS traffic about 1,950; a
 // workgroup has its first queries after about 17,000 (5,500 for the division, the rest the queries, from the caches beside
 // the first copies), and its way out takes 5,000. Before the roles were parted, with eight waves that all scored and
 // multiplied, both took 120 us. Not faster: priorities for either role (61 to 63 us for both kernels in place of 61), all of a
