@@ -328,8 +328,9 @@ class KVCache4:
             raise ValueError("two tokens name one slot")
         return np.ascontiguousarray(slots, np.int64)
 
-    def _sequences(self, table, lengths, counts, t):
-        """The int32 arrays of `t` query rows' sequences: pages, lengths and, with counts, first rows."""
+    def _sequences(self, table, lengths, counts, t, window=0):
+        """The int32 arrays of `t` query rows' sequences: pages, lengths and, with counts, first rows. Pages of which no row
+        sees a token, behind the length or before the windows, may have any number."""
         table, lengths = np.asarray(table), np.asarray(lengths)
         b = lengths.shape[0] if lengths.ndim == 1 else -1
         if (b < 0 or table.ndim != 2 or table.shape[0] != b or table.shape[1] < 1
@@ -337,17 +338,20 @@ class KVCache4:
             raise ValueError("table must be an integer array [B, columns] and lengths one [B]")
         if b and (lengths.min() < 0 or lengths.max() > table.shape[1] * self.page):
             raise ValueError("lengths must fit their pages")
-        used = np.arange(table.shape[1]) * self.page < lengths[:, None]
-        if np.any(used & ((table < 0) | (table >= self.pages))):
-            raise ValueError(f"page numbers in use must be in [0, {self.pages})")
-        first = None
+        first, rows = None, np.full(b, t // max(b, 1))
         if counts is not None:
             counts = np.asarray(counts)
             if counts.shape != (b,) or counts.dtype.kind not in "iu" or (b and counts.min() < 0) or counts.sum() > t:
                 raise ValueError(f"counts must be {b} numbers of query rows, {t} in all")
-            first = np.concatenate([[0], np.cumsum(counts)]).astype(np.int32)
+            rows, first = counts.astype(np.int64), np.concatenate([[0], np.cumsum(counts)]).astype(np.int32)
         elif t % max(b, 1) or (t and not b):
             raise ValueError("query rows do not divide among the sequences")
+        page = np.arange(table.shape[1]) * self.page
+        used = page < lengths[:, None]
+        if window:   # from the first row's first token on
+            used &= page + self.page > (lengths.astype(np.int64) - rows + 1 - _window(window))[:, None]
+        if np.any(used & ((table < 0) | (table >= self.pages))):
+            raise ValueError(f"page numbers in use must be in [0, {self.pages})")
         return np.ascontiguousarray(table, np.int32), np.ascontiguousarray(lengths, np.int32), first
 
     def append(self, k, slots, v=None, rotation: HeadRotation | None = None, positions=None, weight=None) -> dict:
@@ -393,7 +397,7 @@ class KVCache4:
         if dtype != "bf16":
             raise ValueError("q must be BF16 storage bits")
         t = q.shape[0]
-        table, lengths, first = self._sequences(table, lengths, counts, t)
+        table, lengths, first = self._sequences(table, lengths, counts, t, window)
         b = lengths.shape[0]
         if sinks is not None:
             sinks = np.ascontiguousarray(sinks, np.float32)
@@ -550,7 +554,7 @@ class CachedAttention:
                 raise ValueError(f"x must be [T, {self.hidden}] with T of at most {self.max_tokens}")
             positions = self.heads._positions(positions, t)
             slots = self.cache._slots(slots, t)
-            table, lengths, first = self.cache._sequences(table, lengths, counts, t)
+            table, lengths, first = self.cache._sequences(table, lengths, counts, t, self.window)
             dev = []
             try:
                 for a in (x, positions, slots, table, lengths, first):
