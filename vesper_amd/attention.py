@@ -519,6 +519,14 @@ class CachedAttention:
                 raise ValueError(f"the cache was opened for {self.max_tokens} tokens of {self.cache.max_batch} sequences a call")
             if not tokens:
                 return
+            # what the attention would refuse is refused before the tokens' latents are stored
+            if q_first_ptr is None and (not batch or tokens % batch):
+                raise ValueError("query rows do not divide among the sequences")
+            if not 1 <= columns <= (1 << 30) // self.cache.page:
+                raise ValueError(f"columns must be in [1, {(1 << 30) // self.cache.page}]")
+            if batch and (not _lib.ptr(table_ptr) or not _lib.ptr(lengths_ptr) or _lib.ptr(table_ptr) % 4 or _lib.ptr(lengths_ptr) % 4
+                          or (_lib.ptr(q_first_ptr) or 0) % 4):
+                raise ValueError("table, lengths and q_first must be aligned device addresses")
             proj, lib, handle, vp = self.projections, self.ctx.lib, self.ctx._h(), _lib.vp
             rows, width = WO_A[0] // WO_A_GROUPS, WO_A[1]
             proj.project_device("wkv", x_ptr, tokens, self.k.ptr, stream)
