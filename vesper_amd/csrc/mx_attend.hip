@@ -1133,9 +1133,9 @@ __host__ __device__ constexpr int waves(int width) { return width <= 64 ? 3 : wi
 // tile the work of RG waves, one a row group, which share its values; a wave keeps to its tile, and the token groups' sums are
 // added at the end.
 //
-// Measured: one token of 32 heads of 128 over 8 key heads and 64 sequences of 500 to 16,000 tokens, 317 MB: 66 us, 4.8 TB/s,
-// what HBM gives to reads of this kind. Two prompts' 2048 tokens over 4500 and 8192, 322 GFLOP: 340 us, the matrix units busy
-// in 41 % of the cycles: a step's products take 512 clocks of a SIMD and its other instructions (converting, softmax) about
+// Measured: one token of 32 heads of 128 over 8 key heads and 64 sequences of 500 to 16,000 tokens, 317 MB: 65 us, 4.9 TB/s
+// (a large copy's reads and writes 5.1). Two prompts' 2048 tokens over 4500 and 8192, 322 GFLOP: 357 us, the matrix units busy
+// in 39 % of the cycles: a step's products take 512 clocks of a SIMD and its other instructions (converting, softmax) about
 // as many again from each of two waves.
 template <int W, int RG>
 struct Grouped {

@@ -256,7 +256,7 @@ __device__ __forceinline__ void finish_row(const void* row, bool wide, const mx_
     });
 }
 
-// Host: the checks of a rotation that both files make. x_needed: whether positions must be given.
+// Host: the checks of a rotation that both files make.
 int check_rotation(const char* who, const mx_rotation* rot);
 
 inline bool aligned(const void* p, uintptr_t a) { return ((uintptr_t)p & (a - 1)) == 0; }

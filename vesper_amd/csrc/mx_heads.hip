@@ -5,7 +5,7 @@
 //
 // Memory traffic alone: a row is read once into registers, eight values a lane, by as many lanes as it has eights.
 // Measured for 4096 tokens of 32 + 8 heads of 128 in BF16, all of each turned: forward 20.2 us for 86 MB (4.3 TB/s; 27.3 with
-// a row at a time, whose loads waited for the token's position), backward 28.2 us for 128 MB (4.5 TB/s) and 4.6 for the
+// a row at a time, whose loads waited for the token's position), backward 29.2 us for 128 MB (4.4 TB/s) and 4.5 for the
 // workgroups' parts of dweight (46 and 9.4 with 512 workgroups for either set).
 #include <algorithm>
 #include <cstdlib>
