@@ -564,9 +564,10 @@ __device__ __forceinline__ float power(float from, float to) {   // 2^(from - to
 // the first copies), and its way out takes 5,000. Before the roles were parted, with eight waves that all scored and
 // multiplied, both took 120 us. Not faster: priorities for either role (61 to 63 us for both kernels in place of 61), all of a
 // unit's first copies before the rows of the one before go out (windows of 128 over prompts 124 us in place of 122).
+constexpr int kLatentStep = 64;
 template <int WK, int RG>
 struct Latent {
-  static constexpr int WV = 512, RQ = 2 * RG, TT = 4 / RQ, T2 = 4 / TT, kRows = 32 * RG, kStep = 64;
+  static constexpr int WV = 512, RQ = 2 * RG, TT = 4 / RQ, T2 = 4 / TT, kRows = 32 * RG, kStep = kLatentStep;
   static constexpr bool kPart = WK % 128 != 0;             // a last step of 64 columns of the keys
   static constexpr int KS = (WK + 127) / 128;
   static constexpr int kStages = kPart ? 3 : 4;
@@ -1689,7 +1690,7 @@ int mx_kv4_attend(mx_ctx* ctx, const mx_kv4* cache, const mx_kv4_query* query, v
   const double steps = (double)q.batch * cache->heads * ((rows + 31) / 32) * ((held + 31) / 32) / (4. * n);
   int rg = rows <= 32 ? 1 : rows <= 64 ? 2 : 4;
   rg = std::min({rg, most_groups(cache), steps <= (cache->v_codes ? 8 : 5) ? 1 : steps <= 128 ? 2 : 4});
-  const int tile_rows = 32 * rg, step = 128 / rg;
+  const int tile_rows = 32 * rg, step = cache->v_codes ? 128 / rg : kLatentStep;
   a.by_group = Divide(a.group);
   if (!q.q_first) a.rows_each = q.tokens / q.batch, a.tiles_each = (int)(((int64_t)a.rows_each * a.group + tile_rows - 1) / tile_rows);
   a.by_tiles = Divide(std::max(a.tiles_each, 1));
@@ -1699,12 +1700,13 @@ int mx_kv4_attend(mx_ctx* ctx, const mx_kv4* cache, const mx_kv4_query* query, v
   const int by = tiles <= 64 ? kByWave : tiles <= kInlineTiles ? kInLds : kInSpace;   // (at least as many as sequences)
   hipStream_t st = as_stream(stream);
   // Units of few iterations stay whole, by what the tables can hold: parts cost another beginning, their way out and the
-  // second launch, some 9 us. One token each, split and whole: latents of 64 heads 128 x 500 tokens (8 iterations) 25.1 and
-  // 22.9 us, 400 x 500 64.1 and 54.3, but 1 x 320 (5) 14.1 and 15.5; 32 heads over 8 key heads 64 x 1000 (8) 22.7 and 19.5,
-  // 1 x 800 (7) 13.4 and 13.1, 1 x 1000 13.1 and 13.9; prompts of 1000 with a window of 128 (2) 36.5 and 27.4.
+  // second launch, some 9 us. One token each, split and whole: latents of 64 heads 128 x 500 tokens (8 iterations) 26.1 and
+  // 23.9 us, 400 x 500 64.2 and 52.9, of one row group 64 x 700 (11) 33.9 and 27.6, 64 x 1000 (16) 36.1 and 34.8, 256 x 1000 of
+  // 16 heads 41.3 and 39.1, but 1 x 320 (5) 12.2 and 14.7 and 1 x 500 12.7 and 19.3; 32 heads over 8 key heads 64 x 1000 (8)
+  // 22.7 and 19.5, 1 x 800 (7) 13.4 and 13.1, 1 x 1000 13.1 and 13.9; prompts of 1000 with a window of 128 (2) 36.5 and 27.4.
   const int64_t span = std::min<int64_t>(held, q.window ? (int64_t)q.window + 31 + (tile_rows + a.group - 1) / a.group : INT64_MAX);
   const bool few_units = (int64_t)q.batch * cache->heads * ((rows + tile_rows - 1) / tile_rows) < 16;
-  a.whole = span <= (int64_t)step * (!few_units ? 8 : cache->v_codes ? 7 : 4);
+  a.whole = span <= (int64_t)step * (few_units ? cache->v_codes ? 7 : 4 : cache->v_codes || rg > 1 ? 8 : 16);
   if (by == kInSpace) {
     hipLaunchKernelGGL(plan_kernel, dim3(1), dim3(1024), 0, st, a, tile_rows, step);
     MX_LAUNCH_CHECK("plan_kernel");
@@ -1712,6 +1714,7 @@ int mx_kv4_attend(mx_ctx* ctx, const mx_kv4* cache, const mx_kv4_query* query, v
   const int joiners = 8 * kCus;
   auto latent = [&](auto wk, auto groups) {
     constexpr int WK = decltype(wk)::value, RG = decltype(groups)::value;
+    static_assert(Latent<WK, RG>::kRows == 32 * RG && Latent<WK, RG>::kStep == kLatentStep, "the plan is of these tiles and steps");
     hipLaunchKernelGGL((latent_kernel<WK, RG>), dim3(n), dim3(512), 0, st, a, by);
     MX_LAUNCH_CHECK("latent_kernel");
     if (a.whole) return MX_OK;
@@ -1721,6 +1724,7 @@ int mx_kv4_attend(mx_ctx* ctx, const mx_kv4* cache, const mx_kv4_query* query, v
   };
   auto grouped = [&](auto w, auto groups) {
     constexpr int W = decltype(w)::value, RG = decltype(groups)::value;
+    static_assert(Grouped<W, RG>::kRows == 32 * RG && Grouped<W, RG>::kStep == 128 / RG, "the plan is of these tiles and steps");
     hipLaunchKernelGGL((grouped_kernel<W, RG>), dim3(n), dim3(256), 0, st, a, by);
     MX_LAUNCH_CHECK("grouped_kernel");
     if (a.whole) return MX_OK;
